@@ -64,9 +64,12 @@ enum fd_device_error {
   FD_DEVERR_TIMEOUT = 3,   /* a bounded wait on an mbarrier gave up */
   FD_DEVERR_SLOT = 4,      /* KV-write slot outside both tiers */
   FD_DEVERR_SPLITS = 5,    /* lens[i] exceeds the max_len the grid was sized for */
-  FD_DEVERR_PLAN = 6       /* fd_plan_step: bad query offsets, or a request that
+  FD_DEVERR_PLAN = 6,      /* fd_plan_step: bad query offsets, or a request that
                               extends prior context by > 1 token while part of
                               its KV is in the host tier (fastdecode/plan.py:142-149) */
+  FD_DEVERR_TABLES = 7,    /* fd_extend_tables refused the step (FD_TABLES_* bits
+                              in its header say why) */
+  FD_DEVERR_POSITION = 8   /* fd_rope_store_kv: position outside the table */
 };
 
 /* ---------------------------------------------------------------- types */
@@ -527,6 +530,212 @@ FD_API int fd_store_kv(const void *key, int64_t key_stride_n, int64_t key_stride
                 int32_t block_size, int32_t dtype, const fd_kv_tier *tiers,
                 int64_t tier_split, int32_t *error, void *stream);
 
+/* ------------------------------------------------- tables from lengths */
+
+/* Slots of the header fd_extend_tables writes (int32, device memory). */
+enum fd_tables_header {
+  FD_TABLES_FLAGS = 0,       /* FD_TABLES_* bits below; 0: the step was applied */
+  FD_TABLES_N_TOK = 1,       /* new tokens of the step */
+  FD_TABLES_TAKEN_HBM = 2,   /* blocks taken from each tier's free stack */
+  FD_TABLES_TAKEN_HOST = 3,
+  FD_TABLES_FREED_HBM = 4,   /* blocks of ended requests given back */
+  FD_TABLES_FREED_HOST = 5,
+  FD_TABLES_MAX_SEQ = 6,     /* longest request after the step */
+  FD_TABLES_MAX_NEW = 7,     /* most new tokens of a request */
+  FD_TABLES_HEADER_LEN = 8
+};
+enum fd_tables_flags {
+  FD_TABLES_NO_BLOCKS = 1,   /* both free stacks together hold too few blocks */
+  FD_TABLES_WIDTH = 2,       /* a request needs more blocks than a table row holds */
+  FD_TABLES_TOKENS = 4,      /* more new tokens than max_tokens */
+  FD_TABLES_BAD_LEN = 8,     /* prior length below 0 or past the row, or new length below -1 */
+  FD_TABLES_BAD_BLOCK = 16,  /* an ended request holds a block id outside both tiers */
+  FD_TABLES_BAD_POOL = 32    /* a free count outside its stack, or a stack too small
+                                for the blocks given back */
+};
+#define FD_TABLES_MAX_REQS 8192
+
+/* Block tables, slots and positions of a step, from the requests' lengths.
+ * No counterpart in the reference, where the engine's block manager fills
+ * the table on the host.  Request r has prior_lens[r] tokens in the cache,
+ * their ceil(prior / block_size) block ids at the front of its table row, and
+ * brings new_lens[r] >= 0 more; new_lens[r] = -1 ends it.  The free blocks of
+ * each tier are a stack (free_ids[t][0 .. counts[t]), the top last; HBM ids
+ * are below num_gpu_blocks, host ids follow, as everywhere here).
+ *   1. The blocks of ended requests are pushed onto their tier's stack, in
+ *      request and table order.
+ *   2. The blocks that the new tokens need beyond those a request holds are
+ *      popped in request and position order, from the HBM stack while it has
+ *      any, then from the host stack, and written to the table rows.
+ *   3. seq_lens (0 for an ended request), query_start_loc (running sum of the
+ *      new tokens), and per new token its slot (block id * block_size +
+ *      offset) and position; entries behind the last token, up to
+ *      max_tokens, are slot -1 and position 0.
+ * A step that cannot be applied as a whole (any FD_TABLES_* flag) changes
+ * neither table nor stacks: counts_out = counts_in, seq_lens = prior_lens,
+ * query_start_loc 0, slots -1, positions 0, and the error word gets
+ * FD_DEVERR_TABLES.  The outputs are those of fd_plan_step's inputs, so a
+ * step can be set up and planned without the host.  seq_lens may be
+ * prior_lens and counts_out may be counts_in (in place); given separate
+ * buffers, the call can be repeated with the same result.  The ids on the
+ * free stacks are the caller's and are not checked. */
+typedef struct fd_tables_args {
+  const int32_t *new_lens;   /* [R] */
+  const int32_t *prior_lens; /* [R] */
+  int32_t *block_table;      /* [R, bt_stride] */
+  int64_t bt_stride;
+  int32_t bt_width;
+  int32_t num_reqs;          /* R, at most FD_TABLES_MAX_REQS */
+  int32_t *free_ids[2];      /* [free_cap[t]] */
+  int32_t free_cap[2];
+  const int32_t *counts_in;  /* [2] */
+  int32_t *counts_out;       /* [2] */
+  int64_t num_gpu_blocks;
+  int64_t num_cpu_blocks;
+  int32_t block_size;
+  int32_t max_tokens;
+  int32_t *seq_lens;         /* [R] */
+  int32_t *query_start_loc;  /* [R + 1] */
+  int64_t *slot_mapping;     /* [max_tokens] */
+  int64_t *positions;        /* [max_tokens] */
+  int32_t *header;           /* [FD_TABLES_HEADER_LEN] */
+  int32_t *error;            /* optional device error word */
+} fd_tables_args;
+
+FD_API int fd_extend_tables(const fd_tables_args *a, void *stream);
+
+/* sizeof(fd_tables_args) as compiled into the library (binding check). */
+FD_API size_t fd_tables_args_bytes(void);
+
+/* ------------------------------------------- rotary positions + KV write */
+
+#define FD_ROPE_MAX_AXES 4
+#define FD_ROPE_MAX_PAIRS 128
+
+/* Rotary positions with one to four axes, fused with the tier-aware KV write
+ * of fd_store_kv.  No counterpart in the reference, whose models rotate q and
+ * k before the backend is called.  The first rot_dim dims of each head of q
+ * and k are rot_dim / 2 pairs; pair i turns by the angle of position
+ * positions[axis_of_pair[i]][t] :
+ *   (x1, x2) -> (x1 cos - x2 sin, x2 cos + x1 sin),
+ * cos = cos_sin[pos * rot_dim + i], sin = cos_sin[pos * rot_dim +
+ * rot_dim / 2 + i], fp32, computed in fp32 and rounded once.  A pair is dims
+ * (i, i + rot_dim / 2), or (2 i, 2 i + 1) with FD_ROPE_PAIRS.  Dims from
+ * rot_dim on are copied.  q goes to q_out (may be q itself), the rotated k and v to the
+ * slot of the token in whichever tier owns it (slot < 0: nowhere), and the
+ * rotated k also to k_out when given (may be k itself).  A token with a
+ * position outside the table (FD_DEVERR_POSITION) is skipped as a whole; one
+ * whose slot lies outside both tiers (FD_DEVERR_SLOT) writes no K/V but its
+ * q_out and k_out.  Slots >= 0 must differ from one another. */
+typedef struct fd_rope_args {
+  const void *q;             /* [T, H, D] */
+  int64_t q_stride_t, q_stride_h;
+  void *q_out;               /* [T, H, D] */
+  int64_t qo_stride_t, qo_stride_h;
+  const void *k;             /* [T, KVH, D] */
+  int64_t k_stride_t, k_stride_h;
+  const void *v;             /* [T, KVH, D] */
+  int64_t v_stride_t, v_stride_h;
+  void *k_out;               /* [T, KVH, D] or NULL */
+  int64_t ko_stride_t, ko_stride_h;
+  const int64_t *positions;  /* [num_axes, pos_stride] */
+  int64_t pos_stride;
+  const float *cos_sin;      /* [max_pos, rot_dim] contiguous, 16-byte aligned */
+  int64_t max_pos;
+  const int64_t *slots;      /* [T] or NULL (no KV write) */
+  fd_kv_tier tier[2];
+  int64_t tier_split;
+  int32_t num_tokens;
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_size;
+  int32_t rot_dim;           /* even, at most head_size and 2 * FD_ROPE_MAX_PAIRS */
+  int32_t block_size;
+  int32_t dtype;             /* of q, k, v and the tiers */
+  int32_t num_axes;
+  int32_t flags;             /* FD_ROPE_* */
+  uint8_t axis_of_pair[FD_ROPE_MAX_PAIRS];
+  int32_t _pad0;
+  int32_t *error;
+} fd_rope_args;
+
+#define FD_ROPE_PAIRS 1
+
+FD_API int fd_rope_store_kv(const fd_rope_args *a, void *stream);
+
+/* sizeof(fd_rope_args) as compiled into the library (binding check). */
+FD_API size_t fd_rope_args_bytes(void);
+
+/* ------------------------------------------- chunk and cross attention */
+
+/* Arguments of fd_chunk_attn and fd_cross_attn.  Request r has the queries
+ * q_start[r] .. + q_len[r] - 1 of q; requests' query rows must not overlap.
+ * Rows of out (and lse) that belong to no request are left as they were; a
+ * query that sees no key gets out = 0 and lse = -inf. */
+typedef struct fd_attn_args {
+  const void *q;             /* [num_tokens, H, D] */
+  int64_t q_stride_t, q_stride_h;
+  void *out;                 /* [num_tokens, H, D], q's dtype */
+  int64_t out_stride_t, out_stride_h;
+  float *lse;                /* natural log, (h, t) at h * lse_stride_h + t * lse_stride_t; or NULL */
+  int64_t lse_stride_h, lse_stride_t;
+  fd_kv_tier tier[2];        /* cross: tier[0].k / .v are the [rows, KVH, D] states,
+                                tok_stride and head_stride, num_blocks = rows */
+  int64_t tier_split;        /* chunk only */
+  const int32_t *block_table; /* chunk only */
+  int64_t bt_stride;
+  const int32_t *bt_row;     /* chunk: table row of request r (NULL: r) */
+  const int32_t *k_start;    /* cross: first state row of request r */
+  const int32_t *q_start;    /* [n] int32, device memory, as the following */
+  const int32_t *q_len;
+  const int32_t *k_len;
+  int32_t bt_width;
+  int32_t num_tokens;
+  int32_t n;                 /* requests, at most 65535 */
+  int32_t num_heads;
+  int32_t num_kv_heads;
+  int32_t head_size;         /* at most 256, head_size * element size a multiple of 16 bytes */
+  int32_t block_size;        /* chunk only */
+  float scale;               /* positive */
+  int32_t dtype;             /* of q, K, V and out */
+  int32_t max_q_len;         /* the host's bounds on q_len and k_len, 0: unknown.  They choose
+                                between kernels; a wrong one costs time, not the result */
+  int32_t max_k_len;
+  int32_t _pad0;
+  void *workspace;           /* fd_attn_workspace_size() bytes, 16-byte aligned; calls that run at
+                                the same time need one each */
+  size_t workspace_bytes;
+  int32_t *error;            /* optional device error word */
+} fd_attn_args;
+
+/* Scratch bytes of fd_chunk_attn / fd_cross_attn for these shapes (reads
+ * num_heads, num_kv_heads, head_size and dtype only).  Pure host arithmetic. */
+FD_API size_t fd_attn_workspace_size(const fd_attn_args *a);
+
+/* Attention of a chunk of new tokens over the two-tier paged cache:
+ *   o[i,h] = softmax(q[i,h] . K^T * scale) @ V over keys 0 .. k_len - q_len + i
+ * for query i of a request (the last query sees all k_len keys; with q_len >
+ * k_len the first queries see none).  The new tokens' own K/V are in the
+ * cache already (fd_store_kv or fd_rope_store_kv).  Key j lies in block
+ * block_table[bt_row][j / block_size], either tier.  Cache contents behind
+ * k_len are never used, whatever they are; K/V of a request's own keys must
+ * be finite.  The reference refuses such requests when part of their context
+ * is in the host tier (fastdecode/plan.py:142-149) and hands the others to
+ * FlashAttention (fastdecode/backend.py:317-340).  Block ids and lengths are
+ * range-checked on the device: a request whose lengths do not fit its rows
+ * writes nothing (FD_DEVERR_LEN); a block id outside both tiers is not read
+ * (FD_DEVERR_BLOCK_ID; the rows of a request that lists it are undefined). */
+FD_API int fd_chunk_attn(const fd_attn_args *a, void *stream);
+
+/* Cross attention to an encoder's states: every query of request r sees the
+ * k_len[r] rows k_start[r] .. of the states (device memory); requests may
+ * share rows.  q_len[r] = 1 is a decode step.  No counterpart in the
+ * reference, whose backend takes decoder attention only. */
+FD_API int fd_cross_attn(const fd_attn_args *a, void *stream);
+
+/* sizeof(fd_attn_args) as compiled into the library (binding check). */
+FD_API size_t fd_attn_args_bytes(void);
+
 /* ---------------------------------------------------------------- utilities */
 
 /* Message of the last FD_ERR_* returned on this thread. */
@@ -548,7 +757,8 @@ FD_API int fd_host_device_pointer(void *host, void **device_ptr);
 FD_API int fd_host_register(void *host, size_t bytes);
 FD_API int fd_host_unregister(void *host);
 
-/* Library version, e.g. 101 for 0.1.1 (101: fd_plan_step, bt_rows). */
+/* Library version, e.g. 101 for 0.1.1 (101: fd_plan_step, bt_rows; 102:
+ * fd_extend_tables, fd_rope_store_kv, fd_chunk_attn, fd_cross_attn). */
 FD_API int fd_version(void);
 
 /* sizeof(fd_decode_args) and sizeof(fd_kv_tier) as compiled into the

@@ -1,0 +1,561 @@
+"""GPU tests of the multi-token step's operators against plain 64-bit forms
+(tests/step_ref.py): block tables from lengths (exact), multi-axis rotary
+positions with the KV write, chunk attention over both tiers, cross attention,
+and a run of them together."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import step_ref as ref
+import torch
+
+from vllm_fastdecoder_b200 import gpu_ops, plan
+from vllm_fastdecoder_b200.gpu_ops import FreeBlocks, KVTier, StepTables
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def dev():
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+# ------------------------------------------------------------------ tables
+
+
+def _table_case(R, block, ctx, new_hi, end_every, hbm_share, seed, slack=6):
+    rnd = random.Random(seed)
+    prior = [rnd.randint(0, ctx) for _ in range(R)]
+    new = [rnd.choice([0, 1, rnd.randint(0, new_hi)]) for _ in range(R)]
+    if end_every:
+        new = [-1 if i % end_every == end_every - 1 else n for i, n in enumerate(new)]
+    held = [-(-p // block) for p in prior]
+    need = sum(-(-(p + n) // block) - h for p, n, h in zip(prior, new, held) if n >= 0)
+    total = sum(held) + need + slack
+    hbm = max(1, int(total * hbm_share))
+    ids = list(range(total))
+    rnd.shuffle(ids)
+    W = max(-(-(p + max(0, n)) // block) for p, n in zip(prior, new)) + 2
+    table, at = [], 0
+    for h in held:
+        table.append(ids[at:at + h] + [-7] * (W - h))
+        at += h
+    s0, s1 = [b for b in ids[at:] if b < hbm], [b for b in ids[at:] if b >= hbm]
+    counts = [len(s0), len(s1)]
+    return prior, new, table, [s0 + [-1] * (total - len(s0)), s1 + [-1] * (total - len(s1))], counts, hbm, total - hbm
+
+
+def _run_tables(prior, new, table, stacks, counts, hbm, host, block, T, W=None, in_place=False):
+    tt, st, ct, pr = i32(table), i32(stacks), i32(counts), i32(prior)
+    free = FreeBlocks(st[0], st[1], ct)
+    out = StepTables(len(prior), T, dev(), seq_lens=pr if in_place else None, counts=ct if in_place else None)
+    out.slot_mapping.fill_(99)
+    out.positions.fill_(99)
+    gpu_ops.extend_tables(i32(new), pr, tt, free, hbm, host, block, out)
+    return tt, st, out
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("R,block,ctx,new_hi,end_every,share,T", [
+    (1, 16, 0, 1, 0, 1.0, 4), (1, 1, 5, 3, 0, 0.5, 9), (3, 16, 40, 20, 2, 0.5, 70), (33, 8, 100, 9, 4, 0.3, 300),
+    (256, 16, 500, 2, 16, 0.6, 700), (1023, 16, 64, 5, 3, 0.5, 2048), (1024, 32, 64, 5, 0, 0.01, 6000),
+    (1025, 24, 300, 40, 5, 0.5, 50000), (8192, 16, 100, 3, 9, 0.5, 20000), (5, 64, 3000, 9000, 0, 0.7, 50000),
+])
+def test_tables_match_lists(R, block, ctx, new_hi, end_every, share, T, in_place):
+    prior, new, table, stacks, counts, hbm, host = _table_case(R, block, ctx, new_hi, end_every, share, R + T)
+    want = ref.tables(new, prior, table, stacks, counts, hbm, block, T)
+    assert want is not None
+    tt, st, out = _run_tables(prior, new, table, stacks, counts, hbm, host, block, T, in_place=in_place)
+    gpu_ops.check_device_errors(dev())
+    h = out.read_header()
+    w_table, w_stacks, w_counts, w_seq, w_qsl, w_slots, w_pos = want
+    assert tt.tolist() == w_table and out.counts.tolist() == w_counts
+    for t in range(2):
+        top = max(w_counts[t], counts[t])
+        assert st[t].tolist()[:w_counts[t]] == w_stacks[t][:w_counts[t]]
+        assert st[t].tolist()[top:] == w_stacks[t][top:]
+    assert out.seq_lens.tolist() == w_seq and out.query_start_loc.tolist() == w_qsl
+    assert out.slot_mapping.tolist() == w_slots and out.positions.tolist() == w_pos
+    assert h["n_tok"] == w_qsl[-1] and h["max_seq"] == max(s for s, n in zip(w_seq, new))
+    assert h["max_new"] == max(0, max(new))
+
+
+def test_tables_of_no_requests_and_no_tokens():
+    e = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = StepTables(0, 3, dev())
+    gpu_ops.extend_tables(e, e, torch.zeros(0, 4, dtype=torch.int32, device="cuda"), FreeBlocks(e, None, i32([0, 0])), 4, 0,
+                          16, out)
+    assert out.read_header()["n_tok"] == 0 and out.slot_mapping.tolist() == [-1] * 3
+    out = StepTables(2, 0, dev())
+    gpu_ops.extend_tables(i32([0, -1]), i32([5, 5]), i32([[1], [2]]), FreeBlocks(i32([0]), i32([0]), i32([0, 0])), 8, 0, 16,
+                          out)
+    assert out.read_header()["freed_hbm"] == 1 and out.seq_lens.tolist() == [5, 0] and out.counts.tolist() == [1, 0]
+
+
+@pytest.mark.parametrize("big", [False, True])
+@pytest.mark.parametrize("why,flag", [("blocks", 1), ("width", 2), ("tokens", 4), ("prior", 8), ("new", 8), ("block", 16),
+                                      ("count", 32), ("room", 32)])
+def test_refused_steps_change_nothing(why, flag, big):
+    R = 1500 if big else 6
+    prior, new = [20] * R, [3] * R
+    table = [[2 * r, 2 * r + 1, -7] for r in range(R)]
+    T, counts, caps = 4 * R + 10, [4, 4], [8 * R, 8 * R]
+    new[1] = -1
+    if why == "blocks":
+        new = [13] * R  # a block more for every request
+        T = 20 * R
+        counts = [R - 2, 1]
+    elif why == "width":
+        new[R - 1] = 29
+        counts = [R, R]
+    elif why == "tokens":
+        T = 3 * (R - 1) - 1
+    elif why == "prior":
+        prior[0] = -1
+    elif why == "new":
+        new[0] = -2
+    elif why == "block":
+        table[1][1] = 8 * R
+    elif why == "count":
+        counts = [-1, 3]
+    elif why == "room":
+        caps = [5, 5]
+    stacks = [[1000000 + i for i in range(caps[0])], [2000000 + i for i in range(caps[1])]]
+    tt, st, out = _run_tables(prior, new, table, stacks, counts, 4 * R, 4 * R, 16, T)
+    with pytest.raises(RuntimeError, match="block tables"):
+        gpu_ops.check_device_errors(dev())
+    assert out.header.tolist()[0] & flag
+    with pytest.raises(RuntimeError, match="refused"):
+        out.read_header()
+    assert tt.tolist() == table and st.tolist() == stacks and out.counts.tolist() == counts
+    assert out.seq_lens.tolist() == prior and out.query_start_loc.tolist() == [0] * (R + 1)
+    assert out.slot_mapping.tolist() == [-1] * T and out.positions.tolist() == [0] * T
+
+
+# ------------------------------------------------------------------ rope
+
+
+def _cos_sin(positions, rot):
+    ang = torch.arange(positions, dtype=torch.float64).unsqueeze(1) * 10000.0 ** (
+        -torch.arange(0, rot, 2, dtype=torch.float64) / rot)
+    return torch.cat([ang.cos(), ang.sin()], 1).float().cuda()
+
+
+def _rope_ok(got, want, x, dtype):
+    # two products and a sum in fp32 (three half steps of at most |x1| + |x2|), rounded once to the type
+    tol = ref.half_step(dtype) * want.abs() + 3 * 2.0 ** -24 * 2 * x.double().abs().max() + 2.0 ** -24
+    err = (got.double() - want).abs()
+    assert bool((err <= tol).all()), float((err - tol).max())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("T,H,KVH,D,rot,sections,turns,pairs,block", [
+    (1, 4, 1, 64, 64, None, False, False, 16), (37, 8, 2, 128, 128, (24, 20, 20), False, False, 16),
+    (130, 8, 2, 128, 128, (24, 20, 20), True, False, 16), (65, 6, 3, 80, 40, (7, 7, 6), True, True, 24),
+    (50, 5, 5, 80, 20, (10,), False, False, 1), (33, 2, 1, 256, 256, (32, 32, 32, 32), True, True, 7),
+    (3000, 4, 2, 64, 32, (16,), False, True, 64), (20, 3, 1, 96, 2, None, False, True, 16),
+])
+def test_rope_writes_rotated_rows(dtype, T, H, KVH, D, rot, sections, turns, pairs, block):
+    g = torch.Generator(device="cuda").manual_seed(T)
+    A = 1 if sections is None else len(sections)
+    qkv = torch.randn(T, (H + 2 * KVH) * D, generator=g, device="cuda").to(dtype)
+    q, k, v = (x.unflatten(1, (-1, D)) for x in qkv.split((H * D, KVH * D, KVH * D), 1))
+    pos = torch.randint(0, 5000, (A, T + 3), generator=g, device="cuda")
+    pos[:, 0] = 4999
+    cs = _cos_sin(5000, rot)
+    hbm, host = -(-T // block) // 2 + 1, -(-T // block) // 2 + 2
+    cache = torch.full((hbm, block, KVH, 2 * D), NAN, device="cuda").to(dtype)
+    hk = torch.full((host, KVH, block, D), NAN).to(dtype).pin_memory()
+    hv = torch.full((host, KVH, block, D), NAN).to(dtype).pin_memory()
+    logical = cache.permute(0, 2, 1, 3)
+    tiers = (KVTier(logical[..., :D], logical[..., D:]), KVTier(hk, hv))
+    slots = torch.randperm((hbm + host) * block, generator=g, device="cuda")[:T]
+    slots[::5] = -1
+    q_out = torch.full((T, H + 1, D), NAN, device="cuda").to(dtype)[:, :H]
+    k_out = torch.full((T, KVH, D), NAN, device="cuda").to(dtype)
+    before = qkv.clone()
+    got = gpu_ops.rope_store_kv(q, k, v, pos[0] if sections is None else pos, cs, slots, tiers, hbm, sections=sections,
+                                turns=turns, pairs=pairs, q_out=q_out, k_out=k_out)
+    gpu_ops.check_device_errors(dev())
+    assert got is q_out and torch.equal(qkv, before)
+    axis = gpu_ops.rope_axes((rot // 2,) if sections is None else sections, turns)
+    want_k = ref.rope(k, pos[:, :T], cs, axis, pairs)
+    _rope_ok(q_out, ref.rope(q, pos[:, :T], cs, axis, pairs), q, dtype)
+    _rope_ok(k_out, want_k, k, dtype)
+    rows_k = torch.cat([logical[..., :D].transpose(1, 2).reshape(-1, KVH, D),
+                        hk.transpose(1, 2).reshape(-1, KVH, D).cuda()])
+    rows_v = torch.cat([logical[..., D:].transpose(1, 2).reshape(-1, KVH, D),
+                        hv.transpose(1, 2).reshape(-1, KVH, D).cuda()])
+    kept = slots >= 0
+    assert torch.equal(rows_k[slots[kept]], k_out[kept]) and torch.equal(rows_v[slots[kept]], v[kept])
+    rest = torch.ones(rows_k.shape[0], dtype=torch.bool, device="cuda")
+    rest[slots[kept]] = False
+    assert bool(rows_k[rest].isnan().all()) and bool(rows_v[rest].isnan().all())
+    # in place, without a KV write
+    q2, k2 = q.clone(), k.clone()
+    assert gpu_ops.rope_store_kv(q2, k2, v, pos[0] if sections is None else pos, cs, None, (None, None), 0,
+                                 sections=sections, turns=turns, pairs=pairs, k_out=k2) is q2
+    assert torch.equal(q2, q_out) and torch.equal(k2, k_out)
+
+
+def test_rope_skips_what_is_out_of_range():
+    T, H, KVH, D = 6, 2, 1, 64
+    q, k, v = (torch.randn(T, h, D, device="cuda") for h in (H, KVH, KVH))
+    cache = torch.zeros(2, 4, KVH, 2 * D, device="cuda")
+    lg = cache.permute(0, 2, 1, 3)
+    tiers = (KVTier(lg[..., :D], lg[..., D:]), None)
+    pos = torch.tensor([[0, 1, 8, 3, 4, 5], [0, -1, 2, 3, 4, 5]], device="cuda")
+    slots = torch.tensor([0, 1, 2, 8, 5, 6], device="cuda")
+    out = torch.full_like(q, NAN)
+    gpu_ops.rope_store_kv(q, k, v, pos, _cos_sin(8, 64), slots, tiers, 2, sections=(16, 16), q_out=out)
+    with pytest.raises(RuntimeError, match="position|slot"):
+        gpu_ops.check_device_errors(dev())
+    assert bool(out[1:3].isnan().all()) and not bool(out[[0, 3, 4, 5]].isnan().any())
+    rows = cache.view(8, 2 * D)
+    assert bool((rows[[1, 2, 3, 4, 7]] == 0).all()) and torch.equal(rows[[0, 5, 6], D:], v[[0, 4, 5], 0])
+
+
+def test_rope_of_no_tokens_and_refusals():
+    z = torch.zeros(0, 2, 64, device="cuda", dtype=torch.float16)
+    gpu_ops.rope_store_kv(z, z, z, torch.zeros(0, dtype=torch.int64, device="cuda"), _cos_sin(4, 64), None, (None, None), 0)
+    q = torch.zeros(3, 2, 64, device="cuda", dtype=torch.float16)
+    pos, cs = torch.zeros(3, dtype=torch.int64, device="cuda"), _cos_sin(4, 64)
+    for kw, match in ((dict(sections=(16, 16)), "row per axis"), (dict(sections=(30,)), "add up"),
+                      (dict(q_out=q[:2]), "shape")):
+        with pytest.raises(RuntimeError, match=match):
+            gpu_ops.rope_store_kv(q, q, q, pos, cs, None, (None, None), 0, **kw)
+    for args, match in (((q, q, q.float(), pos, cs), "dtype"), ((q, q, q, pos.int(), cs), "int64"),
+                        ((q, q, q, pos, cs.double()), "fp32"), ((q, q, q, pos[:2], cs), "int64"),
+                        ((q, q[:2], q[:2], pos, cs), "KVH")):
+        with pytest.raises(RuntimeError, match=match):
+            gpu_ops.rope_store_kv(*args, None, (None, None), 0)
+    with pytest.raises(RuntimeError, match="tier is required"):
+        gpu_ops.rope_store_kv(q, q, q, pos, cs, pos, (None, None), 0)
+
+
+# ------------------------------------------------------------------ attention
+
+
+def _rounded(dtype):
+    return dtype != torch.float32
+
+
+def _paged(kl, KVH, D, block, dtype, g, host_share=0.0, pad=0):
+    """A cache whose blocks hold the requests' K/V and NaN everywhere else."""
+    held = [-(-x // block) for x in kl]
+    total = sum(held) + 3
+    n_host = int(total * host_share)
+    n_hbm = total - n_host
+    cache = torch.full((n_hbm, block, KVH, 2 * D + pad), NAN, device="cuda").to(dtype)
+    hk = torch.full((max(1, n_host), KVH, block, D), NAN).to(dtype)
+    hv = hk.clone()
+    perm = torch.randperm(total, generator=torch.Generator().manual_seed(5)).tolist()
+    W = max(held) + 2
+    table = torch.full((len(kl), W), 1 << 29, dtype=torch.int32)  # unused entries are never read
+    keys, vals = [], []
+    for r, n in enumerate(kl):
+        k = torch.randn(n, KVH, D, generator=g, device="cuda").to(dtype)
+        v = torch.randn(n, KVH, D, generator=g, device="cuda").to(dtype)
+        keys.append(k)
+        vals.append(v)
+        kc, vc = k.cpu(), v.cpu()
+        for b in range(held[r]):
+            i = perm.pop()
+            table[r, b] = i
+            lo, hi = b * block, min(n, (b + 1) * block)
+            if i < n_hbm:
+                cache[i, :hi - lo, :, :D], cache[i, :hi - lo, :, D:2 * D] = k[lo:hi], v[lo:hi]
+            else:
+                hk[i - n_hbm, :, :hi - lo] = kc[lo:hi].transpose(0, 1)
+                hv[i - n_hbm, :, :hi - lo] = vc[lo:hi].transpose(0, 1)
+    lg = cache.permute(0, 2, 1, 3)
+    tiers = (KVTier(lg[..., :D], lg[..., D:2 * D]), KVTier(hk.pin_memory(), hv.pin_memory()) if n_host else None)
+    return keys, vals, table.cuda(), tiers, n_hbm
+
+
+def _queries(ql, H, D, dtype, g, gap=2):
+    start, at = [], 1
+    for n in ql:
+        start.append(at)
+        at += n + gap
+    T = at + 1
+    q = torch.randn(T, H + 1, D, generator=g, device="cuda").to(dtype)[:, :H]
+    covered = torch.zeros(T, dtype=torch.bool, device="cuda")
+    for s, n in zip(start, ql):
+        covered[s:s + n] = True
+    q.masked_fill_(~covered[:, None, None], NAN)  # rows of no request are never used
+    out = torch.full((T, H, D), NAN, device="cuda").to(dtype)
+    lse = torch.full((T, H), NAN, device="cuda").T
+    return q, start, out, lse
+
+
+def _refs(q, start, ql, keys, vals, limits, scale):
+    return [ref.attend(q[s:s + n], k, v, lim, scale) + (k.shape[0],)
+            for s, n, k, v, lim in zip(start, ql, keys, vals, limits)]
+
+
+LENS = {
+    "edges": ([1, 0, 3, 1, 5, 130, 2], [1, 4, 3, 700, 2, 130, 0]),
+    "verify": ([4, 7, 1, 5], [1000, 33, 129, 2049]),
+    "one": ([3], [5000]),
+    "chunks": ([300, 65, 257], [300, 1100, 640]),
+}
+
+
+@pytest.mark.parametrize("dtype,H,KVH,D,block,host,lens", [
+    (torch.bfloat16, 8, 2, 128, 16, 0.0, "edges"), (torch.bfloat16, 8, 2, 128, 16, 0.0, "verify"),
+    (torch.bfloat16, 8, 2, 128, 16, 0.0, "chunks"), (torch.bfloat16, 32, 8, 128, 16, 0.0, "one"),
+    (torch.float16, 4, 4, 64, 16, 0.0, "edges"), (torch.float16, 8, 1, 64, 32, 0.0, "chunks"),
+    (torch.float16, 8, 2, 128, 16, 0.4, "edges"), (torch.bfloat16, 8, 2, 128, 16, 0.4, "chunks"),
+    (torch.float16, 5, 1, 80, 24, 0.3, "edges"), (torch.bfloat16, 14, 2, 96, 8, 0.0, "chunks"),
+    (torch.bfloat16, 6, 2, 72, 1, 0.2, "verify"), (torch.float16, 3, 1, 40, 16, 0.0, "edges"),
+    (torch.bfloat16, 20, 4, 128, 64, 0.0, "chunks"), (torch.float16, 64, 1, 128, 16, 0.0, "verify"),
+    (torch.bfloat16, 4, 2, 8, 5, 0.0, "edges"), (torch.bfloat16, 8, 2, 192, 16, 0.3, "edges"),
+    (torch.float16, 4, 1, 256, 16, 0.0, "chunks"), (torch.float32, 8, 2, 64, 16, 0.3, "edges"),
+    (torch.float32, 8, 2, 128, 16, 0.0, "verify"), (torch.float32, 4, 4, 256, 24, 0.0, "edges"),
+    (torch.float32, 6, 2, 36, 16, 0.0, "chunks"), (torch.float32, 64, 1, 64, 16, 0.0, "verify"),
+])
+def test_chunk_attention(dtype, H, KVH, D, block, host, lens):
+    ql, kl = LENS[lens]
+    g = torch.Generator(device="cuda").manual_seed(H * D + block)
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, block, dtype, g, host, pad=8 if dtype != torch.float32 else 4)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    scale = D ** -0.5
+    lim = [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)]
+    refs = _refs(q, start, ql, keys, vals, lim, scale)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), scale, out, lse, max_q_len=max(ql),
+                       max_k_len=max(kl))
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
+    # table rows in another order, no bounds, no lse: the same result
+    order = list(range(len(ql)))[::-1]
+    out2 = torch.full_like(out, NAN)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table[order].contiguous(), i32(start), i32(ql), i32(kl), scale, out2,
+                       bt_row=i32([order.index(r) for r in range(len(ql))]))
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out2, None, refs, start, ql, dtype, D, _rounded(dtype))
+
+
+@pytest.mark.parametrize("dtype,H,KVH,D", [
+    (torch.bfloat16, 8, 2, 128), (torch.float16, 20, 20, 64), (torch.float16, 5, 1, 80), (torch.bfloat16, 7, 1, 112),
+    (torch.float32, 4, 4, 64), (torch.float32, 8, 1, 128), (torch.bfloat16, 4, 2, 256),
+])
+@pytest.mark.parametrize("lens", ["edges", "verify", "chunks"])
+def test_cross_attention(dtype, H, KVH, D, lens):
+    ql, kl = LENS[lens]
+    g = torch.Generator(device="cuda").manual_seed(H * D)
+    S = sum(kl) + 9
+    kv = torch.randn(S, KVH, 2 * D, generator=g, device="cuda").to(dtype)
+    k_start = [3 + sum(kl[:i]) for i in range(len(kl))]
+    k_start[-1] = min(k_start[-1], 2)  # shares the first requests' states
+    used = torch.zeros(S, dtype=torch.bool, device="cuda")
+    for s, n in zip(k_start, kl):
+        used[s:s + n] = True
+    kv.masked_fill_(~used[:, None, None], NAN)
+    k, v = kv[..., :D], kv[..., D:]
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    lim = [torch.full((n,), x - 1, device="cuda") for n, x in zip(ql, kl)]
+    refs = _refs(q, start, ql, [k[s:s + n] for s, n in zip(k_start, kl)], [v[s:s + n] for s, n in zip(k_start, kl)], lim,
+                 0.11)
+    gpu_ops.cross_attn(q, k, v, i32(start), i32(ql), i32(k_start), i32(kl), 0.11, out, lse)
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_many_requests_more_than_one_scan_round(dtype):
+    rnd = random.Random(3)
+    n = 700
+    ql = [rnd.choice([0, 1, 2, 40]) for _ in range(n)]
+    kl = [rnd.choice([0, q, q + rnd.randint(0, 90)]) for q in ql]
+    g = torch.Generator(device="cuda").manual_seed(1)
+    H, KVH, D = 4, 2, 64
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
+    q, start, out, lse = _queries(ql, H, D, dtype, g, gap=0)
+    refs = _refs(q, start, ql, keys, vals, [k - m + torch.arange(m, device="cuda") for m, k in zip(ql, kl)], 0.125)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), 0.125, out, lse)
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_scores_far_apart(dtype):
+    """Rows whose maximum grows late and by a lot, and rows of equal scores."""
+    H, KVH, D, nk = 4, 1, 64, 700
+    g = torch.Generator(device="cuda").manual_seed(2)
+    keys, vals, table, tiers, n_hbm = _paged([nk], KVH, D, 16, dtype, g)
+    q, start, out, lse = _queries([6], H, D, dtype, g)
+    q[1:7, 0] *= 40
+    q[1:7, 1] = 0
+    refs = _refs(q, start, [6], keys, vals, [nk - 6 + torch.arange(6, device="cuda")], 0.7)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32([6]), i32([nk]), 0.7, out, lse)
+    ref.check_attn(out, lse, refs, start, [6], dtype, D, _rounded(dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_requests_that_do_not_fit_write_nothing(dtype):
+    H, KVH, D = 4, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(2)
+    ql, kl = [2, 3, 2, 2], [40, 30, 50, 20]
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    T = q.shape[0]
+    refs = _refs(q, start, ql, keys, vals, [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)], 0.1)
+    W = table.shape[1]
+    for bad in ([start, ql, [40, 30, 16 * W + 1, 20]], [start[:2] + [T - 1] + start[3:], ql, kl], [start, [2, 3, -1, 2], kl],
+                [start, ql, [40, 30, -5, 20]], [start[:2] + [-1] + start[3:], ql, kl]):
+        out.fill_(NAN)
+        lse.fill_(NAN)
+        gpu_ops.chunk_attn(q, tiers, n_hbm, table, *(i32(x) for x in bad), 0.1, out, lse)
+        with pytest.raises(RuntimeError, match="sequence length"):
+            gpu_ops.check_device_errors(dev())
+        some = [0, 1, 3]
+        ref.check_attn(out, lse, [refs[i] for i in some], [start[i] for i in some], [ql[i] for i in some], dtype, D,
+                       _rounded(dtype))
+    # a block id outside both tiers is not read, the others' rows are right
+    t2 = table.clone()
+    t2[2, 1] = n_hbm + 100
+    out.fill_(NAN)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, t2, i32(start), i32(ql), i32(kl), 0.1, out)
+    with pytest.raises(RuntimeError, match="block id"):
+        gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, None, [refs[i] for i in some], [start[i] for i in some], [ql[i] for i in some], dtype, D,
+                   _rounded(dtype), untouched=False)
+    k = torch.randn(50, KVH, D, device="cuda").to(dtype)
+    o2 = torch.full_like(out, NAN)
+    gpu_ops.cross_attn(q, k, k, i32(start), i32(ql), i32([0, 30, -1, 49]), i32([5, 21, 3, 2]), 0.1, o2)
+    with pytest.raises(RuntimeError, match="sequence length"):
+        gpu_ops.check_device_errors(dev())
+    assert bool(o2[start[1]:].isnan().all()) and not bool(o2[start[0]:start[0] + 2].isnan().any())
+
+
+def test_attention_refusals():
+    q = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
+    i, one = i32([0]), i32([1])
+    for args, match in (((q, q.float(), q, i, one, i, one), "alike|dtype"), ((q, q, q, i.long(), one, i, one), "int32"),
+                        ((q, q, q, i, one, i[:0], one), "int32"), ((q, q[..., :56], q[..., :56], i, one, i, one), "head")):
+        with pytest.raises(RuntimeError, match=match):
+            gpu_ops.cross_attn(*args, 1.0, torch.empty_like(q))
+    with pytest.raises(RuntimeError, match="lse"):
+        gpu_ops.cross_attn(q, q, q, i, one, i, one, 1.0, torch.empty_like(q), torch.empty(4, 2, device="cuda"))
+    with pytest.raises(RuntimeError, match="scale"):
+        gpu_ops.cross_attn(q, q, q, i, one, i, one, 0.0, torch.empty_like(q))
+    with pytest.raises(RuntimeError, match="workspace_buf"):
+        gpu_ops.cross_attn(q, q, q, i, one, i, one, 1.0, torch.empty_like(q),
+                           workspace_buf=torch.empty(16, dtype=torch.uint8, device="cuda"))
+    with pytest.raises(RuntimeError, match="row per request"):
+        gpu_ops.chunk_attn(q, (KVTier(q.view(1, 4, 2, 64), q.view(1, 4, 2, 64)), None), 1, i32([[0]]), i32([0, 1]),
+                           i32([1, 1]), i32([1, 1]), 1.0, torch.empty_like(q))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_two_streams_and_two_graphs_at_once(dtype):
+    """Calls share no scratch memory: two captured graphs replayed on two
+    streams at the same time give what each gives alone, bit for bit."""
+    H, KVH, D = 8, 2, 128
+    g = torch.Generator(device="cuda").manual_seed(4)
+    sides = []
+    for ql, kl in (([3, 5], [3000, 2000]), ([2, 4, 1], [2500, 100, 4000])):
+        keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
+        q, start, out, lse = _queries(ql, H, D, dtype, g)
+        args = (q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), 0.1)
+        gpu_ops.chunk_attn(*args, out, lse)
+        torch.cuda.synchronize()
+        alone = out.clone()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            gpu_ops.chunk_attn(*args, out, lse)
+        sides.append((graph, torch.cuda.Stream(), out, alone, args, lse))
+    for _ in range(20):
+        for graph, stream, out, *_ in sides:
+            with torch.cuda.stream(stream):
+                out.fill_(NAN)
+                graph.replay()
+    torch.cuda.synchronize()
+    for _, stream, out, alone, args, lse in sides:
+        assert torch.equal(torch.nan_to_num(out.float()), torch.nan_to_num(alone.float()))
+    for _ in range(20):
+        for _, stream, out, alone, args, lse in sides:
+            with torch.cuda.stream(stream):
+                gpu_ops.chunk_attn(*args, out, lse)
+    torch.cuda.synchronize()
+    for _, stream, out, alone, *_ in sides:
+        assert torch.equal(torch.nan_to_num(out.float()), torch.nan_to_num(alone.float()))
+
+
+# ------------------------------------------------------------------ together
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_steps_together(dtype, D):
+    """Several steps of a changing batch: tables from lengths, planned on the
+    GPU, rotated K/V written to both tiers, the new tokens attending over the
+    cache and over an encoder's states, all inputs staying on the device;
+    against dense attention over each request's own history."""
+    H, KVH, block, R, W = 8, 2, 16, 5, 24
+    hbm, host = 20, 60
+    g = torch.Generator(device="cuda").manual_seed(9)
+    cache = torch.full((hbm, block, KVH, 2 * D), NAN, device="cuda").to(dtype)
+    lg = cache.permute(0, 2, 1, 3)
+    hk = torch.full((host, KVH, block, D), NAN).to(dtype).pin_memory()
+    tiers = (KVTier(lg[..., :D], lg[..., D:]), KVTier(hk, hk.clone().pin_memory()))
+    table = torch.full((R, W), -1, dtype=torch.int32, device="cuda")
+    lens = torch.zeros(R, dtype=torch.int32, device="cuda")
+    free = FreeBlocks(torch.zeros(hbm, dtype=torch.int32, device="cuda"), torch.zeros(host, dtype=torch.int32, device="cuda"),
+                      i32([hbm, host]))
+    free.hbm.copy_(torch.arange(hbm))
+    free.host.copy_(hbm + torch.arange(host))
+    enc_len, enc_start = [90, 1, 200, 33, 64], [0, 90, 91, 291, 324]
+    enc_k = torch.randn(400, KVH, D, generator=g, device="cuda").to(dtype)
+    enc_v = torch.randn(400, KVH, D, generator=g, device="cuda").to(dtype)
+    cs = _cos_sin(600, D)
+    axis = gpu_ops.rope_axes((D // 4, D // 8, D // 8))
+    hist = [([], []) for _ in range(R)]
+    out_tabs = StepTables(R, 700, dev(), seq_lens=lens, counts=free.counts)
+    steps = [[100, 1, 257, 0, 40], [1, 4, 1, 70, 5], [5, 5, -1, 1, 0], [3, 1, 60, -1, 8], [1, 1, 1, 1, 1]]
+    for new in steps:
+        qsl_before = [0]
+        for n in new:
+            qsl_before.append(qsl_before[-1] + max(0, n))
+        T = qsl_before[-1]
+        gpu_ops.extend_tables(i32(new), lens, table, free, hbm, host, block, out_tabs)
+        plan.plan_on_device(out_tabs.query_start_loc, lens, table, out_tabs.slot_mapping, hbm, host, block, max_tokens=T)
+        if max(new) > 1:  # the planner's own refusal of extended requests in the host tier is expected here
+            gpu_ops.error_word(dev()).zero_()
+        q, k, v = (torch.randn(T, h, D, generator=g, device="cuda").to(dtype) for h in (H, KVH, KVH))
+        pos = out_tabs.positions[:T].expand(3, T).contiguous()
+        k_rot, q_in = torch.empty_like(k), q.clone()
+        gpu_ops.rope_store_kv(q, k, v, pos, cs, out_tabs.slot_mapping[:T], tiers, hbm,
+                              sections=(D // 4, D // 8, D // 8), k_out=k_rot)
+        q_start = out_tabs.query_start_loc[:R]
+        q_len = i32([max(0, n) for n in new])
+        out, lse = torch.full((T, H, D), NAN, device="cuda").to(dtype), torch.full((H, T), NAN, device="cuda")
+        gpu_ops.chunk_attn(q, tiers, hbm, table, q_start, q_len, lens, D ** -0.5, out, lse)
+        out_x = torch.full_like(out, NAN)
+        gpu_ops.cross_attn(q, enc_k, enc_v, q_start, q_len, i32(enc_start), i32(enc_len), D ** -0.5, out_x)
+        gpu_ops.check_device_errors(dev())
+        _rope_ok(q, ref.rope(q_in, pos, cs, axis, False), q_in, dtype)
+        refs, refs_x = [], []
+        for r, n in enumerate(new):
+            a, b = qsl_before[r], qsl_before[r + 1]
+            if n < 0:
+                hist[r] = ([], [])
+            hist[r][0].append(k_rot[a:b])
+            hist[r][1].append(v[a:b])
+            kk, vv = torch.cat(hist[r][0]), torch.cat(hist[r][1])
+            assert int(lens[r]) == kk.shape[0]
+            refs.append(ref.attend(q[a:b], kk, vv, kk.shape[0] - (b - a) + torch.arange(b - a, device="cuda"), D ** -0.5)
+                        + (kk.shape[0],))
+            e, s = enc_len[r], enc_start[r]
+            refs_x.append(ref.attend(q[a:b], enc_k[s:s + e], enc_v[s:s + e], torch.full((b - a,), e - 1, device="cuda"),
+                                     D ** -0.5) + (e,))
+        ql = [max(0, n) for n in new]
+        ref.check_attn(out, lse, refs, qsl_before[:R], ql, dtype, D, True)
+        ref.check_attn(out_x, None, refs_x, qsl_before[:R], ql, dtype, D, True)
+    assert bool((table >= hbm).any())  # the batch did spill

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 import threading
-from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_void_p
+from ctypes import POINTER, c_char_p, c_float, c_int32, c_int64, c_size_t, c_uint8, c_void_p
 from pathlib import Path
 
 from vllm_fastdecoder_b200.build import library_path
@@ -105,6 +105,53 @@ class FdPrefillArgs(ctypes.Structure):
     ]
 
 
+TABLES_HEADER_LEN = 8  # FD_TABLES_HEADER_LEN
+TABLES_FIELDS = {"flags": 0, "n_tok": 1, "taken_hbm": 2, "taken_host": 3, "freed_hbm": 4, "freed_host": 5, "max_seq": 6,
+                 "max_new": 7}
+TABLES_FLAGS = {1: "no free blocks", 2: "table too narrow", 4: "more tokens than max_tokens", 8: "bad length",
+                16: "bad block id", 32: "bad free stack"}
+ROPE_MAX_AXES, ROPE_MAX_PAIRS, ROPE_PAIRS = 4, 128, 1  # FD_ROPE_*
+
+
+class FdTablesArgs(ctypes.Structure):
+    _fields_ = [
+        ("new_lens", c_void_p), ("prior_lens", c_void_p), ("block_table", c_void_p), ("bt_stride", c_int64),
+        ("bt_width", c_int32), ("num_reqs", c_int32), ("free_ids", c_void_p * 2), ("free_cap", c_int32 * 2),
+        ("counts_in", c_void_p), ("counts_out", c_void_p), ("num_gpu_blocks", c_int64), ("num_cpu_blocks", c_int64),
+        ("block_size", c_int32), ("max_tokens", c_int32), ("seq_lens", c_void_p), ("query_start_loc", c_void_p),
+        ("slot_mapping", c_void_p), ("positions", c_void_p), ("header", c_void_p), ("error", c_void_p),
+    ]
+
+
+class FdRopeArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+        ("q_out", c_void_p), ("qo_stride_t", c_int64), ("qo_stride_h", c_int64),
+        ("k", c_void_p), ("k_stride_t", c_int64), ("k_stride_h", c_int64),
+        ("v", c_void_p), ("v_stride_t", c_int64), ("v_stride_h", c_int64),
+        ("k_out", c_void_p), ("ko_stride_t", c_int64), ("ko_stride_h", c_int64),
+        ("positions", c_void_p), ("pos_stride", c_int64), ("cos_sin", c_void_p), ("max_pos", c_int64),
+        ("slots", c_void_p), ("tier", FdKvTier * 2), ("tier_split", c_int64),
+        ("num_tokens", c_int32), ("num_heads", c_int32), ("num_kv_heads", c_int32), ("head_size", c_int32),
+        ("rot_dim", c_int32), ("block_size", c_int32), ("dtype", c_int32), ("num_axes", c_int32), ("flags", c_int32),
+        ("axis_of_pair", c_uint8 * ROPE_MAX_PAIRS), ("_pad0", c_int32), ("error", c_void_p),
+    ]
+
+
+class FdAttnArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", c_void_p), ("q_stride_t", c_int64), ("q_stride_h", c_int64),
+        ("out", c_void_p), ("out_stride_t", c_int64), ("out_stride_h", c_int64),
+        ("lse", c_void_p), ("lse_stride_h", c_int64), ("lse_stride_t", c_int64),
+        ("tier", FdKvTier * 2), ("tier_split", c_int64), ("block_table", c_void_p), ("bt_stride", c_int64),
+        ("bt_row", c_void_p), ("k_start", c_void_p), ("q_start", c_void_p), ("q_len", c_void_p), ("k_len", c_void_p),
+        ("bt_width", c_int32), ("num_tokens", c_int32), ("n", c_int32), ("num_heads", c_int32),
+        ("num_kv_heads", c_int32), ("head_size", c_int32), ("block_size", c_int32), ("scale", c_float),
+        ("dtype", c_int32), ("max_q_len", c_int32), ("max_k_len", c_int32), ("_pad0", c_int32),
+        ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("error", c_void_p),
+    ]
+
+
 class FdPeerExchange(ctypes.Structure):
     _fields_ = [("base", c_void_p * MAX_PEERS), ("rank", c_int32), ("world", c_int32), ("slot_floats", c_int64)]
 
@@ -153,6 +200,15 @@ SIGNATURES = {
     "fd_plan_args_bytes": (c_size_t, []),
     "fd_prefill_attn": (c_int32, [POINTER(FdPrefillArgs), c_void_p]),
     "fd_prefill_args_bytes": (c_size_t, []),
+    # void *: these take their struct as packed bytes (gpu_ops) or byref()
+    "fd_extend_tables": (c_int32, [c_void_p, c_void_p]),
+    "fd_tables_args_bytes": (c_size_t, []),
+    "fd_rope_store_kv": (c_int32, [c_void_p, c_void_p]),
+    "fd_rope_args_bytes": (c_size_t, []),
+    "fd_attn_workspace_size": (c_size_t, [POINTER(FdAttnArgs)]),
+    "fd_chunk_attn": (c_int32, [c_void_p, c_void_p]),
+    "fd_cross_attn": (c_int32, [c_void_p, c_void_p]),
+    "fd_attn_args_bytes": (c_size_t, []),
     "fd_version": (c_int32, []),
     "fd_abi_sizes": (c_int32, [POINTER(c_size_t), POINTER(c_size_t)]),
 }

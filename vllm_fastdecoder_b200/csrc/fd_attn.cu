@@ -1,0 +1,459 @@
+// Chunk and cross attention on the CUDA cores, the combine of cut items, and
+// the host side of both entry points.
+//
+// fd_attn_kernel takes what the tensor-core kernel (fd_attn_mma.cu) does not:
+// fp32, and 16-bit heads of more than 128 dims.  With q the tile's rows and j
+// its keys, for every key tile
+//   s = scale log2(e) q.K^T,  m' = max(m, max_j s),  p = 2^(s - m'),
+//   l = l 2^(m - m') + sum_j p,  O = O 2^(m - m') + p V
+// and o = O / l, lse = ln 2 (m + log2 l), all in fp32.  A CTA of 16 x 16
+// threads holds 64 rows and 32 keys in shared memory as fp32; thread (y, x)
+// owns rows 4 y .. 4 y + 3: two scores of each (keys x and x + 16), and D / 16
+// dims of O in registers, so a float4 from shared memory feeds 4 x 2 or 4 x 4
+// FMAs and the fp32 pipe and the shared-memory reads are about evenly loaded.
+// The K/V rows of the next tile are fetched into registers during this one.
+
+#include <math.h>
+
+#include "fd_attn.cuh"
+
+namespace fdk {
+namespace at {
+
+constexpr int kRows = 64;   // rows per tile
+constexpr int kKeys = 32;   // keys per tile
+constexpr int kThreads = 256;
+constexpr int kFixed = 2;   // an item's fixed cost in key tiles
+constexpr int kMinPer = 4;  // least positions of a CTA
+constexpr int kMaxCtas = 320;
+typedef Sched<kKeys, false, kFixed> Walk;
+
+constexpr int smem_bytes(int DP) { return ((kRows + 2 * kKeys) * (DP + 4) + kRows * (kKeys + 1)) * 4; }
+
+// Byte offset of K (and V) row j of the request for kv head kh within its tier,
+// -1 when there is none (behind klen, or a block id outside both tiers).
+__device__ __forceinline__ int64_t key_offset(const AttnParams& p, const Req& q, int kh, int j, int* tier) {
+  *tier = 0;
+  if (j >= q.klen) return -1;
+  if (p.bt == nullptr) return ((int64_t)q.kbase + j) * p.tok_sb[0] + kh * p.head_sb[0];
+  int64_t id = p.bt[(int64_t)q.kbase * p.bt_stride + j / p.BS];
+  int t = 0;
+  if (id >= p.split) {
+    t = 1;
+    id -= p.split;
+  }
+  if (id < 0 || id >= p.nblk[t]) {
+    set_error(p.err, FD_DEVERR_BLOCK_ID);
+    return -1;
+  }
+  *tier = t;
+  return id * p.blk_sb[t] + kh * p.head_sb[t] + (int64_t)(j % p.BS) * p.tok_sb[t];
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(const __grid_constant__ AttnParams p) {
+  constexpr int VE = 16 / (int)sizeof(T);      // elements per 16-byte load
+  constexpr int LD = DP + 4;                   // row stride of the tiles (floats)
+  constexpr int kVecs = kKeys * DP / VE / kThreads;  // 16-byte loads of K (and of V) per thread
+  constexpr int kDim4 = DP / 64;               // float4 of O per row and thread
+  extern __shared__ float4 smem4[];
+  float* sq = reinterpret_cast<float*>(smem4);
+  float* sk = sq + kRows * LD;
+  float* sv = sk + kKeys * LD;
+  float* sp = sv + kKeys * LD;  // [kRows][kKeys + 1]
+  __shared__ Walk::Scratch scratch;
+  __shared__ const unsigned char* k_row[kKeys];
+  __shared__ const unsigned char* v_row[kKeys];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+  const int cta = blockIdx.x;
+  const int D = p.D, nvec = D / VE;
+
+  if (tid == 0) p.cuts[cta].nparts = 0;
+  Walk walk(p);
+  if (!walk.init<kThreads>(&scratch, cta, kMinPer)) return;
+  Walk::Seg g;
+  while (walk.next(g)) {
+    const Req rq = walk.seg_q;
+    const int tok0 = g.tile0 * p.tq;
+    const int rows = min(p.tq, rq.qlen - tok0) * p.G;
+    // the query rows as fp32 (zeros behind them and behind D)
+    __syncthreads();  // the last segment's reads of shared memory are done
+    for (int x = tid; x < kRows * (DP / VE); x += kThreads) {
+      const int row = x / (DP / VE), c = x % (DP / VE);
+      float f[VE];
+#pragma unroll
+      for (int e = 0; e < VE; ++e) f[e] = 0.f;
+      if (row < rows && c < nvec)
+        Dt<T>::widen(*reinterpret_cast<const uint4*>(p.q + (int64_t)(rq.qst + tok0 + row / p.G) * p.q_st +
+                                                     (int64_t)(g.kh * p.G + row % p.G) * p.q_sh + c * 16),
+                     f);
+#pragma unroll
+      for (int e = 0; e < VE; e += 4)
+        *reinterpret_cast<float4*>(sq + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+    }
+    const bool active = (ty & ~1) * 4 < rows;  // some row of this warp is real
+    int lim[4];                                // last key that each row sees
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * ty + i;
+      lim[i] = row >= rows ? -1 : p.bt != nullptr ? rq.klen - rq.qlen + tok0 + row / p.G : rq.klen - 1;
+    }
+    float m[4], l[4];
+    float4 o[4][kDim4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+#pragma unroll
+      for (int d = 0; d < kDim4; ++d) o[i][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    uint4 kr[kVecs], vr[kVecs];
+    auto fetch = [&](int j) {  // all threads: the rows of key tile j into registers
+      if (tid < kKeys) {
+        int t;
+        const int64_t at = key_offset(p, rq, g.kh, j * kKeys + tid, &t);
+        k_row[tid] = at < 0 ? nullptr : p.k[t] + at;
+        v_row[tid] = at < 0 ? nullptr : p.v[t] + at;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) {
+        const int i = tid + x * kThreads, row = i / (DP / VE), c = i % (DP / VE);
+        const bool real = c < nvec && k_row[row] != nullptr;
+        kr[x] = real ? *reinterpret_cast<const uint4*>(k_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+        vr[x] = real ? *reinterpret_cast<const uint4*>(v_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+      }
+    };
+    if (g.j0 < g.j1) fetch(g.j0);
+    for (int j = g.j0; j < g.j1; ++j) {
+      __syncthreads();  // the last tile's reads are done
+#pragma unroll
+      for (int x = 0; x < kVecs; ++x) {
+        const int i = tid + x * kThreads, row = i / (DP / VE), c = i % (DP / VE);
+        float f[VE];
+        Dt<T>::widen(kr[x], f);
+#pragma unroll
+        for (int e = 0; e < VE; e += 4)
+          *reinterpret_cast<float4*>(sk + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+        Dt<T>::widen(vr[x], f);
+#pragma unroll
+        for (int e = 0; e < VE; e += 4)
+          *reinterpret_cast<float4*>(sv + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      }
+      __syncthreads();
+      if (j + 1 < g.j1) fetch(j + 1);
+      if (!active) continue;
+      float s[4][2];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        const float4 b0 = *reinterpret_cast<const float4*>(sk + tx * LD + d);
+        const float4 b1 = *reinterpret_cast<const float4*>(sk + (tx + 16) * LD + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float4 a = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * LD + d);
+          s[i][0] = fmaf(a.x, b0.x, fmaf(a.y, b0.y, fmaf(a.z, b0.z, fmaf(a.w, b0.w, s[i][0]))));
+          s[i][1] = fmaf(a.x, b1.x, fmaf(a.y, b1.y, fmaf(a.z, b1.z, fmaf(a.w, b1.w, s[i][1]))));
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int key = j * kKeys + tx;
+        s[i][0] = key <= lim[i] ? s[i][0] * p.sl2 : -INFINITY;
+        s[i][1] = key + 16 <= lim[i] ? s[i][1] * p.sl2 : -INFINITY;
+        float mx = fmaxf(s[i][0], s[i][1]);
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+        const float mn = fmaxf(m[i], mx);
+        const float base = mn == -INFINITY ? 0.f : mn;  // no key seen so far: every p is 2^-inf = 0
+        const float alpha = exp2f(m[i] - base);
+        const float p0 = exp2f(s[i][0] - base), p1 = exp2f(s[i][1] - base);
+        float sum = p0 + p1;
+#pragma unroll
+        for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
+        l[i] = l[i] * alpha + sum;
+        m[i] = mn;
+        sp[(4 * ty + i) * (kKeys + 1) + tx] = p0;
+        sp[(4 * ty + i) * (kKeys + 1) + tx + 16] = p1;
+#pragma unroll
+        for (int d = 0; d < kDim4; ++d) {
+          o[i][d].x *= alpha;
+          o[i][d].y *= alpha;
+          o[i][d].z *= alpha;
+          o[i][d].w *= alpha;
+        }
+      }
+      __syncwarp();  // a row's scores are written and read by one half-warp
+#pragma unroll 4
+      for (int c = 0; c < kKeys; ++c) {
+        float4 b[kDim4];
+#pragma unroll
+        for (int d = 0; d < kDim4; ++d) b[d] = *reinterpret_cast<const float4*>(sv + c * LD + 64 * d + 4 * tx);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float a = sp[(4 * ty + i) * (kKeys + 1) + c];
+#pragma unroll
+          for (int d = 0; d < kDim4; ++d) {
+            o[i][d].x = fmaf(a, b[d].x, o[i][d].x);
+            o[i][d].y = fmaf(a, b[d].y, o[i][d].y);
+            o[i][d].z = fmaf(a, b[d].z, o[i][d].z);
+            o[i][d].w = fmaf(a, b[d].w, o[i][d].w);
+          }
+        }
+      }
+    }
+    // the rows' results, or this segment's partials
+    const int slot = 2 * cta + (g.j0 > 0 ? 0 : 1);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int row = 4 * ty + i;
+      if (row >= rows) continue;
+      const int64_t tok = rq.qst + tok0 + row / p.G;
+      const int h = g.kh * p.G + row % p.G;
+      if (!g.whole) {
+        float* po = p.part_o + ((int64_t)slot * kRows + row) * D;
+        if (tx == 0) {
+          p.part_ml[((int64_t)slot * kRows + row) * 2] = m[i];
+          p.part_ml[((int64_t)slot * kRows + row) * 2 + 1] = l[i];
+        }
+#pragma unroll
+        for (int d = 0; d < kDim4; ++d)
+          if (64 * d + 4 * tx < D) *reinterpret_cast<float4*>(po + 64 * d + 4 * tx) = o[i][d];
+        continue;
+      }
+      const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+      if (tx == 0 && p.lse != nullptr)
+        p.lse[h * p.lse_sh + tok * p.lse_st] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+      T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
+#pragma unroll
+      for (int d = 0; d < kDim4; ++d) {
+        const int c = 64 * d + 4 * tx;
+        if (c >= D) continue;
+        const float f[4] = {o[i][d].x * inv, o[i][d].y * inv, o[i][d].z * inv, o[i][d].w * inv};
+        T t[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t[e] = Dt<T>::narrow(f[e]);
+        if (sizeof(T) == 4)
+          *reinterpret_cast<uint4*>(po + c) = *reinterpret_cast<const uint4*>(t);
+        else
+          *reinterpret_cast<uint2*>(po + c) = *reinterpret_cast<const uint2*>(t);
+      }
+    }
+    if (g.nparts > 0 && tid == 0) p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, rows, g.kh};
+  }
+}
+
+// The cut items' partials joined: o = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m),
+// parts in ascending CTA order.  CTA (c, y) takes rows 8 y .. of the item
+// whose first part CTA c wrote, one warp per row, so a long item's parts are
+// read by many SMs at once; it is a programmatic dependent of the attention
+// kernel, whose end it awaits.
+constexpr int kCombineWarps = 8;
+template <typename T>
+__global__ void __launch_bounds__(kCombineWarps * 32) fd_attn_combine_kernel(const __grid_constant__ AttnParams p,
+                                                                             int item_rows) {
+  griddep_wait();
+  const int c = blockIdx.x;
+  const Cut cut = p.cuts[c];
+  if (cut.nparts == 0) return;
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5);
+  if (row >= cut.rows) return;
+  // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
+  auto at = [&](int i) { return ((int64_t)(2 * (c + i) + (i == 0 ? 1 : 0))) * item_rows + row; };
+  float m = -INFINITY;
+  for (int i = lane; i < cut.nparts; i += 32) m = fmaxf(m, p.part_ml[2 * at(i)]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+  const float base = m == -INFINITY ? 0.f : m;
+  float l = 0.f;
+  for (int i = 0; i < cut.nparts; ++i) l += p.part_ml[2 * at(i) + 1] * exp2f(p.part_ml[2 * at(i)] - base);
+  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const int64_t tok = cut.row0 + row / p.G;
+  const int h = cut.kh * p.G + row % p.G;
+  if (lane == 0 && p.lse != nullptr)
+    p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
+  for (int d = 4 * lane; d < p.D; d += 128) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int i = 0; i < cut.nparts; ++i) {
+      const float w = exp2f(p.part_ml[2 * at(i)] - base);
+      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at(i) * p.D + d);
+      acc.x = fmaf(w, x.x, acc.x);
+      acc.y = fmaf(w, x.y, acc.y);
+      acc.z = fmaf(w, x.z, acc.z);
+      acc.w = fmaf(w, x.w, acc.w);
+    }
+    const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+    T t[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) t[e] = Dt<T>::narrow(f[e]);
+    if (sizeof(T) == 4)
+      *reinterpret_cast<uint4*>(po + d) = *reinterpret_cast<const uint4*>(t);
+    else
+      *reinterpret_cast<uint2*>(po + d) = *reinterpret_cast<const uint2*>(t);
+  }
+}
+
+int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + kCombineWarps - 1) / kCombineWarps));
+  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  const void* kern = dtype == FD_DTYPE_F16    ? reinterpret_cast<const void*>(fd_attn_combine_kernel<__half>)
+                     : dtype == FD_DTYPE_BF16 ? reinterpret_cast<const void*>(fd_attn_combine_kernel<__nv_bfloat16>)
+                                              : reinterpret_cast<const void*>(fd_attn_combine_kernel<float>);
+  void* args[2] = {const_cast<AttnParams*>(&p), &rows};
+  return fdh::cuda_status(cudaLaunchKernelExC(&cfg, kern, args), "fd_attn_combine_kernel launch");
+}
+
+namespace {
+
+size_t core_workspace(const fd_attn_args* a) {
+  const size_t slots = 2 * (size_t)kMaxCtas * kRows;
+  return kMaxCtas * sizeof(Cut) + slots * 2 * 4 + slots * (size_t)a->head_size * 4;
+}
+
+template <typename T, int DP>
+int core_launch_dp(AttnParams& p, int dtype, cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(fd_attn_kernel<T, DP>);
+  static unsigned long long done = 0;
+  int st = fdh::ensure_smem(kern, smem_bytes(DP), &done);
+  if (st != FD_OK) return st;
+  int dev = 0, sms = 0;
+  st = fdh::device_sms(&dev, &sms);
+  if (st != FD_OK) return st;
+  p.ctas = sms * (DP <= 128 ? 2 : 1);
+  if (p.ctas > kMaxCtas) p.ctas = kMaxCtas;
+  const dim3 grid((unsigned)p.ctas);
+  st = fdh::launch_maybe_pdl(kern, grid, dim3(kThreads), smem_bytes(DP), s, false, p, "fd_attn_kernel launch");
+  if (st != FD_OK) return st;
+  return combine_launch(p, dtype, kRows, s);
+}
+
+template <typename T>
+int core_launch(AttnParams& p, int dtype, cudaStream_t s) {
+  if (p.D <= 64) return core_launch_dp<T, 64>(p, dtype, s);
+  if (p.D <= 128) return core_launch_dp<T, 128>(p, dtype, s);
+  return core_launch_dp<T, 256>(p, dtype, s);
+}
+
+// Shared checks and parameters; `what` names the entry point in messages.
+int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream) {
+  if (a == nullptr) return fdh::fail(FD_ERR_INVALID, "%s: null args", what);
+  const int es = fdh::elem_size(a->dtype);
+  if (es == 0) return fdh::fail(FD_ERR_UNSUPPORTED, "%s: unsupported dtype %d", what, a->dtype);
+  if (a->n < 0 || a->num_tokens < 0) return fdh::fail(FD_ERR_INVALID, "%s: negative n or num_tokens", what);
+  if (a->n > 65535) return fdh::fail(FD_ERR_UNSUPPORTED, "%s: %d requests (at most 65535)", what, a->n);
+  if (a->num_kv_heads <= 0 || a->num_heads <= 0 || a->num_heads % a->num_kv_heads != 0)
+    return fdh::fail(FD_ERR_INVALID, "%s: num_heads must be a multiple of num_kv_heads", what);
+  const int G = a->num_heads / a->num_kv_heads;
+  if (G > kRows) return fdh::fail(FD_ERR_UNSUPPORTED, "%s: query group %d (at most %d)", what, G, kRows);
+  if (a->head_size <= 0 || a->head_size > 256)
+    return fdh::fail(FD_ERR_UNSUPPORTED, "%s: head_size must be 1 to 256", what);
+  if (((int64_t)a->head_size * es) % 16 != 0)
+    return fdh::fail(FD_ERR_ALIGN, "%s: head_size*elem_size must be a multiple of 16", what);
+  if (!(a->scale > 0.f) || !(a->scale < 3.0e38f))
+    return fdh::fail(FD_ERR_INVALID, "%s: scale must be positive and finite", what);
+  if (a->n == 0 || a->num_tokens == 0) return FD_OK;
+  if (a->q == nullptr || a->out == nullptr || a->q_start == nullptr || a->q_len == nullptr || a->k_len == nullptr)
+    return fdh::fail(FD_ERR_INVALID, "%s: q, out, q_start, q_len and k_len are required", what);
+  if (chunk && (a->block_table == nullptr || a->bt_width <= 0 || a->bt_stride < 0 || a->block_size <= 0))
+    return fdh::fail(FD_ERR_INVALID, "%s: block_table, bt_width and block_size are required", what);
+  if (!chunk && (a->k_start == nullptr || a->tier[0].k == nullptr || a->tier[0].v == nullptr))
+    return fdh::fail(FD_ERR_INVALID, "%s: states and k_start are required", what);
+  if (!chunk && a->tier[0].host_mapped)
+    return fdh::fail(FD_ERR_UNSUPPORTED, "%s: states must be device memory", what);
+  if (!fdh::aligned16(a->q) || !fdh::aligned16(a->out) || (a->q_stride_t * es) % 16 != 0 ||
+      (a->q_stride_h * es) % 16 != 0 || (a->out_stride_t * es) % 16 != 0 || (a->out_stride_h * es) % 16 != 0)
+    return fdh::fail(FD_ERR_ALIGN, "%s: q / out pointers and strides must be 16-byte aligned", what);
+  AttnParams p{};
+  for (int t = 0; t < (chunk ? 2 : 1); ++t) {
+    const fd_kv_tier& tr = a->tier[t];
+    p.nblk[t] = tr.num_blocks > 0 ? tr.num_blocks : 0;
+    if (p.nblk[t] == 0) continue;
+    if (tr.k == nullptr || tr.v == nullptr)
+      return fdh::fail(FD_ERR_INVALID, "%s: tier %d has blocks but no K/V pointer", what, t);
+    if (!fdh::aligned16(tr.k) || !fdh::aligned16(tr.v) || (tr.blk_stride * es) % 16 != 0 ||
+        (tr.head_stride * es) % 16 != 0 || (tr.tok_stride * es) % 16 != 0)
+      return fdh::fail(FD_ERR_ALIGN, "%s: tier %d pointers/strides must be 16-byte aligned", what, t);
+    p.k[t] = static_cast<const unsigned char*>(tr.k);
+    p.v[t] = static_cast<const unsigned char*>(tr.v);
+    p.blk_sb[t] = tr.blk_stride * es;
+    p.head_sb[t] = tr.head_stride * es;
+    p.tok_sb[t] = tr.tok_stride * es;
+    p.host[t] = tr.host_mapped ? 1 : 0;
+  }
+  p.split = chunk ? a->tier_split : 0;
+  p.q = static_cast<const unsigned char*>(a->q);
+  p.out = static_cast<unsigned char*>(a->out);
+  p.lse = a->lse;
+  p.q_st = a->q_stride_t * es;
+  p.q_sh = a->q_stride_h * es;
+  p.o_st = a->out_stride_t * es;
+  p.o_sh = a->out_stride_h * es;
+  p.lse_sh = a->lse_stride_h;
+  p.lse_st = a->lse_stride_t;
+  p.bt = chunk ? a->block_table : nullptr;
+  p.bt_stride = a->bt_stride;
+  p.bt_row = a->bt_row;
+  p.k_start = a->k_start;
+  p.q_start = a->q_start;
+  p.q_len = a->q_len;
+  p.k_len = a->k_len;
+  p.bt_width = a->bt_width;
+  p.n = a->n;
+  p.T = a->num_tokens;
+  p.H = a->num_heads;
+  p.KVH = a->num_kv_heads;
+  p.G = G;
+  p.D = a->head_size;
+  p.BS = chunk ? a->block_size : 1;
+  p.sl2 = a->scale * kLog2e;
+  p.err = a->error;
+  const size_t need = fd_attn_workspace_size(a);
+  if (a->workspace == nullptr || a->workspace_bytes < need || !fdh::aligned16(a->workspace))
+    return fdh::fail(FD_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (mma_covers(a)) return mma_launch(p, a, s);
+  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
+  p.cuts = reinterpret_cast<Cut*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + kMaxCtas * sizeof(Cut));
+  p.part_o = p.part_ml + 2 * (size_t)kMaxCtas * kRows * 2;
+  p.tq = kRows / G;
+  switch (a->dtype) {
+    case FD_DTYPE_F16:
+      return core_launch<__half>(p, a->dtype, s);
+    case FD_DTYPE_BF16:
+      return core_launch<__nv_bfloat16>(p, a->dtype, s);
+    default:
+      return core_launch<float>(p, a->dtype, s);
+  }
+}
+
+}  // namespace
+}  // namespace at
+}  // namespace fdk
+
+extern "C" size_t fd_attn_workspace_size(const fd_attn_args* a) {
+  if (a == nullptr || a->head_size <= 0 || a->head_size > 256) return 0;
+  const size_t b = fdk::at::mma_covers(a) ? fdk::at::mma_workspace(a) : fdk::at::core_workspace(a);
+  return (b + 255) / 256 * 256;
+}
+
+extern "C" int fd_chunk_attn(const fd_attn_args* a, void* stream) {
+  return fdk::at::attn_impl(a, true, "fd_chunk_attn", stream);
+}
+
+extern "C" int fd_cross_attn(const fd_attn_args* a, void* stream) {
+  return fdk::at::attn_impl(a, false, "fd_cross_attn", stream);
+}
+
+extern "C" size_t fd_attn_args_bytes(void) { return sizeof(fd_attn_args); }

@@ -1,0 +1,310 @@
+// Chunk and cross attention: what the tensor-core kernel (fd_attn_mma.cu), the
+// CUDA-core kernel and the combine (fd_attn.cu) share: parameters, the
+// schedule, and the layout of the partials.
+//
+// Work.  The query tokens of a request are cut into tiles of `tq` tokens times
+// the G query heads of a kv head (row = token * G + head).  An ITEM is one
+// tile (or, with kPairs, two neighbouring tiles that share every K/V tile; an
+// odd last tile is an item of its own) of one request and kv head, over the n
+// key tiles of kt keys that its last query sees.  Items of all requests, kv
+// heads and tiles in that order form a line of POSITIONS: an item takes w
+// (its fixed cost: the query load, the pipeline's start, the epilogue) plus u
+// per key tile (u = 2 for a pair, else 1).
+//
+// Schedule.  The line is cut into equal ranges, one per CTA of a grid that
+// fills the GPU once, so a call with few queries over long keys and one with
+// many queries both load all SMs, and no CTA waits for another.  An item cut by a range's end leaves fp32
+// partials (O, m, l) of its rows that the combine kernel joins in ascending
+// CTA order: results do not depend on timing.  A CTA's range holds at most
+// one segment of an item that began earlier (slot 0) and one of an item that
+// ends later (slot 1); all others are whole and written directly.  The
+// lengths are device data, so each CTA finds its start itself: the cost of a
+// request is a closed form (sums of floor((a i + b) / c) by the Euclidean
+// recursion), one thread per request, then one scan.
+#pragma once
+
+#include "fd_common.cuh"
+#include "fd_internal.h"
+
+namespace fdk {
+namespace at {
+
+constexpr int kMaxLen = 1 << 30;  // q_len and k_len: the closed forms stay in 32 bits
+
+// One cut item, written by the CTA that holds its first segment.
+struct Cut {
+  int nparts;   // 0: none
+  int row0;     // first query row (token) of the item in q / out
+  int rows;     // token * G + head rows of the item
+  int kh;
+};
+
+struct AttnParams {
+  const unsigned char* q;
+  unsigned char* out;
+  float* lse;
+  int64_t q_st, q_sh, o_st, o_sh;  // bytes
+  int64_t lse_sh, lse_st;          // elements
+  const unsigned char* k[2];
+  const unsigned char* v[2];
+  int64_t blk_sb[2], head_sb[2], tok_sb[2], nblk[2];  // bytes
+  int64_t split;
+  const int32_t* bt;       // null: cross attention (k[0], v[0] are rows, nblk[0] of them)
+  int64_t bt_stride;
+  const int32_t* bt_row;
+  const int32_t* k_start;
+  const int32_t *q_start, *q_len, *k_len;
+  int bt_width;
+  int n, T, H, KVH, G, D, BS;
+  int host[2];             // tier is mapped host memory
+  float sl2;               // scale * log2(e)
+  int tq;                  // tokens per query tile
+  int ctas;
+  Cut* cuts;               // [ctas]
+  float* part_ml;          // [ctas][2][rows per item][2]: m (log2 domain), l
+  float* part_o;           // [ctas][2][rows per item][D]
+  int32_t* err;
+};
+
+// sum of floor((a i + b) / m) over 0 <= i < n, by the Euclidean recursion on
+// (a, m); a n + b < 2^32.
+__device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  long long ans = 0;
+  while (n > 0) {
+    if (a >= m) {
+      ans += (long long)n * (n - 1) / 2 * (a / m);
+      a %= m;
+    }
+    if (b >= m) {
+      ans += (long long)n * (b / m);
+      b %= m;
+    }
+    const uint32_t y = a * n + b;
+    if (y < m) break;
+    n = y / m;
+    b = y % m;
+    const uint32_t t = m;
+    m = a;
+    a = t;
+  }
+  return ans;
+}
+
+// A request's lengths, or qlen = 0 when it has no work (or does not fit its
+// rows: FD_DEVERR_LEN).
+struct Req {
+  int qlen, klen, qst, kbase;  // kbase: table row, or first state row
+};
+
+__device__ __forceinline__ Req load_req(const AttnParams& p, int r) {
+  Req q;
+  q.qlen = p.q_len[r];
+  q.klen = p.k_len[r];
+  q.qst = p.q_start[r];
+  q.kbase = p.bt != nullptr ? (p.bt_row != nullptr ? p.bt_row[r] : r) : p.k_start[r];
+  bool ok = q.qlen >= 0 && q.qlen <= kMaxLen && q.klen >= 0 && q.klen <= kMaxLen;
+  if (q.qlen > 0) {
+    ok = ok && q.qst >= 0 && (long long)q.qst + q.qlen <= p.T;
+    if (p.bt != nullptr)
+      ok = ok && ((long long)q.klen + p.BS - 1) / p.BS <= p.bt_width;
+    else
+      ok = ok && (q.klen == 0 || (q.kbase >= 0 && (long long)q.kbase + q.klen <= p.nblk[0]));
+  }
+  if (!ok) {
+    set_error(p.err, FD_DEVERR_LEN);
+    q.qlen = 0;
+  }
+  return q;
+}
+
+// kKT keys per tile, items of two query tiles with kPairs, fixed cost kW.
+template <int kKT, bool kPairs, int kW>
+struct Sched {
+  struct Seg {
+    int kh, tile0;   // kv head, first query tile of the item
+    bool pair;
+    int n, j0, j1;   // key tiles of the item, and of this segment
+    bool whole;
+    int nparts;      // slot 1 segments: parts of the cut item
+  };
+
+  const AttnParams& p;
+  long long p0, p1, per;  // this CTA's range, and every CTA's length
+  long long s;            // position of the current item
+  int r, kh, item;
+  Req rq;
+
+  __device__ __forceinline__ Sched(const AttnParams& params) : p(params) {}
+
+  __device__ __forceinline__ static int tiles(const AttnParams& p, const Req& q) { return (q.qlen + p.tq - 1) / p.tq; }
+  __device__ __forceinline__ static int items(const AttnParams& p, const Req& q) {
+    const int t = tiles(p, q);
+    return kPairs ? (t + 1) >> 1 : t;
+  }
+  __device__ __forceinline__ static bool is_pair(const AttnParams& p, const Req& q, int i) {
+    return kPairs && 2 * i + 1 < tiles(p, q);
+  }
+  // key tiles that the queries before token `te` of the request see
+  __device__ __forceinline__ static int ntiles(const AttnParams& p, const Req& q, int te) {
+    const int vis = p.bt != nullptr ? q.klen - q.qlen + te : q.klen;
+    return vis > 0 ? (vis + kKT - 1) / kKT : 0;
+  }
+  __device__ __forceinline__ static int item_end(const AttnParams& p, const Req& q, int i) {
+    return (int)min((long long)(i + 1) * (kPairs ? 2 : 1) * p.tq, (long long)q.qlen);
+  }
+  // positions of items 0 .. i - 1 of a request and kv head
+  __device__ static long long before(const AttnParams& p, const Req& q, int i) {
+    const int ni = items(p, q);
+    long long ans = (long long)i * kW;
+    // the last item may end early, or be a single tile
+    const int reg = min(i, ni - 1);
+    constexpr int u = kPairs ? 2 : 1;
+    if (reg > 0) {
+      if (p.bt == nullptr) {
+        ans += (long long)u * reg * ntiles(p, q, 0);
+      } else {
+        const int st = u * p.tq, b = q.klen - q.qlen;
+        const int m0 = b + st > 0 ? 0 : min(reg, -b / st);  // items whose queries see nothing
+        if (reg > m0)
+          ans += u * floor_sum((uint32_t)(reg - m0), kKT, (uint32_t)st,
+                               (uint32_t)((long long)b + (long long)(m0 + 1) * st + kKT - 1));
+      }
+    }
+    if (i == ni) ans += (is_pair(p, q, ni - 1) ? 2 : 1) * (long long)ntiles(p, q, q.qlen);
+    return ans;
+  }
+  __device__ __forceinline__ static long long cost(const AttnParams& p, const Req& q) {
+    return q.qlen > 0 ? before(p, q, items(p, q)) : 0;
+  }
+
+  struct Scratch {
+    long long warp_sum[32];
+    long long total, start;  // sum over all requests; position of the request found
+    int found, item;
+    long long item_start;
+  };
+
+  // All threads of the block (NT of them) together: the range of CTA `c` and
+  // the item it starts in.  False: no work.
+  template <int NT>
+  __device__ bool init(Scratch* sc, int c, int min_per) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    constexpr int kWarps = NT / 32;
+    long long total = 0, mine = 0, mine_at = 0;
+    // pass 0 adds up all requests, pass 1 finds this CTA's (from the values
+    // that pass 0 left when one round holds all requests)
+    const bool one = p.n <= NT;
+    if (tid == 0) sc->found = -1;
+    for (int pass = 0; pass < 2; ++pass) {
+      long long carry = 0;
+      for (int base = 0; base < p.n; base += NT) {
+        if (pass == 0 || !one) {
+          const int i = base + tid;
+          mine = i < p.n ? cost(p, load_req(p, i)) * p.KVH : 0;
+          long long x = mine;
+#pragma unroll
+          for (int off = 1; off < 32; off <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, x, off);
+            if (lane >= off) x += y;
+          }
+          if (lane == 31) sc->warp_sum[warp] = x;
+          __syncthreads();
+          long long ahead = 0, all = 0;
+          for (int w = 0; w < kWarps; ++w) {
+            if (w == warp) ahead = all;
+            all += sc->warp_sum[w];
+          }
+          mine_at = carry + ahead + x - mine;
+          carry += all;
+          __syncthreads();
+        }
+        if (pass == 1 && mine > 0 && mine_at <= p0 && p0 < mine_at + mine) {
+          sc->found = base + tid;
+          sc->start = mine_at;
+        }
+      }
+      if (pass == 0) {
+        total = carry;
+        per = (total + p.ctas - 1) / p.ctas;
+        if (per < min_per) per = min_per;
+        p0 = (long long)c * per;
+        p1 = min(p0 + per, total);
+        if (p0 >= total) return false;
+      }
+    }
+    __syncthreads();
+    r = sc->found;
+    rq = load_req(p, r);
+    const long long per_head = cost(p, rq);
+    const long long off = p0 - sc->start;
+    kh = (int)(off / per_head);
+    const long long x = off - (long long)kh * per_head;
+    if (warp == 0) {  // the last item that starts at or before x, 32 candidates at a time
+      int lo = 0, hi = items(p, rq);
+      while (hi - lo > 1) {
+        const int gap = (hi - lo + 31) / 32;
+        const int i = lo + lane * gap;
+        const unsigned at = __ballot_sync(0xffffffffu, i < hi && before(p, rq, i) <= x);
+        lo += (31 - __clz(at)) * gap;  // lane 0 always: before(lo) <= x
+        hi = min(hi, lo + gap);
+      }
+      if (lane == 0) {
+        sc->item = lo;
+        sc->item_start = sc->start + (long long)kh * per_head + before(p, rq, lo);
+      }
+    }
+    __syncthreads();
+    item = sc->item;
+    s = sc->item_start;
+    return true;
+  }
+
+  // The next segment of this CTA's range.
+  __device__ __forceinline__ bool next(Seg& g) {
+    while (s < p1) {
+      const bool pr = is_pair(p, rq, item);
+      const int u = pr ? 2 : 1;
+      const int n = ntiles(p, rq, item_end(p, rq, item));
+      const long long a = p0 - s - kW, b = p1 - s - kW;
+      // tile j belongs to the range that holds position s + kW + u j
+      g.j0 = (int)max(0ll, min((long long)n, (a + u - 1) >> (u - 1)));
+      g.j1 = (int)max(0ll, min((long long)n, (b + u - 1) >> (u - 1)));
+      g.n = n;
+      g.kh = kh;
+      g.tile0 = (kPairs ? 2 : 1) * item;
+      g.pair = pr;
+      g.whole = g.j0 == 0 && g.j1 == n;
+      g.nparts = 0;
+      if (!g.whole && g.j0 == 0 && g.j1 > 0) {
+        const long long last = s + kW + (long long)u * (n - 1);
+        g.nparts = (int)(last / per - p0 / per) + 1;
+      }
+      const bool has = g.j0 < g.j1 || (n == 0 && s >= p0);
+      seg_q = rq;
+      s += kW + (long long)u * n;
+      if (++item == items(p, rq)) {
+        item = 0;
+        if (++kh == p.KVH) {
+          kh = 0;
+          while (s < p1) {  // the next request with work
+            rq = load_req(p, ++r);
+            if (rq.qlen > 0) break;
+          }
+        }
+      }
+      if (has) return true;
+    }
+    return false;
+  }
+  Req seg_q;  // the request of the segment returned last
+};
+
+// The kernels' entry points for the host code in fd_attn.cu.
+bool mma_covers(const fd_attn_args* a);
+size_t mma_workspace(const fd_attn_args* a);
+int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s);
+// Joins the cut items: `rows` rows per item at most.
+int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s);
+
+}  // namespace at
+}  // namespace fdk

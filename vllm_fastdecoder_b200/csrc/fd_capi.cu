@@ -70,6 +70,11 @@ extern "C" const char* fd_device_error_string(int32_t code) {
     case FD_DEVERR_PLAN:
       return "step planner: query offsets not 0-based, decreasing or past the token capacity, or a request "
              "extending prior context by more than one token while part of its KV is in the host tier";
+    case FD_DEVERR_TABLES:
+      return "block tables: the step does not fit the free blocks, the table's width or the token capacity, or a "
+             "length or count is invalid";
+    case FD_DEVERR_POSITION:
+      return "rotary position outside the cos / sin table";
     default:
       return "unknown device error";
   }
@@ -121,7 +126,7 @@ extern "C" int fd_host_unregister(void* host) {
   return fdh::cuda_status(cudaHostUnregister(host), "cudaHostUnregister");
 }
 
-extern "C" int fd_version(void) { return 101; }
+extern "C" int fd_version(void) { return 102; }
 
 extern "C" int fd_abi_sizes(size_t* decode_args_bytes, size_t* kv_tier_bytes) {
   if (decode_args_bytes != nullptr) *decode_args_bytes = sizeof(fd_decode_args);

@@ -17,7 +17,11 @@ fastdecode/csrc/cpu_attn.cpp:
   merge_attn_states(out, o_a, lse_a, o_b, lse_b)
                                       vLLM's op as called at backend.py:54-55
 plus the two-tier entry points the backend uses (decode_tiered, store_kv_tiered,
-merge_partials).  Every call is asynchronous on the current CUDA stream.
+merge_partials), and the operators of a step whose requests bring several new
+tokens: extend_tables (block tables, slots and positions from lengths),
+rope_store_kv (multi-axis rotary positions with the KV write), chunk_attn (the
+new tokens' attention over the cached context of either tier) and cross_attn
+(attention to an encoder's states).  Every call is asynchronous on the current CUDA stream.
 There is no CPU path: without the native library or a CUDA device these raise.
 """
 
@@ -26,7 +30,9 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+import struct
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -628,7 +634,7 @@ def store_kv(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, k_cache: tor
             raise RuntimeError(f"CPU slot out of range ({e})") from None
 
 
-# ------------------------------------------------------------- merge
+# ------------------------------------------------------------- prefill
 
 
 def prefill_attn(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -692,6 +698,300 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_le
     a.total_q = int(q_len.sum().item()) if total_q is None else int(total_q)
     a.error = error_word(dev).data_ptr()
     nat.check(lib.fd_prefill_attn(ctypes.byref(a), _stream(dev)), "fd_prefill_attn")
+
+
+# ------------------------------------------------------------- multi-token steps
+#
+# These calls pack their C struct in one struct.pack (a ctypes field store each
+# would cost more than the launch), run on the device of their tensors whatever
+# the current one is, and take their workspace from torch's caching allocator
+# per call: it belongs to the current stream, and to the graph when one is
+# being captured, so calls on other streams and other graphs never share it.
+
+_TIER_FMT = "PPqqqqii"
+_ATTN_STRUCT = struct.Struct("@PqqPqqPqq" + 2 * _TIER_FMT + "qPqPPPPPiiiiiiifiiiiPNP")
+_ROPE_STRUCT = struct.Struct("@" + 5 * "Pqq" + "PqPqP" + 2 * _TIER_FMT + f"q9i{nat.ROPE_MAX_PAIRS}siP")
+_TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPP")
+_NO_TIER = (0, 0, 0, 0, 0, 0, 0, 0)
+
+
+def _launch(fn, packed: bytes, device: torch.device, what: str) -> None:
+    """Call a C entry point on the current stream of `device`."""
+    idx = device.index
+    if idx != torch.cuda.current_device():
+        with torch.cuda.device(idx):
+            status = fn(packed, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        status = fn(packed, torch._C._cuda_getCurrentRawStream(idx))
+    if status:
+        nat.check(status, what)
+
+
+def _tier_fields(t: KVTier | None, dev: torch.device, dtype: torch.dtype) -> tuple:
+    if t is None:
+        return _NO_TIER
+    k, v = t.k, t.v
+    _check(k.dtype == dtype and v.dtype == dtype, "the KV tier's dtype differs")
+    s = k.stride()
+    if k.device.type == "cpu":
+        return (host_device_pointer(k), host_device_pointer(v), s[0], s[1], s[2], k.shape[0], 1, 0)
+    _check(k.device == dev and v.device == dev, "a device tier must live on the tensors' device")
+    return (k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], k.shape[0], 0, 0)
+
+
+def _need_i32(t: torch.Tensor, dev: torch.device, n: int, name: str) -> int:
+    _check(t.dtype == torch.int32 and t.device == dev and t.dim() == 1 and t.shape[0] >= n and (n < 2 or t.stride(0) == 1),
+           f"{name} must be a contiguous int32 tensor of at least {n} entries on the call's device")
+    return t.data_ptr()
+
+
+@dataclass
+class FreeBlocks:
+    """The free blocks of both tiers as stacks in device memory: hbm / host
+    int32 [capacity] (host ids start at num_gpu_blocks; None: no such tier),
+    counts int32 [2], the next block to take at counts - 1."""
+
+    hbm: torch.Tensor | None
+    host: torch.Tensor | None
+    counts: torch.Tensor
+
+
+class StepTables:
+    """Device buffers that extend_tables fills for a step of up to R requests
+    and T new tokens.  seq_lens and counts may be the caller's own tensors:
+    the prior lengths and the free stacks' counts, to step them in place."""
+
+    def __init__(self, R: int, T: int, device, seq_lens: torch.Tensor | None = None,
+                 counts: torch.Tensor | None = None):
+        z = lambda n, dt: torch.zeros(n, dtype=dt, device=device)  # noqa: E731
+        self.R, self.T = int(R), int(T)
+        self.seq_lens = z(R, torch.int32) if seq_lens is None else seq_lens
+        self.counts = z(2, torch.int32) if counts is None else counts
+        self.query_start_loc = z(R + 1, torch.int32)
+        self.slot_mapping, self.positions = z(T, torch.int64), z(T, torch.int64)
+        self.header = z(nat.TABLES_HEADER_LEN, torch.int32)
+
+    def read_header(self) -> dict[str, int]:
+        """The header by name (synchronises); raises if the step was refused."""
+        h = self.header.tolist()
+        flags = h[nat.TABLES_FIELDS["flags"]]
+        if flags:
+            why = ", ".join(text for bit, text in nat.TABLES_FLAGS.items() if flags & bit)
+            raise RuntimeError(f"extend_tables refused the step: {why}")
+        return {k: h[i] for k, i in nat.TABLES_FIELDS.items()}
+
+
+def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table: torch.Tensor, free: FreeBlocks,
+                  num_gpu_blocks: int, num_cpu_blocks: int, block_size: int,
+                  out: StepTables | None = None, max_tokens: int | None = None) -> StepTables:
+    """Block tables, slots and positions of a step from the requests' lengths
+    (fd_extend_tables), on the GPU without any host synchronisation.
+
+    new_lens int32 [R]: new tokens of each request (0: none, -1: the request
+    ends and gives its blocks back); prior_lens int32 [R]: its tokens in the
+    cache; block_table int32 [R, W], changed in place; free: the stacks, HBM
+    blocks are taken first.  Fills and returns `out` (or a new StepTables for
+    max_tokens new tokens): seq_lens, query_start_loc, slot_mapping (-1 behind
+    the last token), positions, counts and the header; its seq_lens,
+    query_start_loc and slot_mapping are what plan.plan_on_device takes.  A
+    step that cannot be applied as a whole changes nothing and sets
+    the error word (check_device_errors; StepTables.read_header says why)."""
+    dev = block_table.device
+    _check(dev.type == "cuda", "block_table must be a CUDA tensor")
+    _check(block_table.dtype == torch.int32 and block_table.dim() == 2 and (block_table.shape[1] == 1
+                                                                            or block_table.stride(1) == 1),
+           "block_table must be int32 [R, W] with contiguous rows")
+    R, W = block_table.shape
+    if out is None:
+        _check(max_tokens is not None, "give out or max_tokens")
+        out = StepTables(R, max_tokens, dev)
+    T = out.T if max_tokens is None else int(max_tokens)
+    _check(out.R >= R and out.T >= T, "out is too small for the step")
+    _check(out.query_start_loc.device == dev, "out must be on block_table's device")
+    stacks = [(0, 0) if t is None else (_need_i32(t, dev, 0, "a free stack"), t.shape[0]) for t in (free.hbm, free.host)]
+    for t in (free.hbm, free.host):
+        _check(t is None or t.shape[0] < 2 or t.stride(0) == 1, "a free stack must be contiguous")
+    packed = _TABLES_STRUCT.pack(
+        _need_i32(new_lens, dev, R, "new_lens"), _need_i32(prior_lens, dev, R, "prior_lens"), block_table.data_ptr(),
+        max(W, block_table.stride(0)), W, R, stacks[0][0], stacks[1][0], stacks[0][1], stacks[1][1],
+        _need_i32(free.counts, dev, 2, "free.counts"), _need_i32(out.counts, dev, 2, "out.counts"),
+        int(num_gpu_blocks), int(num_cpu_blocks), int(block_size), T, _need_i32(out.seq_lens, dev, R, "out.seq_lens"),
+        out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.header.data_ptr(),
+        error_word(dev).data_ptr())
+    _launch(nat.load().fd_extend_tables, packed, dev, "fd_extend_tables")
+    return out
+
+
+@lru_cache(maxsize=64)
+def rope_axes(sections: tuple[int, ...], turns: bool = False) -> bytes:
+    """The axis of each rotated pair.  sections[a] pairs belong to axis a: in
+    blocks (axis 0's pairs first), or, with turns, dealt out one after the
+    other, an axis that has all its pairs being passed over."""
+    _check(1 <= len(sections) <= nat.ROPE_MAX_AXES and all(n >= 0 for n in sections) and sum(sections) > 0,
+           f"sections: the pairs of 1 to {nat.ROPE_MAX_AXES} axes")
+    _check(sum(sections) <= nat.ROPE_MAX_PAIRS, f"at most {nat.ROPE_MAX_PAIRS} rotated pairs")
+    if not turns:
+        return bytes(a for a, n in enumerate(sections) for _ in range(n))
+    order: list[int] = []
+    for i in range(max(sections)):
+        order += [a for a, n in enumerate(sections) if i < n]
+    return bytes(order)
+
+
+def rope_store_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos_sin: torch.Tensor,
+                  slots: torch.Tensor | None, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, *,
+                  sections: tuple[int, ...] | None = None, turns: bool = False, pairs: bool = False,
+                  q_out: torch.Tensor | None = None, k_out: torch.Tensor | None = None) -> torch.Tensor:
+    """Rotate q and k by multi-axis positions and write the rotated k, and v,
+    to their cache slots in either tier, in one pass (fd_rope_store_kv).
+
+    q [T, H, D], k and v [T, KVH, D], one of fp16 / bf16 / fp32; positions
+    int64 [A, T] (or [T]): the token's place on each axis; cos_sin fp32
+    [max_pos, rot_dim]: cosines of the rot_dim / 2 pairs, then sines; slots
+    int64 [T] (-1: not written; the others differ) or None (no KV write).
+    sections / turns: which pair takes which axis (rope_axes; default one
+    axis).  A pair is dims (i, i + rot_dim / 2), or neighbours (2i, 2i + 1)
+    with pairs.  The rotated q goes to q_out (default: q itself), which is
+    returned; k_out takes a copy of the rotated k, e.g. for prefill_attn over
+    a fresh prompt's own rows."""
+    dev, dt = q.device, q.dtype
+    _check(dev.type == "cuda", "q must be a CUDA tensor")
+    _check(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and k.shape[0] == q.shape[0]
+           and k.shape[2] == q.shape[2], "q must be [T, H, D], k and v [T, KVH, D]")
+    T, H, D = q.shape
+    KVH = k.shape[1]
+    q_out = q if q_out is None else q_out
+    _check(q_out.shape == q.shape and (k_out is None or k_out.shape == k.shape), "q_out / k_out must have q's / k's shape")
+    for t in (q, k, v, q_out) if k_out is None else (q, k, v, q_out, k_out):
+        _check(t.dtype == dt and t.device == dev and t.stride(2) == 1,
+               "q, k, v and the outputs must share dtype and device and have a contiguous head dim")
+    if positions.dim() == 1:
+        positions = positions.unsqueeze(0)
+    A = positions.shape[0]
+    _check(positions.dtype == torch.int64 and positions.device == dev and positions.dim() == 2
+           and positions.shape[1] >= T and (T < 2 or positions.stride(1) == 1),
+           "positions must be int64 [axes, T] on q's device with contiguous rows")
+    _check(cos_sin.dtype == torch.float32 and cos_sin.device == dev and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
+           "cos_sin must be contiguous fp32 [max_pos, rot_dim] on q's device")
+    rot = cos_sin.shape[1]
+    axes = rope_axes((rot // 2,) if sections is None else tuple(sections), bool(turns))
+    _check(2 * len(axes) == rot, "sections must add up to rot_dim / 2 pairs")
+    _check(A == (1 if sections is None else len(sections)), "positions must have one row per axis")
+    BS = 0
+    f0 = f1 = _NO_TIER
+    if slots is not None:
+        _check(slots.dtype == torch.int64 and slots.device == dev and slots.dim() == 1 and slots.shape[0] >= T
+               and (T < 2 or slots.stride(0) == 1), "slots must be contiguous int64 with T entries on q's device")
+        for t in tiers:
+            if t is not None:
+                _check(t.k.shape[1] == KVH and t.k.shape[3] == D and BS in (0, t.k.shape[2]),
+                       "the KV tiers must be [blocks, KVH, block_size, D]")
+                BS = t.k.shape[2]
+        _check(BS > 0, "at least one KV tier is required")
+        f0, f1 = _tier_fields(tiers[0], dev, dt), _tier_fields(tiers[1], dev, dt)
+    st = [x for t in (q, q_out, k, v) for x in (t.data_ptr(), t.stride(0), t.stride(1))]
+    st += (0, 0, 0) if k_out is None else (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+    packed = _ROPE_STRUCT.pack(
+        *st, positions.data_ptr(), positions.stride(0), cos_sin.data_ptr(), cos_sin.shape[0],
+        0 if slots is None else slots.data_ptr(), *f0, *f1, int(tier_split), T, H, KVH, D, rot, BS, dtype_code(dt), A,
+        nat.ROPE_PAIRS if pairs else 0, axes, 0, error_word(dev).data_ptr())
+    _launch(nat.load().fd_rope_store_kv, packed, dev, "fd_rope_store_kv")
+    return q_out
+
+
+@lru_cache(maxsize=256)
+def _attn_workspace_bytes(H: int, KVH: int, D: int, dtype: torch.dtype) -> int:
+    a = nat.FdAttnArgs()
+    a.num_heads, a.num_kv_heads, a.head_size, a.dtype = H, KVH, D, dtype_code(dtype)
+    return nat.load().fd_attn_workspace_size(ctypes.byref(a))
+
+
+def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, tiers, tier_split, table, bt_row, k_start, BS,
+          max_q_len, max_k_len, workspace_buf) -> None:
+    dev, dt = q.device, q.dtype
+    _check(dev.type == "cuda", "q must be a CUDA tensor")
+    _check(q.dim() == 3 and out.shape == q.shape and out.dtype == dt and out.device == dev,
+           "q and out must be [T, H, D] alike")
+    _check(q.stride(2) == 1 and out.stride(2) == 1, "q and out need a contiguous head dim")
+    T, H, D = q.shape
+    n = q_len.shape[0]
+    ptrs = (_need_i32(q_start, dev, n, "q_start"), _need_i32(q_len, dev, n, "q_len"), _need_i32(k_len, dev, n, "k_len"))
+    if lse is None:
+        lse_f = (0, 0, 0)
+    else:
+        _check(lse.dtype == torch.float32 and lse.device == dev and lse.shape == (H, T), "lse must be fp32 [H, T] on q's device")
+        lse_f = (lse.data_ptr(), lse.stride(0), lse.stride(1))
+    need = _attn_workspace_bytes(H, KVH, D, dt)
+    if workspace_buf is None:
+        workspace_buf = torch.empty(need, dtype=torch.uint8, device=dev)
+    else:
+        _check(workspace_buf.device == dev and workspace_buf.dtype == torch.uint8 and workspace_buf.is_contiguous()
+               and workspace_buf.numel() >= need, f"workspace_buf must be uint8 on q's device with >= {need} bytes")
+    bt = (0, 0) if table is None else (table.data_ptr(), table.stride(0))
+    packed = _ATTN_STRUCT.pack(
+        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), *lse_f,
+        *tiers[0], *tiers[1], tier_split, *bt, 0 if bt_row is None else _need_i32(bt_row, dev, n, "bt_row"),
+        0 if k_start is None else _need_i32(k_start, dev, n, "k_start"), *ptrs, 0 if table is None else table.shape[1], T,
+        n, H, KVH, D, BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, workspace_buf.data_ptr(), workspace_buf.numel(),
+        error_word(dev).data_ptr())
+    _launch(fn, packed, dev, what)
+
+
+def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
+               q_start: torch.Tensor, q_len: torch.Tensor, k_len: torch.Tensor, scale: float, out: torch.Tensor,
+               lse: torch.Tensor | None = None, *, bt_row: torch.Tensor | None = None, max_q_len: int = 0,
+               max_k_len: int = 0, workspace_buf: torch.Tensor | None = None) -> None:
+    """Attention of each request's new tokens over its paged cache in both
+    tiers (fd_chunk_attn): chunks of prompts, draft tokens to verify, single
+    tokens.  Unlike prefill_attn it reads the host tier too, takes any head
+    size, block size and dtype, splits long contexts over the GPU when there
+    are few queries, and returns the log-sum-exp.
+
+    q, out [T, H, D]; per request (int32 [n] on the device) q_start, q_len,
+    k_len: its queries are rows q_start .. of q and its K/V, the new tokens'
+    included, k_len tokens in the blocks of row bt_row[r] (default r) of
+    block_table [R, W] int32; query i sees keys 0 .. k_len - q_len + i.  lse
+    fp32 [H, T] or None.  Rows of no request stay as they were; a query that
+    sees nothing gets 0 and -inf.  max_q_len / max_k_len: the lengths' bounds,
+    if the host knows them.  workspace_buf (uint8) replaces the call's own
+    scratch memory."""
+    t0, t1 = tiers
+    ref = t0 if t0 is not None else t1
+    _check(ref is not None, "at least one KV tier is required")
+    dev = q.device
+    _, KVH, BS, D = ref.k.shape
+    _check(q.dim() == 3 and q.shape[2] == D, "head size mismatch")
+    _check(t0 is None or t1 is None or t0.k.shape[1:] == t1.k.shape[1:], "tiers must share [KVH, BS, D]")
+    _check(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2
+           and (block_table.shape[1] < 2 or block_table.stride(1) == 1),
+           "block_table must be int32 [R, W] on q's device with contiguous rows")
+    _check(bt_row is not None or block_table.shape[0] >= q_len.shape[0], "block_table must have a row per request")
+    _attn(nat.load().fd_chunk_attn, "fd_chunk_attn", q, out, lse, q_start, q_len, k_len, scale, KVH,
+          (_tier_fields(t0, dev, q.dtype), _tier_fields(t1, dev, q.dtype)), int(tier_split), block_table, bt_row, None, BS,
+          max_q_len, max_k_len, workspace_buf)
+
+
+def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
+               k_start: torch.Tensor, k_len: torch.Tensor, scale: float, out: torch.Tensor,
+               lse: torch.Tensor | None = None, *, max_q_len: int = 0, max_k_len: int = 0,
+               workspace_buf: torch.Tensor | None = None) -> None:
+    """Cross attention to an encoder's states (fd_cross_attn): request r's
+    queries (rows q_start .. q_start + q_len - 1 of q [T, H, D]) each see all
+    of rows k_start .. k_start + k_len - 1 of k and v [S, KVH, D]; requests may
+    share states.  q_len = 1 is a decode step.  The other arguments are
+    chunk_attn's."""
+    dev = q.device
+    _check(k.dim() == 3 and k.shape == v.shape and k.stride() == v.stride() and (k.stride(2) == 1),
+           "k and v must be [S, KVH, D] alike with a contiguous head dim")
+    _check(k.dtype == q.dtype and v.dtype == q.dtype and k.device == dev and v.device == dev and q.dim() == 3
+           and k.shape[2] == q.shape[2], "k / v dtype, device or head size differs from q's")
+    S, KVH, _ = k.shape
+    states = (k.data_ptr(), v.data_ptr(), 0, k.stride(1), k.stride(0), S, 0, 0)
+    _attn(nat.load().fd_cross_attn, "fd_cross_attn", q, out, lse, q_start, q_len, k_len, scale, KVH, (states, _NO_TIER), 0,
+          None, None, k_start, 0, max_q_len, max_k_len, workspace_buf)
+
+
+# ------------------------------------------------------------- merge
 
 
 def merge_attn_states(out: torch.Tensor, o_a: torch.Tensor, lse_a: torch.Tensor, o_b: torch.Tensor,
