@@ -1,6 +1,811 @@
+// Chunk and cross attention on the 5th-generation tensor cores (tcgen05): fp16
+// and bf16, head sizes 64 to 128 (padded to 64 or 128 dims in shared memory).
+//
+//   S [128 rows x 128 keys] = Q . K^T,  P = 2^(scale log2(e) S - m),
+//   l = sum P,  O [128 rows x D] += P . V,  o = O / l, lse = ln 2 (m + log2 l)
+//
+// A CTA walks its range of the schedule (fd_attn.cuh) segment by segment and
+// runs two STREAMS of such products at a time, so that one stream's softmax
+// overlaps the other's matrix products.  In a pair (256 rows and more) the
+// streams are two neighbouring query tiles and share every K/V tile; in a
+// single tile (few query rows: bound by the bytes of the cache) stream A
+// takes the even key tiles and stream B the odd ones of the same query tile,
+// and the two are joined in registers at the end.  Eleven warps:
+//   8   schedule, Q tiles and K tiles   } TMA boxes of 16 keys with the
+//   10  V tiles                         } 128-byte swizzle the MMA reads, or
+//       16-byte loads stored in the same layout where a box is in the host
+//       tier, spans blocks (block sizes that are no multiple of 16), or is
+//       cut by the end of a request's V (rows behind it must be 0: P is 0
+//       there, and 0 x NaN is not)
+//   9   one thread issues the MMAs: q.K^T of step k + 1 of a stream right
+//       after its P.V of step k
+//   0-3, 4-7  softmax of stream A, B: one thread per row with all 128 keys of
+//       a tile.  P overwrites the first half of its S in TMEM as 16-bit
+//       values (the A operand of P.V); O stays in TMEM over a segment and is
+//       rescaled only when a row's maximum passes its reference m by more
+//       than 2^8, so P stays below 2^8; row sums add the fp32 values of P.
+// TMEM: S/P of A [0, 128), of B [128, 256), O of A [256, 384), of B [384, 512).
+// Scores, sums and O are fp32; P is rounded to the input type (the tensor
+// core's operand type), the result once.  Every wait is bounded, and a role
+// that gives up raises the CTA's abort flag for the others.
+
+#include <math.h>
+
+#include <type_traits>
+
 #include "fd_attn.cuh"
-namespace fdk { namespace at {
-bool mma_covers(const fd_attn_args* a) { return false; }
-size_t mma_workspace(const fd_attn_args* a) { return 0; }
-int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) { return 0; }
-}}
+#include "fd_decode.cuh"
+#include "fd_tcgen05.cuh"
+
+namespace fdk {
+namespace at {
+namespace mm {
+
+constexpr int kM = 128;             // rows per query tile (MMA M)
+constexpr int kKT = 128;            // keys per tile (MMA N of S, K of P.V)
+constexpr int kSub = 16;            // keys per TMA box
+constexpr int kSubs = kKT / kSub;
+constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims
+constexpr int kWarpK = 8, kWarpMma = 9, kWarpV = 10;
+constexpr int kThreads = 11 * 32;
+constexpr int kSegs = 4;            // segments in flight between the roles
+constexpr int kSegReaders = 10;     // MMA thread, V producer, eight softmax warps
+constexpr int kItemRows = 2 * kM;
+constexpr int kMaxCtas = 160;
+constexpr int kFixed = 3;           // an item's fixed cost in key tiles of a single
+constexpr int kMinPer = 5;          // least positions of a CTA: two key tiles behind the fixed cost
+typedef Sched<kKT, true, kFixed> Walk;
+
+template <int KD>
+struct Geo {
+  static constexpr int kPanels = KD / 64;
+  static constexpr int kTile = kPanels * kPanel;
+  static constexpr int kRingK = KD == 128 ? 3 : 5;
+  static constexpr int kRingV = KD == 128 ? 2 : 5;
+  static constexpr int kOffK = 2 * kTile;
+  static constexpr int kOffV = kOffK + kRingK * kTile;
+  static constexpr int kOffBar = kOffV + kRingV * kTile;
+  // q full/empty, k full/empty, v full/empty, s_full[2], p_full[2], o_full[2],
+  // o_both, o_empty, ml_full, seg full/empty, drain
+  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 2 + 2 + 2 + 3 + 2 * kSegs + 1;
+  static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kOffMl = kOffSeg + kSegs * 64;   // [2 streams][128 rows] float2 (before that: Walk::Scratch)
+  static constexpr int kOffMisc = kOffMl + 2 * kM * 8;  // abort flag, TMEM address
+  static constexpr int kSmem = kOffMisc + 16;
+  static_assert(kSmem <= 227 * 1024, "smem budget");
+};
+
+// One segment as the roles see it.
+struct SegInfo {
+  int live;      // 0: no more segments
+  int pair;
+  int j0, m;     // first key tile, key tiles
+  int n0, n1;    // steps of stream A, B
+  int tok0;      // first query token of the item within the request
+  int qst, qlen, klen, kbase, kh;
+  int slot;      // -1: whole, else its slot of the partials
+  int nparts;    // > 0: this is a cut item's first segment
+  int pad[2];
+};
+static_assert(sizeof(SegInfo) == 64, "segment record");
+
+struct MmaParams {
+  CUtensorMap tmap_q;       // {D, H, T, 1}, box {64, G, tq, 1}
+  CUtensorMap tmap_k[2];    // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}), box {64, 1, 16, 1}
+  CUtensorMap tmap_v[2];
+  AttnParams a;
+  int q_tma, kv_tma[2];     // the view has a tensor map
+};
+
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_try_wait(bar, parity)) return true;
+    if ((it & 63u) == 0) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        set_error(err, FD_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// The same without suspending, for the MMA issuer.
+__device__ __forceinline__ bool poll_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
+  if (mbar_test_wait(bar, parity)) return true;
+  const uint64_t t0 = globaltimer_ns();
+  for (uint32_t it = 1;; ++it) {
+    if (mbar_test_wait(bar, parity)) return true;
+    if ((it & 255u) == 0) {
+      if (*abort_flag) return false;
+      if (globaltimer_ns() - t0 > kWaitLimitNs) {
+        set_error(err, FD_DEVERR_TIMEOUT);
+        return false;
+      }
+    }
+  }
+}
+
+// 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ float fmax3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 v = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// Block id of box `lane` (keys 128 j + 16 lane ..) where boxes lie within
+// blocks, -1 where there is none.  Read one tile ahead of its use.
+__device__ __forceinline__ int box_block(const AttnParams& p, int kbase, int klen, int j, int lane) {
+  const int t = j * kKT + lane * kSub;
+  if (p.bt == nullptr || p.BS % kSub != 0 || lane >= kSubs || t >= klen) return -1;
+  return p.bt[(int64_t)kbase * p.bt_stride + t / p.BS];
+}
+
+// One warp: K or V of key tile j into `dst`, completion on `bar` (bytes of
+// the TMA boxes, and lane 0's arrival once the other boxes are stored).
+template <int KD>
+__device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsigned char* dst, uint64_t* bar, int j,
+                                          int kbase, int klen, int kh, int id, int lane, uint64_t pol) {
+  const AttnParams& p = mp.a;
+  const int t = j * kKT + lane * kSub;
+  const bool boxed = p.bt == nullptr || p.BS % kSub == 0;
+  bool in = lane < kSubs && t < klen;  // the box holds a key
+  int tier = 0, blk = 0, r0 = 0;
+  bool tma = false;
+  if (in && boxed) {
+    if (p.bt == nullptr) {
+      r0 = kbase + t;
+    } else {
+      int64_t b = id;
+      if (b >= p.split) {
+        tier = 1;
+        b -= p.split;
+      }
+      r0 = t % p.BS;
+      if (b < 0 || b >= p.nblk[tier]) {
+        set_error(p.err, FD_DEVERR_BLOCK_ID);
+        in = false;
+      }
+      blk = (int)b;
+    }
+    tma = in && mp.kv_tma[tier] && (!is_v || t + kSub <= klen);
+  }
+  const unsigned tmask = __ballot_sync(0xffffffffu, tma);
+  const unsigned all = (1u << kSubs) - 1u;
+  // K boxes without a key need nothing (the mask replaces their scores)
+  unsigned rest = is_v ? all & ~tmask : __ballot_sync(0xffffffffu, in) & ~tmask;
+  if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(tmask) * (uint32_t)(Geo<KD>::kPanels * kSub * 128));
+  __syncwarp();
+  if (tma) {
+    const CUtensorMap* map = is_v ? &mp.tmap_v[tier] : &mp.tmap_k[tier];
+#pragma unroll
+    for (int x = 0; x < Geo<KD>::kPanels; ++x)
+      tma_load_4d(dst + x * kPanel + lane * kSub * 128, map, 64 * x, kh, r0, blk, bar, pol);
+  }
+  if (rest != 0u) {
+    constexpr int kCh = KD / 8;                   // 16-byte chunks per row
+    constexpr int kPer = kSub * kCh / 32;         // chunks of a box per lane
+    while (rest != 0u) {
+      const int s = __ffs(rest) - 1;
+      rest &= rest - 1u;
+      const bool box_in = __shfl_sync(0xffffffffu, (int)in, s) != 0;
+      const int box_tier = __shfl_sync(0xffffffffu, tier, s);
+      const int box_blk = __shfl_sync(0xffffffffu, blk, s);
+      const int box_r0 = __shfl_sync(0xffffffffu, r0, s);
+      uint4 v[kPer];
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) {
+        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
+        const int key = j * kKT + s * kSub + row;
+        v[c] = make_uint4(0u, 0u, 0u, 0u);
+        if (!box_in || key >= klen || ch * 8 >= p.D) continue;
+        int tr = box_tier, rr = box_r0 + row;
+        int64_t b = box_blk;
+        if (!boxed) {
+          b = p.bt[(int64_t)kbase * p.bt_stride + key / p.BS];
+          rr = key % p.BS;
+          tr = 0;
+          if (b >= p.split) {
+            tr = 1;
+            b -= p.split;
+          }
+          if (b < 0 || b >= p.nblk[tr]) {
+            set_error(p.err, FD_DEVERR_BLOCK_ID);
+            continue;
+          }
+        }
+        const unsigned char* base = is_v ? p.v[tr] : p.k[tr];
+        v[c] = *reinterpret_cast<const uint4*>(base + b * p.blk_sb[tr] + kh * p.head_sb[tr] +
+                                               (int64_t)rr * p.tok_sb[tr] + ch * 16);
+      }
+#pragma unroll
+      for (int c = 0; c < kPer; ++c) {
+        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
+        sts128(dst + (ch >> 3) * kPanel + swz(s * kSub + row, ch & 7), v[c]);
+      }
+    }
+    fence_proxy_async_smem();  // the stores before the tensor cores read the slot
+  }
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+}
+
+// One warp: the query rows of one tile into `dst` without TMA.
+template <int KD>
+__device__ __forceinline__ void load_q(const AttnParams& p, unsigned char* dst, int kh, int tok, int ntok, int lane) {
+  constexpr int kCh = KD / 8;
+  for (int idx = lane; idx < ntok * p.G * kCh; idx += 32) {
+    const int row = idx / kCh, ch = idx % kCh;
+    uint4 v = make_uint4(0u, 0u, 0u, 0u);
+    if (ch * 8 < p.D)
+      v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(tok + row / p.G) * p.q_st +
+                                          (int64_t)(kh * p.G + row % p.G) * p.q_sh + ch * 16);
+    sts128(dst + (ch >> 3) * kPanel + swz(row, ch & 7), v);
+  }
+  fence_proxy_async_smem();
+}
+
+template <typename T, int KD>
+__global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_constant__ MmaParams mp) {
+  typedef Geo<KD> Ge;
+  constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingV = Ge::kRingV;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kIdQK = instr_desc(kBF16, false, kM, kKT);
+  constexpr uint32_t kIdPV = instr_desc(kBF16, false, kM, KD, true);  // V: MN-major B
+  const AttnParams& p = mp.a;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);
+  uint64_t* q_empty = q_full + 1;         // MMA commit after a segment's last q.K^T
+  uint64_t* k_full = q_empty + 1;         // [kRingK]
+  uint64_t* k_empty = k_full + kRingK;    // [kRingK] MMA commit after the q.K^T that read it last
+  uint64_t* v_full = k_empty + kRingK;    // [kRingV]
+  uint64_t* v_empty = v_full + kRingV;    // [kRingV] MMA commit after the P.V that read it last
+  uint64_t* s_full = v_empty + kRingV;    // [2] MMA commit: S of the stream's step ready
+  uint64_t* p_full = s_full + 2;          // [2] the stream's four softmax warps wrote P
+  uint64_t* o_full = p_full + 2;          // [2] pairs: MMA commit after the stream's last P.V
+  uint64_t* o_both = o_full + 2;          // singles: MMA commit after the segment's last P.V
+  uint64_t* o_empty = o_both + 1;         // all eight softmax warps are done with the segment
+  uint64_t* ml_full = o_empty + 1;        // singles: both streams' m and l are in shared memory
+  uint64_t* seg_full = ml_full + 1;       // [kSegs]
+  uint64_t* seg_empty = seg_full + kSegs; // [kSegs]
+  uint64_t* drain = seg_empty + kSegs;
+  SegInfo* segs = reinterpret_cast<SegInfo*>(smem + Ge::kOffSeg);
+  float2* ml = reinterpret_cast<float2*>(smem + Ge::kOffMl);
+  volatile int* misc = reinterpret_cast<volatile int*>(smem + Ge::kOffMisc);  // [0] abort, [1] TMEM address
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+
+  if (threadIdx.x == 0) {
+    p.cuts[cta].nparts = 0;
+    misc[0] = 0;
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int s = 0; s < kRingK; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < kRingV; ++s) {
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 4);
+      mbar_init(&o_full[s], 1);
+    }
+    mbar_init(o_both, 1);
+    mbar_init(o_empty, 8);
+    mbar_init(ml_full, 8);
+    for (int s = 0; s < kSegs; ++s) {
+      mbar_init(&seg_full[s], 1);
+      mbar_init(&seg_empty[s], kSegReaders);
+    }
+    mbar_init(drain, 1);
+    fence_barrier_init();
+  }
+  Walk walk(p);
+  static_assert(sizeof(Walk::Scratch) <= 2 * kM * 8, "scratch of the schedule");
+  if (!walk.init<kThreads>(reinterpret_cast<Walk::Scratch*>(ml), cta, kMinPer)) return;  // all threads alike, before any TMEM is held
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(smem + Ge::kOffMisc + 4)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)misc[1];
+
+  if (warp == kWarpK) {
+    // ------------------------------------------------ schedule, Q and K tiles
+    const uint64_t pol = l2_evict_first_policy();
+    int nseg = 0, nq = 0, st = 0;
+    uint32_t tiles = 0, ph = 0;  // K tiles issued; phase parity of the ring's current round
+    bool ok = true;
+    Walk::Seg g;
+    while (ok) {
+      const bool more = walk.next(g);
+      const int ss = nseg % kSegs;
+      if (nseg >= kSegs)
+        ok = __all_sync(0xffffffffu, wait_or_abort(&seg_empty[ss], (uint32_t)(nseg / kSegs - 1) & 1u, misc, p.err));
+      if (!ok) break;
+      const Req rq = walk.seg_q;
+      const int tok0 = g.tile0 * p.tq;
+      if (lane == 0) {
+        SegInfo& i = segs[ss];
+        i.live = more;
+        if (more) {
+          i.pair = g.pair;
+          i.j0 = g.j0;
+          i.m = g.j1 - g.j0;
+          if (g.pair) {
+            i.n0 = max(0, min(g.j1, Walk::ntiles(p, rq, tok0 + p.tq)) - g.j0);
+            i.n1 = i.m;
+          } else {
+            i.n0 = (i.m + 1) >> 1;
+            i.n1 = i.m >> 1;
+          }
+          i.tok0 = tok0;
+          i.qst = rq.qst;
+          i.qlen = rq.qlen;
+          i.klen = rq.klen;
+          i.kbase = rq.kbase;
+          i.kh = g.kh;
+          i.slot = g.whole ? -1 : 2 * cta + (g.j0 > 0 ? 0 : 1);
+          i.nparts = g.nparts;
+          if (g.nparts > 0)
+            p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, min((g.pair ? 2 : 1) * p.tq, rq.qlen - tok0) * p.G, g.kh};
+        }
+        mbar_arrive(&seg_full[ss]);
+      }
+      __syncwarp();
+      ++nseg;
+      if (!more) break;
+      if (g.j0 >= g.j1) continue;  // no key is seen: the softmax warps write zeros
+      if (nq > 0 && !__all_sync(0xffffffffu, wait_or_abort(q_empty, (uint32_t)(nq - 1) & 1u, misc, p.err))) {
+        ok = false;
+        break;
+      }
+      ++nq;
+      const int nt = g.pair ? 2 : 1;
+      if (mp.q_tma) {
+        if (lane == 0) {
+          mbar_expect_tx(q_full, (uint32_t)(nt * Ge::kPanels * p.tq * p.G * 128));
+          for (int x = 0; x < nt; ++x)
+            for (int c = 0; c < Ge::kPanels; ++c)
+              tma_load_4d(smem + x * kTile + c * kPanel, &mp.tmap_q, 64 * c, g.kh * p.G, rq.qst + tok0 + x * p.tq, 0,
+                          q_full, 0ull);
+          mbar_arrive(q_full);
+        }
+      } else {
+        for (int x = 0; x < nt; ++x)
+          load_q<KD>(p, smem + x * kTile, g.kh, rq.qst + tok0 + x * p.tq, min(p.tq, rq.qlen - tok0 - x * p.tq), lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full);
+      }
+      int id = box_block(p, rq.kbase, rq.klen, g.j0, lane);
+      for (int j = g.j0; j < g.j1; ++j) {
+        const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
+        if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
+        if (!ok) break;
+        load_tile<KD>(mp, false, smem + Ge::kOffK + st * kTile, &k_full[st], j, rq.kbase, rq.klen, g.kh, id, lane, pol);
+        id = id_next;
+        ++tiles;
+        if (++st == kRingK) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) misc[0] = 1;
+    // no copy of this warp is in flight when the CTA ends: the last tile of
+    // each slot and the last Q (at once on the normal path)
+    for (uint32_t s = 0; s < (uint32_t)kRingK && s < tiles; ++s) {
+      const uint32_t last = s + kRingK * ((tiles - 1 - s) / kRingK);
+      mbar_wait(&k_full[s], (last / kRingK) & 1u, p.err);
+    }
+    if (nq > 0) mbar_wait(q_full, (uint32_t)(nq - 1) & 1u, p.err);
+  } else if (warp == kWarpV) {
+    // ------------------------------------------------ V tiles
+    const uint64_t pol = l2_evict_first_policy();
+    int st = 0;
+    uint32_t tiles = 0, ph = 0;
+    bool ok = true;
+    for (int nseg = 0; ok; ++nseg) {
+      const int ss = nseg % kSegs;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
+      if (!ok) break;
+      const SegInfo i = segs[ss];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
+      if (!i.live) break;
+      int id = i.m > 0 ? box_block(p, i.kbase, i.klen, i.j0, lane) : -1;
+      for (int j = i.j0; j < i.j0 + i.m; ++j) {
+        const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
+        if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
+        if (!ok) break;
+        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.kbase, i.klen, i.kh, id, lane, pol);
+        id = id_next;
+        ++tiles;
+        if (++st == kRingV) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) misc[0] = 1;
+    for (uint32_t s = 0; s < (uint32_t)kRingV && s < tiles; ++s) {
+      const uint32_t last = s + kRingV * ((tiles - 1 - s) / kRingV);
+      mbar_wait(&v_full[s], (last / kRingV) & 1u, p.err);
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t sq0 = smem_u32(smem);
+      // ring positions of the next K tile a first q.K^T takes, and of V
+      int kst = 0, vst = 0;
+      uint32_t kph = 0, vph = 0, nq = 0;
+      uint32_t np[2] = {0, 0};  // steps of either stream so far
+      bool ok = true;
+      auto qk = [&](int x, int tile_of_q, int st) {
+        const uint32_t sq = sq0 + tile_of_q * kTile;
+        const uint32_t sk = sq0 + Ge::kOffK + st * kTile;
+#pragma unroll
+        for (int ks = 0; ks < KD / 16; ++ks) {
+          const uint32_t off = (ks >> 2) * kPanel + (ks & 3) * 32;
+          umma_f16(tmem + x * kKT, sw128_desc(sq + off, 16, 1024), sw128_desc(sk + off, 16, 1024), kIdQK,
+                   ks > 0 ? 1u : 0u);
+        }
+        umma_commit(&s_full[x]);
+      };
+      auto pv = [&](int x, int st, bool first) {
+        const uint32_t sv = sq0 + Ge::kOffV + st * kTile;
+#pragma unroll
+        for (int ks = 0; ks < kKT / 16; ++ks)
+          umma_f16_ts(tmem + 2 * kKT + x * kM, tmem + x * kKT + 8 * ks, sw128_desc(sv + ks * 2048, kPanel, 1024),
+                      kIdPV, (!first || ks > 0) ? 1u : 0u);
+      };
+      for (int nseg = 0; ok; ++nseg) {
+        const int ss = nseg % kSegs;
+        if (!poll_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err)) {
+          ok = false;
+          break;
+        }
+        const int live = segs[ss].live, pair = segs[ss].pair, m = segs[ss].m;
+        const int n[2] = {segs[ss].n0, segs[ss].n1};
+        mbar_arrive(&seg_empty[ss]);
+        if (!live) break;
+        if (m > 0) {
+          ok = poll_or_abort(q_full, nq & 1u, misc, p.err);
+          ++nq;
+          if (!ok) break;
+        }
+        // q.K^T of step k of stream x; its K tile is the next one in the ring
+        // unless the pair's other stream took it already
+        auto step_qk = [&](int x, int k) {
+          const bool first_user = !pair || x == 0 || k >= n[0];
+          if (first_user && !poll_or_abort(&k_full[kst], kph, misc, p.err)) return false;
+          tc_fence_after();
+          qk(x, pair ? x : 0, kst);
+          if (!pair || x == 1) {  // the tile's last user (in a pair stream B takes every tile)
+            umma_commit(&k_empty[kst]);
+            if (++kst == kRingK) {
+              kst = 0;
+              kph ^= 1u;
+            }
+          }
+          if (x == (pair || !(m & 1) ? 1 : 0) && k == n[x] - 1) umma_commit(q_empty);  // the segment's last one
+          return true;
+        };
+        if (n[0] > 0) ok = step_qk(0, 0);
+        if (ok && n[1] > 0) ok = step_qk(1, 0);
+        // the last segment's O has been read
+        if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
+        const int steps = max(n[0], n[1]);
+        for (int k = 0; ok && k < steps; ++k) {
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {
+            if (!ok || k >= n[x]) continue;
+            const bool first_user = !pair || x == 0 || k >= n[0];
+            ok = poll_or_abort(&p_full[x], np[x] & 1u, misc, p.err) &&
+                 (!first_user || poll_or_abort(&v_full[vst], vph, misc, p.err));
+            if (!ok) continue;
+            ++np[x];
+            tc_fence_after();
+            pv(x, vst, k == 0);
+            if (!pair || x == 1) {
+              umma_commit(&v_empty[vst]);
+              if (++vst == kRingV) {
+                vst = 0;
+                vph ^= 1u;
+              }
+            }
+            if (k == n[x] - 1) {
+              if (pair)
+                umma_commit(&o_full[x]);
+              else if (x == ((m & 1) ? 0 : 1))
+                umma_commit(o_both);  // the last step of the single tile
+            } else {
+              ok = step_qk(x, k + 1);
+            }
+          }
+        }
+      }
+      if (!ok) misc[0] = 1;
+      umma_commit(drain);  // all MMAs of this thread complete before TMEM is released
+      mbar_wait(drain, 0u, p.err);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------ softmax of stream x
+    const int x = warp >> 2;
+    const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t t_s = tmem + lane_base + x * kKT;
+    const uint32_t t_o = tmem + lane_base + 2 * kKT;  // O of stream A; B's 128 columns on
+    const int hg = row % p.G, tg = row / p.G;         // head and token of the row within a tile
+    uint32_t ns = 0, no = 0, nb = 0;                  // phases of s_full, o_full, o_both / ml_full
+    bool ok = true;
+    for (int nseg = 0; ok; ++nseg) {
+      const int ss = nseg % kSegs;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
+      if (!ok) break;
+      const int live = segs[ss].live, pair = segs[ss].pair, j0 = segs[ss].j0, m_tiles = segs[ss].m;
+      const int n = x ? segs[ss].n1 : segs[ss].n0;
+      const int tok0 = segs[ss].tok0, qst = segs[ss].qst, qlen = segs[ss].qlen, klen = segs[ss].klen;
+      const int kh = segs[ss].kh, slot = segs[ss].slot;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
+      if (!live) break;
+      const int q0 = tok0 + (pair ? x * p.tq : 0);
+      const int qi = q0 + tg;
+      const bool row_ok = tg < p.tq && qi < qlen;
+      const bool any_row = __any_sync(0xffffffffu, row_ok);
+      const int lim = !row_ok ? -1 : p.bt != nullptr ? klen - qlen + qi : klen - 1;  // last key this query sees
+      const int lim_all = p.bt != nullptr ? klen - qlen + q0 : klen - 1;             // keys that all of them see
+      float m = -INFINITY, l = 0.f;
+      for (int k = 0; k < n; ++k) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[x], ns & 1u, misc, p.err));
+        if (!ok) break;
+        ++ns;
+        tc_fence_after();
+        if (any_row) {
+          const int j = pair ? j0 + k : j0 + 2 * k + x;
+          uint32_t sr[4][32];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_ld32_nowait(t_s + 32 * c, sr[c]);
+          tmem_wait_ld();
+          if (j * kKT + kKT - 1 > lim_all) {
+            const int nv = lim - j * kKT + 1;
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int e = 0; e < 32; ++e)
+                if (32 * c + e >= nv) sr[c][e] = __float_as_uint(-INFINITY);
+          }
+          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; e += 2)
+              m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+          const float mxs = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.sl2;
+          const bool grow = m != -INFINITY && mxs > m + 8.f;
+          if (__any_sync(0xffffffffu, grow)) {
+            // O holds the earlier steps: their P.V were issued before this S's commit
+            const float alpha = grow ? exp2f(m - mxs) : 1.f;
+#pragma unroll 1
+            for (int c = 0; c < KD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld16_nowait(t_o + x * kM + 16 * c, o);
+              tmem_wait_ld();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+              tmem_st16(t_o + x * kM + 16 * c, o);
+            }
+            l *= alpha;
+          }
+          if (grow || m == -INFINITY) m = mxs;
+          const float neg_m = m == -INFINITY ? 0.f : -m;
+          const f2_t sl2x2 = f2_pack(p.sl2, p.sl2), nm2 = f2_pack(neg_m, neg_m);
+          f2_t ls[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t pk[16];
+#pragma unroll
+            for (int c = 0; c < 16; ++c) {
+              float a0, a1;
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[q][2 * c]), __uint_as_float(sr[q][2 * c + 1])), sl2x2, nm2),
+                        a0, a1);
+              const float p0 = ex2_approx(a0), p1 = ex2_approx(a1);
+              pk[c] = pack2<T>(p0, p1);
+              ls[c & 1] = f2_add(ls[c & 1], f2_pack(p0, p1));
+            }
+            tmem_st16(t_s + 16 * q, pk);
+          }
+          tmem_wait_st();
+          float a0, a1, b0, b1;
+          f2_unpack(ls[0], a0, a1);
+          f2_unpack(ls[1], b0, b1);
+          l += (a0 + a1) + (b0 + b1);
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[x]);
+      }
+      if (!ok) break;
+      // The rows of this thread's epilogue: a pair's stream has its own tile,
+      // all dims; in a single the two warpgroups take half of the dims each
+      // of the joined streams.
+      const bool single = !pair;
+      float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
+      // everyone has read the m and l of the segment before
+      if (nseg > 0) ok = __all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err));
+      if (!ok) break;
+      if (single && m_tiles > 0) {
+        ml[x * kM + row] = make_float2(m, l);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ml_full);
+        ok = __all_sync(0xffffffffu, wait_or_abort(ml_full, nb & 1u, misc, p.err) &&
+                                         wait_or_abort(o_both, nb & 1u, misc, p.err));
+        if (!ok) break;
+        ++nb;
+        const float2 other = ml[(x ^ 1) * kM + row];
+        const float mm = fmaxf(m, other.x);
+        const float base = mm == -INFINITY ? 0.f : mm;
+        const float wo = exp2f(m - base), wt = exp2f(other.x - base);
+        wa = x ? wt : wo;
+        wb = x ? wo : wt;
+        l = l * wo + other.y * wt;
+        m = mm;
+      } else if (n > 0) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[x], no & 1u, misc, p.err));
+        if (!ok) break;
+        ++no;
+      }
+      tc_fence_after();
+      const int64_t tok = qst + qi;
+      const int h = kh * p.G + hg;
+      const bool have_b = single && m_tiles > 1;
+      const bool have = single ? m_tiles > 0 : n > 0;
+      const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
+      wa *= inv;
+      wb *= inv;
+      const int item_row = (pair ? x * p.tq * p.G : 0) + row;
+      if (row_ok && (!single || x == 0)) {
+        if (slot >= 0) {
+          reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
+        } else if (p.lse != nullptr) {
+          p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+        }
+      }
+      __syncwarp();
+      const int c_lo = single ? x * (KD / 32) : 0, c_hi = single ? c_lo + KD / 32 : KD / 16;  // 16 dims each
+      if (any_row) {
+#pragma unroll 1
+        for (int c = c_lo; c < c_hi; ++c) {
+          if (16 * c >= p.D) break;
+          uint32_t oa[16], ob[16];
+          float f[16];
+          if (have) tmem_ld16_nowait(t_o + (single ? 0 : x * kM) + 16 * c, oa);
+          if (have_b) tmem_ld16_nowait(t_o + kM + 16 * c, ob);
+          tmem_wait_ld();
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            f[e] = have ? __uint_as_float(oa[e]) * wa : 0.f;
+            if (have_b) f[e] = fmaf(__uint_as_float(ob[e]), wb, f[e]);
+          }
+          if (row_ok && slot >= 0) {
+            float* po = p.part_o + ((int64_t)slot * kItemRows + item_row) * p.D + 16 * c;
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+              if (16 * c + e < p.D) *reinterpret_cast<float4*>(po + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+          } else if (row_ok) {
+            unsigned char* po = p.out + tok * p.o_st + h * p.o_sh + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 16; e += 8)
+              if (16 * c + e < p.D)
+                *reinterpret_cast<uint4*>(po + 2 * e) =
+                    make_uint4(pack2<T>(f[e], f[e + 1]), pack2<T>(f[e + 2], f[e + 3]), pack2<T>(f[e + 4], f[e + 5]),
+                               pack2<T>(f[e + 6], f[e + 7]));
+          }
+          __syncwarp();  // the TMEM loads are the whole warp's
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(o_empty);
+    }
+    if (!ok) misc[0] = 1;
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+}
+
+template <typename T, int KD>
+int launch(const MmaParams& mp, cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(fd_attn_mma_kernel<T, KD>);
+  static unsigned long long done = 0;
+  const int st = fdh::ensure_smem(kern, Geo<KD>::kSmem, &done);
+  if (st != FD_OK) return st;
+  return fdh::launch_maybe_pdl(kern, dim3((unsigned)mp.a.ctas), dim3(kThreads), Geo<KD>::kSmem, s, false, mp,
+                               "fd_attn_mma_kernel launch");
+}
+
+}  // namespace mm
+
+bool mma_covers(const fd_attn_args* a) {
+  return (a->dtype == FD_DTYPE_F16 || a->dtype == FD_DTYPE_BF16) && a->head_size >= 64 && a->head_size <= 128;
+}
+
+size_t mma_workspace(const fd_attn_args* a) {
+  const size_t slots = 2 * (size_t)mm::kMaxCtas * mm::kItemRows;
+  return mm::kMaxCtas * sizeof(Cut) + slots * 8 + slots * (size_t)a->head_size * 4;
+}
+
+int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  int st = fdh::device_sms(&dev, &sms);
+  if (st != FD_OK) return st;
+  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
+  p.cuts = reinterpret_cast<Cut*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + mm::kMaxCtas * sizeof(Cut));
+  p.part_o = p.part_ml + 2 * 2 * (size_t)mm::kMaxCtas * mm::kItemRows;
+  p.tq = mm::kM / p.G;
+  p.ctas = sms < mm::kMaxCtas ? sms : mm::kMaxCtas;
+  mm::MmaParams mp{};
+  const int D = p.D;
+  mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
+  for (int t = 0; t < 2; ++t) {
+    if (p.nblk[t] == 0 || p.host[t]) continue;
+    const bool cross = p.bt == nullptr;
+    if (cross && p.nblk[t] > 0x7fffffff) continue;  // rows by 16-byte loads
+    if (!cross && p.BS % mm::kSub != 0) continue;
+    const int rows = cross ? (int)p.nblk[t] : p.BS;
+    const int64_t blocks = cross ? 1 : p.nblk[t];
+    const int64_t blk_sb = cross ? p.tok_sb[t] * rows : p.blk_sb[t];
+    mp.kv_tma[t] = encode_kv_map(&mp.tmap_k[t], p.k[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
+                                 blk_sb, mm::kSub, true) &&
+                   encode_kv_map(&mp.tmap_v[t], p.v[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
+                                 blk_sb, mm::kSub, true);
+  }
+  mp.a = p;
+  if (a->dtype == FD_DTYPE_BF16)
+    st = D <= 64 ? mm::launch<__nv_bfloat16, 64>(mp, s) : mm::launch<__nv_bfloat16, 128>(mp, s);
+  else
+    st = D <= 64 ? mm::launch<__half, 64>(mp, s) : mm::launch<__half, 128>(mp, s);
+  if (st != FD_OK) return st;
+  return combine_launch(p, a->dtype, mm::kItemRows, s);
+}
+
+}  // namespace at
+}  // namespace fdk
