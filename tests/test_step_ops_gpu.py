@@ -438,8 +438,8 @@ def test_requests_that_do_not_fit_write_nothing(dtype):
 def test_attention_refusals():
     q = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
     i, one = i32([0]), i32([1])
-    for args, match in (((q, q.float(), q, i, one, i, one), "alike|dtype"), ((q, q, q, i.long(), one, i, one), "int32"),
-                        ((q, q, q, i, one, i[:0], one), "int32"), ((q, q[..., :56], q[..., :56], i, one, i, one), "head")):
+    for args, match in (((q, q.float(), q, i, one, i, one), "dtype"), ((q, q, q, i.long(), one, i, one), "int32"),
+                        ((q, q, q, i, one, i[:0], one), "int32"), ((q, q[..., :56], q[..., :56], i, one, i, one), "head size")):
         with pytest.raises(RuntimeError, match=match):
             gpu_ops.cross_attn(*args, 1.0, torch.empty_like(q))
     with pytest.raises(RuntimeError, match="lse"):

@@ -144,10 +144,12 @@ struct Sched {
   __device__ __forceinline__ static bool is_pair(const AttnParams& p, const Req& q, int i) {
     return kPairs && 2 * i + 1 < tiles(p, q);
   }
-  // key tiles that the queries before token `te` of the request see
+  // keys, and key tiles, that the queries before token `te` of the request see
+  __device__ __forceinline__ static int visible(const AttnParams& p, const Req& q, int te) {
+    return max(0, p.bt != nullptr ? q.klen - q.qlen + te : q.klen);
+  }
   __device__ __forceinline__ static int ntiles(const AttnParams& p, const Req& q, int te) {
-    const int vis = p.bt != nullptr ? q.klen - q.qlen + te : q.klen;
-    return vis > 0 ? (vis + kKT - 1) / kKT : 0;
+    return (visible(p, q, te) + kKT - 1) / kKT;
   }
   __device__ __forceinline__ static int item_end(const AttnParams& p, const Req& q, int i) {
     return (int)min((long long)(i + 1) * (kPairs ? 2 : 1) * p.tq, (long long)q.qlen);

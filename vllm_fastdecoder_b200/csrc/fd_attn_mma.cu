@@ -5,26 +5,32 @@
 //   l = sum P,  O [128 rows x D] += P . V,  o = O / l, lse = ln 2 (m + log2 l)
 //
 // A CTA walks its range of the schedule (fd_attn.cuh) segment by segment and
-// runs two STREAMS of such products at a time, so that one stream's softmax
-// overlaps the other's matrix products.  In a pair (256 rows and more) the
+// runs two STREAMS of such products.  In a pair (256 rows and more) the
 // streams are two neighbouring query tiles and share every K/V tile; in a
 // single tile (few query rows: bound by the bytes of the cache) stream A
 // takes the even key tiles and stream B the odd ones of the same query tile,
-// and the two are joined in registers at the end.  Eleven warps:
-//   8   schedule, Q tiles and K tiles   } TMA boxes of 16 keys with the
-//   10  V tiles                         } 128-byte swizzle the MMA reads, or
-//       16-byte loads stored in the same layout where a box is in the host
-//       tier, spans blocks (block sizes that are no multiple of 16), or is
-//       cut by the end of a request's V (rows behind it must be 0: P is 0
-//       there, and 0 x NaN is not)
-//   9   one thread issues the MMAs: q.K^T of step k + 1 of a stream right
-//       after its P.V of step k
-//   0-3, 4-7  softmax of stream A, B: one thread per row with all 128 keys of
-//       a tile.  P overwrites the first half of its S in TMEM as 16-bit
-//       values (the A operand of P.V); O stays in TMEM over a segment and is
-//       rescaled only when a row's maximum passes its reference m by more
-//       than 2^8, so P stays below 2^8; row sums add the fp32 values of P.
-// TMEM: S/P of A [0, 128), of B [128, 256), O of A [256, 384), of B [384, 512).
+// and the two are joined in registers at the end.
+//
+// What would bound a stream that takes one step after the other is its chain
+// (scores, softmax, P.V, scores ...), with the tensor cores and the SFU each
+// idle half of the time.  So a stream works on 64 keys at a time with two S
+// buffers: q.K^T of step i + 2 is issued right behind P.V of step i, and the
+// softmax of step i + 1 finds its scores ready.  Twelve warps:
+//   8      schedule, Q tiles and K tiles  } TMA boxes of 16 keys with the
+//   10     V tiles                        } 128-byte swizzle the MMA reads, or
+//          16-byte loads stored in the same layout where a box is in the host
+//          tier, spans blocks (block sizes that are no multiple of 16), or is
+//          cut by the end of a request's V (rows behind it must be 0: P is 0
+//          there, and 0 x NaN is not)
+//   9, 11  one thread each issues the MMAs of stream A, B (one thread alone
+//          issues an MMA per ~70 cycles, more than a 64-key step leaves)
+//   0-3, 4-7  softmax of stream A, B: one thread per row.  P overwrites the
+//          first half of its S buffer in TMEM as 16-bit values (the A operand
+//          of P.V); O stays in TMEM over a segment and is rescaled only when a
+//          row's maximum passes its reference m by more than 2^8, so P stays
+//          below 2^8; row sums add the fp32 values of P.
+// TMEM: S/P of A [0, 128), of B [128, 256), two buffers of 64 columns each; O
+// of A [256, 384), of B [384, 512).
 // Scores, sums and O are fp32; P is rounded to the input type (the tensor
 // core's operand type), the result once.  Every wait is bounded, and a role
 // that gives up raises the CTA's abort flag for the others.
@@ -46,10 +52,11 @@ constexpr int kKT = 128;            // keys per tile (MMA N of S, K of P.V)
 constexpr int kSub = 16;            // keys per TMA box
 constexpr int kSubs = kKT / kSub;
 constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims
-constexpr int kWarpK = 8, kWarpMma = 9, kWarpV = 10;
-constexpr int kThreads = 11 * 32;
+constexpr int kHalf = 64;           // keys per step of a stream
+constexpr int kWarpK = 8, kWarpMmaA = 9, kWarpV = 10, kWarpMmaB = 11;
+constexpr int kThreads = 12 * 32;
 constexpr int kSegs = 4;            // segments in flight between the roles
-constexpr int kSegReaders = 10;     // MMA thread, V producer, eight softmax warps
+constexpr int kSegReaders = 11;     // MMA threads, V producer, eight softmax warps
 constexpr int kItemRows = 2 * kM;
 constexpr int kMaxCtas = 160;
 constexpr int kFixed = 3;           // an item's fixed cost in key tiles of a single
@@ -65,9 +72,9 @@ struct Geo {
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kRingK * kTile;
   static constexpr int kOffBar = kOffV + kRingV * kTile;
-  // q full/empty, k full/empty, v full/empty, s_full[2], p_full[2], o_full[2],
-  // o_both, o_empty, ml_full, seg full/empty, drain
-  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 2 + 2 + 2 + 3 + 2 * kSegs + 1;
+  // q full/empty, k full/empty, v full/empty, s_full[2][2], p_full[2][2], pv_done[2],
+  // o_full[2], o_both, o_empty, ml_full, seg full/empty, drain
+  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 4 + 4 + 2 + 2 + 3 + 2 * kSegs + 1;
   static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kOffMl = kOffSeg + kSegs * 64;   // [2 streams][128 rows] float2 (before that: Walk::Scratch)
   static constexpr int kOffMisc = kOffMl + 2 * kM * 8;  // abort flag, TMEM address
@@ -80,7 +87,7 @@ struct SegInfo {
   int live;      // 0: no more segments
   int pair;
   int j0, m;     // first key tile, key tiles
-  int n0, n1;    // steps of stream A, B
+  int n0, n1;    // steps (64 keys) of stream A, B
   int tok0;      // first query token of the item within the request
   int qst, qlen, klen, kbase, kh;
   int slot;      // -1: whole, else its slot of the partials
@@ -128,6 +135,13 @@ __device__ __forceinline__ bool poll_or_abort(uint64_t* bar, uint32_t parity, vo
   }
 }
 
+// L2 policy for data that other CTAs read too.
+__device__ __forceinline__ uint64_t l2_evict_normal_policy() {
+  uint64_t pol;
+  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
+  return pol;
+}
+
 // 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
@@ -139,6 +153,13 @@ __device__ __forceinline__ float fmax3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
+}
+
+// Scores from the nv-th on are not seen.
+__device__ __forceinline__ void hide(uint32_t (&r)[32], int nv) {
+#pragma unroll
+  for (int e = 0; e < 32; ++e)
+    if (e >= nv) r[e] = __float_as_uint(-INFINITY);
 }
 
 template <typename T>
@@ -266,25 +287,124 @@ __device__ __forceinline__ void load_q(const AttnParams& p, unsigned char* dst, 
   fence_proxy_async_smem();
 }
 
+// The end of a segment for one softmax warp of stream x: o and lse of its
+// rows, or their partials.  A pair's stream has its own tile and all dims; in
+// a single the two warpgroups take half of the dims each of the joined
+// streams.  Not inlined: what it needs stays out of the main loop's registers.
+template <typename T, int KD>
+__device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg, int x, uint32_t t_s, float m, float l,
+                                         bool any_row, int nseg, uint32_t* phases, float2* ml, uint64_t* o_empty,
+                                         volatile int* misc) {
+  uint64_t* o_full = o_empty - 3;  // [2], then o_both, o_empty, ml_full
+  uint64_t* o_both = o_empty - 1;
+  uint64_t* ml_full = o_empty + 1;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n = x ? seg.n1 : seg.n0;
+  uint32_t ph = *phases;
+        const bool pair = seg.pair != 0, single = !pair;
+        const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+        const int tg = row / p.G, hg = row % p.G;
+        const uint32_t t_o = t_s - x * kKT + 2 * kKT;  // O of stream A; B's 128 columns on
+        const int m_tiles = seg.m, slot = seg.slot;
+        const int qi = seg.tok0 + (pair ? x * p.tq : 0) + tg;
+        const bool row_ok = tg < p.tq && qi < seg.qlen;
+        float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
+        // everyone has read the m and l of the segment before
+        if (nseg > 0 && !__all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err)))
+          return false;
+        if (single && m_tiles > 0) {
+          ml[x * kM + row] = make_float2(m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ml_full);
+          if (!__all_sync(0xffffffffu, wait_or_abort(ml_full, (ph >> 3) & 1u, misc, p.err) &&
+                                           wait_or_abort(o_both, (ph >> 3) & 1u, misc, p.err)))
+            return false;
+          ph ^= 8u;
+          const float2 other = ml[(x ^ 1) * kM + row];
+          const float mm = fmaxf(m, other.x);
+          const float base = mm == -INFINITY ? 0.f : mm;
+          const float wo = exp2f(m - base), wt = exp2f(other.x - base);
+          wa = x ? wt : wo;
+          wb = x ? wo : wt;
+          l = l * wo + other.y * wt;
+          m = mm;
+        } else if (n > 0) {
+          if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[x], (ph >> 2) & 1u, misc, p.err))) return false;
+          ph ^= 4u;
+        }
+        tc_fence_after();
+        const int64_t tok = seg.qst + qi;
+        const int h = seg.kh * p.G + hg;
+        const bool have_b = single && seg.n1 > 0;
+        const bool have = single ? m_tiles > 0 : n > 0;
+        const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
+        wa *= inv;
+        wb *= inv;
+        const int item_row = (pair ? x * p.tq * p.G : 0) + row;
+        if (row_ok && (!single || x == 0)) {
+          if (slot >= 0) {
+            reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
+          } else if (p.lse != nullptr) {
+            p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+          }
+        }
+        __syncwarp();
+        const int c_lo = single ? x * (KD / 32) : 0, c_hi = single ? c_lo + KD / 32 : KD / 16;  // 16 dims each
+        if (any_row) {
+  #pragma unroll 1
+          for (int c = c_lo; c < c_hi; ++c) {
+            if (16 * c >= p.D) break;
+            uint32_t oa[16], ob[16];
+            float f[16];
+            if (have) tmem_ld16_nowait(t_o + (single ? 0 : x * kM) + 16 * c, oa);
+            if (have_b) tmem_ld16_nowait(t_o + kM + 16 * c, ob);
+            tmem_wait_ld();
+  #pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              f[e] = have ? __uint_as_float(oa[e]) * wa : 0.f;
+              if (have_b) f[e] = fmaf(__uint_as_float(ob[e]), wb, f[e]);
+            }
+            if (row_ok && slot >= 0) {
+              float* po = p.part_o + ((int64_t)slot * kItemRows + item_row) * p.D + 16 * c;
+  #pragma unroll
+              for (int e = 0; e < 16; e += 4)
+                if (16 * c + e < p.D) *reinterpret_cast<float4*>(po + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+            } else if (row_ok) {
+              unsigned char* po = p.out + tok * p.o_st + h * p.o_sh + 32 * c;
+  #pragma unroll
+              for (int e = 0; e < 16; e += 8)
+                if (16 * c + e < p.D)
+                  *reinterpret_cast<uint4*>(po + 2 * e) =
+                      make_uint4(pack2<T>(f[e], f[e + 1]), pack2<T>(f[e + 2], f[e + 3]), pack2<T>(f[e + 4], f[e + 5]),
+                                 pack2<T>(f[e + 6], f[e + 7]));
+            }
+            __syncwarp();  // the TMEM loads are the whole warp's
+          }
+        }
+  *phases = ph;
+  return true;
+}
+
 template <typename T, int KD>
 __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_constant__ MmaParams mp) {
   typedef Geo<KD> Ge;
   constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingV = Ge::kRingV;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
-  constexpr uint32_t kIdQK = instr_desc(kBF16, false, kM, kKT);
+  constexpr uint32_t kIdQK = instr_desc(kBF16, false, kM, kHalf);
   constexpr uint32_t kIdPV = instr_desc(kBF16, false, kM, KD, true);  // V: MN-major B
   const AttnParams& p = mp.a;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);
-  uint64_t* q_empty = q_full + 1;         // MMA commit after a segment's last q.K^T
+  uint64_t* q_empty = q_full + 1;         // both streams' MMA commits after a segment's last q.K^T
   uint64_t* k_full = q_empty + 1;         // [kRingK]
-  uint64_t* k_empty = k_full + kRingK;    // [kRingK] MMA commit after the q.K^T that read it last
+  uint64_t* k_empty = k_full + kRingK;    // [kRingK] two arrivals: the streams are done with the tile
   uint64_t* v_full = k_empty + kRingK;    // [kRingV]
-  uint64_t* v_empty = v_full + kRingV;    // [kRingV] MMA commit after the P.V that read it last
-  uint64_t* s_full = v_empty + kRingV;    // [2] MMA commit: S of the stream's step ready
-  uint64_t* p_full = s_full + 2;          // [2] the stream's four softmax warps wrote P
-  uint64_t* o_full = p_full + 2;          // [2] pairs: MMA commit after the stream's last P.V
-  uint64_t* o_both = o_full + 2;          // singles: MMA commit after the segment's last P.V
+  uint64_t* v_empty = v_full + kRingV;    // [kRingV] two arrivals
+  uint64_t* s_full = v_empty + kRingV;    // [2][2] MMA commit: S of the stream's step is in its buffer
+  uint64_t* p_full = s_full + 4;          // [2][2] the stream's four softmax warps wrote P there
+  uint64_t* pv_done = p_full + 4;         // [2] MMA commit after each P.V of the stream
+  uint64_t* o_full = pv_done + 2;         // [2] pairs: MMA commit after the stream's last P.V
+  uint64_t* o_both = o_full + 2;          // singles: both streams' last P.V
   uint64_t* o_empty = o_both + 1;         // all eight softmax warps are done with the segment
   uint64_t* ml_full = o_empty + 1;        // singles: both streams' m and l are in shared memory
   uint64_t* seg_full = ml_full + 1;       // [kSegs]
@@ -301,34 +421,37 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     p.cuts[cta].nparts = 0;
     misc[0] = 0;
     mbar_init(q_full, 1);
-    mbar_init(q_empty, 1);
+    mbar_init(q_empty, 2);
     for (int s = 0; s < kRingK; ++s) {
       mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 1);
+      mbar_init(&k_empty[s], 2);
     }
     for (int s = 0; s < kRingV; ++s) {
       mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 1);
+      mbar_init(&v_empty[s], 2);
     }
-    for (int s = 0; s < 2; ++s) {
+    for (int s = 0; s < 4; ++s) {
       mbar_init(&s_full[s], 1);
       mbar_init(&p_full[s], 4);
+    }
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&pv_done[s], 1);
       mbar_init(&o_full[s], 1);
     }
-    mbar_init(o_both, 1);
+    mbar_init(o_both, 2);
     mbar_init(o_empty, 8);
     mbar_init(ml_full, 8);
     for (int s = 0; s < kSegs; ++s) {
       mbar_init(&seg_full[s], 1);
       mbar_init(&seg_empty[s], kSegReaders);
     }
-    mbar_init(drain, 1);
+    mbar_init(drain, 2);
     fence_barrier_init();
   }
   Walk walk(p);
   static_assert(sizeof(Walk::Scratch) <= 2 * kM * 8, "scratch of the schedule");
   if (!walk.init<kThreads>(reinterpret_cast<Walk::Scratch*>(ml), cta, kMinPer)) return;  // all threads alike, before any TMEM is held
-  if (warp == kWarpMma) {
+  if (warp == kWarpMmaA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(smem + Ge::kOffMisc + 4)),
                  "r"(512)
@@ -342,7 +465,10 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
 
   if (warp == kWarpK) {
     // ------------------------------------------------ schedule, Q and K tiles
-    const uint64_t pol = l2_evict_first_policy();
+    const uint64_t pol_once = l2_evict_first_policy(), pol_again = l2_evict_normal_policy();
+    auto steps = [](int vis, int j0, int j1) {
+      return max(0, min(2 * j1, (vis + kHalf - 1) / kHalf) - 2 * j0);
+    };
     int nseg = 0, nq = 0, st = 0;
     uint32_t tiles = 0, ph = 0;  // K tiles issued; phase parity of the ring's current round
     bool ok = true;
@@ -362,12 +488,15 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           i.pair = g.pair;
           i.j0 = g.j0;
           i.m = g.j1 - g.j0;
+          // steps of 64 keys: those that some query of the stream's tile sees
+          const int last = Walk::visible(p, rq, min(tok0 + (g.pair ? 2 : 1) * p.tq, rq.qlen));
           if (g.pair) {
-            i.n0 = max(0, min(g.j1, Walk::ntiles(p, rq, tok0 + p.tq)) - g.j0);
-            i.n1 = i.m;
+            i.n0 = steps(Walk::visible(p, rq, tok0 + p.tq), g.j0, g.j1);
+            i.n1 = steps(last, g.j0, g.j1);
           } else {
-            i.n0 = (i.m + 1) >> 1;
-            i.n1 = i.m >> 1;
+            const int cut = 2 * i.m - steps(last, g.j0, g.j1);  // 1: the last tile's second half is not seen
+            i.n0 = ((i.m + 1) & ~1) - (i.m & 1 ? cut : 0);
+            i.n1 = (i.m & ~1) - (i.m & 1 ? 0 : cut);
           }
           i.tok0 = tok0;
           i.qst = rq.qst;
@@ -407,6 +536,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
+      // a pair's neighbours read the same keys again: they stay in L2
+      const uint64_t pol = g.pair ? pol_again : pol_once;
       int id = box_block(p, rq.kbase, rq.klen, g.j0, lane);
       for (int j = g.j0; j < g.j1; ++j) {
         const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
@@ -431,7 +562,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     if (nq > 0) mbar_wait(q_full, (uint32_t)(nq - 1) & 1u, p.err);
   } else if (warp == kWarpV) {
     // ------------------------------------------------ V tiles
-    const uint64_t pol = l2_evict_first_policy();
+    const uint64_t pol_once = l2_evict_first_policy(), pol_again = l2_evict_normal_policy();
     int st = 0;
     uint32_t tiles = 0, ph = 0;
     bool ok = true;
@@ -443,6 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&seg_empty[ss]);
       if (!i.live) break;
+      const uint64_t pol = i.pair ? pol_again : pol_once;
       int id = i.m > 0 ? box_block(p, i.kbase, i.klen, i.j0, lane) : -1;
       for (int j = i.j0; j < i.j0 + i.m; ++j) {
         const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
@@ -462,170 +594,164 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       const uint32_t last = s + kRingV * ((tiles - 1 - s) / kRingV);
       mbar_wait(&v_full[s], (last / kRingV) & 1u, p.err);
     }
-  } else if (warp == kWarpMma) {
-    // ------------------------------------------------ MMA issuer
+  } else if (warp == kWarpMmaA || warp == kWarpMmaB) {
+    // ------------------------------------------------ MMA issuer of stream x
     if (lane == 0) {
+      const int x = warp == kWarpMmaB ? 1 : 0;
       const uint32_t sq0 = smem_u32(smem);
-      // ring positions of the next K tile a first q.K^T takes, and of V
-      int kst = 0, vst = 0;
-      uint32_t kph = 0, vph = 0, nq = 0;
-      uint32_t np[2] = {0, 0};  // steps of either stream so far
+      const uint32_t t_s = tmem + x * kKT, t_o = tmem + 2 * kKT + x * kM;
+      uint32_t tile0 = 0, nq = 0;   // K/V tiles of earlier segments; segments with keys
+      uint32_t pp = 0;              // phase parities of p_full's two buffers
       bool ok = true;
-      auto qk = [&](int x, int tile_of_q, int st) {
-        const uint32_t sq = sq0 + tile_of_q * kTile;
-        const uint32_t sk = sq0 + Ge::kOffK + st * kTile;
-#pragma unroll
-        for (int ks = 0; ks < KD / 16; ++ks) {
-          const uint32_t off = (ks >> 2) * kPanel + (ks & 3) * 32;
-          umma_f16(tmem + x * kKT, sw128_desc(sq + off, 16, 1024), sw128_desc(sk + off, 16, 1024), kIdQK,
-                   ks > 0 ? 1u : 0u);
-        }
-        umma_commit(&s_full[x]);
-      };
-      auto pv = [&](int x, int st, bool first) {
-        const uint32_t sv = sq0 + Ge::kOffV + st * kTile;
-#pragma unroll
-        for (int ks = 0; ks < kKT / 16; ++ks)
-          umma_f16_ts(tmem + 2 * kKT + x * kM, tmem + x * kKT + 8 * ks, sw128_desc(sv + ks * 2048, kPanel, 1024),
-                      kIdPV, (!first || ks > 0) ? 1u : 0u);
-      };
       for (int nseg = 0; ok; ++nseg) {
         const int ss = nseg % kSegs;
-        if (!poll_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err)) {
-          ok = false;
-          break;
-        }
+        ok = poll_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err);
+        if (!ok) break;
         const int live = segs[ss].live, pair = segs[ss].pair, m = segs[ss].m;
-        const int n[2] = {segs[ss].n0, segs[ss].n1};
+        const int n = x ? segs[ss].n1 : segs[ss].n0;
         mbar_arrive(&seg_empty[ss]);
         if (!live) break;
+        // the ring's tile that step i takes, and whether it is the tile's last step
+        auto tile_of = [&](int i) { return tile0 + (pair ? (i >> 1) : 2 * (i >> 1) + x); };
+        // a single's tile has one user, which arrives for both
+        auto release = [&](uint64_t* empty) {
+          umma_commit(empty);
+          if (!pair) mbar_arrive(empty);
+        };
+        auto qk = [&](int i) {
+          const uint32_t t = tile_of(i);
+          const int st = t % kRingK;
+          if (!(i & 1) && !poll_or_abort(&k_full[st], (t / kRingK) & 1u, misc, p.err)) return false;
+          tc_fence_after();
+          const uint32_t sq = sq0 + (pair ? x : 0) * kTile;
+          const uint32_t sk = sq0 + Ge::kOffK + st * kTile + (i & 1) * (kHalf * 128);
+#pragma unroll
+          for (int ks = 0; ks < KD / 16; ++ks) {
+            const uint32_t off = (ks >> 2) * kPanel + (ks & 3) * 32;
+            umma_f16(t_s + (i & 1) * kHalf, sw128_desc(sq + off, 16, 1024), sw128_desc(sk + off, 16, 1024), kIdQK,
+                     ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[2 * x + (i & 1)]);
+          if ((i & 1) || i == n - 1) release(&k_empty[st]);
+          if (i == n - 1) umma_commit(q_empty);
+          return true;
+        };
         if (m > 0) {
           ok = poll_or_abort(q_full, nq & 1u, misc, p.err);
           ++nq;
-          if (!ok) break;
+          if (ok && n == 0) mbar_arrive(q_empty);
         }
-        // q.K^T of step k of stream x; its K tile is the next one in the ring
-        // unless the pair's other stream took it already
-        auto step_qk = [&](int x, int k) {
-          const bool first_user = !pair || x == 0 || k >= n[0];
-          if (first_user && !poll_or_abort(&k_full[kst], kph, misc, p.err)) return false;
-          tc_fence_after();
-          qk(x, pair ? x : 0, kst);
-          if (!pair || x == 1) {  // the tile's last user (in a pair stream B takes every tile)
-            umma_commit(&k_empty[kst]);
-            if (++kst == kRingK) {
-              kst = 0;
-              kph ^= 1u;
-            }
-          }
-          if (x == (pair || !(m & 1) ? 1 : 0) && k == n[x] - 1) umma_commit(q_empty);  // the segment's last one
-          return true;
-        };
-        if (n[0] > 0) ok = step_qk(0, 0);
-        if (ok && n[1] > 0) ok = step_qk(1, 0);
+        if (ok && n > 0) ok = qk(0);
+        if (ok && n > 1) ok = qk(1);
         // the last segment's O has been read
         if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
-        const int steps = max(n[0], n[1]);
-        for (int k = 0; ok && k < steps; ++k) {
+        for (int i = 0; ok && i < n; ++i) {
+          const uint32_t t = tile_of(i);
+          const int st = t % kRingV, h = i & 1;
+          ok = poll_or_abort(&p_full[2 * x + h], (pp >> h) & 1u, misc, p.err) &&
+               (h || poll_or_abort(&v_full[st], (t / kRingV) & 1u, misc, p.err));
+          if (!ok) break;
+          pp ^= 1u << h;
+          tc_fence_after();
+          const uint32_t sv = sq0 + Ge::kOffV + st * kTile + h * (kHalf * 128);
 #pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            if (!ok || k >= n[x]) continue;
-            const bool first_user = !pair || x == 0 || k >= n[0];
-            ok = poll_or_abort(&p_full[x], np[x] & 1u, misc, p.err) &&
-                 (!first_user || poll_or_abort(&v_full[vst], vph, misc, p.err));
-            if (!ok) continue;
-            ++np[x];
-            tc_fence_after();
-            pv(x, vst, k == 0);
-            if (!pair || x == 1) {
-              umma_commit(&v_empty[vst]);
-              if (++vst == kRingV) {
-                vst = 0;
-                vph ^= 1u;
-              }
-            }
-            if (k == n[x] - 1) {
-              if (pair)
-                umma_commit(&o_full[x]);
-              else if (x == ((m & 1) ? 0 : 1))
-                umma_commit(o_both);  // the last step of the single tile
-            } else {
-              ok = step_qk(x, k + 1);
-            }
+          for (int ks = 0; ks < kHalf / 16; ++ks)
+            umma_f16_ts(t_o, t_s + h * kHalf + 8 * ks, sw128_desc(sv + ks * 2048, kPanel, 1024), kIdPV,
+                        (i > 0 || ks > 0) ? 1u : 0u);
+          umma_commit(&pv_done[x]);
+          if (h || i == n - 1) release(&v_empty[st]);
+          if (i + 2 < n) ok = qk(i + 2);
+        }
+        if (!ok) break;
+        if (m > 0) {
+          if (n == 0) {
+            if (!pair) mbar_arrive(o_both);
+          } else {
+            umma_commit(pair ? &o_full[x] : o_both);
           }
+          // a pair's tiles that only the other stream sees
+          for (int t = (n + 1) >> 1; ok && pair && t < m; ++t) {
+            const uint32_t u = tile0 + t;
+            ok = poll_or_abort(&k_full[u % kRingK], (u / kRingK) & 1u, misc, p.err);
+            if (ok) mbar_arrive(&k_empty[u % kRingK]);
+            ok = ok && poll_or_abort(&v_full[u % kRingV], (u / kRingV) & 1u, misc, p.err);
+            if (ok) mbar_arrive(&v_empty[u % kRingV]);
+          }
+          tile0 += m;
         }
       }
       if (!ok) misc[0] = 1;
-      umma_commit(drain);  // all MMAs of this thread complete before TMEM is released
+      umma_commit(drain);  // all MMAs of both threads complete before TMEM is released
       mbar_wait(drain, 0u, p.err);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------ softmax of stream x
     const int x = warp >> 2;
-    const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
-    const uint32_t lane_base = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t t_s = tmem + lane_base + x * kKT;
-    const uint32_t t_o = tmem + lane_base + 2 * kKT;  // O of stream A; B's 128 columns on
-    const int hg = row % p.G, tg = row / p.G;         // head and token of the row within a tile
-    uint32_t ns = 0, no = 0, nb = 0;                  // phases of s_full, o_full, o_both / ml_full
+    const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kKT;
+    // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3), pv_done (4)
+    uint32_t ph = 0;
     bool ok = true;
     for (int nseg = 0; ok; ++nseg) {
       const int ss = nseg % kSegs;
       ok = __all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
       if (!ok) break;
-      const int live = segs[ss].live, pair = segs[ss].pair, j0 = segs[ss].j0, m_tiles = segs[ss].m;
-      const int n = x ? segs[ss].n1 : segs[ss].n0;
-      const int tok0 = segs[ss].tok0, qst = segs[ss].qst, qlen = segs[ss].qlen, klen = segs[ss].klen;
-      const int kh = segs[ss].kh, slot = segs[ss].slot;
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[ss]);
-      if (!live) break;
-      const int q0 = tok0 + (pair ? x * p.tq : 0);
-      const int qi = q0 + tg;
-      const bool row_ok = tg < p.tq && qi < qlen;
-      const bool any_row = __any_sync(0xffffffffu, row_ok);
-      const int lim = !row_ok ? -1 : p.bt != nullptr ? klen - qlen + qi : klen - 1;  // last key this query sees
-      const int lim_all = p.bt != nullptr ? klen - qlen + q0 : klen - 1;             // keys that all of them see
+      const SegInfo& seg = segs[ss];  // stays until this segment's end
+      if (!seg.live) break;
+      const int n = x ? seg.n1 : seg.n0;
+      const int jstep = seg.pair ? kKT : 2 * kKT, jfirst = (seg.j0 + (seg.pair ? 0 : x)) * kKT;
+      bool any_row;
+      int lim, lim_all;  // last key that this row sees, that all rows of the tile see
+      {
+        const int tg = ((warp & 3) * 32 + lane) / p.G;  // token of the row within the tile
+        const int q0 = seg.tok0 + (seg.pair ? x * p.tq : 0), qi = q0 + tg;
+        const bool row_ok = tg < p.tq && qi < seg.qlen;
+        any_row = __any_sync(0xffffffffu, row_ok);
+        lim = !row_ok ? -1 : p.bt != nullptr ? seg.klen - seg.qlen + qi : seg.klen - 1;
+        lim_all = p.bt != nullptr ? seg.klen - seg.qlen + q0 : seg.klen - 1;
+      }
       float m = -INFINITY, l = 0.f;
-      for (int k = 0; k < n; ++k) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[x], ns & 1u, misc, p.err));
+      for (int i = 0; i < n; ++i) {
+        const int h = i & 1;
+        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * x + h], (ph >> h) & 1u, misc, p.err));
         if (!ok) break;
-        ++ns;
+        ph ^= 1u << h;
         tc_fence_after();
         if (any_row) {
-          const int j = pair ? j0 + k : j0 + 2 * k + x;
-          uint32_t sr[4][32];
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_ld32_nowait(t_s + 32 * c, sr[c]);
+          const int key0 = jfirst + (i >> 1) * jstep + h * kHalf;
+          uint32_t ra[32], rb[32];
+          tmem_ld32_nowait(t_s + h * kHalf, ra);
+          tmem_ld32_nowait(t_s + h * kHalf + 32, rb);
           tmem_wait_ld();
-          if (j * kKT + kKT - 1 > lim_all) {
-            const int nv = lim - j * kKT + 1;
-#pragma unroll
-            for (int c = 0; c < 4; ++c)
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (32 * c + e >= nv) sr[c][e] = __float_as_uint(-INFINITY);
+          if (key0 + kHalf - 1 > lim_all) {
+            hide(ra, lim - key0 + 1);
+            hide(rb, lim - key0 + 1 - 32);
           }
           float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-#pragma unroll
-            for (int e = 0; e < 32; e += 2)
-              m4[(e >> 1) & 3] = fmax3(m4[(e >> 1) & 3], __uint_as_float(sr[c][e]), __uint_as_float(sr[c][e + 1]));
+          for (int e = 0; e < 32; e += 4) {
+            m4[0] = fmax3(m4[0], __uint_as_float(ra[e]), __uint_as_float(ra[e + 1]));
+            m4[1] = fmax3(m4[1], __uint_as_float(rb[e]), __uint_as_float(rb[e + 1]));
+            m4[2] = fmax3(m4[2], __uint_as_float(ra[e + 2]), __uint_as_float(ra[e + 3]));
+            m4[3] = fmax3(m4[3], __uint_as_float(rb[e + 2]), __uint_as_float(rb[e + 3]));
+          }
           const float mxs = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.sl2;
           const bool grow = m != -INFINITY && mxs > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {
-            // O holds the earlier steps: their P.V were issued before this S's commit
+            // O takes the earlier steps: the last one's P.V may still run (the
+            // ones before it were issued before this S's q.K^T)
+            ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[x], ((ph >> 4) & 1u) ^ 1u, misc, p.err));
+            if (!ok) break;
+            tc_fence_after();
             const float alpha = grow ? exp2f(m - mxs) : 1.f;
 #pragma unroll 1
             for (int c = 0; c < KD / 16; ++c) {
               uint32_t o[16];
-              tmem_ld16_nowait(t_o + x * kM + 16 * c, o);
+              tmem_ld16_nowait(t_s + 2 * kKT + 16 * c, o);
               tmem_wait_ld();
 #pragma unroll
               for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-              tmem_st16(t_o + x * kM + 16 * c, o);
+              tmem_st16(t_s + 2 * kKT + 16 * c, o);
             }
             l *= alpha;
           }
@@ -633,112 +759,40 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           const float neg_m = m == -INFINITY ? 0.f : -m;
           const f2_t sl2x2 = f2_pack(p.sl2, p.sl2), nm2 = f2_pack(neg_m, neg_m);
           f2_t ls[2] = {f2_pack(0.f, 0.f), f2_pack(0.f, 0.f)};
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          auto expo = [&](const uint32_t (&r)[32], int col) {
             uint32_t pk[16];
 #pragma unroll
-            for (int c = 0; c < 16; ++c) {
+            for (int e = 0; e < 16; ++e) {
               float a0, a1;
-              f2_unpack(f2_fma(f2_pack(__uint_as_float(sr[q][2 * c]), __uint_as_float(sr[q][2 * c + 1])), sl2x2, nm2),
-                        a0, a1);
+              f2_unpack(f2_fma(f2_pack(__uint_as_float(r[2 * e]), __uint_as_float(r[2 * e + 1])), sl2x2, nm2), a0, a1);
               const float p0 = ex2_approx(a0), p1 = ex2_approx(a1);
-              pk[c] = pack2<T>(p0, p1);
-              ls[c & 1] = f2_add(ls[c & 1], f2_pack(p0, p1));
+              pk[e] = pack2<T>(p0, p1);
+              ls[e & 1] = f2_add(ls[e & 1], f2_pack(p0, p1));
             }
-            tmem_st16(t_s + 16 * q, pk);
-          }
+            tmem_st16(t_s + h * kHalf + col, pk);
+          };
+          expo(ra, 0);
+          expo(rb, 16);
           tmem_wait_st();
+          tc_fence_before();
           float a0, a1, b0, b1;
           f2_unpack(ls[0], a0, a1);
           f2_unpack(ls[1], b0, b1);
           l += (a0 + a1) + (b0 + b1);
-          tc_fence_before();
         }
         __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[x]);
+        if (lane == 0) mbar_arrive(&p_full[2 * x + h]);
+        ph ^= 16u;  // bit 4: parity of this step's P.V
       }
       if (!ok) break;
-      // The rows of this thread's epilogue: a pair's stream has its own tile,
-      // all dims; in a single the two warpgroups take half of the dims each
-      // of the joined streams.
-      const bool single = !pair;
-      float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
-      // everyone has read the m and l of the segment before
-      if (nseg > 0) ok = __all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err));
+      ok = __all_sync(0xffffffffu, finish_rows<T, KD>(p, seg, x, t_s, m, l, any_row, nseg, &ph, ml, o_empty, misc));
       if (!ok) break;
-      if (single && m_tiles > 0) {
-        ml[x * kM + row] = make_float2(m, l);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(ml_full);
-        ok = __all_sync(0xffffffffu, wait_or_abort(ml_full, nb & 1u, misc, p.err) &&
-                                         wait_or_abort(o_both, nb & 1u, misc, p.err));
-        if (!ok) break;
-        ++nb;
-        const float2 other = ml[(x ^ 1) * kM + row];
-        const float mm = fmaxf(m, other.x);
-        const float base = mm == -INFINITY ? 0.f : mm;
-        const float wo = exp2f(m - base), wt = exp2f(other.x - base);
-        wa = x ? wt : wo;
-        wb = x ? wo : wt;
-        l = l * wo + other.y * wt;
-        m = mm;
-      } else if (n > 0) {
-        ok = __all_sync(0xffffffffu, wait_or_abort(&o_full[x], no & 1u, misc, p.err));
-        if (!ok) break;
-        ++no;
-      }
-      tc_fence_after();
-      const int64_t tok = qst + qi;
-      const int h = kh * p.G + hg;
-      const bool have_b = single && m_tiles > 1;
-      const bool have = single ? m_tiles > 0 : n > 0;
-      const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
-      wa *= inv;
-      wb *= inv;
-      const int item_row = (pair ? x * p.tq * p.G : 0) + row;
-      if (row_ok && (!single || x == 0)) {
-        if (slot >= 0) {
-          reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
-        } else if (p.lse != nullptr) {
-          p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-        }
-      }
-      __syncwarp();
-      const int c_lo = single ? x * (KD / 32) : 0, c_hi = single ? c_lo + KD / 32 : KD / 16;  // 16 dims each
-      if (any_row) {
-#pragma unroll 1
-        for (int c = c_lo; c < c_hi; ++c) {
-          if (16 * c >= p.D) break;
-          uint32_t oa[16], ob[16];
-          float f[16];
-          if (have) tmem_ld16_nowait(t_o + (single ? 0 : x * kM) + 16 * c, oa);
-          if (have_b) tmem_ld16_nowait(t_o + kM + 16 * c, ob);
-          tmem_wait_ld();
-#pragma unroll
-          for (int e = 0; e < 16; ++e) {
-            f[e] = have ? __uint_as_float(oa[e]) * wa : 0.f;
-            if (have_b) f[e] = fmaf(__uint_as_float(ob[e]), wb, f[e]);
-          }
-          if (row_ok && slot >= 0) {
-            float* po = p.part_o + ((int64_t)slot * kItemRows + item_row) * p.D + 16 * c;
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-              if (16 * c + e < p.D) *reinterpret_cast<float4*>(po + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-          } else if (row_ok) {
-            unsigned char* po = p.out + tok * p.o_st + h * p.o_sh + 32 * c;
-#pragma unroll
-            for (int e = 0; e < 16; e += 8)
-              if (16 * c + e < p.D)
-                *reinterpret_cast<uint4*>(po + 2 * e) =
-                    make_uint4(pack2<T>(f[e], f[e + 1]), pack2<T>(f[e + 2], f[e + 3]), pack2<T>(f[e + 4], f[e + 5]),
-                               pack2<T>(f[e + 6], f[e + 7]));
-          }
-          __syncwarp();  // the TMEM loads are the whole warp's
-        }
-      }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(o_empty);
+      if (lane == 0) {
+        mbar_arrive(o_empty);
+        mbar_arrive(&seg_empty[ss]);
+      }
     }
     if (!ok) misc[0] = 1;
   }
@@ -747,7 +801,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kWarpMma)
+  if (warp == kWarpMmaA)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
 }
 

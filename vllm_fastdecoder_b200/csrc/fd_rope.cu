@@ -5,11 +5,11 @@
 //
 // One pass over q, k and v: three flops per element, so bytes bound it (HBM
 // for prompts, launch and three dependent loads for a decode step).  A CTA
-// takes kTok tokens: it gathers their cos / sin rows once into shared memory
+// takes up to kMaxTok tokens: it gathers their cos / sin rows once into shared memory
 // (every head of a token turns by the same angles, each axis by its own row
-// of the table) and then walks the tokens' vectors: a "unit" is two vectors
-// of VE elements that hold VE whole pairs (one of either half, or two
-// neighbours), the dims behind rot_dim and v are plain vectors.  A thread
+// of the table) and then walks the tokens' vectors: two vectors of VE elements
+// that hold VE whole pairs (one of either half, or two neighbours) of every
+// head, then plain vectors of v and of the dims behind rot_dim.  A thread
 // loads kBatch of them before it stores the first, so enough loads are in
 // flight and q_out = q (in place) stays safe: every element is read and
 // written by one thread, in that order.
@@ -36,7 +36,6 @@ struct RopeParams {
   int64_t split;
   int T, H, KVH, D, rot, BS;
   int pairs;    // 1: neighbouring dims form a pair
-  int rot_heads;  // units of the rotated part per token: (H + KVH) * upr
   int upr;      // units per head: rot / 2 / VE
   int rest;     // vectors per head behind rot_dim: (D - rot) / VE
   int vch;      // vectors per head of v: D / VE (0: no KV write)
@@ -45,6 +44,8 @@ struct RopeParams {
   int32_t* err;
 };
 
+constexpr int kThreads = 256;
+constexpr int kCtasPerSm = 4;
 constexpr int kBatch = 4;
 constexpr int kMaxTok = 8;
 
@@ -72,26 +73,28 @@ __device__ __forceinline__ float to_f(__nv_bfloat16 x) { return __bfloat162float
 __device__ __forceinline__ float to_f(float x) { return x; }
 
 template <typename T, int VE>
-__global__ void __launch_bounds__(256) fd_rope_kernel(const __grid_constant__ RopeParams p) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) fd_rope_kernel(const __grid_constant__ RopeParams p) {
   typedef typename VecOf<VE * sizeof(T)>::type V;
   union Vec {
     V v;
     T e[VE];
   };
+  constexpr int VB = VE * (int)sizeof(T);
   extern __shared__ float cs[];  // [tok][rot]: cos of the pairs, then sin
-  __shared__ int64_t k_at[kMaxTok];   // byte offset of the token's K/V row in its tier, -1: none
+  __shared__ int64_t k_at[kMaxTok];  // byte offset of the token's K/V row in its tier, -1: none
   __shared__ int tier_of[kMaxTok];
   __shared__ int live[kMaxTok];
+  const int tid = threadIdx.x;
   const int t0 = blockIdx.x * p.tok;
   const int nt = min(p.tok, p.T - t0);
   const int half = p.rot / 2;
 
-  for (int x = threadIdx.x; x < nt; x += blockDim.x) {
-    live[x] = 1;
+  if (tid < nt) {
+    live[tid] = 1;
     int64_t at = -1;
     int tr = 0;
     if (p.slots != nullptr) {
-      const int64_t s = p.slots[t0 + x];
+      const int64_t s = p.slots[t0 + tid];
       if (s >= 0) {
         int64_t b = s / p.BS;
         const int64_t off = s - b * p.BS;
@@ -105,11 +108,11 @@ __global__ void __launch_bounds__(256) fd_rope_kernel(const __grid_constant__ Ro
           set_error(p.err, FD_DEVERR_SLOT);
       }
     }
-    k_at[x] = at;
-    tier_of[x] = tr;
+    k_at[tid] = at;
+    tier_of[tid] = tr;
   }
   __syncthreads();
-  for (int x = threadIdx.x; x < nt * half; x += blockDim.x) {
+  for (int x = tid; x < nt * half; x += kThreads) {
     const int t = x / half, i = x - t * half;
     const int64_t pos = p.pos[(int64_t)p.axis[i] * p.pos_stride + t0 + t];
     if (pos < 0 || pos >= p.max_pos) {
@@ -120,73 +123,76 @@ __global__ void __launch_bounds__(256) fd_rope_kernel(const __grid_constant__ Ro
       cs[t * p.rot + half + i] = p.cs[pos * p.rot + half + i];
     }
   }
-  __syncthreads();
 
-  const int heads = p.H + p.KVH;
-  const int n_rest = heads * p.rest;
-  const int per_tok = p.rot_heads + n_rest + p.KVH * p.vch;
-  const int total = nt * per_tok;
-  constexpr int VB = VE * (int)sizeof(T);
-  for (int base = threadIdx.x; base < total; base += blockDim.x * kBatch) {
-    Vec a[kBatch], b[kBatch];
-    int tok[kBatch], pair0[kBatch];              // pair0 < 0: a plain copy
-    unsigned char *d1[kBatch], *d2[kBatch];      // destinations of the first vector (second one: + gap)
-    int gap[kBatch];
+  // v: its first loads are under way while the angles arrive
+  const int v_lane = p.vch > 0 ? tid % p.vch : 0, v_row = p.vch > 0 ? tid / p.vch : 0;
+  const int v_step = p.vch > 0 ? kThreads / p.vch : 1;
+  const int v_rows = p.vch > 0 && v_row < v_step ? nt * p.KVH : 0;
+  for (int f0 = v_row;; f0 += v_step * kBatch) {
+    const bool first = f0 == v_row;
+    if (f0 >= v_rows && !first) break;
+    V a[kBatch];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const int x = base + u * blockDim.x;
-      tok[u] = -1;
-      d1[u] = d2[u] = nullptr;
-      pair0[u] = -1;
-      gap[u] = 0;
-      if (x >= total) continue;
-      const int t = x / per_tok;
-      int rem = x - t * per_tok;
-      if (!live[t]) continue;
-      tok[u] = t;
-      const int64_t tt = t0 + t, at = k_at[t];
-      const int tr = tier_of[t];
-      if (rem >= p.rot_heads + n_rest) {  // v
-        rem -= p.rot_heads + n_rest;
-        const int h = rem / p.vch, c = rem - h * p.vch;
-        if (at < 0) continue;
-        a[u].v = *reinterpret_cast<const V*>(p.v + tt * p.v_st + h * p.v_sh + c * VB);
-        d1[u] = p.tv[tr] + at + h * p.head_sb[tr] + c * VB;
-        continue;
-      }
-      int h, off;
-      if (rem < p.rot_heads) {
-        h = rem / p.upr;
-        const int c = rem - h * p.upr;
-        pair0[u] = c * VE;
-        off = p.pairs ? 2 * c * VB : c * VB;
-        gap[u] = p.pairs ? VB : half * (int)sizeof(T);
-      } else {
-        rem -= p.rot_heads;
-        h = rem / p.rest;
-        off = p.rot * (int)sizeof(T) + (rem - h * p.rest) * VB;
-      }
-      const unsigned char* src;
-      if (h < p.H) {
-        src = p.q + tt * p.q_st + h * p.q_sh + off;
-        d1[u] = p.q_out + tt * p.qo_st + h * p.qo_sh + off;
-      } else {
-        h -= p.H;
-        src = p.k + tt * p.k_st + h * p.k_sh + off;
-        if (at >= 0) d1[u] = p.tk[tr] + at + h * p.head_sb[tr] + off;
-        if (p.k_out != nullptr) d2[u] = p.k_out + tt * p.ko_st + h * p.ko_sh + off;
-      }
-      a[u].v = *reinterpret_cast<const V*>(src);
-      if (pair0[u] >= 0) b[u].v = *reinterpret_cast<const V*>(src + gap[u]);
+      const int f = f0 + u * v_step;
+      if (f >= v_rows) continue;
+      const int t = f / p.KVH, h = f - t * p.KVH;
+      a[u] = *reinterpret_cast<const V*>(p.v + (int64_t)(t0 + t) * p.v_st + h * p.v_sh + v_lane * VB);
     }
+    if (first) __syncthreads();  // angles, slots and live tokens (every thread comes here once)
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      if (tok[u] < 0) continue;
-      if (pair0[u] >= 0) {
-        const float* c = cs + tok[u] * p.rot + pair0[u];
+      const int f = f0 + u * v_step;
+      if (f >= v_rows) continue;
+      const int t = f / p.KVH, h = f - t * p.KVH;
+      const int tr = tier_of[t];
+      if (live[t] && k_at[t] >= 0)
+        *reinterpret_cast<V*>(p.tv[tr] + k_at[t] + h * p.head_sb[tr] + v_lane * VB) = a[u];
+    }
+  }
+
+  // Where vector `off` of head h (q's, then k's) of token t is read.
+  auto source = [&](int t, int h, int off) -> const unsigned char* {
+    return h < p.H ? p.q + (int64_t)(t0 + t) * p.q_st + h * p.q_sh + off
+                   : p.k + (int64_t)(t0 + t) * p.k_st + (h - p.H) * p.k_sh + off;
+  };
+  // The destinations of it: q_out, or the cache row and k_out.
+  auto put = [&](int t, int h, int off, const V& x) {
+    if (h < p.H) {
+      *reinterpret_cast<V*>(p.q_out + (int64_t)(t0 + t) * p.qo_st + h * p.qo_sh + off) = x;
+      return;
+    }
+    const int kh = h - p.H, tr = tier_of[t];
+    if (k_at[t] >= 0) *reinterpret_cast<V*>(p.tk[tr] + k_at[t] + kh * p.head_sb[tr] + off) = x;
+    if (p.k_out != nullptr)
+      *reinterpret_cast<V*>(p.k_out + (int64_t)(t0 + t) * p.ko_st + kh * p.ko_sh + off) = x;
+  };
+  const int heads = p.H + p.KVH, rows = nt * heads;
+
+  // the rotated dims: thread `lane` of a head's upr takes pairs lane * VE ..
+  {
+    const int lane = tid % p.upr, row = tid / p.upr, step = kThreads / p.upr;
+    const int off = (p.pairs ? 2 * lane : lane) * VB, gap = p.pairs ? VB : half * (int)sizeof(T);
+    for (int f0 = row; row < step && f0 < rows; f0 += step * kBatch) {
+      Vec a[kBatch], b[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int f = f0 + u * step;
+        if (f >= rows) continue;
+        const int t = f / heads, h = f - t * heads;
+        const unsigned char* src = source(t, h, off);
+        a[u].v = *reinterpret_cast<const V*>(src);
+        b[u].v = *reinterpret_cast<const V*>(src + gap);
+      }
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int f = f0 + u * step;
+        if (f >= rows) continue;
+        const int t = f / heads, h = f - t * heads;
+        if (!live[t]) continue;
+        const float* c = cs + t * p.rot + lane * VE;
         Vec ra, rb;
-        if (p.pairs) {
-          // the two vectors hold pairs (2 i, 2 i + 1) in turn
+        if (p.pairs) {  // the two vectors hold pairs (2 i, 2 i + 1) in turn
           T in[2 * VE], out[2 * VE];
 #pragma unroll
           for (int e = 0; e < VE; ++e) {
@@ -212,17 +218,19 @@ __global__ void __launch_bounds__(256) fd_rope_kernel(const __grid_constant__ Ro
             rb.e[e] = Dt<T>::narrow(x2 * c[e] + x1 * c[half + e]);
           }
         }
-        a[u] = ra;
-        b[u] = rb;
+        put(t, h, off, ra.v);
+        put(t, h, off + gap, rb.v);
       }
-      if (d1[u] != nullptr) {
-        *reinterpret_cast<V*>(d1[u]) = a[u].v;
-        if (pair0[u] >= 0) *reinterpret_cast<V*>(d1[u] + gap[u]) = b[u].v;
-      }
-      if (d2[u] != nullptr) {
-        *reinterpret_cast<V*>(d2[u]) = a[u].v;
-        if (pair0[u] >= 0) *reinterpret_cast<V*>(d2[u] + gap[u]) = b[u].v;
-      }
+    }
+  }
+
+  // the dims behind rot_dim
+  if (p.rest > 0) {
+    for (int x = tid; x < rows * p.rest; x += kThreads) {
+      const int f = x / p.rest, t = f / heads, h = f - t * heads;
+      if (!live[t]) continue;
+      const int off = p.rot * (int)sizeof(T) + (x - f * p.rest) * VB;
+      put(t, h, off, *reinterpret_cast<const V*>(source(t, h, off)));
     }
   }
 }
@@ -231,7 +239,6 @@ template <typename T, int VE>
 int launch(RopeParams& p, cudaStream_t s) {
   p.upr = p.rot / 2 / VE;
   p.rest = (p.D - p.rot) / VE;
-  p.rot_heads = (p.H + p.KVH) * p.upr;
   p.vch = p.slots != nullptr ? p.D / VE : 0;
   int dev = 0, sms = 0;
   const int st = fdh::device_sms(&dev, &sms);
@@ -242,7 +249,7 @@ int launch(RopeParams& p, cudaStream_t s) {
   p.tok = 1;
   while (p.tok < kMaxTok && (int64_t)p.T > (int64_t)p.tok * sms * 8) p.tok *= 2;
   const unsigned grid = (unsigned)((p.T + p.tok - 1) / p.tok);
-  fd_rope_kernel<T, VE><<<grid, 256, (size_t)p.tok * p.rot * 4, s>>>(p);
+  fd_rope_kernel<T, VE><<<grid, kThreads, (size_t)p.tok * p.rot * 4, s>>>(p);
   return fdh::cuda_status(cudaGetLastError(), "fd_rope_kernel launch");
 }
 

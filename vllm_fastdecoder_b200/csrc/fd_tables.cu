@@ -28,6 +28,11 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 1024;
 constexpr int kWarps = kThreads / 32;
 constexpr int kCluster = 8;
+constexpr int kBatch = 8;  // rows of 32 block ids that a warp has in flight
+constexpr int kShare = 8;   // warps that share 32 requests' ended ones
+constexpr int kFew = 4;     // new tokens that one thread places
+constexpr int kChunk = 256; // tokens per warp otherwise,
+constexpr int kTok = 4;     // and a lane's tokens in flight
 // Calls of at most this many tokens and requests run on one CTA: its 1024
 // threads place them in two passes, and the cluster's barriers cost more than
 // the other CTAs save.
@@ -48,15 +53,18 @@ __device__ __forceinline__ Sum4 add(const Sum4& a, const Sum4& b) {
   return {a.tok + b.tok, a.need + b.need, a.f0 + b.f0, a.f1 + b.f1};
 }
 
-__device__ __forceinline__ Sum4 shfl_up(const Sum4& a, int off) {
-  return {__shfl_up_sync(0xffffffffu, a.tok, off), __shfl_up_sync(0xffffffffu, a.need, off),
-          __shfl_up_sync(0xffffffffu, a.f0, off), __shfl_up_sync(0xffffffffu, a.f1, off)};
+__device__ __forceinline__ Sum4 shfl_up(const Sum4& a, int off, bool freed) {
+  Sum4 r = {__shfl_up_sync(0xffffffffu, a.tok, off), __shfl_up_sync(0xffffffffu, a.need, off), 0, 0};
+  if (freed) {
+    r.f0 = __shfl_up_sync(0xffffffffu, a.f0, off);
+    r.f1 = __shfl_up_sync(0xffffffffu, a.f1, off);
+  }
+  return r;
 }
 
-// The request that owns entry x of a running sum: the last r with sum[r] <= x
-// (sum[R] > x).
-__device__ __forceinline__ int owner(const int* sum, int R, int x) {
-  int lo = 0, hi = R;  // sum[lo] <= x < sum[hi]
+// The request that owns entry x of a running sum: the last r in [lo, hi) with
+// sum[r] <= x, given sum[lo] <= x < sum[hi].
+__device__ __forceinline__ int owner(const int* sum, int lo, int hi, int x) {
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
     if (sum[mid] <= x)
@@ -67,16 +75,29 @@ __device__ __forceinline__ int owner(const int* sum, int R, int x) {
   return lo;
 }
 
-__device__ __forceinline__ int ceil_div(long long a, int b) { return (int)((a + b - 1) / b); }
+// Lengths (at most bt_width * block_size, an int32) in blocks; block sizes
+// are powers of two as a rule, and a shift is a twentieth of a division.
+template <bool kPow2>
+struct Blocks {
+  int bs, sh;
+  __device__ __forceinline__ explicit Blocks(int block_size) : bs(block_size), sh(0) {
+    while ((2 << sh) <= bs && sh < 29) ++sh;
+  }
+  __device__ __forceinline__ int of(int pos) const { return kPow2 ? pos >> sh : (int)((unsigned)pos / (unsigned)bs); }
+  __device__ __forceinline__ int hold(int len) const { return len > 0 ? of(len - 1) + 1 : 0; }
+};
 
+template <bool kPow2>
 __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_constant__ fd_tables_args a) {
   extern __shared__ int sm[];
   __shared__ Sum4 warp_sum[kWarps];
+  __shared__ unsigned ended[FD_TABLES_MAX_REQS / 32];  // bit i of word w: request 32 w + i ends
   __shared__ int shared_flags;
   __shared__ int shared_max[2];
   cg::cluster_group cluster = cg::this_cluster();
   const int nct = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int R = a.num_reqs, BS = a.block_size, W = a.bt_width;
+  const Blocks<kPow2> blocks(BS);
   int* s_new = sm;
   int* s_prior = s_new + R;
   int* s_tok = s_prior + R;
@@ -90,34 +111,60 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
     shared_max[0] = shared_max[1] = 0;
   }
   bool ends = false;
-  for (int r = tid; r < R; r += kThreads) {
-    s_new[r] = a.new_lens[r];
-    s_prior[r] = a.prior_lens[r];
-    s_f0[r] = s_f1[r] = 0;
-    ends |= s_new[r] == -1;
+  for (int base = 0; base < R; base += kThreads) {
+    const int r = base + tid;
+    bool e = false;
+    if (r < R) {
+      const int nw = a.new_lens[r];
+      s_new[r] = nw;
+      s_prior[r] = a.prior_lens[r];
+      s_f0[r] = s_f1[r] = 0;
+      e = nw == -1;
+    }
+    const unsigned word = __ballot_sync(0xffffffffu, e);
+    if (lane == 0 && r < R) ended[r >> 5] = word;
+    ends |= e;
   }
   const int c0_in = a.counts_in[0], c1_in = a.counts_in[1];
   // the same in every CTA of the cluster: all of them read all lengths
   const bool any_end = __syncthreads_or(ends ? 1 : 0) != 0;
 
-  // blocks of ended requests by tier: one warp per request, requests dealt
-  // out over the CTAs, the counts sent to all of them
+  // A warp per ended request: the set bits of a word of `ended` are dealt out
+  // over kShare warps, those over all CTAs.
+  auto for_ended = [&](auto&& body) {
+    const int units = (R + 31) / 32 * kShare;
+    for (int x = rank + nct * warp; x < units; x += nct * kWarps) {
+      unsigned w = ended[x / kShare];
+      for (int i = 0; w != 0u; ++i, w &= w - 1u)
+        if (i % kShare == x % kShare) body(x / kShare * 32 + __ffs(w) - 1);
+    }
+  };
+
+  // their blocks by tier, the counts sent to every CTA
   int flags = 0;
   if (any_end) {
     if (nct > 1) cluster.sync();  // every CTA's zeros are in place before counts arrive
-    for (int r = rank + nct * warp; r < R; r += nct * kWarps) {
-      if (s_new[r] != -1) continue;
+    for_ended([&](int r) {
       const int prior = s_prior[r];
-      if (prior < 0 || (long long)prior > (long long)W * BS) continue;  // flagged below
-      const int held = ceil_div(prior, BS);
+      if (prior < 0 || (long long)prior > (long long)W * BS) return;  // flagged below
+      const int held = blocks.hold(prior);
       int n0 = 0, n1 = 0;
-      for (int c = lane; c < held; c += 32) {
-        const long long id = a.block_table[(int64_t)r * a.bt_stride + c];
-        if (id < 0 || id >= a.num_gpu_blocks + a.num_cpu_blocks) flags |= FD_TABLES_BAD_BLOCK;
-        if (id < a.num_gpu_blocks)
-          ++n0;
-        else
-          ++n1;
+      for (int base = 0; base < held; base += 32 * kBatch) {
+        int id[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int c = base + 32 * u + lane;
+          id[u] = c < held ? a.block_table[(int64_t)r * a.bt_stride + c] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          if (base + 32 * u + lane >= held) continue;
+          if (id[u] < 0 || id[u] >= a.num_gpu_blocks + a.num_cpu_blocks) flags |= FD_TABLES_BAD_BLOCK;
+          if (id[u] < a.num_gpu_blocks)
+            ++n0;
+          else
+            ++n1;
+        }
       }
       n0 = __reduce_add_sync(0xffffffffu, n0);
       n1 = __reduce_add_sync(0xffffffffu, n1);
@@ -125,8 +172,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
         cluster.map_shared_rank(s_f0, lane)[r] = n0;
         cluster.map_shared_rank(s_f1, lane)[r] = n1;
       }
-    }
-    if (flags != 0 && lane < 32)
+    });
+    if (flags != 0)
       for (int c = 0; c < nct; ++c) atomicOr(cluster.map_shared_rank(&shared_flags, c), flags);
     if (nct > 1)
       cluster.sync();
@@ -156,14 +203,14 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
       continue;
     }
     mine.tok += nw;
-    mine.need += ceil_div(seq, BS) - ceil_div(prior, BS);
+    mine.need += blocks.hold((int)seq) - blocks.hold(prior);
     max_seq = max(max_seq, (int)seq);
     max_new = max(max_new, nw);
   }
   Sum4 v = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const Sum4 u = shfl_up(v, off);
+    const Sum4 u = shfl_up(v, off, any_end);
     if (lane >= off) v = add(v, u);
   }
   if (lane == 31) warp_sum[warp] = v;
@@ -176,12 +223,18 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
     atomicMax(&shared_max[1], max_new);
   }
   __syncthreads();
-  Sum4 before = {0, 0, 0, 0}, total = {0, 0, 0, 0};
-#pragma unroll 4
-  for (int w = 0; w < kWarps; ++w) {
-    if (w == warp) before = total;
-    total = add(total, warp_sum[w]);
+  if (warp == 0) {  // running sums of the warps
+    Sum4 w = warp_sum[lane];
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const Sum4 u = shfl_up(w, off, any_end);
+      if (lane >= off) w = add(w, u);
+    }
+    warp_sum[lane] = w;
   }
+  __syncthreads();
+  const Sum4 zero = {0, 0, 0, 0};
+  const Sum4 before = warp > 0 ? warp_sum[warp - 1] : zero, total = warp_sum[kWarps - 1];
   flags = shared_flags;
   Sum4 run = add(before, {v.tok - mine.tok, v.need - mine.need, v.f0 - mine.f0, v.f1 - mine.f1});
   const long long c0 = (long long)c0_in + total.f0, c1 = (long long)c1_in + total.f1;
@@ -225,7 +278,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
     run.f1 += f1;
     if (nw >= 0) {
       run.tok += nw;
-      run.need += ceil_div((long long)prior + nw, BS) - ceil_div(prior, BS);
+      run.need += blocks.hold(prior + nw) - blocks.hold(prior);
     }
   }
   if (tid == 0) {
@@ -235,28 +288,29 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
   __syncthreads();
 
   if (any_end) {  // push, in request and table order within each tier
-    for (int r = rank + nct * warp; r < R; r += nct * kWarps) {
-      if (s_new[r] != -1) continue;
-      const int held = ceil_div(s_prior[r], BS);
+    for_ended([&](int r) {
+      const int held = blocks.hold(s_prior[r]);
       int at0 = c0_in + s_f0[r], at1 = c1_in + s_f1[r];
-      for (int base = 0; base < held; base += 32) {
-        const int c = base + lane;
-        const int id = c < held ? a.block_table[(int64_t)r * a.bt_stride + c] : 0;
-        const bool hbm = id < a.num_gpu_blocks;
-        const unsigned in0 = __ballot_sync(0xffffffffu, c < held && hbm);
-        const unsigned in1 = __ballot_sync(0xffffffffu, c < held && !hbm);
-        const unsigned below = (1u << lane) - 1u;
-        if (c < held) {
-          if (hbm)
-            a.free_ids[0][at0 + __popc(in0 & below)] = id;
-          else
-            a.free_ids[1][at1 + __popc(in1 & below)] = id;
+      const unsigned below = (1u << lane) - 1u;
+      for (int base = 0; base < held; base += 32 * kBatch) {
+        int id[kBatch];
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const int c = base + 32 * u + lane;
+          id[u] = c < held ? a.block_table[(int64_t)r * a.bt_stride + c] : 0;
         }
-        at0 += __popc(in0);
-        at1 += __popc(in1);
+#pragma unroll
+        for (int u = 0; u < kBatch; ++u) {
+          const bool in = base + 32 * u + lane < held, hbm = id[u] < a.num_gpu_blocks;
+          const unsigned in0 = __ballot_sync(0xffffffffu, in && hbm), in1 = __ballot_sync(0xffffffffu, in && !hbm);
+          if (in && hbm) a.free_ids[0][at0 + __popc(in0 & below)] = id[u];
+          if (in && !hbm) a.free_ids[1][at1 + __popc(in1 & below)] = id[u];
+          at0 += __popc(in0);
+          at1 += __popc(in1);
+        }
       }
-    }
-    __threadfence();
+    });
+    // the barriers order the pushes before the pops at their scope
     if (nct > 1)
       cluster.sync();
     else
@@ -272,24 +326,55 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
     a.query_start_loc[r] = s_tok[r];
   }
   for (int j = gt; j < need; j += step) {
-    const int r = owner(s_need, R, j);
-    a.block_table[(int64_t)r * a.bt_stride + ceil_div(s_prior[r], BS) + (j - s_need[r])] = pop(j);
+    const int r = owner(s_need, 0, R, j);
+    a.block_table[(int64_t)r * a.bt_stride + blocks.hold(s_prior[r]) + (j - s_need[r])] = pop(j);
   }
-  int r = 0;
+  // Tokens.  Requests of at most kFew new ones: a thread each, no search.
   const int ntok = (int)total.tok;
-  for (int t = gt; t < a.max_tokens; t += step) {
-    long long slot = -1, pos = 0;
-    if (t < ntok) {
-      if (t >= s_tok[r + 1] || t < s_tok[r]) r = owner(s_tok, R, t);
-      const int prior = s_prior[r];
-      const int at = prior + (t - s_tok[r]);
-      const int held = ceil_div(prior, BS), b = at / BS;
-      const int id = b < held ? a.block_table[(int64_t)r * a.bt_stride + b] : pop(s_need[r] + b - held);
-      slot = (long long)id * BS + (at - b * BS);
-      pos = at;
+  auto block_at = [&](int at, int r, int held, int first_need) {
+    const int b = blocks.of(at);
+    return b < held ? a.block_table[(int64_t)r * a.bt_stride + b] : pop(first_need + b - held);
+  };
+  auto put = [&](int t, int at, int id) {
+    a.slot_mapping[t] = (long long)id * BS + (at - blocks.of(at) * BS);
+    a.positions[t] = at;
+  };
+  for (int r = gt; r < R; r += step) {
+    const int nw = s_new[r];
+    if (nw <= 0 || nw > kFew) continue;
+    const int prior = s_prior[r];
+    for (int i = 0; i < nw; ++i)
+      put(s_tok[r] + i, prior + i, block_at(prior + i, r, blocks.hold(prior), s_need[r]));
+  }
+  // The others: a warp per kChunk neighbouring tokens walks the requests that
+  // they belong to, 32 lengths at a time, and places a request's tokens
+  // together.
+  if (shared_max[1] > kFew) {
+    for (int t0 = (rank * kWarps + warp) * kChunk; t0 < ntok; t0 += nct * kWarps * kChunk) {
+      const int t1 = min(t0 + kChunk, ntok);
+      for (int r0 = owner(s_tok, 0, R, t0); r0 < R && s_tok[r0] < t1; r0 += 32) {
+        const int mine = r0 + lane;
+        unsigned large = __ballot_sync(0xffffffffu, mine < R && s_tok[min(mine, R)] < t1 && s_new[min(mine, R - 1)] > kFew);
+        for (; large != 0u; large &= large - 1u) {
+          const int r = r0 + __ffs(large) - 1;
+          const int from = s_tok[r], prior = s_prior[r], held = blocks.hold(prior), need0 = s_need[r];
+          const int lo = max(t0, from), hi = min(t1, from + s_new[r]);
+          for (int t = lo + lane; t < hi; t += 32 * kTok) {
+            int id[kTok];
+#pragma unroll
+            for (int u = 0; u < kTok; ++u)
+              id[u] = t + 32 * u < hi ? block_at(prior + (t + 32 * u - from), r, held, need0) : 0;
+#pragma unroll
+            for (int u = 0; u < kTok; ++u)
+              if (t + 32 * u < hi) put(t + 32 * u, prior + (t + 32 * u - from), id[u]);
+          }
+        }
+      }
     }
-    a.slot_mapping[t] = slot;
-    a.positions[t] = pos;
+  }
+  for (int t = ntok + gt; t < a.max_tokens; t += step) {
+    a.slot_mapping[t] = -1;
+    a.positions[t] = 0;
   }
   if (rank == 0 && tid == 0) {
     a.query_start_loc[R] = ntok;
@@ -334,9 +419,11 @@ extern "C" int fd_extend_tables(const fd_tables_args* a, void* stream) {
   for (int t = 0; t < 2; ++t)
     if (a->free_cap[t] < 0 || (a->free_cap[t] > 0 && a->free_ids[t] == nullptr))
       return fdh::fail(FD_ERR_INVALID, "fd_extend_tables: free stack %d has a capacity but no memory", t);
-  static unsigned long long done = 0;
-  const void* kern = reinterpret_cast<const void*>(fd_tables_kernel);
-  int st = fdh::ensure_smem(kern, smem_bytes(FD_TABLES_MAX_REQS), &done);
+  const bool pow2 = (a->block_size & (a->block_size - 1)) == 0;
+  static unsigned long long done[2] = {0, 0};
+  const void* kern = pow2 ? reinterpret_cast<const void*>(fd_tables_kernel<true>)
+                          : reinterpret_cast<const void*>(fd_tables_kernel<false>);
+  int st = fdh::ensure_smem(kern, smem_bytes(FD_TABLES_MAX_REQS), &done[pow2 ? 1 : 0]);
   if (st != FD_OK) return st;
   const int ctas = a->max_tokens <= kOneCtaTokens && a->num_reqs <= kOneCtaReqs ? 1 : kCluster;
   cudaLaunchConfig_t cfg = {};

@@ -703,10 +703,12 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_le
 # ------------------------------------------------------------- multi-token steps
 #
 # These calls pack their C struct in one struct.pack (a ctypes field store each
-# would cost more than the launch), run on the device of their tensors whatever
-# the current one is, and take their workspace from torch's caching allocator
-# per call: it belongs to the current stream, and to the graph when one is
-# being captured, so calls on other streams and other graphs never share it.
+# would cost more than the launch) and read each tensor's metadata once, since a
+# decode step's call is bound by this code; they run on the device of their
+# tensors whatever the current one is, and take their workspace from torch's
+# caching allocator per call: it belongs to the current stream, and to the
+# graph when one is being captured, so calls on other streams and other graphs
+# never share it.
 
 _TIER_FMT = "PPqqqqii"
 _ATTN_STRUCT = struct.Struct("@PqqPqqPqq" + 2 * _TIER_FMT + "qPqPPPPPiiiiiiifiiiiPNP")
@@ -715,10 +717,9 @@ _TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPP")
 _NO_TIER = (0, 0, 0, 0, 0, 0, 0, 0)
 
 
-def _launch(fn, packed: bytes, device: torch.device, what: str) -> None:
-    """Call a C entry point on the current stream of `device`."""
-    idx = device.index
-    if idx != torch.cuda.current_device():
+def _launch(fn, packed: bytes, idx: int, what: str) -> None:
+    """Call a C entry point on the current stream of device `idx`."""
+    if idx != torch._C._cuda_getDevice():
         with torch.cuda.device(idx):
             status = fn(packed, torch._C._cuda_getCurrentRawStream(idx))
     else:
@@ -727,22 +728,41 @@ def _launch(fn, packed: bytes, device: torch.device, what: str) -> None:
         nat.check(status, what)
 
 
-def _tier_fields(t: KVTier | None, dev: torch.device, dtype: torch.dtype) -> tuple:
+def _error_ptr(idx: int) -> int:
+    w = _ERR.get(idx)
+    return (w if w is not None else error_word(torch.device("cuda", idx))).data_ptr()
+
+
+def _tier_fields(t: KVTier | None, idx: int, dtype: torch.dtype, shape: tuple) -> tuple:
+    """The C fields of a tier of [KVH, BS, D] = shape blocks."""
     if t is None:
         return _NO_TIER
     k, v = t.k, t.v
-    _check(k.dtype == dtype and v.dtype == dtype, "the KV tier's dtype differs")
+    if k.dtype is not dtype:
+        raise RuntimeError("the KV tier's dtype differs")
+    B, *rest = k.shape
+    if tuple(rest) != shape:
+        raise RuntimeError("the KV tiers must be [blocks, KVH, block_size, D] alike")
     s = k.stride()
-    if k.device.type == "cpu":
-        return (host_device_pointer(k), host_device_pointer(v), s[0], s[1], s[2], k.shape[0], 1, 0)
-    _check(k.device == dev and v.device == dev, "a device tier must live on the tensors' device")
-    return (k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], k.shape[0], 0, 0)
+    if k.get_device() == idx and v.get_device() == idx:
+        return (k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], B, 0, 0)
+    if k.is_cuda or v.is_cuda:
+        raise RuntimeError("a device tier must live on the tensors' device")
+    return (host_device_pointer(k), host_device_pointer(v), s[0], s[1], s[2], B, 1, 0)
 
 
-def _need_i32(t: torch.Tensor, dev: torch.device, n: int, name: str) -> int:
-    _check(t.dtype == torch.int32 and t.device == dev and t.dim() == 1 and t.shape[0] >= n and (n < 2 or t.stride(0) == 1),
-           f"{name} must be a contiguous int32 tensor of at least {n} entries on the call's device")
+def _i32(t: torch.Tensor, idx: int, n: int, name: str) -> int:
+    if t.dtype is not torch.int32 or t.get_device() != idx or t.numel() < n or not t.is_contiguous():
+        raise RuntimeError(f"{name} must be a contiguous int32 tensor of at least {n} entries on the call's device")
     return t.data_ptr()
+
+
+def _rows3(t: torch.Tensor, idx: int, dtype: torch.dtype, name: str) -> tuple:
+    """(pointer, stride 0, stride 1) of a [*, *, D] tensor with contiguous rows."""
+    s0, s1, s2 = t.stride()
+    if s2 != 1 or t.dtype is not dtype or t.get_device() != idx:
+        raise RuntimeError(f"{name} must share q's dtype and device and have a contiguous head dim")
+    return t.data_ptr(), s0, s1
 
 
 @dataclass
@@ -796,29 +816,29 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
     query_start_loc and slot_mapping are what plan.plan_on_device takes.  A
     step that cannot be applied as a whole changes nothing and sets
     the error word (check_device_errors; StepTables.read_header says why)."""
-    dev = block_table.device
-    _check(dev.type == "cuda", "block_table must be a CUDA tensor")
-    _check(block_table.dtype == torch.int32 and block_table.dim() == 2 and (block_table.shape[1] == 1
-                                                                            or block_table.stride(1) == 1),
-           "block_table must be int32 [R, W] with contiguous rows")
+    idx = block_table.get_device()
+    if idx < 0:
+        raise RuntimeError("block_table must be a CUDA tensor")
+    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or (block_table.stride(1) != 1
+                                                                          and block_table.shape[1] != 1):
+        raise RuntimeError("block_table must be int32 [R, W] with contiguous rows")
     R, W = block_table.shape
     if out is None:
         _check(max_tokens is not None, "give out or max_tokens")
-        out = StepTables(R, max_tokens, dev)
+        out = StepTables(R, max_tokens, block_table.device)
     T = out.T if max_tokens is None else int(max_tokens)
-    _check(out.R >= R and out.T >= T, "out is too small for the step")
-    _check(out.query_start_loc.device == dev, "out must be on block_table's device")
-    stacks = [(0, 0) if t is None else (_need_i32(t, dev, 0, "a free stack"), t.shape[0]) for t in (free.hbm, free.host)]
-    for t in (free.hbm, free.host):
-        _check(t is None or t.shape[0] < 2 or t.stride(0) == 1, "a free stack must be contiguous")
+    if out.R < R or out.T < T or out.header.get_device() != idx:
+        raise RuntimeError("out is too small for the step, or on another device")
+    hbm, host, counts = free.hbm, free.host, free.counts
     packed = _TABLES_STRUCT.pack(
-        _need_i32(new_lens, dev, R, "new_lens"), _need_i32(prior_lens, dev, R, "prior_lens"), block_table.data_ptr(),
-        max(W, block_table.stride(0)), W, R, stacks[0][0], stacks[1][0], stacks[0][1], stacks[1][1],
-        _need_i32(free.counts, dev, 2, "free.counts"), _need_i32(out.counts, dev, 2, "out.counts"),
-        int(num_gpu_blocks), int(num_cpu_blocks), int(block_size), T, _need_i32(out.seq_lens, dev, R, "out.seq_lens"),
+        _i32(new_lens, idx, R, "new_lens"), _i32(prior_lens, idx, R, "prior_lens"), block_table.data_ptr(),
+        max(W, block_table.stride(0)), W, R, 0 if hbm is None else _i32(hbm, idx, 0, "free.hbm"),
+        0 if host is None else _i32(host, idx, 0, "free.host"), 0 if hbm is None else hbm.numel(),
+        0 if host is None else host.numel(), _i32(counts, idx, 2, "free.counts"), _i32(out.counts, idx, 2, "out.counts"),
+        num_gpu_blocks, num_cpu_blocks, block_size, T, _i32(out.seq_lens, idx, R, "out.seq_lens"),
         out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.header.data_ptr(),
-        error_word(dev).data_ptr())
-    _launch(nat.load().fd_extend_tables, packed, dev, "fd_extend_tables")
+        _error_ptr(idx))
+    _launch(nat.load().fd_extend_tables, packed, idx, "fd_extend_tables")
     return out
 
 
@@ -854,48 +874,49 @@ def rope_store_kv(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     with pairs.  The rotated q goes to q_out (default: q itself), which is
     returned; k_out takes a copy of the rotated k, e.g. for prefill_attn over
     a fresh prompt's own rows."""
-    dev, dt = q.device, q.dtype
-    _check(dev.type == "cuda", "q must be a CUDA tensor")
-    _check(q.dim() == 3 and k.dim() == 3 and v.shape == k.shape and k.shape[0] == q.shape[0]
-           and k.shape[2] == q.shape[2], "q must be [T, H, D], k and v [T, KVH, D]")
-    T, H, D = q.shape
+    idx, dt = q.get_device(), q.dtype
+    if idx < 0:
+        raise RuntimeError("q must be a CUDA tensor")
+    if q.dim() != 3 or k.dim() != 3:
+        raise RuntimeError("q must be [T, H, D], k and v [T, KVH, D]")
+    T, H, D = shape = q.shape
     KVH = k.shape[1]
+    if k.shape != (T, KVH, D) or v.shape != k.shape:
+        raise RuntimeError("q must be [T, H, D], k and v [T, KVH, D]")
     q_out = q if q_out is None else q_out
-    _check(q_out.shape == q.shape and (k_out is None or k_out.shape == k.shape), "q_out / k_out must have q's / k's shape")
-    for t in (q, k, v, q_out) if k_out is None else (q, k, v, q_out, k_out):
-        _check(t.dtype == dt and t.device == dev and t.stride(2) == 1,
-               "q, k, v and the outputs must share dtype and device and have a contiguous head dim")
+    if q_out.shape != shape or (k_out is not None and k_out.shape != k.shape):
+        raise RuntimeError("q_out / k_out must have q's / k's shape")
     if positions.dim() == 1:
         positions = positions.unsqueeze(0)
-    A = positions.shape[0]
-    _check(positions.dtype == torch.int64 and positions.device == dev and positions.dim() == 2
-           and positions.shape[1] >= T and (T < 2 or positions.stride(1) == 1),
-           "positions must be int64 [axes, T] on q's device with contiguous rows")
-    _check(cos_sin.dtype == torch.float32 and cos_sin.device == dev and cos_sin.dim() == 2 and cos_sin.is_contiguous(),
-           "cos_sin must be contiguous fp32 [max_pos, rot_dim] on q's device")
-    rot = cos_sin.shape[1]
-    axes = rope_axes((rot // 2,) if sections is None else tuple(sections), bool(turns))
-    _check(2 * len(axes) == rot, "sections must add up to rot_dim / 2 pairs")
-    _check(A == (1 if sections is None else len(sections)), "positions must have one row per axis")
-    BS = 0
+    A = 1 if sections is None else len(sections)
+    p0, p1 = positions.stride()
+    if (positions.dtype is not torch.int64 or positions.get_device() != idx or positions.shape[1] < T
+            or (p1 != 1 and T > 1)):
+        raise RuntimeError("positions must be int64 [axes, T] on q's device with contiguous rows")
+    if positions.shape[0] != A:
+        raise RuntimeError("positions must have one row per axis")
+    if cos_sin.dtype is not torch.float32 or cos_sin.get_device() != idx or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        raise RuntimeError("cos_sin must be contiguous fp32 [max_pos, rot_dim] on q's device")
+    max_pos, rot = cos_sin.shape
+    axes = rope_axes((rot // 2,) if sections is None else tuple(sections), turns)
+    if 2 * len(axes) != rot:
+        raise RuntimeError("sections must add up to rot_dim / 2 pairs")
+    BS, slots_ptr = 0, 0
     f0 = f1 = _NO_TIER
     if slots is not None:
-        _check(slots.dtype == torch.int64 and slots.device == dev and slots.dim() == 1 and slots.shape[0] >= T
-               and (T < 2 or slots.stride(0) == 1), "slots must be contiguous int64 with T entries on q's device")
-        for t in tiers:
-            if t is not None:
-                _check(t.k.shape[1] == KVH and t.k.shape[3] == D and BS in (0, t.k.shape[2]),
-                       "the KV tiers must be [blocks, KVH, block_size, D]")
-                BS = t.k.shape[2]
-        _check(BS > 0, "at least one KV tier is required")
-        f0, f1 = _tier_fields(tiers[0], dev, dt), _tier_fields(tiers[1], dev, dt)
-    st = [x for t in (q, q_out, k, v) for x in (t.data_ptr(), t.stride(0), t.stride(1))]
-    st += (0, 0, 0) if k_out is None else (k_out.data_ptr(), k_out.stride(0), k_out.stride(1))
+        if slots.dtype is not torch.int64 or slots.get_device() != idx or slots.numel() < T or not slots.is_contiguous():
+            raise RuntimeError("slots must be contiguous int64 with T entries on q's device")
+        t0, t1 = tiers
+        if t0 is None and t1 is None:
+            raise RuntimeError("at least one KV tier is required")
+        slots_ptr, BS = slots.data_ptr(), (t0 if t0 is not None else t1).k.shape[2]
+        f0, f1 = _tier_fields(t0, idx, dt, (KVH, BS, D)), _tier_fields(t1, idx, dt, (KVH, BS, D))
     packed = _ROPE_STRUCT.pack(
-        *st, positions.data_ptr(), positions.stride(0), cos_sin.data_ptr(), cos_sin.shape[0],
-        0 if slots is None else slots.data_ptr(), *f0, *f1, int(tier_split), T, H, KVH, D, rot, BS, dtype_code(dt), A,
-        nat.ROPE_PAIRS if pairs else 0, axes, 0, error_word(dev).data_ptr())
-    _launch(nat.load().fd_rope_store_kv, packed, dev, "fd_rope_store_kv")
+        *_rows3(q, idx, dt, "q"), *_rows3(q_out, idx, dt, "q_out"), *_rows3(k, idx, dt, "k"), *_rows3(v, idx, dt, "v"),
+        *((0, 0, 0) if k_out is None else _rows3(k_out, idx, dt, "k_out")), positions.data_ptr(), p0, cos_sin.data_ptr(),
+        max_pos, slots_ptr, *f0, *f1, tier_split, T, H, KVH, D, rot, BS, dtype_code(dt), A, nat.ROPE_PAIRS if pairs else 0,
+        axes, 0, _error_ptr(idx))
+    _launch(nat.load().fd_rope_store_kv, packed, idx, "fd_rope_store_kv")
     return q_out
 
 
@@ -906,35 +927,32 @@ def _attn_workspace_bytes(H: int, KVH: int, D: int, dtype: torch.dtype) -> int:
     return nat.load().fd_attn_workspace_size(ctypes.byref(a))
 
 
-def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, tiers, tier_split, table, bt_row, k_start, BS,
+def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, table, W, bt_row, k_start, BS,
           max_q_len, max_k_len, workspace_buf) -> None:
-    dev, dt = q.device, q.dtype
-    _check(dev.type == "cuda", "q must be a CUDA tensor")
-    _check(q.dim() == 3 and out.shape == q.shape and out.dtype == dt and out.device == dev,
-           "q and out must be [T, H, D] alike")
-    _check(q.stride(2) == 1 and out.stride(2) == 1, "q and out need a contiguous head dim")
+    idx, dt = q.get_device(), q.dtype
+    if out.shape != q.shape:
+        raise RuntimeError("q and out must be [T, H, D] alike")
     T, H, D = q.shape
-    n = q_len.shape[0]
-    ptrs = (_need_i32(q_start, dev, n, "q_start"), _need_i32(q_len, dev, n, "q_len"), _need_i32(k_len, dev, n, "k_len"))
-    if lse is None:
-        lse_f = (0, 0, 0)
-    else:
-        _check(lse.dtype == torch.float32 and lse.device == dev and lse.shape == (H, T), "lse must be fp32 [H, T] on q's device")
-        lse_f = (lse.data_ptr(), lse.stride(0), lse.stride(1))
+    n = q_len.numel()
+    lse_f = (0, 0, 0)
+    if lse is not None:
+        if lse.dtype is not torch.float32 or lse.get_device() != idx or lse.shape != (H, T):
+            raise RuntimeError("lse must be fp32 [H, T] on q's device")
+        lse_f = (lse.data_ptr(), *lse.stride())
     need = _attn_workspace_bytes(H, KVH, D, dt)
     if workspace_buf is None:
-        workspace_buf = torch.empty(need, dtype=torch.uint8, device=dev)
-    else:
-        _check(workspace_buf.device == dev and workspace_buf.dtype == torch.uint8 and workspace_buf.is_contiguous()
-               and workspace_buf.numel() >= need, f"workspace_buf must be uint8 on q's device with >= {need} bytes")
-    bt = (0, 0) if table is None else (table.data_ptr(), table.stride(0))
+        workspace_buf = torch.empty(need, dtype=torch.uint8, device=q.device)
+    elif (workspace_buf.get_device() != idx or workspace_buf.dtype is not torch.uint8 or not workspace_buf.is_contiguous()
+          or workspace_buf.numel() < need):
+        raise RuntimeError(f"workspace_buf must be contiguous uint8 on q's device with >= {need} bytes")
     packed = _ATTN_STRUCT.pack(
-        q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(), out.stride(0), out.stride(1), *lse_f,
-        *tiers[0], *tiers[1], tier_split, *bt, 0 if bt_row is None else _need_i32(bt_row, dev, n, "bt_row"),
-        0 if k_start is None else _need_i32(k_start, dev, n, "k_start"), *ptrs, 0 if table is None else table.shape[1], T,
-        n, H, KVH, D, BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, workspace_buf.data_ptr(), workspace_buf.numel(),
-        error_word(dev).data_ptr())
-    _launch(fn, packed, dev, what)
+        *_rows3(q, idx, dt, "q"), *_rows3(out, idx, dt, "out"), *lse_f, *f0, *f1, tier_split,
+        *((0, 0) if table is None else (table.data_ptr(), table.stride(0))),
+        0 if bt_row is None else _i32(bt_row, idx, n, "bt_row"), 0 if k_start is None else _i32(k_start, idx, n, "k_start"),
+        _i32(q_start, idx, n, "q_start"), _i32(q_len, idx, n, "q_len"), _i32(k_len, idx, n, "k_len"), W, T, n, H, KVH, D,
+        BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, workspace_buf.data_ptr(), workspace_buf.numel(),
+        _error_ptr(idx))
+    _launch(fn, packed, idx, what)
 
 
 def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
@@ -956,19 +974,24 @@ def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier
     if the host knows them.  workspace_buf (uint8) replaces the call's own
     scratch memory."""
     t0, t1 = tiers
-    ref = t0 if t0 is not None else t1
-    _check(ref is not None, "at least one KV tier is required")
-    dev = q.device
-    _, KVH, BS, D = ref.k.shape
-    _check(q.dim() == 3 and q.shape[2] == D, "head size mismatch")
-    _check(t0 is None or t1 is None or t0.k.shape[1:] == t1.k.shape[1:], "tiers must share [KVH, BS, D]")
-    _check(block_table.dtype == torch.int32 and block_table.device == dev and block_table.dim() == 2
-           and (block_table.shape[1] < 2 or block_table.stride(1) == 1),
-           "block_table must be int32 [R, W] on q's device with contiguous rows")
-    _check(bt_row is not None or block_table.shape[0] >= q_len.shape[0], "block_table must have a row per request")
+    if t0 is None and t1 is None:
+        raise RuntimeError("at least one KV tier is required")
+    idx = q.get_device()
+    if idx < 0:
+        raise RuntimeError("q must be a CUDA tensor")
+    _, KVH, BS, D = (t0 if t0 is not None else t1).k.shape
+    if q.dim() != 3 or q.shape[2] != D:
+        raise RuntimeError("q must be [T, H, D] with the cache's head size")
+    if block_table.dtype is not torch.int32 or block_table.get_device() != idx or block_table.dim() != 2:
+        raise RuntimeError("block_table must be int32 [R, W] on q's device")
+    R, W = block_table.shape
+    if W > 1 and block_table.stride(1) != 1:
+        raise RuntimeError("block_table rows must be contiguous")
+    if bt_row is None and R < q_len.numel():
+        raise RuntimeError("block_table must have a row per request")
     _attn(nat.load().fd_chunk_attn, "fd_chunk_attn", q, out, lse, q_start, q_len, k_len, scale, KVH,
-          (_tier_fields(t0, dev, q.dtype), _tier_fields(t1, dev, q.dtype)), int(tier_split), block_table, bt_row, None, BS,
-          max_q_len, max_k_len, workspace_buf)
+          _tier_fields(t0, idx, q.dtype, (KVH, BS, D)), _tier_fields(t1, idx, q.dtype, (KVH, BS, D)), tier_split, block_table,
+          W, bt_row, None, BS, max_q_len, max_k_len, workspace_buf)
 
 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -980,15 +1003,16 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch
     of rows k_start .. k_start + k_len - 1 of k and v [S, KVH, D]; requests may
     share states.  q_len = 1 is a decode step.  The other arguments are
     chunk_attn's."""
-    dev = q.device
-    _check(k.dim() == 3 and k.shape == v.shape and k.stride() == v.stride() and (k.stride(2) == 1),
-           "k and v must be [S, KVH, D] alike with a contiguous head dim")
-    _check(k.dtype == q.dtype and v.dtype == q.dtype and k.device == dev and v.device == dev and q.dim() == 3
-           and k.shape[2] == q.shape[2], "k / v dtype, device or head size differs from q's")
+    idx, dt = q.get_device(), q.dtype
+    if idx < 0:
+        raise RuntimeError("q must be a CUDA tensor")
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.stride() != v.stride() or k.shape[2] != q.shape[2]:
+        raise RuntimeError("k and v must be [S, KVH, D] alike with q's head size")
     S, KVH, _ = k.shape
-    states = (k.data_ptr(), v.data_ptr(), 0, k.stride(1), k.stride(0), S, 0, 0)
-    _attn(nat.load().fd_cross_attn, "fd_cross_attn", q, out, lse, q_start, q_len, k_len, scale, KVH, (states, _NO_TIER), 0,
-          None, None, k_start, 0, max_q_len, max_k_len, workspace_buf)
+    k_ptr, k_st, k_sh = _rows3(k, idx, dt, "k")
+    _attn(nat.load().fd_cross_attn, "fd_cross_attn", q, out, lse, q_start, q_len, k_len, scale, KVH,
+          (k_ptr, _rows3(v, idx, dt, "v")[0], 0, k_sh, k_st, S, 0, 0), _NO_TIER, 0, None, 0, None, k_start, 0, max_q_len,
+          max_k_len, workspace_buf)
 
 
 # ------------------------------------------------------------- merge
