@@ -212,14 +212,14 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
       const int64_t tok = rq.qst + tok0 + row / p.G;
       const int h = g.kh * p.G + row % p.G;
       if (!g.whole) {
-        float* po = p.part_o + ((int64_t)slot * kRows + row) * D;
+        float4* po = reinterpret_cast<float4*>(p.part_o) + (int64_t)slot * (D / 4) * kRows + row;
         if (tx == 0) {
           p.part_ml[((int64_t)slot * kRows + row) * 2] = m[i];
           p.part_ml[((int64_t)slot * kRows + row) * 2 + 1] = l[i];
         }
 #pragma unroll
         for (int d = 0; d < kDim4; ++d)
-          if (64 * d + 4 * tx < D) *reinterpret_cast<float4*>(po + 64 * d + 4 * tx) = o[i][d];
+          if (64 * d + 4 * tx < D) po[(16 * d + tx) * kRows] = o[i][d];
         continue;
       }
       const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
@@ -244,43 +244,51 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
   }
 }
 
-// The cut items' partials joined: o = sum_p O_p 2^(m_p - m) / sum_p l_p 2^(m_p - m),
-// parts in ascending CTA order.  CTA (c, y) takes rows 8 y .. of the item
-// whose first part CTA c wrote, one warp per row, so a long item's parts are
-// read by many SMs at once; it is a programmatic dependent of the attention
-// kernel, whose end it awaits.
-constexpr int kCombineWarps = 8;
+// The cut items' partials joined: o = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m),
+// parts in ascending CTA order.  CTA (c, y) takes rows 32 y .. of the item
+// whose first part CTA c wrote, so a long item's parts are read by many SMs
+// at once; a warp's lanes are 8 rows times 4 groups of 4 dims: the partials
+// lie row by row within a group of dims (whole lines), and the 4 groups are
+// 32 bytes of an output row.  A programmatic dependent of the attention
+// kernel: its CTAs start while that one's last ones run, and await its end.
+constexpr int kCombineRows = 32, kCombineThreads = 256;
 template <typename T>
-__global__ void __launch_bounds__(kCombineWarps * 32) fd_attn_combine_kernel(const __grid_constant__ AttnParams p,
-                                                                             int item_rows) {
+__global__ void __launch_bounds__(kCombineThreads) fd_attn_combine_kernel(const __grid_constant__ AttnParams p,
+                                                                          int item_rows) {
   griddep_wait();
   const int c = blockIdx.x;
   const Cut cut = p.cuts[c];
-  if (cut.nparts == 0) return;
-  const int lane = threadIdx.x & 31;
-  const int row = blockIdx.y * kCombineWarps + (threadIdx.x >> 5);
+  const int row0 = blockIdx.y * kCombineRows;
+  if (row0 >= cut.rows || cut.nparts == 0) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int row = row0 + (warp & 3) * 8 + (lane & 7);
   if (row >= cut.rows) return;
   // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
-  auto at = [&](int i) { return ((int64_t)(2 * (c + i) + (i == 0 ? 1 : 0))) * item_rows + row; };
+  auto slot = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float m = -INFINITY;
-  for (int i = lane; i < cut.nparts; i += 32) m = fmaxf(m, p.part_ml[2 * at(i)]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, off));
+#pragma unroll 4
+  for (int i = 0; i < cut.nparts; ++i) m = fmaxf(m, ml[slot(i) * item_rows + row].x);
   const float base = m == -INFINITY ? 0.f : m;
   float l = 0.f;
-  for (int i = 0; i < cut.nparts; ++i) l += p.part_ml[2 * at(i) + 1] * exp2f(p.part_ml[2 * at(i)] - base);
+#pragma unroll 4
+  for (int i = 0; i < cut.nparts; ++i) {
+    const float2 v = ml[slot(i) * item_rows + row];
+    l += v.y * exp2f(v.x - base);
+  }
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t tok = cut.row0 + row / p.G;
   const int h = cut.kh * p.G + row % p.G;
-  if (lane == 0 && p.lse != nullptr)
+  if (warp < 4 && lane < 8 && p.lse != nullptr)
     p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
   T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
-  for (int d = 4 * lane; d < p.D; d += 128) {
+  const int groups = p.D / 4;
+  for (int d = (warp >> 2) * 4 + (lane >> 3); d < groups; d += 8) {
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
     for (int i = 0; i < cut.nparts; ++i) {
-      const float w = exp2f(p.part_ml[2 * at(i)] - base);
-      const float4 x = *reinterpret_cast<const float4*>(p.part_o + at(i) * p.D + d);
+      const float w = exp2f(ml[slot(i) * item_rows + row].x - base);
+      const float4 x = reinterpret_cast<const float4*>(p.part_o)[(slot(i) * groups + d) * item_rows + row];
       acc.x = fmaf(w, x.x, acc.x);
       acc.y = fmaf(w, x.y, acc.y);
       acc.z = fmaf(w, x.z, acc.z);
@@ -291,16 +299,16 @@ __global__ void __launch_bounds__(kCombineWarps * 32) fd_attn_combine_kernel(con
 #pragma unroll
     for (int e = 0; e < 4; ++e) t[e] = Dt<T>::narrow(f[e]);
     if (sizeof(T) == 4)
-      *reinterpret_cast<uint4*>(po + d) = *reinterpret_cast<const uint4*>(t);
+      *reinterpret_cast<uint4*>(po + 4 * d) = *reinterpret_cast<const uint4*>(t);
     else
-      *reinterpret_cast<uint2*>(po + d) = *reinterpret_cast<const uint2*>(t);
+      *reinterpret_cast<uint2*>(po + 4 * d) = *reinterpret_cast<const uint2*>(t);
   }
 }
 
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + kCombineWarps - 1) / kCombineWarps));
-  cfg.blockDim = dim3(kCombineWarps * 32);
+  cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + kCombineRows - 1) / kCombineRows));
+  cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;

@@ -62,7 +62,8 @@ struct AttnParams {
   int ctas;
   Cut* cuts;               // [ctas]
   float* part_ml;          // [ctas][2][rows per item][2]: m (log2 domain), l
-  float* part_o;           // [ctas][2][rows per item][D]
+  float* part_o;           // [ctas][2][D / 4][rows per item][4]
+  int out32;               // rows of out are 32-byte aligned (fd_attn_mma.cu)
   int32_t* err;
 };
 
@@ -181,10 +182,16 @@ struct Sched {
 
   struct Scratch {
     long long warp_sum[32];
-    long long total, start;  // sum over all requests; position of the request found
-    int found, item;
+    long long start, per_head;  // position of the request found; its cost per kv head
     long long item_start;
+    int found, item;
+    Req rq;
   };
+
+  // a / b (b > 0), in 32 bits where they fit: a 64-bit division is a routine of hundreds of cycles
+  __device__ __forceinline__ static long long quot(long long a, long long b) {
+    return ((a | b) >> 32) == 0 ? (long long)((uint32_t)a / (uint32_t)b) : a / b;
+  }
 
   // All threads of the block (NT of them) together: the range of CTA `c` and
   // the item it starts in.  False: no work.
@@ -192,7 +199,8 @@ struct Sched {
   __device__ bool init(Scratch* sc, int c, int min_per) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kWarps = NT / 32;
-    long long total = 0, mine = 0, mine_at = 0;
+    long long total = 0, mine = 0, mine_at = 0, per_head = 0;
+    Req mine_rq = {0, 0, 0, 0};
     // pass 0 adds up all requests, pass 1 finds this CTA's (from the values
     // that pass 0 left when one round holds all requests)
     const bool one = p.n <= NT;
@@ -202,7 +210,10 @@ struct Sched {
       for (int base = 0; base < p.n; base += NT) {
         if (pass == 0 || !one) {
           const int i = base + tid;
-          mine = i < p.n ? cost(p, load_req(p, i)) * p.KVH : 0;
+          mine_rq.qlen = 0;
+          if (i < p.n) mine_rq = load_req(p, i);
+          per_head = cost(p, mine_rq);
+          mine = per_head * p.KVH;
           long long x = mine;
 #pragma unroll
           for (int off = 1; off < 32; off <<= 1) {
@@ -223,11 +234,13 @@ struct Sched {
         if (pass == 1 && mine > 0 && mine_at <= p0 && p0 < mine_at + mine) {
           sc->found = base + tid;
           sc->start = mine_at;
+          sc->per_head = per_head;
+          sc->rq = mine_rq;
         }
       }
       if (pass == 0) {
         total = carry;
-        per = (total + p.ctas - 1) / p.ctas;
+        per = quot(total + p.ctas - 1, p.ctas);
         if (per < min_per) per = min_per;
         p0 = (long long)c * per;
         p1 = min(p0 + per, total);
@@ -236,23 +249,27 @@ struct Sched {
     }
     __syncthreads();
     r = sc->found;
-    rq = load_req(p, r);
-    const long long per_head = cost(p, rq);
+    rq = sc->rq;
+    per_head = sc->per_head;
     const long long off = p0 - sc->start;
-    kh = (int)(off / per_head);
+    kh = (int)quot(off, per_head);
     const long long x = off - (long long)kh * per_head;
     if (warp == 0) {  // the last item that starts at or before x, 32 candidates at a time
       int lo = 0, hi = items(p, rq);
+      long long at = 0;
       while (hi - lo > 1) {
         const int gap = (hi - lo + 31) / 32;
         const int i = lo + lane * gap;
-        const unsigned at = __ballot_sync(0xffffffffu, i < hi && before(p, rq, i) <= x);
-        lo += (31 - __clz(at)) * gap;  // lane 0 always: before(lo) <= x
+        const long long v = i < hi ? before(p, rq, i) : 0;
+        const unsigned in = __ballot_sync(0xffffffffu, i < hi && v <= x);
+        const int last = 31 - __clz(in);  // lane 0 always: before(lo) <= x
+        at = __shfl_sync(0xffffffffu, v, last);
+        lo += last * gap;
         hi = min(hi, lo + gap);
       }
       if (lane == 0) {
         sc->item = lo;
-        sc->item_start = sc->start + (long long)kh * per_head + before(p, rq, lo);
+        sc->item_start = p0 - x + at;
       }
     }
     __syncthreads();
@@ -279,7 +296,7 @@ struct Sched {
       g.nparts = 0;
       if (!g.whole && g.j0 == 0 && g.j1 > 0) {
         const long long last = s + kW + (long long)u * (n - 1);
-        g.nparts = (int)(last / per - p0 / per) + 1;
+        g.nparts = (int)(quot(last, per) - quot(p0, per)) + 1;
       }
       const bool has = g.j0 < g.j1 || (n == 0 && s >= p0);
       seg_q = rq;

@@ -72,9 +72,9 @@ struct Geo {
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kRingK * kTile;
   static constexpr int kOffBar = kOffV + kRingV * kTile;
-  // q full/empty, k full/empty, v full/empty, s_full[2][2], p_full[2][2], pv_done[2],
-  // o_full[2], o_both, o_empty, ml_full, seg full/empty, drain
-  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 4 + 4 + 2 + 2 + 3 + 2 * kSegs + 1;
+  // q full/empty, k full/empty, v full/empty, s_full[2][2], p_full[2][2], o_full[2],
+  // o_both, o_empty, ml_full, seg full/empty, drain
+  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 4 + 4 + 2 + 3 + 2 * kSegs + 1;
   static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kOffMl = kOffSeg + kSegs * 64;   // [2 streams][128 rows] float2 (before that: Walk::Scratch)
   static constexpr int kOffMisc = kOffMl + 2 * kM * 8;  // abort flag, TMEM address
@@ -173,6 +173,51 @@ template <>
 __device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
   const __half2 v = __floats2half2_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+// A ring position moved on by `by` slots.
+template <int R>
+__device__ __forceinline__ void advance(int& slot, uint32_t& phase, int by) {
+  if (by > R) {
+    phase ^= (uint32_t)(by / R) & 1u;
+    by %= R;
+  }
+  slot += by;
+  if (slot >= R) {
+    slot -= R;
+    phase ^= 1u;
+  }
+}
+
+// The products with 128-byte swizzled operands, descriptors by their low
+// words (address and leading offset, 16-byte units); the high word (stride
+// 1024 bytes, version, swizzle) is the same for all of them.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ void umma_f16_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      : "memory");
+}
+__device__ __forceinline__ void umma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
+                                               uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %5};\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      : "memory");
+}
+
+// 32 bytes in one store (both 32-byte aligned).
+__device__ __forceinline__ void stg256(void* p, const uint32_t (&v)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
+               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
 }
 
 // Block id of box `lane` (keys 128 j + 16 lane ..) where boxes lie within
@@ -301,86 +346,90 @@ __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int n = x ? seg.n1 : seg.n0;
   uint32_t ph = *phases;
-        const bool pair = seg.pair != 0, single = !pair;
-        const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
-        const int tg = row / p.G, hg = row % p.G;
-        const uint32_t t_o = t_s - x * kKT + 2 * kKT;  // O of stream A; B's 128 columns on
-        const int m_tiles = seg.m, slot = seg.slot;
-        const int qi = seg.tok0 + (pair ? x * p.tq : 0) + tg;
-        const bool row_ok = tg < p.tq && qi < seg.qlen;
-        float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
-        // everyone has read the m and l of the segment before
-        if (nseg > 0 && !__all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err)))
-          return false;
-        if (single && m_tiles > 0) {
-          ml[x * kM + row] = make_float2(m, l);
-          __syncwarp();
-          if (lane == 0) mbar_arrive(ml_full);
-          if (!__all_sync(0xffffffffu, wait_or_abort(ml_full, (ph >> 3) & 1u, misc, p.err) &&
-                                           wait_or_abort(o_both, (ph >> 3) & 1u, misc, p.err)))
-            return false;
-          ph ^= 8u;
-          const float2 other = ml[(x ^ 1) * kM + row];
-          const float mm = fmaxf(m, other.x);
-          const float base = mm == -INFINITY ? 0.f : mm;
-          const float wo = exp2f(m - base), wt = exp2f(other.x - base);
-          wa = x ? wt : wo;
-          wb = x ? wo : wt;
-          l = l * wo + other.y * wt;
-          m = mm;
-        } else if (n > 0) {
-          if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[x], (ph >> 2) & 1u, misc, p.err))) return false;
-          ph ^= 4u;
+  const bool pair = seg.pair != 0, single = !pair;
+  const int row = (warp & 3) * 32 + lane;  // row of the tile = TMEM lane
+  const int tg = row / p.G, hg = row % p.G;
+  const uint32_t t_o = t_s - x * kKT + 2 * kKT;  // O of stream A; B's 128 columns on
+  const int m_tiles = seg.m, slot = seg.slot;
+  const int qi = seg.tok0 + (pair ? x * p.tq : 0) + tg;
+  const bool row_ok = tg < p.tq && qi < seg.qlen;
+  float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
+  // everyone has read the m and l of the segment before
+  if (nseg > 0 && !__all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err)))
+    return false;
+  if (single && m_tiles > 0) {
+    ml[x * kM + row] = make_float2(m, l);
+    __syncwarp();
+    if (lane == 0) mbar_arrive(ml_full);
+    if (!__all_sync(0xffffffffu, wait_or_abort(ml_full, (ph >> 3) & 1u, misc, p.err) &&
+                                     wait_or_abort(o_both, (ph >> 3) & 1u, misc, p.err)))
+      return false;
+    ph ^= 8u;
+    const float2 other = ml[(x ^ 1) * kM + row];
+    const float mm = fmaxf(m, other.x);
+    const float base = mm == -INFINITY ? 0.f : mm;
+    const float wo = exp2f(m - base), wt = exp2f(other.x - base);
+    wa = x ? wt : wo;
+    wb = x ? wo : wt;
+    l = l * wo + other.y * wt;
+    m = mm;
+  } else if (n > 0) {
+    if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[x], (ph >> 2) & 1u, misc, p.err))) return false;
+    ph ^= 4u;
+  }
+  tc_fence_after();
+  const int64_t tok = seg.qst + qi;
+  const int h = seg.kh * p.G + hg;
+  const bool have_b = single && seg.n1 > 0;
+  const bool have = single ? m_tiles > 0 : n > 0;
+  const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
+  wa *= inv;
+  wb *= inv;
+  const int item_row = (pair ? x * p.tq * p.G : 0) + row;
+  if (row_ok && (!single || x == 0)) {
+    if (slot >= 0) {
+      reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
+    } else if (p.lse != nullptr) {
+      p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    }
+  }
+  __syncwarp();
+  const int c_lo = single ? x * (KD / 32) : 0, c_hi = single ? c_lo + KD / 32 : KD / 16;  // 16 dims each
+  if (any_row) {
+#pragma unroll 1
+    for (int c = c_lo; c < c_hi; ++c) {
+      if (16 * c >= p.D) break;
+      uint32_t oa[16], ob[16];
+      float f[16];
+      if (have) tmem_ld16_nowait(t_o + (single ? 0 : x * kM) + 16 * c, oa);
+      if (have_b) tmem_ld16_nowait(t_o + kM + 16 * c, ob);
+      tmem_wait_ld();
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        f[e] = have ? __uint_as_float(oa[e]) * wa : 0.f;
+        if (have_b) f[e] = fmaf(__uint_as_float(ob[e]), wb, f[e]);
+      }
+      if (row_ok && slot >= 0) {  // [dim / 4][row][dim % 4]: a warp's rows side by side
+        float4* po = reinterpret_cast<float4*>(p.part_o) +
+                     ((int64_t)slot * (p.D / 4) + 4 * c) * kItemRows + item_row;
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          if (16 * c + e < p.D) po[(e / 4) * kItemRows] = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      } else if (row_ok) {
+        unsigned char* po = p.out + tok * p.o_st + h * p.o_sh + 32 * c;
+        uint32_t w[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) w[e] = pack2<T>(f[2 * e], f[2 * e + 1]);
+        if (p.out32) {
+          stg256(po, w);
+        } else {
+          *reinterpret_cast<uint4*>(po) = make_uint4(w[0], w[1], w[2], w[3]);
+          if (16 * c + 8 < p.D) *reinterpret_cast<uint4*>(po + 16) = make_uint4(w[4], w[5], w[6], w[7]);
         }
-        tc_fence_after();
-        const int64_t tok = seg.qst + qi;
-        const int h = seg.kh * p.G + hg;
-        const bool have_b = single && seg.n1 > 0;
-        const bool have = single ? m_tiles > 0 : n > 0;
-        const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
-        wa *= inv;
-        wb *= inv;
-        const int item_row = (pair ? x * p.tq * p.G : 0) + row;
-        if (row_ok && (!single || x == 0)) {
-          if (slot >= 0) {
-            reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
-          } else if (p.lse != nullptr) {
-            p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-          }
-        }
-        __syncwarp();
-        const int c_lo = single ? x * (KD / 32) : 0, c_hi = single ? c_lo + KD / 32 : KD / 16;  // 16 dims each
-        if (any_row) {
-  #pragma unroll 1
-          for (int c = c_lo; c < c_hi; ++c) {
-            if (16 * c >= p.D) break;
-            uint32_t oa[16], ob[16];
-            float f[16];
-            if (have) tmem_ld16_nowait(t_o + (single ? 0 : x * kM) + 16 * c, oa);
-            if (have_b) tmem_ld16_nowait(t_o + kM + 16 * c, ob);
-            tmem_wait_ld();
-  #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              f[e] = have ? __uint_as_float(oa[e]) * wa : 0.f;
-              if (have_b) f[e] = fmaf(__uint_as_float(ob[e]), wb, f[e]);
-            }
-            if (row_ok && slot >= 0) {
-              float* po = p.part_o + ((int64_t)slot * kItemRows + item_row) * p.D + 16 * c;
-  #pragma unroll
-              for (int e = 0; e < 16; e += 4)
-                if (16 * c + e < p.D) *reinterpret_cast<float4*>(po + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-            } else if (row_ok) {
-              unsigned char* po = p.out + tok * p.o_st + h * p.o_sh + 32 * c;
-  #pragma unroll
-              for (int e = 0; e < 16; e += 8)
-                if (16 * c + e < p.D)
-                  *reinterpret_cast<uint4*>(po + 2 * e) =
-                      make_uint4(pack2<T>(f[e], f[e + 1]), pack2<T>(f[e + 2], f[e + 3]), pack2<T>(f[e + 4], f[e + 5]),
-                                 pack2<T>(f[e + 6], f[e + 7]));
-            }
-            __syncwarp();  // the TMEM loads are the whole warp's
-          }
-        }
+      }
+      __syncwarp();  // the TMEM loads are the whole warp's
+    }
+  }
   *phases = ph;
   return true;
 }
@@ -402,8 +451,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   uint64_t* v_empty = v_full + kRingV;    // [kRingV] two arrivals
   uint64_t* s_full = v_empty + kRingV;    // [2][2] MMA commit: S of the stream's step is in its buffer
   uint64_t* p_full = s_full + 4;          // [2][2] the stream's four softmax warps wrote P there
-  uint64_t* pv_done = p_full + 4;         // [2] MMA commit after each P.V of the stream
-  uint64_t* o_full = pv_done + 2;         // [2] pairs: MMA commit after the stream's last P.V
+  uint64_t* o_full = p_full + 4;          // [2] pairs: MMA commit after the stream's last P.V
   uint64_t* o_both = o_full + 2;          // singles: both streams' last P.V
   uint64_t* o_empty = o_both + 1;         // all eight softmax warps are done with the segment
   uint64_t* ml_full = o_empty + 1;        // singles: both streams' m and l are in shared memory
@@ -435,7 +483,6 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       mbar_init(&p_full[s], 4);
     }
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&pv_done[s], 1);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(o_both, 2);
@@ -520,6 +567,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         break;
       }
       ++nq;
+      int id = box_block(p, rq.kbase, rq.klen, g.j0, lane);
       const int nt = g.pair ? 2 : 1;
       if (mp.q_tma) {
         if (lane == 0) {
@@ -538,7 +586,6 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       }
       // a pair's neighbours read the same keys again: they stay in L2
       const uint64_t pol = g.pair ? pol_again : pol_once;
-      int id = box_block(p, rq.kbase, rq.klen, g.j0, lane);
       for (int j = g.j0; j < g.j1; ++j) {
         const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
@@ -598,10 +645,15 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     // ------------------------------------------------ MMA issuer of stream x
     if (lane == 0) {
       const int x = warp == kWarpMmaB ? 1 : 0;
-      const uint32_t sq0 = smem_u32(smem);
       const uint32_t t_s = tmem + x * kKT, t_o = tmem + 2 * kKT + x * kM;
-      uint32_t tile0 = 0, nq = 0;   // K/V tiles of earlier segments; segments with keys
-      uint32_t pp = 0;              // phase parities of p_full's two buffers
+      const uint32_t base = smem_u32(smem) >> 4;
+      uint64_t* const my_s = s_full + 2 * x;
+      uint64_t* const my_p = p_full + 2 * x;
+      uint32_t nq = 0;  // segments with keys
+      uint32_t pp = 0;  // phase parities of p_full's two buffers
+      // ring slots (and phases) of the segment's first tile
+      int k0 = 0, v0 = 0;
+      uint32_t kp0 = 0, vp0 = 0;
       bool ok = true;
       for (int nseg = 0; ok; ++nseg) {
         const int ss = nseg % kSegs;
@@ -611,29 +663,41 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         const int n = x ? segs[ss].n1 : segs[ss].n0;
         mbar_arrive(&seg_empty[ss]);
         if (!live) break;
-        // the ring's tile that step i takes, and whether it is the tile's last step
-        auto tile_of = [&](int i) { return tile0 + (pair ? (i >> 1) : 2 * (i >> 1) + x); };
+        // this stream's next K and V tile: every tile of a pair, every other one of a single
+        const int stride = pair ? 1 : 2;
+        int ks_ = k0, vs_ = v0;
+        uint32_t kp = kp0, vp = vp0;
+        if (!pair && x) {
+          advance<kRingK>(ks_, kp, 1);
+          advance<kRingV>(vs_, vp, 1);
+        }
         // a single's tile has one user, which arrives for both
         auto release = [&](uint64_t* empty) {
           umma_commit(empty);
           if (!pair) mbar_arrive(empty);
         };
+        const uint32_t q_lo = base + (uint32_t)((pair ? x : 0) * (kTile >> 4)) + (1u << 16);
+        // q.K^T of step i into its S buffer; step n is none: its commit tells
+        // that the P.V before it are done
         auto qk = [&](int i) {
-          const uint32_t t = tile_of(i);
-          const int st = t % kRingK;
-          if (!(i & 1) && !poll_or_abort(&k_full[st], (t / kRingK) & 1u, misc, p.err)) return false;
-          tc_fence_after();
-          const uint32_t sq = sq0 + (pair ? x : 0) * kTile;
-          const uint32_t sk = sq0 + Ge::kOffK + st * kTile + (i & 1) * (kHalf * 128);
+          const int h = i & 1;
+          if (i < n) {
+            if (h == 0 && !poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
+            tc_fence_after();
+            const uint32_t k_lo =
+                base + (uint32_t)((Ge::kOffK + ks_ * kTile + h * (kHalf * 128)) >> 4) + (1u << 16);
 #pragma unroll
-          for (int ks = 0; ks < KD / 16; ++ks) {
-            const uint32_t off = (ks >> 2) * kPanel + (ks & 3) * 32;
-            umma_f16(t_s + (i & 1) * kHalf, sw128_desc(sq + off, 16, 1024), sw128_desc(sk + off, 16, 1024), kIdQK,
-                     ks > 0 ? 1u : 0u);
+            for (int ks = 0; ks < KD / 16; ++ks) {
+              const uint32_t off = (uint32_t)((ks >> 2) * kPanel + (ks & 3) * 32) >> 4;
+              umma_f16_lo(t_s + h * kHalf, q_lo + off, k_lo + off, kIdQK, ks > 0 ? 1u : 0u);
+            }
           }
-          umma_commit(&s_full[2 * x + (i & 1)]);
-          if ((i & 1) || i == n - 1) release(&k_empty[st]);
-          if (i == n - 1) umma_commit(q_empty);
+          umma_commit(&my_s[h]);
+          if (i < n && (h || i == n - 1)) {
+            release(&k_empty[ks_]);
+            advance<kRingK>(ks_, kp, stride);
+            if (i == n - 1) umma_commit(q_empty);
+          }
           return true;
         };
         if (m > 0) {
@@ -641,26 +705,27 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           ++nq;
           if (ok && n == 0) mbar_arrive(q_empty);
         }
-        if (ok && n > 0) ok = qk(0);
-        if (ok && n > 1) ok = qk(1);
+        if (ok && n > 0) ok = qk(0) && qk(1);
         // the last segment's O has been read
         if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
         for (int i = 0; ok && i < n; ++i) {
-          const uint32_t t = tile_of(i);
-          const int st = t % kRingV, h = i & 1;
-          ok = poll_or_abort(&p_full[2 * x + h], (pp >> h) & 1u, misc, p.err) &&
-               (h || poll_or_abort(&v_full[st], (t / kRingV) & 1u, misc, p.err));
+          const int h = i & 1;
+          if (h == 0) ok = poll_or_abort(&v_full[vs_], vp, misc, p.err);
+          ok = ok && poll_or_abort(&my_p[h], (pp >> h) & 1u, misc, p.err);
           if (!ok) break;
           pp ^= 1u << h;
           tc_fence_after();
-          const uint32_t sv = sq0 + Ge::kOffV + st * kTile + h * (kHalf * 128);
+          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile + h * (kHalf * 128)) >> 4) +
+                                ((uint32_t)(kPanel >> 4) << 16);
 #pragma unroll
           for (int ks = 0; ks < kHalf / 16; ++ks)
-            umma_f16_ts(t_o, t_s + h * kHalf + 8 * ks, sw128_desc(sv + ks * 2048, kPanel, 1024), kIdPV,
-                        (i > 0 || ks > 0) ? 1u : 0u);
-          umma_commit(&pv_done[x]);
-          if (h || i == n - 1) release(&v_empty[st]);
-          if (i + 2 < n) ok = qk(i + 2);
+            umma_f16_ts_lo(t_o, t_s + h * kHalf + 8 * ks, v_lo + (uint32_t)(ks * 2048 >> 4), kIdPV,
+                           (i > 0 || ks > 0) ? 1u : 0u);
+          if (i + 2 <= n) ok = qk(i + 2);
+          if (h || i == n - 1) {
+            release(&v_empty[vs_]);
+            advance<kRingV>(vs_, vp, stride);
+          }
         }
         if (!ok) break;
         if (m > 0) {
@@ -671,13 +736,15 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           }
           // a pair's tiles that only the other stream sees
           for (int t = (n + 1) >> 1; ok && pair && t < m; ++t) {
-            const uint32_t u = tile0 + t;
-            ok = poll_or_abort(&k_full[u % kRingK], (u / kRingK) & 1u, misc, p.err);
-            if (ok) mbar_arrive(&k_empty[u % kRingK]);
-            ok = ok && poll_or_abort(&v_full[u % kRingV], (u / kRingV) & 1u, misc, p.err);
-            if (ok) mbar_arrive(&v_empty[u % kRingV]);
+            ok = poll_or_abort(&k_full[ks_], kp, misc, p.err);
+            if (ok) mbar_arrive(&k_empty[ks_]);
+            ok = ok && poll_or_abort(&v_full[vs_], vp, misc, p.err);
+            if (ok) mbar_arrive(&v_empty[vs_]);
+            advance<kRingK>(ks_, kp, 1);
+            advance<kRingV>(vs_, vp, 1);
           }
-          tile0 += m;
+          advance<kRingK>(k0, kp0, m);
+          advance<kRingV>(v0, vp0, m);
         }
       }
       if (!ok) misc[0] = 1;
@@ -689,7 +756,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     // ------------------------------------------------ softmax of stream x
     const int x = warp >> 2;
     const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kKT;
-    // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3), pv_done (4)
+    // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3)
     uint32_t ph = 0;
     bool ok = true;
     for (int nseg = 0; ok; ++nseg) {
@@ -738,9 +805,9 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           const float mxs = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.sl2;
           const bool grow = m != -INFINITY && mxs > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {
-            // O takes the earlier steps: the last one's P.V may still run (the
-            // ones before it were issued before this S's q.K^T)
-            ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[x], ((ph >> 4) & 1u) ^ 1u, misc, p.err));
+            // O takes the earlier steps: the last one's P.V may still run; the
+            // commit of the next S follows it
+            ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * x + (h ^ 1)], (ph >> (h ^ 1)) & 1u, misc, p.err));
             if (!ok) break;
             tc_fence_after();
             const float alpha = grow ? exp2f(m - mxs) : 1.f;
@@ -775,14 +842,18 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           expo(rb, 16);
           tmem_wait_st();
           tc_fence_before();
-          float a0, a1, b0, b1;
-          f2_unpack(ls[0], a0, a1);
-          f2_unpack(ls[1], b0, b1);
-          l += (a0 + a1) + (b0 + b1);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[2 * x + h]);
+          float a0, a1;
+          f2_unpack(f2_add(ls[0], ls[1]), a0, a1);
+          l += a0 + a1;
+        } else if (lane == 0) {
+          mbar_arrive(&p_full[2 * x + h]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[2 * x + h]);
-        ph ^= 16u;  // bit 4: parity of this step's P.V
+      }
+      if (ok && n > 0) {  // the commit of step n, which holds no scores
+        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * x + (n & 1)], (ph >> (n & 1)) & 1u, misc, p.err));
+        ph ^= 1u << (n & 1);
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, finish_rows<T, KD>(p, seg, x, t_s, m, l, any_row, nseg, &ph, ml, o_empty, misc));
@@ -834,6 +905,7 @@ int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
   p.cuts = reinterpret_cast<Cut*>(ws);
   p.part_ml = reinterpret_cast<float*>(ws + mm::kMaxCtas * sizeof(Cut));
   p.part_o = p.part_ml + 2 * 2 * (size_t)mm::kMaxCtas * mm::kItemRows;
+  p.out32 = ((reinterpret_cast<uintptr_t>(p.out) | (uint64_t)p.o_st | (uint64_t)p.o_sh) & 31u) == 0 && p.D % 16 == 0;
   p.tq = mm::kM / p.G;
   p.ctas = sms < mm::kMaxCtas ? sms : mm::kMaxCtas;
   mm::MmaParams mp{};
