@@ -305,6 +305,7 @@ LENS = {
     "verify": ([4, 7, 1, 5], [1000, 33, 129, 2049]),
     "one": ([3], [5000]),
     "chunks": ([300, 65, 257], [300, 1100, 640]),
+    "tokens": ([1, 1, 0, 1, 1, 1, 1, 1], [1, 5000, 4, 0, 129, 128, 127, 640]),
 }
 
 
@@ -333,6 +334,11 @@ def test_chunk_attention(dtype, H, KVH, D, block, host, lens):
                        max_k_len=max(kl))
     gpu_ops.check_device_errors(dev())
     ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
+    # bounds that are too small cost time, not the result
+    out3 = torch.full_like(out, NAN)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), scale, out3, lse, max_q_len=1, max_k_len=1)
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out3, lse, refs, start, ql, dtype, D, _rounded(dtype))
     # table rows in another order, no bounds, no lse: the same result
     order = list(range(len(ql)))[::-1]
     out2 = torch.full_like(out, NAN)
@@ -346,7 +352,7 @@ def test_chunk_attention(dtype, H, KVH, D, block, host, lens):
     (torch.bfloat16, 8, 2, 128), (torch.float16, 20, 20, 64), (torch.float16, 5, 1, 80), (torch.bfloat16, 7, 1, 112),
     (torch.float32, 4, 4, 64), (torch.float32, 8, 1, 128), (torch.bfloat16, 4, 2, 256),
 ])
-@pytest.mark.parametrize("lens", ["edges", "verify", "chunks"])
+@pytest.mark.parametrize("lens", ["edges", "verify", "chunks", "tokens"])
 def test_cross_attention(dtype, H, KVH, D, lens):
     ql, kl = LENS[lens]
     g = torch.Generator(device="cuda").manual_seed(H * D)
@@ -363,7 +369,9 @@ def test_cross_attention(dtype, H, KVH, D, lens):
     lim = [torch.full((n,), x - 1, device="cuda") for n, x in zip(ql, kl)]
     refs = _refs(q, start, ql, [k[s:s + n] for s, n in zip(k_start, kl)], [v[s:s + n] for s, n in zip(k_start, kl)], lim,
                  0.11)
-    gpu_ops.cross_attn(q, k, v, i32(start), i32(ql), i32(k_start), i32(kl), 0.11, out, lse)
+    for bound in (0, max(ql)):
+        out.fill_(NAN)
+        gpu_ops.cross_attn(q, k, v, i32(start), i32(ql), i32(k_start), i32(kl), 0.11, out, lse, max_q_len=bound)
     gpu_ops.check_device_errors(dev())
     ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
 
@@ -384,17 +392,22 @@ def test_many_requests_more_than_one_scan_round(dtype):
     ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
 
 
+@pytest.mark.parametrize("bound", [0, 6])
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
-def test_scores_far_apart(dtype):
+def test_scores_far_apart(dtype, bound):
     """Rows whose maximum grows late and by a lot, and rows of equal scores."""
-    H, KVH, D, nk = 4, 1, 64, 700
+    H, KVH, D, nk = 4, 1, 64, 2500
     g = torch.Generator(device="cuda").manual_seed(2)
     keys, vals, table, tiers, n_hbm = _paged([nk], KVH, D, 16, dtype, g)
     q, start, out, lse = _queries([6], H, D, dtype, g)
     q[1:7, 0] *= 40
     q[1:7, 1] = 0
+    for i, j in enumerate(range(200, nk, 450)):  # ever larger scores, far apart
+        page, at = int(table[0, j // 16]), j % 16
+        keys[0][j] = (q[3, 2] * (1 + i)).unsqueeze(0)
+        tiers[0].k[page, :, at] = keys[0][j]
     refs = _refs(q, start, [6], keys, vals, [nk - 6 + torch.arange(6, device="cuda")], 0.7)
-    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32([6]), i32([nk]), 0.7, out, lse)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32([6]), i32([nk]), 0.7, out, lse, max_q_len=bound)
     ref.check_attn(out, lse, refs, start, [6], dtype, D, _rounded(dtype))
 
 
@@ -454,24 +467,27 @@ def test_attention_refusals():
                            i32([1, 1]), i32([1, 1]), 1.0, torch.empty_like(q))
 
 
+@pytest.mark.parametrize("many", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
-def test_two_streams_and_two_graphs_at_once(dtype):
+def test_two_streams_and_two_graphs_at_once(dtype, many):
     """Calls share no scratch memory: two captured graphs replayed on two
     streams at the same time give what each gives alone, bit for bit."""
     H, KVH, D = 8, 2, 128
     g = torch.Generator(device="cuda").manual_seed(4)
     sides = []
-    for ql, kl in (([3, 5], [3000, 2000]), ([2, 4, 1], [2500, 100, 4000])):
+    for ql, kl in ((([300, 5], [3000, 2000]), ([2, 400, 1], [2500, 500, 4000])) if many else
+                   (([3, 5], [3000, 2000]), ([2, 4, 1], [2500, 100, 4000]))):
         keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
         q, start, out, lse = _queries(ql, H, D, dtype, g)
         args = (q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), 0.1)
-        gpu_ops.chunk_attn(*args, out, lse)
+        args_kw = dict(max_q_len=max(ql))
+        gpu_ops.chunk_attn(*args, out, lse, **args_kw)
         torch.cuda.synchronize()
         alone = out.clone()
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
-            gpu_ops.chunk_attn(*args, out, lse)
-        sides.append((graph, torch.cuda.Stream(), out, alone, args, lse))
+            gpu_ops.chunk_attn(*args, out, lse, **args_kw)
+        sides.append((graph, torch.cuda.Stream(), out, alone, args, (lse, args_kw)))
     for _ in range(20):
         for graph, stream, out, *_ in sides:
             with torch.cuda.stream(stream):
@@ -481,9 +497,9 @@ def test_two_streams_and_two_graphs_at_once(dtype):
     for _, stream, out, alone, args, lse in sides:
         assert torch.equal(torch.nan_to_num(out.float()), torch.nan_to_num(alone.float()))
     for _ in range(20):
-        for _, stream, out, alone, args, lse in sides:
+        for _, stream, out, alone, args, (lse, kw) in sides:
             with torch.cuda.stream(stream):
-                gpu_ops.chunk_attn(*args, out, lse)
+                gpu_ops.chunk_attn(*args, out, lse, **kw)
     torch.cuda.synchronize()
     for _, stream, out, alone, *_ in sides:
         assert torch.equal(torch.nan_to_num(out.float()), torch.nan_to_num(alone.float()))

@@ -68,12 +68,13 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
   const int cta = blockIdx.x;
   const int D = p.D, nvec = D / VE;
 
+  griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
   if (tid == 0) p.cuts[cta].nparts = 0;
   Walk walk(p);
   if (!walk.init<kThreads>(&scratch, cta, kMinPer)) return;
   Walk::Seg g;
   while (walk.next(g)) {
-    const Req rq = walk.seg_q;
+    const Req rq = walk.rq;
     const int tok0 = g.tile0 * p.tq;
     const int rows = min(p.tq, rq.qlen - tok0) * p.G;
     // the query rows as fp32 (zeros behind them and behind D)

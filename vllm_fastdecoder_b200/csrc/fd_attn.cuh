@@ -124,16 +124,19 @@ struct Sched {
   struct Seg {
     int kh, tile0;   // kv head, first query tile of the item
     bool pair;
-    int n, j0, j1;   // key tiles of the item, and of this segment
+    int j0, j1;      // key tiles of this segment
     bool whole;
     int nparts;      // slot 1 segments: parts of the cut item
   };
 
   const AttnParams& p;
-  long long p0, p1, per;  // this CTA's range, and every CTA's length
-  long long s;            // position of the current item
+  // positions relative to the start of this CTA's range (the current item may
+  // have begun before it): 32 bits, the line itself has 64
+  int len, per;  // positions of this CTA, and of every CTA
+  int s;         // the current item
   int r, kh, item;
-  Req rq;
+  Req rq;        // of request r
+  bool behind;   // the current item has been returned: step to the next one first
 
   __device__ __forceinline__ Sched(const AttnParams& params) : p(params) {}
 
@@ -199,7 +202,7 @@ struct Sched {
   __device__ bool init(Scratch* sc, int c, int min_per) {
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kWarps = NT / 32;
-    long long total = 0, mine = 0, mine_at = 0, per_head = 0;
+    long long total = 0, mine = 0, mine_at = 0, per_head = 0, p0 = 0;
     Req mine_rq = {0, 0, 0, 0};
     // pass 0 adds up all requests, pass 1 finds this CTA's (from the values
     // that pass 0 left when one round holds all requests)
@@ -240,11 +243,11 @@ struct Sched {
       }
       if (pass == 0) {
         total = carry;
-        per = quot(total + p.ctas - 1, p.ctas);
+        per = (int)quot(total + p.ctas - 1, p.ctas);
         if (per < min_per) per = min_per;
         p0 = (long long)c * per;
-        p1 = min(p0 + per, total);
         if (p0 >= total) return false;
+        len = (int)min((long long)per, total - p0);
       }
     }
     __syncthreads();
@@ -269,59 +272,63 @@ struct Sched {
       }
       if (lane == 0) {
         sc->item = lo;
-        sc->item_start = p0 - x + at;
+        sc->item_start = at - x;
       }
     }
     __syncthreads();
     item = sc->item;
-    s = sc->item_start;
+    s = (int)sc->item_start;
+    behind = false;
     return true;
   }
 
-  // The next segment of this CTA's range.
+  // The next segment of this CTA's range.  (Stepping on is left to the next
+  // call: it may read the next request's lengths, which the first segment's
+  // loads need not wait for.)
   __device__ __forceinline__ bool next(Seg& g) {
-    while (s < p1) {
+    while (true) {
+      if (behind) {
+        s += kW + (is_pair(p, rq, item) ? 2 : 1) * ntiles(p, rq, item_end(p, rq, item));
+        if (++item == items(p, rq)) {
+          item = 0;
+          if (++kh == p.KVH) {
+            kh = 0;
+            while (s < len) {  // the next request with work
+              rq = load_req(p, ++r);
+              if (rq.qlen > 0) break;
+            }
+          }
+        }
+      }
+      if (s >= len) return false;
+      behind = true;
       const bool pr = is_pair(p, rq, item);
       const int u = pr ? 2 : 1;
       const int n = ntiles(p, rq, item_end(p, rq, item));
-      const long long a = p0 - s - kW, b = p1 - s - kW;
+      const int a = -s - kW, b = len - s - kW;
       // tile j belongs to the range that holds position s + kW + u j
-      g.j0 = (int)max(0ll, min((long long)n, (a + u - 1) >> (u - 1)));
-      g.j1 = (int)max(0ll, min((long long)n, (b + u - 1) >> (u - 1)));
-      g.n = n;
+      g.j0 = max(0, min(n, (a + u - 1) >> (u - 1)));
+      g.j1 = max(0, min(n, (b + u - 1) >> (u - 1)));
       g.kh = kh;
       g.tile0 = (kPairs ? 2 : 1) * item;
       g.pair = pr;
       g.whole = g.j0 == 0 && g.j1 == n;
       g.nparts = 0;
-      if (!g.whole && g.j0 == 0 && g.j1 > 0) {
-        const long long last = s + kW + (long long)u * (n - 1);
-        g.nparts = (int)(quot(last, per) - quot(p0, per)) + 1;
-      }
-      const bool has = g.j0 < g.j1 || (n == 0 && s >= p0);
-      seg_q = rq;
-      s += kW + (long long)u * n;
-      if (++item == items(p, rq)) {
-        item = 0;
-        if (++kh == p.KVH) {
-          kh = 0;
-          while (s < p1) {  // the next request with work
-            rq = load_req(p, ++r);
-            if (rq.qlen > 0) break;
-          }
-        }
-      }
-      if (has) return true;
+      // the range that holds the last tile (ranges start at multiples of per)
+      if (!g.whole && g.j0 == 0 && g.j1 > 0) g.nparts = (s + kW + u * (n - 1)) / per + 1;
+      if (g.j0 < g.j1 || (n == 0 && s >= 0)) return true;
     }
-    return false;
   }
-  Req seg_q;  // the request of the segment returned last
 };
 
 // The kernels' entry points for the host code in fd_attn.cu.
 bool mma_covers(const fd_attn_args* a);
 size_t mma_workspace(const fd_attn_args* a);
 int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s);
+// At most kFewRows query rows (tokens x heads of a kv head) per request, as
+// the caller says: `rows` of them (fd_attn_rows.cu; right for more, too).
+constexpr int kFewRows = 32;
+int rows_launch(AttnParams& p, const fd_attn_args* a, int rows, cudaStream_t s);
 // Joins the cut items: `rows` rows per item at most.
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s);
 

@@ -39,19 +39,13 @@
 
 #include <type_traits>
 
-#include "fd_attn.cuh"
-#include "fd_decode.cuh"
-#include "fd_tcgen05.cuh"
+#include "fd_attn_mma.cuh"
 
 namespace fdk {
 namespace at {
 namespace mm {
 
 constexpr int kM = 128;             // rows per query tile (MMA M)
-constexpr int kKT = 128;            // keys per tile (MMA N of S, K of P.V)
-constexpr int kSub = 16;            // keys per TMA box
-constexpr int kSubs = kKT / kSub;
-constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims
 constexpr int kHalf = 64;           // keys per step of a stream
 constexpr int kWarpK = 8, kWarpMmaA = 9, kWarpV = 10, kWarpMmaB = 11;
 constexpr int kThreads = 12 * 32;
@@ -95,242 +89,6 @@ struct SegInfo {
   int pad[2];
 };
 static_assert(sizeof(SegInfo) == 64, "segment record");
-
-struct MmaParams {
-  CUtensorMap tmap_q;       // {D, H, T, 1}, box {64, G, tq, 1}
-  CUtensorMap tmap_k[2];    // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}), box {64, 1, 16, 1}
-  CUtensorMap tmap_v[2];
-  AttnParams a;
-  int q_tma, kv_tma[2];     // the view has a tensor map
-};
-
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
-  if (mbar_try_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_try_wait(bar, parity)) return true;
-    if ((it & 63u) == 0) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        set_error(err, FD_DEVERR_TIMEOUT);
-        return false;
-      }
-    }
-  }
-}
-
-// The same without suspending, for the MMA issuer.
-__device__ __forceinline__ bool poll_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
-  if (mbar_test_wait(bar, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
-  for (uint32_t it = 1;; ++it) {
-    if (mbar_test_wait(bar, parity)) return true;
-    if ((it & 255u) == 0) {
-      if (*abort_flag) return false;
-      if (globaltimer_ns() - t0 > kWaitLimitNs) {
-        set_error(err, FD_DEVERR_TIMEOUT);
-        return false;
-      }
-    }
-  }
-}
-
-// L2 policy for data that other CTAs read too.
-__device__ __forceinline__ uint64_t l2_evict_normal_policy() {
-  uint64_t pol;
-  asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
-  return pol;
-}
-
-// 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ float fmax3(float a, float b, float c) {
-  float d;
-  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-  return d;
-}
-
-// Scores from the nv-th on are not seen.
-__device__ __forceinline__ void hide(uint32_t (&r)[32], int nv) {
-#pragma unroll
-  for (int e = 0; e < 32; ++e)
-    if (e >= nv) r[e] = __float_as_uint(-INFINITY);
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 v = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&v);
-}
-
-// A ring position moved on by `by` slots.
-template <int R>
-__device__ __forceinline__ void advance(int& slot, uint32_t& phase, int by) {
-  if (by > R) {
-    phase ^= (uint32_t)(by / R) & 1u;
-    by %= R;
-  }
-  slot += by;
-  if (slot >= R) {
-    slot -= R;
-    phase ^= 1u;
-  }
-}
-
-// The products with 128-byte swizzled operands, descriptors by their low
-// words (address and leading offset, 16-byte units); the high word (stride
-// 1024 bytes, version, swizzle) is the same for all of them.
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ void umma_f16_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
-      : "memory");
-}
-__device__ __forceinline__ void umma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
-                                               uint32_t acc) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
-      "mov.b64 b, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
-      : "memory");
-}
-
-// 32 bytes in one store (both 32-byte aligned).
-__device__ __forceinline__ void stg256(void* p, const uint32_t (&v)[8]) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]),
-               "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
-// Block id of box `lane` (keys 128 j + 16 lane ..) where boxes lie within
-// blocks, -1 where there is none.  Read one tile ahead of its use.
-__device__ __forceinline__ int box_block(const AttnParams& p, int kbase, int klen, int j, int lane) {
-  const int t = j * kKT + lane * kSub;
-  if (p.bt == nullptr || p.BS % kSub != 0 || lane >= kSubs || t >= klen) return -1;
-  return p.bt[(int64_t)kbase * p.bt_stride + t / p.BS];
-}
-
-// One warp: K or V of key tile j into `dst`, completion on `bar` (bytes of
-// the TMA boxes, and lane 0's arrival once the other boxes are stored).
-template <int KD>
-__device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsigned char* dst, uint64_t* bar, int j,
-                                          int kbase, int klen, int kh, int id, int lane, uint64_t pol) {
-  const AttnParams& p = mp.a;
-  const int t = j * kKT + lane * kSub;
-  const bool boxed = p.bt == nullptr || p.BS % kSub == 0;
-  bool in = lane < kSubs && t < klen;  // the box holds a key
-  int tier = 0, blk = 0, r0 = 0;
-  bool tma = false;
-  if (in && boxed) {
-    if (p.bt == nullptr) {
-      r0 = kbase + t;
-    } else {
-      int64_t b = id;
-      if (b >= p.split) {
-        tier = 1;
-        b -= p.split;
-      }
-      r0 = t % p.BS;
-      if (b < 0 || b >= p.nblk[tier]) {
-        set_error(p.err, FD_DEVERR_BLOCK_ID);
-        in = false;
-      }
-      blk = (int)b;
-    }
-    tma = in && mp.kv_tma[tier] && (!is_v || t + kSub <= klen);
-  }
-  const unsigned tmask = __ballot_sync(0xffffffffu, tma);
-  const unsigned all = (1u << kSubs) - 1u;
-  // K boxes without a key need nothing (the mask replaces their scores)
-  unsigned rest = is_v ? all & ~tmask : __ballot_sync(0xffffffffu, in) & ~tmask;
-  if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(tmask) * (uint32_t)(Geo<KD>::kPanels * kSub * 128));
-  __syncwarp();
-  if (tma) {
-    const CUtensorMap* map = is_v ? &mp.tmap_v[tier] : &mp.tmap_k[tier];
-#pragma unroll
-    for (int x = 0; x < Geo<KD>::kPanels; ++x)
-      tma_load_4d(dst + x * kPanel + lane * kSub * 128, map, 64 * x, kh, r0, blk, bar, pol);
-  }
-  if (rest != 0u) {
-    constexpr int kCh = KD / 8;                   // 16-byte chunks per row
-    constexpr int kPer = kSub * kCh / 32;         // chunks of a box per lane
-    while (rest != 0u) {
-      const int s = __ffs(rest) - 1;
-      rest &= rest - 1u;
-      const bool box_in = __shfl_sync(0xffffffffu, (int)in, s) != 0;
-      const int box_tier = __shfl_sync(0xffffffffu, tier, s);
-      const int box_blk = __shfl_sync(0xffffffffu, blk, s);
-      const int box_r0 = __shfl_sync(0xffffffffu, r0, s);
-      uint4 v[kPer];
-#pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
-        const int key = j * kKT + s * kSub + row;
-        v[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (!box_in || key >= klen || ch * 8 >= p.D) continue;
-        int tr = box_tier, rr = box_r0 + row;
-        int64_t b = box_blk;
-        if (!boxed) {
-          b = p.bt[(int64_t)kbase * p.bt_stride + key / p.BS];
-          rr = key % p.BS;
-          tr = 0;
-          if (b >= p.split) {
-            tr = 1;
-            b -= p.split;
-          }
-          if (b < 0 || b >= p.nblk[tr]) {
-            set_error(p.err, FD_DEVERR_BLOCK_ID);
-            continue;
-          }
-        }
-        const unsigned char* base = is_v ? p.v[tr] : p.k[tr];
-        v[c] = *reinterpret_cast<const uint4*>(base + b * p.blk_sb[tr] + kh * p.head_sb[tr] +
-                                               (int64_t)rr * p.tok_sb[tr] + ch * 16);
-      }
-#pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
-        sts128(dst + (ch >> 3) * kPanel + swz(s * kSub + row, ch & 7), v[c]);
-      }
-    }
-    fence_proxy_async_smem();  // the stores before the tensor cores read the slot
-  }
-  __syncwarp();
-  if (lane == 0) mbar_arrive(bar);
-}
-
-// One warp: the query rows of one tile into `dst` without TMA.
-template <int KD>
-__device__ __forceinline__ void load_q(const AttnParams& p, unsigned char* dst, int kh, int tok, int ntok, int lane) {
-  constexpr int kCh = KD / 8;
-  for (int idx = lane; idx < ntok * p.G * kCh; idx += 32) {
-    const int row = idx / kCh, ch = idx % kCh;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (ch * 8 < p.D)
-      v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(tok + row / p.G) * p.q_st +
-                                          (int64_t)(kh * p.G + row % p.G) * p.q_sh + ch * 16);
-    sts128(dst + (ch >> 3) * kPanel + swz(row, ch & 7), v);
-  }
-  fence_proxy_async_smem();
-}
 
 // The end of a segment for one softmax warp of stream x: o and lse of its
 // rows, or their partials.  A pair's stream has its own tile and all dims; in
@@ -465,35 +223,15 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
 
+  griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
+  init_barriers(q_full, Ge::kNumBars, [&](int i) -> uint32_t {
+    uint64_t* b = q_full + i;
+    if (b == q_empty || b == o_both || b == drain || (b >= k_empty && b < v_full) || (b >= v_empty && b < s_full)) return 2;
+    return b >= p_full && b < o_full ? 4 : b == o_empty || b == ml_full ? 8 : b >= seg_empty ? kSegReaders : 1;
+  });
   if (threadIdx.x == 0) {
     p.cuts[cta].nparts = 0;
     misc[0] = 0;
-    mbar_init(q_full, 1);
-    mbar_init(q_empty, 2);
-    for (int s = 0; s < kRingK; ++s) {
-      mbar_init(&k_full[s], 1);
-      mbar_init(&k_empty[s], 2);
-    }
-    for (int s = 0; s < kRingV; ++s) {
-      mbar_init(&v_full[s], 1);
-      mbar_init(&v_empty[s], 2);
-    }
-    for (int s = 0; s < 4; ++s) {
-      mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 4);
-    }
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(&o_full[s], 1);
-    }
-    mbar_init(o_both, 2);
-    mbar_init(o_empty, 8);
-    mbar_init(ml_full, 8);
-    for (int s = 0; s < kSegs; ++s) {
-      mbar_init(&seg_full[s], 1);
-      mbar_init(&seg_empty[s], kSegReaders);
-    }
-    mbar_init(drain, 2);
-    fence_barrier_init();
   }
   Walk walk(p);
   static_assert(sizeof(Walk::Scratch) <= 2 * kM * 8, "scratch of the schedule");
@@ -526,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       if (nseg >= kSegs)
         ok = __all_sync(0xffffffffu, wait_or_abort(&seg_empty[ss], (uint32_t)(nseg / kSegs - 1) & 1u, misc, p.err));
       if (!ok) break;
-      const Req rq = walk.seg_q;
+      const Req rq = walk.rq;
       const int tok0 = g.tile0 * p.tq;
       if (lane == 0) {
         SegInfo& i = segs[ss];
@@ -580,7 +318,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         }
       } else {
         for (int x = 0; x < nt; ++x)
-          load_q<KD>(p, smem + x * kTile, g.kh, rq.qst + tok0 + x * p.tq, min(p.tq, rq.qlen - tok0 - x * p.tq), lane);
+          load_q<KD>(p, smem + x * kTile, kPanel, g.kh, rq.qst + tok0 + x * p.tq, min(p.tq, rq.qlen - tok0 - x * p.tq), lane);
         __syncwarp();
         if (lane == 0) mbar_arrive(q_full);
       }
@@ -886,6 +624,25 @@ int launch(const MmaParams& mp, cudaStream_t s) {
                                "fd_attn_mma_kernel launch");
 }
 
+void encode_maps(MmaParams& mp, const fd_attn_args* a) {
+  const AttnParams& p = mp.a;
+  const int D = p.D;
+  mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
+  for (int t = 0; t < 2; ++t) {
+    if (p.nblk[t] == 0 || p.host[t]) continue;
+    const bool cross = p.bt == nullptr;
+    if (cross && p.nblk[t] > 0x7fffffff) continue;  // rows by 16-byte loads
+    if (!cross && p.BS % kSub != 0) continue;
+    const int rows = cross ? (int)p.nblk[t] : p.BS;
+    const int64_t blocks = cross ? 1 : p.nblk[t];
+    const int64_t blk_sb = cross ? p.tok_sb[t] * rows : p.blk_sb[t];
+    mp.kv_tma[t] = encode_kv_map(&mp.tmap_k[t], p.k[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
+                                 blk_sb, kSub, true) &&
+                   encode_kv_map(&mp.tmap_v[t], p.v[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
+                                 blk_sb, kSub, true);
+  }
+}
+
 }  // namespace mm
 
 bool mma_covers(const fd_attn_args* a) {
@@ -898,6 +655,10 @@ size_t mma_workspace(const fd_attn_args* a) {
 }
 
 int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
+  // few query rows per request and kv head: the kernel made for them, which
+  // spends no softmax on rows that are not there
+  const int64_t rows = (int64_t)(a->max_q_len > 0 && a->max_q_len < p.T ? a->max_q_len : p.T) * p.G;
+  if (rows <= kFewRows) return rows_launch(p, a, (int)rows, s);
   int dev = 0, sms = 0;
   int st = fdh::device_sms(&dev, &sms);
   if (st != FD_OK) return st;
@@ -910,21 +671,8 @@ int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
   p.ctas = sms < mm::kMaxCtas ? sms : mm::kMaxCtas;
   mm::MmaParams mp{};
   const int D = p.D;
-  mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
-  for (int t = 0; t < 2; ++t) {
-    if (p.nblk[t] == 0 || p.host[t]) continue;
-    const bool cross = p.bt == nullptr;
-    if (cross && p.nblk[t] > 0x7fffffff) continue;  // rows by 16-byte loads
-    if (!cross && p.BS % mm::kSub != 0) continue;
-    const int rows = cross ? (int)p.nblk[t] : p.BS;
-    const int64_t blocks = cross ? 1 : p.nblk[t];
-    const int64_t blk_sb = cross ? p.tok_sb[t] * rows : p.blk_sb[t];
-    mp.kv_tma[t] = encode_kv_map(&mp.tmap_k[t], p.k[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
-                                 blk_sb, mm::kSub, true) &&
-                   encode_kv_map(&mp.tmap_v[t], p.v[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
-                                 blk_sb, mm::kSub, true);
-  }
   mp.a = p;
+  mm::encode_maps(mp, a);
   if (a->dtype == FD_DTYPE_BF16)
     st = D <= 64 ? mm::launch<__nv_bfloat16, 64>(mp, s) : mm::launch<__nv_bfloat16, 128>(mp, s);
   else

@@ -1,0 +1,583 @@
+// Chunk and cross attention of few query rows (at most 32 per request and kv
+// head: single tokens, draft tokens) on the tensor cores: fp16 and bf16, head
+// sizes 64 to 128.
+//
+// Such calls are bound by the bytes of K and V, as long as the work per key
+// tile stays below its load time (0.7 us for 32 KB at an SM's share of HBM).
+// With the queries as the 128 rows of an MMA tile (fd_attn_mma.cu) it does
+// not: a softmax thread has a row's 128 exponentials per tile however few rows
+// are real.  So the products are turned over:
+//   S^T [128 keys x N] = K . Q^T,  P = 2^(scale log2(e) S - m),  l = sum P,
+//   O^T [dims x N] += V^T . P^T,   N = 16 or 32 query rows,
+// a softmax thread has one KEY and N exponentials, K and V are the MMA's A
+// operands as they lie in shared memory, and the rows of O^T are dims, so a
+// warp's output stores are whole lines.  The reference m of a column moves
+// only when some score passes it by more than 2^8 (then, and on a segment's
+// first tile, the 128 threads take the column's maximum together and rescale
+// O); the sums l stay with their threads until the segment's end.
+//
+// A CTA walks its range of the schedule (fd_attn.cuh); seven warps: 0-3
+// softmax, 4 schedule, Q and K tiles, 5 V tiles, 6 (one thread) the MMAs,
+// q.K^T two tiles ahead of P.V over two S and two P buffers.  Heads of 64 dims
+// take half of the shared memory, and two CTAs share an SM: one's loads run
+// on while the other changes from one request to the next.
+// Scores, sums and O are fp32; P is rounded to the input type (the tensor
+// core's operand type), the result once.  Every wait is bounded; the four
+// softmax warps agree at their barriers on going on.
+
+#include <math.h>
+
+#include <type_traits>
+
+#include "fd_attn_mma.cuh"
+
+namespace fdk {
+namespace at {
+namespace rw {
+
+using namespace mm;
+
+constexpr int kWarpK = 4, kWarpV = 5, kWarpMma = 6;
+constexpr int kThreads = 7 * 32;
+constexpr int kSoft = 4 * 32;       // softmax threads
+constexpr int kSegs = 4;            // segments in flight between the roles
+constexpr int kSegReaders = 6;      // MMA thread, V producer, four softmax warps
+constexpr int kMaxCtas = 320;
+constexpr int kFixed = 2;           // an item's fixed cost in key tiles
+constexpr int kMinPer = 4;          // least positions of a CTA
+constexpr int kTmemCols = 128;      // S [0, 32), [32, 64), O [64, 96)
+constexpr int kOcol = 64;
+typedef Sched<kKT, false, kFixed> Walk;
+
+template <int KD, int N>
+struct Geo {
+  static constexpr int kPanels = KD / 64;
+  static constexpr int kTile = kPanels * kPanel;
+  static constexpr int kRingK = KD == 64 && N == 32 ? 2 : 3;
+  static constexpr int kRingV = 3;
+  static constexpr int kQ = kPanels * N * 128;   // one Q buffer
+  static constexpr int kP = 2 * N * 128;         // one P buffer: two panels of 64 keys
+  static constexpr int kOffV = kRingK * kTile;
+  static constexpr int kOffQ = kOffV + kRingV * kTile;
+  static constexpr int kOffP = kOffQ + 2 * kQ;
+  static constexpr int kOffBar = kOffP + 2 * kP;
+  // k full/empty, v full/empty, q full/empty[2], s_full[2], p_full[2], o_full, o_empty, seg full/empty, drain
+  static constexpr int kNumBars = 2 * kRingK + 2 * kRingV + 4 + 2 + 2 + 2 + 2 * kSegs + 1;
+  static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
+  static constexpr int kOffRed = kOffSeg + kSegs * 64;   // [4 warps][N] maxima, then sums (before that: Walk::Scratch)
+  static constexpr int kOffM = kOffRed + 4 * N * 4 + 512;  // [N] m, then [N] factors of l and O
+  static constexpr int kOffMisc = kOffM + 2 * N * 4;     // abort flag, TMEM address
+  static constexpr int kSmem = kOffMisc + 16;
+  static_assert(kSmem <= (KD == 64 ? 113 : 227) * 1024, "smem budget");
+};
+
+struct SegInfo {
+  int live;    // 0: no more segments
+  int j0, m;   // first key tile, key tiles
+  int tok0;    // first query token of the item within the request
+  int qst, qlen, klen, kbase, kh;
+  int slot;    // -1: whole, else its slot of the partials
+  int pad[6];
+};
+static_assert(sizeof(SegInfo) == 64, "segment record");
+
+// Barrier of the softmax threads that also tells whether any / all of them say so.
+__device__ __forceinline__ bool sync_or(bool v) {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\t"
+      "barrier.cta.red.or.pred p, 1, %2, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r)
+      : "r"((uint32_t)v), "n"(kSoft)
+      : "memory");
+  return r != 0;
+}
+__device__ __forceinline__ bool sync_and(bool v) { return !sync_or(!v); }
+
+// Maximum over the warp.
+__device__ __forceinline__ float warp_max(float v) {
+  float r;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+  return r;
+}
+
+// The N sums over the warp's lanes of v[0 .. N - 1]: lane c (of every 32 or,
+// with N = 16, of either half) ends with the sum of column c % N.
+template <int N>
+__device__ __forceinline__ float column_sum(float (&v)[N], int lane) {
+#pragma unroll
+  for (int w = N / 2; w >= 1; w >>= 1) {
+    const bool up = (lane & w) != 0;
+#pragma unroll
+    for (int i = 0; i < w; ++i) {
+      const float give = up ? v[i] : v[i + w], keep = up ? v[i + w] : v[i];
+      v[i] = keep + __shfl_xor_sync(0xffffffffu, give, w);
+    }
+  }
+  float s = v[0];
+  if (N == 16) s += __shfl_xor_sync(0xffffffffu, s, 16);
+  return s;
+}
+
+// N consecutive TMEM columns of this warp's lanes.
+__device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[16]) { tmem_ld16_nowait(t, r); }
+__device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[32]) { tmem_ld32_nowait(t, r); }
+__device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[16]) { tmem_st16(t, r); }
+__device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[32]) { tmem_st32(t, r); }
+
+__device__ __forceinline__ void tmem_ld4_nowait(uint32_t t, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(t));
+}
+
+template <typename T, int KD, int N>
+__global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kernel(const __grid_constant__ MmaParams mp) {
+  typedef Geo<KD, N> Ge;
+  constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingV = Ge::kRingV;
+  constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
+  constexpr uint32_t kIdQK = instr_desc(kBF16, false, kKT, N);
+  constexpr uint32_t kIdPV = instr_desc(kBF16, true, 128, N);  // V: MN-major A
+  // V's second 64 dims; heads of 64 dims have the first ones twice (rows 64 .. 127 of O^T are not read)
+  constexpr uint32_t kLbo = KD == 128 ? (uint32_t)(kPanel >> 4) : 0u;
+  const AttnParams& p = mp.a;
+  extern __shared__ __align__(1024) unsigned char smem[];
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);
+  uint64_t* k_empty = k_full + kRingK;     // MMA commit after the q.K^T that read it
+  uint64_t* v_full = k_empty + kRingK;
+  uint64_t* v_empty = v_full + kRingV;     // MMA commit after the P.V that read it
+  uint64_t* q_full = v_empty + kRingV;     // [2]
+  uint64_t* q_empty = q_full + 2;          // [2] MMA commit after a segment's last q.K^T
+  uint64_t* s_full = q_empty + 2;          // [2] MMA commit: S of a tile
+  uint64_t* p_full = s_full + 2;           // [2] the four softmax warps wrote P
+  uint64_t* o_full = p_full + 2;           // MMA commit after a segment's last P.V
+  uint64_t* o_empty = o_full + 1;          // the four softmax warps are done with the segment
+  uint64_t* seg_full = o_empty + 1;        // [kSegs]
+  uint64_t* seg_empty = seg_full + kSegs;  // [kSegs]
+  uint64_t* drain = seg_empty + kSegs;
+  SegInfo* segs = reinterpret_cast<SegInfo*>(smem + Ge::kOffSeg);
+  float* red = reinterpret_cast<float*>(smem + Ge::kOffRed);
+  float* m_sh = reinterpret_cast<float*>(smem + Ge::kOffM);
+  float* f_sh = m_sh + N;
+  volatile int* misc = reinterpret_cast<volatile int*>(smem + Ge::kOffMisc);  // [0] abort, [1] TMEM address
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int cta = blockIdx.x;
+  griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
+  init_barriers(k_full, Ge::kNumBars, [&](int i) -> uint32_t {
+    uint64_t* b = k_full + i;
+    return b >= p_full && b < o_full ? 4 : b == o_empty ? 4 : b >= seg_empty && b < drain ? kSegReaders : 1;
+  });
+  if (threadIdx.x == 0) {
+    p.cuts[cta].nparts = 0;
+    misc[0] = 0;
+  }
+  // rows of the Q buffers that no load writes (behind the tile's tokens) stay 0
+  for (int x = threadIdx.x; x < 2 * Ge::kQ / 16; x += kThreads) sts128(smem + Ge::kOffQ + 16 * x, make_uint4(0, 0, 0, 0));
+  fence_proxy_async_smem();
+  Walk walk(p);
+  static_assert(sizeof(Walk::Scratch) <= 4 * N * 4 + 512, "scratch of the schedule");
+  if (!walk.init<kThreads>(reinterpret_cast<Walk::Scratch*>(red), cta, kMinPer)) return;  // all threads alike
+  if (warp == kWarpMma) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
+                     smem_u32(smem + Ge::kOffMisc + 4)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = (uint32_t)misc[1];
+
+  if (warp == kWarpK) {
+    // ------------------------------------------------ schedule, Q and K tiles
+    const uint64_t pol = l2_evict_first_policy();
+    int nseg = 0, nq = 0, st = 0;
+    uint32_t tiles = 0, ph = 0;
+    bool ok = true;
+    Walk::Seg g;
+    while (ok) {
+      const bool more = walk.next(g);
+      const Req rq = walk.rq;
+      int id = more && g.j0 < g.j1 ? box_block(p, rq.kbase, rq.klen, g.j0, lane) : -1;
+      const int ss = nseg % kSegs;
+      if (nseg >= kSegs)
+        ok = __all_sync(0xffffffffu, wait_or_abort(&seg_empty[ss], (uint32_t)(nseg / kSegs - 1) & 1u, misc, p.err));
+      if (!ok) break;
+      const int tok0 = g.tile0 * p.tq;
+      if (lane == 0) {
+        SegInfo& i = segs[ss];
+        i.live = more;
+        if (more) {
+          i.j0 = g.j0;
+          i.m = g.j1 - g.j0;
+          i.tok0 = tok0;
+          i.qst = rq.qst;
+          i.qlen = rq.qlen;
+          i.klen = rq.klen;
+          i.kbase = rq.kbase;
+          i.kh = g.kh;
+          i.slot = g.whole ? -1 : 2 * cta + (g.j0 > 0 ? 0 : 1);
+          if (g.nparts > 0) p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, min(p.tq, rq.qlen - tok0) * p.G, g.kh};
+        }
+        mbar_arrive(&seg_full[ss]);
+      }
+      __syncwarp();
+      ++nseg;
+      if (!more) break;
+      if (g.j0 >= g.j1) continue;  // no key is seen: the softmax warps write zeros
+      const int qb = nq & 1;
+      if (nq >= 2 && !__all_sync(0xffffffffu, wait_or_abort(&q_empty[qb], (uint32_t)(nq / 2 - 1) & 1u, misc, p.err))) {
+        ok = false;
+        break;
+      }
+      ++nq;
+      unsigned char* sq = smem + Ge::kOffQ + qb * Ge::kQ;
+      if (mp.q_tma) {
+        if (lane == 0) {
+          mbar_expect_tx(&q_full[qb], (uint32_t)(Ge::kPanels * p.tq * p.G * 128));
+          for (int c = 0; c < Ge::kPanels; ++c)
+            tma_load_4d(sq + c * N * 128, &mp.tmap_q, 64 * c, g.kh * p.G, rq.qst + tok0, 0, &q_full[qb], 0ull);
+          mbar_arrive(&q_full[qb]);
+        }
+      } else {
+        load_q<KD>(p, sq, N * 128, g.kh, rq.qst + tok0, min(p.tq, rq.qlen - tok0), lane);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&q_full[qb]);
+      }
+      for (int j = g.j0; j < g.j1; ++j) {
+        const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
+        if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
+        if (!ok) break;
+        load_tile<KD>(mp, false, smem + st * kTile, &k_full[st], j, rq.kbase, rq.klen, g.kh, id, lane, pol);
+        id = id_next;
+        ++tiles;
+        if (++st == kRingK) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) misc[0] = 1;
+    // no copy of this warp is in flight when the CTA ends
+    for (uint32_t s = 0; s < (uint32_t)kRingK && s < tiles; ++s) {
+      const uint32_t last = s + kRingK * ((tiles - 1 - s) / kRingK);
+      mbar_wait(&k_full[s], (last / kRingK) & 1u, p.err);
+    }
+    for (int b = 0; b < 2 && b < nq; ++b) mbar_wait(&q_full[b], (uint32_t)((nq - 1 - b) / 2) & 1u, p.err);
+  } else if (warp == kWarpV) {
+    // ------------------------------------------------ V tiles
+    const uint64_t pol = l2_evict_first_policy();
+    int st = 0;
+    uint32_t tiles = 0, ph = 0;
+    bool ok = true;
+    for (int nseg = 0; ok; ++nseg) {
+      const int ss = nseg % kSegs;
+      ok = __all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
+      if (!ok) break;
+      const SegInfo i = segs[ss];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
+      if (!i.live) break;
+      int id = i.m > 0 ? box_block(p, i.kbase, i.klen, i.j0, lane) : -1;
+      for (int j = i.j0; j < i.j0 + i.m; ++j) {
+        const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
+        if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
+        if (!ok) break;
+        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.kbase, i.klen, i.kh, id, lane, pol);
+        id = id_next;
+        ++tiles;
+        if (++st == kRingV) {
+          st = 0;
+          ph ^= 1u;
+        }
+      }
+    }
+    if (!ok) misc[0] = 1;
+    for (uint32_t s = 0; s < (uint32_t)kRingV && s < tiles; ++s) {
+      const uint32_t last = s + kRingV * ((tiles - 1 - s) / kRingV);
+      mbar_wait(&v_full[s], (last / kRingV) & 1u, p.err);
+    }
+  } else if (warp == kWarpMma) {
+    // ------------------------------------------------ MMA issuer
+    if (lane == 0) {
+      const uint32_t base = smem_u32(smem) >> 4;
+      int ks_ = 0, vs_ = 0, nq = 0;
+      uint32_t kp = 0, vp = 0, pp = 0;  // ring phases; parities of p_full's two buffers
+      bool ok = true;
+      for (int nseg = 0; ok; ++nseg) {
+        const int ss = nseg % kSegs;
+        ok = poll_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err);
+        if (!ok) break;
+        const int live = segs[ss].live, m = segs[ss].m;
+        mbar_arrive(&seg_empty[ss]);
+        if (!live) break;
+        const int qb = nq & 1;
+        const uint32_t q_lo = base + (uint32_t)((Ge::kOffQ + qb * Ge::kQ) >> 4) + (1u << 16);
+        // q.K^T of tile t; tile m is none: its commit tells that the P.V before it are done
+        auto qk = [&](int t) {
+          if (t < m) {
+            if (!poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
+            tc_fence_after();
+            const uint32_t k_lo = base + (uint32_t)((ks_ * kTile) >> 4) + (1u << 16);
+#pragma unroll
+            for (int ks = 0; ks < KD / 16; ++ks)
+              umma_f16_lo(tmem + 32 * (t & 1), k_lo + (uint32_t)(((ks >> 2) * kPanel + (ks & 3) * 32) >> 4),
+                          q_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), kIdQK, ks > 0 ? 1u : 0u);
+          }
+          umma_commit(&s_full[t & 1]);
+          if (t < m) {
+            umma_commit(&k_empty[ks_]);
+            advance<kRingK>(ks_, kp, 1);
+            if (t == m - 1) umma_commit(&q_empty[qb]);
+          }
+          return true;
+        };
+        if (m > 0) {
+          ok = poll_or_abort(&q_full[qb], (uint32_t)(nq / 2) & 1u, misc, p.err);
+          ++nq;
+          ok = ok && qk(0) && qk(1);
+        }
+        // the last segment's O has been read
+        if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
+        for (int t = 0; ok && t < m; ++t) {
+          const int h = t & 1;
+          ok = poll_or_abort(&v_full[vs_], vp, misc, p.err) && poll_or_abort(&p_full[h], (pp >> h) & 1u, misc, p.err);
+          if (!ok) break;
+          pp ^= 1u << h;
+          tc_fence_after();
+          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (kLbo << 16);
+          const uint32_t p_lo = base + (uint32_t)((Ge::kOffP + h * Ge::kP) >> 4) + (1u << 16);
+#pragma unroll
+          for (int ks = 0; ks < kKT / 16; ++ks)
+            umma_f16_lo(tmem + kOcol, v_lo + (uint32_t)(ks * 2048 >> 4),
+                        p_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), kIdPV,
+                        (t > 0 || ks > 0) ? 1u : 0u);
+          if (t + 2 <= m) ok = qk(t + 2);
+          umma_commit(&v_empty[vs_]);
+          advance<kRingV>(vs_, vp, 1);
+        }
+        if (ok && m > 0) umma_commit(o_full);
+      }
+      if (!ok) misc[0] = 1;
+      umma_commit(drain);  // all MMAs complete before TMEM is released
+      mbar_wait(drain, 0u, p.err);
+    }
+    __syncwarp();
+  } else {
+    // ------------------------------------------------ softmax: one key per thread, then one dim
+    const int tid = threadIdx.x;
+    const uint32_t lanes = (uint32_t)(warp * 32) << 16;
+    uint32_t ph = 0;  // phase parities of s_full (bits 0, 1) and o_full (2)
+    bool ok = true;
+    for (int nseg = 0;; ++nseg) {
+      const int ss = nseg % kSegs;
+      ok = sync_and(wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
+      if (!ok) break;
+      const SegInfo& seg = segs[ss];  // stays until this segment's end
+      if (!seg.live) break;
+      const int m_tiles = seg.m;
+      // column n (token tok0 + n / G) sees key j: j <= first + n / G, so n >= (j - first) G
+      const int first = p.bt != nullptr ? seg.klen - seg.qlen + seg.tok0 : seg.klen - 1;
+      float l[N];
+#pragma unroll
+      for (int n = 0; n < N; ++n) l[n] = 0.f;
+      for (int t = 0; t < m_tiles; ++t) {
+        const int h = t & 1;
+        ok = wait_or_abort(&s_full[h], (ph >> h) & 1u, misc, p.err);
+        ph ^= 1u << h;
+        __syncwarp();
+        tc_fence_after();
+        uint32_t s[N];
+        tmem_load(tmem + lanes + 32 * h, s);
+        tmem_wait_ld();
+        const int key0 = (seg.j0 + t) * kKT;
+        if (key0 + kKT - 1 > first) {
+          const int over = key0 + tid - first;
+          const int from = over <= 0 ? 0 : p.bt != nullptr ? over * p.G : N;
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            if (n < from) s[n] = __float_as_uint(-INFINITY);
+        }
+        // does some score pass its column's reference by more than 2^8?
+        bool past = t == 0;
+        if (t > 0) {
+#pragma unroll
+          for (int n = 0; n < N; n += 4) {
+            const float4 m = *reinterpret_cast<const float4*>(m_sh + n);
+            past |= fmaf(__uint_as_float(s[n]), p.sl2, -m.x) > 8.f;
+            past |= fmaf(__uint_as_float(s[n + 1]), p.sl2, -m.y) > 8.f;
+            past |= fmaf(__uint_as_float(s[n + 2]), p.sl2, -m.z) > 8.f;
+            past |= fmaf(__uint_as_float(s[n + 3]), p.sl2, -m.w) > 8.f;
+          }
+        }
+        if (sync_or(past || !ok)) {
+          // O takes the earlier tiles: the commit of the next S follows the last one's P.V
+          ok = ok && (t == 0 || wait_or_abort(&s_full[h ^ 1], (ph >> (h ^ 1)) & 1u, misc, p.err));
+          __syncwarp();
+#pragma unroll
+          for (int n = 0; n < N; ++n) {
+            const float mx = warp_max(__uint_as_float(s[n]));
+            if (lane == 0) red[warp * N + n] = mx;
+          }
+          if (!sync_and(ok)) {
+            ok = false;
+            break;
+          }
+          if (tid < N) {
+            const float mx = fmaxf(fmaxf(red[tid], red[N + tid]), fmaxf(red[2 * N + tid], red[3 * N + tid])) * p.sl2;
+            const float old = t == 0 ? -INFINITY : m_sh[tid];
+            const bool set = old == -INFINITY, grow = !set && mx > old + 8.f;
+            f_sh[tid] = grow ? exp2f(old - mx) : 1.f;
+            m_sh[tid] = set || grow ? mx : old;
+          }
+          sync_or(false);
+          if (t > 0) {
+            tc_fence_after();
+            uint32_t o[N];
+            tmem_load(tmem + lanes + kOcol, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int n = 0; n < N; ++n) {
+              l[n] *= f_sh[n];
+              o[n] = __float_as_uint(__uint_as_float(o[n]) * f_sh[n]);
+            }
+            tmem_store(tmem + lanes + kOcol, o);
+            tmem_wait_st();
+          }
+        }
+        // P: row n of the B operand, key `tid`
+        unsigned char* pb = smem + Ge::kOffP + h * Ge::kP + (tid >> 6) * (N * 128) + (tid & 7) * 2;
+        const int ch = (tid & 63) >> 3;
+#pragma unroll
+        for (int n = 0; n < N; n += 4) {
+          const float4 m4 = *reinterpret_cast<const float4*>(m_sh + n);
+          const float m[4] = {m4.x, m4.y, m4.z, m4.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float e = ex2_approx(fmaf(__uint_as_float(s[n + i]), p.sl2, m[i] == -INFINITY ? 0.f : -m[i]));
+            l[n + i] += e;
+            *reinterpret_cast<T*>(pb + swz(n + i, ch)) = Dt<T>::narrow(e);
+          }
+        }
+        fence_proxy_async_smem();  // P before the tensor cores read it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[h]);
+      }
+      if (!ok) break;
+      // the segment's end: sums over the keys' threads, then rows
+      if (m_tiles > 0) {
+        const int e = m_tiles & 1;  // the commit of tile m_tiles, which holds no scores
+        ok = wait_or_abort(&s_full[e], (ph >> e) & 1u, misc, p.err) && wait_or_abort(o_full, (ph >> 2) & 1u, misc, p.err);
+        ph ^= (1u << e) | 4u;
+        __syncwarp();
+      }
+      const float sum = column_sum<N>(l, lane);
+      if (lane < N) red[warp * N + lane] = sum;
+      if (!sync_and(ok)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      const int rows = min(p.tq, seg.qlen - seg.tok0) * p.G;
+      const int slot = seg.slot;
+      const int64_t tok0 = seg.qst + seg.tok0;
+      if (tid < N) {
+        const float lt = red[tid] + red[N + tid] + red[2 * N + tid] + red[3 * N + tid];
+        const float mt = m_tiles > 0 ? m_sh[tid] : -INFINITY;
+        f_sh[tid] = slot >= 0 ? 1.f : lt > 0.f ? 1.f / lt : 0.f;
+        if (tid < rows) {
+          if (slot >= 0)
+            reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * N + tid] = make_float2(mt, lt);
+          else if (p.lse != nullptr)
+            p.lse[(seg.kh * p.G + tid % p.G) * p.lse_sh + (tok0 + tid / p.G) * p.lse_st] =
+                lt > 0.f ? (mt + log2f(lt)) * kLn2 : -INFINITY;
+        }
+      }
+      sync_or(false);
+      // thread `tid` has dim `tid` of every row; four rows at a time
+      unsigned char* po = p.out + tok0 * p.o_st + (int64_t)(seg.kh * p.G) * p.o_sh + tid * 2;
+      float* pp = p.part_o + (((int64_t)slot * (p.D / 4) + (tid >> 2)) * N) * 4 + (tid & 3);
+      int hg = 0;
+#pragma unroll 1
+      for (int n = 0; n < rows; n += 4) {
+        uint32_t o[4];
+        if (m_tiles > 0) {
+          tmem_ld4_nowait(tmem + lanes + kOcol + n, o);
+          tmem_wait_ld();
+        }
+        const float4 f = *reinterpret_cast<const float4*>(f_sh + n);
+        const float w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float v = m_tiles > 0 ? __uint_as_float(o[i]) * w[i] : 0.f;
+          const bool live = tid < p.D && n + i < rows;
+          if (live && slot >= 0) pp[4 * (n + i)] = v;
+          if (live && slot < 0) *reinterpret_cast<T*>(po + hg * p.o_sh) = Dt<T>::narrow(v);
+          if (++hg == p.G) {
+            hg = 0;
+            po += p.o_st;
+          }
+        }
+        __syncwarp();  // the TMEM loads are the whole warp's
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(o_empty);
+        mbar_arrive(&seg_empty[ss]);
+      }
+    }
+    if (!ok) misc[0] = 1;
+  }
+
+  // ---------------------------------------------------------------- teardown
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kWarpMma)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
+}
+
+template <typename T, int KD, int N>
+int launch(const MmaParams& mp, cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(fd_attn_rows_kernel<T, KD, N>);
+  static unsigned long long done = 0;
+  const int st = fdh::ensure_smem(kern, Geo<KD, N>::kSmem, &done);
+  if (st != FD_OK) return st;
+  return fdh::launch_maybe_pdl(kern, dim3((unsigned)mp.a.ctas), dim3(kThreads), Geo<KD, N>::kSmem, s, false, mp,
+                               "fd_attn_rows_kernel launch");
+}
+
+template <typename T>
+int launch_for(const MmaParams& mp, int N, cudaStream_t s) {
+  if (mp.a.D <= 64) return N == 16 ? launch<T, 64, 16>(mp, s) : launch<T, 64, 32>(mp, s);
+  return N == 16 ? launch<T, 128, 16>(mp, s) : launch<T, 128, 32>(mp, s);
+}
+
+}  // namespace rw
+
+int rows_launch(AttnParams& p, const fd_attn_args* a, int rows, cudaStream_t s) {
+  int dev = 0, sms = 0;
+  int st = fdh::device_sms(&dev, &sms);
+  if (st != FD_OK) return st;
+  const int N = rows <= 16 ? 16 : 32;
+  unsigned char* ws = static_cast<unsigned char*>(a->workspace);
+  p.ctas = sms * (p.D <= 64 ? 2 : 1);
+  if (p.ctas > rw::kMaxCtas) p.ctas = rw::kMaxCtas;
+  p.cuts = reinterpret_cast<Cut*>(ws);
+  p.part_ml = reinterpret_cast<float*>(ws + rw::kMaxCtas * sizeof(Cut));
+  p.part_o = p.part_ml + 2 * 2 * (size_t)rw::kMaxCtas * N;
+  p.tq = N / p.G;
+  mm::MmaParams mp{};
+  mp.a = p;
+  mm::encode_maps(mp, a);
+  st = a->dtype == FD_DTYPE_BF16 ? rw::launch_for<__nv_bfloat16>(mp, N, s) : rw::launch_for<__half>(mp, N, s);
+  if (st != FD_OK) return st;
+  return combine_launch(p, a->dtype, N, s);
+}
+
+}  // namespace at
+}  // namespace fdk
