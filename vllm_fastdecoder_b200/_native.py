@@ -205,7 +205,7 @@ SIGNATURES = {
     "fd_tables_args_bytes": (c_size_t, []),
     "fd_rope_store_kv": (c_int32, [c_void_p, c_void_p]),
     "fd_rope_args_bytes": (c_size_t, []),
-    "fd_attn_workspace_size": (c_size_t, [POINTER(FdAttnArgs)]),
+    "fd_attn_workspace_size": (c_size_t, [c_void_p]),
     "fd_chunk_attn": (c_int32, [c_void_p, c_void_p]),
     "fd_cross_attn": (c_int32, [c_void_p, c_void_p]),
     "fd_attn_args_bytes": (c_size_t, []),

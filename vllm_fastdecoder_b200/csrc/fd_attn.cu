@@ -32,20 +32,13 @@ constexpr int smem_bytes(int DP) { return ((kRows + 2 * kKeys) * (DP + 4) + kRow
 
 // Byte offset of K (and V) row j of the request for kv head kh within its tier,
 // -1 when there is none (behind klen, or a block id outside both tiers).
-__device__ __forceinline__ int64_t key_offset(const AttnParams& p, const Req& q, int kh, int j, int* tier) {
+__device__ __forceinline__ int64_t key_offset(const AttnParams& p, const Req& q, int r, int kh, int j, int* tier) {
   *tier = 0;
   if (j >= q.klen) return -1;
   if (p.bt == nullptr) return ((int64_t)q.kbase + j) * p.tok_sb[0] + kh * p.head_sb[0];
   int64_t id = p.bt[(int64_t)q.kbase * p.bt_stride + j / p.BS];
-  int t = 0;
-  if (id >= p.split) {
-    t = 1;
-    id -= p.split;
-  }
-  if (id < 0 || id >= p.nblk[t]) {
-    set_error(p.err, FD_DEVERR_BLOCK_ID);
-    return -1;
-  }
+  const int t = locate(p, r, j / p.BS, id);
+  if (t < 0) return -1;
   *tier = t;
   return id * p.blk_sb[t] + kh * p.head_sb[t] + (int64_t)(j % p.BS) * p.tok_sb[t];
 }
@@ -112,7 +105,7 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
     auto fetch = [&](int j) {  // all threads: the rows of key tile j into registers
       if (tid < kKeys) {
         int t;
-        const int64_t at = key_offset(p, rq, g.kh, j * kKeys + tid, &t);
+        const int64_t at = key_offset(p, rq, walk.r, g.kh, j * kKeys + tid, &t);
         k_row[tid] = at < 0 ? nullptr : p.k[t] + at;
         v_row[tid] = at < 0 ? nullptr : p.v[t] + at;
       }
@@ -323,11 +316,69 @@ int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
   return fdh::cuda_status(cudaLaunchKernelExC(&cfg, kern, args), "fd_attn_combine_kernel launch");
 }
 
+// Host blocks that several items read (more query rows per kv head than one
+// item has) are copied to device memory first: read in place they would cross
+// PCIe once per item, and an SM's loads do not keep them in L2.  CTA (j, r)
+// copies block j of request r, when it lies in the host tier, to block
+// r * stage_w + j of the copies.
+constexpr int kStageThreads = 256, kStageBatch = 8;
+__global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __grid_constant__ AttnParams p, int vec) {
+  const int j = blockIdx.x, r = blockIdx.y;
+  const Req q = load_req(p, r);
+  if (q.qlen <= 0 || j * (long long)p.BS >= q.klen) return;
+  const int64_t id = p.bt[(int64_t)q.kbase * p.bt_stride + j];
+  if (id < p.split || id - p.split >= p.nblk[1]) return;
+  const int rows = p.KVH * p.BS, total = 2 * rows * vec;  // K, then V
+  const int64_t src = (id - p.split) * p.blk_sb[1], dst = ((int64_t)r * p.stage_w + j) * p.blk_sb[2];
+  for (int x0 = threadIdx.x; x0 < total; x0 += kStageThreads * kStageBatch) {
+    uint4 v[kStageBatch];
+    int64_t to[kStageBatch];
+#pragma unroll
+    for (int u = 0; u < kStageBatch; ++u) {
+      const int x = x0 + u * kStageThreads;
+      to[u] = -1;
+      if (x >= total) continue;
+      const int row = x / vec % rows, c = x % vec, h = row / p.BS, t = row - h * p.BS;
+      const unsigned char* base = x < rows * vec ? p.k[1] : p.v[1];
+      v[u] = *reinterpret_cast<const uint4*>(base + src + h * p.head_sb[1] + t * p.tok_sb[1] + c * 16);
+      to[u] = dst + h * p.head_sb[2] + t * p.tok_sb[2] + c * 16;
+    }
+#pragma unroll
+    for (int u = 0; u < kStageBatch; ++u) {
+      if (to[u] < 0) continue;
+      const int x = x0 + u * kStageThreads;
+      *reinterpret_cast<uint4*>(const_cast<unsigned char*>(x < rows * vec ? p.k[2] : p.v[2]) + to[u]) = v[u];
+    }
+  }
+}
+
 namespace {
+
+// Blocks per request whose host-tier ones are copied (0: read in place), and
+// the bytes of K (and of V) of one.  Copies pay when a host block has several
+// readers, and are left out where they would take more than kStageBytes.
+constexpr int64_t kStageBytes = (int64_t)1 << 30;
+int stage_blocks(const fd_attn_args* a, int64_t* block_bytes) {
+  *block_bytes = (int64_t)a->num_kv_heads * a->block_size * a->head_size * fdh::elem_size(a->dtype);
+  if (a->block_table == nullptr || !a->tier[1].host_mapped || a->tier[1].num_blocks <= 0 || a->block_size <= 0 ||
+      a->num_kv_heads <= 0 || a->n <= 0)
+    return 0;
+  const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
+  const int64_t item_rows = mma_covers(a) ? 256 : kRows;
+  if (q * (a->num_heads / a->num_kv_heads) <= item_rows) return 0;
+  int64_t w = a->max_k_len > 0 ? ((int64_t)a->max_k_len + a->block_size - 1) / a->block_size : a->bt_width;
+  if (w > a->bt_width) w = a->bt_width;
+  return w * a->n * 2 * *block_bytes <= kStageBytes ? (int)w : 0;
+}
 
 size_t core_workspace(const fd_attn_args* a) {
   const size_t slots = 2 * (size_t)kMaxCtas * kRows;
   return kMaxCtas * sizeof(Cut) + slots * 2 * 4 + slots * (size_t)a->head_size * 4;
+}
+
+size_t base_workspace(const fd_attn_args* a) {
+  const size_t b = mma_covers(a) ? mma_workspace(a) : core_workspace(a);
+  return (b + 255) / 256 * 256;
 }
 
 template <typename T, int DP>
@@ -431,6 +482,21 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   if (a->workspace == nullptr || a->workspace_bytes < need || !fdh::aligned16(a->workspace))
     return fdh::fail(FD_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
+  int64_t block_bytes = 0;
+  p.stage_w = chunk ? stage_blocks(a, &block_bytes) : 0;
+  if (p.stage_w > 0) {
+    const int64_t blocks = (int64_t)p.stage_w * p.n;
+    const unsigned char* at = static_cast<const unsigned char*>(a->workspace) + base_workspace(a);
+    p.k[2] = at;
+    p.v[2] = at + blocks * block_bytes;
+    p.tok_sb[2] = (int64_t)p.D * es;
+    p.head_sb[2] = p.tok_sb[2] * p.BS;
+    p.blk_sb[2] = block_bytes;
+    p.nblk[2] = blocks;
+    fd_attn_stage_kernel<<<dim3((unsigned)p.stage_w, (unsigned)p.n), kStageThreads, 0, s>>>(p, p.D * es / 16);
+    const int st = fdh::cuda_status(cudaGetLastError(), "fd_attn_stage_kernel launch");
+    if (st != FD_OK) return st;
+  }
   if (mma_covers(a)) return mma_launch(p, a, s);
   unsigned char* ws = static_cast<unsigned char*>(a->workspace);
   p.cuts = reinterpret_cast<Cut*>(ws);
@@ -453,8 +519,9 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
 
 extern "C" size_t fd_attn_workspace_size(const fd_attn_args* a) {
   if (a == nullptr || a->head_size <= 0 || a->head_size > 256) return 0;
-  const size_t b = fdk::at::mma_covers(a) ? fdk::at::mma_workspace(a) : fdk::at::core_workspace(a);
-  return (b + 255) / 256 * 256;
+  int64_t block_bytes = 0;
+  const int w = fdk::at::stage_blocks(a, &block_bytes);
+  return fdk::at::base_workspace(a) + (size_t)(2 * (int64_t)w * a->n * block_bytes);
 }
 
 extern "C" int fd_chunk_attn(const fd_attn_args* a, void* stream) {

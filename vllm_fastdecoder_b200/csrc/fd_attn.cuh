@@ -45,9 +45,12 @@ struct AttnParams {
   float* lse;
   int64_t q_st, q_sh, o_st, o_sh;  // bytes
   int64_t lse_sh, lse_st;          // elements
-  const unsigned char* k[2];
-  const unsigned char* v[2];
-  int64_t blk_sb[2], head_sb[2], tok_sb[2], nblk[2];  // bytes
+  // the tiers, and third the copies of host blocks (stage_w > 0: block j <
+  // stage_w of request r is block r * stage_w + j there)
+  const unsigned char* k[3];
+  const unsigned char* v[3];
+  int64_t blk_sb[3], head_sb[3], tok_sb[3], nblk[3];  // bytes
+  int stage_w;
   int64_t split;
   const int32_t* bt;       // null: cross attention (k[0], v[0] are rows, nblk[0] of them)
   int64_t bt_stride;
@@ -320,6 +323,26 @@ struct Sched {
     }
   }
 };
+
+// Where block `j` of a request lies, given its entry `id` of the block table:
+// the tier (2: its staged copy) and, in `id`, the block within it; -1: id is
+// outside both tiers.
+__device__ __forceinline__ int locate(const AttnParams& p, int r, int j, int64_t& id) {
+  int t = 0;
+  if (id >= p.split) {
+    t = 1;
+    id -= p.split;
+  }
+  if (id < 0 || id >= p.nblk[t]) {
+    set_error(p.err, FD_DEVERR_BLOCK_ID);
+    return -1;
+  }
+  if (t == 1 && j < p.stage_w) {
+    id = (int64_t)r * p.stage_w + j;
+    t = 2;
+  }
+  return t;
+}
 
 // The kernels' entry points for the host code in fd_attn.cu.
 bool mma_covers(const fd_attn_args* a);

@@ -83,9 +83,8 @@ struct SegInfo {
   int j0, m;     // first key tile, key tiles
   int n0, n1;    // steps (64 keys) of stream A, B
   int tok0;      // first query token of the item within the request
-  int qst, qlen, klen, kbase, kh;
+  int req, qst, qlen, klen, kbase, kh;
   int slot;      // -1: whole, else its slot of the partials
-  int nparts;    // > 0: this is a cut item's first segment
   int pad[2];
 };
 static_assert(sizeof(SegInfo) == 64, "segment record");
@@ -290,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           i.kbase = rq.kbase;
           i.kh = g.kh;
           i.slot = g.whole ? -1 : 2 * cta + (g.j0 > 0 ? 0 : 1);
-          i.nparts = g.nparts;
+          i.req = walk.r;
           if (g.nparts > 0)
             p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, min((g.pair ? 2 : 1) * p.tq, rq.qlen - tok0) * p.G, g.kh};
         }
@@ -328,7 +327,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
-        load_tile<KD>(mp, false, smem + Ge::kOffK + st * kTile, &k_full[st], j, rq.kbase, rq.klen, g.kh, id, lane, pol);
+        load_tile<KD>(mp, false, smem + Ge::kOffK + st * kTile, &k_full[st], j, walk.r, rq.kbase, rq.klen, g.kh, id, lane, pol);
         id = id_next;
         ++tiles;
         if (++st == kRingK) {
@@ -365,7 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
-        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.kbase, i.klen, i.kh, id, lane, pol);
+        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.req, i.kbase, i.klen, i.kh, id, lane, pol);
         id = id_next;
         ++tiles;
         if (++st == kRingV) {
@@ -628,8 +627,8 @@ void encode_maps(MmaParams& mp, const fd_attn_args* a) {
   const AttnParams& p = mp.a;
   const int D = p.D;
   mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
-  for (int t = 0; t < 2; ++t) {
-    if (p.nblk[t] == 0 || p.host[t]) continue;
+  for (int t = 0; t < 3; ++t) {
+    if (p.nblk[t] == 0 || (t < 2 && p.host[t])) continue;
     const bool cross = p.bt == nullptr;
     if (cross && p.nblk[t] > 0x7fffffff) continue;  // rows by 16-byte loads
     if (!cross && p.BS % kSub != 0) continue;

@@ -18,10 +18,10 @@ constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims of 16 bits
 
 struct MmaParams {
   CUtensorMap tmap_q;       // {D, H, T, 1}, box {64, G, tq, 1}
-  CUtensorMap tmap_k[2];    // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}), box {64, 1, 16, 1}
-  CUtensorMap tmap_v[2];
+  CUtensorMap tmap_k[3];    // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}), box {64, 1, 16, 1}
+  CUtensorMap tmap_v[3];
   AttnParams a;
-  int q_tma, kv_tma[2];     // the view has a tensor map
+  int q_tma, kv_tma[3];     // the view has a tensor map
 };
 
 __device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int32_t* err) {
@@ -161,7 +161,7 @@ __device__ __forceinline__ int box_block(const AttnParams& p, int kbase, int kle
 // the TMA boxes, and lane 0's arrival once the other boxes are stored).
 template <int KD>
 __device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsigned char* dst, uint64_t* bar, int j,
-                                          int kbase, int klen, int kh, int id, int lane, uint64_t pol) {
+                                          int r, int kbase, int klen, int kh, int id, int lane, uint64_t pol) {
   const AttnParams& p = mp.a;
   const int t = j * kKT + lane * kSub;
   const bool boxed = p.bt == nullptr || p.BS % kSub == 0;
@@ -173,14 +173,12 @@ __device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsign
       r0 = kbase + t;
     } else {
       int64_t b = id;
-      if (b >= p.split) {
-        tier = 1;
-        b -= p.split;
-      }
-      r0 = t % p.BS;
-      if (b < 0 || b >= p.nblk[tier]) {
-        set_error(p.err, FD_DEVERR_BLOCK_ID);
+      const int page = t / p.BS;
+      r0 = t - page * p.BS;
+      tier = locate(p, r, page, b);
+      if (tier < 0) {
         in = false;
+        tier = 0;
       }
       blk = (int)b;
     }
@@ -218,17 +216,11 @@ __device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsign
         int tr = box_tier, rr = box_r0 + row;
         int64_t b = box_blk;
         if (!boxed) {
-          b = p.bt[(int64_t)kbase * p.bt_stride + key / p.BS];
-          rr = key % p.BS;
-          tr = 0;
-          if (b >= p.split) {
-            tr = 1;
-            b -= p.split;
-          }
-          if (b < 0 || b >= p.nblk[tr]) {
-            set_error(p.err, FD_DEVERR_BLOCK_ID);
-            continue;
-          }
+          const int page = key / p.BS;
+          b = p.bt[(int64_t)kbase * p.bt_stride + page];
+          rr = key - page * p.BS;
+          tr = locate(p, r, page, b);
+          if (tr < 0) continue;
         }
         const unsigned char* base = is_v ? p.v[tr] : p.k[tr];
         v[c] = *reinterpret_cast<const uint4*>(base + b * p.blk_sb[tr] + kh * p.head_sb[tr] +

@@ -75,9 +75,9 @@ struct SegInfo {
   int live;    // 0: no more segments
   int j0, m;   // first key tile, key tiles
   int tok0;    // first query token of the item within the request
-  int qst, qlen, klen, kbase, kh;
+  int req, qst, qlen, klen, kbase, kh;
   int slot;    // -1: whole, else its slot of the partials
-  int pad[6];
+  int pad[5];
 };
 static_assert(sizeof(SegInfo) == 64, "segment record");
 
@@ -213,6 +213,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           i.j0 = g.j0;
           i.m = g.j1 - g.j0;
           i.tok0 = tok0;
+          i.req = walk.r;
           i.qst = rq.qst;
           i.qlen = rq.qlen;
           i.klen = rq.klen;
@@ -250,7 +251,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
-        load_tile<KD>(mp, false, smem + st * kTile, &k_full[st], j, rq.kbase, rq.klen, g.kh, id, lane, pol);
+        load_tile<KD>(mp, false, smem + st * kTile, &k_full[st], j, walk.r, rq.kbase, rq.klen, g.kh, id, lane, pol);
         id = id_next;
         ++tiles;
         if (++st == kRingK) {
@@ -285,7 +286,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
-        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.kbase, i.klen, i.kh, id, lane, pol);
+        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.req, i.kbase, i.klen, i.kh, id, lane, pol);
         id = id_next;
         ++tiles;
         if (++st == kRingV) {

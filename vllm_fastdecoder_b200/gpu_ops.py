@@ -939,20 +939,23 @@ def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1,
         if lse.dtype is not torch.float32 or lse.get_device() != idx or lse.shape != (H, T):
             raise RuntimeError("lse must be fp32 [H, T] on q's device")
         lse_f = (lse.data_ptr(), *lse.stride())
-    need = _attn_workspace_bytes(H, KVH, D, dt)
+    packed = [
+        *_rows3(q, idx, dt, "q"), *_rows3(out, idx, dt, "out"), *lse_f, *f0, *f1, tier_split,
+        *((0, 0) if table is None else (table.data_ptr(), table.stride(0))),
+        0 if bt_row is None else _i32(bt_row, idx, n, "bt_row"), 0 if k_start is None else _i32(k_start, idx, n, "k_start"),
+        _i32(q_start, idx, n, "q_start"), _i32(q_len, idx, n, "q_len"), _i32(k_len, idx, n, "k_len"), W, T, n, H, KVH, D,
+        BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, 0, 0, _error_ptr(idx)]
+    if f1[-2]:  # a host tier: its copies count
+        need = nat.load().fd_attn_workspace_size(_ATTN_STRUCT.pack(*packed))
+    else:
+        need = _attn_workspace_bytes(H, KVH, D, dt)
     if workspace_buf is None:
         workspace_buf = torch.empty(need, dtype=torch.uint8, device=q.device)
     elif (workspace_buf.get_device() != idx or workspace_buf.dtype is not torch.uint8 or not workspace_buf.is_contiguous()
           or workspace_buf.numel() < need):
         raise RuntimeError(f"workspace_buf must be contiguous uint8 on q's device with >= {need} bytes")
-    packed = _ATTN_STRUCT.pack(
-        *_rows3(q, idx, dt, "q"), *_rows3(out, idx, dt, "out"), *lse_f, *f0, *f1, tier_split,
-        *((0, 0) if table is None else (table.data_ptr(), table.stride(0))),
-        0 if bt_row is None else _i32(bt_row, idx, n, "bt_row"), 0 if k_start is None else _i32(k_start, idx, n, "k_start"),
-        _i32(q_start, idx, n, "q_start"), _i32(q_len, idx, n, "q_len"), _i32(k_len, idx, n, "k_len"), W, T, n, H, KVH, D,
-        BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, workspace_buf.data_ptr(), workspace_buf.numel(),
-        _error_ptr(idx))
-    _launch(fn, packed, idx, what)
+    packed[-3], packed[-2] = workspace_buf.data_ptr(), workspace_buf.numel()
+    _launch(fn, _ATTN_STRUCT.pack(*packed), idx, what)
 
 
 def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
