@@ -7,11 +7,14 @@
 //   s = scale log2(e) q.K^T,  m' = max(m, max_j s),  p = 2^(s - m'),
 //   l = l 2^(m - m') + sum_j p,  O = O 2^(m - m') + p V
 // and o = O / l, lse = ln 2 (m + log2 l), all in fp32.  A CTA of 16 x 16
-// threads holds 64 rows and 32 keys in shared memory as fp32; thread (y, x)
-// owns rows 4 y .. 4 y + 3: two scores of each (keys x and x + 16), and D / 16
-// dims of O in registers, so a float4 from shared memory feeds 4 x 2 or 4 x 4
-// FMAs and the fp32 pipe and the shared-memory reads are about evenly loaded.
-// The K/V rows of the next tile are fetched into registers during this one.
+// threads holds 64 rows and 64 keys (32 for heads of more than 64 dims) in
+// shared memory as fp32; thread (y, x) owns rows 4 y .. 4 y + 3: the scores of
+// keys x, x + 16, .. and D / 16 dims of O in registers.  A float4 of K or V
+// then feeds 4 rows, one of Q or P 4 keys or dims (64 FMAs per 12
+// shared-memory wavefronts of a warp), which keeps the fp32 pipe the bound,
+// and four warps per scheduler hide each other's latencies (8 x 4 scores in
+// half the threads took 2.1 cycles per FMA).  The next tile's K/V are fetched
+// into registers during this one's products.
 
 #include <math.h>
 
@@ -21,14 +24,17 @@ namespace fdk {
 namespace at {
 
 constexpr int kRows = 64;   // rows per tile
-constexpr int kKeys = 32;   // keys per tile
 constexpr int kThreads = 256;
-constexpr int kFixed = 2;   // an item's fixed cost in key tiles
-constexpr int kMinPer = 4;  // least positions of a CTA
+constexpr int kFixed = 1;   // an item's fixed cost in key tiles
+constexpr int kMinPer = 2;  // least positions of a CTA
+constexpr int kWhole = 2;   // key tiles up to which no item is cut (whole_items)
 constexpr int kMaxCtas = 320;
-typedef Sched<kKeys, false, kFixed> Walk;
 
-constexpr int smem_bytes(int DP) { return ((kRows + 2 * kKeys) * (DP + 4) + kRows * (kKeys + 1)) * 4; }
+constexpr int keys_of(int DP) { return DP <= 64 ? 64 : 32; }           // keys per tile
+constexpr int ctas_of(int DP) { return DP <= 128 ? 2 : 1; }  // CTAs per SM
+constexpr int smem_bytes(int DP) {
+  return ((kRows + 2 * keys_of(DP)) * (DP + 4) + kRows * (keys_of(DP) + 4)) * 4;
+}
 
 // Byte offset of K (and V) row j of the request for kv head kh within its tier,
 // -1 when there is none (behind klen, or a block id outside both tiers).
@@ -44,17 +50,22 @@ __device__ __forceinline__ int64_t key_offset(const AttnParams& p, const Req& q,
 }
 
 template <typename T, int DP>
-__global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(const __grid_constant__ AttnParams p) {
+__global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_attn_kernel(const __grid_constant__ AttnParams p) {
   constexpr int VE = 16 / (int)sizeof(T);      // elements per 16-byte load
+  constexpr int NV = DP / VE;                  // loads per row
+  constexpr int kKeys = keys_of(DP);
+  constexpr int KN = kKeys / 16;               // keys of a thread
   constexpr int LD = DP + 4;                   // row stride of the tiles (floats)
-  constexpr int kVecs = kKeys * DP / VE / kThreads;  // 16-byte loads of K (and of V) per thread
+  constexpr int LP = kKeys + 4;                // row stride of P
   constexpr int kDim4 = DP / 64;               // float4 of O per row and thread
+  constexpr int kVecs = kKeys * NV / kThreads;  // loads of K (and of V) per thread and tile
+  typedef Sched<kKeys, false, kFixed> Walk;
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
   float* sk = sq + kRows * LD;
   float* sv = sk + kKeys * LD;
-  float* sp = sv + kKeys * LD;  // [kRows][kKeys + 1]
-  __shared__ Walk::Scratch scratch;
+  float* sp = sv + kKeys * LD;  // [kRows][LP]
+  __shared__ typename Walk::Scratch scratch;
   __shared__ const unsigned char* k_row[kKeys];
   __shared__ const unsigned char* v_row[kKeys];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
@@ -64,45 +75,34 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
   griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
   if (tid == 0) p.cuts[cta].nparts = 0;
   Walk walk(p);
-  if (!walk.init<kThreads>(&scratch, cta, kMinPer)) return;
-  Walk::Seg g;
+  if (!walk.template init<kThreads>(&scratch, cta, kMinPer)) return;
+
+  // 16 bytes of a tile's row as fp32
+  auto put = [&](float* dst, int x, const uint4& v) {
+    float f[VE];
+    Dt<T>::widen(v, f);
+#pragma unroll
+    for (int e = 0; e < VE; e += 4)
+      *reinterpret_cast<float4*>(dst + x / NV * LD + x % NV * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+  };
+  typename Walk::Seg g;
   while (walk.next(g)) {
     const Req rq = walk.rq;
     const int tok0 = g.tile0 * p.tq;
     const int rows = min(p.tq, rq.qlen - tok0) * p.G;
-    // the query rows as fp32 (zeros behind them and behind D)
-    __syncthreads();  // the last segment's reads of shared memory are done
-    for (int x = tid; x < kRows * (DP / VE); x += kThreads) {
-      const int row = x / (DP / VE), c = x % (DP / VE);
-      float f[VE];
-#pragma unroll
-      for (int e = 0; e < VE; ++e) f[e] = 0.f;
-      if (row < rows && c < nvec)
-        Dt<T>::widen(*reinterpret_cast<const uint4*>(p.q + (int64_t)(rq.qst + tok0 + row / p.G) * p.q_st +
-                                                     (int64_t)(g.kh * p.G + row % p.G) * p.q_sh + c * 16),
-                     f);
-#pragma unroll
-      for (int e = 0; e < VE; e += 4)
-        *reinterpret_cast<float4*>(sq + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-    }
     const bool active = (ty & ~1) * 4 < rows;  // some row of this warp is real
-    int lim[4];                                // last key that each row sees
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int row = 4 * ty + i;
-      lim[i] = row >= rows ? -1 : p.bt != nullptr ? rq.klen - rq.qlen + tok0 + row / p.G : rq.klen - 1;
-    }
+    const int lim0 = p.bt != nullptr ? rq.klen - rq.qlen + tok0 : rq.klen - 1;  // last key that the first token sees
     float m[4], l[4];
-    float4 o[4][kDim4];
+    ulonglong2 o[4][kDim4];  // four dims, packed in pairs
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       m[i] = -INFINITY;
       l[i] = 0.f;
 #pragma unroll
-      for (int d = 0; d < kDim4; ++d) o[i][d] = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int d = 0; d < kDim4; ++d) o[i][d] = make_ulonglong2(0ull, 0ull);
     }
     uint4 kr[kVecs], vr[kVecs];
-    auto fetch = [&](int j) {  // all threads: the rows of key tile j into registers
+    auto fetch = [&](int j) {  // all threads: key tile j into registers (zeros where there is no key or dim)
       if (tid < kKeys) {
         int t;
         const int64_t at = key_offset(p, rq, walk.r, g.kh, j * kKeys + tid, &t);
@@ -111,88 +111,113 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
       }
       __syncthreads();
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) {
-        const int i = tid + x * kThreads, row = i / (DP / VE), c = i % (DP / VE);
+      for (int u = 0; u < kVecs; ++u) {
+        const int x = tid + u * kThreads, row = x / NV, c = x % NV;
         const bool real = c < nvec && k_row[row] != nullptr;
-        kr[x] = real ? *reinterpret_cast<const uint4*>(k_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
-        vr[x] = real ? *reinterpret_cast<const uint4*>(v_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+        kr[u] = real ? *reinterpret_cast<const uint4*>(k_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
+        vr[u] = real ? *reinterpret_cast<const uint4*>(v_row[row] + c * 16) : make_uint4(0u, 0u, 0u, 0u);
       }
     };
-    if (g.j0 < g.j1) fetch(g.j0);
+    __syncthreads();  // the last segment's reads of shared memory are done
+    if (g.j0 < g.j1) {
+      fetch(g.j0);
+#pragma unroll 4
+      for (int x = tid; x < kRows * NV; x += kThreads) {  // the query rows, zeros behind them
+        const int row = x / NV, c = x % NV, t = row / p.G;
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows && c < nvec)
+          v = *reinterpret_cast<const uint4*>(p.q + (int64_t)(rq.qst + tok0 + t) * p.q_st +
+                                              (int64_t)(g.kh * p.G + row - t * p.G) * p.q_sh + c * 16);
+        put(sq, x, v);
+      }
+    }
     for (int j = g.j0; j < g.j1; ++j) {
       __syncthreads();  // the last tile's reads are done
 #pragma unroll
-      for (int x = 0; x < kVecs; ++x) {
-        const int i = tid + x * kThreads, row = i / (DP / VE), c = i % (DP / VE);
-        float f[VE];
-        Dt<T>::widen(kr[x], f);
-#pragma unroll
-        for (int e = 0; e < VE; e += 4)
-          *reinterpret_cast<float4*>(sk + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
-        Dt<T>::widen(vr[x], f);
-#pragma unroll
-        for (int e = 0; e < VE; e += 4)
-          *reinterpret_cast<float4*>(sv + row * LD + c * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
+      for (int u = 0; u < kVecs; ++u) {
+        put(sk, tid + u * kThreads, kr[u]);
+        put(sv, tid + u * kThreads, vr[u]);
       }
       __syncthreads();
       if (j + 1 < g.j1) fetch(j + 1);
       if (!active) continue;
-      float s[4][2];
+      // even and odd dims' sums in the two halves of a packed FMA
+      float s[4][KN];
+      f2_t s2[4][KN];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
-#pragma unroll 4
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < KN; ++c) s2[i][c] = 0ull;
+#pragma unroll 2
       for (int d = 0; d < D; d += 4) {
-        const float4 b0 = *reinterpret_cast<const float4*>(sk + tx * LD + d);
-        const float4 b1 = *reinterpret_cast<const float4*>(sk + (tx + 16) * LD + d);
+        ulonglong2 b[KN];
+#pragma unroll
+        for (int c = 0; c < KN; ++c) b[c] = *reinterpret_cast<const ulonglong2*>(sk + (tx + 16 * c) * LD + d);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float4 a = *reinterpret_cast<const float4*>(sq + (4 * ty + i) * LD + d);
-          s[i][0] = fmaf(a.x, b0.x, fmaf(a.y, b0.y, fmaf(a.z, b0.z, fmaf(a.w, b0.w, s[i][0]))));
-          s[i][1] = fmaf(a.x, b1.x, fmaf(a.y, b1.y, fmaf(a.z, b1.z, fmaf(a.w, b1.w, s[i][1]))));
+          const ulonglong2 a = *reinterpret_cast<const ulonglong2*>(sq + (4 * ty + i) * LD + d);
+#pragma unroll
+          for (int c = 0; c < KN; ++c) s2[i][c] = f2_fma(a.y, b[c].y, f2_fma(a.x, b[c].x, s2[i][c]));
         }
       }
 #pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int c = 0; c < KN; ++c) {
+          float even, odd;
+          f2_unpack(s2[i][c], even, odd);
+          s[i][c] = even + odd;
+        }
+      const bool cut = j * kKeys + kKeys - 1 > lim0;
+#pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int key = j * kKeys + tx;
-        s[i][0] = key <= lim[i] ? s[i][0] * p.sl2 : -INFINITY;
-        s[i][1] = key + 16 <= lim[i] ? s[i][1] * p.sl2 : -INFINITY;
-        float mx = fmaxf(s[i][0], s[i][1]);
+        const int row = 4 * ty + i;
+        const int lim = row >= rows ? -1 : p.bt != nullptr ? lim0 + row / p.G : lim0;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int c = 0; c < KN; ++c) {
+          s[i][c] = cut && j * kKeys + tx + 16 * c > lim ? -INFINITY : s[i][c] * p.sl2;
+          mx = fmaxf(mx, s[i][c]);
+        }
 #pragma unroll
         for (int off = 8; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
         const float mn = fmaxf(m[i], mx);
         const float base = mn == -INFINITY ? 0.f : mn;  // no key seen so far: every p is 2^-inf = 0
-        const float alpha = exp2f(m[i] - base);
-        const float p0 = exp2f(s[i][0] - base), p1 = exp2f(s[i][1] - base);
-        float sum = p0 + p1;
+        const float alpha = ex2_approx(m[i] - base);
+        float sum = 0.f;
 #pragma unroll
-        for (int off = 8; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
-        l[i] = l[i] * alpha + sum;
+        for (int c = 0; c < KN; ++c) {
+          const float e = ex2_approx(s[i][c] - base);
+          sp[row * LP + tx + 16 * c] = e;
+          sum += e;
+        }
+        l[i] = l[i] * alpha + sum;  // this thread's keys; the row's threads are added up at the end
         m[i] = mn;
-        sp[(4 * ty + i) * (kKeys + 1) + tx] = p0;
-        sp[(4 * ty + i) * (kKeys + 1) + tx + 16] = p1;
+        const f2_t alpha2 = f2_pack(alpha, alpha);
 #pragma unroll
         for (int d = 0; d < kDim4; ++d) {
-          o[i][d].x *= alpha;
-          o[i][d].y *= alpha;
-          o[i][d].z *= alpha;
-          o[i][d].w *= alpha;
+          o[i][d].x = f2_mul(o[i][d].x, alpha2);
+          o[i][d].y = f2_mul(o[i][d].y, alpha2);
         }
       }
-      __syncwarp();  // a row's scores are written and read by one half-warp
-#pragma unroll 4
-      for (int c = 0; c < kKeys; ++c) {
-        float4 b[kDim4];
+      __syncwarp();  // a row's P is written and read by one half-warp
+#pragma unroll 1
+      for (int c = 0; c < kKeys; c += 4) {
+        float4 a[4];
 #pragma unroll
-        for (int d = 0; d < kDim4; ++d) b[d] = *reinterpret_cast<const float4*>(sv + c * LD + 64 * d + 4 * tx);
+        for (int i = 0; i < 4; ++i) a[i] = *reinterpret_cast<const float4*>(sp + (4 * ty + i) * LP + c);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float a = sp[(4 * ty + i) * (kKeys + 1) + c];
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
           for (int d = 0; d < kDim4; ++d) {
-            o[i][d].x = fmaf(a, b[d].x, o[i][d].x);
-            o[i][d].y = fmaf(a, b[d].y, o[i][d].y);
-            o[i][d].z = fmaf(a, b[d].z, o[i][d].z);
-            o[i][d].w = fmaf(a, b[d].w, o[i][d].w);
+            const ulonglong2 b = *reinterpret_cast<const ulonglong2*>(sv + (c + e) * LD + 64 * d + 4 * tx);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float w = e == 0 ? a[i].x : e == 1 ? a[i].y : e == 2 ? a[i].z : a[i].w;
+              const f2_t w2 = f2_pack(w, w);
+              o[i][d].x = f2_fma(w2, b.x, o[i][d].x);
+              o[i][d].y = f2_fma(w2, b.y, o[i][d].y);
+            }
           }
         }
       }
@@ -201,37 +226,41 @@ __global__ void __launch_bounds__(kThreads, DP <= 128 ? 2 : 1) fd_attn_kernel(co
     const int slot = 2 * cta + (g.j0 > 0 ? 0 : 1);
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      float li = l[i];
+#pragma unroll
+      for (int off = 8; off > 0; off >>= 1) li += __shfl_xor_sync(0xffffffffu, li, off);
       const int row = 4 * ty + i;
       if (row >= rows) continue;
-      const int64_t tok = rq.qst + tok0 + row / p.G;
-      const int h = g.kh * p.G + row % p.G;
+      const int t = row / p.G;
+      const int64_t tok = rq.qst + tok0 + t;
+      const int h = g.kh * p.G + row - t * p.G;
       if (!g.whole) {
         float4* po = reinterpret_cast<float4*>(p.part_o) + (int64_t)slot * (D / 4) * kRows + row;
-        if (tx == 0) {
-          p.part_ml[((int64_t)slot * kRows + row) * 2] = m[i];
-          p.part_ml[((int64_t)slot * kRows + row) * 2 + 1] = l[i];
-        }
+        if (tx == 0)
+          reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kRows + row] = make_float2(m[i], li);
 #pragma unroll
         for (int d = 0; d < kDim4; ++d)
-          if (64 * d + 4 * tx < D) po[(16 * d + tx) * kRows] = o[i][d];
+          if (64 * d + 4 * tx < D) po[(16 * d + tx) * kRows] = *reinterpret_cast<const float4*>(&o[i][d]);
         continue;
       }
-      const float inv = l[i] > 0.f ? 1.f / l[i] : 0.f;
+      const float inv = li > 0.f ? 1.f / li : 0.f;
       if (tx == 0 && p.lse != nullptr)
-        p.lse[h * p.lse_sh + tok * p.lse_st] = l[i] > 0.f ? (m[i] + log2f(l[i])) * kLn2 : -INFINITY;
+        p.lse[h * p.lse_sh + tok * p.lse_st] = li > 0.f ? (m[i] + log2f(li)) * kLn2 : -INFINITY;
       T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
 #pragma unroll
       for (int d = 0; d < kDim4; ++d) {
         const int c = 64 * d + 4 * tx;
         if (c >= D) continue;
-        const float f[4] = {o[i][d].x * inv, o[i][d].y * inv, o[i][d].z * inv, o[i][d].w * inv};
-        T t[4];
+        float f[4];
+        f2_unpack(o[i][d].x, f[0], f[1]);
+        f2_unpack(o[i][d].y, f[2], f[3]);
+        T t4[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) t[e] = Dt<T>::narrow(f[e]);
+        for (int e = 0; e < 4; ++e) t4[e] = Dt<T>::narrow(f[e] * inv);
         if (sizeof(T) == 4)
-          *reinterpret_cast<uint4*>(po + c) = *reinterpret_cast<const uint4*>(t);
+          *reinterpret_cast<uint4*>(po + c) = *reinterpret_cast<const uint4*>(t4);
         else
-          *reinterpret_cast<uint2*>(po + c) = *reinterpret_cast<const uint2*>(t);
+          *reinterpret_cast<uint2*>(po + c) = *reinterpret_cast<const uint2*>(t4);
       }
     }
     if (g.nparts > 0 && tid == 0) p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, rows, g.kh};
@@ -297,6 +326,15 @@ __global__ void __launch_bounds__(kCombineThreads) fd_attn_combine_kernel(const 
     else
       *reinterpret_cast<uint2*>(po + 4 * d) = *reinterpret_cast<const uint2*>(t);
   }
+}
+
+bool whole_items(const fd_attn_args* a, int ctas, int item_rows, int keys, int most) {
+  if (a->max_k_len <= 0) return false;
+  const int G = a->num_heads / a->num_kv_heads;
+  const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
+  const int64_t items = (q + item_rows / G - 1) / (item_rows / G) * a->n * a->num_kv_heads;
+  const int64_t tiles = ((int64_t)a->max_k_len + keys - 1) / keys;
+  return items <= ctas && tiles <= most;
 }
 
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
@@ -382,7 +420,8 @@ size_t base_workspace(const fd_attn_args* a) {
 }
 
 template <typename T, int DP>
-int core_launch_dp(AttnParams& p, int dtype, cudaStream_t s) {
+int core_launch_dp(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
+  const int dtype = a->dtype;
   const void* kern = reinterpret_cast<const void*>(fd_attn_kernel<T, DP>);
   static unsigned long long done = 0;
   int st = fdh::ensure_smem(kern, smem_bytes(DP), &done);
@@ -390,19 +429,20 @@ int core_launch_dp(AttnParams& p, int dtype, cudaStream_t s) {
   int dev = 0, sms = 0;
   st = fdh::device_sms(&dev, &sms);
   if (st != FD_OK) return st;
-  p.ctas = sms * (DP <= 128 ? 2 : 1);
+  p.ctas = sms * ctas_of(DP);
   if (p.ctas > kMaxCtas) p.ctas = kMaxCtas;
   const dim3 grid((unsigned)p.ctas);
+  p.snap = whole_items(a, p.ctas, kRows, keys_of(DP), kWhole);
   st = fdh::launch_maybe_pdl(kern, grid, dim3(kThreads), smem_bytes(DP), s, false, p, "fd_attn_kernel launch");
-  if (st != FD_OK) return st;
+  if (st != FD_OK || p.snap) return st;
   return combine_launch(p, dtype, kRows, s);
 }
 
 template <typename T>
-int core_launch(AttnParams& p, int dtype, cudaStream_t s) {
-  if (p.D <= 64) return core_launch_dp<T, 64>(p, dtype, s);
-  if (p.D <= 128) return core_launch_dp<T, 128>(p, dtype, s);
-  return core_launch_dp<T, 256>(p, dtype, s);
+int core_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
+  if (p.D <= 64) return core_launch_dp<T, 64>(p, a, s);
+  if (p.D <= 128) return core_launch_dp<T, 128>(p, a, s);
+  return core_launch_dp<T, 256>(p, a, s);
 }
 
 // Shared checks and parameters; `what` names the entry point in messages.
@@ -505,11 +545,11 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   p.tq = kRows / G;
   switch (a->dtype) {
     case FD_DTYPE_F16:
-      return core_launch<__half>(p, a->dtype, s);
+      return core_launch<__half>(p, a, s);
     case FD_DTYPE_BF16:
-      return core_launch<__nv_bfloat16>(p, a->dtype, s);
+      return core_launch<__nv_bfloat16>(p, a, s);
     default:
-      return core_launch<float>(p, a->dtype, s);
+      return core_launch<float>(p, a, s);
   }
 }
 

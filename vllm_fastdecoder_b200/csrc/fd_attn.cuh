@@ -63,12 +63,20 @@ struct AttnParams {
   float sl2;               // scale * log2(e)
   int tq;                  // tokens per query tile
   int ctas;
+  int snap;                // no item is cut: each is its start's CTA's (whole_items)
   Cut* cuts;               // [ctas]
   float* part_ml;          // [ctas][2][rows per item][2]: m (log2 domain), l
   float* part_o;           // [ctas][2][D / 4][rows per item][4]
   int out32;               // rows of out are 32-byte aligned (fd_attn_mma.cu)
   int32_t* err;
 };
+
+// 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
 
 // sum of floor((a i + b) / m) over 0 <= i < n, by the Euclidean recursion on
 // (a, m); a n + b < 2^32.
@@ -308,7 +316,8 @@ struct Sched {
       const bool pr = is_pair(p, rq, item);
       const int u = pr ? 2 : 1;
       const int n = ntiles(p, rq, item_end(p, rq, item));
-      const int a = -s - kW, b = len - s - kW;
+      if (p.snap && s < 0) continue;  // the CTA before has it
+      const int a = p.snap ? -kW : -s - kW, b = p.snap ? u * n : len - s - kW;
       // tile j belongs to the range that holds position s + kW + u j
       g.j0 = max(0, min(n, (a + u - 1) >> (u - 1)));
       g.j1 = max(0, min(n, (b + u - 1) >> (u - 1)));
@@ -352,6 +361,10 @@ int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s);
 // the caller says: `rows` of them (fd_attn_rows.cu; right for more, too).
 constexpr int kFewRows = 32;
 int rows_launch(AttnParams& p, const fd_attn_args* a, int rows, cudaStream_t s);
+// Whether to give every item to one CTA whole: at most one item per CTA, of
+// `most` key tiles at most, as far as the caller's bounds tell.  Cutting such a
+// call shortens its longest CTA by less than the combine's launch takes.
+bool whole_items(const fd_attn_args* a, int ctas, int item_rows, int keys, int most);
 // Joins the cut items: `rows` rows per item at most.
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s);
 

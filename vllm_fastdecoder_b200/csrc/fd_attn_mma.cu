@@ -669,14 +669,14 @@ int mma_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
   p.tq = mm::kM / p.G;
   p.ctas = sms < mm::kMaxCtas ? sms : mm::kMaxCtas;
   mm::MmaParams mp{};
-  const int D = p.D;
+  p.snap = whole_items(a, p.ctas, 2 * mm::kM, mm::kKT, mm::kWhole);
   mp.a = p;
   mm::encode_maps(mp, a);
   if (a->dtype == FD_DTYPE_BF16)
-    st = D <= 64 ? mm::launch<__nv_bfloat16, 64>(mp, s) : mm::launch<__nv_bfloat16, 128>(mp, s);
+    st = p.D <= 64 ? mm::launch<__nv_bfloat16, 64>(mp, s) : mm::launch<__nv_bfloat16, 128>(mp, s);
   else
-    st = D <= 64 ? mm::launch<__half, 64>(mp, s) : mm::launch<__half, 128>(mp, s);
-  if (st != FD_OK) return st;
+    st = p.D <= 64 ? mm::launch<__half, 64>(mp, s) : mm::launch<__half, 128>(mp, s);
+  if (st != FD_OK || p.snap) return st;
   return combine_launch(p, a->dtype, mm::kItemRows, s);
 }
 

@@ -12,6 +12,7 @@ namespace at {
 namespace mm {
 
 constexpr int kKT = 128;            // keys per K/V tile
+constexpr int kWhole = 8;           // key tiles up to which no item is cut (whole_items)
 constexpr int kSub = 16;            // keys per TMA box
 constexpr int kSubs = kKT / kSub;
 constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims of 16 bits
@@ -60,13 +61,6 @@ __device__ __forceinline__ uint64_t l2_evict_normal_policy() {
   uint64_t pol;
   asm volatile("createpolicy.fractional.L2::evict_normal.b64 %0, 1.0;" : "=l"(pol));
   return pol;
-}
-
-// 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
-__device__ __forceinline__ float ex2_approx(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
 }
 
 __device__ __forceinline__ float fmax3(float a, float b, float c) {

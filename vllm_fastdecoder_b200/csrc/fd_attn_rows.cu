@@ -572,11 +572,12 @@ int rows_launch(AttnParams& p, const fd_attn_args* a, int rows, cudaStream_t s) 
   p.part_ml = reinterpret_cast<float*>(ws + rw::kMaxCtas * sizeof(Cut));
   p.part_o = p.part_ml + 2 * 2 * (size_t)rw::kMaxCtas * N;
   p.tq = N / p.G;
+  p.snap = whole_items(a, p.ctas, N, mm::kKT, mm::kWhole);
   mm::MmaParams mp{};
   mp.a = p;
   mm::encode_maps(mp, a);
   st = a->dtype == FD_DTYPE_BF16 ? rw::launch_for<__nv_bfloat16>(mp, N, s) : rw::launch_for<__half>(mp, N, s);
-  if (st != FD_OK) return st;
+  if (st != FD_OK || p.snap) return st;
   return combine_launch(p, a->dtype, N, s);
 }
 
