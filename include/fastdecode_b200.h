@@ -711,8 +711,8 @@ typedef struct fd_attn_args {
 /* Scratch bytes of fd_chunk_attn / fd_cross_attn for these arguments (reads
  * the sizes and bounds, tier[1].host_mapped and num_blocks, and whether there
  * is a block table; without a host tier the heads, head_size and dtype are
- * enough).  Host blocks that several query tiles read are copied there first,
- * up to 1 GiB of them.  Pure host arithmetic. */
+ * enough).  Host blocks are copied there first, where n requests of max_k_len
+ * keys take at most 1 GiB.  Pure host arithmetic. */
 FD_API size_t fd_attn_workspace_size(const fd_attn_args *a);
 
 /* Attention of a chunk of new tokens over the two-tier paged cache:

@@ -319,6 +319,12 @@ LENS = {
     (torch.bfloat16, 20, 4, 128, 64, 0.0, "chunks"), (torch.float16, 64, 1, 128, 16, 0.0, "verify"),
     (torch.bfloat16, 4, 2, 8, 5, 0.0, "edges"), (torch.bfloat16, 8, 2, 192, 16, 0.3, "edges"),
     (torch.float16, 4, 1, 256, 16, 0.0, "chunks"), (torch.float32, 8, 2, 64, 16, 0.3, "edges"),
+    (torch.bfloat16, 8, 2, 128, 16, 0.0, "tokens"), (torch.float16, 4, 4, 64, 16, 0.5, "tokens"),
+    (torch.bfloat16, 32, 1, 64, 16, 0.0, "tokens"), (torch.float16, 20, 1, 112, 8, 0.2, "tokens"),
+    (torch.float16, 8, 2, 64, 16, 0.0, "verify"), (torch.bfloat16, 2, 2, 80, 64, 0.0, "verify"),
+    (torch.float16, 3, 1, 64, 24, 0.0, "verify"), (torch.bfloat16, 4, 2, 128, 128, 0.3, "chunks"),
+    (torch.float16, 4, 2, 64, 12, 0.3, "chunks"), (torch.bfloat16, 8, 2, 128, 40, 0.0, "verify"),
+    (torch.float16, 8, 8, 128, 256, 0.0, "tokens"), (torch.bfloat16, 8, 2, 64, 32, 0.2, "edges"),
     (torch.float32, 8, 2, 128, 16, 0.0, "verify"), (torch.float32, 4, 4, 256, 24, 0.0, "edges"),
     (torch.float32, 6, 2, 36, 16, 0.0, "chunks"), (torch.float32, 64, 1, 64, 16, 0.0, "verify"),
 ])

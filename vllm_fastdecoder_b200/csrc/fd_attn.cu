@@ -354,11 +354,11 @@ int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
   return fdh::cuda_status(cudaLaunchKernelExC(&cfg, kern, args), "fd_attn_combine_kernel launch");
 }
 
-// Host blocks that several items read (more query rows per kv head than one
-// item has) are copied to device memory first: read in place they would cross
-// PCIe once per item, and an SM's loads do not keep them in L2.  CTA (j, r)
-// copies block j of request r, when it lies in the host tier, to block
-// r * stage_w + j of the copies.
+// Host blocks are copied to device memory first, by all SMs: read in place
+// they would cross PCIe once per item that sees them (an SM's loads do not
+// keep them in L2), and a few CTAs, those whose requests have spilled, would
+// wait for it one tile after another.  CTA (j, r) copies block j of request
+// r, when it lies in the host tier, to block r * stage_w + j of the copies.
 constexpr int kStageThreads = 256, kStageBatch = 8;
 __global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __grid_constant__ AttnParams p, int vec) {
   const int j = blockIdx.x, r = blockIdx.y;
@@ -392,18 +392,15 @@ __global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __gr
 
 namespace {
 
-// Blocks per request whose host-tier ones are copied (0: read in place), and
-// the bytes of K (and of V) of one.  Copies pay when a host block has several
-// readers, and are left out where they would take more than kStageBytes.
+// Blocks per request whose host-tier ones are copied (0: read in place, where
+// the copies could take more than kStageBytes), and the bytes of K (and of V)
+// of one.
 constexpr int64_t kStageBytes = (int64_t)1 << 30;
 int stage_blocks(const fd_attn_args* a, int64_t* block_bytes) {
   *block_bytes = (int64_t)a->num_kv_heads * a->block_size * a->head_size * fdh::elem_size(a->dtype);
   if (a->block_table == nullptr || !a->tier[1].host_mapped || a->tier[1].num_blocks <= 0 || a->block_size <= 0 ||
       a->num_kv_heads <= 0 || a->n <= 0)
     return 0;
-  const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
-  const int64_t item_rows = mma_covers(a) ? 256 : kRows;
-  if (q * (a->num_heads / a->num_kv_heads) <= item_rows) return 0;
   int64_t w = a->max_k_len > 0 ? ((int64_t)a->max_k_len + a->block_size - 1) / a->block_size : a->bt_width;
   if (w > a->bt_width) w = a->bt_width;
   return w * a->n * 2 * *block_bytes <= kStageBytes ? (int)w : 0;

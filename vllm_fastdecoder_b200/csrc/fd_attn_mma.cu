@@ -16,12 +16,12 @@
 // idle half of the time.  So a stream works on 64 keys at a time with two S
 // buffers: q.K^T of step i + 2 is issued right behind P.V of step i, and the
 // softmax of step i + 1 finds its scores ready.  Twelve warps:
-//   8      schedule, Q tiles and K tiles  } TMA boxes of 16 keys with the
-//   10     V tiles                        } 128-byte swizzle the MMA reads, or
-//          16-byte loads stored in the same layout where a box is in the host
-//          tier, spans blocks (block sizes that are no multiple of 16), or is
-//          cut by the end of a request's V (rows behind it must be 0: P is 0
-//          there, and 0 x NaN is not)
+//   8      schedule, Q tiles and K tiles  } TMA boxes of 8 to 128 keys (what
+//   10     V tiles                        } divides a block) with the 128-byte
+//          swizzle the MMA reads, or 16-byte loads stored in the same layout
+//          where a box is in the host tier, spans blocks (block sizes that are
+//          no multiple of 8), or is cut by the end of a request's V (rows
+//          behind it must be 0: P is 0 there, and 0 x NaN is not)
 //   9, 11  one thread each issues the MMAs of stream A, B (one thread alone
 //          issues an MMA per ~70 cycles, more than a 64-key step leaves)
 //   0-3, 4-7  softmax of stream A, B: one thread per row.  P overwrites the
@@ -66,9 +66,9 @@ struct Geo {
   static constexpr int kOffK = 2 * kTile;
   static constexpr int kOffV = kOffK + kRingK * kTile;
   static constexpr int kOffBar = kOffV + kRingV * kTile;
-  // q full/empty, k full/empty, v full/empty, s_full[2][2], p_full[2][2], o_full[2],
-  // o_both, o_empty, ml_full, seg full/empty, drain
-  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 4 + 4 + 2 + 3 + 2 * kSegs + 1;
+  // q full/empty, k full/empty, v full/empty, s_full[2][2], p_full[2][2], pv_done[2],
+  // o_full[2], o_both, o_empty, ml_full, seg full/empty, drain
+  static constexpr int kNumBars = 2 + 2 * kRingK + 2 * kRingV + 4 + 4 + 2 + 2 + 3 + 2 * kSegs + 1;
   static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kOffMl = kOffSeg + kSegs * 64;   // [2 streams][128 rows] float2 (before that: Walk::Scratch)
   static constexpr int kOffMisc = kOffMl + 2 * kM * 8;  // abort flag, TMEM address
@@ -208,7 +208,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   uint64_t* v_empty = v_full + kRingV;    // [kRingV] two arrivals
   uint64_t* s_full = v_empty + kRingV;    // [2][2] MMA commit: S of the stream's step is in its buffer
   uint64_t* p_full = s_full + 4;          // [2][2] the stream's four softmax warps wrote P there
-  uint64_t* o_full = p_full + 4;          // [2] pairs: MMA commit after the stream's last P.V
+  uint64_t* pv_done = p_full + 4;         // [2] MMA commit after each P.V of the stream
+  uint64_t* o_full = pv_done + 2;         // [2] pairs: MMA commit after the stream's last P.V
   uint64_t* o_both = o_full + 2;          // singles: both streams' last P.V
   uint64_t* o_empty = o_both + 1;         // all eight softmax warps are done with the segment
   uint64_t* ml_full = o_empty + 1;        // singles: both streams' m and l are in shared memory
@@ -223,10 +224,11 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   const int cta = blockIdx.x;
 
   griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
+  prefetch_maps(mp, (int)threadIdx.x - 64);
   init_barriers(q_full, Ge::kNumBars, [&](int i) -> uint32_t {
     uint64_t* b = q_full + i;
     if (b == q_empty || b == o_both || b == drain || (b >= k_empty && b < v_full) || (b >= v_empty && b < s_full)) return 2;
-    return b >= p_full && b < o_full ? 4 : b == o_empty || b == ml_full ? 8 : b >= seg_empty ? kSegReaders : 1;
+    return b >= p_full && b < pv_done ? 4 : b == o_empty || b == ml_full ? 8 : b >= seg_empty ? kSegReaders : 1;
   });
   if (threadIdx.x == 0) {
     p.cuts[cta].nparts = 0;
@@ -304,7 +306,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         break;
       }
       ++nq;
-      int id = box_block(p, rq.kbase, rq.klen, g.j0, lane);
+      int id = box_block(mp, false, rq.kbase, rq.klen, g.j0, lane);
       const int nt = g.pair ? 2 : 1;
       if (mp.q_tma) {
         if (lane == 0) {
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       // a pair's neighbours read the same keys again: they stay in L2
       const uint64_t pol = g.pair ? pol_again : pol_once;
       for (int j = g.j0; j < g.j1; ++j) {
-        const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
+        const int id_next = j + 1 < g.j1 ? box_block(mp, false, rq.kbase, rq.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
         load_tile<KD>(mp, false, smem + Ge::kOffK + st * kTile, &k_full[st], j, walk.r, rq.kbase, rq.klen, g.kh, id, lane, pol);
@@ -359,9 +361,9 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       if (lane == 0) mbar_arrive(&seg_empty[ss]);
       if (!i.live) break;
       const uint64_t pol = i.pair ? pol_again : pol_once;
-      int id = i.m > 0 ? box_block(p, i.kbase, i.klen, i.j0, lane) : -1;
+      int id = i.m > 0 ? box_block(mp, true, i.kbase, i.klen, i.j0, lane) : -1;
       for (int j = i.j0; j < i.j0 + i.m; ++j) {
-        const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
+        const int id_next = j + 1 < i.j0 + i.m ? box_block(mp, true, i.kbase, i.klen, j + 1, lane) : -1;
         if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
         load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.req, i.kbase, i.klen, i.kh, id, lane, pol);
@@ -384,6 +386,9 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       const int x = warp == kWarpMmaB ? 1 : 0;
       const uint32_t t_s = tmem + x * kKT, t_o = tmem + 2 * kKT + x * kM;
       const uint32_t base = smem_u32(smem) >> 4;
+      // 16-byte units: from one half (64 keys) of a K/V tile to the other, and between its panels
+      const uint32_t half = (uint32_t)mp.group * 8 >> 4, panel = (uint32_t)mp.panel >> 4;
+      const uint32_t q_hi = desc_hi(1024), kv_hi = desc_hi((uint32_t)mp.group);
       uint64_t* const my_s = s_full + 2 * x;
       uint64_t* const my_p = p_full + 2 * x;
       uint32_t nq = 0;  // segments with keys
@@ -414,23 +419,18 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           if (!pair) mbar_arrive(empty);
         };
         const uint32_t q_lo = base + (uint32_t)((pair ? x : 0) * (kTile >> 4)) + (1u << 16);
-        // q.K^T of step i into its S buffer; step n is none: its commit tells
-        // that the P.V before it are done
-        auto qk = [&](int i) {
+        auto qk = [&](int i) {  // q.K^T of step i into its S buffer
           const int h = i & 1;
-          if (i < n) {
-            if (h == 0 && !poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
-            tc_fence_after();
-            const uint32_t k_lo =
-                base + (uint32_t)((Ge::kOffK + ks_ * kTile + h * (kHalf * 128)) >> 4) + (1u << 16);
+          if (h == 0 && !poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
+          tc_fence_after();
+          const uint32_t k_lo = base + (uint32_t)((Ge::kOffK + ks_ * kTile) >> 4) + (uint32_t)h * half + (1u << 16);
 #pragma unroll
-            for (int ks = 0; ks < KD / 16; ++ks) {
-              const uint32_t off = (uint32_t)((ks >> 2) * kPanel + (ks & 3) * 32) >> 4;
-              umma_f16_lo(t_s + h * kHalf, q_lo + off, k_lo + off, kIdQK, ks > 0 ? 1u : 0u);
-            }
-          }
+          for (int ks = 0; ks < KD / 16; ++ks)
+            umma_f16_lo(t_s + h * kHalf, q_lo + (uint32_t)(((ks >> 2) * kPanel + (ks & 3) * 32) >> 4), q_hi,
+                        k_lo + (uint32_t)(ks >> 2) * panel + (uint32_t)((ks & 3) * 32 >> 4), kv_hi, kIdQK,
+                        ks > 0 ? 1u : 0u);
           umma_commit(&my_s[h]);
-          if (i < n && (h || i == n - 1)) {
+          if (h || i == n - 1) {
             release(&k_empty[ks_]);
             advance<kRingK>(ks_, kp, stride);
             if (i == n - 1) umma_commit(q_empty);
@@ -442,7 +442,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           ++nq;
           if (ok && n == 0) mbar_arrive(q_empty);
         }
-        if (ok && n > 0) ok = qk(0) && qk(1);
+        if (ok && n > 0) ok = qk(0) && (n < 2 || qk(1));
         // the last segment's O has been read
         if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
         for (int i = 0; ok && i < n; ++i) {
@@ -452,13 +452,13 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           if (!ok) break;
           pp ^= 1u << h;
           tc_fence_after();
-          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile + h * (kHalf * 128)) >> 4) +
-                                ((uint32_t)(kPanel >> 4) << 16);
+          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (uint32_t)h * half + (panel << 16);
 #pragma unroll
           for (int ks = 0; ks < kHalf / 16; ++ks)
-            umma_f16_ts_lo(t_o, t_s + h * kHalf + 8 * ks, v_lo + (uint32_t)(ks * 2048 >> 4), kIdPV,
+            umma_f16_ts_lo(t_o, t_s + h * kHalf + 8 * ks, v_lo + (uint32_t)ks * (half / 4), kv_hi, kIdPV,
                            (i > 0 || ks > 0) ? 1u : 0u);
-          if (i + 2 <= n) ok = qk(i + 2);
+          umma_commit(&pv_done[x]);
+          if (i + 2 < n) ok = qk(i + 2);
           if (h || i == n - 1) {
             release(&v_empty[vs_]);
             advance<kRingV>(vs_, vp, stride);
@@ -493,7 +493,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     // ------------------------------------------------ softmax of stream x
     const int x = warp >> 2;
     const uint32_t t_s = tmem + ((uint32_t)((warp & 3) * 32) << 16) + x * kKT;
-    // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3)
+    // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3),
+    // pv_done of the step at hand (4)
     uint32_t ph = 0;
     bool ok = true;
     for (int nseg = 0; ok; ++nseg) {
@@ -542,9 +543,10 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           const float mxs = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.sl2;
           const bool grow = m != -INFINITY && mxs > m + 8.f;
           if (__any_sync(0xffffffffu, grow)) {
-            // O takes the earlier steps: the last one's P.V may still run; the
-            // commit of the next S follows it
-            ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * x + (h ^ 1)], (ph >> (h ^ 1)) & 1u, misc, p.err));
+            // O takes the earlier steps: the last one's P.V may still run (that
+            // of the one before it is done: this S's q.K^T was issued behind
+            // it, so the phase before the awaited one is known to have passed)
+            ok = __all_sync(0xffffffffu, wait_or_abort(&pv_done[x], ((ph >> 4) & 1u) ^ 1u, misc, p.err));
             if (!ok) break;
             tc_fence_after();
             const float alpha = grow ? exp2f(m - mxs) : 1.f;
@@ -587,10 +589,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         } else if (lane == 0) {
           mbar_arrive(&p_full[2 * x + h]);
         }
-      }
-      if (ok && n > 0) {  // the commit of step n, which holds no scores
-        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[2 * x + (n & 1)], (ph >> (n & 1)) & 1u, misc, p.err));
-        ph ^= 1u << (n & 1);
+        ph ^= 16u;
       }
       if (!ok) break;
       ok = __all_sync(0xffffffffu, finish_rows<T, KD>(p, seg, x, t_s, m, l, any_row, nseg, &ph, ml, o_empty, misc));
@@ -626,19 +625,40 @@ int launch(const MmaParams& mp, cudaStream_t s) {
 void encode_maps(MmaParams& mp, const fd_attn_args* a) {
   const AttnParams& p = mp.a;
   const int D = p.D;
+  mp.box_sh = 3;
+  while (mp.box_sh < 7 && (p.bt == nullptr || p.BS % (2 << mp.box_sh) == 0)) ++mp.box_sh;
+  // heads of 128 dims in small blocks: whole rows per copy, where every device
+  // tier's blocks are whole numbers of its heads' strides (both usual layouts)
+  bool by_lines = D == 128 && p.bt != nullptr && p.BS % kFine == 0 && mp.box_sh < 6;
+  for (int t = 0; t < 3; ++t)
+    if (p.nblk[t] > 0 && !(t < 2 && p.host[t]))
+      by_lines = by_lines && p.head_sb[t] > 0 && p.blk_sb[t] >= p.head_sb[t] && p.blk_sb[t] % p.head_sb[t] == 0 &&
+                 p.nblk[t] * (p.blk_sb[t] / p.head_sb[t]) < (1ll << 31);
+  mp.group = by_lines ? 2048 : 1024;
+  mp.panel = by_lines ? 1024 : kPanel;
   mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
   for (int t = 0; t < 3; ++t) {
     if (p.nblk[t] == 0 || (t < 2 && p.host[t])) continue;
     const bool cross = p.bt == nullptr;
     if (cross && p.nblk[t] > 0x7fffffff) continue;  // rows by 16-byte loads
-    if (!cross && p.BS % kSub != 0) continue;
+    if (!cross && p.BS % kFine != 0) continue;
     const int rows = cross ? (int)p.nblk[t] : p.BS;
     const int64_t blocks = cross ? 1 : p.nblk[t];
     const int64_t blk_sb = cross ? p.tok_sb[t] * rows : p.blk_sb[t];
-    mp.kv_tma[t] = encode_kv_map(&mp.tmap_k[t], p.k[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
-                                 blk_sb, kSub, true) &&
-                   encode_kv_map(&mp.tmap_v[t], p.v[t], a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t],
-                                 blk_sb, kSub, true);
+    auto map = [&](CUtensorMap* m, const unsigned char* base, int keys) {
+      return encode_kv_map(m, base, a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t], blk_sb, keys, true);
+    };
+    if (by_lines) {
+      mp.lines[t] = (int)(p.blk_sb[t] / p.head_sb[t]);
+      auto lines = [&](CUtensorMap* m, const unsigned char* base) {
+        return encode_kv_lines(m, base, a->dtype, p.BS, (p.nblk[t] - 1) * mp.lines[t] + p.KVH, p.head_sb[t], p.tok_sb[t],
+                               1 << mp.box_sh);
+      };
+      mp.kv_tma[t] = lines(&mp.tmap_k[t], p.k[t]) && lines(&mp.tmap_v[t], p.v[t]);
+    } else {
+      mp.kv_tma[t] = map(&mp.tmap_k[t], p.k[t], 1 << mp.box_sh) && map(&mp.tmap_v[t], p.v[t], 1 << mp.box_sh);
+    }
+    mp.kv_tma[t] = mp.kv_tma[t] && map(&mp.tmap_vf[t], p.v[t], kFine);
   }
 }
 

@@ -13,15 +13,27 @@ namespace mm {
 
 constexpr int kKT = 128;            // keys per K/V tile
 constexpr int kWhole = 8;           // key tiles up to which no item is cut (whole_items)
-constexpr int kSub = 16;            // keys per TMA box
-constexpr int kSubs = kKT / kSub;
+constexpr int kFine = 8;            // keys per TMA box at a request's end, and per box of plain loads
+constexpr int kFines = kKT / kFine;
 constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims of 16 bits
 
 struct MmaParams {
   CUtensorMap tmap_q;       // {D, H, T, 1}, box {64, G, tq, 1}
-  CUtensorMap tmap_k[3];    // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}), box {64, 1, 16, 1}
+  // per tier {D, KVH, BS, blocks} (cross: {D, KVH, rows, 1}): boxes {64, 1,
+  // 2^box_sh, 1} of whole tiles, and of kFine keys for the tile that holds the end of V
+  CUtensorMap tmap_k[3];
   CUtensorMap tmap_v[3];
+  CUtensorMap tmap_vf[3];
   AttnParams a;
+  int box_sh;               // log2 of the keys per box: the largest power of two (8 to 128) that divides a block
+  // Layout of a K/V tile in shared memory: groups of 8 keys `group` bytes
+  // apart, the second 64 dims `panel` bytes behind the first.  One TMA copy
+  // takes one 64-dim panel of a box (1024, kPanel), or, of heads of 128 dims,
+  // whole rows (2048, 1024: the maps are encode_kv_lines', a block
+  // of tier t having lines[t] lines): an SM's copies come at ~80 cycles apiece
+  // whatever their size, and boxes of 16 keys leave no slack at 2 KB each.
+  int group, panel;
+  int lines[3];
   int q_tma, kv_tma[3];     // the view has a tensor map
 };
 
@@ -113,26 +125,38 @@ __device__ __forceinline__ void advance(int& slot, uint32_t& phase, int by) {
 }
 
 // The products with 128-byte swizzled operands, descriptors by their low
-// words (address and leading offset, 16-byte units); the high word (stride
-// 1024 bytes, version, swizzle) is the same for all of them.
-constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
-__device__ __forceinline__ void umma_f16_lo(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t acc) {
+// words (address and leading offset, 16-byte units) and high words (stride of
+// the 8-row groups, version, swizzle).
+__device__ __forceinline__ uint32_t desc_hi(uint32_t group) { return (group >> 4) | (1u << 14) | (2u << 29); }
+__device__ __forceinline__ void umma_f16_lo(uint32_t d, uint32_t a_lo, uint32_t a_hi, uint32_t b_lo, uint32_t b_hi,
+                                            uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\t"
-      "mov.b64 a, {%1, %5};\n\tmov.b64 b, {%2, %5};\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      "mov.b64 a, {%1, %2};\n\tmov.b64 b, {%3, %4};\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %5, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(a_hi), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(acc)
       : "memory");
 }
-__device__ __forceinline__ void umma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
-                                               uint32_t acc) {
+__device__ __forceinline__ void umma_f16_ts_lo(uint32_t d, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi,
+                                               uint32_t idesc, uint32_t acc) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t.reg .b64 b;\n\t"
       "mov.b64 b, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
       "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}" ::"r"(d),
-      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(kDescHi)
+      "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"(acc), "r"(b_hi)
+      : "memory");
+}
+
+// Tiled TMA load of a 5-D box (see tma_load_4d).
+__device__ __forceinline__ void tma_load_5d(void* smem_dst, const CUtensorMap* map, int c0, int c1, int c2, int c3,
+                                            int c4, uint64_t* bar, uint64_t policy) {
+  asm volatile(
+      "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
+      "[%0], [%1, {%2, %3, %4, %5, %6}], [%7], %8;" ::"r"(smem_u32(smem_dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(c4), "r"(smem_u32(bar)),
+      "l"(policy)
       : "memory");
 }
 
@@ -143,23 +167,54 @@ __device__ __forceinline__ void stg256(void* p, const uint32_t (&v)[8]) {
                : "memory");
 }
 
-// Block id of box `lane` (keys 128 j + 16 lane ..) where boxes lie within
-// blocks, -1 where there is none.  Read one tile ahead of its use.
-__device__ __forceinline__ int box_block(const AttnParams& p, int kbase, int klen, int j, int lane) {
-  const int t = j * kKT + lane * kSub;
-  if (p.bt == nullptr || p.BS % kSub != 0 || lane >= kSubs || t >= klen) return -1;
+// Fetch the tensor maps that the call's loads use (one thread per map).
+__device__ __forceinline__ void prefetch_maps(const MmaParams& mp, int x) {
+  const CUtensorMap* map = nullptr;
+  if (x >= 0 && x < 9) {
+    const int t = x / 3;
+    if (mp.kv_tma[t]) map = x % 3 == 0 ? &mp.tmap_k[t] : x % 3 == 1 ? &mp.tmap_v[t] : &mp.tmap_vf[t];
+  } else if (x == 9 && mp.q_tma) {
+    map = &mp.tmap_q;
+  }
+  if (map != nullptr) asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
+}
+
+// The box of key tile j that lane `lane` loads: its first key (of the tile)
+// and its keys.  Lanes below 16 have the boxes of 2^box_sh keys; for V, whose
+// rows behind the request's end must be 0, lanes 16 .. have the kFine-key
+// pieces of a large box that the end cuts (of a box of up to 32 keys, plain
+// loads fetch them as fast).
+struct Box {
+  int at, keys;  // keys = 0: none
+};
+__device__ __forceinline__ Box box_of(const MmaParams& mp, bool is_v, int left, int lane) {  // left: klen - 128 j
+  const int sh = mp.box_sh;
+  if (lane < 16) return {lane << sh, (lane << sh) < kKT ? 1 << sh : 0};
+  const int cut = left >> sh, at = (cut << sh) + (lane - 16) * kFine;  // the box that is cut, if any
+  return {at, is_v && left < kKT && at + kFine <= left && sh > 5 ? kFine : 0};
+}
+
+// Block id of this lane's box where boxes lie within blocks, -1 where there
+// is none.  Read one tile ahead of its use.
+__device__ __forceinline__ int box_block(const MmaParams& mp, bool is_v, int kbase, int klen, int j, int lane) {
+  const AttnParams& p = mp.a;
+  const Box box = box_of(mp, is_v, klen - j * kKT, lane);
+  const int t = j * kKT + box.at;
+  if (p.bt == nullptr || p.BS % kFine != 0 || box.keys == 0 || t >= klen) return -1;
   return p.bt[(int64_t)kbase * p.bt_stride + t / p.BS];
 }
 
 // One warp: K or V of key tile j into `dst`, completion on `bar` (bytes of
-// the TMA boxes, and lane 0's arrival once the other boxes are stored).
+// the TMA boxes, and lane 0's arrival once what TMA does not load is stored).
 template <int KD>
 __device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsigned char* dst, uint64_t* bar, int j,
                                           int r, int kbase, int klen, int kh, int id, int lane, uint64_t pol) {
   const AttnParams& p = mp.a;
-  const int t = j * kKT + lane * kSub;
-  const bool boxed = p.bt == nullptr || p.BS % kSub == 0;
-  bool in = lane < kSubs && t < klen;  // the box holds a key
+  const int sh = mp.box_sh, left = klen - j * kKT;
+  const Box box = box_of(mp, is_v, left, lane);
+  const int t = j * kKT + box.at;
+  const bool boxed = p.bt == nullptr || p.BS % kFine == 0;
+  bool in = box.keys > 0 && t < klen;  // the box holds a key
   int tier = 0, blk = 0, r0 = 0;
   bool tma = false;
   if (in && boxed) {
@@ -176,54 +231,80 @@ __device__ __forceinline__ void load_tile(const MmaParams& mp, bool is_v, unsign
       }
       blk = (int)b;
     }
-    tma = in && mp.kv_tma[tier] && (!is_v || t + kSub <= klen);
+    tma = in && mp.kv_tma[tier] && (!is_v || box.at + box.keys <= left);
   }
   const unsigned tmask = __ballot_sync(0xffffffffu, tma);
-  const unsigned all = (1u << kSubs) - 1u;
-  // K boxes without a key need nothing (the mask replaces their scores)
-  unsigned rest = is_v ? all & ~tmask : __ballot_sync(0xffffffffu, in) & ~tmask;
-  if (lane == 0) mbar_expect_tx(bar, (uint32_t)__popc(tmask) * (uint32_t)(KD / 64 * kSub * 128));
+  if (lane == 0)
+    mbar_expect_tx(bar, (uint32_t)(KD / 64 * 128) * (((uint32_t)__popc(tmask & 0xffffu) << sh) +
+                                                     (uint32_t)__popc(tmask >> 16) * (uint32_t)kFine));
   __syncwarp();
-  if (tma) {
+  unsigned char* const to = dst + (box.at >> 3) * mp.group;
+  if (tma && lane < 16) {
     const CUtensorMap* map = is_v ? &mp.tmap_v[tier] : &mp.tmap_k[tier];
+    if (KD == 128 && mp.group == 2048) {
+      tma_load_5d(to, map, 0, 0, 0, r0 >> 3, blk * mp.lines[tier] + kh, bar, pol);
+    } else {
+#pragma unroll
+      for (int x = 0; x < KD / 64; ++x) tma_load_4d(to + x * mp.panel, map, 64 * x, kh, r0, blk, bar, pol);
+    }
+  }
+  if (tmask >> 16 != 0u && tma && lane >= 16) {
 #pragma unroll
     for (int x = 0; x < KD / 64; ++x)
-      tma_load_4d(dst + x * kPanel + lane * kSub * 128, map, 64 * x, kh, r0, blk, bar, pol);
+      tma_load_4d(to + x * mp.panel, &mp.tmap_vf[tier], 64 * x, kh, r0, blk, bar, pol);
   }
-  if (rest != 0u) {
-    constexpr int kCh = KD / 8;                   // 16-byte chunks per row
-    constexpr int kPer = kSub * kCh / 32;         // chunks of a box per lane
-    while (rest != 0u) {
-      const int s = __ffs(rest) - 1;
-      rest &= rest - 1u;
-      const bool box_in = __shfl_sync(0xffffffffu, (int)in, s) != 0;
-      const int box_tier = __shfl_sync(0xffffffffu, tier, s);
-      const int box_blk = __shfl_sync(0xffffffffu, blk, s);
-      const int box_r0 = __shfl_sync(0xffffffffu, r0, s);
-      uint4 v[kPer];
+  // kFine-key pieces that no TMA box covers: K's without a key need nothing
+  // (the mask replaces their scores), V's are zeros
+  const unsigned imask = __ballot_sync(0xffffffffu, in);
+  const int owner = lane >> (sh - 3);  // the box that piece `lane` lies in
+  const int fine = 16 + lane - ((left >> sh) << (sh - 3));
+  const bool covered = ((tmask >> owner) & 1u) || (fine >= 16 && fine < 32 && ((tmask >> fine) & 1u));
+  unsigned need = __ballot_sync(0xffffffffu, lane < kFines && !covered && (is_v || lane * kFine < left));
+  if (need != 0u) {
+    constexpr int kCh = KD / 8;             // 16-byte chunks per row
+    constexpr int kPer = kFine * kCh / 32;  // chunks of a piece per lane
+    constexpr int kPair = 2;                // pieces in flight
+#pragma unroll 1
+    while (need != 0u) {
+      uint4 v[kPair][kPer];
+      int piece[kPair];
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
-        const int key = j * kKT + s * kSub + row;
-        v[c] = make_uint4(0u, 0u, 0u, 0u);
-        if (!box_in || key >= klen || ch * 8 >= p.D) continue;
-        int tr = box_tier, rr = box_r0 + row;
-        int64_t b = box_blk;
-        if (!boxed) {
-          const int page = key / p.BS;
-          b = p.bt[(int64_t)kbase * p.bt_stride + page];
-          rr = key - page * p.BS;
-          tr = locate(p, r, page, b);
-          if (tr < 0) continue;
+      for (int w = 0; w < kPair; ++w) {
+        piece[w] = __ffs(need) - 1;  // -1: none
+        need &= need - 1u;
+        const int own = max(piece[w], 0) >> (sh - 3);
+        const bool have = piece[w] >= 0 && ((imask >> own) & 1u);
+        const int box_tier = __shfl_sync(0xffffffffu, tier, own);
+        const int box_blk = __shfl_sync(0xffffffffu, blk, own);
+        const int box_r0 = __shfl_sync(0xffffffffu, r0, own) + piece[w] * kFine - (own << sh);
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+          const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
+          const int key = j * kKT + piece[w] * kFine + row;
+          v[w][c] = make_uint4(0u, 0u, 0u, 0u);
+          if (!have || key >= klen || ch * 8 >= p.D) continue;
+          int tr = box_tier, rr = box_r0 + row;
+          int64_t b = box_blk;
+          if (!boxed) {
+            const int page = key / p.BS;
+            b = p.bt[(int64_t)kbase * p.bt_stride + page];
+            rr = key - page * p.BS;
+            tr = locate(p, r, page, b);
+            if (tr < 0) continue;
+          }
+          const unsigned char* base = is_v ? p.v[tr] : p.k[tr];
+          v[w][c] = *reinterpret_cast<const uint4*>(base + b * p.blk_sb[tr] + kh * p.head_sb[tr] +
+                                                    (int64_t)rr * p.tok_sb[tr] + ch * 16);
         }
-        const unsigned char* base = is_v ? p.v[tr] : p.k[tr];
-        v[c] = *reinterpret_cast<const uint4*>(base + b * p.blk_sb[tr] + kh * p.head_sb[tr] +
-                                               (int64_t)rr * p.tok_sb[tr] + ch * 16);
       }
 #pragma unroll
-      for (int c = 0; c < kPer; ++c) {
-        const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
-        sts128(dst + (ch >> 3) * kPanel + swz(s * kSub + row, ch & 7), v[c]);
+      for (int w = 0; w < kPair; ++w) {
+        if (piece[w] < 0) continue;
+#pragma unroll
+        for (int c = 0; c < kPer; ++c) {
+          const int idx = c * 32 + lane, row = idx / kCh, ch = idx % kCh;
+          sts128(dst + piece[w] * mp.group + (ch >> 3) * mp.panel + swz(row, ch & 7), v[w][c]);
+        }
       }
     }
     fence_proxy_async_smem();  // the stores before the tensor cores read the slot

@@ -16,8 +16,9 @@
 // first tile, the 128 threads take the column's maximum together and rescale
 // O); the sums l stay with their threads until the segment's end.
 //
-// A CTA walks its range of the schedule (fd_attn.cuh); seven warps: 0-3
-// softmax, 4 schedule, Q and K tiles, 5 V tiles, 6 (one thread) the MMAs,
+// A CTA walks its range of the schedule (fd_attn.cuh); eight warps: 0-3
+// softmax, 4 schedule and Q tiles (segments ahead, so that the loads never
+// wait for its arithmetic), 5 and 6 K and V tiles, 7 (one thread) the MMAs,
 // q.K^T two tiles ahead of P.V over two S and two P buffers.  Heads of 64 dims
 // take half of the shared memory, and two CTAs share an SM: one's loads run
 // on while the other changes from one request to the next.
@@ -37,11 +38,11 @@ namespace rw {
 
 using namespace mm;
 
-constexpr int kWarpK = 4, kWarpV = 5, kWarpMma = 6;
-constexpr int kThreads = 7 * 32;
+constexpr int kWarpSched = 4, kWarpK = 5, kWarpV = 6, kWarpMma = 7;
+constexpr int kThreads = 8 * 32;
 constexpr int kSoft = 4 * 32;       // softmax threads
 constexpr int kSegs = 4;            // segments in flight between the roles
-constexpr int kSegReaders = 6;      // MMA thread, V producer, four softmax warps
+constexpr int kSegReaders = 7;      // MMA thread, two producers, four softmax warps
 constexpr int kMaxCtas = 320;
 constexpr int kFixed = 2;           // an item's fixed cost in key tiles
 constexpr int kMinPer = 4;          // least positions of a CTA
@@ -61,12 +62,13 @@ struct Geo {
   static constexpr int kOffQ = kOffV + kRingV * kTile;
   static constexpr int kOffP = kOffQ + 2 * kQ;
   static constexpr int kOffBar = kOffP + 2 * kP;
-  // k full/empty, v full/empty, q full/empty[2], s_full[2], p_full[2], o_full, o_empty, seg full/empty, drain
-  static constexpr int kNumBars = 2 * kRingK + 2 * kRingV + 4 + 2 + 2 + 2 + 2 * kSegs + 1;
+  // k full/empty, v full/empty, q full/empty[2], s_full[2], p_full[2], pv_done, o_full, o_empty, seg full/empty, drain
+  static constexpr int kNumBars = 2 * kRingK + 2 * kRingV + 4 + 2 + 2 + 3 + 2 * kSegs + 1;
   static constexpr int kOffSeg = (kOffBar + kNumBars * 8 + 15) / 16 * 16;
   static constexpr int kOffRed = kOffSeg + kSegs * 64;   // [4 warps][N] maxima, then sums (before that: Walk::Scratch)
   static constexpr int kOffM = kOffRed + 4 * N * 4 + 512;  // [N] m, then [N] factors of l and O
-  static constexpr int kOffMisc = kOffM + 2 * N * 4;     // abort flag, TMEM address
+  static constexpr int kOffRow = kOffM + 2 * N * 4;      // [N] where the segment's rows go
+  static constexpr int kOffMisc = kOffRow + N * 8;       // abort flag, TMEM address
   static constexpr int kSmem = kOffMisc + 16;
   static_assert(kSmem <= (KD == 64 ? 113 : 227) * 1024, "smem budget");
 };
@@ -125,12 +127,6 @@ __device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[32]) { tmem_
 __device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[16]) { tmem_st16(t, r); }
 __device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[32]) { tmem_st32(t, r); }
 
-__device__ __forceinline__ void tmem_ld4_nowait(uint32_t t, uint32_t (&r)[4]) {
-  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
-               : "r"(t));
-}
-
 template <typename T, int KD, int N>
 __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kernel(const __grid_constant__ MmaParams mp) {
   typedef Geo<KD, N> Ge;
@@ -138,8 +134,6 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdQK = instr_desc(kBF16, false, kKT, N);
   constexpr uint32_t kIdPV = instr_desc(kBF16, true, 128, N);  // V: MN-major A
-  // V's second 64 dims; heads of 64 dims have the first ones twice (rows 64 .. 127 of O^T are not read)
-  constexpr uint32_t kLbo = KD == 128 ? (uint32_t)(kPanel >> 4) : 0u;
   const AttnParams& p = mp.a;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);
@@ -150,7 +144,8 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
   uint64_t* q_empty = q_full + 2;          // [2] MMA commit after a segment's last q.K^T
   uint64_t* s_full = q_empty + 2;          // [2] MMA commit: S of a tile
   uint64_t* p_full = s_full + 2;           // [2] the four softmax warps wrote P
-  uint64_t* o_full = p_full + 2;           // MMA commit after a segment's last P.V
+  uint64_t* pv_done = p_full + 2;          // MMA commit after each P.V
+  uint64_t* o_full = pv_done + 1;          // MMA commit after a segment's last P.V
   uint64_t* o_empty = o_full + 1;          // the four softmax warps are done with the segment
   uint64_t* seg_full = o_empty + 1;        // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;  // [kSegs]
@@ -159,14 +154,16 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
   float* red = reinterpret_cast<float*>(smem + Ge::kOffRed);
   float* m_sh = reinterpret_cast<float*>(smem + Ge::kOffM);
   float* f_sh = m_sh + N;
+  int64_t* row_sh = reinterpret_cast<int64_t*>(smem + Ge::kOffRow);
   volatile int* misc = reinterpret_cast<volatile int*>(smem + Ge::kOffMisc);  // [0] abort, [1] TMEM address
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int cta = blockIdx.x;
   griddep_launch_dependents();  // the combine's CTAs may start, and wait for this grid's end
+  prefetch_maps(mp, (int)threadIdx.x - 64);
   init_barriers(k_full, Ge::kNumBars, [&](int i) -> uint32_t {
     uint64_t* b = k_full + i;
-    return b >= p_full && b < o_full ? 4 : b == o_empty ? 4 : b >= seg_empty && b < drain ? kSegReaders : 1;
+    return (b >= p_full && b < pv_done) || b == o_empty ? 4 : b >= seg_empty && b < drain ? kSegReaders : 1;
   });
   if (threadIdx.x == 0) {
     p.cuts[cta].nparts = 0;
@@ -190,17 +187,14 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
   tc_fence_after();
   const uint32_t tmem = (uint32_t)misc[1];
 
-  if (warp == kWarpK) {
-    // ------------------------------------------------ schedule, Q and K tiles
-    const uint64_t pol = l2_evict_first_policy();
-    int nseg = 0, nq = 0, st = 0;
-    uint32_t tiles = 0, ph = 0;
+  if (warp == kWarpSched) {
+    // ------------------------------------------------ schedule and Q tiles
+    int nseg = 0, nq = 0;
     bool ok = true;
     Walk::Seg g;
     while (ok) {
       const bool more = walk.next(g);
       const Req rq = walk.rq;
-      int id = more && g.j0 < g.j1 ? box_block(p, rq.kbase, rq.klen, g.j0, lane) : -1;
       const int ss = nseg % kSegs;
       if (nseg >= kSegs)
         ok = __all_sync(0xffffffffu, wait_or_abort(&seg_empty[ss], (uint32_t)(nseg / kSegs - 1) & 1u, misc, p.err));
@@ -220,9 +214,9 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           i.kbase = rq.kbase;
           i.kh = g.kh;
           i.slot = g.whole ? -1 : 2 * cta + (g.j0 > 0 ? 0 : 1);
-          if (g.nparts > 0) p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, min(p.tq, rq.qlen - tok0) * p.G, g.kh};
         }
         mbar_arrive(&seg_full[ss]);
+        if (more && g.nparts > 0) p.cuts[cta] = Cut{g.nparts, rq.qst + tok0, min(p.tq, rq.qlen - tok0) * p.G, g.kh};
       }
       __syncwarp();
       ++nseg;
@@ -247,14 +241,51 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_full[qb]);
       }
-      for (int j = g.j0; j < g.j1; ++j) {
-        const int id_next = j + 1 < g.j1 ? box_block(p, rq.kbase, rq.klen, j + 1, lane) : -1;
-        if (tiles >= (uint32_t)kRingK) ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[st], ph ^ 1u, misc, p.err));
+    }
+    if (!ok) misc[0] = 1;
+    // no copy of this warp is in flight when the CTA ends
+    for (int b = 0; b < 2 && b < nq; ++b) mbar_wait(&q_full[b], (uint32_t)((nq - 1 - b) / 2) & 1u, p.err);
+  } else if (warp == kWarpK || warp == kWarpV) {
+    // ------------------------------------------------ K or V tiles
+    const bool is_v = warp == kWarpV;
+    const int ring = is_v ? kRingV : kRingK;
+    uint64_t* const full = is_v ? v_full : k_full;
+    uint64_t* const empty = is_v ? v_empty : k_empty;
+    unsigned char* const slots = smem + (is_v ? Ge::kOffV : 0);
+    const uint64_t pol = l2_evict_first_policy();
+    int st = 0, nseg = 0;
+    uint32_t tiles = 0, ph = 0;
+    // the next segment, and the block ids of its first tile on their way:
+    // taken before the last tile of the one before is loaded
+    SegInfo seg;
+    int first_id = -1;
+    auto take = [&]() {
+      const int ss = nseg % kSegs;
+      if (!__all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err)))
+        return false;
+      seg = segs[ss];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&seg_empty[ss]);
+      ++nseg;
+      first_id = seg.live && seg.m > 0 ? box_block(mp, is_v, seg.kbase, seg.klen, seg.j0, lane) : -1;
+      return true;
+    };
+    bool ok = take();
+    while (ok && seg.live) {
+      const SegInfo i = seg;
+      int id = first_id;
+      if (i.m == 0) ok = take();
+      for (int j = i.j0; j < i.j0 + i.m; ++j) {
+        const bool last = j + 1 == i.j0 + i.m;
+        const int id_next = last ? -1 : box_block(mp, is_v, i.kbase, i.klen, j + 1, lane);
+        if (last) ok = take();
+        if (ok && tiles >= (uint32_t)ring)
+          ok = __all_sync(0xffffffffu, wait_or_abort(&empty[st], ph ^ 1u, misc, p.err));
         if (!ok) break;
-        load_tile<KD>(mp, false, smem + st * kTile, &k_full[st], j, walk.r, rq.kbase, rq.klen, g.kh, id, lane, pol);
+        load_tile<KD>(mp, is_v, slots + st * kTile, &full[st], j, i.req, i.kbase, i.klen, i.kh, id, lane, pol);
         id = id_next;
         ++tiles;
-        if (++st == kRingK) {
+        if (++st == ring) {
           st = 0;
           ph ^= 1u;
         }
@@ -262,48 +293,19 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
     }
     if (!ok) misc[0] = 1;
     // no copy of this warp is in flight when the CTA ends
-    for (uint32_t s = 0; s < (uint32_t)kRingK && s < tiles; ++s) {
-      const uint32_t last = s + kRingK * ((tiles - 1 - s) / kRingK);
-      mbar_wait(&k_full[s], (last / kRingK) & 1u, p.err);
-    }
-    for (int b = 0; b < 2 && b < nq; ++b) mbar_wait(&q_full[b], (uint32_t)((nq - 1 - b) / 2) & 1u, p.err);
-  } else if (warp == kWarpV) {
-    // ------------------------------------------------ V tiles
-    const uint64_t pol = l2_evict_first_policy();
-    int st = 0;
-    uint32_t tiles = 0, ph = 0;
-    bool ok = true;
-    for (int nseg = 0; ok; ++nseg) {
-      const int ss = nseg % kSegs;
-      ok = __all_sync(0xffffffffu, wait_or_abort(&seg_full[ss], (uint32_t)(nseg / kSegs) & 1u, misc, p.err));
-      if (!ok) break;
-      const SegInfo i = segs[ss];
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&seg_empty[ss]);
-      if (!i.live) break;
-      int id = i.m > 0 ? box_block(p, i.kbase, i.klen, i.j0, lane) : -1;
-      for (int j = i.j0; j < i.j0 + i.m; ++j) {
-        const int id_next = j + 1 < i.j0 + i.m ? box_block(p, i.kbase, i.klen, j + 1, lane) : -1;
-        if (tiles >= (uint32_t)kRingV) ok = __all_sync(0xffffffffu, wait_or_abort(&v_empty[st], ph ^ 1u, misc, p.err));
-        if (!ok) break;
-        load_tile<KD>(mp, true, smem + Ge::kOffV + st * kTile, &v_full[st], j, i.req, i.kbase, i.klen, i.kh, id, lane, pol);
-        id = id_next;
-        ++tiles;
-        if (++st == kRingV) {
-          st = 0;
-          ph ^= 1u;
-        }
-      }
-    }
-    if (!ok) misc[0] = 1;
-    for (uint32_t s = 0; s < (uint32_t)kRingV && s < tiles; ++s) {
-      const uint32_t last = s + kRingV * ((tiles - 1 - s) / kRingV);
-      mbar_wait(&v_full[s], (last / kRingV) & 1u, p.err);
+    for (uint32_t s = 0; s < (uint32_t)ring && s < tiles; ++s) {
+      const uint32_t last = s + ring * ((tiles - 1 - s) / ring);
+      mbar_wait(&full[s], (last / ring) & 1u, p.err);
     }
   } else if (warp == kWarpMma) {
     // ------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t base = smem_u32(smem) >> 4;
+      // 16-byte units: 16 keys of a K/V tile on, and from its first 64 dims to
+      // the second; heads of 64 dims have V's twice (rows 64 .. 127 of O^T are not read)
+      const uint32_t two = (uint32_t)mp.group * 2 >> 4, panel = (uint32_t)mp.panel >> 4;
+      const uint32_t lbo = KD == 128 ? panel : 0u;
+      const uint32_t q_hi = desc_hi(1024), kv_hi = desc_hi((uint32_t)mp.group);
       int ks_ = 0, vs_ = 0, nq = 0;
       uint32_t kp = 0, vp = 0, pp = 0;  // ring phases; parities of p_full's two buffers
       bool ok = true;
@@ -316,29 +318,24 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         if (!live) break;
         const int qb = nq & 1;
         const uint32_t q_lo = base + (uint32_t)((Ge::kOffQ + qb * Ge::kQ) >> 4) + (1u << 16);
-        // q.K^T of tile t; tile m is none: its commit tells that the P.V before it are done
-        auto qk = [&](int t) {
-          if (t < m) {
-            if (!poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
-            tc_fence_after();
-            const uint32_t k_lo = base + (uint32_t)((ks_ * kTile) >> 4) + (1u << 16);
+        auto qk = [&](int t) {  // q.K^T of tile t
+          if (!poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
+          tc_fence_after();
+          const uint32_t k_lo = base + (uint32_t)((ks_ * kTile) >> 4) + (1u << 16);
 #pragma unroll
-            for (int ks = 0; ks < KD / 16; ++ks)
-              umma_f16_lo(tmem + 32 * (t & 1), k_lo + (uint32_t)(((ks >> 2) * kPanel + (ks & 3) * 32) >> 4),
-                          q_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), kIdQK, ks > 0 ? 1u : 0u);
-          }
+          for (int ks = 0; ks < KD / 16; ++ks)
+            umma_f16_lo(tmem + 32 * (t & 1), k_lo + (uint32_t)(ks >> 2) * panel + (uint32_t)((ks & 3) * 32 >> 4), kv_hi,
+                        q_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), q_hi, kIdQK, ks > 0 ? 1u : 0u);
           umma_commit(&s_full[t & 1]);
-          if (t < m) {
-            umma_commit(&k_empty[ks_]);
-            advance<kRingK>(ks_, kp, 1);
-            if (t == m - 1) umma_commit(&q_empty[qb]);
-          }
+          umma_commit(&k_empty[ks_]);
+          advance<kRingK>(ks_, kp, 1);
+          if (t == m - 1) umma_commit(&q_empty[qb]);
           return true;
         };
         if (m > 0) {
           ok = poll_or_abort(&q_full[qb], (uint32_t)(nq / 2) & 1u, misc, p.err);
           ++nq;
-          ok = ok && qk(0) && qk(1);
+          ok = ok && qk(0) && (m < 2 || qk(1));
         }
         // the last segment's O has been read
         if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
@@ -348,14 +345,15 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           if (!ok) break;
           pp ^= 1u << h;
           tc_fence_after();
-          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (kLbo << 16);
+          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (lbo << 16);
           const uint32_t p_lo = base + (uint32_t)((Ge::kOffP + h * Ge::kP) >> 4) + (1u << 16);
 #pragma unroll
           for (int ks = 0; ks < kKT / 16; ++ks)
-            umma_f16_lo(tmem + kOcol, v_lo + (uint32_t)(ks * 2048 >> 4),
-                        p_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), kIdPV,
+            umma_f16_lo(tmem + kOcol, v_lo + (uint32_t)ks * two, kv_hi,
+                        p_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), q_hi, kIdPV,
                         (t > 0 || ks > 0) ? 1u : 0u);
-          if (t + 2 <= m) ok = qk(t + 2);
+          umma_commit(pv_done);
+          if (t + 2 < m) ok = qk(t + 2);
           umma_commit(&v_empty[vs_]);
           advance<kRingV>(vs_, vp, 1);
         }
@@ -370,7 +368,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
     // ------------------------------------------------ softmax: one key per thread, then one dim
     const int tid = threadIdx.x;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
-    uint32_t ph = 0;  // phase parities of s_full (bits 0, 1) and o_full (2)
+    uint32_t ph = 0;  // phase parities of s_full (bits 0, 1), o_full (2), pv_done of the tile at hand (3)
     bool ok = true;
     for (int nseg = 0;; ++nseg) {
       const int ss = nseg % kSegs;
@@ -414,8 +412,10 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           }
         }
         if (sync_or(past || !ok)) {
-          // O takes the earlier tiles: the commit of the next S follows the last one's P.V
-          ok = ok && (t == 0 || wait_or_abort(&s_full[h ^ 1], (ph >> (h ^ 1)) & 1u, misc, p.err));
+          // O takes the earlier tiles: P.V of the last one may still run (that
+          // of the one before it is done: this S's q.K^T was issued behind it,
+          // so the phase before the awaited one is known to have passed)
+          ok = ok && (t == 0 || wait_or_abort(pv_done, ((ph >> 3) & 1u) ^ 1u, misc, p.err));
           __syncwarp();
 #pragma unroll
           for (int n = 0; n < N; ++n) {
@@ -466,13 +466,13 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(&p_full[h]);
+        ph ^= 8u;
       }
       if (!ok) break;
       // the segment's end: sums over the keys' threads, then rows
       if (m_tiles > 0) {
-        const int e = m_tiles & 1;  // the commit of tile m_tiles, which holds no scores
-        ok = wait_or_abort(&s_full[e], (ph >> e) & 1u, misc, p.err) && wait_or_abort(o_full, (ph >> 2) & 1u, misc, p.err);
-        ph ^= (1u << e) | 4u;
+        ok = wait_or_abort(o_full, (ph >> 2) & 1u, misc, p.err);
+        ph ^= 4u;
         __syncwarp();
       }
       const float sum = column_sum<N>(l, lane);
@@ -484,51 +484,53 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       tc_fence_after();
       const int rows = min(p.tq, seg.qlen - seg.tok0) * p.G;
       const int slot = seg.slot;
-      const int64_t tok0 = seg.qst + seg.tok0;
       if (tid < N) {
         const float lt = red[tid] + red[N + tid] + red[2 * N + tid] + red[3 * N + tid];
         const float mt = m_tiles > 0 ? m_sh[tid] : -INFINITY;
         f_sh[tid] = slot >= 0 ? 1.f : lt > 0.f ? 1.f / lt : 0.f;
+        const int t = tid / p.G, h = seg.kh * p.G + tid - t * p.G;
+        const int64_t tok = seg.qst + seg.tok0 + t;
+        row_sh[tid] = tok * p.o_st + h * p.o_sh;
         if (tid < rows) {
           if (slot >= 0)
             reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * N + tid] = make_float2(mt, lt);
           else if (p.lse != nullptr)
-            p.lse[(seg.kh * p.G + tid % p.G) * p.lse_sh + (tok0 + tid / p.G) * p.lse_st] =
-                lt > 0.f ? (mt + log2f(lt)) * kLn2 : -INFINITY;
+            p.lse[h * p.lse_sh + tok * p.lse_st] = lt > 0.f ? (mt + log2f(lt)) * kLn2 : -INFINITY;
         }
       }
-      sync_or(false);
-      // thread `tid` has dim `tid` of every row; four rows at a time
-      unsigned char* po = p.out + tok0 * p.o_st + (int64_t)(seg.kh * p.G) * p.o_sh + tid * 2;
-      float* pp = p.part_o + (((int64_t)slot * (p.D / 4) + (tid >> 2)) * N) * 4 + (tid & 3);
-      int hg = 0;
-#pragma unroll 1
-      for (int n = 0; n < rows; n += 4) {
-        uint32_t o[4];
-        if (m_tiles > 0) {
-          tmem_ld4_nowait(tmem + lanes + kOcol + n, o);
-          tmem_wait_ld();
-        }
-        const float4 f = *reinterpret_cast<const float4*>(f_sh + n);
-        const float w[4] = {f.x, f.y, f.z, f.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float v = m_tiles > 0 ? __uint_as_float(o[i]) * w[i] : 0.f;
-          const bool live = tid < p.D && n + i < rows;
-          if (live && slot >= 0) pp[4 * (n + i)] = v;
-          if (live && slot < 0) *reinterpret_cast<T*>(po + hg * p.o_sh) = Dt<T>::narrow(v);
-          if (++hg == p.G) {
-            hg = 0;
-            po += p.o_st;
-          }
-        }
-        __syncwarp();  // the TMEM loads are the whole warp's
+      uint32_t o[N];
+      if (m_tiles > 0) {
+        tmem_load(tmem + lanes + kOcol, o);
+        tmem_wait_ld();
       }
       tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
+      sync_or(false);
+      if (lane == 0) {  // O and the segment's record are read
         mbar_arrive(o_empty);
         mbar_arrive(&seg_empty[ss]);
+      }
+      // thread `tid` has dim `tid` of every row
+      if (tid < p.D && m_tiles > 0) {
+        if (slot >= 0) {
+          float* pp = p.part_o + (((int64_t)slot * (p.D / 4) + (tid >> 2)) * N) * 4 + (tid & 3);
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            if (n < rows) pp[4 * n] = __uint_as_float(o[n]);
+        } else {
+          unsigned char* po = p.out + tid * 2;
+#pragma unroll
+          for (int n = 0; n < N; n += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(f_sh + n);
+            const float w[4] = {f.x, f.y, f.z, f.w};
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              if (n + i < rows)
+                *reinterpret_cast<T*>(po + row_sh[n + i]) = Dt<T>::narrow(__uint_as_float(o[n + i]) * w[i]);
+          }
+        }
+      } else if (tid < p.D) {  // no key: zeros (never a partial)
+#pragma unroll 1
+        for (int n = 0; n < rows; ++n) *reinterpret_cast<T*>(p.out + tid * 2 + row_sh[n]) = Dt<T>::narrow(0.f);
       }
     }
     if (!ok) misc[0] = 1;
