@@ -1,8 +1,9 @@
 // Chunk and cross attention on the CUDA cores, the combine of cut items, and
 // the host side of both entry points.
 //
-// fd_attn_kernel takes what the tensor-core kernel (fd_attn_mma.cu) does not:
-// fp32, and 16-bit heads of more than 128 dims.  With q the tile's rows and j
+// fd_attn_kernel takes what the tensor-core kernels (fd_attn_mma.cu,
+// fd_attn_rows.cu) do not: fp32, and 16-bit heads of fewer than 64 or more
+// than 128 dims.  With q the tile's rows and j
 // its keys, for every key tile
 //   s = scale log2(e) q.K^T,  m' = max(m, max_j s),  p = 2^(s - m'),
 //   l = l 2^(m - m') + sum_j p,  O = O 2^(m - m') + p V
@@ -26,8 +27,8 @@ namespace at {
 constexpr int kRows = 64;   // rows per tile
 constexpr int kThreads = 256;
 constexpr int kFixed = 1;   // an item's fixed cost in key tiles
-constexpr int kMinPer = 2;  // least positions of a CTA
-constexpr int kWhole = 2;   // key tiles up to which no item is cut (whole_items)
+constexpr int kMinPer = 1;  // least positions of a CTA (9 rows x 20 heads over 300 keys: 16.9 us; with 2, 21.9)
+constexpr int kWhole = 2;   // key tiles up to which no item is cut (128 keys: 17.7 us, cut 21.4; 256: 29.3 and 22.1)
 constexpr int kMaxCtas = 320;
 
 constexpr int keys_of(int DP) { return DP <= 64 ? 64 : 32; }           // keys per tile
@@ -357,7 +358,10 @@ int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
 // Host blocks are copied to device memory first, by all SMs: read in place
 // they would cross PCIe once per item that sees them (an SM's loads do not
 // keep them in L2), and a few CTAs, those whose requests have spilled, would
-// wait for it one tile after another.  CTA (j, r) copies block j of request
+// wait for it one tile after another.  (64 requests of up to 8 tokens and 4000
+// keys, a twentieth in host memory: 678 us, in place 1190; 8 of 200 tokens and
+// 2000 keys, a fifth: 365 and 1125; of one token: 286 and 279.  PCIe at ~55
+// GB/s bounds it.)  CTA (j, r) copies block j of request
 // r, when it lies in the host tier, to block r * stage_w + j of the copies.
 constexpr int kStageThreads = 256, kStageBatch = 8;
 __global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __grid_constant__ AttnParams p, int vec) {
