@@ -66,6 +66,7 @@ def _run_tables(prior, new, table, stacks, counts, hbm, host, block, T, W=None, 
     (1, 16, 0, 1, 0, 1.0, 4), (1, 1, 5, 3, 0, 0.5, 9), (3, 16, 40, 20, 2, 0.5, 70), (33, 8, 100, 9, 4, 0.3, 300),
     (256, 16, 500, 2, 16, 0.6, 700), (1023, 16, 64, 5, 3, 0.5, 2048), (1024, 32, 64, 5, 0, 0.01, 6000),
     (1025, 24, 300, 40, 5, 0.5, 50000), (8192, 16, 100, 3, 9, 0.5, 20000), (5, 64, 3000, 9000, 0, 0.7, 50000),
+    (150, 16, 300, 2000, 5, 0.5, 70000), (700, 8, 90, 400, 3, 0.4, 60000), (8, 16, 30, 40000, 0, 0.9, 90000),
 ])
 def test_tables_match_lists(R, block, ctx, new_hi, end_every, share, T, in_place):
     prior, new, table, stacks, counts, hbm, host = _table_case(R, block, ctx, new_hi, end_every, share, R + T)

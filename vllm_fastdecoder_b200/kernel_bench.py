@@ -34,6 +34,18 @@ serves (and larger than the 126 MB L2 where the kernel streams data):
                     decode step of the config-4 trace
   exchange1         fd_exchange_merge_kernel with one rank (push, flags, merge
                     of config 3's partial)
+  extend_tables     fd_tables_kernel: block tables, slots and positions of 601
+                    requests with 0 to 400 new tokens over up to 1000 cached
+  rope_store_kv     fd_rope_kernel: 16384 tokens x 32/8 heads x D128 bf16, three
+                    position axes, q in place, k and v to the HBM tier
+  chunk_few         fd_attn_rows_kernel: 32 requests of 4 new tokens over 4096
+                    keys, 32/8 heads, D128, bf16 (bytes of the cache)
+  chunk_many        fd_attn_mma_kernel: 2 requests of 2048 new tokens over 8192
+                    keys, same heads (achieved TFLOP/s)
+  cross_few         fd_attn_rows_kernel: 24 requests of one token over 1500
+                    encoder states, 20 heads, D64, fp16
+  cross_fp32        fd_attn_kernel: 4 requests of 64 tokens over 1500 encoder
+                    states, 8 heads, D64, fp32 (achieved TFLOP/s)
 
 Each line: the kernel, the mean device time per launch (CUDA events around
 `--launches` back-to-back launches after warm-up), the algorithmic bytes per
@@ -275,6 +287,76 @@ def case_exchange1(dev):
     return (lambda: ex.exchange_and_merge(None, None, final)), nbytes, "fd_exchange_merge_kernel"
 
 
+def case_extend_tables(dev):
+    R, bs, T = 601, 16, 131072
+    g = torch.Generator().manual_seed(2)
+    new = torch.randint(0, 401, (R,), generator=g, dtype=torch.int32)
+    prior = torch.randint(0, 1001, (R,), generator=g, dtype=torch.int32)
+    held, after = -(-prior // bs), -(-(prior + new) // bs)
+    W, need, n_held = 96, int((after - held).sum()), int(held.sum())
+    table = torch.full((R, W), -1, dtype=torch.int32)
+    table[torch.arange(W) < held[:, None]] = torch.arange(n_held, dtype=torch.int32)
+    free = gpu_ops.FreeBlocks(torch.arange(n_held, n_held + need, dtype=torch.int32, device=dev), None,
+                              torch.tensor([need, 0], dtype=torch.int32, device=dev))
+    new, prior, table = new.to(dev), prior.to(dev), table.to(dev)
+    out = gpu_ops.StepTables(R, T, dev)
+    nbytes = 16 * R + 8 * need + 16 * T
+    return lambda: gpu_ops.extend_tables(new, prior, table, free, n_held + need, 0, bs, out), nbytes, "fd_tables_kernel"
+
+
+def case_rope_store_kv(dev):
+    T, H, KVH, D, bs, max_pos = 16384, 32, 8, 128, 16, 16384
+    q, k, v = (torch.randn(T, h, D, device=dev, dtype=torch.bfloat16) for h in (H, KVH, KVH))
+    pos = torch.randint(0, max_pos, (3, T), device=dev)
+    ang = torch.rand(max_pos, D // 2, device=dev)
+    cs = torch.cat((ang.cos(), ang.sin()), 1)
+    kc, vc = (torch.empty(T // bs, KVH, bs, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    slots = torch.randperm(T, device=dev)
+    nbytes = 2 * D * T * (2 * H + 4 * KVH) + T * (3 * D * 4 + 32)
+    return (lambda: gpu_ops.rope_store_kv(q, k, v, pos, cs, slots, (KVTier(kc, vc), None), T // bs, sections=(24, 20, 20)),
+            nbytes, "fd_rope_kernel")
+
+
+def _chunk(dev, R, ql, kl, flops: bool):
+    H, KVH, D, bs = 32, 8, 128, 16
+    W = kl // bs
+    kc, vc = (torch.randn(R * W, KVH, bs, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    table = torch.randperm(R * W, device=dev).to(torch.int32).view(R, W)
+    q = torch.randn(R * ql, H, D, device=dev, dtype=torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty(H, R * ql, device=dev)
+    start = torch.arange(R, device=dev, dtype=torch.int32) * ql
+    qlen, klen = (torch.full((R,), n, device=dev, dtype=torch.int32) for n in (ql, kl))
+    work = 4 * R * H * D * (ql * kl - ql * (ql - 1) // 2) if flops else R * (4 * KVH * D * kl + 4 * ql * H * D)
+    return (lambda: gpu_ops.chunk_attn(q, (KVTier(kc, vc), None), R * W, table, start, qlen, klen, D ** -0.5, out, lse,
+                                       max_q_len=ql, max_k_len=kl),
+            work, "fd_attn_mma_kernel" if flops else "fd_attn_rows_kernel")
+
+
+def case_chunk_few(dev):
+    return _chunk(dev, 32, 4, 4096, False)
+
+
+def case_chunk_many(dev):
+    return _chunk(dev, 2, 2048, 8192, True)
+
+
+def _cross(dev, dtype, R, H, D, ql, kl):
+    q = torch.randn(R * ql, H, D, device=dev, dtype=dtype)
+    k, v = (torch.randn(R * kl, H, D, device=dev, dtype=dtype) for _ in range(2))
+    out, lse = torch.empty_like(q), torch.empty(H, R * ql, device=dev)
+    start, k_start = (torch.arange(R, device=dev, dtype=torch.int32) * n for n in (ql, kl))
+    qlen, klen = (torch.full((R,), n, device=dev, dtype=torch.int32) for n in (ql, kl))
+    return lambda: gpu_ops.cross_attn(q, k, v, start, qlen, k_start, klen, D ** -0.5, out, lse, max_q_len=ql, max_k_len=kl)
+
+
+def case_cross_few(dev):
+    return _cross(dev, torch.float16, 24, 20, 64, 1, 1500), 2 * 24 * 20 * 64 * (2 * 1500 + 2), "fd_attn_rows_kernel"
+
+
+def case_cross_fp32(dev):
+    return _cross(dev, torch.float32, 4, 8, 64, 64, 1500), 4 * 4 * 8 * 64 * 64 * 1500, "fd_attn_kernel"
+
+
 CASES = {
     "store_kv_prefill": lambda dev: case_store_kv(dev, False),
     "store_kv_decode": lambda dev: case_store_kv(dev, True),
@@ -287,6 +369,8 @@ CASES = {
     "prefill_fa": case_prefill_fa,
     "plan": case_plan,
     "exchange1": case_exchange1,
+    "extend_tables": case_extend_tables, "rope_store_kv": case_rope_store_kv, "chunk_few": case_chunk_few,
+    "chunk_many": case_chunk_many, "cross_few": case_cross_few, "cross_fp32": case_cross_fp32,
 }
 
 
@@ -305,7 +389,12 @@ def main() -> None:
         gbs = nbytes / t / 1e9
         line = {"case": name, "kernel": kernel, "us_per_launch": round(t * 1e6, 2),
                 "algorithmic_bytes": int(nbytes), "achieved_gbs": round(gbs, 1)}
-        if name in ("prefill", "prefill_fa"):  # flops, not bytes
+        if name == "cross_fp32":  # flops of the fp32 pipe
+            line = {"case": name, "kernel": kernel, "us_per_launch": round(t * 1e6, 2), "flops": int(nbytes),
+                    "achieved_tflops": round(nbytes / t / 1e12, 1), "launches": args.launches}
+            print(json.dumps(line), flush=True)
+            continue
+        if name in ("prefill", "prefill_fa", "chunk_many"):  # flops, not bytes
             tf = nbytes / t / 1e12
             peak_tf = _bf16_peak()
             line = {"case": name, "kernel": kernel, "us_per_launch": round(t * 1e6, 2), "flops": int(nbytes),
