@@ -99,6 +99,18 @@ def test_tables_of_no_requests_and_no_tokens():
     assert out.read_header()["freed_hbm"] == 1 and out.seq_lens.tolist() == [5, 0] and out.counts.tolist() == [1, 0]
 
 
+def test_tables_whose_rows_overlap_are_refused():
+    with pytest.raises(RuntimeError, match="overlap"):
+        _run_tables_on(i32([[1, 2]]).expand(3, 2))
+    _run_tables_on(i32([[1, 2]]))
+
+
+def _run_tables_on(table):
+    R = table.shape[0]
+    gpu_ops.extend_tables(i32([0] * R), i32([0] * R), table, FreeBlocks(i32([0]), None, i32([1, 0])), 8, 0, 16, max_tokens=4)
+    gpu_ops.check_device_errors(dev())
+
+
 @pytest.mark.parametrize("big", [False, True])
 @pytest.mark.parametrize("why,flag", [("blocks", 1), ("width", 2), ("tokens", 4), ("prior", 8), ("new", 8), ("block", 16),
                                       ("count", 32), ("room", 32)])
@@ -353,6 +365,38 @@ def test_chunk_attention(dtype, H, KVH, D, block, host, lens):
                        bt_row=i32([order.index(r) for r in range(len(ql))]))
     gpu_ops.check_device_errors(dev())
     ref.check_attn(out2, None, refs, start, ql, dtype, D, _rounded(dtype))
+
+
+@pytest.mark.parametrize("dtype,D,block", [(torch.bfloat16, 128, 16), (torch.float16, 128, 8), (torch.float16, 64, 16),
+                                           (torch.bfloat16, 96, 64), (torch.float32, 64, 16)])
+@pytest.mark.parametrize("lens", ["verify", "chunks"])
+@pytest.mark.parametrize("layout", ["heads first", "gap behind blocks", "tokens first"])
+def test_chunk_attention_over_other_layouts(dtype, D, block, lens, layout):
+    ql, kl = LENS[lens]
+    H, KVH = 6, 2
+    g = torch.Generator(device="cuda").manual_seed(D + block)
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, block, dtype, g)
+    _, start, out, lse = _queries(ql, H, D, dtype, g)
+
+    def lay(t):
+        B = t.shape[0]
+        if layout == "heads first":
+            return t.contiguous()
+        if layout == "tokens first":
+            return t.permute(0, 2, 1, 3).contiguous().permute(0, 2, 1, 3)
+        n = KVH * block * D  # the block stride is no multiple of the head stride
+        x = torch.full((B, n + 16), NAN, device="cuda").to(dtype).as_strided((B, KVH, block, D), (n + 16, block * D, D, 1))
+        return x.copy_(t)
+
+    tiers = (KVTier(lay(tiers[0].k), lay(tiers[0].v)), None)
+    q = torch.randn(1, H, D, generator=g, device="cuda").to(dtype).expand(out.shape)  # one query row for all tokens
+    scale = D ** -0.5
+    lim = [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)]
+    refs = _refs(q, start, ql, keys, vals, lim, scale)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), scale, out, lse, max_q_len=max(ql),
+                       max_k_len=max(kl))
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
 
 
 @pytest.mark.parametrize("dtype,H,KVH,D", [

@@ -823,6 +823,8 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
                                                                           and block_table.shape[1] != 1):
         raise RuntimeError("block_table must be int32 [R, W] with contiguous rows")
     R, W = block_table.shape
+    if R > 1 and block_table.stride(0) < W:
+        raise RuntimeError("block_table's rows must not overlap")
     if out is None:
         _check(max_tokens is not None, "give out or max_tokens")
         out = StepTables(R, max_tokens, block_table.device)
