@@ -269,63 +269,116 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_attn_kernel(const __
 }
 
 // The cut items' partials joined: o = sum_i O_i 2^(m_i - m) / sum_i l_i 2^(m_i - m),
-// parts in ascending CTA order.  CTA (c, y) takes rows 32 y .. of the item
-// whose first part CTA c wrote, so a long item's parts are read by many SMs
-// at once; a warp's lanes are 8 rows times 4 groups of 4 dims: the partials
-// lie row by row within a group of dims (whole lines), and the 4 groups are
-// 32 bytes of an output row.  A programmatic dependent of the attention
-// kernel: its CTAs start while that one's last ones run, and await its end.
-constexpr int kCombineRows = 32, kCombineThreads = 256;
+// every sum in a fixed order of the parts.  CTA (c, y, z) takes rows 32 y ..
+// and dims 64 z .. of the item whose first part CTA c wrote, so a long item's
+// parts are read by many SMs at once.  An item of few rows and many keys has
+// dozens of parts, and a thread that walked them one load after another would
+// wait longer than the products took (8 items of 36 rows and 4096 keys of fp32
+// heads x 64: 38.6 us in all, walked 47.8; 5 tokens over 8192 keys x 128: 22.5 and
+// 36): the parts' weights are taken by eight
+// threads per row at once, and 16 loads of O are in flight per thread.  A
+// warp's lanes are 8 rows times 4 groups of 4 dims: the partials lie row by row
+// within a group of dims (whole lines), and the 4 groups are 32 bytes of an
+// output row.  A programmatic dependent of the attention kernel: its CTAs start
+// while that one's last ones run (5 KB of shared memory fit beside two of the
+// row kernel's), and await its end.
+constexpr int kCombineRows = 32, kCombineThreads = 256, kCombineDims = 64;
+constexpr int kCombineLanes = kCombineThreads / kCombineRows;  // threads per row that take weights
+constexpr int kCombineParts = 32;                              // parts per round
 template <typename T>
 __global__ void __launch_bounds__(kCombineThreads) fd_attn_combine_kernel(const __grid_constant__ AttnParams p,
                                                                           int item_rows) {
+  __shared__ float weight[kCombineParts][kCombineRows];
+  __shared__ float red[kCombineLanes][kCombineRows];
   griddep_wait();
   const int c = blockIdx.x;
   const Cut cut = p.cuts[c];
   const int row0 = blockIdx.y * kCombineRows;
   if (row0 >= cut.rows || cut.nparts == 0) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int row = row0 + (warp & 3) * 8 + (lane & 7);
-  if (row >= cut.rows) return;
   // part 0 is slot 1 of CTA c, part i slot 0 of CTA c + i
   auto slot = [&](int i) { return (int64_t)(2 * (c + i) + (i == 0 ? 1 : 0)); };
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  float m = -INFINITY;
+  // warp w takes the weights of parts w, w + 8, ..: lane = row
+  const bool mine = row0 + lane < cut.rows;
+  float m = -INFINITY, l = 0.f;
+  if (mine) {
 #pragma unroll 4
-  for (int i = 0; i < cut.nparts; ++i) m = fmaxf(m, ml[slot(i) * item_rows + row].x);
-  const float base = m == -INFINITY ? 0.f : m;
-  float l = 0.f;
-#pragma unroll 4
-  for (int i = 0; i < cut.nparts; ++i) {
-    const float2 v = ml[slot(i) * item_rows + row];
-    l += v.y * exp2f(v.x - base);
+    for (int i = warp; i < cut.nparts; i += kCombineLanes) m = fmaxf(m, ml[slot(i) * item_rows + row0 + lane].x);
   }
+  red[warp][lane] = m;
+  __syncthreads();
+#pragma unroll
+  for (int x = 0; x < kCombineLanes; ++x) m = fmaxf(m, red[x][lane]);
+  const float base = m == -INFINITY ? 0.f : m;
+  // and adds up the O of 8 rows, two groups of dims per lane
+  const int sub = (warp & 3) * 8 + (lane & 7), row = row0 + sub;
+  const int groups = p.D / 4, d0 = blockIdx.z * (kCombineDims / 4) + (warp >> 2) * 4 + (lane >> 3);
+  const bool ok[2] = {row < cut.rows && d0 < groups, row < cut.rows && d0 + 8 < groups};
+  float4 acc[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+  for (int i0 = 0; i0 < cut.nparts; i0 += kCombineParts) {
+    const int n = min(kCombineParts, cut.nparts - i0);
+    if (i0 > 0) __syncthreads();  // the last round's weights have been read
+    if (mine) {
+#pragma unroll
+      for (int x = 0; x < kCombineParts / kCombineLanes; ++x) {
+        const int i = warp + x * kCombineLanes;
+        if (i >= n) break;
+        const float2 v = ml[slot(i0 + i) * item_rows + row0 + lane];
+        const float w = exp2f(v.x - base);
+        weight[i][lane] = w;
+        l += v.y * w;
+      }
+    }
+    __syncthreads();
+    if (ok[0]) {
+      const float4* po = reinterpret_cast<const float4*>(p.part_o) + row;
+      const int second = ok[1] ? 8 * item_rows : 0;
+#pragma unroll 8
+      for (int i = 0; i < n; ++i) {
+        const float4* at = po + (slot(i0 + i) * groups + d0) * item_rows;
+        const float w = weight[i][sub];
+        const float4 x = at[0], y = at[second];
+        acc[0].x = fmaf(w, x.x, acc[0].x);
+        acc[0].y = fmaf(w, x.y, acc[0].y);
+        acc[0].z = fmaf(w, x.z, acc[0].z);
+        acc[0].w = fmaf(w, x.w, acc[0].w);
+        acc[1].x = fmaf(w, y.x, acc[1].x);
+        acc[1].y = fmaf(w, y.y, acc[1].y);
+        acc[1].z = fmaf(w, y.z, acc[1].z);
+        acc[1].w = fmaf(w, y.w, acc[1].w);
+      }
+    }
+  }
+  __syncthreads();  // m has been read
+  red[warp][lane] = l;
+  __syncthreads();
+  if (warp == 0 && blockIdx.z == 0 && mine && p.lse != nullptr) {
+    l = 0.f;
+    for (int x = 0; x < kCombineLanes; ++x) l += red[x][lane];
+    const int at = row0 + lane;
+    p.lse[(cut.kh * p.G + at % p.G) * p.lse_sh + (int64_t)(cut.row0 + at / p.G) * p.lse_st] =
+        l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+  }
+  if (!ok[0]) return;
+  l = 0.f;
+#pragma unroll
+  for (int x = 0; x < kCombineLanes; ++x) l += red[x][sub];
   const float inv = l > 0.f ? 1.f / l : 0.f;
   const int64_t tok = cut.row0 + row / p.G;
-  const int h = cut.kh * p.G + row % p.G;
-  if (warp < 4 && lane < 8 && p.lse != nullptr)
-    p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
-  T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
-  const int groups = p.D / 4;
-  for (int d = (warp >> 2) * 4 + (lane >> 3); d < groups; d += 8) {
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int i = 0; i < cut.nparts; ++i) {
-      const float w = exp2f(ml[slot(i) * item_rows + row].x - base);
-      const float4 x = reinterpret_cast<const float4*>(p.part_o)[(slot(i) * groups + d) * item_rows + row];
-      acc.x = fmaf(w, x.x, acc.x);
-      acc.y = fmaf(w, x.y, acc.y);
-      acc.z = fmaf(w, x.z, acc.z);
-      acc.w = fmaf(w, x.w, acc.w);
-    }
-    const float f[4] = {acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv};
+  T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + (cut.kh * p.G + row % p.G) * p.o_sh);
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    if (!ok[e]) continue;
+    const float f[4] = {acc[e].x * inv, acc[e].y * inv, acc[e].z * inv, acc[e].w * inv};
     T t[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) t[e] = Dt<T>::narrow(f[e]);
+    for (int u = 0; u < 4; ++u) t[u] = Dt<T>::narrow(f[u]);
+    T* const to = po + 4 * (d0 + 8 * e);
     if (sizeof(T) == 4)
-      *reinterpret_cast<uint4*>(po + 4 * d) = *reinterpret_cast<const uint4*>(t);
+      *reinterpret_cast<uint4*>(to) = *reinterpret_cast<const uint4*>(t);
     else
-      *reinterpret_cast<uint2*>(po + 4 * d) = *reinterpret_cast<const uint2*>(t);
+      *reinterpret_cast<uint2*>(to) = *reinterpret_cast<const uint2*>(t);
   }
 }
 
@@ -340,7 +393,8 @@ bool whole_items(const fd_attn_args* a, int ctas, int item_rows, int keys, int m
 
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + kCombineRows - 1) / kCombineRows));
+  cfg.gridDim = dim3((unsigned)p.ctas, (unsigned)((rows + kCombineRows - 1) / kCombineRows),
+                     (unsigned)((p.D + kCombineDims - 1) / kCombineDims));
   cfg.blockDim = dim3(kCombineThreads);
   cfg.stream = s;
   cudaLaunchAttribute attr[1];
@@ -407,6 +461,7 @@ int stage_blocks(const fd_attn_args* a, int64_t* block_bytes) {
     return 0;
   int64_t w = a->max_k_len > 0 ? ((int64_t)a->max_k_len + a->block_size - 1) / a->block_size : a->bt_width;
   if (w > a->bt_width) w = a->bt_width;
+  if (a->n > 65535) return 0;  // the copies' grid has a row per request
   return w * a->n * 2 * *block_bytes <= kStageBytes ? (int)w : 0;
 }
 
