@@ -27,8 +27,10 @@ namespace at {
 constexpr int kRows = 64;   // rows per tile
 constexpr int kThreads = 256;
 constexpr int kFixed = 1;   // an item's fixed cost in key tiles
-constexpr int kMinPer = 1;  // least positions of a CTA (9 rows x 20 heads over 300 keys: 16.9 us; with 2, 21.9)
-constexpr int kWhole = 2;   // key tiles up to which no item is cut (128 keys: 17.7 us, cut 21.4; 256: 29.3 and 22.1)
+constexpr int kMinPer = 1;  // least positions of a CTA (9 tokens of 32 heads over 300 keys: 15.6 us; with 2, 20.3)
+// Key tiles whose saving does not pay for a cut (whole_items): 9 tokens of 2
+// requests and 8 kv heads, 64 keys 12.0 us, cut 12.8; 128 keys 17.4 and 14.6.
+constexpr int kWhole = 1;
 constexpr int kMaxCtas = 320;
 
 constexpr int keys_of(int DP) { return DP <= 64 ? 64 : 32; }           // keys per tile
@@ -274,12 +276,11 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_attn_kernel(const __
 // parts are read by many SMs at once.  An item of few rows and many keys has
 // dozens of parts, and a thread that walked them one load after another would
 // wait longer than the products took (8 items of 36 rows and 4096 keys of fp32
-// heads x 64: 38.6 us in all, walked 47.8; 5 tokens over 8192 keys x 128: 22.5 and
-// 36): the parts' weights are taken by eight
-// threads per row at once, and 16 loads of O are in flight per thread.  A
-// warp's lanes are 8 rows times 4 groups of 4 dims: the partials lie row by row
-// within a group of dims (whole lines), and the 4 groups are 32 bytes of an
-// output row.  A programmatic dependent of the attention kernel: its CTAs start
+// heads x 64: 38.6 us in all, walked 47.8; 5 tokens over 8192 keys x 128: 22.5
+// and 36): the parts' weights are taken by eight threads per row at once, and
+// 16 loads of O are in flight per thread.  A warp's lanes are 8 rows times 4
+// groups of 4 dims: the partials lie row by row within a group of dims (whole
+// lines), and the 4 groups are 32 bytes of an output row.  A programmatic dependent of the attention kernel: its CTAs start
 // while that one's last ones run (5 KB of shared memory fit beside two of the
 // row kernel's), and await its end.
 constexpr int kCombineRows = 32, kCombineThreads = 256, kCombineDims = 64;
@@ -388,7 +389,7 @@ bool whole_items(const fd_attn_args* a, int ctas, int item_rows, int keys, int m
   const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
   const int64_t items = (q + item_rows / G - 1) / (item_rows / G) * a->n * a->num_kv_heads;
   const int64_t tiles = ((int64_t)a->max_k_len + keys - 1) / keys;
-  return items <= ctas && tiles <= most;
+  return items <= ctas && tiles * (ctas - items) <= (int64_t)most * ctas;
 }
 
 int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {

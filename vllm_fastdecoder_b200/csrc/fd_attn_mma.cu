@@ -64,10 +64,10 @@ constexpr int kSegReaders = 11;     // MMA threads, V producer, eight softmax wa
 constexpr int kItemRows = 2 * kM;
 constexpr int kMaxCtas = 160;
 constexpr int kFixed = 3;           // an item's fixed cost in key tiles of a single
-// Least positions of a CTA, two key tiles behind the fixed cost: 64 tokens of
-// 32 heads over 1500 and 2048 keys 29.9 and 32.2 us; with 2, 38 (2048), with
-// 10, 30.8 and 29.3, and four such requests 36.9 us where 5 takes 30.5.
-constexpr int kMinPer = 5;
+// Least positions of a CTA: 64 tokens of 32 heads over 1500 and 2048 keys 23.4
+// and 24.2 us; with 2, 23.8 and 25.5; with 5, 24.6 and 25.2; with 7, 26.6 and
+// 25.9.
+constexpr int kMinPer = 4;
 typedef Sched<kKT, true, kFixed> Walk;
 
 template <int KD>

@@ -12,10 +12,11 @@ namespace at {
 namespace mm {
 
 constexpr int kKT = 128;            // keys per K/V tile
-// Key tiles up to which no item is cut (whole_items): one request, 5 and 100
-// tokens of 32 heads, 512 keys 13.7 and 22 us, cut 18.4 and 28; 1024 keys as
-// fast cut; 2048 keys 30.5 and 44.7 us, cut 21.3 and 35.
-constexpr int kWhole = 8;
+// Key tiles whose saving does not pay for a cut (whole_items): 5 tokens of one request
+// and 100 of two, 32 heads, 512 keys 13.7 and 22.0 us, cut 16.4 and 25.3; 700
+// keys 18.5 and 25.4, cut 18.6 and 25.7; 1024 keys 19.5 and 29.3, cut 16.3 and
+// 26.5.
+constexpr int kWhole = 5;
 constexpr int kFine = 8;            // keys per TMA box at a request's end, and per box of plain loads
 constexpr int kFines = kKT / kFine;
 constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims of 16 bits

@@ -50,8 +50,9 @@ constexpr int kSegs = 4;            // segments in flight between the roles
 constexpr int kSegReaders = 7;      // MMA thread, two producers, four softmax warps
 constexpr int kMaxCtas = 320;
 constexpr int kFixed = 2;           // an item's fixed cost in key tiles
-// Least positions of a CTA: one request of 5 tokens over 1500 and 3500 keys
-// 19.7 and 26.9 us; with 8, 25.3 and 28.3 (8192 keys: 36.0 and 32.1).
+// Least positions of a CTA: one request of 5 tokens over 1500 and 3500 keys of
+// 8 heads x 128 17.3 and 20.2 us, 8192 keys of 8 x 64 22.5; with 2, 16.2, 20.7
+// and 28.5; with 7, 18.4, 21.0 and 22.1.
 constexpr int kMinPer = 4;
 constexpr int kTmemCols = 128;      // S [0, 32), [32, 64), O [64, 96)
 constexpr int kOcol = 64;
