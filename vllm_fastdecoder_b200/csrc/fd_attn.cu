@@ -462,7 +462,6 @@ int stage_blocks(const fd_attn_args* a, int64_t* block_bytes) {
     return 0;
   int64_t w = a->max_k_len > 0 ? ((int64_t)a->max_k_len + a->block_size - 1) / a->block_size : a->bt_width;
   if (w > a->bt_width) w = a->bt_width;
-  if (a->n > 65535) return 0;  // the copies' grid has a row per request
   return w * a->n * 2 * *block_bytes <= kStageBytes ? (int)w : 0;
 }
 

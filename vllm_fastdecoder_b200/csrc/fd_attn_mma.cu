@@ -635,6 +635,27 @@ int launch(const MmaParams& mp, cudaStream_t s) {
                                "fd_attn_mma_kernel launch");
 }
 
+// {D, heads, tokens, blocks} (strides in bytes), box {64, box_heads, box_tokens, 1}.
+bool encode_rows(CUtensorMap* m, const void* base, int dtype, int D, int heads, int tokens, int64_t blocks,
+                 int64_t head_sb, int64_t tok_sb, int64_t blk_sb, int box_heads, int box_tokens) {
+  const cuuint64_t dims[4] = {(cuuint64_t)D, (cuuint64_t)heads, (cuuint64_t)tokens, (cuuint64_t)blocks};
+  const cuuint64_t strides[3] = {(cuuint64_t)head_sb, (cuuint64_t)tok_sb, (cuuint64_t)blk_sb};
+  const cuuint32_t box[4] = {64, (cuuint32_t)box_heads, (cuuint32_t)box_tokens, 1};
+  return blocks <= 0x7fffffff && encode_map(m, base, dtype, 4, dims, strides, box);
+}
+
+// Heads of 128 dims: {64 dims, 8 tokens, 2 halves of the dims, BS / 8, lines},
+// where a line is the BS tokens of one head of one block (line l at l *
+// head_sb: heads and blocks in one dimension), box {64, 8, 2, box_tokens / 8,
+// 1}: both halves of box_tokens rows in one copy.
+bool encode_lines(CUtensorMap* m, const void* base, int dtype, int BS, int64_t lines, int64_t head_sb, int64_t tok_sb,
+                  int box_tokens) {
+  const cuuint64_t dims[5] = {64, 8, 2, (cuuint64_t)(BS / 8), (cuuint64_t)lines};
+  const cuuint64_t strides[4] = {(cuuint64_t)tok_sb, 128, (cuuint64_t)(8 * tok_sb), (cuuint64_t)head_sb};
+  const cuuint32_t box[5] = {64, 8, 2, (cuuint32_t)(box_tokens / 8), 1};
+  return encode_map(m, base, dtype, 5, dims, strides, box);
+}
+
 void encode_maps(MmaParams& mp, const fd_attn_args* a) {
   const AttnParams& p = mp.a;
   const int D = p.D;
@@ -649,7 +670,7 @@ void encode_maps(MmaParams& mp, const fd_attn_args* a) {
                  p.nblk[t] * (p.blk_sb[t] / p.head_sb[t]) < (1ll << 31);
   mp.group = by_lines ? 2048 : 1024;
   mp.panel = by_lines ? 1024 : kPanel;
-  mp.q_tma = encode_kv_map(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.tq, true, p.G);
+  mp.q_tma = encode_rows(&mp.tmap_q, a->q, a->dtype, D, p.H, p.T, 1, p.q_sh, p.q_st, p.q_st * p.T, p.G, p.tq);
   for (int t = 0; t < 3; ++t) {
     if (p.nblk[t] == 0 || (t < 2 && p.host[t])) continue;
     const bool cross = p.bt == nullptr;
@@ -659,19 +680,19 @@ void encode_maps(MmaParams& mp, const fd_attn_args* a) {
     const int64_t blocks = cross ? 1 : p.nblk[t];
     const int64_t blk_sb = cross ? p.tok_sb[t] * rows : p.blk_sb[t];
     auto map = [&](CUtensorMap* m, const unsigned char* base, int keys) {
-      return encode_kv_map(m, base, a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t], blk_sb, keys, true);
+      return encode_rows(m, base, a->dtype, D, p.KVH, rows, blocks, p.head_sb[t], p.tok_sb[t], blk_sb, 1, keys);
     };
     if (by_lines) {
       mp.lines[t] = (int)(p.blk_sb[t] / p.head_sb[t]);
       auto lines = [&](CUtensorMap* m, const unsigned char* base) {
-        return encode_kv_lines(m, base, a->dtype, p.BS, (p.nblk[t] - 1) * mp.lines[t] + p.KVH, p.head_sb[t], p.tok_sb[t],
-                               1 << mp.box_sh);
+        return encode_lines(m, base, a->dtype, p.BS, (p.nblk[t] - 1) * mp.lines[t] + p.KVH, p.head_sb[t], p.tok_sb[t],
+                            1 << mp.box_sh);
       };
       mp.kv_tma[t] = lines(&mp.tmap_k[t], p.k[t]) && lines(&mp.tmap_v[t], p.v[t]);
     } else {
       mp.kv_tma[t] = map(&mp.tmap_k[t], p.k[t], 1 << mp.box_sh) && map(&mp.tmap_v[t], p.v[t], 1 << mp.box_sh);
     }
-    mp.kv_tma[t] = mp.kv_tma[t] && map(&mp.tmap_vf[t], p.v[t], kFine);
+    if (mp.box_sh > kFineSh) mp.kv_tma[t] = mp.kv_tma[t] && map(&mp.tmap_vf[t], p.v[t], kFine);
   }
 }
 

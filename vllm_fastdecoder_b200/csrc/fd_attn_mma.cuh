@@ -19,6 +19,7 @@ constexpr int kKT = 128;            // keys per K/V tile
 constexpr int kWhole = 5;
 constexpr int kFine = 8;            // keys per TMA box at a request's end, and per box of plain loads
 constexpr int kFines = kKT / kFine;
+constexpr int kFineSh = 5;          // log2 of the box whose cut rows plain loads fetch as fast as boxes of kFine
 constexpr int kPanel = 128 * 128;   // 128 rows x 64 dims of 16 bits
 
 struct MmaParams {
@@ -33,7 +34,7 @@ struct MmaParams {
   // Layout of a K/V tile in shared memory: groups of 8 keys `group` bytes
   // apart, the second 64 dims `panel` bytes behind the first.  One TMA copy
   // takes one 64-dim panel of a box (1024, kPanel), or, of heads of 128 dims,
-  // whole rows (2048, 1024: the maps are encode_kv_lines'; a block
+  // whole rows (2048, 1024: the maps are encode_lines'; a block
   // of tier t having lines[t] lines): an SM's copies come at ~80 cycles apiece
   // whatever their size, and small boxes leave no slack (32 requests of 4
   // tokens over 4096 keys: blocks of 8 keys 104 us, by panels 135; of 16, 92
@@ -178,7 +179,8 @@ __device__ __forceinline__ void prefetch_maps(const MmaParams& mp, int x) {
   const CUtensorMap* map = nullptr;
   if (x >= 0 && x < 9) {
     const int t = x / 3;
-    if (mp.kv_tma[t]) map = x % 3 == 0 ? &mp.tmap_k[t] : x % 3 == 1 ? &mp.tmap_v[t] : &mp.tmap_vf[t];
+    if (mp.kv_tma[t] && (x % 3 < 2 || mp.box_sh > kFineSh))
+      map = x % 3 == 0 ? &mp.tmap_k[t] : x % 3 == 1 ? &mp.tmap_v[t] : &mp.tmap_vf[t];
   } else if (x == 9 && mp.q_tma) {
     map = &mp.tmap_q;
   }
@@ -197,7 +199,7 @@ __device__ __forceinline__ Box box_of(const MmaParams& mp, bool is_v, int left, 
   const int sh = mp.box_sh;
   if (lane < 16) return {lane << sh, (lane << sh) < kKT ? 1 << sh : 0};
   const int cut = left >> sh, at = (cut << sh) + (lane - 16) * kFine;  // the box that is cut, if any
-  return {at, is_v && left < kKT && at + kFine <= left && sh > 5 ? kFine : 0};
+  return {at, is_v && left < kKT && at + kFine <= left && sh > kFineSh ? kFine : 0};
 }
 
 // Block id of this lane's box where boxes lie within blocks, -1 where there

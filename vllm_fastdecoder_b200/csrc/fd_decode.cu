@@ -1014,51 +1014,16 @@ bool encode_tier_map(CUtensorMap* m, const void* base, int dtype, int D, int KVH
 }  // namespace
 
 namespace fdk {
-bool encode_kv_lines(CUtensorMap* m, const void* base, int dtype, int BS, int64_t lines, int64_t head_sb,
-                     int64_t tok_sb, int box_tokens) {
-  struct Key {
-    const void* base;
-    int64_t lines, head_sb, tok_sb;
-    int dtype, BS, box;
-  };
-  constexpr int kSlots = 16;
-  static Key keys[kSlots];
-  static CUtensorMap maps[kSlots];
-  static bool used[kSlots];
-  static int next = 0;
-  static std::mutex mu;
-  Key key;
-  memset(&key, 0, sizeof(key));  // padding bytes take part in the comparison
-  key.base = base;
-  key.lines = lines;
-  key.head_sb = head_sb;
-  key.tok_sb = tok_sb;
-  key.dtype = dtype;
-  key.BS = BS;
-  key.box = box_tokens;
-  std::lock_guard<std::mutex> lock(mu);
-  for (int i = 0; i < kSlots; ++i)
-    if (used[i] && memcmp(&keys[i], &key, sizeof(key)) == 0) {
-      *m = maps[i];
-      return true;
-    }
+bool encode_map(CUtensorMap* m, const void* base, int dtype, int rank, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box) {
   PFN_cuTensorMapEncodeTiled_v12000 enc = tensor_map_encoder();
-  if (enc == nullptr || lines <= 0 || lines > (int64_t)0x7fffffff) return false;
+  if (enc == nullptr) return false;
   const CUtensorMapDataType dt =
       dtype == FD_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  const cuuint64_t dims[5] = {64, 8, 2, (cuuint64_t)(BS / 8), (cuuint64_t)lines};
-  const cuuint64_t strides[4] = {(cuuint64_t)tok_sb, 128, (cuuint64_t)(8 * tok_sb), (cuuint64_t)head_sb};
-  const cuuint32_t box[5] = {64, 8, 2, (cuuint32_t)(box_tokens / 8), 1};
   const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
-  if (enc(m, dt, 5, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return false;
-  keys[next] = key;
-  maps[next] = *m;
-  used[next] = true;
-  next = (next + 1) % kSlots;
-  return true;
+  return enc(m, dt, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, estr,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Cached 4-D tiled tensor map {D, heads, BS, blocks} with box {64 or D,

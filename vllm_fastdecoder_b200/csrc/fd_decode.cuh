@@ -274,13 +274,10 @@ bool encode_kv_map(CUtensorMap* m, const void* base, int dtype, int D, int heads
                    int64_t head_sb, int64_t tok_sb, int64_t blk_sb, int box_tokens, bool swizzle128,
                    int box_heads = 1);
 
-// Cached 5-D tiled tensor map of the heads of 128 16-bit dims of a paged view:
-// {64 dims, 8 tokens, 2 halves of the dims, BS / 8, lines}, where a line is
-// the BS tokens of one head of one block (line l at l * head_sb: heads and
-// blocks in one dimension), box {64, 8, 2, box_tokens / 8, 1}, 128-byte
-// swizzle: both halves of box_tokens rows in one copy.
-bool encode_kv_lines(CUtensorMap* m, const void* base, int dtype, int BS, int64_t lines, int64_t head_sb,
-                     int64_t tok_sb, int box_tokens);
+// Tiled tensor map of a 16-bit view of up to 5 dimensions (strides in bytes,
+// of dimension 1 on), 128-byte swizzle; false when the driver rejects it.
+bool encode_map(CUtensorMap* m, const void* base, int dtype, int rank, const cuuint64_t* dims,
+                const cuuint64_t* strides, const cuuint32_t* box);
 
 // Whether the tcgen05 kernel covers this shape (16-bit KV, head size 128,
 // query group 2, 4 or 8, block size a multiple of 16).
