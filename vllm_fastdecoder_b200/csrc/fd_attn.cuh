@@ -254,12 +254,12 @@ struct Sched {
       }
       if (pass == 0) {
         total = carry;
-        const long long want = quot(total + p.ctas - 1, p.ctas);
-        if (want > kMaxLen) {  // positions of a range are 32 bits
+        if (total > (long long)kMaxLen * p.ctas) {  // positions of a range are 32 bits
           set_error(p.err, FD_DEVERR_LEN);
           return false;
         }
-        per = max((int)want, min_per);
+        per = (int)quot(total + p.ctas - 1, p.ctas);
+        if (per < min_per) per = min_per;
         p0 = (long long)c * per;
         if (p0 >= total) return false;
         len = (int)min((long long)per, total - p0);
