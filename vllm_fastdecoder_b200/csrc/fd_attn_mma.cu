@@ -36,14 +36,15 @@
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 2 x 2048 tokens of 32 heads over up to 12288 keys of 8 heads x 128
-// in 600 us, 985 TFLOP/s.  The tensor pipe is busy for 68% of the time: q.K^T
-// of 64 keys is held up by the shared memory that feeds it (48 cycles per MMA
-// for 32 of arithmetic, ~68 beside the other stream's and the TMA's writes),
-// and a step of both streams takes 1750 cycles where 1270 of MMAs alone would
-// do and the SFU needs 1024.  Tried and slower: q.K^T of 128 keys into both
-// buffers at once (the streams fall into step: 700 us), a quarter of the
-// exponentials by a polynomial on the FMA pipe (623 us); as fast: the row
-// maximum found in the SFU's shadow (605 us), fewer commits (602 us).
+// in 600 us, 985 TFLOP/s (over 8192: 446 us, 1078).  The tensor pipe is busy
+// for 68% of the time: q.K^T of 64 keys is held up by the shared memory that
+// feeds it (48 cycles per MMA for 32 of arithmetic, ~68 beside the other
+// stream's and the TMA's writes), and a step of both streams takes 1750 cycles
+// where 1270 of MMAs alone would do and the SFU needs 1024.  Tried and slower:
+// q.K^T of 128 keys into both buffers at once (the streams fall into step: 700
+// us), a quarter of the exponentials by a polynomial on the FMA pipe (623 us);
+// as fast: the row maximum found in the SFU's shadow (605 us), fewer commits
+// (602 us).
 
 #include <math.h>
 
