@@ -9,7 +9,7 @@
 // are real.  So the products are turned over:
 //   S^T [128 keys x N] = K . Q^T,  P = 2^(scale log2(e) S - m),  l = sum P,
 //   O^T [dims x N] += V^T . P^T,   N = 16 or 32 query rows,
-// a softmax thread has one KEY and N exponentials, K and V are the MMA's A
+// a softmax thread has one KEY and an exponential per row, K and V are the MMA's A
 // operands as they lie in shared memory, and the rows of O^T are dims, so a
 // warp's output stores are whole lines.  The reference m of a column moves
 // only when some score passes it by more than 2^8 (then, and on a segment's
@@ -27,9 +27,9 @@
 // softmax warps agree at their barriers on going on.
 //
 // Measured: 32 requests of 1, 4 and 8 tokens of 32 heads over 4096 keys of 8
-// heads x 128 in 92, 92 and 97 us (5.8 TB/s of cache read; fd_attn_mma 118 to
-// 120); 24 of one token over 1500 keys of 20 heads x 64 in 49 us (fd_attn_mma
-// 76); one request of 16384 keys, 1 and 8 tokens, in 39 and 42 us (47 and 48).
+// heads x 128 in 88, 90 and 95 us (6.0 TB/s of cache read; fd_attn_mma 118 to
+// 120); 24 of one token over 1500 keys of 20 heads x 64 in 48 us (fd_attn_mma
+// 76); one request of 16384 keys, 1 token, in 24 us.
 
 #include <math.h>
 
@@ -111,8 +111,8 @@ __device__ __forceinline__ float warp_max(float v) {
   return r;
 }
 
-// The N sums over the warp's lanes of v[0 .. N - 1]: lane c (of every 32 or,
-// with N = 16, of either half) ends with the sum of column c % N.
+// The N sums over the warp's lanes of v[0 .. N - 1]: lane c ends with the sum
+// of column c % N.
 template <int N>
 __device__ __forceinline__ float column_sum(float (&v)[N], int lane) {
 #pragma unroll
@@ -125,17 +125,32 @@ __device__ __forceinline__ float column_sum(float (&v)[N], int lane) {
     }
   }
   float s = v[0];
-  if (N == 16) s += __shfl_xor_sync(0xffffffffu, s, 16);
+#pragma unroll
+  for (int w = N; w < 32; w <<= 1) s += __shfl_xor_sync(0xffffffffu, s, w);
   return s;
 }
 
 // N consecutive TMEM columns of this warp's lanes.
+__device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[4]) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x4.b32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(t));
+}
 __device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[16]) { tmem_ld16_nowait(t, r); }
 __device__ __forceinline__ void tmem_load(uint32_t t, uint32_t (&r)[32]) { tmem_ld32_nowait(t, r); }
+__device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(t), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
 __device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[16]) { tmem_st16(t, r); }
 __device__ __forceinline__ void tmem_store(uint32_t t, const uint32_t (&r)[32]) { tmem_st32(t, r); }
 
-template <typename T, int KD, int N>
+// N: columns of the MMAs; NC: those that hold rows, the only ones that the
+// softmax works on.  Items of at most 4 rows have NC = 4 (the least N of an MMA
+// is 16): 64 single tokens of 32 heads over up to 2000 keys of 8 x 128 in 68.4
+// us, with all 16 columns 76.5; 24 over 1500 keys of 20 x 64 in 47.6 and 49.3.
+template <typename T, int KD, int N, int NC>
 __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kernel(const __grid_constant__ MmaParams mp) {
   typedef Geo<KD, N> Ge;
   constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingV = Ge::kRingV;
@@ -387,31 +402,31 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       const int m_tiles = seg.m;
       // column n (token tok0 + n / G) sees key j: j <= first + n / G, so n >= (j - first) G
       const int first = p.bt != nullptr ? seg.klen - seg.qlen + seg.tok0 : seg.klen - 1;
-      float l[N];
+      float l[NC];
 #pragma unroll
-      for (int n = 0; n < N; ++n) l[n] = 0.f;
+      for (int n = 0; n < NC; ++n) l[n] = 0.f;
       for (int t = 0; t < m_tiles; ++t) {
         const int h = t & 1;
         ok = wait_or_abort(&s_full[h], (ph >> h) & 1u, misc, p.err);
         ph ^= 1u << h;
         __syncwarp();
         tc_fence_after();
-        uint32_t s[N];
+        uint32_t s[NC];
         tmem_load(tmem + lanes + 32 * h, s);
         tmem_wait_ld();
         const int key0 = (seg.j0 + t) * kKT;
         if (key0 + kKT - 1 > first) {
           const int over = key0 + tid - first;
-          const int from = over <= 0 ? 0 : p.bt != nullptr ? over * p.G : N;
+          const int from = over <= 0 ? 0 : p.bt != nullptr ? over * p.G : NC;
 #pragma unroll
-          for (int n = 0; n < N; ++n)
+          for (int n = 0; n < NC; ++n)
             if (n < from) s[n] = __float_as_uint(-INFINITY);
         }
         // does some score pass its column's reference by more than 2^8?
         bool past = t == 0;
         if (t > 0) {
 #pragma unroll
-          for (int n = 0; n < N; n += 4) {
+          for (int n = 0; n < NC; n += 4) {
             const float4 m = *reinterpret_cast<const float4*>(m_sh + n);
             past |= fmaf(__uint_as_float(s[n]), p.sl2, -m.x) > 8.f;
             past |= fmaf(__uint_as_float(s[n + 1]), p.sl2, -m.y) > 8.f;
@@ -426,16 +441,16 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           ok = ok && (t == 0 || wait_or_abort(pv_done, ((ph >> 3) & 1u) ^ 1u, misc, p.err));
           __syncwarp();
 #pragma unroll
-          for (int n = 0; n < N; ++n) {
+          for (int n = 0; n < NC; ++n) {
             const float mx = warp_max(__uint_as_float(s[n]));
-            if (lane == 0) red[warp * N + n] = mx;
+            if (lane == 0) red[warp * NC + n] = mx;
           }
           if (!sync_and(ok)) {
             ok = false;
             break;
           }
-          if (tid < N) {
-            const float mx = fmaxf(fmaxf(red[tid], red[N + tid]), fmaxf(red[2 * N + tid], red[3 * N + tid])) * p.sl2;
+          if (tid < NC) {
+            const float mx = fmaxf(fmaxf(red[tid], red[NC + tid]), fmaxf(red[2 * NC + tid], red[3 * NC + tid])) * p.sl2;
             const float old = t == 0 ? -INFINITY : m_sh[tid];
             const bool set = old == -INFINITY, grow = !set && mx > old + 8.f;
             f_sh[tid] = grow ? exp2f(old - mx) : 1.f;
@@ -444,11 +459,11 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           sync_or(false);
           if (t > 0) {
             tc_fence_after();
-            uint32_t o[N];
+            uint32_t o[NC];
             tmem_load(tmem + lanes + kOcol, o);
             tmem_wait_ld();
 #pragma unroll
-            for (int n = 0; n < N; ++n) {
+            for (int n = 0; n < NC; ++n) {
               l[n] *= f_sh[n];
               o[n] = __float_as_uint(__uint_as_float(o[n]) * f_sh[n]);
             }
@@ -460,7 +475,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         unsigned char* pb = smem + Ge::kOffP + h * Ge::kP + (tid >> 6) * (N * 128) + (tid & 7) * 2;
         const int ch = (tid & 63) >> 3;
 #pragma unroll
-        for (int n = 0; n < N; n += 4) {
+        for (int n = 0; n < NC; n += 4) {
           const float4 m4 = *reinterpret_cast<const float4*>(m_sh + n);
           const float m[4] = {m4.x, m4.y, m4.z, m4.w};
 #pragma unroll
@@ -483,8 +498,8 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         ph ^= 4u;
         __syncwarp();
       }
-      const float sum = column_sum<N>(l, lane);
-      if (lane < N) red[warp * N + lane] = sum;
+      const float sum = column_sum<NC>(l, lane);
+      if (lane < NC) red[warp * NC + lane] = sum;
       if (!sync_and(ok)) {
         ok = false;
         break;
@@ -492,8 +507,8 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       tc_fence_after();
       const int rows = min(p.tq, seg.qlen - seg.tok0) * p.G;
       const int slot = seg.slot;
-      if (tid < N) {
-        const float lt = red[tid] + red[N + tid] + red[2 * N + tid] + red[3 * N + tid];
+      if (tid < NC) {
+        const float lt = red[tid] + red[NC + tid] + red[2 * NC + tid] + red[3 * NC + tid];
         const float mt = m_tiles > 0 ? m_sh[tid] : -INFINITY;
         f_sh[tid] = slot >= 0 ? 1.f : lt > 0.f ? 1.f / lt : 0.f;
         const int t = tid / p.G, h = seg.kh * p.G + tid - t * p.G;
@@ -501,12 +516,12 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
         row_sh[tid] = tok * p.o_st + h * p.o_sh;
         if (tid < rows) {
           if (slot >= 0)
-            reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * N + tid] = make_float2(mt, lt);
+            reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * NC + tid] = make_float2(mt, lt);
           else if (p.lse != nullptr)
             p.lse[h * p.lse_sh + tok * p.lse_st] = lt > 0.f ? (mt + log2f(lt)) * kLn2 : -INFINITY;
         }
       }
-      uint32_t o[N];
+      uint32_t o[NC];
       if (m_tiles > 0) {
         tmem_load(tmem + lanes + kOcol, o);
         tmem_wait_ld();
@@ -520,14 +535,14 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       // thread `tid` has dim `tid` of every row
       if (tid < p.D && m_tiles > 0) {
         if (slot >= 0) {
-          float* pp = p.part_o + (((int64_t)slot * (p.D / 4) + (tid >> 2)) * N) * 4 + (tid & 3);
+          float* pp = p.part_o + (((int64_t)slot * (p.D / 4) + (tid >> 2)) * NC) * 4 + (tid & 3);
 #pragma unroll
-          for (int n = 0; n < N; ++n)
+          for (int n = 0; n < NC; ++n)
             if (n < rows) pp[4 * n] = __uint_as_float(o[n]);
         } else {
           unsigned char* po = p.out + tid * 2;
 #pragma unroll
-          for (int n = 0; n < N; n += 4) {
+          for (int n = 0; n < NC; n += 4) {
             const float4 f = *reinterpret_cast<const float4*>(f_sh + n);
             const float w[4] = {f.x, f.y, f.z, f.w};
 #pragma unroll
@@ -552,9 +567,9 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols) : "memory");
 }
 
-template <typename T, int KD, int N>
+template <typename T, int KD, int N, int NC>
 int launch(const MmaParams& mp, cudaStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(fd_attn_rows_kernel<T, KD, N>);
+  const void* kern = reinterpret_cast<const void*>(fd_attn_rows_kernel<T, KD, N, NC>);
   static unsigned long long done = 0;
   const int st = fdh::ensure_smem(kern, Geo<KD, N>::kSmem, &done);
   if (st != FD_OK) return st;
@@ -563,9 +578,14 @@ int launch(const MmaParams& mp, cudaStream_t s) {
 }
 
 template <typename T>
-int launch_for(const MmaParams& mp, int N, cudaStream_t s) {
-  if (mp.a.D <= 64) return N == 16 ? launch<T, 64, 16>(mp, s) : launch<T, 64, 32>(mp, s);
-  return N == 16 ? launch<T, 128, 16>(mp, s) : launch<T, 128, 32>(mp, s);
+int launch_for(const MmaParams& mp, int rows, cudaStream_t s) {
+  if (mp.a.D <= 64)
+    return rows == 4    ? launch<T, 64, 16, 4>(mp, s)
+           : rows == 16 ? launch<T, 64, 16, 16>(mp, s)
+                        : launch<T, 64, 32, 32>(mp, s);
+  return rows == 4    ? launch<T, 128, 16, 4>(mp, s)
+         : rows == 16 ? launch<T, 128, 16, 16>(mp, s)
+                      : launch<T, 128, 32, 32>(mp, s);
 }
 
 }  // namespace rw
@@ -574,7 +594,7 @@ int rows_launch(AttnParams& p, const fd_attn_args* a, int rows, cudaStream_t s) 
   int dev = 0, sms = 0;
   int st = fdh::device_sms(&dev, &sms);
   if (st != FD_OK) return st;
-  const int N = rows <= 16 ? 16 : 32;
+  const int N = rows <= 4 ? 4 : rows <= 16 ? 16 : 32;  // rows of an item
   unsigned char* ws = static_cast<unsigned char*>(a->workspace);
   p.ctas = sms * (p.D <= 64 ? 2 : 1);
   if (p.ctas > rw::kMaxCtas) p.ctas = rw::kMaxCtas;
