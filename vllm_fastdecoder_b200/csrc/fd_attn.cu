@@ -33,7 +33,9 @@ constexpr int kMinPer = 1;  // least positions of a CTA (9 tokens of 32 heads ov
 constexpr int kWhole = 1;
 constexpr int kMaxCtas = 320;
 
-constexpr int keys_of(int DP) { return DP <= 64 ? 64 : 32; }           // keys per tile
+// Keys per tile (heads of up to 64 dims, 8 x 256 tokens of 32 heads over 1024
+// keys: 570 us, with 32 keys 604; larger heads have shared memory for 32).
+constexpr int keys_of(int DP) { return DP <= 64 ? 64 : 32; }
 constexpr int ctas_of(int DP) { return DP <= 128 ? 2 : 1; }  // CTAs per SM
 constexpr int smem_bytes(int DP) {
   return ((kRows + 2 * keys_of(DP)) * (DP + 4) + kRows * (keys_of(DP) + 4)) * 4;
