@@ -367,6 +367,22 @@ def test_chunk_attention(dtype, H, KVH, D, block, host, lens):
     ref.check_attn(out2, None, refs, start, ql, dtype, D, _rounded(dtype))
 
 
+@pytest.mark.parametrize("dtype,D,ql,kl", [
+    (torch.float32, 64, 3, 6000), (torch.float32, 256, 1, 6000), (torch.float16, 256, 2, 6000), (torch.bfloat16, 64, 1, 40000),
+    (torch.float16, 128, 20, 30000), (torch.bfloat16, 128, 50, 40000), (torch.float16, 80, 200, 20000),
+])
+def test_one_item_over_most_of_the_gpu(dtype, D, ql, kl):
+    """An item cut into more parts than the combine takes per round."""
+    g = torch.Generator(device="cuda").manual_seed(kl + D)
+    keys, vals, table, tiers, n_hbm = _paged([kl], 1, D, 16, dtype, g)
+    q, start, out, lse = _queries([ql], 1, D, dtype, g)
+    scale = D ** -0.5
+    refs = _refs(q, start, [ql], keys, vals, [kl - ql + torch.arange(ql, device="cuda")], scale)
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32([ql]), i32([kl]), scale, out, lse, max_q_len=ql, max_k_len=kl)
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, [ql], dtype, D, _rounded(dtype))
+
+
 @pytest.mark.parametrize("dtype,D,block", [(torch.bfloat16, 128, 16), (torch.float16, 128, 8), (torch.float16, 64, 16),
                                            (torch.bfloat16, 96, 64), (torch.float32, 64, 16)])
 @pytest.mark.parametrize("lens", ["verify", "chunks"])

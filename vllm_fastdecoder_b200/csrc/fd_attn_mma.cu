@@ -64,7 +64,7 @@ constexpr int kSegs = 4;            // segments in flight between the roles
 constexpr int kSegReaders = 11;     // MMA threads, V producer, eight softmax warps
 constexpr int kItemRows = 2 * kM;
 constexpr int kMaxCtas = 160;
-constexpr int kFixed = 3;           // an item's fixed cost in key tiles of a single
+constexpr int kFixed = 3;           // an item's fixed cost in key tiles of a single (of 2, 5 and 8 none is better throughout)
 // Least positions of a CTA: 64 tokens of 32 heads over 1500 and 2048 keys 23.4
 // and 24.2 us; with 2, 23.8 and 25.5; with 5, 24.6 and 25.2; with 7, 26.6 and
 // 25.9.
