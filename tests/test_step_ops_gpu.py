@@ -217,6 +217,34 @@ def test_rope_writes_rotated_rows(dtype, T, H, KVH, D, rot, sections, turns, pai
     assert torch.equal(q2, q_out) and torch.equal(k2, k_out)
 
 
+@pytest.mark.parametrize("dtype,D,rot", [
+    (torch.float32, 264, 2), (torch.bfloat16, 320, 20), (torch.float16, 264, 6), (torch.bfloat16, 1032, 8),
+    (torch.float16, 2056, 16), (torch.bfloat16, 256, 2), (torch.float32, 1028, 8), (torch.float32, 516, 4),
+])
+def test_rope_of_heads_with_more_vectors_than_threads(dtype, D, rot):
+    """v's rows of more than 256 vectors (of 1, 2, 4 and 8 elements) reach the cache whole."""
+    T, H, KVH, block = 11, 2, 2, 4
+    g = torch.Generator(device="cuda").manual_seed(D)
+    q, k, v = (torch.randn(T, h, D, generator=g, device="cuda").to(dtype) for h in (H, KVH, KVH))
+    cache = torch.full((5, block, KVH, 2 * D), NAN, device="cuda").to(dtype)
+    lg = cache.permute(0, 2, 1, 3)
+    pos = torch.randint(0, 50, (T,), generator=g, device="cuda")
+    cs = _cos_sin(50, rot)
+    slots = torch.randperm(5 * block, generator=g, device="cuda")[:T]
+    slots[3] = -1
+    q_out, k_out = torch.full_like(q, NAN), torch.full_like(k, NAN)
+    gpu_ops.rope_store_kv(q, k, v, pos, cs, slots, (KVTier(lg[..., :D], lg[..., D:]), None), 5, q_out=q_out, k_out=k_out)
+    gpu_ops.check_device_errors(dev())
+    axis = gpu_ops.rope_axes((rot // 2,))
+    _rope_ok(q_out, ref.rope(q, pos[None], cs, axis, False), q, dtype)
+    _rope_ok(k_out, ref.rope(k, pos[None], cs, axis, False), k, dtype)
+    rows, kept = cache.view(-1, KVH, 2 * D), slots >= 0
+    assert torch.equal(rows[slots[kept], :, D:], v[kept]) and torch.equal(rows[slots[kept], :, :D], k_out[kept])
+    rest = torch.ones(rows.shape[0], dtype=torch.bool, device="cuda")
+    rest[slots[kept]] = False
+    assert bool(rows[rest].isnan().all())
+
+
 def test_rope_skips_what_is_out_of_range():
     T, H, KVH, D = 6, 2, 1, 64
     q, k, v = (torch.randn(T, h, D, device="cuda") for h in (H, KVH, KVH))

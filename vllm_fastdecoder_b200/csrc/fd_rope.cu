@@ -127,10 +127,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) fd_rope_kernel(const __g
     }
   }
 
-  // v: its first loads are under way while the angles arrive
-  const int v_lane = p.vch > 0 ? tid % p.vch : 0, v_row = p.vch > 0 ? tid / p.vch : 0;
-  const int v_step = p.vch > 0 ? kThreads / p.vch : 1;
-  const int v_rows = p.vch > 0 && v_row < v_step ? nt * p.KVH : 0;
+  // v: its first loads are under way while the angles arrive.  A row has a
+  // thread per vector, as far as there are threads
+  const int v_lanes = min(p.vch, kThreads);
+  const int v_lane = v_lanes > 0 ? tid % v_lanes : 0, v_row = v_lanes > 0 ? tid / v_lanes : 0;
+  const int v_step = v_lanes > 0 ? kThreads / v_lanes : 1;
+  const int v_rows = v_lanes > 0 && v_row < v_step ? nt * p.KVH : 0;
   for (int f0 = v_row;; f0 += v_step * kBatch) {
     const bool first = f0 == v_row;
     if (f0 >= v_rows && !first) break;
@@ -151,6 +153,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) fd_rope_kernel(const __g
       const int tr = tier_of[t];
       if (live[t] && k_at[t] >= 0)
         *reinterpret_cast<V*>(p.tv[tr] + k_at[t] + h * p.head_sb[tr] + v_lane * VB) = a[u];
+    }
+  }
+  // the vectors of a row behind the first kThreads
+  if (const int tail = p.vch - v_lanes; tail > 0) {
+    for (int x = tid; x < nt * p.KVH * tail; x += kThreads) {
+      const int f = x / tail, t = f / p.KVH, h = f - t * p.KVH, tr = tier_of[t];
+      const int off = (kThreads + x - f * tail) * VB;
+      if (live[t] && k_at[t] >= 0)
+        *reinterpret_cast<V*>(p.tv[tr] + k_at[t] + h * p.head_sb[tr] + off) =
+            *reinterpret_cast<const V*>(p.v + (int64_t)(t0 + t) * p.v_st + h * p.v_sh + off);
     }
   }
 
