@@ -600,6 +600,48 @@ def test_two_streams_and_two_graphs_at_once(dtype, many):
         assert torch.equal(torch.nan_to_num(out.float()), torch.nan_to_num(alone.float()))
 
 
+def _repeat_beside_copies(call, out, times):
+    """Call again and again while another stream copies, so that loads land late
+    and out of order; every result has to be the first one, bit for bit."""
+    out.fill_(NAN)
+    call()
+    gpu_ops.check_device_errors(dev())
+    first, differ = out.clone(), torch.zeros((), dtype=torch.int64, device="cuda")
+    side, big = torch.cuda.Stream(), torch.empty(1 << 27, dtype=torch.uint8, device="cuda")
+    bits = torch.int16 if out.element_size() == 2 else torch.int32
+    for i in range(times):
+        if i % 8 == 0:
+            with torch.cuda.stream(side):
+                big[: 1 << 26].copy_(big[1 << 26:])
+        out.fill_(NAN)
+        call()
+        differ += (out.view(bits) != first.view(bits)).sum()
+    torch.cuda.synchronize()
+    gpu_ops.check_device_errors(dev())
+    assert int(differ) == 0
+
+
+@pytest.mark.parametrize("dtype,D,block", [(torch.bfloat16, 128, 16), (torch.float16, 64, 16), (torch.bfloat16, 96, 64)])
+def test_single_tiles_over_many_key_tiles(dtype, D, block):
+    """Requests of one query tile, whose key tiles both streams of the tensor-core
+    kernel share: over more tiles than the rings hold, the last one half or
+    barely seen."""
+    H, KVH = 8, 2
+    ql = [9, 32, 20, 31, 12, 32, 10]
+    kl = [9000, 4097, 129, 2048, 2049, 6464, 65]
+    g = torch.Generator(device="cuda").manual_seed(D)
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, block, dtype, g)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    scale = D ** -0.5
+    refs = _refs(q, start, ql, keys, vals, [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)], scale)
+    args = (q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), scale, out, lse)
+    call = lambda: gpu_ops.chunk_attn(*args, max_q_len=max(ql), max_k_len=max(kl))  # noqa: E731
+    call()
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, True)
+    _repeat_beside_copies(call, out, 400)
+
+
 # ------------------------------------------------------------------ together
 
 

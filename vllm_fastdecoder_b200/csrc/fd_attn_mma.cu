@@ -8,8 +8,12 @@
 // runs two STREAMS of such products.  In a pair (256 rows and more) the
 // streams are two neighbouring query tiles and share every K/V tile; in a
 // single tile (few query rows: bound by the bytes of the cache) stream A
-// takes the even key tiles and stream B the odd ones of the same query tile,
-// and the two are joined in registers at the end.
+// takes the first 64 keys of every key tile and stream B the second 64, for
+// the same query tile, and the two are joined in registers at the end.  Either
+// way both streams wait for every tile and release it: a stream that waited
+// only for every other one would, in a ring of 3 or 5 slots, see every other
+// phase of a slot's barrier, and the parity of the phase before the last
+// would let it pass before the tile between has landed.
 //
 // What would bound a stream that takes one step after the other is its chain
 // (scores, softmax, P.V, scores ...), with the tensor cores and the SFU each
@@ -217,7 +221,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   uint64_t* q_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);
   uint64_t* q_empty = q_full + 1;         // both streams' MMA commits after a segment's last q.K^T
   uint64_t* k_full = q_empty + 1;         // [kRingK]
-  uint64_t* k_empty = k_full + kRingK;    // [kRingK] two arrivals: the streams are done with the tile
+  uint64_t* k_empty = k_full + kRingK;    // [kRingK] two arrivals: both streams are done with the tile
   uint64_t* v_full = k_empty + kRingK;    // [kRingV]
   uint64_t* v_empty = v_full + kRingV;    // [kRingV] two arrivals
   uint64_t* s_full = v_empty + kRingV;    // [2][2] MMA commit: S of the stream's step is in its buffer
@@ -294,9 +298,9 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
             i.n0 = steps(Walk::visible(p, rq, tok0 + p.tq), g.j0, g.j1);
             i.n1 = steps(last, g.j0, g.j1);
           } else {
-            const int cut = 2 * i.m - steps(last, g.j0, g.j1);  // 1: the last tile's second half is not seen
-            i.n0 = ((i.m + 1) & ~1) - (i.m & 1 ? cut : 0);
-            i.n1 = (i.m & ~1) - (i.m & 1 ? 0 : cut);
+            const int halves = steps(last, g.j0, g.j1);  // the last tile's second half may not be seen
+            i.n0 = (halves + 1) >> 1;
+            i.n1 = halves >> 1;
           }
           i.tok0 = tok0;
           i.qst = rq.qst;
@@ -407,9 +411,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       uint64_t* const my_p = p_full + 2 * x;
       uint32_t nq = 0;  // segments with keys
       uint32_t pp = 0;  // phase parities of p_full's two buffers
-      // ring slots (and phases) of the segment's first tile
-      int k0 = 0, v0 = 0;
-      uint32_t kp0 = 0, vp0 = 0;
+      int ks_ = 0, vs_ = 0;  // ring slots (and phases) of the next K and V tile
+      uint32_t kp = 0, vp = 0;
       bool ok = true;
       for (int nseg = 0; ok; ++nseg) {
         const int ss = nseg % kSegs;
@@ -419,34 +422,24 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         const int n = x ? segs[ss].n1 : segs[ss].n0;
         mbar_arrive(&seg_empty[ss]);
         if (!live) break;
-        // this stream's next K and V tile: every tile of a pair, every other one of a single
-        const int stride = pair ? 1 : 2;
-        int ks_ = k0, vs_ = v0;
-        uint32_t kp = kp0, vp = vp0;
-        if (!pair && x) {
-          advance<kRingK>(ks_, kp, 1);
-          advance<kRingV>(vs_, vp, 1);
-        }
-        // a single's tile has one user, which arrives for both
-        auto release = [&](uint64_t* empty) {
-          umma_commit(empty);
-          if (!pair) mbar_arrive(empty);
-        };
+        // of a pair step i takes half i & 1 of tile i / 2, of a single half x of tile i
+        auto first_of_tile = [&](int i) { return !pair || (i & 1) == 0; };
+        auto last_of_tile = [&](int i) { return !pair || (i & 1) || i == n - 1; };
         const uint32_t q_lo = base + (uint32_t)((pair ? x : 0) * (kTile >> 4)) + (1u << 16);
         auto qk = [&](int i) {  // q.K^T of step i into its S buffer
           const int h = i & 1;
-          if (h == 0 && !poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
+          if (first_of_tile(i) && !poll_or_abort(&k_full[ks_], kp, misc, p.err)) return false;
           tc_fence_after();
-          const uint32_t k_lo = base + (uint32_t)((Ge::kOffK + ks_ * kTile) >> 4) + (uint32_t)h * half + (1u << 16);
+          const uint32_t k_lo = base + (uint32_t)((Ge::kOffK + ks_ * kTile) >> 4) + (uint32_t)(pair ? h : x) * half + (1u << 16);
 #pragma unroll
           for (int ks = 0; ks < KD / 16; ++ks)
             umma_f16_lo(t_s + h * kHalf, q_lo + (uint32_t)(((ks >> 2) * kPanel + (ks & 3) * 32) >> 4), q_hi,
                         k_lo + (uint32_t)(ks >> 2) * panel + (uint32_t)((ks & 3) * 32 >> 4), kv_hi, kIdQK,
                         ks > 0 ? 1u : 0u);
           umma_commit(&my_s[h]);
-          if (h || i == n - 1) {
-            release(&k_empty[ks_]);
-            advance<kRingK>(ks_, kp, stride);
+          if (last_of_tile(i)) {
+            umma_commit(&k_empty[ks_]);
+            advance<kRingK>(ks_, kp);
             if (i == n - 1) umma_commit(q_empty);
           }
           return true;
@@ -461,21 +454,22 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
         for (int i = 0; ok && i < n; ++i) {
           const int h = i & 1;
-          if (h == 0) ok = poll_or_abort(&v_full[vs_], vp, misc, p.err);
+          if (first_of_tile(i)) ok = poll_or_abort(&v_full[vs_], vp, misc, p.err);
           ok = ok && poll_or_abort(&my_p[h], (pp >> h) & 1u, misc, p.err);
           if (!ok) break;
           pp ^= 1u << h;
           tc_fence_after();
-          const uint32_t v_lo = base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (uint32_t)h * half + (panel << 16);
+          const uint32_t v_lo =
+              base + (uint32_t)((Ge::kOffV + vs_ * kTile) >> 4) + (uint32_t)(pair ? h : x) * half + (panel << 16);
 #pragma unroll
           for (int ks = 0; ks < kHalf / 16; ++ks)
             umma_f16_ts_lo(t_o, t_s + h * kHalf + 8 * ks, v_lo + (uint32_t)ks * (half / 4), kv_hi, kIdPV,
                            (i > 0 || ks > 0) ? 1u : 0u);
           umma_commit(&pv_done[x]);
           if (i + 2 < n) ok = qk(i + 2);
-          if (h || i == n - 1) {
-            release(&v_empty[vs_]);
-            advance<kRingV>(vs_, vp, stride);
+          if (last_of_tile(i)) {
+            umma_commit(&v_empty[vs_]);
+            advance<kRingV>(vs_, vp);
           }
         }
         if (!ok) break;
@@ -485,17 +479,15 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           } else {
             umma_commit(pair ? &o_full[x] : o_both);
           }
-          // a pair's tiles that only the other stream sees
-          for (int t = (n + 1) >> 1; ok && pair && t < m; ++t) {
+          // tiles that only the other stream sees
+          for (int t = pair ? (n + 1) >> 1 : n; ok && t < m; ++t) {
             ok = poll_or_abort(&k_full[ks_], kp, misc, p.err);
             if (ok) mbar_arrive(&k_empty[ks_]);
             ok = ok && poll_or_abort(&v_full[vs_], vp, misc, p.err);
             if (ok) mbar_arrive(&v_empty[vs_]);
-            advance<kRingK>(ks_, kp, 1);
-            advance<kRingV>(vs_, vp, 1);
+            advance<kRingK>(ks_, kp);
+            advance<kRingV>(vs_, vp);
           }
-          advance<kRingK>(k0, kp0, m);
-          advance<kRingV>(v0, vp0, m);
         }
       }
       if (!ok) misc[0] = 1;
@@ -518,7 +510,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
       const SegInfo& seg = segs[ss];  // stays until this segment's end
       if (!seg.live) break;
       const int n = x ? seg.n1 : seg.n0;
-      const int jstep = seg.pair ? kKT : 2 * kKT, jfirst = (seg.j0 + (seg.pair ? 0 : x)) * kKT;
+      // step i's first key: of a pair half i & 1 of tile i / 2, of a single half x of tile i
+      const int per = seg.pair ? 1 : 0, jfirst = seg.j0 * kKT + (seg.pair ? 0 : x * kHalf);
       bool any_row;
       int lim, lim_all;  // last key that this row sees, that all rows of the tile see
       {
@@ -537,7 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         ph ^= 1u << h;
         tc_fence_after();
         if (any_row) {
-          const int key0 = jfirst + (i >> 1) * jstep + h * kHalf;
+          const int key0 = jfirst + (i >> per) * kKT + (i & per) * kHalf;
           uint32_t ra[32], rb[32];
           tmem_ld32_nowait(t_s + h * kHalf, ra);
           tmem_ld32_nowait(t_s + h * kHalf + 32, rb);

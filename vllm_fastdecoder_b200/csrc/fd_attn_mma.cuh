@@ -117,16 +117,11 @@ __device__ __forceinline__ void init_barriers(uint64_t* bars, int num, F count) 
   }
 }
 
-// A ring position moved on by `by` slots.
+// The next slot of a ring, and its phase's parity.
 template <int R>
-__device__ __forceinline__ void advance(int& slot, uint32_t& phase, int by) {
-  if (by > R) {
-    phase ^= (uint32_t)(by / R) & 1u;
-    by %= R;
-  }
-  slot += by;
-  if (slot >= R) {
-    slot -= R;
+__device__ __forceinline__ void advance(int& slot, uint32_t& phase) {
+  if (++slot == R) {
+    slot = 0;
     phase ^= 1u;
   }
 }

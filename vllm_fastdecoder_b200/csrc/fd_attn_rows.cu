@@ -27,9 +27,9 @@
 // softmax warps agree at their barriers on going on.
 //
 // Measured: 32 requests of 1, 4 and 8 tokens of 32 heads over 4096 keys of 8
-// heads x 128 in 88, 90 and 92 us (6.0 TB/s of cache read; fd_attn_mma 114 to
-// 115); 24 of one token over 1500 keys of 20 heads x 64 in 48 us (fd_attn_mma
-// 76); one request of 16384 keys, 1 and 8 tokens, in 25 and 28 us (33 and 34).
+// heads x 128 in 88, 90 and 92 us (6.0 TB/s of cache read; fd_attn_mma 98 to
+// 101); 24 of one token over 1500 keys of 20 heads x 64 in 48 us (fd_attn_mma
+// 72); one request of 16384 keys, 1 and 8 tokens, in 25 and 28 us (33 and 34).
 
 #include <math.h>
 
@@ -351,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
                         q_lo + (uint32_t)(((ks >> 2) * (N * 128) + (ks & 3) * 32) >> 4), q_hi, kIdQK, ks > 0 ? 1u : 0u);
           umma_commit(&s_full[t & 1]);
           umma_commit(&k_empty[ks_]);
-          advance<kRingK>(ks_, kp, 1);
+          advance<kRingK>(ks_, kp);
           if (t == m - 1) umma_commit(&q_empty[qb]);
           return true;
         };
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           umma_commit(pv_done);
           if (t + 2 < m) ok = qk(t + 2);
           umma_commit(&v_empty[vs_]);
-          advance<kRingV>(vs_, vp, 1);
+          advance<kRingV>(vs_, vp);
         }
         if (ok && m > 0) umma_commit(o_full);
       }
