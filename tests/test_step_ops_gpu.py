@@ -642,6 +642,32 @@ def test_single_tiles_over_many_key_tiles(dtype, D, block):
     _repeat_beside_copies(call, out, 400)
 
 
+def _keyless_batch(dtype, KVH, G, D, nq, n, seed):
+    """cross_attn of n requests of up to nq tokens, most of which have no states."""
+    rnd = random.Random(seed)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    ql = [rnd.randint(max(1, nq // 2), nq) for _ in range(n)]
+    kl = [rnd.choice([0, 0, 0, rnd.randint(1, 700)]) for _ in range(n)]
+    S = sum(kl)
+    k, v = (torch.randn(S, KVH, D, generator=g, device="cuda").to(dtype) for _ in range(2))
+    k_start = [sum(kl[:i]) for i in range(n)]
+    q, start, out, lse = _queries(ql, KVH * G, D, dtype, g, gap=0)
+    refs = _refs(q, start, ql, [k[s:s + x] for s, x in zip(k_start, kl)], [v[s:s + x] for s, x in zip(k_start, kl)],
+                 [torch.full((m,), x - 1, device="cuda") for m, x in zip(ql, kl)], 0.1)
+    return ql, start, out, lse, refs, (q, k, v, i32(start), i32(ql), i32(k_start), i32(kl), 0.1, out, lse)
+
+
+@pytest.mark.parametrize("dtype,KVH,G,D,nq", [(torch.bfloat16, 2, 4, 128, 1), (torch.float16, 5, 1, 64, 1),
+                                              (torch.bfloat16, 2, 4, 128, 4), (torch.float16, 3, 2, 64, 14)])
+def test_requests_without_keys_among_others_few_rows(dtype, KVH, G, D, nq):
+    ql, start, out, lse, refs, args = _keyless_batch(dtype, KVH, G, D, nq, 300, nq + D)
+    call = lambda: gpu_ops.cross_attn(*args, max_q_len=nq)  # noqa: E731
+    call()
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, True)
+    _repeat_beside_copies(call, out, 2000)
+
+
 # ------------------------------------------------------------------ together
 
 

@@ -169,7 +169,10 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
   uint64_t* p_full = s_full + 2;           // [2] the four softmax warps wrote P
   uint64_t* pv_done = p_full + 2;          // MMA commit after each P.V
   uint64_t* o_full = pv_done + 1;          // MMA commit after a segment's last P.V
-  uint64_t* o_empty = o_full + 1;          // the four softmax warps are done with the segment
+  // the four softmax warps are done with a segment that has keys.  One without
+  // is left out: its softmax awaits nothing of the MMA thread's, which could
+  // then find this barrier a phase past the one that it waits for
+  uint64_t* o_empty = o_full + 1;
   uint64_t* seg_full = o_empty + 1;        // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs;  // [kSegs]
   uint64_t* drain = seg_empty + kSegs;
@@ -329,7 +332,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       const uint32_t two = (uint32_t)mp.group * 2 >> 4, panel = (uint32_t)mp.panel >> 4;
       const uint32_t lbo = KD == 128 ? panel : 0u;
       const uint32_t q_hi = desc_hi(1024), kv_hi = desc_hi((uint32_t)mp.group);
-      int ks_ = 0, vs_ = 0, nq = 0;
+      int ks_ = 0, vs_ = 0, nq = 0;  // nq: segments with keys
       uint32_t kp = 0, vp = 0, pp = 0;  // ring phases; parities of p_full's two buffers
       bool ok = true;
       for (int nseg = 0; ok; ++nseg) {
@@ -360,8 +363,8 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           ++nq;
           ok = ok && qk(0) && (m < 2 || qk(1));
         }
-        // the last segment's O has been read
-        if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
+        // the O of the segment with keys before has been read
+        if (ok && m > 0 && nq > 1) ok = poll_or_abort(o_empty, (uint32_t)(nq - 2) & 1u, misc, p.err);
         for (int t = 0; ok && t < m; ++t) {
           const int h = t & 1;
           ok = poll_or_abort(&v_full[vs_], vp, misc, p.err) && poll_or_abort(&p_full[h], (pp >> h) & 1u, misc, p.err);
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       tc_fence_before();
       sync_or(false);
       if (lane == 0) {  // O and the segment's record are read
-        mbar_arrive(o_empty);
+        if (m_tiles > 0) mbar_arrive(o_empty);
         mbar_arrive(&seg_empty[ss]);
       }
       // thread `tid` has dim `tid` of every row
