@@ -668,6 +668,36 @@ def test_requests_without_keys_among_others_few_rows(dtype, KVH, G, D, nq):
     _repeat_beside_copies(call, out, 2000)
 
 
+@pytest.mark.parametrize("dtype,KVH,G,D,nq", [(torch.bfloat16, 2, 4, 128, 30), (torch.float16, 3, 1, 64, 90),
+                                              (torch.bfloat16, 1, 4, 96, 150)])
+def test_requests_without_keys_among_others_many_rows(dtype, KVH, G, D, nq):
+    ql, start, out, lse, refs, args = _keyless_batch(dtype, KVH, G, D, nq, 300, nq + D)
+    call = lambda: gpu_ops.cross_attn(*args, max_q_len=nq)  # noqa: E731
+    call()
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, True)
+    _repeat_beside_copies(call, out, 1000)
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_pairs_of_tiles_of_which_the_first_sees_nothing(dtype, D):
+    """Chunks with more queries than keys: whole pairs of query tiles without keys,
+    and pairs whose first tile (32 tokens of 4 heads) has none."""
+    H, KVH = 4, 1
+    ql = [64, 200, 64, 33, 128, 64, 300, 64] * 12
+    kl = [32, 30, 1, 1, 90, 10, 20, 0] * 12
+    g = torch.Generator(device="cuda").manual_seed(D)
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    refs = _refs(q, start, ql, keys, vals, [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)], 0.1)
+    args = (q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), 0.1, out, lse)
+    call = lambda: gpu_ops.chunk_attn(*args, max_q_len=300)  # noqa: E731
+    call()
+    gpu_ops.check_device_errors(dev())
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, True)
+    _repeat_beside_copies(call, out, 1000)
+
+
 # ------------------------------------------------------------------ together
 
 

@@ -110,10 +110,11 @@ static_assert(sizeof(SegInfo) == 64, "segment record");
 // The end of a segment for one softmax warp of stream x: o and lse of its
 // rows, or their partials.  A pair's stream has its own tile and all dims; in
 // a single the two warpgroups take half of the dims each of the joined
-// streams.  Not inlined: what it needs stays out of the main loop's registers.
+// streams.  nkey: segments with keys before this one.  Not inlined: what it
+// needs stays out of the main loop's registers.
 template <typename T, int KD>
 __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg, int x, uint32_t t_s, float m, float l,
-                                         bool any_row, int nseg, uint32_t* phases, float2* ml, uint64_t* o_empty,
+                                         bool any_row, int nkey, uint32_t* phases, float2* ml, uint64_t* o_empty,
                                          volatile int* misc) {
   uint64_t* o_full = o_empty - 3;  // [2], then o_both, o_empty, ml_full
   uint64_t* o_both = o_empty - 1;
@@ -129,8 +130,9 @@ __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg
   const int qi = seg.tok0 + (pair ? x * p.tq : 0) + tg;
   const bool row_ok = tg < p.tq && qi < seg.qlen;
   float wa = 1.f, wb = 0.f;  // weights of stream A's and B's O
-  // everyone has read the m and l of the segment before
-  if (nseg > 0 && !__all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err)))
+  // everyone has read the m and l of the segment with keys before
+  if (m_tiles > 0 && nkey > 0 &&
+      !__all_sync(0xffffffffu, wait_or_abort(o_empty, (uint32_t)(nkey - 1) & 1u, misc, p.err)))
     return false;
   if (single && m_tiles > 0) {
     ml[x * kM + row] = make_float2(m, l);
@@ -148,7 +150,7 @@ __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg
     wb = x ? wo : wt;
     l = l * wo + other.y * wt;
     m = mm;
-  } else if (n > 0) {
+  } else if (m_tiles > 0) {
     if (!__all_sync(0xffffffffu, wait_or_abort(&o_full[x], (ph >> 2) & 1u, misc, p.err))) return false;
     ph ^= 4u;
   }
@@ -227,9 +229,13 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
   uint64_t* s_full = v_empty + kRingV;    // [2][2] MMA commit: S of the stream's step is in its buffer
   uint64_t* p_full = s_full + 4;          // [2][2] the stream's four softmax warps wrote P there
   uint64_t* pv_done = p_full + 4;         // [2] MMA commit after each P.V of the stream
-  uint64_t* o_full = pv_done + 2;         // [2] pairs: MMA commit after the stream's last P.V
-  uint64_t* o_both = o_full + 2;          // singles: both streams' last P.V
-  uint64_t* o_empty = o_both + 1;         // all eight softmax warps are done with the segment
+  uint64_t* o_full = pv_done + 2;         // [2] pairs: MMA commit after the stream's last P.V, if it has any
+  uint64_t* o_both = o_full + 2;          // singles: both streams' last P.V, likewise
+  // all eight softmax warps are done with a segment that has keys.  In such a
+  // segment they await both MMA threads (o_full or o_both, also of a stream
+  // without steps), so those never find this barrier a phase past the one
+  // that they wait for; a segment without keys is left out
+  uint64_t* o_empty = o_both + 1;
   uint64_t* ml_full = o_empty + 1;        // singles: both streams' m and l are in shared memory
   uint64_t* seg_full = ml_full + 1;       // [kSegs]
   uint64_t* seg_empty = seg_full + kSegs; // [kSegs]
@@ -450,8 +456,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
           if (ok && n == 0) mbar_arrive(q_empty);
         }
         if (ok && n > 0) ok = qk(0) && (n < 2 || qk(1));
-        // the last segment's O has been read
-        if (ok && nseg > 0) ok = poll_or_abort(o_empty, (uint32_t)(nseg - 1) & 1u, misc, p.err);
+        // the O of the segment with keys before has been read
+        if (ok && m > 0 && nq > 1) ok = poll_or_abort(o_empty, (nq - 2) & 1u, misc, p.err);
         for (int i = 0; ok && i < n; ++i) {
           const int h = i & 1;
           if (first_of_tile(i)) ok = poll_or_abort(&v_full[vs_], vp, misc, p.err);
@@ -474,11 +480,11 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         }
         if (!ok) break;
         if (m > 0) {
-          if (n == 0) {
-            if (!pair) mbar_arrive(o_both);
-          } else {
-            umma_commit(pair ? &o_full[x] : o_both);
-          }
+          uint64_t* const done = pair ? &o_full[x] : o_both;
+          if (n == 0)
+            mbar_arrive(done);
+          else
+            umma_commit(done);
           // tiles that only the other stream sees
           for (int t = pair ? (n + 1) >> 1 : n; ok && t < m; ++t) {
             ok = poll_or_abort(&k_full[ks_], kp, misc, p.err);
@@ -502,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
     // phase parities of s_full (bits 0, 1), o_full (2), o_both / ml_full (3),
     // pv_done of the step at hand (4)
     uint32_t ph = 0;
+    int nkey = 0;  // segments with keys
     bool ok = true;
     for (int nseg = 0; ok; ++nseg) {
       const int ss = nseg % kSegs;
@@ -599,12 +606,14 @@ __global__ void __launch_bounds__(kThreads, 1) fd_attn_mma_kernel(const __grid_c
         ph ^= 16u;
       }
       if (!ok) break;
-      ok = __all_sync(0xffffffffu, finish_rows<T, KD>(p, seg, x, t_s, m, l, any_row, nseg, &ph, ml, o_empty, misc));
+      ok = __all_sync(0xffffffffu, finish_rows<T, KD>(p, seg, x, t_s, m, l, any_row, nkey, &ph, ml, o_empty, misc));
       if (!ok) break;
       tc_fence_before();
+      const bool keyed = seg.m > 0;
+      nkey += keyed ? 1 : 0;
       __syncwarp();
       if (lane == 0) {
-        mbar_arrive(o_empty);
+        if (keyed) mbar_arrive(o_empty);
         mbar_arrive(&seg_empty[ss]);
       }
     }
