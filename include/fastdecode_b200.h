@@ -701,7 +701,7 @@ typedef struct fd_attn_args {
   int32_t max_q_len;         /* the host's bounds on q_len and k_len, 0: unknown.  They choose
                                 between kernels; a wrong one costs time, not the result */
   int32_t max_k_len;
-  int32_t _pad0;
+  int32_t bt_rows;           /* chunk: rows of block_table, 0: not known (bt_row is then the caller's to keep) */
   void *workspace;           /* fd_attn_workspace_size() bytes, 16-byte aligned; calls that run at
                                 the same time need one each */
   size_t workspace_bytes;
@@ -725,8 +725,8 @@ FD_API size_t fd_attn_workspace_size(const fd_attn_args *a);
  * be finite.  The reference refuses such requests when part of their context
  * is in the host tier (fastdecode/plan.py:142-149) and hands the others to
  * FlashAttention (fastdecode/backend.py:317-340).  Block ids and lengths are
- * range-checked on the device: a request whose lengths do not fit its rows
- * writes nothing (FD_DEVERR_LEN); a block id outside both tiers is not read
+ * range-checked on the device: a request whose lengths do not fit its rows, or
+ * whose table row is not one of bt_rows, writes nothing (FD_DEVERR_LEN); a block id outside both tiers is not read
  * (FD_DEVERR_BLOCK_ID; the rows of a request that lists it are undefined). */
 FD_API int fd_chunk_attn(const fd_attn_args *a, void *stream);
 

@@ -181,6 +181,13 @@ def test_attention_rejects_what_only_one_form_needs():
         assert lib.fd_cross_attn(None, None) == 1
 
 
+def test_chunk_attention_rejects_a_negative_number_of_table_rows():
+    a = _attn()
+    a.bt_rows = -1
+    assert nat.load().fd_chunk_attn(ctypes.byref(a), None) == 1
+    assert b"bt_rows" in nat.load().fd_last_error_message()
+
+
 def test_workspace_grows_with_the_head_and_is_zero_for_no_head():
     lib = nat.load()
     a = _attn()

@@ -543,6 +543,29 @@ def test_requests_that_do_not_fit_write_nothing(dtype):
     assert bool(o2[start[1]:].isnan().all()) and not bool(o2[start[0]:start[0] + 2].isnan().any())
 
 
+@pytest.mark.parametrize("dtype,H,q_extra", [(torch.bfloat16, 4, 0), (torch.float16, 8, 60), (torch.float32, 4, 0)])
+def test_requests_whose_table_row_does_not_exist_write_nothing(dtype, H, q_extra):
+    KVH, D = 2, 64
+    g = torch.Generator(device="cuda").manual_seed(8)
+    ql, kl = [2, 3, 2 + q_extra, 2], [40, 30, 80, 20]
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g, host_share=0.3)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    refs = _refs(q, start, ql, keys, vals, [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)], 0.1)
+    some = [0, 1, 3]
+    for row in (4, -1, 1 << 30, -(1 << 31), 2**31 - 1):
+        out.fill_(NAN)
+        lse.fill_(NAN)
+        gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), 0.1, out, lse, bt_row=i32([0, 1, row, 3]),
+                           max_q_len=max(ql))
+        with pytest.raises(RuntimeError, match="sequence length"):
+            gpu_ops.check_device_errors(dev())
+        ref.check_attn(out, lse, [refs[i] for i in some], [start[i] for i in some], [ql[i] for i in some], dtype, D,
+                       _rounded(dtype))
+    # a request without queries needs no row
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32([2, 3, 0, 2]), i32(kl), 0.1, out, lse, bt_row=i32([0, 1, 99, 3]))
+    gpu_ops.check_device_errors(dev())
+
+
 def test_attention_refusals():
     q = torch.zeros(4, 2, 64, dtype=torch.float16, device="cuda")
     i, one = i32([0]), i32([1])

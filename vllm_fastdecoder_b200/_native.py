@@ -147,7 +147,7 @@ class FdAttnArgs(ctypes.Structure):
         ("bt_row", c_void_p), ("k_start", c_void_p), ("q_start", c_void_p), ("q_len", c_void_p), ("k_len", c_void_p),
         ("bt_width", c_int32), ("num_tokens", c_int32), ("n", c_int32), ("num_heads", c_int32),
         ("num_kv_heads", c_int32), ("head_size", c_int32), ("block_size", c_int32), ("scale", c_float),
-        ("dtype", c_int32), ("max_q_len", c_int32), ("max_k_len", c_int32), ("_pad0", c_int32),
+        ("dtype", c_int32), ("max_q_len", c_int32), ("max_k_len", c_int32), ("bt_rows", c_int32),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("error", c_void_p),
     ]
 

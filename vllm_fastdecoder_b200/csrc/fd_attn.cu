@@ -525,6 +525,7 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
     return fdh::fail(FD_ERR_INVALID, "%s: q, out, q_start, q_len and k_len are required", what);
   if (chunk && (a->block_table == nullptr || a->bt_width <= 0 || a->bt_stride < 0 || a->block_size <= 0))
     return fdh::fail(FD_ERR_INVALID, "%s: block_table, bt_width and block_size are required", what);
+  if (chunk && a->bt_rows < 0) return fdh::fail(FD_ERR_INVALID, "%s: bt_rows must not be negative", what);
   if (!chunk && (a->k_start == nullptr || a->tier[0].k == nullptr || a->tier[0].v == nullptr))
     return fdh::fail(FD_ERR_INVALID, "%s: states and k_start are required", what);
   if (!chunk && a->tier[0].host_mapped)
@@ -567,6 +568,7 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   p.q_len = a->q_len;
   p.k_len = a->k_len;
   p.bt_width = a->bt_width;
+  p.bt_rows = a->bt_rows;
   p.n = a->n;
   p.T = a->num_tokens;
   p.H = a->num_heads;

@@ -57,7 +57,7 @@ struct AttnParams {
   const int32_t* bt_row;
   const int32_t* k_start;
   const int32_t *q_start, *q_len, *k_len;
-  int bt_width;
+  int bt_width, bt_rows;   // bt_rows 0: not known
   int n, T, H, KVH, G, D, BS;
   int host[2];             // tier is mapped host memory
   float sl2;               // scale * log2(e)
@@ -118,7 +118,8 @@ __device__ __forceinline__ Req load_req(const AttnParams& p, int r) {
   if (q.qlen > 0) {
     ok = ok && q.qst >= 0 && (long long)q.qst + q.qlen <= p.T;
     if (p.bt != nullptr)
-      ok = ok && ((long long)q.klen + p.BS - 1) / p.BS <= p.bt_width;
+      ok = ok && ((long long)q.klen + p.BS - 1) / p.BS <= p.bt_width && q.kbase >= 0 &&
+           (p.bt_rows == 0 || q.kbase < p.bt_rows);
     else
       ok = ok && (q.klen == 0 || (q.kbase >= 0 && (long long)q.kbase + q.klen <= p.nblk[0]));
   }

@@ -946,7 +946,7 @@ def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1,
         *((0, 0) if table is None else (table.data_ptr(), table.stride(0))),
         0 if bt_row is None else _i32(bt_row, idx, n, "bt_row"), 0 if k_start is None else _i32(k_start, idx, n, "k_start"),
         _i32(q_start, idx, n, "q_start"), _i32(q_len, idx, n, "q_len"), _i32(k_len, idx, n, "k_len"), W, T, n, H, KVH, D,
-        BS, scale, dtype_code(dt), max_q_len, max_k_len, 0, 0, 0, _error_ptr(idx)]
+        BS, scale, dtype_code(dt), max_q_len, max_k_len, 0 if table is None else table.shape[0], 0, 0, _error_ptr(idx)]
     if f1[-2]:  # a host tier: its copies count
         need = nat.load().fd_attn_workspace_size(_ATTN_STRUCT.pack(*packed))
     else:
@@ -972,7 +972,8 @@ def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier
 
     q, out [T, H, D]; per request (int32 [n] on the device) q_start, q_len,
     k_len: its queries are rows q_start .. of q and its K/V, the new tokens'
-    included, k_len tokens in the blocks of row bt_row[r] (default r) of
+    included, k_len tokens in the blocks of row bt_row[r] (default r; a row
+    outside the table: the request writes nothing and raises the error word) of
     block_table [R, W] int32; query i sees keys 0 .. k_len - q_len + i.  lse
     fp32 [H, T] or None.  Rows of no request stay as they were; a query that
     sees nothing gets 0 and -inf.  max_q_len / max_k_len: the lengths' bounds,
