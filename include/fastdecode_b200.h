@@ -567,16 +567,18 @@ enum fd_tables_flags {
  *   2. The blocks that the new tokens need beyond those a request holds are
  *      popped in request and position order, from the HBM stack while it has
  *      any, then from the host stack, and written to the table rows.
- *   3. seq_lens (0 for an ended request), query_start_loc (running sum of the
- *      new tokens), and per new token its slot (block id * block_size +
+ *   3. seq_lens (0 for an ended request), query_lens (the new tokens, 0 for an
+ *      ended request), query_start_loc (their running sum), and per new token its slot (block id * block_size +
  *      offset) and position; entries behind the last token, up to
  *      max_tokens, are slot -1 and position 0.
  * A step that cannot be applied as a whole (any FD_TABLES_* flag) changes
  * neither table nor stacks: counts_out = counts_in, seq_lens = prior_lens,
- * query_start_loc 0, slots -1, positions 0, and the error word gets
+ * query_lens and query_start_loc 0, slots -1, positions 0, and the error word gets
  * FD_DEVERR_TABLES.  The outputs are those of fd_plan_step's inputs, so a
- * step can be set up and planned without the host.  seq_lens may be
- * prior_lens and counts_out may be counts_in (in place); given separate
+ * step can be set up and planned without the host; query_lens and the first R
+ * of query_start_loc are fd_chunk_attn's and fd_cross_attn's q_len and q_start
+ * (new_lens is not: -1 is no length there).  seq_lens may be prior_lens,
+ * query_lens may be new_lens and counts_out may be counts_in (in place); given separate
  * buffers, the call can be repeated with the same result.  The ids on the
  * free stacks are the caller's and are not checked. */
 typedef struct fd_tables_args {
@@ -600,6 +602,7 @@ typedef struct fd_tables_args {
   int64_t *positions;        /* [max_tokens] */
   int32_t *header;           /* [FD_TABLES_HEADER_LEN] */
   int32_t *error;            /* optional device error word */
+  int32_t *query_lens;       /* [R] or NULL */
 } fd_tables_args;
 
 FD_API int fd_extend_tables(const fd_tables_args *a, void *stream);
@@ -761,7 +764,8 @@ FD_API int fd_host_register(void *host, size_t bytes);
 FD_API int fd_host_unregister(void *host);
 
 /* Library version, e.g. 101 for 0.1.1 (101: fd_plan_step, bt_rows; 102:
- * fd_extend_tables, fd_rope_store_kv, fd_chunk_attn, fd_cross_attn). */
+ * fd_extend_tables, fd_rope_store_kv, fd_chunk_attn, fd_cross_attn; 103:
+ * fd_tables_args.query_lens, fd_attn_args.bt_rows). */
 FD_API int fd_version(void);
 
 /* sizeof(fd_decode_args) and sizeof(fd_kv_tier) as compiled into the

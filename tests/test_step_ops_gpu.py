@@ -151,6 +151,30 @@ def test_refused_steps_change_nothing(why, flag, big):
     assert out.slot_mapping.tolist() == [-1] * T and out.positions.tolist() == [0] * T
 
 
+@pytest.mark.parametrize("R", [1, 40, 257, 3000])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_query_lens_are_what_the_attention_takes(R, in_place):
+    prior, new, table, stacks, counts, hbm, host = _table_case(R, 16, 60, 9, 3, 0.5, R)
+    free = FreeBlocks(i32(stacks[0]), i32(stacks[1]), i32(counts))
+    given = i32(new)
+    T = sum(max(0, n) for n in new) + 1
+    out = StepTables(R, T, dev())
+    if in_place:
+        out.query_lens = given
+    else:
+        out.query_lens.fill_(77)
+    gpu_ops.extend_tables(given, i32(prior), i32(table), free, hbm, host, 16, out)
+    assert out.read_header()["n_tok"] == T - 1
+    gpu_ops.check_device_errors(dev())
+    assert out.query_lens.tolist() == [max(0, n) for n in new]
+    # a step that is refused (more tokens than room) has none
+    given.copy_(i32([2] * R))
+    gpu_ops.extend_tables(given, i32(prior), i32(table), free, hbm, host, 16, out, max_tokens=2 * R - 1 if 2 * R <= T else 0)
+    with pytest.raises(RuntimeError, match="block tables"):
+        gpu_ops.check_device_errors(dev())
+    assert out.query_lens.tolist() == [0] * R and given.tolist() == ([0] * R if in_place else [2] * R)
+
+
 # ------------------------------------------------------------------ rope
 
 
@@ -790,4 +814,75 @@ def test_steps_together(dtype, D):
         ql = [max(0, n) for n in new]
         ref.check_attn(out, lse, refs, qsl_before[:R], ql, dtype, D, True)
         ref.check_attn(out_x, None, refs_x, qsl_before[:R], ql, dtype, D, True)
+    assert bool((table >= hbm).any())  # the batch did spill
+
+
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 128), (torch.float16, 64), (torch.float32, 64)])
+def test_one_graph_of_a_step_serves_every_step(dtype, D):
+    """The step as it is documented, captured once with room for T tokens: steps
+    of any size, that end requests, and one that does not fit, each a replay.
+    The device's error word is read after every one."""
+    H, KVH, block, R, W, T = 8, 2, 16, 6, 20, 420
+    hbm, host = 24, 70
+    g = torch.Generator(device="cuda").manual_seed(19)
+    cache = torch.full((hbm, block, KVH, 2 * D), NAN, device="cuda").to(dtype)
+    lg = cache.permute(0, 2, 1, 3)
+    hk = torch.full((host, KVH, block, D), NAN).to(dtype).pin_memory()
+    tiers = (KVTier(lg[..., :D], lg[..., D:]), KVTier(hk, hk.clone().pin_memory()))
+    table = torch.full((R, W), -1, dtype=torch.int32, device="cuda")
+    new_lens, prior_lens = (torch.zeros(R, dtype=torch.int32, device="cuda") for _ in range(2))
+    free = FreeBlocks(torch.arange(hbm, dtype=torch.int32, device="cuda"),
+                      hbm + torch.arange(host, dtype=torch.int32, device="cuda"), i32([hbm, host]))
+    cs = _cos_sin(600, D)
+    axis = gpu_ops.rope_axes((D // 2,))
+    t = StepTables(R, T, dev(), seq_lens=prior_lens, counts=free.counts)
+    q, k, v = (torch.zeros(T, h, D, device="cuda").to(dtype) for h in (H, KVH, KVH))
+    q_rot, k_rot, out = torch.empty_like(q), torch.empty_like(k), torch.empty_like(q)
+    lse = torch.empty(H, T, device="cuda")
+
+    def step():
+        gpu_ops.extend_tables(new_lens, prior_lens, table, free, hbm, host, block, t)
+        gpu_ops.rope_store_kv(q, k, v, t.positions, cs, t.slot_mapping, tiers, hbm, q_out=q_rot, k_out=k_rot)
+        gpu_ops.chunk_attn(q_rot, tiers, hbm, table, t.query_start_loc[:-1], t.query_lens, t.seq_lens, D ** -0.5, out, lse)
+
+    step()  # no new tokens: nothing but the warm-up
+    gpu_ops.check_device_errors(dev())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    hist = [([], []) for _ in range(R)]
+    for new in ([100, 1, 257, 0, 40, 7], [1, 4, 1, 70, 5, -1], [5, 5, -1, 1, 0, 33], [500, 1, 1, 1, 1, 1], [-1, -1, 9, -1, 8, 1],
+                [-1] * R, [2, 130, 1, 0, 1, 19]):
+        for x in (q, k, v):
+            x.copy_(torch.randn(x.shape, generator=g, device="cuda"))
+        out.fill_(NAN)
+        lse.fill_(NAN)
+        before = (table.clone(), prior_lens.clone(), free.counts.clone())
+        new_lens.copy_(i32(new))
+        graph.replay()
+        if sum(max(0, n) for n in new) > T:  # refused: nothing changes, no row is written
+            with pytest.raises(RuntimeError, match="block tables"):
+                gpu_ops.check_device_errors(dev())
+            assert all(torch.equal(a, b) for a, b in zip(before, (table, prior_lens, free.counts)))
+            assert bool(out.isnan().all()) and bool(lse.isnan().all())
+            continue
+        gpu_ops.check_device_errors(dev())
+        assert t.read_header()["n_tok"] == sum(max(0, n) for n in new)
+        ql = [max(0, n) for n in new]
+        start = [sum(ql[:r]) for r in range(R)]
+        refs = []
+        for r, n in enumerate(new):
+            a, b = start[r], start[r] + ql[r]
+            if n < 0:
+                hist[r] = ([], [])
+            hist[r][0].append(k_rot[a:b].clone())
+            hist[r][1].append(v[a:b].clone())
+            kk, vv = torch.cat(hist[r][0]), torch.cat(hist[r][1])
+            assert int(prior_lens[r]) == kk.shape[0]
+            refs.append(ref.attend(q_rot[a:b], kk, vv, kk.shape[0] - ql[r] + torch.arange(ql[r], device="cuda"), D ** -0.5)
+                        + (kk.shape[0],))
+        n = sum(ql)
+        if n > 0:
+            _rope_ok(q_rot[:n], ref.rope(q[:n], t.positions[None, :n], cs, axis, False), q[:n], dtype)
+        ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
     assert bool((table >= hbm).any())  # the batch did spill

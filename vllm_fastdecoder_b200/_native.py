@@ -120,6 +120,7 @@ class FdTablesArgs(ctypes.Structure):
         ("counts_in", c_void_p), ("counts_out", c_void_p), ("num_gpu_blocks", c_int64), ("num_cpu_blocks", c_int64),
         ("block_size", c_int32), ("max_tokens", c_int32), ("seq_lens", c_void_p), ("query_start_loc", c_void_p),
         ("slot_mapping", c_void_p), ("positions", c_void_p), ("header", c_void_p), ("error", c_void_p),
+        ("query_lens", c_void_p),
     ]
 
 

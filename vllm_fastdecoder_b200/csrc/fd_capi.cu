@@ -126,7 +126,7 @@ extern "C" int fd_host_unregister(void* host) {
   return fdh::cuda_status(cudaHostUnregister(host), "cudaHostUnregister");
 }
 
-extern "C" int fd_version(void) { return 102; }
+extern "C" int fd_version(void) { return 103; }
 
 extern "C" int fd_abi_sizes(size_t* decode_args_bytes, size_t* kv_tier_bytes) {
   if (decode_args_bytes != nullptr) *decode_args_bytes = sizeof(fd_decode_args);

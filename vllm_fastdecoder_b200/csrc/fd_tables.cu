@@ -254,6 +254,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
     for (int r = rank * kThreads + tid; r < R; r += step) {
       a.seq_lens[r] = s_prior[r];
       a.query_start_loc[r] = 0;
+      if (a.query_lens != nullptr) a.query_lens[r] = 0;
     }
     for (int t = rank * kThreads + tid; t < a.max_tokens; t += step) {
       a.slot_mapping[t] = -1;
@@ -329,6 +330,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
   for (int r = gt; r < R; r += step) {
     a.seq_lens[r] = s_new[r] < 0 ? 0 : s_prior[r] + s_new[r];
     a.query_start_loc[r] = s_tok[r];
+    if (a.query_lens != nullptr) a.query_lens[r] = max(s_new[r], 0);
   }
   for (int j = gt; j < need; j += step) {
     const int r = owner(s_need, 0, R, j);

@@ -713,7 +713,7 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_le
 _TIER_FMT = "PPqqqqii"
 _ATTN_STRUCT = struct.Struct("@PqqPqqPqq" + 2 * _TIER_FMT + "qPqPPPPPiiiiiiifiiiiPNP")
 _ROPE_STRUCT = struct.Struct("@" + 5 * "Pqq" + "PqPqP" + 2 * _TIER_FMT + f"q9i{nat.ROPE_MAX_PAIRS}siP")
-_TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPP")
+_TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPPP")
 _NO_TIER = (0, 0, 0, 0, 0, 0, 0, 0)
 
 
@@ -787,7 +787,7 @@ class StepTables:
         self.R, self.T = int(R), int(T)
         self.seq_lens = z(R, torch.int32) if seq_lens is None else seq_lens
         self.counts = z(2, torch.int32) if counts is None else counts
-        self.query_start_loc = z(R + 1, torch.int32)
+        self.query_lens, self.query_start_loc = z(R, torch.int32), z(R + 1, torch.int32)
         self.slot_mapping, self.positions = z(T, torch.int64), z(T, torch.int64)
         self.header = z(nat.TABLES_HEADER_LEN, torch.int32)
 
@@ -811,11 +811,14 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
     ends and gives its blocks back); prior_lens int32 [R]: its tokens in the
     cache; block_table int32 [R, W], changed in place; free: the stacks, HBM
     blocks are taken first.  Fills and returns `out` (or a new StepTables for
-    max_tokens new tokens): seq_lens, query_start_loc, slot_mapping (-1 behind
-    the last token), positions, counts and the header; its seq_lens,
-    query_start_loc and slot_mapping are what plan.plan_on_device takes.  A
-    step that cannot be applied as a whole changes nothing and sets
-    the error word (check_device_errors; StepTables.read_header says why)."""
+    max_tokens new tokens): seq_lens, query_lens, query_start_loc, slot_mapping
+    (-1 behind the last token), positions, counts and the header; its seq_lens,
+    query_start_loc and slot_mapping are what plan.plan_on_device takes, its
+    query_lens (0 where new_lens is -1) and query_start_loc chunk_attn's and
+    cross_attn's q_len and q_start.  The next step's prior_lens and free.counts
+    are its seq_lens and counts, which may be the same tensors.  A step that
+    cannot be applied as a whole changes nothing, has no tokens and sets the
+    error word (check_device_errors; StepTables.read_header says why)."""
     idx = block_table.get_device()
     if idx < 0:
         raise RuntimeError("block_table must be a CUDA tensor")
@@ -839,7 +842,7 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
         0 if host is None else host.numel(), _i32(counts, idx, 2, "free.counts"), _i32(out.counts, idx, 2, "out.counts"),
         num_gpu_blocks, num_cpu_blocks, block_size, T, _i32(out.seq_lens, idx, R, "out.seq_lens"),
         out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.header.data_ptr(),
-        _error_ptr(idx))
+        _error_ptr(idx), _i32(out.query_lens, idx, R, "out.query_lens"))
     _launch(nat.load().fd_extend_tables, packed, idx, "fd_extend_tables")
     return out
 
