@@ -734,8 +734,8 @@ FD_API size_t fd_attn_workspace_size(const fd_attn_args *a);
 FD_API int fd_chunk_attn(const fd_attn_args *a, void *stream);
 
 /* Cross attention to an encoder's states: every query of request r sees the
- * k_len[r] rows k_start[r] .. of the states (device memory); requests may
- * share rows.  q_len[r] = 1 is a decode step.  No counterpart in the
+ * k_len[r] rows k_start[r] .. of the states (device memory; none at all when
+ * num_blocks is 0, k and v may then be NULL); requests may share rows.  q_len[r] = 1 is a decode step.  No counterpart in the
  * reference, whose backend takes decoder attention only. */
 FD_API int fd_cross_attn(const fd_attn_args *a, void *stream);
 

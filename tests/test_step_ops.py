@@ -188,6 +188,17 @@ def test_chunk_attention_rejects_a_negative_number_of_table_rows():
     assert b"bt_rows" in nat.load().fd_last_error_message()
 
 
+def test_cross_attention_needs_pointers_of_states_that_are_there():
+    lib = nat.load()
+    for field in ("k", "v"):
+        a = _attn(False)
+        setattr(a.tier[0], field, None)
+        assert lib.fd_cross_attn(ctypes.byref(a), None) == 1
+        assert b"states" in lib.fd_last_error_message()
+        a.tier[0].num_blocks, a.workspace = 0, None  # none are: on to the next check
+        assert lib.fd_cross_attn(ctypes.byref(a), None) == 4
+
+
 def test_workspace_grows_with_the_head_and_is_zero_for_no_head():
     lib = nat.load()
     a = _attn()

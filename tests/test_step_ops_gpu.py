@@ -689,6 +689,27 @@ def test_single_tiles_over_many_key_tiles(dtype, D, block):
     _repeat_beside_copies(call, out, 400)
 
 
+@pytest.mark.parametrize("dtype,D,nq", [(torch.bfloat16, 128, 1), (torch.float16, 64, 40), (torch.float32, 64, 3),
+                                        (torch.bfloat16, 256, 5)])
+def test_cross_attention_without_any_states(dtype, D, nq):
+    H, KVH, n = 8, 2, 3
+    q = torch.randn(n * nq + 2, H, D, device="cuda").to(dtype)
+    k = torch.empty(0, KVH, D, device="cuda", dtype=dtype)
+    start, ql, none = i32([i * nq for i in range(n)]), i32([nq] * n), i32([0] * n)
+    for bound in (0, nq):
+        out, lse = torch.full_like(q, NAN), torch.full((H, q.shape[0]), NAN, device="cuda")
+        gpu_ops.cross_attn(q, k, k, start, ql, none, none, 0.1, out, lse, max_q_len=bound)
+        gpu_ops.check_device_errors(dev())
+        assert bool((out[:n * nq] == 0).all()) and bool((lse[:, :n * nq] == float("-inf")).all())
+        assert bool(out[n * nq:].isnan().all()) and bool(lse[:, n * nq:].isnan().all())
+    # a request that claims a key writes nothing
+    out.fill_(NAN)
+    gpu_ops.cross_attn(q, k, k, start, ql, none, i32([0, 1, 0]), 0.1, out, lse)
+    with pytest.raises(RuntimeError, match="sequence length"):
+        gpu_ops.check_device_errors(dev())
+    assert bool(out[nq:2 * nq].isnan().all()) and bool((out[:nq] == 0).all())
+
+
 def _keyless_batch(dtype, KVH, G, D, nq, n, seed):
     """cross_attn of n requests of up to nq tokens, most of which have no states."""
     rnd = random.Random(seed)

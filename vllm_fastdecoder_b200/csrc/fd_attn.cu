@@ -526,7 +526,9 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   if (chunk && (a->block_table == nullptr || a->bt_width <= 0 || a->bt_stride < 0 || a->block_size <= 0))
     return fdh::fail(FD_ERR_INVALID, "%s: block_table, bt_width and block_size are required", what);
   if (chunk && a->bt_rows < 0) return fdh::fail(FD_ERR_INVALID, "%s: bt_rows must not be negative", what);
-  if (!chunk && (a->k_start == nullptr || a->tier[0].k == nullptr || a->tier[0].v == nullptr))
+  // no state rows at all: no pointers either, and no request has keys
+  if (!chunk && (a->k_start == nullptr ||
+                 (a->tier[0].num_blocks > 0 && (a->tier[0].k == nullptr || a->tier[0].v == nullptr))))
     return fdh::fail(FD_ERR_INVALID, "%s: states and k_start are required", what);
   if (!chunk && a->tier[0].host_mapped)
     return fdh::fail(FD_ERR_UNSUPPORTED, "%s: states must be device memory", what);
