@@ -674,7 +674,8 @@ FD_API size_t fd_rope_args_bytes(void);
 /* Arguments of fd_chunk_attn and fd_cross_attn.  Request r has the queries
  * q_start[r] .. + q_len[r] - 1 of q; requests' query rows must not overlap.
  * Rows of out (and lse) that belong to no request are left as they were; a
- * query that sees no key gets out = 0 and lse = -inf. */
+ * query that sees no key gets out = 0 and lse = -inf, one whose scores hold a
+ * NaN gets NaN in both. */
 typedef struct fd_attn_args {
   const void *q;             /* [num_tokens, H, D] */
   int64_t q_stride_t, q_stride_h;

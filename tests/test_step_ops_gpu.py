@@ -530,6 +530,33 @@ def test_scores_far_apart(dtype, bound):
     ref.check_attn(out, lse, refs, start, [6], dtype, D, _rounded(dtype))
 
 
+@pytest.mark.parametrize("dtype,D,ql,kl", [
+    (torch.bfloat16, 128, [1, 4], [70, 9000]), (torch.float16, 64, [2, 1], [3000, 5]), (torch.bfloat16, 128, [20, 30], [40, 9000]),
+    (torch.float16, 64, [90, 300], [90, 5000]), (torch.float32, 64, [3, 40], [100, 4000]), (torch.bfloat16, 256, [2, 9], [50, 3000]),
+])
+def test_a_nan_in_a_query_is_its_own_rows_alone(dtype, D, ql, kl):
+    """o and lse of the (query, head) are NaN, whole or cut into parts; the lse of a
+    row without keys, -inf, stays apart."""
+    H, KVH = 4, 2
+    g = torch.Generator(device="cuda").manual_seed(D)
+    keys, vals, table, tiers, n_hbm = _paged(kl, KVH, D, 16, dtype, g)
+    q, start, out, lse = _queries(ql, H, D, dtype, g)
+    scale = D ** -0.5
+    lim = [k - n + torch.arange(n, device="cuda") for n, k in zip(ql, kl)]
+    refs = _refs(q, start, ql, keys, vals, lim, scale)
+    hit = [(start[0], 1, 0), (start[1] + ql[1] - 1, 3, D - 1), (start[1], 0, 7)]
+    for t, h, d in hit:
+        q[t, h, d] = NAN
+    gpu_ops.chunk_attn(q, tiers, n_hbm, table, i32(start), i32(ql), i32(kl), scale, out, lse, max_q_len=max(ql),
+                       max_k_len=max(kl))
+    gpu_ops.check_device_errors(dev())
+    for t, h, _ in hit:
+        assert bool(out[t, h].isnan().all()) and bool(lse[h, t].isnan())
+        r = 0 if t == start[0] else 1
+        out[t, h], lse[h, t] = refs[r][0][t - start[r], h].to(dtype), refs[r][1][h, t - start[r]].float()
+    ref.check_attn(out, lse, refs, start, ql, dtype, D, _rounded(dtype))
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_requests_that_do_not_fit_write_nothing(dtype):
     H, KVH, D = 4, 2, 64

@@ -17,8 +17,6 @@
 // half the threads took 2.1 cycles per FMA).  The next tile's K/V are fetched
 // into registers during this one's products.
 
-#include <math.h>
-
 #include "fd_attn.cuh"
 
 namespace fdk {
@@ -248,9 +246,9 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_attn_kernel(const __
           if (64 * d + 4 * tx < D) po[(16 * d + tx) * kRows] = *reinterpret_cast<const float4*>(&o[i][d]);
         continue;
       }
-      const float inv = li > 0.f ? 1.f / li : 0.f;
+      const float inv = row_inv(li);
       if (tx == 0 && p.lse != nullptr)
-        p.lse[h * p.lse_sh + tok * p.lse_st] = li > 0.f ? (m[i] + log2f(li)) * kLn2 : -INFINITY;
+        p.lse[h * p.lse_sh + tok * p.lse_st] = row_lse(m[i], li);
       T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + h * p.o_sh);
 #pragma unroll
       for (int d = 0; d < kDim4; ++d) {
@@ -360,14 +358,13 @@ __global__ void __launch_bounds__(kCombineThreads) fd_attn_combine_kernel(const 
     l = 0.f;
     for (int x = 0; x < kCombineLanes; ++x) l += red[x][lane];
     const int at = row0 + lane;
-    p.lse[(cut.kh * p.G + at % p.G) * p.lse_sh + (int64_t)(cut.row0 + at / p.G) * p.lse_st] =
-        l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+    p.lse[(cut.kh * p.G + at % p.G) * p.lse_sh + (int64_t)(cut.row0 + at / p.G) * p.lse_st] = row_lse(m, l);
   }
   if (!ok[0]) return;
   l = 0.f;
 #pragma unroll
   for (int x = 0; x < kCombineLanes; ++x) l += red[x][sub];
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = row_inv(l);
   const int64_t tok = cut.row0 + row / p.G;
   T* po = reinterpret_cast<T*>(p.out + tok * p.o_st + (cut.kh * p.G + row % p.G) * p.o_sh);
 #pragma unroll

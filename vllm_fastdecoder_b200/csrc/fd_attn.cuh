@@ -23,6 +23,8 @@
 // recursion), one thread per request, then one scan.
 #pragma once
 
+#include <math.h>
+
 #include "fd_common.cuh"
 #include "fd_internal.h"
 
@@ -70,6 +72,11 @@ struct AttnParams {
   int out32;               // rows of out are 32-byte aligned (fd_attn_mma.cu)
   int32_t* err;
 };
+
+// 1 / l, and the natural log-sum-exp, of a row with maximum m (log2 domain) and
+// sum l: 0 and -inf where no key is seen (l = 0), and a NaN stays a NaN.
+__device__ __forceinline__ float row_inv(float l) { return l == 0.f ? 0.f : 1.f / l; }
+__device__ __forceinline__ float row_lse(float m, float l) { return l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2; }
 
 // 2^x by the SFU's ex2 instruction (relative error a few ulp; 2^-inf = 0).
 __device__ __forceinline__ float ex2_approx(float x) {

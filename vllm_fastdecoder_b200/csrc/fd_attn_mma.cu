@@ -50,8 +50,6 @@
 // as fast: the row maximum found in the SFU's shadow (605 us), fewer commits
 // (602 us).
 
-#include <math.h>
-
 #include <type_traits>
 
 #include "fd_attn_mma.cuh"
@@ -159,7 +157,7 @@ __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg
   const int h = seg.kh * p.G + hg;
   const bool have_b = single && seg.n1 > 0;
   const bool have = single ? m_tiles > 0 : n > 0;
-  const float inv = slot >= 0 ? 1.f : l > 0.f ? 1.f / l : 0.f;
+  const float inv = slot >= 0 ? 1.f : row_inv(l);
   wa *= inv;
   wb *= inv;
   const int item_row = (pair ? x * p.tq * p.G : 0) + row;
@@ -167,7 +165,7 @@ __device__ __noinline__ bool finish_rows(const AttnParams& p, const SegInfo& seg
     if (slot >= 0) {
       reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * kItemRows + item_row] = make_float2(m, l);
     } else if (p.lse != nullptr) {
-      p.lse[h * p.lse_sh + tok * p.lse_st] = l > 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
+      p.lse[h * p.lse_sh + tok * p.lse_st] = row_lse(m, l);
     }
   }
   __syncwarp();

@@ -31,8 +31,6 @@
 // 101); 24 of one token over 1500 keys of 20 heads x 64 in 48 us (fd_attn_mma
 // 72); one request of 16384 keys, 1 and 8 tokens, in 25 and 28 us (33 and 34).
 
-#include <math.h>
-
 #include <type_traits>
 
 #include "fd_attn_mma.cuh"
@@ -513,7 +511,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
       if (tid < NC) {
         const float lt = red[tid] + red[NC + tid] + red[2 * NC + tid] + red[3 * NC + tid];
         const float mt = m_tiles > 0 ? m_sh[tid] : -INFINITY;
-        f_sh[tid] = slot >= 0 ? 1.f : lt > 0.f ? 1.f / lt : 0.f;
+        f_sh[tid] = slot >= 0 ? 1.f : row_inv(lt);
         const int t = tid / p.G, h = seg.kh * p.G + tid - t * p.G;
         const int64_t tok = seg.qst + seg.tok0 + t;
         row_sh[tid] = tok * p.o_st + h * p.o_sh;
@@ -521,7 +519,7 @@ __global__ void __launch_bounds__(kThreads, KD == 64 ? 2 : 1) fd_attn_rows_kerne
           if (slot >= 0)
             reinterpret_cast<float2*>(p.part_ml)[(int64_t)slot * NC + tid] = make_float2(mt, lt);
           else if (p.lse != nullptr)
-            p.lse[h * p.lse_sh + tok * p.lse_st] = lt > 0.f ? (mt + log2f(lt)) * kLn2 : -INFINITY;
+            p.lse[h * p.lse_sh + tok * p.lse_st] = row_lse(mt, lt);
         }
       }
       uint32_t o[NC];
