@@ -19,8 +19,7 @@
 // one segment of an item that began earlier (slot 0) and one of an item that
 // ends later (slot 1); all others are whole and written directly.  The
 // lengths are device data, so each CTA finds its start itself: the cost of a
-// request is a closed form (sums of floor((a i + b) / c) by the Euclidean
-// recursion), one thread per request, then one scan.
+// request is a closed form (staircase), one thread per request, then one scan.
 #pragma once
 
 #include <math.h>
@@ -85,28 +84,36 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 
-// sum of floor((a i + b) / m) over 0 <= i < n, by the Euclidean recursion on
-// (a, m); a n + b < 2^32.
-__device__ __forceinline__ long long floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-  long long ans = 0;
-  while (n > 0) {
+// The sum of floor((a i + b) / m) over 0 <= i < n, for a n + b + m < 2^32: a
+// staircase of key tiles.  The whole multiples of m in a and b are added at
+// once.  What is left is the number of points (i, y) with 1 <= y and m y <=
+// a i + b, none of them above `top`.  It is n top less the points above the
+// line, and at height y those are the i below ceil((m y - b) / a) =
+// floor((m (y - 1) + m - b + a - 1) / a): a staircase again, over top steps
+// and with a and m exchanged, so that the numbers shrink as in Euclid's
+// division.
+__device__ __forceinline__ long long staircase(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+  long long sum = 0;
+  for (bool minus = false; n > 0; minus = !minus) {
+    long long part = 0;
     if (a >= m) {
-      ans += (long long)n * (n - 1) / 2 * (a / m);
+      part = (long long)(a / m) * ((long long)n * (n - 1) / 2);
       a %= m;
     }
     if (b >= m) {
-      ans += (long long)n * (b / m);
+      part += (long long)(b / m) * n;
       b %= m;
     }
-    const uint32_t y = a * n + b;
-    if (y < m) break;
-    n = y / m;
-    b = y % m;
-    const uint32_t t = m;
+    const uint32_t top = (a * (n - 1) + b) / m;
+    part += (long long)n * top;
+    sum += minus ? -part : part;
+    const uint32_t was_m = m;
+    b = m - b + a - 1;
     m = a;
-    a = t;
+    a = was_m;
+    n = top;  // 0: no point is left (m may be 0 then)
   }
-  return ans;
+  return sum;
 }
 
 // A request's lengths, or qlen = 0 when it has no work (or does not fit its
@@ -191,7 +198,7 @@ struct Sched {
         const int st = u * p.tq, b = q.klen - q.qlen;
         const int m0 = b + st > 0 ? 0 : min(reg, -b / st);  // items whose queries see nothing
         if (reg > m0)
-          ans += u * floor_sum((uint32_t)(reg - m0), kKT, (uint32_t)st,
+          ans += u * staircase((uint32_t)(reg - m0), kKT, (uint32_t)st,
                                (uint32_t)((long long)b + (long long)(m0 + 1) * st + kKT - 1));
       }
     }
