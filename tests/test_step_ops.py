@@ -10,7 +10,7 @@ import pytest
 import torch
 
 from vllm_fastdecoder_b200 import _native as nat
-from vllm_fastdecoder_b200 import gpu_ops
+from vllm_fastdecoder_b200 import gpu_ops, kernel_bench
 
 
 def test_struct_mirrors_and_packers_match_the_library():
@@ -216,6 +216,14 @@ def test_axes_of_pairs():
     for bad in ((), (0, 0), (1, 1, 1, 1, 1), (3, -1), (129,)):
         with pytest.raises(RuntimeError):
             gpu_ops.rope_axes(bad)
+
+
+def test_bench_counts_a_cosine_and_a_sine_per_pair():
+    """Bytes of the rotary bench: q, k, v in and out, and per token the angles of
+    its pairs, each from one axis, three positions and a slot."""
+    _, nbytes, _ = kernel_bench.case_rope_store_kv(torch.device("meta"))
+    T, H, KVH, D = 16384, 32, 8, 128
+    assert nbytes == 2 * T * (H + 2 * KVH) * D * 2 + T * (2 * (D // 2) * 4 + 3 * 8 + 8)
 
 
 def test_front_end_refuses_host_tensors():

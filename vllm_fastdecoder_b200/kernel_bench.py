@@ -312,7 +312,8 @@ def case_rope_store_kv(dev):
     cs = torch.cat((ang.cos(), ang.sin()), 1)
     kc, vc = (torch.empty(T // bs, KVH, bs, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
     slots = torch.randperm(T, device=dev)
-    nbytes = 2 * D * T * (2 * H + 4 * KVH) + T * (3 * D * 4 + 32)
+    # a token's cosines and sines: one of each per pair, from the pair's own axis
+    nbytes = 2 * D * T * (2 * H + 4 * KVH) + T * (D * 4 + 32)
     return (lambda: gpu_ops.rope_store_kv(q, k, v, pos, cs, slots, (KVTier(kc, vc), None), T // bs, sections=(24, 20, 20)),
             nbytes, "fd_rope_kernel")
 
