@@ -1,7 +1,7 @@
 // Chunk and cross attention on the 5th-generation tensor cores (tcgen05): fp16
 // and bf16, head sizes 64 to 128 (padded to 64 or 128 dims in shared memory).
 //
-//   S [128 rows x 128 keys] = Q . K^T,  P = 2^(scale log2(e) S - m),
+//   S [128 rows x 64 keys] = Q . K^T,  P = 2^(scale log2(e) S - m),
 //   l = sum P,  O [128 rows x D] += P . V,  o = O / l, lse = ln 2 (m + log2 l)
 //
 // A CTA walks its range of the schedule (fd_attn.cuh) segment by segment and
@@ -40,8 +40,8 @@
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 2 x 2048 tokens of 32 heads over up to 12288 keys of 8 heads x 128
-// in 600 us, 985 TFLOP/s (over 8192: 446 us, 1078).  The tensor pipe is busy
-// for 68% of the time: q.K^T of 64 keys is held up by the shared memory that
+// in 594 us, 995 TFLOP/s (over 8192: 440 us, 1093).  The tensor pipe is busy
+// for 67% of the time: q.K^T of 64 keys is held up by the shared memory that
 // feeds it (48 cycles per MMA for 32 of arithmetic, ~68 beside the other
 // stream's and the TMA's writes), and a step of both streams takes 1750 cycles
 // where 1270 of MMAs alone would do and the SFU needs 1024.  Tried and slower:

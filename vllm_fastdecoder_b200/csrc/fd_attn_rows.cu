@@ -27,9 +27,9 @@
 // softmax warps agree at their barriers on going on.
 //
 // Measured: 32 requests of 1, 4 and 8 tokens of 32 heads over 4096 keys of 8
-// heads x 128 in 88, 90 and 92 us (6.0 TB/s of cache read; fd_attn_mma 98 to
-// 101); 24 of one token over 1500 keys of 20 heads x 64 in 48 us (fd_attn_mma
-// 72); one request of 16384 keys, 1 and 8 tokens, in 25 and 28 us (33 and 34).
+// heads x 128 in 87, 88 and 92 us (6.0 TB/s of cache read; fd_attn_mma 98 to
+// 101); 24 of one token over 1500 keys of 20 heads x 64 in 47 us (fd_attn_mma
+// 71); one request of 16384 keys, 1 and 8 tokens, in 25 and 28 us (31 and 31).
 
 #include <type_traits>
 

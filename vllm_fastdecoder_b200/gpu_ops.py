@@ -779,7 +779,9 @@ class FreeBlocks:
 class StepTables:
     """Device buffers that extend_tables fills for a step of up to R requests
     and T new tokens.  seq_lens and counts may be the caller's own tensors:
-    the prior lengths and the free stacks' counts, to step them in place."""
+    the prior lengths and the free stacks' counts, to step them in place.  A
+    call for fewer requests fills the first entries of each and leaves those
+    behind as they were."""
 
     def __init__(self, R: int, T: int, device, seq_lens: torch.Tensor | None = None,
                  counts: torch.Tensor | None = None):
