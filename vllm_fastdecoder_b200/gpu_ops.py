@@ -971,8 +971,8 @@ def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier
                max_k_len: int = 0, workspace_buf: torch.Tensor | None = None) -> None:
     """Attention of each request's new tokens over its paged cache in both
     tiers (fd_chunk_attn): chunks of prompts, draft tokens to verify, single
-    tokens.  Unlike prefill_attn it reads the host tier too, takes any head
-    size, block size and dtype, splits long contexts over the GPU when there
+    tokens.  Unlike prefill_attn it reads the host tier too, takes head sizes
+    up to 256 (of whole 16 bytes) and any block size and dtype, splits long contexts over the GPU when there
     are few queries, and returns the log-sum-exp.
 
     q, out [T, H, D]; per request (int32 [n] on the device) q_start, q_len,
