@@ -308,7 +308,7 @@ def _prepare_trim(case, seed):
     for t in range(2):
         stack[t, :len(free[t])] = torch.tensor(free[t], dtype=torch.int32)
     s = dict(seq=_i32(seq), keep=_i32(keep), table=_i32(rows), stack=stack.to(DEV), counts=_i32([len(f) for f in free]),
-             n_gpu=n_gpu, n_cpu=total - n_gpu, bs=bs)
+             n_gpu=n_gpu, n_cpu=total - n_gpu, bs=bs, max_cut=case["cut_hi"])
     if own:
         from vllm_fastdecoder_b200 import gpu_ops
 
@@ -435,7 +435,8 @@ def _run_trim(s):
     if own:
         from vllm_fastdecoder_b200 import gpu_ops
 
-        t = gpu_ops.trim_tables(s["keep"], s["seq"], s["table"], s["free"], s["n_gpu"], s["n_cpu"], s["bs"], s["out"])
+        t = gpu_ops.trim_tables(s["keep"], s["seq"], s["table"], s["free"], s["n_gpu"], s["n_cpu"], s["bs"], s["out"],
+                                max_cut=s["max_cut"])
         return [s["stack"], t.counts, t.seq_lens]
     seq, table, stack, bs = s["seq"], s["table"], s["stack"], s["bs"]
     cap = stack.shape[1]
