@@ -69,7 +69,9 @@ enum fd_device_error {
                               its KV is in the host tier (fastdecode/plan.py:142-149) */
   FD_DEVERR_TABLES = 7,    /* fd_extend_tables refused the step (FD_TABLES_* bits
                               in its header say why) */
-  FD_DEVERR_POSITION = 8   /* fd_rope_store_kv: position outside the table */
+  FD_DEVERR_POSITION = 8,  /* fd_rope_store_kv: position outside the table */
+  FD_DEVERR_TOKEN = 9,     /* fd_verify_drafts: drafted token outside the vocabulary */
+  FD_DEVERR_PROBS = 10     /* fd_verify_drafts: a row of the target without any probability */
 };
 
 /* ---------------------------------------------------------------- types */
@@ -603,12 +605,112 @@ typedef struct fd_tables_args {
   int32_t *header;           /* [FD_TABLES_HEADER_LEN] */
   int32_t *error;            /* optional device error word */
   int32_t *query_lens;       /* [R] or NULL */
+  int32_t *evicted;          /* [R] or NULL: tokens that fd_trim_tables cut from the request to meet a
+                                budget.  Positions are ahead of cache indices by as many; an ended
+                                request's entry becomes 0 */
 } fd_tables_args;
 
 FD_API int fd_extend_tables(const fd_tables_args *a, void *stream);
 
 /* sizeof(fd_tables_args) as compiled into the library (binding check). */
 FD_API size_t fd_tables_args_bytes(void);
+
+/* ------------------------------------------------------- shorter tables */
+
+/* Cuts requests to their first keep_lens tokens and gives the blocks behind
+ * them back: what follows a step whose drafted tokens were partly rejected
+ * (fd_verify_drafts) or whose caches were cut to a budget (fd_move_keys, once
+ * every layer has moved its keys).  No counterpart in the reference, where the
+ * engine's block manager keeps the lengths.  A request with keep_lens below 0
+ * or not below lens_in is left as it is.  For the others the blocks of columns
+ * ceil(keep / block_size) .. ceil(len / block_size) - 1 of their table row are
+ * pushed onto their tier's stack, in request and column order, lens_out = keep,
+ * and, where given, evicted grows by len - keep.  The table itself is not
+ * written: what it lists behind a request's length is never read.  A call that
+ * cannot be applied as a whole (FD_TABLES_BAD_LEN: a length below 0 or past the
+ * row; FD_TABLES_BAD_BLOCK; FD_TABLES_BAD_POOL) changes neither stacks nor
+ * evicted, copies lens_in and counts_in and sets FD_DEVERR_TABLES.  lens_out may be
+ * lens_in or keep_lens, counts_out may be counts_in; given separate buffers (and no
+ * evicted), the call can be repeated with the same result. */
+typedef struct fd_trim_args {
+  const int32_t *keep_lens;  /* [R] */
+  const int32_t *lens_in;    /* [R] */
+  int32_t *lens_out;         /* [R] */
+  int32_t *evicted;          /* [R] or NULL */
+  const int32_t *block_table; /* [R, bt_stride] */
+  int64_t bt_stride;
+  int32_t bt_width;
+  int32_t num_reqs;          /* R, at most FD_TABLES_MAX_REQS */
+  int32_t *free_ids[2];      /* [free_cap[t]] */
+  int32_t free_cap[2];
+  const int32_t *counts_in;  /* [2] */
+  int32_t *counts_out;       /* [2] */
+  int64_t num_gpu_blocks;
+  int64_t num_cpu_blocks;
+  int32_t block_size;
+  int32_t max_cut;           /* the host's bound on len - keep, 0: unknown.  It chooses the launch;
+                                a wrong one costs time, not the result */
+  int32_t *header;           /* [FD_TABLES_HEADER_LEN]: FLAGS, FREED_HBM, FREED_HOST and MAX_SEQ; others 0 */
+  int32_t *error;            /* optional device error word */
+} fd_trim_args;
+
+FD_API int fd_trim_tables(const fd_trim_args *a, void *stream);
+
+/* sizeof(fd_trim_args) as compiled into the library (binding check). */
+FD_API size_t fd_trim_args_bytes(void);
+
+/* --------------------------------------------------------- drafted tokens */
+
+#define FD_VERIFY_MAX_DRAFTS 1024
+
+/* Speculative sampling's verification.  Request r has q_len[r] rows of the
+ * target's probabilities from row q_start[r] on (its step's queries), the
+ * first q_len - 1 of which its drafted tokens are held against; q_len = 0: it
+ * takes no part.  With p the target's row of draft d, q the draft's own
+ * probabilities of it (1 at the token where draft_probs is NULL) and x the
+ * token, d is accepted while
+ *   accept_u[r][d] q(x) < p(x)
+ * holds for it and all before it.  The token that follows the accepted ones is
+ * drawn with the weights w = max(p - q, 0) of the rejected draft's rows (p with
+ * the token struck out where draft_probs is NULL), or, when all were accepted,
+ * w = p of the last row: the first token whose running sum of w passes
+ * sample_u[r] times the whole sum.  Where w is 0 throughout it is p; where that
+ * is, too, the token is -1 (FD_DEVERR_PROBS).  Values that are negative or not finite
+ * count as 0; sample_u counts as if clamped to [0, 1), a NaN as 0.  Products,
+ * differences and sums are fp64, so the probabilities need not add up to 1.
+ * tokens[r]: the accepted drafts, the drawn token, then -1.  keep_lens (with
+ * lens): lens less the rejected drafts, fd_trim_tables' keep_lens.  A request
+ * whose lengths do not fit (FD_DEVERR_LEN) gets no tokens and keeps its length; a
+ * draft outside the vocabulary is rejected (FD_DEVERR_TOKEN). */
+typedef struct fd_verify_args {
+  const void *target;        /* [num_rows, V], rows target_stride apart */
+  int64_t target_stride;
+  const void *draft_probs;   /* [R, K, V], contiguous in V, or NULL; target's dtype */
+  int64_t draft_stride_r, draft_stride_k;
+  const int64_t *draft_tokens; /* [R, K] */
+  int64_t tokens_stride;
+  const int32_t *q_start;    /* [R] */
+  const int32_t *q_len;      /* [R], at most K + 1 */
+  const float *accept_u;     /* [R, K] */
+  int64_t accept_stride;
+  const float *sample_u;     /* [R] */
+  const int32_t *lens;       /* [R] or NULL */
+  int64_t *tokens;           /* [R, K + 1] */
+  int32_t *accepted;         /* [R] */
+  int32_t *keep_lens;        /* [R], with lens */
+  int32_t num_reqs;
+  int32_t num_drafts;        /* K, at most FD_VERIFY_MAX_DRAFTS */
+  int32_t vocab;             /* V */
+  int32_t num_rows;
+  int32_t dtype;
+  int32_t _pad0;
+  int32_t *error;            /* optional device error word */
+} fd_verify_args;
+
+FD_API int fd_verify_drafts(const fd_verify_args *a, void *stream);
+
+/* sizeof(fd_verify_args) as compiled into the library (binding check). */
+FD_API size_t fd_verify_args_bytes(void);
 
 /* ------------------------------------------- rotary positions + KV write */
 
@@ -743,6 +845,117 @@ FD_API int fd_cross_attn(const fd_attn_args *a, void *stream);
 /* sizeof(fd_attn_args) as compiled into the library (binding check). */
 FD_API size_t fd_attn_args_bytes(void);
 
+/* ------------------------------------------- keys by their attention weight */
+
+/* What each cached key has received: weights fp32 and positions int32, both
+ * [num_blocks, KVH, block_size] contiguous in device memory and indexed by
+ * block id, host-tier blocks included. */
+typedef struct fd_key_stats {
+  float *weights;
+  int32_t *positions;
+  int64_t num_blocks;
+} fd_key_stats;
+
+/* The attention weight that a step's queries gave to each key of their paged
+ * caches, added up per kv head:
+ *   w[j] = sum over the heads h of the kv head and the queries i that see j of
+ *          exp(scale q[i,h] . k[j] - lse[h, i])
+ * with chunk attention's arguments (`attn`, whose lse is an input here and
+ * must be given; out is not used) and its rules for who sees what.  A request's
+ * q_len newest keys are new: their weight is set and their position becomes
+ * their index plus evicted[r]; older keys' weights are added to.  A row with
+ * lse = -inf or +inf gives nothing, one with a NaN makes the weights of the keys that
+ * it sees NaN.  Every key gets one addition, so results do not depend on timing (a
+ * block that several requests list gets one of each, in no fixed order).  A
+ * request whose lengths do not fit its rows changes nothing (FD_DEVERR_LEN); a block id
+ * outside the tiers or the stats is passed over (FD_DEVERR_BLOCK_ID).  No counterpart in
+ * the reference, which keeps every key. */
+typedef struct fd_key_weights_args {
+  fd_attn_args attn;         /* workspace: fd_key_weights_workspace_size() bytes */
+  fd_key_stats stats;
+  const int32_t *evicted;    /* [n] int32 or NULL */
+} fd_key_weights_args;
+
+FD_API int fd_key_weights(const fd_key_weights_args *a, void *stream);
+
+/* Scratch bytes of fd_key_weights for these arguments (see
+ * fd_attn_workspace_size). */
+FD_API size_t fd_key_weights_workspace_size(const fd_key_weights_args *a);
+
+/* sizeof(fd_key_weights_args) as compiled into the library (binding check). */
+FD_API size_t fd_key_weights_args_bytes(void);
+
+/* Which keys stay when request r's cache of lens[r] tokens is cut to
+ * keep_lens[r]: per kv head the first keep in the order of
+ *   1. guarded keys: position < sinks or position >= lens + evicted - recent,
+ *   2. weight, the greatest first (a NaN last),
+ *   3. index, the lowest first (among guarded ones this alone).
+ * Keys that stay and lie at keep or behind it move into the places of keys
+ * before keep that go, both in ascending order: pair i moves key src[i] to
+ * dst[i], src >= keep > dst.  counts[r][h] pairs are written; entries behind
+ * them are left as they were.  A request with keep_lens below 0 or not below
+ * lens has none, and so has one whose lengths do not fit its table row or whose
+ * pairs could be more than `room` (min(keep, lens - keep); FD_DEVERR_LEN), or that lists a
+ * block outside the stats (FD_DEVERR_BLOCK_ID).  Nothing but src, dst and counts is
+ * written: fd_move_keys moves. */
+typedef struct fd_select_args {
+  fd_key_stats stats;
+  const int32_t *block_table; /* [R, bt_stride] */
+  int64_t bt_stride;
+  const int32_t *lens;       /* [R] */
+  const int32_t *keep_lens;  /* [R] */
+  const int32_t *evicted;    /* [R] or NULL */
+  int32_t *src;              /* [R, KVH, room] */
+  int32_t *dst;              /* [R, KVH, room] */
+  int32_t *counts;           /* [R, KVH] */
+  int32_t bt_width;
+  int32_t num_reqs;          /* at most 65535 */
+  int32_t num_kv_heads;
+  int32_t block_size;
+  int32_t room;
+  int32_t sinks;
+  int32_t recent;
+  int32_t max_len;           /* the host's bound on lens, 0: unknown.  It chooses the launch; a wrong
+                                one costs time, not the result */
+  int32_t *error;            /* optional device error word */
+} fd_select_args;
+
+FD_API int fd_select_keys(const fd_select_args *a, void *stream);
+
+/* sizeof(fd_select_args) as compiled into the library (binding check). */
+FD_API size_t fd_select_args_bytes(void);
+
+/* Moves the K and V rows of fd_select_keys' pairs within each request's
+ * blocks, in either tier, and, with stats.weights, their weights and
+ * positions.  Per request and kv head the src and the dst indices have to
+ * differ from one another and no src may be a dst (as fd_select_keys gives
+ * them).  A pair with an index outside the table row (FD_DEVERR_LEN) or a block outside
+ * the tiers (FD_DEVERR_BLOCK_ID) is passed over, and so is a count outside 0 .. room (FD_DEVERR_LEN). */
+typedef struct fd_move_args {
+  const int32_t *src;        /* [R, KVH, room] */
+  const int32_t *dst;        /* [R, KVH, room] */
+  const int32_t *counts;     /* [R, KVH] */
+  fd_kv_tier tier[2];
+  int64_t tier_split;
+  const int32_t *block_table; /* [R, bt_stride] */
+  int64_t bt_stride;
+  fd_key_stats stats;        /* weights NULL: K and V alone */
+  int32_t bt_width;
+  int32_t num_reqs;          /* at most 65535 */
+  int32_t num_kv_heads;
+  int32_t head_size;         /* head_size * element size a multiple of 16 bytes */
+  int32_t block_size;
+  int32_t room;
+  int32_t dtype;
+  int32_t _pad0;
+  int32_t *error;            /* optional device error word */
+} fd_move_args;
+
+FD_API int fd_move_keys(const fd_move_args *a, void *stream);
+
+/* sizeof(fd_move_args) as compiled into the library (binding check). */
+FD_API size_t fd_move_args_bytes(void);
+
 /* ---------------------------------------------------------------- utilities */
 
 /* Message of the last FD_ERR_* returned on this thread. */
@@ -766,7 +979,9 @@ FD_API int fd_host_unregister(void *host);
 
 /* Library version, e.g. 101 for 0.1.1 (101: fd_plan_step, bt_rows; 102:
  * fd_extend_tables, fd_rope_store_kv, fd_chunk_attn, fd_cross_attn; 103:
- * fd_tables_args.query_lens, fd_attn_args.bt_rows). */
+ * fd_tables_args.query_lens, fd_attn_args.bt_rows; 104: fd_trim_tables,
+ * fd_verify_drafts, fd_key_weights, fd_select_keys, fd_move_keys,
+ * fd_tables_args.evicted). */
 FD_API int fd_version(void);
 
 /* sizeof(fd_decode_args) and sizeof(fd_kv_tier) as compiled into the

@@ -1,0 +1,733 @@
+"""GPU tests of the operators behind a step's attention against plain forms
+(tests/serving_ref.py): weights per cached key, the choice and the move of the
+keys that stay, trimmed tables, verified drafts, and a run of them together."""
+
+from __future__ import annotations
+
+import math
+import random
+
+import pytest
+import serving_ref as ref
+import torch
+
+from vllm_fastdecoder_b200 import gpu_ops
+from vllm_fastdecoder_b200.gpu_ops import DraftVerdict, FreeBlocks, KeyMoves, KeyStats, KVTier, StepTables, TrimTables
+
+pytestmark = pytest.mark.gpu
+NAN = float("nan")
+
+
+def dev():
+    return torch.device("cuda", torch.cuda.current_device())
+
+
+def i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def ok():
+    gpu_ops.check_device_errors(dev())
+
+
+def fails(text):
+    with pytest.raises(RuntimeError, match=text):
+        gpu_ops.check_device_errors(dev())
+
+
+# ------------------------------------------------------------------ a paged cache
+
+
+class Paged:
+    """Requests of these lengths over shuffled blocks of both tiers; what no
+    request holds is NaN."""
+
+    def __init__(self, lens, KVH, BS, D, dtype, host=0.0, seed=0, layout="interleaved", spare=3):
+        rnd = random.Random(seed)
+        g = torch.Generator().manual_seed(seed)
+        held = [-(-n // BS) for n in lens]
+        total = sum(held)
+        self.C = int(total * host)
+        self.G = total - self.C + spare
+        ids = [b if b < total - self.C else self.G + b - (total - self.C) for b in range(total)]
+        rnd.shuffle(ids)
+        W = max(held + [1]) + 2
+        rows, at = [], 0
+        for h in held:
+            rows.append(ids[at:at + h] + [-9] * (W - h))
+            at += h
+        self.rows, self.lens, self.BS, self.KVH, self.D = rows, lens, BS, KVH, D
+        self.table = i32(rows)
+        blocks = self.G + self.C
+        keys = [torch.randn(n, KVH, D, generator=g).to(dtype) for n in lens]
+        vals = [torch.randn(n, KVH, D, generator=g).to(dtype) for n in lens]
+        k = torch.full((blocks, KVH, BS, D), NAN).to(dtype)
+        v = k.clone()
+        for r, n in enumerate(lens):
+            for b in range(held[r]):
+                m = min(BS, n - b * BS)
+                k[rows[r][b], :, :m] = keys[r][b * BS:b * BS + m].transpose(0, 1)
+                v[rows[r][b], :, :m] = vals[r][b * BS:b * BS + m].transpose(0, 1)
+        self.k0, self.v0, self.keys, self.vals = k, v, keys, vals
+        if layout == "interleaved":
+            c = torch.cat([k[:self.G], v[:self.G]], -1).transpose(1, 2).contiguous().cuda()
+            hk, hv = c.transpose(1, 2)[..., :D], c.transpose(1, 2)[..., D:]
+        elif layout == "tokens":
+            hk, hv = (x[:self.G].transpose(1, 2).contiguous().cuda().transpose(1, 2) for x in (k, v))
+        else:
+            hk, hv = (x[:self.G].contiguous().cuda() for x in (k, v))
+        host_tier = KVTier(k[self.G:].contiguous().pin_memory(), v[self.G:].contiguous().pin_memory()) if self.C else None
+        self.tiers = (KVTier(hk, hv), host_tier)
+
+    def now(self):
+        """K and V of all blocks as they are now, on the host."""
+        torch.cuda.synchronize()
+        out = []
+        for name in ("k", "v"):
+            parts = [getattr(self.tiers[0], name).cpu()]
+            if self.tiers[1] is not None:
+                parts.append(getattr(self.tiers[1], name).clone())
+            out.append(torch.cat(parts))
+        return out
+
+    def stats(self, seed=1):
+        g = torch.Generator().manual_seed(seed)
+        shape = (self.G + self.C, self.KVH, self.BS)
+        return KeyStats(torch.rand(shape, generator=g).cuda(), torch.randint(0, 99, shape, generator=g, dtype=torch.int32).cuda())
+
+    def places(self, r, n=None):
+        """(blocks, offsets) of request r's keys."""
+        j = torch.arange(self.lens[r] if n is None else n)
+        return torch.tensor(self.rows[r], dtype=torch.int64)[j // self.BS], j % self.BS
+
+
+# ------------------------------------------------------------------ weights
+
+
+def _lse(q, keys, q_lens, scale):
+    """[H, T] fp32, of float64."""
+    H = q.shape[1]
+    out, at = torch.zeros(H, q.shape[0], device="cuda"), 0
+    for k, nq in zip(keys, q_lens):
+        nk, KVH = k.shape[0], k.shape[1]
+        kd = k.cuda().double().transpose(0, 1).repeat_interleave(H // KVH, 0)
+        s = q[at:at + nq].double().transpose(0, 1) @ kd.transpose(1, 2) * scale
+        seen = torch.arange(nk, device="cuda") <= (nk - nq + torch.arange(nq, device="cuda"))[:, None]
+        s = s.masked_fill(~seen, -math.inf)
+        out[:, at:at + nq] = (torch.logsumexp(s, -1) if nk else torch.full((H, nq), -math.inf, device="cuda")).float()
+        at += nq
+    return out
+
+
+def _weights_case(q_lens, k_lens, H, KVH, D, BS, dtype, host=0.0, layout="interleaved", seed=0, gap=0, hints=None, evicted=True):
+    pg = Paged(k_lens, KVH, BS, D, dtype, host, seed, layout)
+    T = sum(q_lens) + gap
+    g = torch.Generator().manual_seed(seed + 9)
+    q = torch.randn(T, H, D, generator=g).to(dtype).cuda()
+    q[sum(q_lens):] = NAN
+    scale = D ** -0.5
+    lse = _lse(q[:sum(q_lens)], pg.keys, q_lens, scale)
+    lse = torch.cat([lse, torch.full((H, gap), NAN, device="cuda")], 1)
+    start = [sum(q_lens[:i]) for i in range(len(q_lens))]
+    stats = pg.stats()
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    gone = [7 * r for r in range(len(q_lens))]
+    mq, mk = hints if hints is not None else (max(q_lens), max(k_lens))
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32(start), i32(q_lens), i32(k_lens), scale, lse, stats,
+                        evicted=i32(gone) if evicted else None, max_q_len=mq, max_k_len=mk)
+    ok()
+    _check_weights(pg, q, lse, q_lens, k_lens, start, scale, stats, w0, p0, gone if evicted else [0] * len(gone))
+    return pg, q, lse, start, scale, stats
+
+
+def _check_weights(pg, q, lse, q_lens, k_lens, start, scale, stats, w0, p0, gone):
+    want, tol, pos = w0.cpu().double(), torch.zeros(w0.shape, dtype=torch.float64), p0.cpu()
+    for r, (nq, nk) in enumerate(zip(q_lens, k_lens)):
+        if nq == 0 or nk == 0:
+            continue
+        blk, off = pg.places(r, nk)
+        old = w0.cpu()[blk, :, off].T
+        w, e = ref.key_weights(q[start[r]:start[r] + nq], pg.keys[r][:nk].cuda(), lse[:, start[r]:start[r] + nq], old.cuda(), scale)
+        want[blk, :, off], tol[blk, :, off] = w.T.cpu(), e.T.cpu()
+        first = max(0, nk - nq)
+        pos[blk[first:], :, off[first:]] = (torch.arange(first, nk) + gone[r]).int()[:, None].expand(-1, pg.KVH)
+    got = stats.weights.cpu().double()
+    assert torch.equal(got.isnan(), want.isnan())
+    err = torch.where(want.isnan(), 0.0, (got - want).abs())
+    assert bool((err <= torch.where(tol.isnan(), math.inf, tol)).all()), (float((err - tol).max()), float(err.max()))
+    assert torch.equal(stats.positions.cpu(), pos)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "tokens", "heads"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float32])
+def test_weights_ragged(dtype, layout):
+    _weights_case([1, 5, 0, 3, 2, 1], [1, 300, 40, 3, 129, 128], 8, 2, 64, 16, dtype, layout=layout, gap=3)
+
+
+@pytest.mark.parametrize("D,BS,H,KVH", [(64, 16, 4, 4), (128, 16, 32, 8), (80, 24, 20, 4), (96, 8, 6, 2), (128, 64, 8, 1), (16, 16, 4, 2),
+                                        (256, 16, 4, 2), (128, 1, 4, 2), (72, 5, 12, 4), (128, 128, 64, 1), (64, 32, 32, 1), (112, 48, 3, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_weights_shapes(dtype, D, BS, H, KVH):
+    _weights_case([1, 40, 7], [200, 77, 600], H, KVH, D, BS, dtype, seed=D + BS)
+    _weights_case([1, 1, 1], [513, 1, 128], H, KVH, D, BS, dtype, seed=D + BS + 1)
+
+
+@pytest.mark.parametrize("D,BS,H,KVH", [(64, 16, 8, 8), (128, 24, 8, 2), (256, 16, 2, 1), (4, 3, 4, 1)])
+def test_weights_fp32(D, BS, H, KVH):
+    _weights_case([1, 70, 7], [200, 77, 300], H, KVH, D, BS, torch.float32, seed=D)
+
+
+@pytest.mark.parametrize("q_lens,k_lens", [([1], [1]), ([1], [20000]), ([700], [700]), ([300, 2, 900], [5000, 2, 901]), ([64], [64]),
+                                           ([257, 31, 32, 33], [1000, 31, 64, 3000]), ([1] * 300, list(range(1, 301))),
+                                           ([9, 9], [5, 1]), ([1, 200], [0, 0]), ([2000], [4096])])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_lengths(dtype, q_lens, k_lens):
+    if dtype == torch.float32 and max(k_lens) > 6000:
+        k_lens = [min(k, 6000) for k in k_lens]
+    _weights_case(q_lens, k_lens, 8, 2, 128 if dtype == torch.bfloat16 else 64, 16, dtype, seed=len(q_lens))
+
+
+@pytest.mark.parametrize("hints", [(0, 0), (1, 1), (100000, 100000), (1, 0), (0, 1)])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+def test_weights_hints_change_only_the_time(dtype, hints):
+    _weights_case([3, 150, 1], [600, 150, 90], 8, 2, 64, 16, dtype, host=0.3, hints=hints)
+
+
+@pytest.mark.parametrize("host", [0.2, 1.0])
+@pytest.mark.parametrize("dtype,D,BS", [(torch.bfloat16, 128, 16), (torch.float16, 64, 24), (torch.float32, 64, 16)])
+def test_weights_of_host_blocks(dtype, D, BS, host):
+    _weights_case([1, 30, 5], [400, 333, 50], 8, 2, D, BS, dtype, host=host, evicted=False)
+
+
+@pytest.mark.parametrize("dtype,ql", [(torch.bfloat16, 3), (torch.bfloat16, 200), (torch.float32, 100)])
+def test_weights_of_rows_without_keys_and_nan(dtype, ql):
+    """lse = -inf or +inf gives nothing, a NaN spoils the keys that its row sees and no other."""
+    pg = Paged([400, 300], 2, 16, 64, dtype, seed=3)
+    T, H, scale = 2 * ql, 4, 0.125
+    q = torch.randn(T, H, 64, generator=torch.Generator().manual_seed(2)).to(dtype).cuda()
+    lse = _lse(q, pg.keys, [ql, ql], scale)
+    lse[0, 1], lse[1, 2], lse[2, ql] = -math.inf, math.inf, NAN
+    stats = pg.stats()
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([0, ql]), i32([ql, ql]), i32([400, 300]), scale, lse, stats,
+                        max_q_len=ql, max_k_len=400)
+    ok()
+    _check_weights(pg, q, lse, [ql, ql], [400, 300], [0, ql], scale, stats, w0, p0, [0, 0])
+    assert int(stats.weights.isnan().sum()) == 300 - ql + 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_weights_strides_and_table_rows(dtype):
+    """q out of a wider projection, lse [T, H] transposed, requests on other table rows."""
+    pg = Paged([200, 333, 90], 2, 16, 64, dtype, seed=5)
+    q_lens, rows, H = [4, 50], [2, 1], 4
+    g = torch.Generator().manual_seed(4)
+    q = torch.randn(54 + 6, 3 * H, 64, generator=g).to(dtype).cuda()[6:, H:2 * H]
+    keys = [pg.keys[r] for r in rows]
+    lse = _lse(q, keys, q_lens, 0.125).T.contiguous().T
+    assert lse.stride(0) == 1
+    stats = pg.stats()
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([0, 4]), i32(q_lens), i32([90, 333]), 0.125, lse, stats, bt_row=i32(rows),
+                        max_q_len=50, max_k_len=333)
+    ok()
+    pg.rows, pg.lens, pg.keys = [pg.rows[r] for r in rows], [90, 333], keys
+    _check_weights(pg, q, lse, q_lens, [90, 333], [0, 4], 0.125, stats, w0, p0, [0, 0])
+
+
+@pytest.mark.parametrize("dtype,ql", [(torch.float16, 2), (torch.float16, 90), (torch.float32, 2)])
+def test_weights_refuse_bad_requests_alone(dtype, ql):
+    def call(k_len, start, table_edit=None, nstat=None, bt_row=None):
+        pg = Paged([100, 200, 300], 2, 16, 64, dtype, seed=6)
+        q = torch.randn(3 * ql, 4, 64, generator=torch.Generator().manual_seed(1)).to(dtype).cuda()
+        lse = _lse(q, pg.keys, [ql] * 3, 0.125)
+        stats = pg.stats()
+        if nstat is not None:
+            stats = KeyStats(stats.weights[:nstat].clone(), stats.positions[:nstat].clone())
+        w0 = stats.weights.clone()
+        if table_edit is not None:
+            pg.table[table_edit[0], table_edit[1]] = table_edit[2]
+        gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32(start), i32([ql] * 3), i32(k_len), 0.125, lse, stats,
+                            bt_row=bt_row, max_q_len=ql, max_k_len=300)
+        return pg, stats, w0
+
+    for k_len, start, bt_row in (([100, 5000, 300], [0, ql, 2 * ql], None), ([100, 200, 300], [0, 2 * ql + 1, 2 * ql], None),
+                                 ([100, -1, 300], [0, ql, 2 * ql], None), ([100, 200, 300], [0, ql, 2 * ql], [0, 9, 2])):
+        pg, stats, w0 = call(k_len, start, bt_row=None if bt_row is None else i32(bt_row))
+        fails("sequence length")
+        for r, changed in ((0, True), (1, False), (2, True)):
+            blk, off = pg.places(r)
+            assert torch.equal(stats.weights.cpu()[blk, :, off], w0.cpu()[blk, :, off]) != changed
+    for bad in (-1, 1 << 20):
+        pg, stats, w0 = call([100, 200, 300], [0, ql, 2 * ql], (1, 3, bad))
+        fails("block id")
+        blk, off = pg.places(2)
+        assert not torch.equal(stats.weights.cpu()[blk, :, off], w0.cpu()[blk, :, off])
+    pg, stats, w0 = call([100, 200, 300], [0, ql, 2 * ql], nstat=10)  # blocks behind the stats
+    fails("block id")
+
+
+def test_weights_of_chunks_add_up_to_the_prompt_s():
+    """A prompt in chunks gives each key what the prompt as a whole gives it."""
+    n, cuts, H, KVH, D = 500, [200, 250, 251, 500], 8, 2, 128
+    pg = Paged([n], KVH, 16, D, torch.bfloat16, seed=8)
+    q = torch.randn(n, H, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    lse = _lse(q, pg.keys, [n], D ** -0.5)
+    a, b = pg.stats(2), pg.stats(3)
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([0]), i32([n]), i32([n]), D ** -0.5, lse, a)
+    at = 0
+    for c in cuts:
+        gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([at]), i32([c - at]), i32([c]), D ** -0.5, lse, b)
+        at = c
+    ok()
+    blk, off = pg.places(0)
+    wa, wb = a.weights.cpu()[blk, :, off], b.weights.cpu()[blk, :, off]
+    # the same terms, summed in another order: n G roundings each
+    assert bool(((wa - wb).abs() <= 2 * (n * 4 + 64) * 2.0 ** -24 * wa).all())
+    # every query spreads a weight of 1 per head: off by its exponents' errors, 2^-12 at |s| below 2^6
+    assert abs(float(wa.double().sum()) / (n * H) - 1) <= 2.0 ** -12
+    assert torch.equal(a.positions.cpu()[blk, :, off], b.positions.cpu()[blk, :, off])
+
+
+# ------------------------------------------------------------------ select
+
+
+def _select(lens, keep, KVH=2, BS=16, sinks=0, recent=0, gone=None, seed=0, room=None, hint=None, weights=None, gaps=True):
+    pg = Paged(lens, KVH, BS, 8, torch.float32, seed=seed)
+    stats = pg.stats()
+    g = torch.Generator().manual_seed(seed + 1)
+    gone = [3 * r for r in range(len(lens))] if gone is None else gone
+    w_l, p_l = [], []
+    for r, n in enumerate(lens):
+        w = torch.randn(KVH, n, generator=g).exp() if weights is None else weights(KVH, n, g)
+        p = torch.stack([torch.randperm(n + gone[r], generator=g)[:n].int() for _ in range(KVH)]) if n else torch.zeros(KVH, 0)
+        blk, off = pg.places(r)
+        stats.weights[blk.cuda(), :, off.cuda()] = w.T.cuda()
+        stats.positions[blk.cuda(), :, off.cuda()] = p.T.int().cuda()
+        w_l.append(w)
+        p_l.append(p)
+    room = max([1] + [min(b, n - b) for n, b in zip(lens, keep) if 0 <= b < n]) if room is None else room
+    m = KeyMoves(len(lens), KVH, room, dev())
+    m.src.fill_(-5)
+    m.dst.fill_(-6)
+    gpu_ops.select_keys(stats, pg.table, i32(lens), i32(keep), m, sinks=sinks, recent=recent, evicted=i32(gone),
+                        max_k_len=max(lens) if hint is None else hint)
+    return pg, stats, m, w_l, p_l, gone
+
+
+def _check_select(m, lens, keep, w_l, p_l, gone, sinks, recent, skip=()):
+    src, dst, counts = m.src.tolist(), m.dst.tolist(), m.counts.tolist()
+    for r, n in enumerate(lens):
+        for h in range(m.KVH):
+            a, b = ([], []) if r in skip else ref.select(w_l[r][h].tolist(), p_l[r][h].tolist(), n, keep[r], gone[r], sinks, recent)
+            assert counts[r][h] == len(a) == len(b), (r, h)
+            assert src[r][h] == a + [-5] * (m.room - len(a)) and dst[r][h] == b + [-6] * (m.room - len(b)), (r, h)
+
+
+@pytest.mark.parametrize("sinks,recent", [(0, 0), (4, 0), (0, 40), (4, 16), (1000, 0), (0, 100000)])
+def test_select_ragged(sinks, recent):
+    lens = [1, 2, 50, 200, 0, 333, 1000, 64]
+    keep = [0, 1, 20, 200, 0, 332, 100, -1]
+    _, _, m, w, p, gone = _select(lens, keep, sinks=sinks, recent=recent)
+    ok()
+    _check_select(m, lens, keep, w, p, gone, sinks, recent)
+
+
+@pytest.mark.parametrize("BS,KVH", [(1, 1), (5, 3), (64, 8), (24, 2)])
+def test_select_blocks_and_heads(BS, KVH):
+    lens, keep = [77, 500, 129], [33, 499, 64]
+    _, _, m, w, p, gone = _select(lens, keep, KVH, BS, 2, 10, seed=BS)
+    ok()
+    _check_select(m, lens, keep, w, p, gone, 2, 10)
+
+
+def _ties(KVH, n, g):
+    return torch.randint(0, 3, (KVH, n), generator=g).float() * torch.where(torch.rand(KVH, n, generator=g) < 0.5, -1.0, 1.0)
+
+
+def _odd(KVH, n, g):
+    v = torch.tensor([NAN, math.inf, -math.inf, 0.0, -0.0, 1e-42, -1e-42, 3e38, 1.0, -NAN])
+    return v[torch.randint(0, len(v), (KVH, n), generator=g)]
+
+
+@pytest.mark.parametrize("weights", [_ties, _odd, lambda K, n, g: torch.zeros(K, n), lambda K, n, g: torch.full((K, n), NAN)])
+def test_select_ties_go_to_the_lowest_index(weights):
+    lens, keep = [300, 1025, 40], [100, 512, 39]
+    _, _, m, w, p, gone = _select(lens, keep, 2, 16, 3, 9, seed=4, weights=weights)
+    ok()
+    _check_select(m, lens, keep, w, p, gone, 3, 9)
+
+
+@pytest.mark.parametrize("n,keep,KVH,hint", [(20000, 2048, 2, None), (70000, 30000, 1, None), (70000, 69000, 1, 100), (100000, 5, 1, 0),
+                                             (9000, 8999, 3, 1 << 30)])
+def test_select_long(n, keep, KVH, hint):
+    """Several CTAs, keys beyond a CTA's shared memory (a hint that is too small), exact order against a stable sort."""
+    _, stats, m, w, p, gone = _select([n, 5], [keep, 5], KVH, 16, 4, keep // 3, seed=n, hint=hint)
+    ok()
+    for h in range(KVH):
+        guard = (p[0][h] < 4) | (p[0][h] >= n + gone[0] - keep // 3)
+        score = torch.where(guard, math.inf, w[0][h].double())
+        order = torch.sort(score, descending=True, stable=True)[1]
+        stays = torch.zeros(n, dtype=torch.bool)
+        stays[order[:keep]] = True
+        a, b = stays[keep:].nonzero().flatten() + keep, (~stays[:keep]).nonzero().flatten()
+        c = int(m.counts[0, h])
+        assert c == len(a) and m.src[0, h, :c].tolist() == a.tolist() and m.dst[0, h, :c].tolist() == b.tolist()
+        assert int(m.counts[1, h]) == 0
+
+
+def test_select_refuses_bad_requests_alone():
+    lens, keep = [100, 90, 80], [50, 45, 40]
+    _, _, m, w, p, gone = _select(lens, keep, room=45)
+    fails("sequence length")
+    _check_select(m, lens, keep, w, p, gone, 0, 0, skip=(0,))
+    for n in (-1, 10000):
+        pg, stats, m, w, p, gone = _select(lens, keep)
+        ok()
+        m.src.fill_(-5), m.dst.fill_(-6)
+        gpu_ops.select_keys(stats, pg.table, i32([100, n, 80]), i32(keep), m, evicted=i32(gone), max_k_len=100)
+        fails("sequence length")
+        _check_select(m, lens, keep, w, p, gone, 0, 0, skip=(1,))
+    for bad in (-1, 1 << 20):
+        pg, stats, m, w, p, gone = _select(lens, keep)
+        ok()
+        m.src.fill_(-5), m.dst.fill_(-6)
+        pg.table[1, 4] = bad
+        gpu_ops.select_keys(stats, pg.table, i32(lens), i32(keep), m, evicted=i32(gone), max_k_len=100)
+        fails("block id")
+        _check_select(m, lens, keep, w, p, gone, 0, 0, skip=(1,))
+
+
+def test_select_refuses_a_bad_block_in_a_cluster():
+    pg, stats, m, w, p, gone = _select([40000], [1000], KVH=1, seed=2)
+    ok()
+    m.src.fill_(-5)
+    pg.table[0, 2400] = -1
+    gpu_ops.select_keys(stats, pg.table, i32([40000]), i32([1000]), m, evicted=i32(gone), max_k_len=40000)
+    fails("block id")
+    assert m.counts.tolist() == [[0]] and bool((m.src == -5).all())
+
+
+# ------------------------------------------------------------------ move
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "tokens", "heads"])
+@pytest.mark.parametrize("dtype,D,BS,host", [(torch.bfloat16, 128, 16, 0.0), (torch.float16, 64, 24, 0.4), (torch.float32, 4, 5, 0.5),
+                                             (torch.bfloat16, 8, 16, 1.0), (torch.float32, 256, 64, 0.0)])
+def test_move_selected_keys(dtype, D, BS, host, layout):
+    """After select and move the first keys of every request are those that stay, with their weights and positions."""
+    lens, keep, KVH = [500, 33, 70, 1, 200], [200, 20, 69, 1, 0], 3
+    pg = Paged(lens, KVH, BS, D, dtype, host, seed=D, layout=layout)
+    stats = pg.stats()
+    w0, p0 = stats.weights.cpu(), stats.positions.cpu()
+    k0, v0 = pg.now()
+    m = gpu_ops.select_keys(stats, pg.table, i32(lens), i32(keep), KeyMoves(5, KVH, 200, dev()), recent=5)
+    gpu_ops.move_keys(m, pg.tiers, pg.G, pg.table, stats)
+    ok()
+    k1, v1 = pg.now()
+    w1, p1 = stats.weights.cpu(), stats.positions.cpu()
+    for r, n in enumerate(lens):
+        blk, off = pg.places(r)
+        for h in range(KVH):
+            c = int(m.counts[r, h])
+            a, b = m.src[r, h, :c].cpu().long(), m.dst[r, h, :c].cpu().long()
+            at = torch.arange(n)
+            at[b] = a
+            for x0, x1 in ((k0, k1), (v0, v1), (w0, w1), (p0, p1)):
+                want = x0[blk, h, off][at]
+                assert torch.equal(x1[blk, h, off], want), (r, h)
+                x0[blk, h, off] = want
+    for x0, x1 in ((k0, k1), (v0, v1), (w0, w1), (p0, p1)):  # nothing else changed
+        assert torch.equal(x0.nan_to_num(123.0) if x0.is_floating_point() else x0, x1.nan_to_num(123.0) if x1.is_floating_point() else x1)
+
+
+def test_move_without_stats_and_many_small_units():
+    lens = [40] * 300
+    pg = Paged(lens, 1, 16, 64, torch.bfloat16, seed=1)
+    k0, v0 = pg.now()
+    src = torch.arange(20, 30, dtype=torch.int32).repeat(300, 1, 1).cuda()
+    dst = torch.arange(0, 20, 2, dtype=torch.int32).repeat(300, 1, 1).cuda()
+    gpu_ops.move_keys(KeyMoves(300, 1, 10, dev(), src=src, dst=dst, counts=i32([[10]] * 300)), pg.tiers, pg.G, pg.table)
+    ok()
+    k1, v1 = pg.now()
+    for r in range(300):
+        blk, off = pg.places(r)
+        at = torch.arange(40)
+        at[0:20:2] = torch.arange(20, 30)
+        assert torch.equal(k1[blk, 0, off], k0[blk, 0, off][at]) and torch.equal(v1[blk, 0, off], v0[blk, 0, off][at])
+
+
+def test_move_passes_over_bad_pairs():
+    pg = Paged([60, 60], 1, 16, 64, torch.float16, seed=2)
+    k0, v0 = pg.now()
+    W = pg.table.shape[1] * 16
+    m = KeyMoves(2, 1, 4, dev(), src=i32([[[30, W, -1, 33]], [[30, 31, 32, 33]]]), dst=i32([[[0, 1, 2, 3]], [[0, 1, 2, 3]]]),
+                 counts=i32([[4], [5]]))
+    gpu_ops.move_keys(m, pg.tiers, pg.G, pg.table)
+    fails("sequence length")
+    k1, _ = pg.now()
+    blk, off = pg.places(0)
+    at = torch.arange(60)
+    at[0], at[3] = 30, 33
+    assert torch.equal(k1[blk, 0, off], k0[blk, 0, off][at])
+    blk, off = pg.places(1)  # a count beyond the room: nothing
+    assert torch.equal(k1[blk, 0, off], k0[blk, 0, off])
+    m.counts.copy_(i32([[0], [4]]))
+    pg.table[1, 0] = 1 << 20
+    gpu_ops.move_keys(m, pg.tiers, pg.G, pg.table)
+    fails("block id")
+    assert torch.equal(pg.now()[0][blk, 0, off], k0[blk, 0, off])
+
+
+# ------------------------------------------------------------------ trim
+
+
+def _trim(lens, keep, block, share, seed=0, slack=4, cap=None):
+    rnd = random.Random(seed)
+    held = [-(-max(0, n) // block) for n in lens]
+    total = sum(held) + slack
+    hbm = max(1, int(total * share))
+    ids = list(range(total))
+    rnd.shuffle(ids)
+    W = max(held + [1]) + 1
+    table, at = [], 0
+    for h in held:
+        table.append(ids[at:at + h] + [-3] * (W - h))
+        at += h
+    s0, s1 = [b for b in ids[at:] if b < hbm], [b for b in ids[at:] if b >= hbm]
+    cap = total if cap is None else cap
+    return table, [s0 + [-1] * (cap - len(s0)), s1 + [-1] * (cap - len(s1))], [len(s0), len(s1)], hbm, total - hbm
+
+
+@pytest.mark.parametrize("in_place", [False, True])
+@pytest.mark.parametrize("hint", [0, 1])
+@pytest.mark.parametrize("R,block,hi,cut,share", [(1, 16, 5, 9, 1.0), (3, 1, 40, 50, 0.5), (40, 24, 500, 300, 0.3), (256, 16, 900, 7, 0.7),
+                                                  (1000, 16, 700, 700, 0.5), (8192, 8, 60, 60, 0.5), (4, 16, 200000, 200000, 0.6),
+                                                  (1025, 64, 100, 100, 0.0), (600, 1, 300, 300, 0.5)])
+def test_trim_matches_lists(R, block, hi, cut, share, hint, in_place):
+    rnd = random.Random(R + block)
+    lens = [rnd.randint(0, hi) for _ in range(R)]
+    keep = [rnd.choice([-1, n + rnd.randint(0, 5), max(0, n - rnd.randint(0, cut))]) for n in lens]
+    table, stacks, counts, hbm, host = _trim(lens, keep, block, share, R)
+    w_stacks, w_counts, left = ref.trim(keep, lens, table, stacks, counts, hbm, block)
+    tt, st, ct, ln, gone = i32(table), i32(stacks), i32(counts), i32(lens), i32([5] * R)
+    out = TrimTables(R, dev(), seq_lens=ln if in_place else None, counts=ct if in_place else None)
+    gpu_ops.trim_tables(i32(keep), ln, tt, FreeBlocks(st[0], st[1], ct), hbm, host, block, out, evicted=gone, max_cut=hint)
+    ok()
+    h = out.read_header()
+    assert out.seq_lens.tolist() == left and out.counts.tolist() == w_counts
+    assert st.tolist() == w_stacks and tt.tolist() == table
+    assert gone.tolist() == [5 + n - b for n, b in zip(lens, left)]
+    assert (h["freed_hbm"], h["freed_host"], h["max_seq"]) == (w_counts[0] - counts[0], w_counts[1] - counts[1], max(left))
+    assert h["n_tok"] == h["taken_hbm"] == h["taken_host"] == h["max_new"] == 0
+
+
+@pytest.mark.parametrize("R", [3, 900])
+@pytest.mark.parametrize("why,flag", [("len", "bad length"), ("long", "bad length"), ("block", "bad block id"), ("count", "bad free stack"),
+                                      ("room", "bad free stack")])
+def test_refused_trims_change_nothing(R, why, flag):
+    lens, keep = [50] * R, [20] * R
+    table, stacks, counts, hbm, host = _trim(lens, keep, 16, 0.5, 1)
+    if why == "room":
+        stacks = [s[:c + 1] for s, c in zip(stacks, counts)]
+        stacks = [s + [0] * (max(map(len, stacks)) - len(s)) for s in stacks]
+    if why == "block":
+        table[R - 1][3] = hbm + host
+    if why == "count":
+        counts[1] = -1
+    if why == "len":
+        lens[R // 2] = -1
+    if why == "long":
+        lens[R // 2] = 5 * 16 + 1
+    tt, st, ct, ln, gone = i32(table), i32(stacks), i32(counts), i32(lens), i32([5] * R)
+    out = TrimTables(R, dev())
+    gpu_ops.trim_tables(i32(keep), ln, tt, FreeBlocks(st[0], st[1], ct), hbm, host, 16, out, evicted=gone)
+    fails("block tables")
+    with pytest.raises(RuntimeError, match="trim_tables refused the step: " + flag):
+        out.read_header()
+    assert out.seq_lens.tolist() == lens and out.counts.tolist() == counts and st.tolist() == stacks
+    assert tt.tolist() == table and gone.tolist() == [5] * R
+
+
+def test_trim_of_no_requests():
+    e = torch.zeros(0, dtype=torch.int32, device="cuda")
+    out = gpu_ops.trim_tables(e, e, torch.zeros(0, 3, dtype=torch.int32, device="cuda"), FreeBlocks(e, None, i32([0, 0])), 4, 0, 16)
+    ok()
+    assert out.read_header()["freed_hbm"] == 0 and out.counts.tolist() == [0, 0]
+
+
+def test_extend_tables_positions_run_ahead_of_evicted_tokens():
+    """Positions are index plus evicted, for each way of placing tokens; an ended request's count becomes 0."""
+    for new in ([1, 3, -1, 0, 4], [1, 9, -1, 0, 40], [1, 5000, -1, 0, 4000]):
+        prior, gone = [5, 16, 20, 7, 0], [100, 0, 9, 3, 50]
+        need = [0 if n < 0 else -(-(p + n) // 16) for p, n in zip(prior, new)]
+        W, at, table = max(need) + 2, 0, []
+        for p in prior:
+            h = -(-p // 16)
+            table.append(list(range(at, at + h)) + [0] * (W - h))
+            at += h
+        free = list(range(at, at + sum(need)))
+        tt, g = i32(table), i32(gone)
+        t = StepTables(5, sum(max(0, n) for n in new) + 3, dev())
+        plain = StepTables(5, t.T, dev())
+        stack = i32(free)
+        for out, ev, tab in ((plain, None, tt.clone()), (t, g, tt)):
+            pool = FreeBlocks(torch.cat([stack, i32([-1] * 9)]), None, i32([len(free), 0]))
+            gpu_ops.extend_tables(i32(new), i32(prior), tab, pool, 10 ** 6, 0, 16, out, evicted=ev)
+        ok()
+        assert torch.equal(t.slot_mapping, plain.slot_mapping)
+        want = [p + gone[r] + i for r, (p, n) in enumerate(zip(prior, new)) for i in range(max(0, n))]
+        assert t.positions.tolist() == want + [0] * 3
+        assert g.tolist() == [100, 0, 0, 3, 50]
+
+
+# ------------------------------------------------------------------ verify
+
+
+def _probs(g, *shape, dtype=torch.float32, spread=2.0):
+    return (torch.randn(*shape, generator=g) * spread).softmax(-1).to(dtype)
+
+
+def _verify(target, tokens, draft, start, q_len, au, su, seq=None, out=None):
+    v = gpu_ops.verify_drafts(target.cuda(), tokens.cuda(), None if draft is None else draft.cuda(), i32(start), i32(q_len), au.cuda(),
+                              su.cuda(), seq_lens=None if seq is None else i32(seq), out=out)
+    return v
+
+
+def _check_verify(v, target, tokens, draft, start, q_len, au, su, seq=None):
+    K = tokens.shape[1]
+    t64 = target.double().tolist()
+    for r in range(len(q_len)):
+        got, a = ref.verify(t64, tokens[r].tolist(), None if draft is None else draft[r].double().tolist(), start[r], q_len[r],
+                            au[r].double().tolist(), float(su[r]))
+        assert v.tokens[r].tolist() == got + [-1] * (K + 1 - len(got)), r
+        assert int(v.accepted[r]) == a
+        if seq is not None:
+            assert int(v.keep_lens[r]) == seq[r] - (max(0, q_len[r] - 1) - a)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("V,K,R", [(1, 1, 2), (2, 3, 5), (100, 4, 9), (1003, 3, 6), (5000, 2, 4), (33001, 1, 3), (32768, 2, 2)])
+@pytest.mark.parametrize("with_draft", [True, False])
+def test_verify(V, K, R, dtype, with_draft):
+    g = torch.Generator().manual_seed(V + K)
+    q_len = [min(K + 1, max(0, r % (K + 2))) for r in range(R - 1)] + [K + 1]
+    start = [sum(q_len[:r]) for r in range(R)]
+    target = _probs(g, sum(q_len), V, dtype=dtype)
+    draft = _probs(g, R, K, V, dtype=dtype)
+    for r in range(R):  # drafts near the target, so that some are accepted
+        for d in range(max(0, q_len[r] - 1)):
+            draft[r, d] = (0.7 * target[start[r] + d].float() + 0.3 * draft[r, d].float()).to(dtype)
+    tokens = torch.stack([torch.multinomial(draft[r].float(), 1, generator=g).flatten() for r in range(R)])
+    au, su = torch.rand(R, K, generator=g), torch.rand(R, generator=g)
+    seq = [50 + r for r in range(R)]
+    v = _verify(target, tokens, draft if with_draft else None, start, q_len, au, su, seq)
+    ok()
+    _check_verify(v, target, tokens, draft if with_draft else None, start, q_len, au, su, seq)
+
+
+def test_verify_more_drafts_than_a_warp_and_no_drafts():
+    g = torch.Generator().manual_seed(3)
+    for K, q_len in ((70, [71, 40, 33, 32, 1, 0]), (0, [1, 1, 0, 1])):
+        R, V = len(q_len), 64
+        start = [sum(q_len[:r]) for r in range(R)]
+        target, draft = _probs(g, sum(q_len), V, spread=0.1), _probs(g, R, K, V, spread=0.1)
+        tokens = torch.randint(0, V, (R, K), generator=g)
+        au, su = torch.rand(R, K, generator=g) * 0.9, torch.rand(R, generator=g)
+        if K:
+            au[0], au[1, 36] = 0.0, 0.999999
+        v = _verify(target, tokens, draft, start, q_len, au, su)
+        ok()
+        _check_verify(v, target, tokens, draft, start, q_len, au, su)
+        if K:
+            assert int(v.accepted[0]) == 70
+
+
+def test_verify_greedy_rows_and_extreme_numbers():
+    """One-hot rows accept their token alone and are drawn for any number; numbers of 0, almost 1, 1, NaN."""
+    V = 5000
+    hot = torch.zeros(3, V)
+    hot[0, 4999] = hot[1, 17] = hot[2, 0] = 1.0
+    tokens = torch.tensor([[4999, 17], [4999, 3], [5, 17]])
+    for u in (0.0, 1.0 - 2.0 ** -24, 1.0, NAN, -1.0):
+        target = hot.repeat(3, 1)
+        au, su = torch.full((3, 2), min(max(u, 0.0), 1 - 2 ** -24) if u == u else 0.0), torch.full((3,), u)
+        v = _verify(target, tokens, None, [0, 3, 6], [3] * 3, au, su)
+        ok()
+        assert v.tokens.tolist() == [[4999, 17, 0], [4999, 17, -1], [4999, -1, -1]]
+    g = torch.Generator().manual_seed(1)
+    target = _probs(g, 4, 777)
+    target[:, 700:] = 0.0
+    target[:, :30] = 0.0
+    for u in (0.0, 1.0 - 2.0 ** -24, 1.0, NAN):
+        su = torch.full((4,), u)
+        e = torch.zeros(4, 0)
+        v = _verify(target, e.long(), None, [0, 1, 2, 3], [1] * 4, e, su)
+        ok()
+        _check_verify(v, target, e.long(), None, [0, 1, 2, 3], [1] * 4, e, su)
+        assert v.tokens.flatten().tolist() == [30 if u != u or u == 0.0 else 699] * 4
+
+
+def test_verify_odd_probabilities():
+    """Negative, infinite and NaN values count as 0; a residual of nothing falls back to the target's row; a row of nothing gives -1."""
+    g = torch.Generator().manual_seed(2)
+    V = 300
+    target, draft = _probs(g, 6, V), _probs(g, 3, 1, V)
+    target[0, 5], target[1, 7], draft[0, 0, 9], draft[0, 0, 11] = NAN, math.inf, -3.0, NAN
+    draft[1, 0] = target[2]          # p = q: nothing left where the draft is rejected all the same
+    target[4] = 0.0                  # the third request's rejected draft: no probability at all
+    tokens = torch.tensor([[5], [3], [8]])
+    au, su = torch.tensor([[0.5], [1.0], [0.5]]), torch.tensor([0.3, 0.6, 0.2])
+    v = _verify(target, tokens, draft, [0, 2, 4], [2, 2, 2], au, su)
+    fails("without any positive")
+    _check_verify(v, target, tokens, draft, [0, 2, 4], [2, 2, 2], au, su)
+    assert v.tokens[2].tolist() == [-1, -1] and v.accepted.tolist() == [0, 0, 0]
+
+
+def test_verify_refuses_bad_requests_alone():
+    g = torch.Generator().manual_seed(5)
+    target, draft = _probs(g, 9, 50), _probs(g, 3, 2, 50)
+    tokens, au, su = torch.randint(0, 50, (3, 2), generator=g), torch.rand(3, 2, generator=g), torch.rand(3, generator=g)
+    for start, q_len in (([0, 3, 6], [3, 4, 3]), ([0, 7, 6], [3, 3, 3]), ([0, -1, 6], [3, 3, 3]), ([0, 3, 6], [3, -1, 3])):
+        v = _verify(target, tokens, draft, start, q_len, au, su, [20, 30, 40])
+        fails("sequence length")
+        assert v.tokens[1].tolist() == [-1] * 3 and int(v.accepted[1]) == 0 and int(v.keep_lens[1]) == 30
+        for r in (0, 2):
+            assert v.tokens[r].tolist()[0] >= 0
+    for bad in (-1, 50, 1 << 40):
+        t = tokens.clone()
+        t[1, 0] = bad
+        v = _verify(target, t, draft, [0, 3, 6], [3] * 3, au, su)
+        fails("outside the vocabulary")
+        assert int(v.accepted[1]) == 0
+        _check_verify(v, target, t, draft, [0, 3, 6], [3] * 3, au, su)
+
+
+def test_verify_strides():
+    """Rows of a padded vocabulary, drafts stacked step by step, numbers out of wider tables."""
+    g = torch.Generator().manual_seed(6)
+    R, K, V = 5, 3, 999
+    wide = torch.full((R * 4, 1024), 9.0)
+    wide[:, :V] = _probs(g, R * 4, V)
+    steps = _probs(g, K, R, V)
+    toks = torch.randint(0, V, (R, 8), generator=g)
+    au = torch.rand(R, 7, generator=g)
+    start, q_len, su = [4 * r for r in range(R)], [4] * R, torch.rand(R, generator=g)
+    wc, sc = wide.cuda(), steps.cuda()
+    v = gpu_ops.verify_drafts(wc[:, :V], toks.cuda()[:, 2:5], sc.transpose(0, 1), i32(start), i32(q_len), au.cuda()[:, 1:4], su.cuda())
+    ok()
+    _check_verify(v, wide[:, :V], toks[:, 2:5], steps.transpose(0, 1), start, q_len, au[:, 1:4], su)
+
+
+def test_verify_draws_by_the_probabilities():
+    """The accepted and drawn first tokens of many requests follow the target, whatever the draft: 40000 draws over 8 tokens,
+    each count within 5 standard deviations."""
+    g = torch.Generator().manual_seed(7)
+    R, V = 40000, 8
+    p, q = _probs(g, V, spread=1.0), _probs(g, V, spread=1.0)
+    tokens = torch.multinomial(q, R, replacement=True, generator=g).view(R, 1)
+    v = _verify(p.expand(2 * R, V).contiguous(), tokens, q.expand(R, 1, V).contiguous(), [2 * r for r in range(R)], [2] * R,
+                torch.rand(R, 1, generator=g), torch.rand(R, generator=g))
+    ok()
+    got = torch.bincount(v.tokens[:, 0].cpu(), minlength=V).double()
+    assert bool(((got - R * p.double()).abs() <= 5 * (R * p * (1 - p)).double().sqrt()).all())

@@ -120,7 +120,31 @@ class FdTablesArgs(ctypes.Structure):
         ("counts_in", c_void_p), ("counts_out", c_void_p), ("num_gpu_blocks", c_int64), ("num_cpu_blocks", c_int64),
         ("block_size", c_int32), ("max_tokens", c_int32), ("seq_lens", c_void_p), ("query_start_loc", c_void_p),
         ("slot_mapping", c_void_p), ("positions", c_void_p), ("header", c_void_p), ("error", c_void_p),
-        ("query_lens", c_void_p),
+        ("query_lens", c_void_p), ("evicted", c_void_p),
+    ]
+
+
+class FdTrimArgs(ctypes.Structure):
+    _fields_ = [
+        ("keep_lens", c_void_p), ("lens_in", c_void_p), ("lens_out", c_void_p), ("evicted", c_void_p),
+        ("block_table", c_void_p), ("bt_stride", c_int64), ("bt_width", c_int32), ("num_reqs", c_int32),
+        ("free_ids", c_void_p * 2), ("free_cap", c_int32 * 2), ("counts_in", c_void_p), ("counts_out", c_void_p),
+        ("num_gpu_blocks", c_int64), ("num_cpu_blocks", c_int64), ("block_size", c_int32), ("max_cut", c_int32),
+        ("header", c_void_p), ("error", c_void_p),
+    ]
+
+
+VERIFY_MAX_DRAFTS = 1024  # FD_VERIFY_MAX_DRAFTS
+
+
+class FdVerifyArgs(ctypes.Structure):
+    _fields_ = [
+        ("target", c_void_p), ("target_stride", c_int64), ("draft_probs", c_void_p), ("draft_stride_r", c_int64),
+        ("draft_stride_k", c_int64), ("draft_tokens", c_void_p), ("tokens_stride", c_int64), ("q_start", c_void_p),
+        ("q_len", c_void_p), ("accept_u", c_void_p), ("accept_stride", c_int64), ("sample_u", c_void_p),
+        ("lens", c_void_p), ("tokens", c_void_p), ("accepted", c_void_p), ("keep_lens", c_void_p),
+        ("num_reqs", c_int32), ("num_drafts", c_int32), ("vocab", c_int32), ("num_rows", c_int32), ("dtype", c_int32),
+        ("_pad0", c_int32), ("error", c_void_p),
     ]
 
 
@@ -150,6 +174,32 @@ class FdAttnArgs(ctypes.Structure):
         ("num_kv_heads", c_int32), ("head_size", c_int32), ("block_size", c_int32), ("scale", c_float),
         ("dtype", c_int32), ("max_q_len", c_int32), ("max_k_len", c_int32), ("bt_rows", c_int32),
         ("workspace", c_void_p), ("workspace_bytes", c_size_t), ("error", c_void_p),
+    ]
+
+
+class FdKeyStats(ctypes.Structure):
+    _fields_ = [("weights", c_void_p), ("positions", c_void_p), ("num_blocks", c_int64)]
+
+
+class FdKeyWeightsArgs(ctypes.Structure):
+    _fields_ = [("attn", FdAttnArgs), ("stats", FdKeyStats), ("evicted", c_void_p)]
+
+
+class FdSelectArgs(ctypes.Structure):
+    _fields_ = [
+        ("stats", FdKeyStats), ("block_table", c_void_p), ("bt_stride", c_int64), ("lens", c_void_p),
+        ("keep_lens", c_void_p), ("evicted", c_void_p), ("src", c_void_p), ("dst", c_void_p), ("counts", c_void_p),
+        ("bt_width", c_int32), ("num_reqs", c_int32), ("num_kv_heads", c_int32), ("block_size", c_int32),
+        ("room", c_int32), ("sinks", c_int32), ("recent", c_int32), ("max_len", c_int32), ("error", c_void_p),
+    ]
+
+
+class FdMoveArgs(ctypes.Structure):
+    _fields_ = [
+        ("src", c_void_p), ("dst", c_void_p), ("counts", c_void_p), ("tier", FdKvTier * 2), ("tier_split", c_int64),
+        ("block_table", c_void_p), ("bt_stride", c_int64), ("stats", FdKeyStats), ("bt_width", c_int32),
+        ("num_reqs", c_int32), ("num_kv_heads", c_int32), ("head_size", c_int32), ("block_size", c_int32),
+        ("room", c_int32), ("dtype", c_int32), ("_pad0", c_int32), ("error", c_void_p),
     ]
 
 
@@ -210,6 +260,17 @@ SIGNATURES = {
     "fd_chunk_attn": (c_int32, [c_void_p, c_void_p]),
     "fd_cross_attn": (c_int32, [c_void_p, c_void_p]),
     "fd_attn_args_bytes": (c_size_t, []),
+    "fd_trim_tables": (c_int32, [c_void_p, c_void_p]),
+    "fd_trim_args_bytes": (c_size_t, []),
+    "fd_verify_drafts": (c_int32, [c_void_p, c_void_p]),
+    "fd_verify_args_bytes": (c_size_t, []),
+    "fd_key_weights": (c_int32, [c_void_p, c_void_p]),
+    "fd_key_weights_workspace_size": (c_size_t, [c_void_p]),
+    "fd_key_weights_args_bytes": (c_size_t, []),
+    "fd_select_keys": (c_int32, [c_void_p, c_void_p]),
+    "fd_select_args_bytes": (c_size_t, []),
+    "fd_move_keys": (c_int32, [c_void_p, c_void_p]),
+    "fd_move_args_bytes": (c_size_t, []),
     "fd_version": (c_int32, []),
     "fd_abi_sizes": (c_int32, [POINTER(c_size_t), POINTER(c_size_t)]),
 }

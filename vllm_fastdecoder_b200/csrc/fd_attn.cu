@@ -418,13 +418,14 @@ int combine_launch(const AttnParams& p, int dtype, int rows, cudaStream_t s) {
 // GB/s bounds it.)  CTA (j, r) copies block j of request
 // r, when it lies in the host tier, to block r * stage_w + j of the copies.
 constexpr int kStageThreads = 256, kStageBatch = 8;
-__global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __grid_constant__ AttnParams p, int vec) {
+__global__ void __launch_bounds__(kStageThreads) fd_attn_stage_kernel(const __grid_constant__ AttnParams p, int vec,
+                                                                       int halves) {
   const int j = blockIdx.x, r = blockIdx.y;
   const Req q = load_req(p, r);
   if (q.qlen <= 0 || j * (long long)p.BS >= q.klen) return;
   const int64_t id = p.bt[(int64_t)q.kbase * p.bt_stride + j];
   if (id < p.split || id - p.split >= p.nblk[1]) return;
-  const int rows = p.KVH * p.BS, total = 2 * rows * vec;  // K, then V
+  const int rows = p.KVH * p.BS, total = halves * rows * vec;  // K, then V
   const int64_t src = (id - p.split) * p.blk_sb[1], dst = ((int64_t)r * p.stage_w + j) * p.blk_sb[2];
   for (int x0 = threadIdx.x; x0 < total; x0 += kStageThreads * kStageBatch) {
     uint4 v[kStageBatch];
@@ -500,8 +501,11 @@ int core_launch(AttnParams& p, const fd_attn_args* a, cudaStream_t s) {
   return core_launch_dp<T, 256>(p, a, s);
 }
 
-// Shared checks and parameters; `what` names the entry point in messages.
-int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream) {
+}  // namespace
+
+int fill_params(const fd_attn_args* a, Kind kind, const char* what, AttnParams& p, bool* empty) {
+  const bool chunk = kind != kCross;
+  *empty = false;
   if (a == nullptr) return fdh::fail(FD_ERR_INVALID, "%s: null args", what);
   const int es = fdh::elem_size(a->dtype);
   if (es == 0) return fdh::fail(FD_ERR_UNSUPPORTED, "%s: unsupported dtype %d", what, a->dtype);
@@ -517,8 +521,12 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
     return fdh::fail(FD_ERR_ALIGN, "%s: head_size*elem_size must be a multiple of 16", what);
   if (!(a->scale > 0.f) || !(a->scale < 3.0e38f))
     return fdh::fail(FD_ERR_INVALID, "%s: scale must be positive and finite", what);
-  if (a->n == 0 || a->num_tokens == 0) return FD_OK;
-  if (a->q == nullptr || a->out == nullptr || a->q_start == nullptr || a->q_len == nullptr || a->k_len == nullptr)
+  if (a->n == 0 || a->num_tokens == 0) {
+    *empty = true;
+    return FD_OK;
+  }
+  if (kind == kWeights && a->lse == nullptr) return fdh::fail(FD_ERR_INVALID, "%s: lse is required", what);
+  if (a->q == nullptr || (kind != kWeights && a->out == nullptr) || a->q_start == nullptr || a->q_len == nullptr || a->k_len == nullptr)
     return fdh::fail(FD_ERR_INVALID, "%s: q, out, q_start, q_len and k_len are required", what);
   if (chunk && (a->block_table == nullptr || a->bt_width <= 0 || a->bt_stride < 0 || a->block_size <= 0))
     return fdh::fail(FD_ERR_INVALID, "%s: block_table, bt_width and block_size are required", what);
@@ -529,10 +537,10 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
     return fdh::fail(FD_ERR_INVALID, "%s: states and k_start are required", what);
   if (!chunk && a->tier[0].host_mapped)
     return fdh::fail(FD_ERR_UNSUPPORTED, "%s: states must be device memory", what);
-  if (!fdh::aligned16(a->q) || !fdh::aligned16(a->out) || (a->q_stride_t * es) % 16 != 0 ||
-      (a->q_stride_h * es) % 16 != 0 || (a->out_stride_t * es) % 16 != 0 || (a->out_stride_h * es) % 16 != 0)
+  if (!fdh::aligned16(a->q) || (a->q_stride_t * es) % 16 != 0 || (a->q_stride_h * es) % 16 != 0 ||
+      (kind != kWeights && (!fdh::aligned16(a->out) || (a->out_stride_t * es) % 16 != 0 || (a->out_stride_h * es) % 16 != 0)))
     return fdh::fail(FD_ERR_ALIGN, "%s: q / out pointers and strides must be 16-byte aligned", what);
-  AttnParams p{};
+  p = AttnParams{};
   for (int t = 0; t < (chunk ? 2 : 1); ++t) {
     const fd_kv_tier& tr = a->tier[t];
     p.nblk[t] = tr.num_blocks > 0 ? tr.num_blocks : 0;
@@ -577,23 +585,45 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   p.BS = chunk ? a->block_size : 1;
   p.sl2 = a->scale * kLog2e;
   p.err = a->error;
+  return FD_OK;
+}
+
+int stage_launch(AttnParams& p, const fd_attn_args* a, size_t base, bool k_only, cudaStream_t s) {
+  int64_t block_bytes = 0;
+  p.stage_w = stage_blocks(a, &block_bytes);
+  if (p.stage_w <= 0) return FD_OK;
+  const int64_t blocks = (int64_t)p.stage_w * p.n;
+  const unsigned char* at = static_cast<const unsigned char*>(a->workspace) + base;
+  const int es = fdh::elem_size(a->dtype);
+  p.k[2] = at;
+  p.v[2] = at + blocks * block_bytes;
+  p.tok_sb[2] = (int64_t)p.D * es;
+  p.head_sb[2] = p.tok_sb[2] * p.BS;
+  p.blk_sb[2] = block_bytes;
+  p.nblk[2] = blocks;
+  fd_attn_stage_kernel<<<dim3((unsigned)p.stage_w, (unsigned)p.n), kStageThreads, 0, s>>>(p, p.D * es / 16, k_only ? 1 : 2);
+  return fdh::cuda_status(cudaGetLastError(), "fd_attn_stage_kernel launch");
+}
+
+size_t stage_bytes(const fd_attn_args* a) {
+  int64_t block_bytes = 0;
+  const int w = stage_blocks(a, &block_bytes);
+  return (size_t)(2 * (int64_t)w * a->n * block_bytes);
+}
+
+namespace {
+
+int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream) {
+  AttnParams p;
+  bool empty = false;
+  int st = fill_params(a, chunk ? kChunk : kCross, what, p, &empty);
+  if (st != FD_OK || empty) return st;
   const size_t need = fd_attn_workspace_size(a);
   if (a->workspace == nullptr || a->workspace_bytes < need || !fdh::aligned16(a->workspace))
     return fdh::fail(FD_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  int64_t block_bytes = 0;
-  p.stage_w = chunk ? stage_blocks(a, &block_bytes) : 0;
-  if (p.stage_w > 0) {
-    const int64_t blocks = (int64_t)p.stage_w * p.n;
-    const unsigned char* at = static_cast<const unsigned char*>(a->workspace) + base_workspace(a);
-    p.k[2] = at;
-    p.v[2] = at + blocks * block_bytes;
-    p.tok_sb[2] = (int64_t)p.D * es;
-    p.head_sb[2] = p.tok_sb[2] * p.BS;
-    p.blk_sb[2] = block_bytes;
-    p.nblk[2] = blocks;
-    fd_attn_stage_kernel<<<dim3((unsigned)p.stage_w, (unsigned)p.n), kStageThreads, 0, s>>>(p, p.D * es / 16);
-    const int st = fdh::cuda_status(cudaGetLastError(), "fd_attn_stage_kernel launch");
+  if (chunk) {
+    st = stage_launch(p, a, base_workspace(a), false, s);
     if (st != FD_OK) return st;
   }
   if (mma_covers(a)) return mma_launch(p, a, s);
@@ -601,7 +631,7 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
   p.cuts = reinterpret_cast<Cut*>(ws);
   p.part_ml = reinterpret_cast<float*>(ws + kMaxCtas * sizeof(Cut));
   p.part_o = p.part_ml + 2 * (size_t)kMaxCtas * kRows * 2;
-  p.tq = kRows / G;
+  p.tq = kRows / p.G;
   switch (a->dtype) {
     case FD_DTYPE_F16:
       return core_launch<__half>(p, a, s);
@@ -618,9 +648,7 @@ int attn_impl(const fd_attn_args* a, bool chunk, const char* what, void* stream)
 
 extern "C" size_t fd_attn_workspace_size(const fd_attn_args* a) {
   if (a == nullptr || a->head_size <= 0 || a->head_size > 256) return 0;
-  int64_t block_bytes = 0;
-  const int w = fdk::at::stage_blocks(a, &block_bytes);
-  return fdk::at::base_workspace(a) + (size_t)(2 * (int64_t)w * a->n * block_bytes);
+  return fdk::at::base_workspace(a) + fdk::at::stage_bytes(a);
 }
 
 extern "C" int fd_chunk_attn(const fd_attn_args* a, void* stream) {

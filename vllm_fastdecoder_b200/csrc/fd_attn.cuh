@@ -372,6 +372,15 @@ __device__ __forceinline__ int locate(const AttnParams& p, int r, int j, int64_t
   return t;
 }
 
+// Shared checks and parameters of the entry points over fd_attn_args; `what`
+// names one in messages.  *empty: there is nothing to do.
+enum Kind { kChunk, kCross, kWeights };
+int fill_params(const fd_attn_args* a, Kind kind, const char* what, AttnParams& p, bool* empty);
+// Copies of host blocks (K, or K and V) `base` bytes into the workspace, where
+// they fit, and the bytes that they take.
+int stage_launch(AttnParams& p, const fd_attn_args* a, size_t base, bool k_only, cudaStream_t s);
+size_t stage_bytes(const fd_attn_args* a);
+
 // The kernels' entry points for the host code in fd_attn.cu.
 bool mma_covers(const fd_attn_args* a);
 size_t mma_workspace(const fd_attn_args* a);

@@ -75,6 +75,10 @@ extern "C" const char* fd_device_error_string(int32_t code) {
              "length or count is invalid";
     case FD_DEVERR_POSITION:
       return "rotary position outside the cos / sin table";
+    case FD_DEVERR_TOKEN:
+      return "drafted token outside the vocabulary";
+    case FD_DEVERR_PROBS:
+      return "target row without any positive finite probability";
     default:
       return "unknown device error";
   }
@@ -126,7 +130,7 @@ extern "C" int fd_host_unregister(void* host) {
   return fdh::cuda_status(cudaHostUnregister(host), "cudaHostUnregister");
 }
 
-extern "C" int fd_version(void) { return 103; }
+extern "C" int fd_version(void) { return 104; }
 
 extern "C" int fd_abi_sizes(size_t* decode_args_bytes, size_t* kv_tier_bytes) {
   if (decode_args_bytes != nullptr) *decode_args_bytes = sizeof(fd_decode_args);

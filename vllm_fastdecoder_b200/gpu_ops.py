@@ -21,7 +21,10 @@ merge_partials), and the operators of a step whose requests bring several new
 tokens: extend_tables (block tables, slots and positions from lengths),
 rope_store_kv (multi-axis rotary positions with the KV write), chunk_attn (the
 new tokens' attention over the cached context of either tier) and cross_attn
-(attention to an encoder's states).  Every call is asynchronous on the current CUDA stream.
+(attention to an encoder's states); and of what follows it: verify_drafts
+(drafted tokens against the target's probabilities), key_weights, select_keys
+and move_keys (a cache cut to the keys that get attention) and trim_tables
+(the blocks behind shorter requests given back).  Every call is asynchronous on the current CUDA stream.
 There is no CPU path: without the native library or a CUDA device these raise.
 """
 
@@ -713,7 +716,12 @@ def prefill_attn(q: torch.Tensor, out: torch.Tensor, q_start: torch.Tensor, q_le
 _TIER_FMT = "PPqqqqii"
 _ATTN_STRUCT = struct.Struct("@PqqPqqPqq" + 2 * _TIER_FMT + "qPqPPPPPiiiiiiifiiiiPNP")
 _ROPE_STRUCT = struct.Struct("@" + 5 * "Pqq" + "PqPqP" + 2 * _TIER_FMT + f"q9i{nat.ROPE_MAX_PAIRS}siP")
-_TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPPP")
+_TABLES_STRUCT = struct.Struct("@PPPqiiPPiiPPqqiiPPPPPPPP")
+_TRIM_STRUCT = struct.Struct("@PPPPPqiiPPiiPPqqiiPP")
+_VERIFY_STRUCT = struct.Struct("@PqPqqPqPPPqPPPPPiiiiiiP")
+_KEY_WEIGHTS_STRUCT = struct.Struct(_ATTN_STRUCT.format + "PPqP")
+_SELECT_STRUCT = struct.Struct("@PPqPqPPPPPPiiiiiiiiP")
+_MOVE_STRUCT = struct.Struct("@PPP" + 2 * _TIER_FMT + "qPqPPqiiiiiiiiP")
 _NO_TIER = (0, 0, 0, 0, 0, 0, 0, 0)
 
 
@@ -765,6 +773,16 @@ def _rows3(t: torch.Tensor, idx: int, dtype: torch.dtype, name: str) -> tuple:
     return t.data_ptr(), s0, s1
 
 
+def _block_table(t: torch.Tensor) -> tuple[int, int, int]:
+    """(device index, R, W) of a block table int32 [R, W]."""
+    idx = t.get_device()
+    if idx < 0:
+        raise RuntimeError("block_table must be a CUDA tensor")
+    if t.dtype is not torch.int32 or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
+        raise RuntimeError("block_table must be int32 [R, W] with contiguous rows")
+    return idx, *t.shape
+
+
 @dataclass
 class FreeBlocks:
     """The free blocks of both tiers as stacks in device memory: hbm / host
@@ -774,6 +792,15 @@ class FreeBlocks:
     hbm: torch.Tensor | None
     host: torch.Tensor | None
     counts: torch.Tensor
+
+
+def _read_header(header: torch.Tensor, what: str) -> dict[str, int]:
+    h = header.tolist()
+    flags = h[nat.TABLES_FIELDS["flags"]]
+    if flags:
+        why = ", ".join(text for bit, text in nat.TABLES_FLAGS.items() if flags & bit)
+        raise RuntimeError(f"{what} refused the step: {why}")
+    return {k: h[i] for k, i in nat.TABLES_FIELDS.items()}
 
 
 class StepTables:
@@ -795,17 +822,13 @@ class StepTables:
 
     def read_header(self) -> dict[str, int]:
         """The header by name (synchronises); raises if the step was refused."""
-        h = self.header.tolist()
-        flags = h[nat.TABLES_FIELDS["flags"]]
-        if flags:
-            why = ", ".join(text for bit, text in nat.TABLES_FLAGS.items() if flags & bit)
-            raise RuntimeError(f"extend_tables refused the step: {why}")
-        return {k: h[i] for k, i in nat.TABLES_FIELDS.items()}
+        return _read_header(self.header, "extend_tables")
 
 
 def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table: torch.Tensor, free: FreeBlocks,
                   num_gpu_blocks: int, num_cpu_blocks: int, block_size: int,
-                  out: StepTables | None = None, max_tokens: int | None = None) -> StepTables:
+                  out: StepTables | None = None, max_tokens: int | None = None,
+                  evicted: torch.Tensor | None = None) -> StepTables:
     """Block tables, slots and positions of a step from the requests' lengths
     (fd_extend_tables), on the GPU without any host synchronisation.
 
@@ -820,14 +843,11 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
     cross_attn's q_len and q_start.  The next step's prior_lens and free.counts
     are its seq_lens and counts, which may be the same tensors.  A step that
     cannot be applied as a whole changes nothing, has no tokens and sets the
-    error word (check_device_errors; StepTables.read_header says why)."""
-    idx = block_table.get_device()
-    if idx < 0:
-        raise RuntimeError("block_table must be a CUDA tensor")
-    if block_table.dtype is not torch.int32 or block_table.dim() != 2 or (block_table.stride(1) != 1
-                                                                          and block_table.shape[1] != 1):
-        raise RuntimeError("block_table must be int32 [R, W] with contiguous rows")
-    R, W = block_table.shape
+    error word (check_device_errors; StepTables.read_header says why).
+    evicted int32 [R]: the tokens that trim_tables cut from each request to
+    meet a budget; positions are ahead of cache indices by as many, and an
+    ended request's entry becomes 0."""
+    idx, R, W = _block_table(block_table)
     if R > 1 and block_table.stride(0) < W:
         raise RuntimeError("block_table's rows must not overlap")
     if out is None:
@@ -844,8 +864,60 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
         0 if host is None else host.numel(), _i32(counts, idx, 2, "free.counts"), _i32(out.counts, idx, 2, "out.counts"),
         num_gpu_blocks, num_cpu_blocks, block_size, T, _i32(out.seq_lens, idx, R, "out.seq_lens"),
         out.query_start_loc.data_ptr(), out.slot_mapping.data_ptr(), out.positions.data_ptr(), out.header.data_ptr(),
-        _error_ptr(idx), _i32(out.query_lens, idx, R, "out.query_lens"))
+        _error_ptr(idx), _i32(out.query_lens, idx, R, "out.query_lens"),
+        0 if evicted is None else _i32(evicted, idx, R, "evicted"))
     _launch(nat.load().fd_extend_tables, packed, idx, "fd_extend_tables")
+    return out
+
+
+class TrimTables:
+    """Device buffers that trim_tables fills for up to R requests: the lengths
+    after it, the free stacks' counts and the header.  seq_lens and counts may
+    be the caller's own tensors, to step them in place."""
+
+    def __init__(self, R: int, device, seq_lens: torch.Tensor | None = None, counts: torch.Tensor | None = None):
+        z = lambda n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
+        self.R = int(R)
+        self.seq_lens = z(R) if seq_lens is None else seq_lens
+        self.counts = z(2) if counts is None else counts
+        self.header = z(nat.TABLES_HEADER_LEN)
+
+    def read_header(self) -> dict[str, int]:
+        """The header by name (synchronises); raises if the call was refused."""
+        return _read_header(self.header, "trim_tables")
+
+
+def trim_tables(keep_lens: torch.Tensor, seq_lens: torch.Tensor, block_table: torch.Tensor, free: FreeBlocks,
+                num_gpu_blocks: int, num_cpu_blocks: int, block_size: int, out: TrimTables | None = None, *,
+                evicted: torch.Tensor | None = None, max_cut: int = 0) -> TrimTables:
+    """Cut requests to their first keep_lens tokens and push the blocks behind
+    them onto their tier's free stack (fd_trim_tables), without any host
+    synchronisation: after verify_drafts, whose keep_lens drops the rejected
+    drafts, or after every layer's move_keys.
+
+    keep_lens int32 [R]: the tokens that stay (below 0, or not below seq_lens:
+    the request is left as it is); seq_lens int32 [R]: its tokens in the cache;
+    block_table int32 [R, W], which stays as it is.  Fills and returns `out`:
+    seq_lens, counts and the header (freed_hbm, freed_host, max_seq); they may
+    be the call's own seq_lens and free.counts.  evicted int32 [R] (cuts to a
+    budget only) grows by what each request lost.  max_cut: the host's bound on
+    that, if it knows one.  A call that cannot be applied as a whole changes
+    nothing and sets the error word (check_device_errors;
+    TrimTables.read_header says why)."""
+    idx, R, W = _block_table(block_table)
+    if out is None:
+        out = TrimTables(R, block_table.device)
+    if out.R < R or out.header.get_device() != idx:
+        raise RuntimeError("out is too small, or on another device")
+    hbm, host, counts = free.hbm, free.host, free.counts
+    packed = _TRIM_STRUCT.pack(
+        _i32(keep_lens, idx, R, "keep_lens"), _i32(seq_lens, idx, R, "seq_lens"), _i32(out.seq_lens, idx, R, "out.seq_lens"),
+        0 if evicted is None else _i32(evicted, idx, R, "evicted"), block_table.data_ptr(), block_table.stride(0), W, R,
+        0 if hbm is None else _i32(hbm, idx, 0, "free.hbm"), 0 if host is None else _i32(host, idx, 0, "free.host"),
+        0 if hbm is None else hbm.numel(), 0 if host is None else host.numel(), _i32(counts, idx, 2, "free.counts"),
+        _i32(out.counts, idx, 2, "out.counts"), num_gpu_blocks, num_cpu_blocks, block_size, max_cut, out.header.data_ptr(),
+        _error_ptr(idx))
+    _launch(nat.load().fd_trim_tables, packed, idx, "fd_trim_tables")
     return out
 
 
@@ -934,11 +1006,10 @@ def _attn_workspace_bytes(H: int, KVH: int, D: int, dtype: torch.dtype) -> int:
     return nat.load().fd_attn_workspace_size(ctypes.byref(a))
 
 
-def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, table, W, bt_row, k_start, BS,
-          max_q_len, max_k_len, workspace_buf) -> None:
+def _attn_fields(q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, table, W, bt_row, k_start, BS, max_q_len,
+                 max_k_len) -> list:
+    """The fields of fd_attn_args, its workspace (the third and second last) still 0."""
     idx, dt = q.get_device(), q.dtype
-    if out.shape != q.shape:
-        raise RuntimeError("q and out must be [T, H, D] alike")
     T, H, D = q.shape
     n = q_len.numel()
     lse_f = (0, 0, 0)
@@ -946,23 +1017,57 @@ def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1,
         if lse.dtype is not torch.float32 or lse.get_device() != idx or lse.shape != (H, T):
             raise RuntimeError("lse must be fp32 [H, T] on q's device")
         lse_f = (lse.data_ptr(), *lse.stride())
-    packed = [
-        *_rows3(q, idx, dt, "q"), *_rows3(out, idx, dt, "out"), *lse_f, *f0, *f1, tier_split,
+    return [
+        *_rows3(q, idx, dt, "q"), *((0, 0, 0) if out is None else _rows3(out, idx, dt, "out")), *lse_f, *f0, *f1, tier_split,
         *((0, 0) if table is None else (table.data_ptr(), table.stride(0))),
         0 if bt_row is None else _i32(bt_row, idx, n, "bt_row"), 0 if k_start is None else _i32(k_start, idx, n, "k_start"),
         _i32(q_start, idx, n, "q_start"), _i32(q_len, idx, n, "q_len"), _i32(k_len, idx, n, "k_len"), W, T, n, H, KVH, D,
         BS, scale, dtype_code(dt), max_q_len, max_k_len, 0 if table is None else table.shape[0], 0, 0, _error_ptr(idx)]
+
+
+def _scratch(q: torch.Tensor, workspace_buf: torch.Tensor | None, need: int) -> torch.Tensor:
+    if workspace_buf is None:
+        return torch.empty(need, dtype=torch.uint8, device=q.device)
+    if (workspace_buf.get_device() != q.get_device() or workspace_buf.dtype is not torch.uint8
+            or not workspace_buf.is_contiguous() or workspace_buf.numel() < need):
+        raise RuntimeError(f"workspace_buf must be contiguous uint8 on q's device with >= {need} bytes")
+    return workspace_buf
+
+
+def _attn(fn, what: str, q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, table, W, bt_row, k_start, BS,
+          max_q_len, max_k_len, workspace_buf) -> None:
+    if out.shape != q.shape:
+        raise RuntimeError("q and out must be [T, H, D] alike")
+    packed = _attn_fields(q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, table, W, bt_row, k_start, BS,
+                          max_q_len, max_k_len)
     if f1[-2]:  # a host tier: its copies count
         need = nat.load().fd_attn_workspace_size(_ATTN_STRUCT.pack(*packed))
     else:
-        need = _attn_workspace_bytes(H, KVH, D, dt)
-    if workspace_buf is None:
-        workspace_buf = torch.empty(need, dtype=torch.uint8, device=q.device)
-    elif (workspace_buf.get_device() != idx or workspace_buf.dtype is not torch.uint8 or not workspace_buf.is_contiguous()
-          or workspace_buf.numel() < need):
-        raise RuntimeError(f"workspace_buf must be contiguous uint8 on q's device with >= {need} bytes")
-    packed[-3], packed[-2] = workspace_buf.data_ptr(), workspace_buf.numel()
-    _launch(fn, _ATTN_STRUCT.pack(*packed), idx, what)
+        need = _attn_workspace_bytes(q.shape[1], KVH, q.shape[2], q.dtype)
+    buf = _scratch(q, workspace_buf, need)
+    packed[-3], packed[-2] = buf.data_ptr(), buf.numel()
+    _launch(fn, _ATTN_STRUCT.pack(*packed), q.get_device(), what)
+
+
+def _paged(q, tiers, block_table, bt_row, n: int) -> tuple:
+    """(KVH, BS, C fields of both tiers, W) of a call over the paged cache."""
+    t0, t1 = tiers
+    if t0 is None and t1 is None:
+        raise RuntimeError("at least one KV tier is required")
+    idx = q.get_device()
+    if idx < 0:
+        raise RuntimeError("q must be a CUDA tensor")
+    _, KVH, BS, D = (t0 if t0 is not None else t1).k.shape
+    if q.dim() != 3 or q.shape[2] != D:
+        raise RuntimeError("q must be [T, H, D] with the cache's head size")
+    if block_table.dtype is not torch.int32 or block_table.get_device() != idx or block_table.dim() != 2:
+        raise RuntimeError("block_table must be int32 [R, W] on q's device")
+    R, W = block_table.shape
+    if W > 1 and block_table.stride(1) != 1:
+        raise RuntimeError("block_table rows must be contiguous")
+    if bt_row is None and R < n:
+        raise RuntimeError("block_table must have a row per request")
+    return KVH, BS, _tier_fields(t0, idx, q.dtype, (KVH, BS, D)), _tier_fields(t1, idx, q.dtype, (KVH, BS, D)), W
 
 
 def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
@@ -984,25 +1089,9 @@ def chunk_attn(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier
     sees nothing gets 0 and -inf.  max_q_len / max_k_len: the lengths' bounds,
     if the host knows them.  workspace_buf (uint8) replaces the call's own
     scratch memory."""
-    t0, t1 = tiers
-    if t0 is None and t1 is None:
-        raise RuntimeError("at least one KV tier is required")
-    idx = q.get_device()
-    if idx < 0:
-        raise RuntimeError("q must be a CUDA tensor")
-    _, KVH, BS, D = (t0 if t0 is not None else t1).k.shape
-    if q.dim() != 3 or q.shape[2] != D:
-        raise RuntimeError("q must be [T, H, D] with the cache's head size")
-    if block_table.dtype is not torch.int32 or block_table.get_device() != idx or block_table.dim() != 2:
-        raise RuntimeError("block_table must be int32 [R, W] on q's device")
-    R, W = block_table.shape
-    if W > 1 and block_table.stride(1) != 1:
-        raise RuntimeError("block_table rows must be contiguous")
-    if bt_row is None and R < q_len.numel():
-        raise RuntimeError("block_table must have a row per request")
-    _attn(nat.load().fd_chunk_attn, "fd_chunk_attn", q, out, lse, q_start, q_len, k_len, scale, KVH,
-          _tier_fields(t0, idx, q.dtype, (KVH, BS, D)), _tier_fields(t1, idx, q.dtype, (KVH, BS, D)), tier_split, block_table,
-          W, bt_row, None, BS, max_q_len, max_k_len, workspace_buf)
+    KVH, BS, f0, f1, W = _paged(q, tiers, block_table, bt_row, q_len.numel())
+    _attn(nat.load().fd_chunk_attn, "fd_chunk_attn", q, out, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split,
+          block_table, W, bt_row, None, BS, max_q_len, max_k_len, workspace_buf)
 
 
 def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor, q_len: torch.Tensor,
@@ -1024,6 +1113,208 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch
     _attn(nat.load().fd_cross_attn, "fd_cross_attn", q, out, lse, q_start, q_len, k_len, scale, KVH,
           (k_ptr, _rows3(v, idx, dt, "v")[0], 0, k_sh, k_st, S, 0, 0), _NO_TIER, 0, None, 0, None, k_start, 0, max_q_len,
           max_k_len, workspace_buf)
+
+
+# ------------------------------------------------------------- after the attention
+
+
+@dataclass
+class KeyStats:
+    """What each cached key of one layer has received: weights fp32 and
+    positions int32, both contiguous [blocks, KVH, block_size] on the device and
+    indexed by block id, host-tier blocks included."""
+
+    weights: torch.Tensor
+    positions: torch.Tensor
+
+    def __post_init__(self) -> None:
+        w, p = self.weights, self.positions
+        _check(w.dim() == 3 and w.shape == p.shape, "weights and positions must be [blocks, KVH, block_size] alike")
+        _check(w.dtype == torch.float32 and p.dtype == torch.int32, "weights must be float32, positions int32")
+        _check(w.is_contiguous() and p.is_contiguous() and w.is_cuda and p.device == w.device,
+               "weights and positions must be contiguous on one CUDA device")
+
+    @classmethod
+    def zeros(cls, num_blocks: int, num_kv_heads: int, block_size: int, device) -> "KeyStats":
+        shape = (num_blocks, num_kv_heads, block_size)
+        return cls(torch.zeros(shape, dtype=torch.float32, device=device), torch.zeros(shape, dtype=torch.int32, device=device))
+
+    def _fields(self, idx: int, KVH: int, BS: int) -> tuple:
+        w = self.weights
+        if w.get_device() != idx or tuple(w.shape[1:]) != (KVH, BS):
+            raise RuntimeError("stats must be [blocks, KVH, block_size] of the cache on the call's device")
+        return w.data_ptr(), self.positions.data_ptr(), w.shape[0]
+
+
+class KeyMoves:
+    """Device buffers that select_keys fills and move_keys reads, for R requests
+    of KVH kv heads and up to `room` moves each: src and dst int32 [R, KVH,
+    room], counts int32 [R, KVH].  A request cut from n keys to b needs room for
+    min(b, n - b)."""
+
+    def __init__(self, R: int, KVH: int, room: int, device, src: torch.Tensor | None = None,
+                 dst: torch.Tensor | None = None, counts: torch.Tensor | None = None):
+        z = lambda *n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
+        self.R, self.KVH, self.room = int(R), int(KVH), int(room)
+        self.src = z(R, KVH, room) if src is None else src
+        self.dst = z(R, KVH, room) if dst is None else dst
+        self.counts = z(R, KVH) if counts is None else counts
+
+    def _fields(self, idx: int, R: int, KVH: int) -> tuple:
+        if self.KVH != KVH or self.R < R:
+            raise RuntimeError("moves must be of at least R requests and of KVH kv heads")
+        n = R * KVH * self.room
+        return (_i32(self.src, idx, n, "moves.src"), _i32(self.dst, idx, n, "moves.dst"),
+                _i32(self.counts, idx, R * KVH, "moves.counts"))
+
+
+@lru_cache(maxsize=1)
+def _key_weights_workspace_bytes() -> int:
+    a = nat.FdKeyWeightsArgs()
+    a.attn.head_size = 64  # without a host tier the same for all sizes
+    return nat.load().fd_key_weights_workspace_size(ctypes.byref(a))
+
+
+def key_weights(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
+                q_start: torch.Tensor, q_len: torch.Tensor, k_len: torch.Tensor, scale: float, lse: torch.Tensor,
+                stats: KeyStats, *, evicted: torch.Tensor | None = None, bt_row: torch.Tensor | None = None,
+                max_q_len: int = 0, max_k_len: int = 0, workspace_buf: torch.Tensor | None = None) -> None:
+    """Add up the attention weight that each cached key receives in a step
+    (fd_key_weights): over the queries that see it and the heads of its kv head,
+    exp(scale q.k - lse), with lse [H, T] as chunk_attn (or the decode) wrote
+    it.  The other arguments are chunk_attn's.
+
+    The q_len newest keys of a request are new: their weight in `stats` is set,
+    whatever it was, and their position becomes their index plus evicted[r]
+    (int32 [n], see trim_tables).  Older keys' weights are added to.  So a key
+    needs no reset when its block is handed to another request, and a step whose
+    drafts were rejected can count the accepted ones alone (q_len and k_len
+    without the others)."""
+    KVH, BS, f0, f1, W = _paged(q, tiers, block_table, bt_row, q_len.numel())
+    idx = q.get_device()
+    packed = _attn_fields(q, None, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, block_table, W, bt_row, None, BS,
+                          max_q_len, max_k_len)
+    more = (*stats._fields(idx, KVH, BS), 0 if evicted is None else _i32(evicted, idx, q_len.numel(), "evicted"))
+    if f1[-2]:  # a host tier: its copies count
+        need = nat.load().fd_key_weights_workspace_size(_KEY_WEIGHTS_STRUCT.pack(*packed, *more))
+    else:
+        need = _key_weights_workspace_bytes()
+    buf = _scratch(q, workspace_buf, need)
+    packed[-3], packed[-2] = buf.data_ptr(), buf.numel()
+    _launch(nat.load().fd_key_weights, _KEY_WEIGHTS_STRUCT.pack(*packed, *more), idx, "fd_key_weights")
+
+
+def select_keys(stats: KeyStats, block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens: torch.Tensor,
+                moves: KeyMoves | None = None, *, sinks: int = 0, recent: int = 0, evicted: torch.Tensor | None = None,
+                max_k_len: int = 0) -> KeyMoves:
+    """Choose the keys that stay when caches are cut to a budget
+    (fd_select_keys), per request and kv head: those whose position is below
+    `sinks` or among the newest `recent`, then those with the most weight, the
+    lowest index first where weights are equal (a NaN is the least).
+
+    seq_lens int32 [R]: the tokens in the cache; keep_lens int32 [R]: those to
+    keep (below 0, or not below seq_lens: the request is left as it is);
+    evicted int32 [R]: tokens cut earlier.  Writes to `moves` (default: a new
+    one, with room for max_k_len / 2 moves) which keys move where, all from
+    behind the budget to before it; nothing else changes.  A request that could
+    need more moves than there is room for has none, and sets the error word."""
+    idx, R, W = _block_table(block_table)
+    _, KVH, BS = stats.weights.shape
+    if moves is None:
+        moves = KeyMoves(R, KVH, (max_k_len if max_k_len > 0 else W * BS) // 2, block_table.device)
+    packed = _SELECT_STRUCT.pack(
+        *stats._fields(idx, KVH, BS), block_table.data_ptr(), block_table.stride(0), _i32(seq_lens, idx, R, "seq_lens"),
+        _i32(keep_lens, idx, R, "keep_lens"), 0 if evicted is None else _i32(evicted, idx, R, "evicted"),
+        *moves._fields(idx, R, KVH), W, R, KVH, BS, moves.room, sinks, recent, max_k_len, _error_ptr(idx))
+    _launch(nat.load().fd_select_keys, packed, idx, "fd_select_keys")
+    return moves
+
+
+def move_keys(moves: KeyMoves, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
+              stats: KeyStats | None = None) -> None:
+    """Move the K and V rows that `moves` lists within each request's blocks, in
+    either tier, and their weights and positions in `stats` (fd_move_keys).  Then
+    the first keep_lens tokens of each request are its cache (trim_tables, once
+    all layers have moved theirs).  K rows carry their rotary positions with
+    them, so their order within the cache does not matter to the queries that
+    come after."""
+    t0, t1 = tiers
+    if t0 is None and t1 is None:
+        raise RuntimeError("at least one KV tier is required")
+    idx, R, W = _block_table(block_table)
+    k = (t0 if t0 is not None else t1).k
+    _, KVH, BS, D = k.shape
+    shape = (KVH, BS, D)
+    packed = _MOVE_STRUCT.pack(
+        *moves._fields(idx, R, KVH), *_tier_fields(t0, idx, k.dtype, shape), *_tier_fields(t1, idx, k.dtype, shape), tier_split,
+        block_table.data_ptr(), block_table.stride(0), *((0, 0, 0) if stats is None else stats._fields(idx, KVH, BS)), W, R,
+        KVH, D, BS, moves.room, dtype_code(k.dtype), 0, _error_ptr(idx))
+    _launch(nat.load().fd_move_keys, packed, idx, "fd_move_keys")
+
+
+class DraftVerdict:
+    """Device buffers that verify_drafts fills for R requests of up to K drafted
+    tokens: tokens int64 [R, K + 1] (the accepted drafts, the token that
+    follows, then -1), accepted int32 [R], keep_lens int32 [R]."""
+
+    def __init__(self, R: int, K: int, device):
+        self.R, self.K = int(R), int(K)
+        self.tokens = torch.full((R, K + 1), -1, dtype=torch.int64, device=device)
+        self.accepted = torch.zeros(R, dtype=torch.int32, device=device)
+        self.keep_lens = torch.zeros(R, dtype=torch.int32, device=device)
+
+
+def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_probs: torch.Tensor | None,
+                  q_start: torch.Tensor, q_len: torch.Tensor, accept_u: torch.Tensor, sample_u: torch.Tensor, *,
+                  seq_lens: torch.Tensor | None = None, out: DraftVerdict | None = None) -> DraftVerdict:
+    """Verify drafted tokens against the target's probabilities and draw the
+    token that follows the accepted ones (fd_verify_drafts); q_len = 1 is
+    ordinary sampling.
+
+    target_probs [T, V]: a row per query of the step; q_start, q_len int32 [R]
+    as extend_tables gives them (q_len = 1 + drafts; 0: no part in the step);
+    draft_tokens int64 [R, K]; draft_probs [R, K, V] of target_probs' dtype
+    (fp32, fp16 or bf16), or None where the draft is no distribution;
+    accept_u fp32 [R, K] and sample_u fp32 [R]: uniform numbers in [0, 1).
+    Draft d is accepted while accept_u q < p; the token after the accepted ones
+    comes from max(p - q, 0) of the rejected draft, or from the last row, by
+    sample_u's place in the running sum.  A one-hot row is greedy decoding.
+    Fills and returns `out`; keep_lens, with seq_lens int32 [R] (the drafts
+    included), is the cache that stays: trim_tables' keep_lens."""
+    idx, dt = target_probs.get_device(), target_probs.dtype
+    if idx < 0:
+        raise RuntimeError("target_probs must be a CUDA tensor")
+    if target_probs.dim() != 2 or (target_probs.stride(1) != 1 and target_probs.shape[1] != 1):
+        raise RuntimeError("target_probs must be [T, V] with contiguous rows")
+    T, V = target_probs.shape
+    if draft_tokens.dim() != 2 or draft_tokens.dtype is not torch.int64 or draft_tokens.get_device() != idx or (
+            draft_tokens.stride(1) != 1 and draft_tokens.shape[1] > 1):
+        raise RuntimeError("draft_tokens must be int64 [R, K] with contiguous rows on target_probs' device")
+    R, K = draft_tokens.shape
+    if accept_u.shape != (R, K) or accept_u.dtype is not torch.float32 or accept_u.get_device() != idx or (
+            accept_u.stride(1) != 1 and K > 1):
+        raise RuntimeError("accept_u must be fp32 [R, K] with contiguous rows on target_probs' device")
+    if sample_u.dtype is not torch.float32 or sample_u.get_device() != idx or sample_u.numel() < R or not sample_u.is_contiguous():
+        raise RuntimeError("sample_u must be contiguous fp32 [R] on target_probs' device")
+    probs = (0, 0, 0)
+    if draft_probs is not None:
+        if draft_probs.shape != (R, K, V) or draft_probs.dtype is not dt or draft_probs.get_device() != idx or (
+                draft_probs.stride(2) != 1 and V > 1):
+            raise RuntimeError("draft_probs must be [R, K, V] with contiguous rows and target_probs' dtype and device")
+        probs = (draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1))
+    if out is None:
+        out = DraftVerdict(R, K, target_probs.device)
+    if (out.R < R or out.K != K or out.tokens.dtype is not torch.int64 or out.tokens.get_device() != idx
+            or not out.tokens.is_contiguous()):
+        raise RuntimeError("out must be a DraftVerdict of at least R requests and of K drafts on target_probs' device")
+    packed = _VERIFY_STRUCT.pack(
+        target_probs.data_ptr(), target_probs.stride(0), *probs, draft_tokens.data_ptr(), draft_tokens.stride(0),
+        _i32(q_start, idx, R, "q_start"), _i32(q_len, idx, R, "q_len"), accept_u.data_ptr(), accept_u.stride(0),
+        sample_u.data_ptr(), 0 if seq_lens is None else _i32(seq_lens, idx, R, "seq_lens"), out.tokens.data_ptr(),
+        _i32(out.accepted, idx, R, "out.accepted"), _i32(out.keep_lens, idx, R, "out.keep_lens"), R, K, V, T, dtype_code(dt),
+        0, _error_ptr(idx))
+    _launch(nat.load().fd_verify_drafts, packed, idx, "fd_verify_drafts")
+    return out
 
 
 # ------------------------------------------------------------- merge
