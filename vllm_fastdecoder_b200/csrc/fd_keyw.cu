@@ -267,6 +267,7 @@ extern "C" int fd_key_weights(const fd_key_weights_args* args, void* stream) {
   p.parts = reinterpret_cast<float*>(ws + kw::cut_bytes());
   st = at::stage_launch(p.a, a, kw::base_workspace(), true, s);
   if (st != FD_OK) return st;
+  if (at::mma_covers(a)) return kw::mma_launch(p, a, s);
   p.a.tq = kw::kRows / p.a.G;
   switch (a->dtype) {
     case FD_DTYPE_F16:
