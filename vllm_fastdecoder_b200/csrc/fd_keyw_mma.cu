@@ -12,10 +12,13 @@
 // bytes of K, and shared memory is a ring of K tiles; with more (N = 128) by
 // the exponentials, and it is a ring of query chunks beside two items' K.
 //
-// Warps: 0-3 and 4-7 the epilogue of either key tile, 8 schedule, query chunks
-// and their lse (one step ahead, so that those loads cost no step its time), 9
-// K tiles, 10 (one thread) the MMAs.  A STEP is one chunk against one item; its
-// record goes through a ring to all roles.  Every wait is bounded, and a role
+// Warps: the epilogue's first, four per key tile, and with N = 128 another four
+// per tile, the two groups taking turns at the steps (two warps per scheduler
+// leave the SFU idle while both wait; their sums are joined at the item's end);
+// then one for the schedule, the query chunks and their lse (a step ahead, so
+// that those loads cost no step its time), one per key tile that loads K, and
+// one whose first thread issues the MMAs.  A STEP is one chunk against one item;
+// its record goes through a ring to all roles.  Every wait is bounded, and a role
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 32 single tokens of 32 heads over 512 to 8192 keys of 8 heads x 128
@@ -35,11 +38,6 @@ using namespace at::mm;
 constexpr int kTiles = 2;             // key tiles of an item
 constexpr int kKeys = kTiles * kKT;
 static_assert(kKeys == kMaxKeys, "partials per item");
-constexpr int kSumWarps = 4 * kTiles;
-constexpr int kWarpSched = kSumWarps, kWarpK = kSumWarps + 1, kWarpMma = kSumWarps + 2;
-constexpr int kThreads = (kSumWarps + 3) * 32;
-constexpr int kSteps = 8;             // steps in flight between the roles
-constexpr int kStepReaders = kSumWarps + 2;
 constexpr int kFixed = 2;             // an item's fixed cost in chunks
 constexpr int kMinPer = 3;            // least positions of a CTA
 
@@ -52,6 +50,12 @@ struct KwMmaParams {
 
 template <int KD, int N>
 struct Geo {
+  static constexpr int kGroups = N <= 32 ? 1 : 2;        // epilogue warpgroups of a key tile
+  static constexpr int kSumWarps = 4 * kTiles * kGroups;
+  static constexpr int kWarpSched = kSumWarps, kWarpK = kSumWarps + 1, kWarpMma = kWarpK + kTiles;
+  static constexpr int kThreads = (kWarpMma + 1) * 32;
+  static constexpr int kSteps = N <= 32 ? 8 : 4;         // steps in flight between the roles
+  static constexpr int kStepReaders = kSumWarps + kTiles + 1;
   static constexpr int kPanels = KD / 64;
   static constexpr int kTile = kPanels * kPanel;
   static constexpr int kItem = kTiles * kTile;
@@ -64,26 +68,29 @@ struct Geo {
   static constexpr int kOffQ = kRingK * kItem;
   static constexpr int kOffLse = kOffQ + kRingQ * kQ;    // [kRingQ][N] -lse log2(e)
   static constexpr int kOffStep = kOffLse + kRingQ * (N < 32 ? 32 : N) * 4;
-  static constexpr int kOffBar = kOffStep + kSteps * 64;
-  // k full [ring][tiles], k empty, q full, q empty, s full [bufs][tiles], s empty [bufs][tiles], step full, step empty, drain
-  static constexpr int kNumBars = kRingK * (kTiles + 1) + 2 * kRingQ + 2 * kBufs * kTiles + 2 * kSteps + 1;
+  static constexpr int kOffJoin = kOffStep + kSteps * 48;  // [kTiles][kKT] the second groups' sums
+  static constexpr int kOffBar = kOffJoin + (kGroups - 1) * kKeys * 4;
+  // k full [ring][tiles], k empty, q full, q empty, s full [bufs][tiles], s empty [bufs][tiles], step full, step empty,
+  // join full, empty [tiles], drain
+  static constexpr int kNumBars = kRingK * (kTiles + 1) + 2 * kRingQ + 2 * kBufs * kTiles + 2 * kSteps + 2 * kTiles + 1;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;  // abort flag, TMEM address
   static constexpr int kSmem = kOffMisc + 16;
   static_assert(kSmem <= 227 * 1024, "smem budget");
   static_assert(sizeof(MmaWalk::Scratch) <= kRingQ * (N < 32 ? 32 : N) * 4, "scratch of the schedule");
 };
 
+// What a step is the first or last of: its segment (K), its chunk's stay in a
+// slot (Q).  Flags 0: no more steps.
+enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8, kLastQ = 16 };
 struct Step {
-  int live;          // 0: no more steps
-  int new_k, last_k; // first, last step of the segment
-  int new_q, last_q; // first, last step of the chunk in its slot
+  int flags;
   int r, kh, kt, kbase;
   int tok0, rows;    // of the chunk: its first token, its rows
   int qlen, klen;
   int slot;          // -1: whole, else its slot of the partials
   int pad[2];
 };
-static_assert(sizeof(Step) == 64, "step record");
+static_assert(sizeof(Step) == 48, "step record");
 
 // Wait for this thread's TMEM loads.  The registers are operands, so that
 // nothing that reads them is moved ahead of it.
@@ -130,11 +137,12 @@ __device__ __forceinline__ void add_up(const uint32_t (&s)[32], const float* neg
 }
 
 template <typename T, int KD, int N>
-__global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_constant__ KwMmaParams kp) {
+__global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(const __grid_constant__ KwMmaParams kp) {
   typedef Geo<KD, N> Ge;
   constexpr bool kBF16 = std::is_same<T, __nv_bfloat16>::value;
   constexpr uint32_t kIdQK = instr_desc(kBF16, false, kKT, N);
-  constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingQ = Ge::kRingQ, kBufs = Ge::kBufs;
+  constexpr int kTile = Ge::kTile, kRingK = Ge::kRingK, kRingQ = Ge::kRingQ, kBufs = Ge::kBufs, kSteps = Ge::kSteps;
+  constexpr int kSumWarps = Ge::kSumWarps, kWarpK = Ge::kWarpK, kGroups = Ge::kGroups;
   constexpr int kLseRow = N < 32 ? 32 : N;
   const at::mm::MmaParams& mp = kp.m;
   const AttnParams& p = mp.a;
@@ -147,7 +155,9 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
   uint64_t* s_empty = s_full + kBufs * kTiles;   // [kBufs][kTiles] four epilogue warps have the scores
   uint64_t* step_full = s_empty + kBufs * kTiles;
   uint64_t* step_empty = step_full + kSteps;
-  uint64_t* drain = step_empty + kSteps;
+  uint64_t* join_full = step_empty + kSteps;     // [kTiles] four warps of the second group wrote their sums
+  uint64_t* join_empty = join_full + kTiles;     // [kTiles] four warps of the first have read them
+  uint64_t* drain = join_empty + kTiles;
   Step* steps = reinterpret_cast<Step*>(smem + Ge::kOffStep);
   float* lse_sh = reinterpret_cast<float*>(smem + Ge::kOffLse);
   volatile int* misc = reinterpret_cast<volatile int*>(smem + Ge::kOffMisc);
@@ -160,15 +170,16 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
     uint64_t* b = k_full + i;
     if (b >= q_empty && b < s_full) return 1 + kSumWarps;
     if (b >= s_empty && b < step_full) return 4;
-    return b >= step_empty && b < drain ? kStepReaders : 1;
+    if (b >= join_full && b < drain) return 4;
+    return b >= step_empty && b < join_full ? Ge::kStepReaders : 1;
   });
   if (threadIdx.x == 0) {
     kp.k.cuts[cta].nparts = 0;
     misc[0] = 0;
   }
   MmaWalk walk(p);
-  if (!walk.init<kThreads>(reinterpret_cast<MmaWalk::Scratch*>(lse_sh), cta, kMinPer)) return;  // all threads alike
-  if (warp == kWarpMma) {
+  if (!walk.init<Ge::kThreads>(reinterpret_cast<MmaWalk::Scratch*>(lse_sh), cta, kMinPer)) return;  // all threads alike
+  if (warp == Ge::kWarpMma) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(
                      smem_u32(smem + Ge::kOffMisc + 4)),
                  "r"(Ge::kTmem)
@@ -180,66 +191,65 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
   tc_fence_after();
   const uint32_t tmem = (uint32_t)misc[1];
 
-  if (warp == kWarpSched) {
+  if (warp == Ge::kWarpSched) {
     // ------------------------------------------------ schedule, query chunks and their lse
     constexpr int kPer = kLseRow / 32;  // columns per lane
+    int col_t[kPer], col_h[kPer];       // token and head of each
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      col_t[i] = (32 * i + lane) / p.G;
+      col_h[i] = 32 * i + lane - col_t[i] * p.G;
+    }
     MmaWalk::Seg g;
     int left = 0, chunk = 0;            // chunks left of the segment, the next one
     int last_r = -1, last_kh = -1, last_chunk = -1;
-    auto gen = [&](Step& s, Req& rq, int& c, float (&ls)[kPer]) {  // the next step, its lse on the way
-      s.live = 1;
-      s.new_k = 0;
+    auto gen = [&](Step& s, Req& rq, float (&ls)[kPer]) {  // the next step, its lse on the way
+      s.flags = kLive;
       if (left == 0) {
-        s.live = walk.next(g);
-        if (!s.live) {
-          s.new_q = 1;
+        if (!walk.next(g)) {
+          s.flags = 0;
           return;
         }
         left = g.n;
         chunk = g.c0;
-        s.new_k = 1;
+        s.flags |= kNewK;
+        if (g.nparts > 0 && lane == 0) kp.k.cuts[cta] = Cut{g.nparts, g.r, g.kh, g.kt};
       }
       rq = walk.rq;
-      c = chunk++;
-      s.last_k = --left == 0;
-      s.new_q = g.r != last_r || g.kh != last_kh || c != last_chunk;
-      last_r = g.r;
-      last_kh = g.kh;
-      last_chunk = c;
+      if (--left == 0) s.flags |= kLastK;
       s.r = g.r;
       s.kh = g.kh;
       s.kt = g.kt;
       s.kbase = rq.kbase;
-      s.tok0 = c * p.tq;
+      s.tok0 = chunk * p.tq;
       s.rows = min(p.tq, rq.qlen - s.tok0) * p.G;
       s.qlen = rq.qlen;
       s.klen = rq.klen;
       s.slot = g.whole ? -1 : 2 * cta + (g.head ? 1 : 0);
-      if (s.new_k && g.nparts > 0 && lane == 0) kp.k.cuts[cta] = Cut{g.nparts, g.r, g.kh, g.kt};
-      if (s.new_q) {
+      if (g.r != last_r || g.kh != last_kh || chunk != last_chunk) {
+        s.flags |= kNewQ;
+        const float* at = p.lse + (int64_t)(s.kh * p.G) * p.lse_sh + (int64_t)(rq.qst + s.tok0) * p.lse_st;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-          const int n = 32 * i + lane, t = n / p.G;
-          ls[i] = n < s.rows ? p.lse[(int64_t)(s.kh * p.G + n - t * p.G) * p.lse_sh + (int64_t)(rq.qst + s.tok0 + t) * p.lse_st]
-                             : 0.f;
-        }
+        for (int i = 0; i < kPer; ++i) ls[i] = 32 * i + lane < s.rows ? at[col_h[i] * p.lse_sh + col_t[i] * p.lse_st] : 0.f;
       }
+      last_r = g.r;
+      last_kh = g.kh;
+      last_chunk = chunk++;
     };
     Step cur, nxt;
     Req rq = {0, 0, 0, 0}, rq_next = rq;
-    int c = 0, c_next = 0;
     float ls[kPer], ls_next[kPer];
-    gen(cur, rq, c, ls);
+    gen(cur, rq, ls);
     int qs = -1;
     uint32_t nq = 0;
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
-      if (cur.live) gen(nxt, rq_next, c_next, ls_next);
+      if (cur.flags != 0) gen(nxt, rq_next, ls_next);
       const int ss = i % kSteps;
       if (i >= kSteps)
         ok = __all_sync(0xffffffffu, wait_or_abort(&step_empty[ss], (i / kSteps - 1) & 1u, misc, p.err));
       if (!ok) break;
-      if (cur.live && cur.new_q) {
+      if ((cur.flags & kNewQ) != 0) {
         qs = (int)(nq % kRingQ);
         if (nq >= (uint32_t)kRingQ)
           ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[qs], (nq / kRingQ - 1) & 1u, misc, p.err));
@@ -263,14 +273,13 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
           if (lane == 0) mbar_arrive(&q_full[qs]);
         }
       }
-      cur.last_q = cur.live && nxt.new_q;
+      if (cur.flags != 0 && (nxt.flags == 0 || (nxt.flags & kNewQ) != 0)) cur.flags |= kLastQ;
       if (lane == 0) steps[ss] = cur;
       __syncwarp();
       if (lane == 0) mbar_arrive(&step_full[ss]);
-      if (!cur.live) break;
+      if (cur.flags == 0) break;
       cur = nxt;
       rq = rq_next;
-      c = c_next;
 #pragma unroll
       for (int x = 0; x < kPer; ++x) ls[x] = ls_next[x];
     }
@@ -280,12 +289,13 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
       const uint32_t last = s + kRingQ * ((nq - 1 - s) / kRingQ);
       mbar_wait(&q_full[s], (last / kRingQ) & 1u, p.err);
     }
-  } else if (warp == kWarpK) {
-    // ------------------------------------------------ K tiles
+  } else if (warp >= kWarpK && warp < kWarpK + kTiles) {
+    // ------------------------------------------------ K, key tile t of every item
+    const int t = warp - kWarpK;
     const uint64_t pol = l2_evict_first_policy();
     uint32_t i = 0, items = 0;
     Step item;           // the item to load next, its block ids on the way
-    int id[kTiles];
+    int id = -1;
     auto take = [&]() {  // the next step that begins an item; false: given up
       for (;; ++i) {
         const int ss = i % kSteps;
@@ -293,34 +303,29 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
         item = steps[ss];
         __syncwarp();
         if (lane == 0) mbar_arrive(&step_empty[ss]);
-        if (!item.live || item.new_k) break;
+        if (item.flags == 0 || (item.flags & kNewK) != 0) break;
       }
       ++i;
-      if (item.live) {
-#pragma unroll
-        for (int t = 0; t < kTiles; ++t) id[t] = box_block(mp, false, item.kbase, item.klen, item.kt * kTiles + t, lane);
-      }
+      if (item.flags != 0) id = box_block(mp, false, item.kbase, item.klen, item.kt * kTiles + t, lane);
       return true;
     };
     bool ok = take();
-    while (ok && item.live) {
+    while (ok && item.flags != 0) {
       const int ks = (int)(items % kRingK);
       if (items >= (uint32_t)kRingK)
         ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[ks], (items / kRingK - 1) & 1u, misc, p.err));
       if (!ok) break;
       ++items;
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t)
-        load_tile<KD>(mp, false, smem + ks * Ge::kItem + t * kTile, &k_full[ks * kTiles + t], item.kt * kTiles + t, item.r,
-                      item.kbase, item.klen, item.kh, id[t], lane, pol);
+      load_tile<KD>(mp, false, smem + ks * Ge::kItem + t * kTile, &k_full[ks * kTiles + t], item.kt * kTiles + t, item.r,
+                    item.kbase, item.klen, item.kh, id, lane, pol);
       ok = take();
     }
     if (!ok) misc[0] = 1;
     for (uint32_t s = 0; s < (uint32_t)kRingK && s < items; ++s) {
       const uint32_t last = s + kRingK * ((items - 1 - s) / kRingK);
-      for (int t = 0; t < kTiles; ++t) mbar_wait(&k_full[s * kTiles + t], (last / kRingK) & 1u, p.err);
+      mbar_wait(&k_full[s * kTiles + t], (last / kRingK) & 1u, p.err);
     }
-  } else if (warp == kWarpMma) {
+  } else if (warp == Ge::kWarpMma) {
     // ------------------------------------------------ MMA issuer
     if (lane == 0) {
       const uint32_t base = smem_u32(smem) >> 4;
@@ -332,10 +337,10 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
         const int ss = i % kSteps;
         ok = poll_or_abort(&step_full[ss], (i / kSteps) & 1u, misc, p.err);
         if (!ok) break;
-        const int live = steps[ss].live, new_k = steps[ss].new_k, last_k = steps[ss].last_k, new_q = steps[ss].new_q,
-                  last_q = steps[ss].last_q;
+        const int flags = steps[ss].flags;
         mbar_arrive(&step_empty[ss]);
-        if (!live) break;
+        if (flags == 0) break;
+        const bool new_k = (flags & kNewK) != 0, new_q = (flags & kNewQ) != 0;
         items += new_k;
         nq += new_q;
         const int ks = (int)((items - 1) % kRingK), qs = (int)((nq - 1) % kRingQ), b = (int)(i % kBufs);
@@ -354,8 +359,8 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
                         q_lo + (uint32_t)(((x >> 2) * (N * 128) + (x & 3) * 32) >> 4), q_hi, kIdQK, x > 0 ? 1u : 0u);
           umma_commit(&s_full[b * kTiles + t]);
         }
-        if (ok && last_k) umma_commit(&k_empty[ks]);
-        if (ok && last_q) umma_commit(&q_empty[qs]);
+        if (ok && (flags & kLastK) != 0) umma_commit(&k_empty[ks]);
+        if (ok && (flags & kLastQ) != 0) umma_commit(&q_empty[qs]);
       }
       if (!ok) misc[0] = 1;
       umma_commit(drain);  // all MMAs complete before TMEM is released
@@ -364,10 +369,12 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
     __syncwarp();
   } else {
     // ------------------------------------------------ epilogue: one key per thread
-    const int t = warp >> 2, row = (warp & 3) * 32;  // key tile, first key of the warp in it
+    const int t = (warp >> 2) % kTiles, grp = (warp >> 2) / kTiles;  // key tile, group
+    const int row = (warp & 3) * 32;                                 // first key of the warp in its tile
     const uint32_t lanes = (uint32_t)row << 16;
     const f2_t sl2 = f2_pack(p.sl2, p.sl2);
-    uint32_t nq = 0;
+    float* const joined = reinterpret_cast<float*>(smem + Ge::kOffJoin) + t * kKT + row + lane;
+    uint32_t nq = 0, items = 0;
     f2_t acc[2] = {0ull, 0ull};
     int64_t id = -1;
     bool ok = true;
@@ -378,77 +385,96 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
       const Step s = steps[ss];
       __syncwarp();
       if (lane == 0) mbar_arrive(&step_empty[ss]);
-      if (!s.live) break;
-      nq += s.new_q;
+      if (s.flags == 0) break;
+      if ((s.flags & kNewQ) != 0) ++nq;
       const int qs = (int)((nq - 1) % kRingQ);
       const int key0 = s.kt * kKeys + t * kKT + row, key = key0 + lane;
-      if (s.new_k) {
+      if ((s.flags & kNewK) != 0) {
         acc[0] = acc[1] = 0ull;
         // (of a cut item the combine looks it up)
-        if (key < s.klen && s.slot < 0) id = p.bt[(int64_t)s.kbase * p.bt_stride + (int)((unsigned)key / (unsigned)p.BS)];
+        if (grp == 0 && key < s.klen && s.slot < 0) id = p.bt[(int64_t)s.kbase * p.bt_stride + (int)((unsigned)key / (unsigned)p.BS)];
       }
-      ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[b * kTiles + t], (i / kBufs) & 1u, misc, p.err));
-      if (!ok) break;
-      tc_fence_after();
-      // column n (token tok0 + n / G) sees keys up to klen - qlen + its token
-      const int first = s.klen - s.qlen + s.tok0;
-      const int last_tok = s.rows / p.G - 1;
-      const bool any = key0 < s.klen && key0 <= first + last_tok;  // the warp alike
-      const uint32_t ts = tmem + lanes + (uint32_t)((t * kBufs + b) * Ge::kCols);
-      const float* neg = lse_sh + qs * kLseRow;
-      if (any) {
-        const int over = key - first;
-        const int from = over > 0 ? over * p.G : 0;
-        const bool masked = key0 + 31 > first || s.rows < N;
-        if constexpr (N <= 32) {
-          uint32_t v[32];
-          if constexpr (N == 16) {
-            uint32_t w[16];
-            tmem_ld16_nowait(ts, w);
-            wait_loaded(w);
+      if (kGroups == 1 || (int)(i & 1u) == grp) {
+        ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[b * kTiles + t], (i / kBufs) & 1u, misc, p.err));
+        if (!ok) break;
+        tc_fence_after();
+        // column n (token tok0 + n / G) sees keys up to klen - qlen + its token
+        const int first = s.klen - s.qlen + s.tok0;
+        const int last_tok = s.rows / p.G - 1;
+        const bool any = key0 < s.klen && key0 <= first + last_tok;  // the warp alike
+        const uint32_t ts = tmem + lanes + (uint32_t)((t * kBufs + b) * Ge::kCols);
+        const float* neg = lse_sh + qs * kLseRow;
+        if (any) {
+          const int over = key - first;
+          const int from = over > 0 ? over * p.G : 0;
+          const bool masked = key0 + 31 > first || s.rows < N;
+          if constexpr (N <= 32) {
+            uint32_t v[32];
+            if constexpr (N == 16) {
+              uint32_t w[16];
+              tmem_ld16_nowait(ts, w);
+              wait_loaded(w);
 #pragma unroll
-            for (int x = 0; x < 32; ++x) v[x] = x < 16 ? w[x] : 0u;
+              for (int x = 0; x < 32; ++x) v[x] = x < 16 ? w[x] : 0u;
+            } else {
+              tmem_ld32_nowait(ts, v);
+              wait_loaded(v);
+            }
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
+            add_up<true>(v, neg, sl2, 0, from, s.rows, acc);
           } else {
-            tmem_ld32_nowait(ts, v);
-            wait_loaded(v);
+            uint32_t v[2][32];
+            tmem_ld32_nowait(ts, v[0]);
+#pragma unroll
+            for (int c = 0; c < N / 32; ++c) {
+              wait_loaded(v[c & 1]);
+              if (c + 1 < N / 32) {
+                tmem_ld32_nowait(ts + 32 * (c + 1), v[(c + 1) & 1]);
+              } else {
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
+              }
+              if (masked)
+                add_up<true>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
+              else
+                add_up<false>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
+            }
           }
+        } else {
           tc_fence_before();
           __syncwarp();
           if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
-          add_up<true>(v, neg, sl2, 0, from, s.rows, acc);
-        } else {
-          uint32_t v[2][32];
-          tmem_ld32_nowait(ts, v[0]);
-#pragma unroll
-          for (int c = 0; c < N / 32; ++c) {
-            wait_loaded(v[c & 1]);
-            if (c + 1 < N / 32) {
-              tmem_ld32_nowait(ts + 32 * (c + 1), v[(c + 1) & 1]);
-            } else {
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
-            }
-            if (masked)
-              add_up<true>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
-            else
-              add_up<false>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
-          }
         }
-      } else {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
       }
-      if (s.last_q) {
+      if ((s.flags & kLastQ) != 0) {
         __syncwarp();
         if (lane == 0) mbar_arrive(&q_empty[qs]);
       }
-      if (s.last_k) {
+      if ((s.flags & kLastK) != 0) {
         float a0, a1, a2, a3;
         f2_unpack(acc[0], a0, a1);
         f2_unpack(acc[1], a2, a3);
-        const float w = (a0 + a1) + (a2 + a3);
+        float w = (a0 + a1) + (a2 + a3);
+        if constexpr (kGroups > 1) {
+          if (grp == 1) {
+            if (items > 0) ok = __all_sync(0xffffffffu, wait_or_abort(&join_empty[t], (items - 1) & 1u, misc, p.err));
+            if (!ok) break;
+            *joined = w;
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&join_full[t]);
+            ++items;
+            continue;
+          }
+          ok = __all_sync(0xffffffffu, wait_or_abort(&join_full[t], items & 1u, misc, p.err));
+          if (!ok) break;
+          w += *joined;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&join_empty[t]);
+          ++items;
+        }
         if (s.slot >= 0) {
           kp.k.parts[(int64_t)s.slot * kMaxKeys + t * kKT + row + lane] = w;
         } else if (key < s.klen) {
@@ -464,7 +490,7 @@ __global__ void __launch_bounds__(kThreads, 1) fd_keyw_mma_kernel(const __grid_c
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (warp == kWarpMma)
+  if (warp == Ge::kWarpMma)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(Ge::kTmem) : "memory");
 }
 
@@ -474,7 +500,7 @@ int launch(const KwMmaParams& kp, cudaStream_t s) {
   static unsigned long long done = 0;
   const int st = fdh::ensure_smem(kern, Geo<KD, N>::kSmem, &done);
   if (st != FD_OK) return st;
-  return fdh::launch_maybe_pdl(kern, dim3((unsigned)kp.k.a.ctas), dim3(kThreads), Geo<KD, N>::kSmem, s, false, kp,
+  return fdh::launch_maybe_pdl(kern, dim3((unsigned)kp.k.a.ctas), dim3(Geo<KD, N>::kThreads), Geo<KD, N>::kSmem, s, false, kp,
                                "fd_keyw_mma_kernel launch");
 }
 
