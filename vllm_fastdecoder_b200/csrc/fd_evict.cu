@@ -1,16 +1,20 @@
 // A cache cut to a budget: which keys stay (fd_select_keys) and their move to
 // the front of their request's blocks (fd_move_keys).
 //
-// Select.  With the keys of one request and kv head as 32-bit numbers in the
-// order that the choice wants (guarded ones above all, a NaN below all, ties
-// by index), the keep-th greatest T is found by four rounds of 256 counters,
-// eight bits a round.  A key stays if it is above T, or equals T and is among
-// the first of those that are still wanted.  Two running counts in index order
-// (equals; then places that become free and keys that move) give each pair its
-// place, so src and dst ascend and no result depends on timing.  The keys are
-// read once, into shared memory, by one CTA, or by a cluster that adds its
-// counters up through distributed shared memory where one CTA would be slow.
-// Bound by the latency of that chain (lengths, table, weights, then six
+// Select.  A key's place in the order that the choice wants is one 64-bit
+// number: its weight as an ordered 32-bit number (guarded keys above all, a NaN
+// below all), then its index, the lowest first.  No two are equal, so the
+// keep-th greatest, T, splits the keys without a rule for ties.  It is found by
+// narrowing: the window from the least to the greatest is cut into 512 equal
+// bins, the bin that holds T becomes the window, until few enough candidates
+// are left to rank each against all.  (Weights are spread over exponents and
+// order like their bits, so the bins are filled evenly: two rounds, seldom
+// three.)  Then one running count in index order, of the places that become
+// free and of the keys that move, gives each pair its place, so src and dst
+// ascend and no result depends on timing.  The keys are read once, into shared
+// memory, by one CTA, or by a cluster that adds its counters up through
+// distributed shared memory where one CTA would be slow.
+// Bound by the latency of that chain (lengths, table, weights, then the
 // exchanges), not by its 8 bytes per key.
 // Measured: 32 requests x 8 heads of 2050 keys in 16.4 us, 4 x 8 of 11,000 to
 // 32,000 in 24.6.
@@ -38,6 +42,9 @@ constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
 constexpr int kMaxKeys = 40 * 1024;  // keys of a CTA in shared memory; more are read again in every round
 constexpr int kCtaKeys = 4096;       // keys of a CTA from which on more CTAs are taken
+constexpr int kBinBits = 9, kBins = 1 << kBinBits;
+static_assert(kBins == kThreads, "a bin per thread");
+constexpr int kCand = 128;           // candidates that are ranked one by one
 constexpr unsigned kGuarded = 0xffffffffu;
 
 struct SelectParams {
@@ -52,19 +59,24 @@ __device__ __forceinline__ unsigned ordered(float w) {
   return (u & 0x80000000u) != 0u ? ~u : u | 0x80000000u;
 }
 
-__global__ void __launch_bounds__(kThreads) fd_select_kernel(const __grid_constant__ SelectParams sp) {
+__global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_constant__ SelectParams sp) {
   const fd_select_args& a = sp.a;
+  typedef unsigned long long u64;
   extern __shared__ unsigned s_keys[];
-  __shared__ int hist[2][256];
-  __shared__ int sums[256];
-  __shared__ int found[2];                    // the round's digit, and how many are wanted of it
+  __shared__ int hist[2][kBins];
+  __shared__ u64 cand[kCand];
+  __shared__ unsigned ends[kMaxCluster][3];   // least key, greatest key, a bad block, of every CTA
+  __shared__ int cta_n[2][kMaxCluster];       // free places, moving keys of every CTA
+  __shared__ unsigned warp_u[3][kWarps];
   __shared__ int warp_n[2][kWarps];
-  __shared__ int cta_n[3][kMaxCluster];       // equals, free places, moving keys of every CTA
-  __shared__ int bad;
+  __shared__ int found[3];                    // the round's bin, the keys above it, the keys in it
+  __shared__ int taken;
+  __shared__ u64 s_T;
   cg::cluster_group cluster = cg::this_cluster();
   const int nct = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int unit = blockIdx.x / nct, KVH = a.num_kv_heads, r = unit / KVH, h = unit - r * KVH;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  if (nct > 1) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
   const int n = a.lens[r], keep = a.keep_lens[r], BS = a.block_size;
   auto sync = [&]() {
     if (nct > 1)
@@ -82,17 +94,18 @@ __global__ void __launch_bounds__(kThreads) fd_select_kernel(const __grid_consta
   }
   if (!ok || !cut || keep == 0) {
     if (rank == 0 && tid == 0) a.counts[unit] = 0;
+    if (nct > 1) cluster.barrier_wait();
     return;
   }
   const int per = ((n + nct - 1) / nct + 31) / 32 * 32;  // keys of a CTA
   const int lo = min(n, rank * per), hi = min(n, lo + per);
   const long long newest = (long long)n + (a.evicted != nullptr ? a.evicted[r] : 0) - a.recent;
   const int32_t* table = a.block_table + (int64_t)r * a.bt_stride;
-  auto load = [&](int j) -> unsigned {
+  auto load = [&](int j, unsigned& bad) -> unsigned {
     const int page = (int)((unsigned)j / (unsigned)BS);
     const int64_t id = table[page];
     if (id < 0 || id >= a.stats.num_blocks) {
-      bad = 1;
+      bad = 1u;
       return 0u;
     }
     const int64_t at = (id * KVH + h) * BS + (j - page * BS);
@@ -101,150 +114,180 @@ __global__ void __launch_bounds__(kThreads) fd_select_kernel(const __grid_consta
     return pos < a.sinks || pos >= newest ? kGuarded : ordered(w);
   };
   const bool kept = per <= sp.cap;
-  if (tid == 0) bad = 0;
-  for (int i = tid; i < 512; i += kThreads) hist[i >> 8][i & 255] = 0;
-  __syncthreads();
-  auto key = [&](int j) { return kept ? s_keys[j - lo] : load(j); };
-
-  unsigned T = 0u;   // the digits found so far
-  int want = keep;   // keys wanted of those that share them
-#pragma unroll 1
-  for (int round = 0; round < 4; ++round) {
-    const int sh = 24 - 8 * round;
-    int* const mine = hist[round & 1];
-    if (round == 0 && kept) {
+  unsigned least = 0xffffffffu, most = 0u, bad = 0u;
 #pragma unroll 4
-      for (int j = lo + tid; j < hi; j += kThreads) {
-        const unsigned k = load(j);
-        s_keys[j - lo] = k;
-        atomicAdd(&mine[k >> 24], 1);
-      }
-    } else {
-      for (int j = lo + tid; j < hi; j += kThreads) {
-        const unsigned k = key(j);
-        if (round == 0 || (k ^ T) >> (sh + 8) == 0u) atomicAdd(&mine[(k >> sh) & 255u], 1);
-      }
+  for (int j = lo + tid; j < hi; j += kThreads) {
+    const unsigned k = load(j, bad);
+    if (kept) s_keys[j - lo] = k;
+    least = min(least, k);
+    most = max(most, k);
+  }
+  auto key = [&](int j) {
+    unsigned ignored;
+    return kept ? s_keys[j - lo] : load(j, ignored);
+  };
+  auto place = [&](int j) { return (u64)key(j) << 32 | (0xffffffffu - (unsigned)j); };
+  least = __reduce_min_sync(0xffffffffu, least);
+  most = __reduce_max_sync(0xffffffffu, most);
+  bad = __reduce_or_sync(0xffffffffu, bad);
+  if (lane == 0) {
+    warp_u[0][warp] = least;
+    warp_u[1][warp] = most;
+    warp_u[2][warp] = bad;
+  }
+  for (int i = tid; i < 2 * kBins; i += kThreads) hist[i / kBins][i % kBins] = 0;
+  if (tid == 0) taken = 0;
+  __syncthreads();
+  if (nct > 1) cluster.barrier_wait();
+  if (warp == 0) {
+    const int w = lane % kWarps;
+    least = __reduce_min_sync(0xffffffffu, warp_u[0][w]);
+    most = __reduce_max_sync(0xffffffffu, warp_u[1][w]);
+    bad = __reduce_or_sync(0xffffffffu, warp_u[2][w]);
+    if (lane < nct) {
+      unsigned* to = cluster.map_shared_rank(&ends[rank][0], lane);
+      to[0] = least;
+      to[1] = most;
+      to[2] = bad;
     }
-    sync();
-    if (tid < 256) {
-      int s = 0;
-      for (int c = 0; c < nct; ++c) s += cluster.map_shared_rank(mine, c)[tid];
-      sums[tid] = s;
-      hist[(round + 1) & 1][tid] = 0;  // every CTA has read it: it was the last round's
+  }
+  sync();
+  least = 0xffffffffu;
+  most = bad = 0u;
+  for (int c = 0; c < nct; ++c) {
+    least = min(least, ends[c][0]);
+    most = max(most, ends[c][1]);
+    bad |= ends[c][2];
+  }
+  if (bad != 0u) {  // all threads of the cluster alike
+    if (rank == 0 && tid == 0) {
+      a.counts[unit] = 0;
+      set_error(a.error, FD_DEVERR_BLOCK_ID);
     }
-    if (round == 0) {
-      int any = 0;
-      for (int c = 0; c < nct; ++c) any |= *cluster.map_shared_rank(&bad, c);
-      if (any != 0) {  // all threads of the cluster alike
-        if (rank == 0 && tid == 0) {
-          a.counts[unit] = 0;
-          set_error(a.error, FD_DEVERR_BLOCK_ID);
-        }
-        sync();  // the others may still read this CTA's counters
-        return;
-      }
-    }
-    __syncthreads();
-    if (warp == 0) {  // lane x has digits 255 - 8 x down to 248 - 8 x
-      int c[8], s = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) s += c[i] = sums[255 - 8 * lane - i];
-      int above = s;
-#pragma unroll
-      for (int off = 1; off < 32; off <<= 1) {
-        const int o = __shfl_up_sync(0xffffffffu, above, off);
-        if (lane >= off) above += o;
-      }
-      above -= s;
-      if (above < want && want <= above + s) {  // one lane
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (above < want && want <= above + c[i]) {
-            found[0] = 255 - 8 * lane - i;
-            found[1] = want - above;
-          }
-          above += c[i];
-        }
-      }
-    }
-    __syncthreads();
-    T |= (unsigned)found[0] << sh;
-    want = found[1];
+    return;
   }
 
-  // Keys equal to T, in index order: a warp has a run of neighbours.
+  // the window [base, base + 2^bits) holds the want-th greatest of its keys
+  u64 base = (u64)least << 32, T;
+  int bits = 64 - __clzll((u64)(most - least) << 32 | 0xffffffffu), want = keep;
+#pragma unroll 1
+  for (int round = 0;; ++round) {
+    int* const mine = hist[round & 1];
+    const int sh = max(0, bits - kBinBits);
+    for (int j = lo + tid; j < hi; j += kThreads) {
+      const u64 x = place(j) - base;  // wraps below the window
+      if (bits == 64 || x >> bits == 0) atomicAdd(&mine[x >> sh], 1);
+    }
+    sync();
+    // bins from the greatest down, a thread each: those above, and the window's next
+    const int bin = kBins - 1 - tid;
+    int c = 0;
+    for (int x = 0; x < nct; ++x) c += cluster.map_shared_rank(mine, x)[bin];
+    int above = c;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, above, off);
+      if (lane >= off) above += o;
+    }
+    if (lane == 31) warp_n[0][warp] = above;
+    hist[(round + 1) & 1][bin] = 0;  // the last round's: every CTA has read it
+    __syncthreads();
+    above -= c;
+    for (int w = 0; w < warp; ++w) above += warp_n[0][w];
+    if (above < want && want <= above + c) {  // one thread
+      found[0] = bin;
+      found[1] = above;
+      found[2] = c;
+    }
+    __syncthreads();
+    const int at = found[0], m = found[2];
+    base += (u64)at << sh;
+    bits = sh;
+    want -= found[1];
+    if (want == m || bits == 0) {  // all of the window's (of one key alone, it)
+      T = base;
+      break;
+    }
+    if (m > kCand) continue;
+    // few: every CTA gets them all, and ranks them by itself
+    if (tid == 0) {
+      int ahead = 0;
+      for (int x = 0; x < rank; ++x) ahead += cluster.map_shared_rank(mine, x)[at];
+      taken = ahead;
+    }
+    __syncthreads();
+    for (int j = lo + tid; j < hi; j += kThreads) {
+      const u64 p = place(j);
+      if ((p - base) >> bits != 0) continue;
+      const int slot = atomicAdd(&taken, 1);
+      for (int x = 0; x < nct; ++x) cluster.map_shared_rank(cand, x)[slot] = p;
+    }
+    sync();
+    if (tid < m) {
+      const u64 p = cand[tid];
+      int greater = 0;
+#pragma unroll 8
+      for (int i = 0; i < m; ++i) greater += cand[i] > p;
+      if (greater == want - 1) s_T = p;
+    }
+    __syncthreads();
+    T = s_T;
+    break;
+  }
+
+  // Places that become free, and keys that move there, in index order: a warp
+  // has a run of neighbours.
   const int wper = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
   const int from = min(hi, lo + warp * wper), to = min(hi, from + wper);
   const unsigned below = (1u << lane) - 1u;
   int n0 = 0, n1 = 0;
-  for (int base = from; base < to; base += 32) {
-    const int j = base + lane;
-    n0 += __popc(__ballot_sync(0xffffffffu, j < to && key(j) == T));
-  }
-  if (lane == 0) warp_n[0][warp] = n0;
-  // Sum of the warps' counts k to every CTA, and this warp's own offset.
-  auto exchange = [&](int k, int slot) {
-    __syncthreads();
-    int all = 0, ahead = 0;
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) ahead += warp_n[k][w];
-      all += warp_n[k][w];
-    }
-    if (tid < nct) cluster.map_shared_rank(&cta_n[slot][0], tid)[rank] = all;
-    return ahead;
-  };
-  auto before = [&](int slot) {
-    int s = 0;
-    for (int c = 0; c < rank; ++c) s += cta_n[slot][c];
-    return s;
-  };
-  int eq = exchange(0, 0);
-  sync();
-  eq += before(0);
-  // places that become free, and keys that move there
-  const int eq0 = eq;
-  n0 = n1 = 0;
-  auto stays = [&](int j, int& equals) {  // all lanes together
-    const unsigned k = j < to ? key(j) : 0u;
-    const bool same = j < to && k == T;
-    const unsigned m = __ballot_sync(0xffffffffu, same);
-    const bool stay = j < to && (k > T || (same && equals + __popc(m & below) < want));
-    equals += __popc(m);
-    return stay;
-  };
-  for (int base = from; base < to; base += 32) {
-    const int j = base + lane;
-    const bool stay = stays(j, eq);
+  for (int b = from; b < to; b += 32) {
+    const int j = b + lane;
+    const bool stay = j < to && place(j) >= T;
     n0 += __popc(__ballot_sync(0xffffffffu, j < to && j < keep && !stay));
     n1 += __popc(__ballot_sync(0xffffffffu, j >= keep && stay));
   }
-  __syncthreads();  // warp_n has been read
   if (lane == 0) {
     warp_n[0][warp] = n0;
     warp_n[1][warp] = n1;
   }
-  int at0 = exchange(0, 1), at1 = exchange(1, 2);
+  __syncthreads();
+  int all0 = 0, all1 = 0;
+  n0 = n1 = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) {
+      n0 += warp_n[0][w];
+      n1 += warp_n[1][w];
+    }
+    all0 += warp_n[0][w];
+    all1 += warp_n[1][w];
+  }
+  if (tid < nct) {
+    cluster.map_shared_rank(&cta_n[0][0], tid)[rank] = all0;
+    cluster.map_shared_rank(&cta_n[1][0], tid)[rank] = all1;
+  }
   sync();
-  at0 += before(1);
-  at1 += before(2);
+  all0 = 0;
+  for (int c = 0; c < nct; ++c) {
+    if (c < rank) {
+      n0 += cta_n[0][c];
+      n1 += cta_n[1][c];
+    }
+    all0 += cta_n[0][c];
+  }
   int32_t* const dst = a.dst + (int64_t)unit * a.room;
   int32_t* const src = a.src + (int64_t)unit * a.room;
-  eq = eq0;
-  for (int base = from; base < to; base += 32) {
-    const int j = base + lane;
-    const bool stay = stays(j, eq);
+  for (int b = from; b < to; b += 32) {
+    const int j = b + lane;
+    const bool stay = j < to && place(j) >= T;
     const bool hole = j < to && j < keep && !stay, mover = j >= keep && stay;
     const unsigned m0 = __ballot_sync(0xffffffffu, hole), m1 = __ballot_sync(0xffffffffu, mover);
-    if (hole) dst[at0 + __popc(m0 & below)] = j;
-    if (mover) src[at1 + __popc(m1 & below)] = j;
-    at0 += __popc(m0);
-    at1 += __popc(m1);
+    if (hole) dst[n0 + __popc(m0 & below)] = j;
+    if (mover) src[n1 + __popc(m1 & below)] = j;
+    n0 += __popc(m0);
+    n1 += __popc(m1);
   }
-  if (rank == 0 && tid == 0) {
-    int s = 0;
-    for (int c = 0; c < nct; ++c) s += cta_n[1][c];
-    a.counts[unit] = s;
-  }
+  if (rank == 0 && tid == 0) a.counts[unit] = all0;
 }
 
 // ------------------------------------------------------------------ move

@@ -36,19 +36,18 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kUnroll = 4;  // vectors of each row that a thread has in flight
 
 struct VerifyParams {
   fd_verify_args a;
   int wide;  // rows are 16-byte aligned
 };
 
-__device__ __forceinline__ double as_double(float x) { return (double)x; }
-__device__ __forceinline__ double as_double(__half x) { return (double)__half2float(x); }
-__device__ __forceinline__ double as_double(__nv_bfloat16 x) { return (double)__bfloat162float(x); }
+__device__ __forceinline__ float as_float(float x) { return x; }
+__device__ __forceinline__ float as_float(__half x) { return __half2float(x); }
+__device__ __forceinline__ float as_float(__nv_bfloat16 x) { return __bfloat162float(x); }
 
-// A weight, or 0 where it is negative, infinite or a NaN.
-__device__ __forceinline__ double weight(double x) { return x > 0.0 && x < INFINITY ? x : 0.0; }
+// A probability, or 0 where it is negative, infinite or a NaN.
+__device__ __forceinline__ float prob(float x) { return x > 0.f && x < INFINITY ? x : 0.f; }
 
 __device__ __forceinline__ double warp_sum(double v) {
 #pragma unroll
@@ -56,13 +55,13 @@ __device__ __forceinline__ double warp_sum(double v) {
   return v;
 }
 
-// The weights of one vector: kV values from element i on of p and q (q null:
-// none; `struck`: the element that counts as 0).
+// The weights of a request's rows, a vector of kV values at a time.  Where x <=
+// y the weight is 0, which fp32 tells exactly; only the others become fp64.
 template <typename T, int kV>
 struct Rows {
   const T* p;
-  const T* q;
-  long long struck;
+  const T* q;        // null: none
+  long long struck;  // the element that counts as 0, or -1
   typedef typename std::conditional<kV == 1, T, uint4>::type Vec;
   __device__ __forceinline__ static Vec get(const T* at, long long i) {
     if constexpr (kV == 1)
@@ -70,47 +69,52 @@ struct Rows {
     else
       return __ldg(reinterpret_cast<const uint4*>(at + i));
   }
-  __device__ __forceinline__ void values(const Vec& v, double (&x)[kV]) const {
-    if constexpr (kV == 1) {
-      x[0] = as_double(v);
-    } else {
-      float f[kV];
-      Dt<T>::widen(v, f);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) x[e] = (double)f[e];
-    }
+  __device__ __forceinline__ static void values(const Vec& v, float (&x)[kV]) {
+    if constexpr (kV == 1)
+      x[0] = as_float(v);
+    else
+      Dt<T>::widen(v, x);
   }
-  // w[e], and the plain p[e]
-  __device__ __forceinline__ void weights(const Vec& vp, const Vec& vq, long long i, double (&w)[kV], double (&pl)[kV]) const {
-    double x[kV];
+  __device__ __forceinline__ static double over(float x, float y) {
+    x = prob(x);
+    y = prob(y);
+    return x > y ? (double)x - (double)y : 0.0;
+  }
+  // of the vector from element i on
+  __device__ __forceinline__ void weights(const Vec& vp, const Vec& vq, long long i, double (&w)[kV]) const {
+    float x[kV];
     values(vp, x);
-#pragma unroll
-    for (int e = 0; e < kV; ++e) pl[e] = w[e] = weight(x[e]);
     if (q != nullptr) {
-      double y[kV];
+      float y[kV];
       values(vq, y);
 #pragma unroll
-      for (int e = 0; e < kV; ++e) w[e] = weight(x[e] - weight(y[e]));
-    }
-    if (struck >= i && struck < i + kV) {
+      for (int e = 0; e < kV; ++e) w[e] = over(x[e], y[e]);
+    } else {
 #pragma unroll
-      for (int e = 0; e < kV; ++e)
-        if (i + e == struck) w[e] = 0.0;
+      for (int e = 0; e < kV; ++e) w[e] = i + e == struck ? 0.0 : (double)prob(x[e]);
     }
+  }
+  // of element i alone
+  __device__ __forceinline__ double weight(long long i) const {
+    return i == struck ? 0.0 : over(as_float(p[i]), q != nullptr ? as_float(q[i]) : 0.f);
   }
 };
 
 template <typename T, int kV>
-__global__ void __launch_bounds__(kThreads) fd_verify_kernel(const __grid_constant__ VerifyParams vp) {
+__global__ void __launch_bounds__(kThreads, 2) fd_verify_kernel(const __grid_constant__ VerifyParams vp) {
+  constexpr int kUnroll = kV == 8 ? 3 : 4;  // vectors of each row that a thread has in flight
   const fd_verify_args& a = vp.a;
   __shared__ int s_accepted;  // -1: no tokens
-  __shared__ double part[2][kMaxCluster];
-  __shared__ double warps[2][kWarps];
+  __shared__ double part[2][kMaxCluster];  // the CTAs' sums, of either attempt
+  __shared__ double warps[kWarps];
+  __shared__ double scan[kWarps];
+  __shared__ unsigned s_found[kWarps];
   cg::cluster_group cluster = cg::this_cluster();
   const int nct = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
   const int r = blockIdx.x / nct;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int K = a.num_drafts;
+  if (nct > 1) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
   const int qlen = a.q_len[r], qst = a.q_start[r];
 
   if (warp == 0) {  // the first draft that is not accepted
@@ -120,29 +124,31 @@ __global__ void __launch_bounds__(kThreads) fd_verify_kernel(const __grid_consta
       acc = -1;
       if (qlen != 0 && lane == 0 && rank == 0) set_error(a.error, FD_DEVERR_LEN);
     }
-    for (int base = 0; base < acc; base += 32) {
+    for (int base = 0; base < K; base += 32) {  // (the first tokens and numbers are fetched beside the lengths)
       const int d = base + lane;
       bool good = true;
-      if (d < qlen - 1) {
-        const long long x = a.draft_tokens[(int64_t)r * a.tokens_stride + d];
-        const float u = a.accept_u[(int64_t)r * a.accept_stride + d];
+      long long x = 0;
+      float u = 0.f;
+      if (d < K) {
+        x = a.draft_tokens[(int64_t)r * a.tokens_stride + d];
+        u = a.accept_u[(int64_t)r * a.accept_stride + d];
+      }
+      if (d < acc) {
         good = x >= 0 && x < a.vocab;
         if (good) {
-          const double p = weight(as_double(static_cast<const T*>(a.target)[(int64_t)(qst + d) * a.target_stride + x]));
-          const double q = a.draft_probs == nullptr
-                               ? 1.0
-                               : weight(as_double(static_cast<const T*>(a.draft_probs)[(int64_t)r * a.draft_stride_r +
-                                                                                       (int64_t)d * a.draft_stride_k + x]));
-          good = (double)u * q < p;
+          const float p = prob(as_float(static_cast<const T*>(a.target)[(int64_t)(qst + d) * a.target_stride + x]));
+          const float q = a.draft_probs == nullptr
+                              ? 1.f
+                              : prob(as_float(static_cast<const T*>(a.draft_probs)[(int64_t)r * a.draft_stride_r +
+                                                                                   (int64_t)d * a.draft_stride_k + x]));
+          good = (double)u * (double)q < (double)p;
         } else if (rank == 0) {
           set_error(a.error, FD_DEVERR_TOKEN);
         }
       }
       const unsigned bad = __ballot_sync(0xffffffffu, !good);
-      if (bad != 0u) {
-        acc = base + __ffs(bad) - 1;
-        break;
-      }
+      if (bad != 0u) acc = base + __ffs(bad) - 1;
+      if (bad != 0u || base + 32 >= acc) break;
     }
     if (lane == 0) s_accepted = acc;
   }
@@ -159,7 +165,10 @@ __global__ void __launch_bounds__(kThreads) fd_verify_kernel(const __grid_consta
       if (a.lens != nullptr) a.keep_lens[r] = none ? a.lens[r] : a.lens[r] - (qlen - 1 - acc);
     }
   }
-  if (none) return;
+  if (none) {
+    if (nct > 1) cluster.barrier_wait();
+    return;
+  }
 
   const bool rejected = acc < qlen - 1;
   const long long V = a.vocab;
@@ -172,108 +181,104 @@ __global__ void __launch_bounds__(kThreads) fd_verify_kernel(const __grid_consta
   typedef typename Rows<T, kV>::Vec Vec;
   // whole vectors of the row, cut into equal spans over the CTAs, then over
   // their warps; the elements behind the last whole vector (fewer than kV)
-  // belong to the last warp of the last CTA
+  // follow the last warp's of the last CTA
   const long long nvec = V / kV;
   const long long cta_lo = nvec * rank / nct, cta_n = nvec * (rank + 1) / nct - cta_lo;
-  const long long lo = cta_lo + cta_n * warp / kWarps, hi = cta_lo + cta_n * (warp + 1) / kWarps;
-  const bool tail = rank == nct - 1 && warp == kWarps - 1;
-  auto tail_weights = [&](int e, double& w, double& pl) {  // element e behind the last vector
-    const long long i = nvec * kV + e;
-    w = pl = 0.0;
-    if (i >= V) return;
-    const double x = as_double(rows.p[i]);
-    pl = weight(x);
-    w = rows.q != nullptr ? weight(x - weight(as_double(rows.q[i]))) : i == rows.struck ? 0.0 : pl;
-  };
-  double sw = 0.0, sp = 0.0;
-  for (long long base = lo; base < hi; base += 32 * kUnroll) {
-    Vec x[kUnroll], y[kUnroll];
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long i = base + 32 * u + lane;
-      if (i < hi) {
-        x[u] = Rows<T, kV>::get(rows.p, i * kV);
-        if (rows.q != nullptr) y[u] = Rows<T, kV>::get(rows.q, i * kV);
-      }
-    }
-#pragma unroll
-    for (int u = 0; u < kUnroll; ++u) {
-      const long long i = base + 32 * u + lane;
-      if (i >= hi) continue;
-      double w[kV], pl[kV];
-      rows.weights(x[u], y[u], i * kV, w, pl);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) {
-        sw += w[e];
-        sp += pl[e];
-      }
-    }
-  }
-  if (tail && lane < kV - 1) {
-    double w, pl;
-    tail_weights(lane, w, pl);
-    sw += w;
-    sp += pl;
-  }
-  sw = warp_sum(sw);
-  sp = warp_sum(sp);
-  if (lane == 0) {
-    warps[0][warp] = sw;
-    warps[1][warp] = sp;
-  }
-  __syncthreads();
-  if (nct > 1) cluster.sync();  // every CTA of the cluster has started
-  if (tid < 2 * nct) {
-    const int k = tid / nct, to = tid % nct;
+  const bool last_cta = rank == nct - 1;
+  const int ntail = last_cta ? (int)(V - nvec * kV) : 0;
+
+  double total = 0.0;
+  int attempt = 0;
+  for (;; ++attempt) {
+    const long long lo = cta_lo + cta_n * warp / kWarps, hi = cta_lo + cta_n * (warp + 1) / kWarps;
     double s = 0.0;
-    for (int w = 0; w < kWarps; ++w) s += warps[k][w];
-    cluster.map_shared_rank(&part[k][0], to)[rank] = s;
-  }
-  if (nct > 1)
-    cluster.sync();
-  else
+    for (long long base = lo; base < hi; base += 32 * kUnroll) {
+      Vec x[kUnroll], y[kUnroll];
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const long long i = base + 32 * u + lane;
+        if (i < hi) {
+          x[u] = Rows<T, kV>::get(rows.p, i * kV);
+          if (rows.q != nullptr) y[u] = Rows<T, kV>::get(rows.q, i * kV);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < kUnroll; ++u) {
+        const long long i = base + 32 * u + lane;
+        if (i >= hi) continue;
+        double w[kV];
+        rows.weights(x[u], y[u], i * kV, w);
+#pragma unroll
+        for (int e = 0; e < kV; ++e) s += w[e];
+      }
+    }
+    if (warp == kWarps - 1 && lane < ntail) s += rows.weight(nvec * kV + lane);
+    s = warp_sum(s);
+    if (lane == 0) warps[warp] = s;
     __syncthreads();
-  // All CTAs from the same numbers: the CTA that holds u times the sum.  It
-  // has a prefix <= target < prefix + its part, so its part is positive.
-  if (warp != 0) return;
-  double total = 0.0, total_p = 0.0;
-  for (int c = 0; c < nct; ++c) {
-    total += part[0][c];
-    total_p += part[1][c];
+    if (nct > 1 && attempt == 0) cluster.barrier_wait();
+    if (tid < nct) {
+      s = 0.0;
+      for (int w = 0; w < kWarps; ++w) s += warps[w];
+      cluster.map_shared_rank(&part[attempt][0], tid)[rank] = s;
+    }
+    if (nct > 1)
+      cluster.sync();
+    else
+      __syncthreads();
+    // all CTAs from the same numbers in the same order
+    total = 0.0;
+    for (int c = 0; c < nct; ++c) total += part[attempt][c];
+    if (total > 0.0 || attempt == 1) break;
+    rows.q = nullptr;  // nothing is left of p less q: p itself
+    rows.struck = -1;
   }
-  const int k = total > 0.0 ? 0 : 1;
-  if (k == 1) total = total_p;
-  if (!(total > 0.0) || !(total < INFINITY)) {
-    if (rank == 0 && lane == 0) {
+  if (!(total > 0.0)) {
+    if (rank == 0 && tid == 0) {
       a.tokens[(int64_t)r * (K + 1) + acc] = -1;
       set_error(a.error, FD_DEVERR_PROBS);
     }
     return;
   }
-  const float u = a.sample_u[r];
-  const double target = (double)fminf(fmaxf(u, 0.f), 0x1.fffffep-1f) * total;
+  // The CTA that holds u times the sum: it has a prefix <= target < prefix + its
+  // part, so its part is positive.
+  const double target = (double)fminf(fmaxf(a.sample_u[r], 0.f), 0x1.fffffep-1f) * total;
   double before = 0.0;
   int owner = 0;
-  while (owner < nct - 1 && !(target < before + part[k][owner])) before += part[k][owner++];
+  while (owner < nct - 1 && !(target < before + part[attempt][owner])) before += part[attempt][owner++];
   if (owner != rank) return;
-  // the warp's span: where rounding leaves no span past the target, the last
-  // one with any weight
-  int ws = -1;
-  double ws_before = before, run = before;
+  // the warp's span: where rounding leaves none past the target, the last one
+  // with any weight
+  int ws = 0;
+  double run = before, at_ws = before;
   for (int w = 0; w < kWarps; ++w) {
-    const double s = warps[k][w];
+    const double s = warps[w];
     if (!(s > 0.0)) continue;
     ws = w;
-    ws_before = run;
+    at_ws = run;
     run += s;
     if (target < run) break;
   }
-  if (ws < 0) return;  // (not reached: the CTA's part is positive)
-  const long long from = cta_lo + cta_n * ws / kWarps, to = cta_lo + cta_n * (ws + 1) / kWarps;
-  long long found = -1, last = -1;
-  run = ws_before;
-  auto step = [&](const double (&w)[kV], long long i) {  // the warp's next 32 vectors, in order
-    double s = 0.0;
+  // that span again, a vector per thread
+  const long long from = cta_lo + cta_n * ws / kWarps;
+  const long long to = cta_lo + cta_n * (ws + 1) / kWarps + (ws == kWarps - 1 && ntail > 0 ? 1 : 0);  // (the tail as a vector)
+  long long last = -1;  // the last element with weight so far
+  run = at_ws;
+  for (long long base = from; base < to; base += kThreads) {
+    const long long i = base + tid;
+    double w[kV], s = 0.0;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) w[e] = 0.0;
+    if (i < to && i < nvec) {
+      const Vec x = Rows<T, kV>::get(rows.p, i * kV);
+      Vec y{};
+      if (rows.q != nullptr) y = Rows<T, kV>::get(rows.q, i * kV);
+      rows.weights(x, y, i * kV, w);
+    } else if (i < to) {
+#pragma unroll
+      for (int e = 0; e < kV; ++e)
+        if (e < ntail) w[e] = rows.weight(nvec * kV + e);
+    }
 #pragma unroll
     for (int e = 0; e < kV; ++e) s += w[e];
     double incl = s;
@@ -282,57 +287,41 @@ __global__ void __launch_bounds__(kThreads) fd_verify_kernel(const __grid_consta
       const double o = __shfl_up_sync(0xffffffffu, incl, off);
       if (lane >= off) incl += o;
     }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    double ahead = run;
+    for (int x = 0; x < kWarps; ++x) {
+      if (x < warp) ahead += scan[x];
+      run += scan[x];
+    }
+    // threads with weight, of those the ones that pass the target
     const unsigned any = __ballot_sync(0xffffffffu, s > 0.0);
-    const unsigned past = __ballot_sync(0xffffffffu, s > 0.0 && target < run + incl);
-    const int pick = past != 0u ? __ffs(past) - 1 : any != 0u ? 31 - __clz(any) : -1;
-    if (pick >= 0) {  // the vector's first element past the target, or its last one with weight
-      double b = run + (incl - s);
-      long long at = -1;
-      bool done = false;
+    const unsigned past = __ballot_sync(0xffffffffu, s > 0.0 && target < ahead + incl);
+    if (lane == 0) s_found[warp] = past != 0u ? 64u + (unsigned)(__ffs(past) - 1) : any != 0u ? 32u + (31 - __clz(any)) : 0u;
+    __syncthreads();
+    int pick = -1;
+    bool done = false;
+    for (int x = 0; x < kWarps && !done; ++x) {
+      const unsigned f = s_found[x];
+      if (f != 0u) pick = 32 * x + (int)(f & 31u);
+      done = f >= 64u;
+    }
+    if (pick == tid) {  // the vector's first element past the target, or its last one with weight
+      double b = ahead + (incl - s);
+      bool hit = false;
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
         b += w[e];
-        if (!done && w[e] > 0.0) {
-          at = i + e;
-          done = target < b;
+        if (!hit && w[e] > 0.0) {
+          last = i * kV + e;
+          hit = target < b;
         }
       }
-      at = __shfl_sync(0xffffffffu, at, pick);
-      if (past != 0u)
-        found = at;
-      else
-        last = at;
+      a.tokens[(int64_t)r * (K + 1) + acc] = last;  // (a later pass with weight writes over it)
     }
-    run += __shfl_sync(0xffffffffu, incl, 31);
-  };
-  for (long long base = from; base < to && found < 0; base += 32) {
-    const long long i = base + lane;
-    double w[kV], pl[kV];
-#pragma unroll
-    for (int e = 0; e < kV; ++e) w[e] = pl[e] = 0.0;
-    if (i < to) {
-      const Vec x = Rows<T, kV>::get(rows.p, i * kV);
-      Vec y{};
-      if (rows.q != nullptr) y = Rows<T, kV>::get(rows.q, i * kV);
-      rows.weights(x, y, i * kV, w, pl);
-    }
-    if (k == 1) {
-#pragma unroll
-      for (int e = 0; e < kV; ++e) w[e] = pl[e];
-    }
-    step(w, i * kV);
+    if (done) return;
+    __syncthreads();  // scan and s_found have been read; the write above is ordered before the next one
   }
-  if (rank == nct - 1 && ws == kWarps - 1 && found < 0 && kV > 1) {
-    double w[kV];
-#pragma unroll
-    for (int e = 0; e < kV; ++e) {
-      double x = 0.0, pl = 0.0;
-      if (lane == 0 && e < kV - 1) tail_weights(e, x, pl);
-      w[e] = k == 1 ? pl : x;
-    }
-    step(w, nvec * kV);
-  }
-  if (lane == 0) a.tokens[(int64_t)r * (K + 1) + acc] = found >= 0 ? found : last;
 }
 
 template <typename T, int kV>
@@ -384,9 +373,12 @@ extern "C" int fd_verify_drafts(const fd_verify_args* a, void* stream) {
   auto aligned = [&](const void* p, int64_t stride) { return fdh::aligned16(p) && (stride * es) % 16 == 0; };
   vp.wide = aligned(a->target, a->target_stride) &&
             (vp.a.draft_probs == nullptr || (aligned(a->draft_probs, a->draft_stride_r) && (a->draft_stride_k * es) % 16 == 0));
-  // CTAs per request: all SMs twice over, each with 4096 values at least
+  // CTAs per request: no more than run at once (two per SM), each with 4096 values at least
+  int dev = 0, sms = 0;
+  const int st = fdh::device_sms(&dev, &sms);
+  if (st != FD_OK) return st;
   int ctas = 1;
-  while (ctas < kMaxCluster && (int64_t)ctas * a->num_reqs < 296 && (int64_t)a->vocab > (int64_t)ctas * 4096) ctas *= 2;
+  while (ctas < kMaxCluster && 2 * (int64_t)ctas * a->num_reqs <= 2 * sms && (int64_t)a->vocab > (int64_t)ctas * 4096) ctas *= 2;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (a->dtype) {
     case FD_DTYPE_F16:
