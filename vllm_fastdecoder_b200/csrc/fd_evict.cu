@@ -5,15 +5,15 @@
 // number: its weight as an ordered 32-bit number (guarded keys above all, a NaN
 // below all), then its index, the lowest first.  No two are equal, so the
 // keep-th greatest, T, splits the keys without a rule for ties.  It is found by
-// narrowing: the window from the least to the greatest is cut into 512 equal
-// bins, the bin that holds T becomes the window, until few enough candidates
-// are left to rank each against all.  (Weights are spread over exponents and
-// order like their bits, so the bins are filled evenly: two rounds, seldom
-// three.)  Then one running count in index order, of the places that become
+// narrowing: a window, at first of all 64-bit numbers, is cut into 512 equal
+// bins, and the bin that holds T becomes the window, until few enough candidates
+// are left to rank each against all.  The first round tells exponents apart, the
+// second nine more bits; a third is seldom needed.  Then one running count in
+// index order, of the places that become
 // free and of the keys that move, gives each pair its place, so src and dst
-// ascend and no result depends on timing.  The keys are read once, into shared
-// memory, by one CTA, or by a cluster that adds its counters up through
-// distributed shared memory where one CTA would be slow.
+// ascend and no result depends on timing.  The keys are read once and stay in
+// registers (in shared memory where a CTA has more than 4096), in one CTA, or
+// in a cluster that adds its counters up through distributed shared memory.
 // Bound by the latency of that chain (lengths, table, weights, then the
 // exchanges), not by its 8 bytes per key.
 // Measured: 32 requests x 8 heads of 2050 keys in 16.4 us, 4 x 8 of 11,000 to
@@ -40,16 +40,18 @@ namespace cg = cooperative_groups;
 constexpr int kThreads = 512;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int kMaxKeys = 40 * 1024;  // keys of a CTA in shared memory; more are read again in every round
-constexpr int kCtaKeys = 4096;       // keys of a CTA from which on more CTAs are taken
+constexpr int kPer = 8;                   // keys of a thread:
+constexpr int kTile = kThreads * kPer;    // a CTA of one tile keeps them in registers
+constexpr int kMaxKeys = 40 * 1024;       // keys of a CTA of several tiles in shared memory; more are read again in every pass
 constexpr int kBinBits = 9, kBins = 1 << kBinBits;
 static_assert(kBins == kThreads, "a bin per thread");
-constexpr int kCand = 128;           // candidates that are ranked one by one
+constexpr int kCand = kThreads / 4;       // candidates that are ranked one by one
 constexpr unsigned kGuarded = 0xffffffffu;
 
 struct SelectParams {
   fd_select_args a;
-  int cap;  // keys that fit the CTA's shared memory
+  int cap;  // keys that fit the CTA's shared memory (several tiles)
+  int sh;   // log2 of the block size, or -1
 };
 
 // Weights in order as unsigned numbers: -0 equals 0, a NaN is below all.
@@ -59,30 +61,41 @@ __device__ __forceinline__ unsigned ordered(float w) {
   return (u & 0x80000000u) != 0u ? ~u : u | 0x80000000u;
 }
 
+template <bool kMany>  // several CTAs per request and head
 __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_constant__ SelectParams sp) {
   const fd_select_args& a = sp.a;
   typedef unsigned long long u64;
   extern __shared__ unsigned s_keys[];
-  __shared__ int hist[2][kBins];
-  __shared__ u64 cand[kCand];
-  __shared__ unsigned ends[kMaxCluster][3];   // least key, greatest key, a bad block, of every CTA
-  __shared__ int cta_n[2][kMaxCluster];       // free places, moving keys of every CTA
-  __shared__ unsigned warp_u[3][kWarps];
+  __shared__ int hist[kBins];                 // of the CTA's own keys
+  // Of the cluster's: a CTA adds its bins that are not empty to every CTA's copy
+  // (few; reading all of every other's took 5000 cycles a round).  Three take
+  // turns: the next round's is clean before any CTA can write to it.
+  __shared__ int whole[kMany ? 3 : 1][kMany ? kBins : 1];
+  __shared__ u64 cand[kMany ? kMaxCluster : 1][kCand];  // of every CTA,
+  __shared__ int cand_n[kMaxCluster];                   // and how many
+  __shared__ int cta_n[kMaxCluster][2];       // free places, moving keys of every CTA
   __shared__ int warp_n[2][kWarps];
+  __shared__ __align__(16) int counts[kPer * kWarps];  // of 32 keys each, in index order: free places, moving keys << 16
   __shared__ int found[3];                    // the round's bin, the keys above it, the keys in it
-  __shared__ int taken;
+  __shared__ int taken, any_bad;
   __shared__ u64 s_T;
   cg::cluster_group cluster = cg::this_cluster();
-  const int nct = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  const int nct = kMany ? (int)cluster.num_blocks() : 1, rank = kMany ? (int)cluster.block_rank() : 0;
   const int unit = blockIdx.x / nct, KVH = a.num_kv_heads, r = unit / KVH, h = unit - r * KVH;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (nct > 1) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
+  if constexpr (kMany) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
   const int n = a.lens[r], keep = a.keep_lens[r], BS = a.block_size;
   auto sync = [&]() {
-    if (nct > 1)
+    if constexpr (kMany)
       cluster.sync();
     else
       __syncthreads();
+  };
+  auto at_rank = [&](auto* p, int c) {  // CTA c's copy of a shared variable
+    if constexpr (kMany)
+      return cluster.map_shared_rank(p, c);
+    else
+      return p;
   };
 
   // the whole cluster alike
@@ -92,97 +105,122 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
     if (rank == 0 && tid == 0) set_error(a.error, FD_DEVERR_LEN);
     ok = false;
   }
+  if (ok && cut && a.stats.num_blocks == 0) {
+    if (rank == 0 && tid == 0) set_error(a.error, FD_DEVERR_BLOCK_ID);
+    ok = false;
+  }
   if (!ok || !cut || keep == 0) {
     if (rank == 0 && tid == 0) a.counts[unit] = 0;
-    if (nct > 1) cluster.barrier_wait();
+    if constexpr (kMany) cluster.barrier_wait();
     return;
   }
-  const int per = ((n + nct - 1) / nct + 31) / 32 * 32;  // keys of a CTA
-  const int lo = min(n, rank * per), hi = min(n, lo + per);
-  const long long newest = (long long)n + (a.evicted != nullptr ? a.evicted[r] : 0) - a.recent;
+  const int span = ((n + nct - 1) / nct + 31) / 32 * 32;  // keys of a CTA
+  const int lo = min(n, rank * span), hi = min(n, lo + span);
+  // positions from here on are guarded (its bounds are int32's)
+  const int newest = (int)min(max((long long)n + (a.evicted != nullptr ? a.evicted[r] : 0) - a.recent, -0x80000000ll), 0x7fffffffll);
   const int32_t* table = a.block_table + (int64_t)r * a.bt_stride;
-  auto load = [&](int j, unsigned& bad) -> unsigned {
-    const int page = (int)((unsigned)j / (unsigned)BS);
-    const int64_t id = table[page];
-    if (id < 0 || id >= a.stats.num_blocks) {
-      bad = 1u;
-      return 0u;
+  const unsigned nblk = (unsigned)(a.stats.num_blocks < 0x7fffffff ? a.stats.num_blocks : 0x7fffffff);
+  const int line = KVH * BS, row0 = h * BS;
+  unsigned bad = 0u;
+  // The thread's keys of the tile from t0 on: t0 + u kThreads + tid.
+  unsigned k[kPer];
+  auto load = [&](int t0) {
+    // a level at a time: all its loads are under way before the first is used
+    int id[kPer], off[kPer], pos[kPer];
+    float w[kPer];
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (t0 + u * kThreads >= hi) break;  // the CTA alike
+      const int j = t0 + u * kThreads + tid;
+      const int page = sp.sh >= 0 ? j >> sp.sh : (int)((unsigned)j / (unsigned)BS);
+      off[u] = row0 + j - page * BS;
+      id[u] = j < hi ? table[page] : 0;
     }
-    const int64_t at = (id * KVH + h) * BS + (j - page * BS);
-    const float w = a.stats.weights[at];
-    const int pos = a.stats.positions[at];
-    return pos < a.sinks || pos >= newest ? kGuarded : ordered(w);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (t0 + u * kThreads >= hi) break;
+      const bool in = t0 + u * kThreads + tid < hi, have = (unsigned)id[u] < nblk;
+      const int64_t at = in && have ? (int64_t)id[u] * line + off[u] : 0;
+      w[u] = a.stats.weights[at];
+      pos[u] = a.stats.positions[at];
+      bad |= in && !have ? 1u : 0u;
+    }
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (t0 + u * kThreads >= hi) break;
+      k[u] = pos[u] < a.sinks || pos[u] >= newest ? kGuarded : ordered(w[u]);
+    }
   };
-  const bool kept = per <= sp.cap;
-  unsigned least = 0xffffffffu, most = 0u, bad = 0u;
-#pragma unroll 4
-  for (int j = lo + tid; j < hi; j += kThreads) {
-    const unsigned k = load(j, bad);
-    if (kept) s_keys[j - lo] = k;
-    least = min(least, k);
-    most = max(most, k);
-  }
-  auto key = [&](int j) {
-    unsigned ignored;
-    return kept ? s_keys[j - lo] : load(j, ignored);
+  const bool one = hi - lo <= kTile, kept = hi - lo <= sp.cap;
+  auto fetch = [&](int t0) {  // again, for a pass over several tiles
+    if (one) return;
+    if (!kept) return load(t0);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      const int j = t0 + u * kThreads + tid;
+      if (j < hi) k[u] = s_keys[j - lo];
+    }
   };
-  auto place = [&](int j) { return (u64)key(j) << 32 | (0xffffffffu - (unsigned)j); };
-  least = __reduce_min_sync(0xffffffffu, least);
-  most = __reduce_max_sync(0xffffffffu, most);
-  bad = __reduce_or_sync(0xffffffffu, bad);
-  if (lane == 0) {
-    warp_u[0][warp] = least;
-    warp_u[1][warp] = most;
-    warp_u[2][warp] = bad;
-  }
-  for (int i = tid; i < 2 * kBins; i += kThreads) hist[i / kBins][i % kBins] = 0;
-  if (tid == 0) taken = 0;
+  // body(key, j) for the CTA's keys
+  auto each = [&](int t0, auto&& body) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if (t0 + u * kThreads >= hi) break;
+      const int j = t0 + u * kThreads + tid;
+      if (j < hi) body(k[u], j);
+    }
+  };
+  if (tid == 0) taken = any_bad = 0;
+  hist[tid] = 0;
+  if constexpr (kMany) whole[0][tid] = whole[1][tid] = whole[2][tid] = 0;
   __syncthreads();
-  if (nct > 1) cluster.barrier_wait();
-  if (warp == 0) {
-    const int w = lane % kWarps;
-    least = __reduce_min_sync(0xffffffffu, warp_u[0][w]);
-    most = __reduce_max_sync(0xffffffffu, warp_u[1][w]);
-    bad = __reduce_or_sync(0xffffffffu, warp_u[2][w]);
-    if (lane < nct) {
-      unsigned* to = cluster.map_shared_rank(&ends[rank][0], lane);
-      to[0] = least;
-      to[1] = most;
-      to[2] = bad;
-    }
+  for (int t0 = lo; t0 < hi; t0 += kTile) {
+    load(t0);
+    each(t0, [&](unsigned x, int j) {
+      if (!one && kept) s_keys[j - lo] = x;
+      atomicAdd(&hist[x >> (32 - kBinBits)], 1);  // the first round's bins
+    });
   }
-  sync();
-  least = 0xffffffffu;
-  most = bad = 0u;
-  for (int c = 0; c < nct; ++c) {
-    least = min(least, ends[c][0]);
-    most = max(most, ends[c][1]);
-    bad |= ends[c][2];
-  }
-  if (bad != 0u) {  // all threads of the cluster alike
-    if (rank == 0 && tid == 0) {
-      a.counts[unit] = 0;
-      set_error(a.error, FD_DEVERR_BLOCK_ID);
-    }
-    return;
-  }
+  if constexpr (kMany) cluster.barrier_wait();
+  if (bad != 0u)
+    for (int c = 0; c < nct; ++c) *at_rank(&any_bad, c) = 1;
 
-  // the window [base, base + 2^bits) holds the want-th greatest of its keys
-  u64 base = (u64)least << 32, T;
-  int bits = 64 - __clzll((u64)(most - least) << 32 | 0xffffffffu), want = keep;
+  auto place = [](unsigned x, int j) { return (u64)x << 32 | (0xffffffffu - (unsigned)j); };
+  // the window [base, base + 2^bits) holds the want-th greatest of its places
+  u64 base = 0ull, T;
+  int bits = 64, want = keep;
 #pragma unroll 1
   for (int round = 0;; ++round) {
-    int* const mine = hist[round & 1];
     const int sh = max(0, bits - kBinBits);
-    for (int j = lo + tid; j < hi; j += kThreads) {
-      const u64 x = place(j) - base;  // wraps below the window
-      if (bits == 64 || x >> bits == 0) atomicAdd(&mine[x >> sh], 1);
+    if (round > 0) {  // (its own counters have been read: two barriers ago)
+      hist[tid] = 0;
+      __syncthreads();
+      for (int t0 = lo; t0 < hi; t0 += kTile) {
+        fetch(t0);
+        each(t0, [&](unsigned x, int j) {
+          const u64 y = place(x, j) - base;  // wraps below the window
+          if (y >> bits == 0) atomicAdd(&hist[y >> sh], 1);
+        });
+      }
     }
-    sync();
-    // bins from the greatest down, a thread each: those above, and the window's next
+    __syncthreads();
+    // bins from the greatest down, a thread each: the keys above them, and theirs
     const int bin = kBins - 1 - tid;
-    int c = 0;
-    for (int x = 0; x < nct; ++x) c += cluster.map_shared_rank(mine, x)[bin];
+    int c = hist[bin];
+    if constexpr (kMany) {
+      if (c > 0)
+        for (int x = 0; x < nct; ++x) atomicAdd(cluster.map_shared_rank(&whole[round % 3][bin], x), c);
+      cluster.sync();
+      c = whole[round % 3][bin];
+      whole[(round + 2) % 3][bin] = 0;
+    }
+    if (round == 0 && any_bad != 0) {  // all threads of the cluster alike
+      if (rank == 0 && tid == 0) {
+        a.counts[unit] = 0;
+        set_error(a.error, FD_DEVERR_BLOCK_ID);
+      }
+      return;
+    }
     int above = c;
 #pragma unroll
     for (int off = 1; off < 32; off <<= 1) {
@@ -190,104 +228,164 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
       if (lane >= off) above += o;
     }
     if (lane == 31) warp_n[0][warp] = above;
-    hist[(round + 1) & 1][bin] = 0;  // the last round's: every CTA has read it
     __syncthreads();
-    above -= c;
-    for (int w = 0; w < warp; ++w) above += warp_n[0][w];
+    above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_n[0][lane] : 0) - c;
     if (above < want && want <= above + c) {  // one thread
       found[0] = bin;
       found[1] = above;
       found[2] = c;
     }
     __syncthreads();
-    const int at = found[0], m = found[2];
-    base += (u64)at << sh;
+    const int m = found[2];
+    base += (u64)found[0] << sh;
     bits = sh;
     want -= found[1];
     if (want == m || bits == 0) {  // all of the window's (of one key alone, it)
       T = base;
       break;
     }
-    if (m > kCand) continue;
-    // few: every CTA gets them all, and ranks them by itself
-    if (tid == 0) {
-      int ahead = 0;
-      for (int x = 0; x < rank; ++x) ahead += cluster.map_shared_rank(mine, x)[at];
-      taken = ahead;
+    if (m > kCand || (kMany && bits > 32)) continue;
+    // few: every CTA gets them all, and ranks them by itself (in a cluster another round costs half of that, and as a
+    // rule tells keys of different weights apart)
+    for (int t0 = lo; t0 < hi; t0 += kTile) {
+      fetch(t0);
+      unsigned who[kPer];
+      int mine = 0;
+      const unsigned base_key = (unsigned)(base >> 32);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        who[u] = 0u;
+        if (t0 + u * kThreads >= hi) continue;  // the CTA alike
+        const int j = t0 + u * kThreads + tid;
+        const bool in = bits >= 32 ? (k[u] - base_key) >> (bits - 32) == 0u : (place(k[u], j) - base) >> bits == 0;
+        who[u] = __ballot_sync(0xffffffffu, in && j < hi);
+        mine += __popc(who[u]);
+      }
+      if (mine == 0) continue;
+      int slot = 0;
+      if (lane == 0) slot = atomicAdd(&taken, mine);
+      slot = __shfl_sync(0xffffffffu, slot, 0);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        if (who[u] == 0u) continue;
+        if ((who[u] >> lane) & 1u) {
+          const int to = slot + __popc(who[u] & ((1u << lane) - 1u));
+          for (int x = 0; x < nct; ++x) at_rank(&cand[rank][0], x)[to] = place(k[u], t0 + u * kThreads + tid);
+        }
+        slot += __popc(who[u]);
+      }
     }
     __syncthreads();
-    for (int j = lo + tid; j < hi; j += kThreads) {
-      const u64 p = place(j);
-      if ((p - base) >> bits != 0) continue;
-      const int slot = atomicAdd(&taken, 1);
-      for (int x = 0; x < nct; ++x) cluster.map_shared_rank(cand, x)[slot] = p;
-    }
+    if (tid < nct) *at_rank(&cand_n[rank], tid) = taken;
     sync();
-    if (tid < m) {
-      const u64 p = cand[tid];
+    if (warp < (m + 7) / 8) {  // four threads per candidate
+      int x = tid >> 2, of = 0;
+      while (of < nct && x >= cand_n[of]) x -= cand_n[of++];
+      const u64 y = of < nct ? cand[of][x] : ~0ull;
       int greater = 0;
-#pragma unroll 8
-      for (int i = 0; i < m; ++i) greater += cand[i] > p;
-      if (greater == want - 1) s_T = p;
+      for (int q = 0; q < nct; ++q) {
+        const int many = cand_n[q];
+#pragma unroll 4
+        for (int i = tid & 3; i < many; i += 4) greater += cand[q][i] > y ? 1 : 0;
+      }
+      greater += __shfl_xor_sync(0xffffffffu, greater, 1);
+      greater += __shfl_xor_sync(0xffffffffu, greater, 2);
+      if (of < nct && greater == want - 1) s_T = y;
     }
     __syncthreads();
     T = s_T;
     break;
   }
 
-  // Places that become free, and keys that move there, in index order: a warp
-  // has a run of neighbours.
-  const int wper = ((hi - lo + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int from = min(hi, lo + warp * wper), to = min(hi, from + wper);
-  const unsigned below = (1u << lane) - 1u;
-  int n0 = 0, n1 = 0;
-  for (int b = from; b < to; b += 32) {
-    const int j = b + lane;
-    const bool stay = j < to && place(j) >= T;
-    n0 += __popc(__ballot_sync(0xffffffffu, j < to && j < keep && !stay));
-    n1 += __popc(__ballot_sync(0xffffffffu, j >= keep && stay));
-  }
-  if (lane == 0) {
-    warp_n[0][warp] = n0;
-    warp_n[1][warp] = n1;
-  }
-  __syncthreads();
-  int all0 = 0, all1 = 0;
-  n0 = n1 = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) {
-      n0 += warp_n[0][w];
-      n1 += warp_n[1][w];
+  // Places that become free, and keys that move there, in index order.
+  const unsigned T_key = (unsigned)(T >> 32), T_j = 0xffffffffu - (unsigned)T;
+  auto stays = [&](unsigned x, int j) { return x > T_key || (x == T_key && (unsigned)j <= T_j); };
+  unsigned hole[kPer], mover[kPer];  // the warp's 32 keys of each
+  auto look = [&](int t0) {
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      hole[u] = mover[u] = 0u;
+      if (t0 + u * kThreads >= hi) continue;  // the CTA alike
+      const int j = t0 + u * kThreads + tid;
+      const bool in = j < hi, stay = in && stays(k[u], j);
+      hole[u] = __ballot_sync(0xffffffffu, in && !stay && j < keep);
+      mover[u] = __ballot_sync(0xffffffffu, stay && j >= keep);
     }
-    all0 += warp_n[0][w];
-    all1 += warp_n[1][w];
-  }
-  if (tid < nct) {
-    cluster.map_shared_rank(&cta_n[0][0], tid)[rank] = all0;
-    cluster.map_shared_rank(&cta_n[1][0], tid)[rank] = all1;
-  }
-  sync();
-  all0 = 0;
-  for (int c = 0; c < nct; ++c) {
-    if (c < rank) {
-      n0 += cta_n[0][c];
-      n1 += cta_n[1][c];
+  };
+  int at0 = 0, at1 = 0;  // pairs ahead of this CTA
+  if constexpr (kMany) {
+    int n0 = 0, n1 = 0;
+    for (int t0 = lo; t0 < hi; t0 += kTile) {
+      fetch(t0);
+      look(t0);
+#pragma unroll
+      for (int u = 0; u < kPer; ++u) {
+        n0 += __popc(hole[u]);
+        n1 += __popc(mover[u]);
+      }
     }
-    all0 += cta_n[0][c];
+    if (lane == 0) {
+      warp_n[0][warp] = n0;
+      warp_n[1][warp] = n1;
+    }
+    __syncthreads();
+    n0 = __reduce_add_sync(0xffffffffu, lane < kWarps ? warp_n[0][lane] : 0);
+    n1 = __reduce_add_sync(0xffffffffu, lane < kWarps ? warp_n[1][lane] : 0);
+    if (tid < nct) {
+      int* to = cluster.map_shared_rank(&cta_n[rank][0], tid);
+      to[0] = n0;
+      to[1] = n1;
+    }
+    cluster.sync();
+    int all = 0;
+    for (int c = 0; c < nct; ++c) {
+      if (c < rank) {
+        at0 += cta_n[c][0];
+        at1 += cta_n[c][1];
+      }
+      all += cta_n[c][0];
+    }
+    if (rank == 0 && tid == 0) a.counts[unit] = all;
   }
   int32_t* const dst = a.dst + (int64_t)unit * a.room;
   int32_t* const src = a.src + (int64_t)unit * a.room;
-  for (int b = from; b < to; b += 32) {
-    const int j = b + lane;
-    const bool stay = j < to && place(j) >= T;
-    const bool hole = j < to && j < keep && !stay, mover = j >= keep && stay;
-    const unsigned m0 = __ballot_sync(0xffffffffu, hole), m1 = __ballot_sync(0xffffffffu, mover);
-    if (hole) dst[n0 + __popc(m0 & below)] = j;
-    if (mover) src[n1 + __popc(m1 & below)] = j;
-    n0 += __popc(m0);
-    n1 += __popc(m1);
+  const unsigned below = (1u << lane) - 1u;
+  for (int t0 = lo; t0 < hi; t0 += kTile) {
+    fetch(t0);
+    look(t0);
+    // a running sum over the tile's groups of 32: group 16 u + warp is this warp's u-th
+    int mine = 0;
+#pragma unroll
+    for (int u = 0; u < kPer; ++u)
+      if (lane == u) mine = __popc(hole[u]) | __popc(mover[u]) << 16;
+    if (t0 > lo) __syncthreads();  // the last tile's counts have been read
+    if (lane < kPer) counts[lane * kWarps + warp] = mine;
+    __syncthreads();
+    const int4 c = reinterpret_cast<const int4*>(counts)[lane];
+    const int own = c.x + c.y + c.z + c.w;
+    int incl = own;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
+    }
+    const int x = warp & 3;  // of the lane's four groups, the one that a warp with these low bits has
+    const int ahead = incl - own + (x > 0 ? c.x : 0) + (x > 1 ? c.y : 0) + (x > 2 ? c.z : 0);
+#pragma unroll
+    for (int u = 0; u < kPer; ++u) {
+      if ((hole[u] | mover[u]) == 0u) continue;  // the warp alike
+      const int p = __shfl_sync(0xffffffffu, ahead, (u * kWarps + warp) >> 2);
+      const int j = t0 + u * kThreads + tid;
+      if ((hole[u] >> lane) & 1u) dst[at0 + (p & 0xffff) + __popc(hole[u] & below)] = j;
+      if ((mover[u] >> lane) & 1u) src[at1 + (p >> 16) + __popc(mover[u] & below)] = j;
+    }
+    const int total = __shfl_sync(0xffffffffu, incl, 31);
+    at0 += total & 0xffff;
+    at1 += total >> 16;
   }
-  if (rank == 0 && tid == 0) a.counts[unit] = all0;
+  if constexpr (!kMany) {
+    if (tid == 0) a.counts[unit] = at0;
+  }
 }
 
 // ------------------------------------------------------------------ move
@@ -398,8 +496,8 @@ extern "C" int fd_select_keys(const fd_select_args* a, void* stream) {
   if (a->bt_width <= 0 || a->bt_stride < 0)
     return fdh::fail(FD_ERR_INVALID, "fd_select_keys: bt_width must be positive, bt_stride not negative");
   const int64_t most = (int64_t)a->bt_width * a->block_size;
-  if (most > 0x7fffffff - 512)
-    return fdh::fail(FD_ERR_UNSUPPORTED, "fd_select_keys: bt_width * block_size must fit int32");
+  if (most > 0x7fffffff - 2 * kTile || (int64_t)a->num_kv_heads * a->block_size > 0x7fffffff)
+    return fdh::fail(FD_ERR_UNSUPPORTED, "fd_select_keys: bt_width * block_size and num_kv_heads * block_size must fit int32");
   if (a->block_table == nullptr || a->lens == nullptr || a->keep_lens == nullptr || a->counts == nullptr ||
       (a->stats.num_blocks > 0 && (a->stats.weights == nullptr || a->stats.positions == nullptr)) ||
       (a->room > 0 && (a->src == nullptr || a->dst == nullptr)))
@@ -407,14 +505,18 @@ extern "C" int fd_select_keys(const fd_select_args* a, void* stream) {
   const int64_t len = a->max_len > 0 && a->max_len < most ? a->max_len : most;
   const int64_t units = (int64_t)a->num_reqs * a->num_kv_heads;
   int ctas = 1;
-  while (ctas < kMaxCluster && units * ctas < 296 && len > (int64_t)ctas * kCtaKeys) ctas *= 2;
+  while (ctas < kMaxCluster && units * ctas < 296 && len > (int64_t)ctas * kTile) ctas *= 2;
   SelectParams sp;
   sp.a = *a;
   const int64_t per = ((len + ctas - 1) / ctas + 31) / 32 * 32;
-  sp.cap = (int)(per < kMaxKeys ? per : kMaxKeys);
-  static unsigned long long done = 0;
-  const void* kern = reinterpret_cast<const void*>(fd_select_kernel);
-  const int st = fdh::ensure_smem(kern, kMaxKeys * 4, &done);
+  sp.cap = per <= kTile ? 0 : (int)(per < kMaxKeys ? per : kMaxKeys);
+  sp.sh = -1;
+  for (int sh = 0; sh < 31; ++sh)
+    if (a->block_size == 1 << sh) sp.sh = sh;
+  static unsigned long long done[2] = {0, 0};
+  const void* kern = ctas > 1 ? reinterpret_cast<const void*>(fd_select_kernel<true>)
+                              : reinterpret_cast<const void*>(fd_select_kernel<false>);
+  const int st = fdh::ensure_smem(kern, kMaxKeys * 4, &done[ctas > 1 ? 1 : 0]);
   if (st != FD_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(units * ctas));
