@@ -878,8 +878,9 @@ typedef struct fd_key_weights_args {
 
 FD_API int fd_key_weights(const fd_key_weights_args *a, void *stream);
 
-/* Scratch bytes of fd_key_weights for these arguments (see
- * fd_attn_workspace_size). */
+/* Scratch bytes of fd_key_weights for these arguments (reads the sizes, the
+ * bounds, and what fd_attn_workspace_size reads; often 0).  Pure host
+ * arithmetic, on the current device's number of SMs. */
 FD_API size_t fd_key_weights_workspace_size(const fd_key_weights_args *a);
 
 /* sizeof(fd_key_weights_args) as compiled into the library (binding check). */

@@ -657,7 +657,7 @@ bool encode_lines(CUtensorMap* m, const void* base, int dtype, int BS, int64_t l
   return encode_map(m, base, dtype, 5, dims, strides, box);
 }
 
-void encode_maps(MmaParams& mp, const fd_attn_args* a) {
+void encode_maps(MmaParams& mp, const fd_attn_args* a, bool k_only) {
   const AttnParams& p = mp.a;
   const int D = p.D;
   mp.box_sh = 3;
@@ -689,11 +689,11 @@ void encode_maps(MmaParams& mp, const fd_attn_args* a) {
         return encode_lines(m, base, a->dtype, p.BS, (p.nblk[t] - 1) * mp.lines[t] + p.KVH, p.head_sb[t], p.tok_sb[t],
                             1 << mp.box_sh);
       };
-      mp.kv_tma[t] = lines(&mp.tmap_k[t], p.k[t]) && lines(&mp.tmap_v[t], p.v[t]);
+      mp.kv_tma[t] = lines(&mp.tmap_k[t], p.k[t]) && (k_only || lines(&mp.tmap_v[t], p.v[t]));
     } else {
-      mp.kv_tma[t] = map(&mp.tmap_k[t], p.k[t], 1 << mp.box_sh) && map(&mp.tmap_v[t], p.v[t], 1 << mp.box_sh);
+      mp.kv_tma[t] = map(&mp.tmap_k[t], p.k[t], 1 << mp.box_sh) && (k_only || map(&mp.tmap_v[t], p.v[t], 1 << mp.box_sh));
     }
-    if (mp.box_sh > kFineSh) mp.kv_tma[t] = mp.kv_tma[t] && map(&mp.tmap_vf[t], p.v[t], kFine);
+    if (mp.box_sh > kFineSh && !k_only) mp.kv_tma[t] = mp.kv_tma[t] && map(&mp.tmap_vf[t], p.v[t], kFine);
   }
 }
 

@@ -333,9 +333,9 @@ __device__ __forceinline__ void load_q(const AttnParams& p, unsigned char* dst, 
   fence_proxy_async_smem();
 }
 
-// The tensor maps of a call's q (tiles of p.tq tokens) and K/V views; views
-// that have none are read by 16-byte loads.
-void encode_maps(MmaParams& mp, const fd_attn_args* a);
+// The tensor maps of a call's q (tiles of p.tq tokens) and K/V views (K's alone
+// with k_only); views that have none are read by 16-byte loads.
+void encode_maps(MmaParams& mp, const fd_attn_args* a, bool k_only = false);
 
 }  // namespace mm
 }  // namespace at

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_keyw_kernel(const __
   const int nvec = p.D / VE;
 
   griddep_launch_dependents();
-  if (tid == 0) kp.cuts[cta].nparts = 0;
+  if (tid == 0 && kp.cuts != nullptr) kp.cuts[cta].nparts = 0;
   CoreWalk walk(p);
   if (!walk.init<kThreads>(&scratch, cta, kMinPer)) return;
 
@@ -207,39 +207,63 @@ int combine_launch(const KwParams& p, int kt, cudaStream_t s) {
 
 namespace {
 
-size_t base_workspace() { return (workspace_bytes() + 255) / 256 * 256; }
+size_t base_workspace(const Plan& plan) { return plan.whole ? 0 : (workspace_bytes() + 255) / 256 * 256; }
 
 template <typename T, int DP>
-int core_launch_dp(KwParams& p, cudaStream_t s) {
+int core_launch_dp(KwParams& p, bool whole, cudaStream_t s) {
   const void* kern = reinterpret_cast<const void*>(fd_keyw_kernel<T, DP>);
   static unsigned long long done = 0;
   int st = fdh::ensure_smem(kern, smem_bytes(DP), &done);
   if (st != FD_OK) return st;
-  int dev = 0, sms = 0;
-  st = fdh::device_sms(&dev, &sms);
-  if (st != FD_OK) return st;
-  p.a.ctas = sms * ctas_of(DP);
-  if (p.a.ctas > kMaxCtas) p.a.ctas = kMaxCtas;
   st = fdh::launch_maybe_pdl(kern, dim3((unsigned)p.a.ctas), dim3(kThreads), smem_bytes(DP), s, false, p,
                              "fd_keyw_kernel launch");
-  if (st != FD_OK) return st;
+  if (st != FD_OK || whole) return st;
   return combine_launch(p, kKeys, s);
 }
 
 template <typename T>
-int core_launch(KwParams& p, cudaStream_t s) {
-  if (p.a.D <= 64) return core_launch_dp<T, 64>(p, s);
-  if (p.a.D <= 128) return core_launch_dp<T, 128>(p, s);
-  return core_launch_dp<T, 256>(p, s);
+int core_launch(KwParams& p, bool whole, cudaStream_t s) {
+  if (p.a.D <= 64) return core_launch_dp<T, 64>(p, whole, s);
+  if (p.a.D <= 128) return core_launch_dp<T, 128>(p, whole, s);
+  return core_launch_dp<T, 256>(p, whole, s);
 }
 
 }  // namespace
+
+// Chunks of an item from which on cutting pays: what it evens out is at most
+// one item's time per CTA (or, with fewer items than CTAs, the idle ones'
+// share of it), what it costs the partials and the combine's launch.
+constexpr int kCutFrom = 3;
+
+Plan plan_of(const fd_attn_args* a) {
+  Plan p;
+  int dev = 0, sms = 0;
+  if (fdh::device_sms(&dev, &sms) != FD_OK) sms = 148;
+  const int G = a->num_heads / a->num_kv_heads;
+  const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
+  const bool mma = at::mma_covers(a);
+  p.cols = !mma ? 0 : q * G <= 16 ? 16 : q * G <= 32 ? 32 : 128;
+  p.ctas = mma ? sms : sms * ctas_of(a->head_size <= 64 ? 64 : a->head_size <= 128 ? 128 : 256);
+  if (p.ctas > kMaxCtas) p.ctas = kMaxCtas;
+  const int tq = (mma ? p.cols : kRows) / G, keys = mma ? kMaxKeys : kKeys;
+  const int64_t chunks = (q + tq - 1) / tq;
+  p.whole = p.cols == 16 || p.cols == 32 || chunks < kCutFrom;
+  if (!p.whole && a->max_k_len > 0) {
+    const int64_t items = ((int64_t)a->max_k_len + keys - 1) / keys * a->n * a->num_kv_heads;
+    p.whole = items <= p.ctas && chunks * (p.ctas - items) < kCutFrom * (int64_t)p.ctas;
+  }
+  return p;
+}
+
 }  // namespace kw
 }  // namespace fdk
 
 extern "C" size_t fd_key_weights_workspace_size(const fd_key_weights_args* a) {
   if (a == nullptr || a->attn.head_size <= 0 || a->attn.head_size > 256) return 0;
-  return fdk::kw::base_workspace() + fdk::at::stage_bytes(&a->attn);
+  if (a->attn.num_kv_heads <= 0 || a->attn.num_heads < a->attn.num_kv_heads ||
+      a->attn.num_heads / a->attn.num_kv_heads > fdk::kw::kRows)
+    return 0;
+  return fdk::kw::base_workspace(fdk::kw::plan_of(&a->attn)) + fdk::at::stage_bytes(&a->attn);
 }
 
 extern "C" int fd_key_weights(const fd_key_weights_args* args, void* stream) {
@@ -255,7 +279,7 @@ extern "C" int fd_key_weights(const fd_key_weights_args* args, void* stream) {
       (args->stats.num_blocks > 0 && (args->stats.weights == nullptr || args->stats.positions == nullptr)))
     return fdh::fail(FD_ERR_INVALID, "%s: stats need weights and positions", what);
   const size_t need = fd_key_weights_workspace_size(args);
-  if (a->workspace == nullptr || a->workspace_bytes < need || !fdh::aligned16(a->workspace))
+  if (need > 0 && (a->workspace == nullptr || a->workspace_bytes < need || !fdh::aligned16(a->workspace)))
     return fdh::fail(FD_ERR_WORKSPACE, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   p.weights = args->stats.weights;
@@ -263,19 +287,24 @@ extern "C" int fd_key_weights(const fd_key_weights_args* args, void* stream) {
   p.nstat = args->stats.num_blocks;
   p.evicted = args->evicted;
   unsigned char* ws = static_cast<unsigned char*>(a->workspace);
-  p.cuts = reinterpret_cast<kw::Cut*>(ws);
-  p.parts = reinterpret_cast<float*>(ws + kw::cut_bytes());
-  st = at::stage_launch(p.a, a, kw::base_workspace(), true, s);
+  const kw::Plan plan = kw::plan_of(a);
+  if (!plan.whole) {
+    p.cuts = reinterpret_cast<kw::Cut*>(ws);
+    p.parts = reinterpret_cast<float*>(ws + kw::cut_bytes());
+  }
+  st = at::stage_launch(p.a, a, kw::base_workspace(plan), true, s);
   if (st != FD_OK) return st;
-  if (at::mma_covers(a)) return kw::mma_launch(p, a, s);
+  p.a.ctas = plan.ctas;
+  p.a.snap = plan.whole;
+  if (plan.cols > 0) return kw::mma_launch(p, a, plan, s);
   p.a.tq = kw::kRows / p.a.G;
   switch (a->dtype) {
     case FD_DTYPE_F16:
-      return kw::core_launch<__half>(p, s);
+      return kw::core_launch<__half>(p, plan.whole, s);
     case FD_DTYPE_BF16:
-      return kw::core_launch<__nv_bfloat16>(p, s);
+      return kw::core_launch<__nv_bfloat16>(p, plan.whole, s);
     default:
-      return kw::core_launch<float>(p, s);
+      return kw::core_launch<float>(p, plan.whole, s);
   }
 }
 

@@ -41,7 +41,7 @@ struct KwParams {
   int32_t* positions;
   int64_t nstat;
   const int32_t* evicted;
-  Cut* cuts;     // [ctas]
+  Cut* cuts;     // [ctas], or null where no item is cut
   float* parts;  // [ctas][2][kMaxKeys]
 };
 
@@ -238,8 +238,16 @@ struct Walk {
   }
 };
 
+// The kernel of a call, as far as the caller's bounds tell (a wrong one costs
+// time, not the result).
+struct Plan {
+  int cols;   // query rows per chunk of the tensor-core kernel (its N), 0: the CUDA-core kernel
+  int ctas;
+  bool whole; // no item is cut
+};
+Plan plan_of(const fd_attn_args* a);
 // The tensor-core kernel: fp16 and bf16 heads of 64 to 128 dims.
-int mma_launch(KwParams& p, const fd_attn_args* a, cudaStream_t s);
+int mma_launch(KwParams& p, const fd_attn_args* a, const Plan& plan, cudaStream_t s);
 // Adds up the cut items' partials, KT keys per item.
 int combine_launch(const KwParams& p, int kt, cudaStream_t s);
 

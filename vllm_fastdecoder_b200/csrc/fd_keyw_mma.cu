@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
     return b >= step_empty && b < join_full ? Ge::kStepReaders : 1;
   });
   if (threadIdx.x == 0) {
-    kp.k.cuts[cta].nparts = 0;
+    if (kp.k.cuts != nullptr) kp.k.cuts[cta].nparts = 0;
     misc[0] = 0;
   }
   MmaWalk walk(p);
@@ -513,21 +513,15 @@ int launch_for(const KwMmaParams& kp, int n, cudaStream_t s) {
 
 }  // namespace mm
 
-int mma_launch(KwParams& p, const fd_attn_args* a, cudaStream_t s) {
-  int dev = 0, sms = 0;
-  int st = fdh::device_sms(&dev, &sms);
-  if (st != FD_OK) return st;
-  const int64_t rows = (int64_t)(a->max_q_len > 0 && a->max_q_len < p.a.T ? a->max_q_len : p.a.T) * p.a.G;
-  const int n = rows <= 16 ? 16 : rows <= 32 ? 32 : 128;
-  p.a.ctas = sms < kMaxCtas ? sms : kMaxCtas;
+int mma_launch(KwParams& p, const fd_attn_args* a, const Plan& plan, cudaStream_t s) {
+  const int n = plan.cols;
   p.a.tq = n / p.a.G;
-  p.a.snap = n <= 32;  // one chunk per item: there is nothing to cut
   mm::KwMmaParams kp{};
   kp.k = p;
   kp.m.a = p.a;
-  at::mm::encode_maps(kp.m, a);
-  st = a->dtype == FD_DTYPE_BF16 ? mm::launch_for<__nv_bfloat16>(kp, n, s) : mm::launch_for<__half>(kp, n, s);
-  if (st != FD_OK || p.a.snap) return st;
+  at::mm::encode_maps(kp.m, a, true);
+  const int st = a->dtype == FD_DTYPE_BF16 ? mm::launch_for<__nv_bfloat16>(kp, n, s) : mm::launch_for<__half>(kp, n, s);
+  if (st != FD_OK || plan.whole) return st;
   return combine_launch(p, mm::kKeys, s);
 }
 

@@ -748,10 +748,10 @@ def _tier_fields(t: KVTier | None, idx: int, dtype: torch.dtype, shape: tuple) -
     k, v = t.k, t.v
     if k.dtype is not dtype:
         raise RuntimeError("the KV tier's dtype differs")
-    B, *rest = k.shape
-    if tuple(rest) != shape:
+    sizes = k.shape
+    if sizes[1:] != shape:
         raise RuntimeError("the KV tiers must be [blocks, KVH, block_size, D] alike")
-    s = k.stride()
+    B, s = sizes[0], k.stride()
     if k.get_device() == idx and v.get_device() == idx:
         return (k.data_ptr(), v.data_ptr(), s[0], s[1], s[2], B, 0, 0)
     if k.is_cuda or v.is_cuda:
@@ -1118,7 +1118,7 @@ def cross_attn(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_start: torch
 # ------------------------------------------------------------- after the attention
 
 
-@dataclass
+@dataclass(frozen=True)
 class KeyStats:
     """What each cached key of one layer has received: weights fp32 and
     positions int32, both contiguous [blocks, KVH, block_size] on the device and
@@ -1141,9 +1141,10 @@ class KeyStats:
 
     def _fields(self, idx: int, KVH: int, BS: int) -> tuple:
         w = self.weights
-        if w.get_device() != idx or tuple(w.shape[1:]) != (KVH, BS):
+        B, h, b = w.shape
+        if w.get_device() != idx or h != KVH or b != BS:
             raise RuntimeError("stats must be [blocks, KVH, block_size] of the cache on the call's device")
-        return w.data_ptr(), self.positions.data_ptr(), w.shape[0]
+        return w.data_ptr(), self.positions.data_ptr(), B
 
 
 class KeyMoves:
@@ -1168,13 +1169,6 @@ class KeyMoves:
                 _i32(self.counts, idx, R * KVH, "moves.counts"))
 
 
-@lru_cache(maxsize=1)
-def _key_weights_workspace_bytes() -> int:
-    a = nat.FdKeyWeightsArgs()
-    a.attn.head_size = 64  # without a host tier the same for all sizes
-    return nat.load().fd_key_weights_workspace_size(ctypes.byref(a))
-
-
 def key_weights(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
                 q_start: torch.Tensor, q_len: torch.Tensor, k_len: torch.Tensor, scale: float, lse: torch.Tensor,
                 stats: KeyStats, *, evicted: torch.Tensor | None = None, bt_row: torch.Tensor | None = None,
@@ -1192,16 +1186,17 @@ def key_weights(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tie
     without the others)."""
     KVH, BS, f0, f1, W = _paged(q, tiers, block_table, bt_row, q_len.numel())
     idx = q.get_device()
-    packed = _attn_fields(q, None, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, block_table, W, bt_row, None, BS,
+    lib = nat.load()
+    fields = _attn_fields(q, None, lse, q_start, q_len, k_len, scale, KVH, f0, f1, tier_split, block_table, W, bt_row, None, BS,
                           max_q_len, max_k_len)
     more = (*stats._fields(idx, KVH, BS), 0 if evicted is None else _i32(evicted, idx, q_len.numel(), "evicted"))
-    if f1[-2]:  # a host tier: its copies count
-        need = nat.load().fd_key_weights_workspace_size(_KEY_WEIGHTS_STRUCT.pack(*packed, *more))
-    else:
-        need = _key_weights_workspace_bytes()
-    buf = _scratch(q, workspace_buf, need)
-    packed[-3], packed[-2] = buf.data_ptr(), buf.numel()
-    _launch(nat.load().fd_key_weights, _KEY_WEIGHTS_STRUCT.pack(*packed, *more), idx, "fd_key_weights")
+    packed = _KEY_WEIGHTS_STRUCT.pack(*fields, *more)
+    need = lib.fd_key_weights_workspace_size(packed)
+    if need > 0 or workspace_buf is not None:
+        buf = _scratch(q, workspace_buf, need)
+        fields[-3], fields[-2] = buf.data_ptr(), buf.numel()
+        packed = _KEY_WEIGHTS_STRUCT.pack(*fields, *more)
+    _launch(lib.fd_key_weights, packed, idx, "fd_key_weights")
 
 
 def select_keys(stats: KeyStats, block_table: torch.Tensor, seq_lens: torch.Tensor, keep_lens: torch.Tensor,
