@@ -22,34 +22,34 @@ constexpr int kRows = 64;
 constexpr int kThreads = 256;
 constexpr int kFixed = 1;
 constexpr int kMinPer = 1;
-typedef Walk<kKeys, kFixed> CoreWalk;
 
 constexpr int ctas_of(int DP) { return DP <= 64 ? 3 : DP <= 128 ? 2 : 1; }
 constexpr int smem_bytes(int DP) { return (kRows + kKeys) * (DP + 4) * 4; }
 
-template <typename T, int DP>
+template <typename T, int DP, bool kDirect>
 __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_keyw_kernel(const __grid_constant__ KwParams kp) {
   constexpr int VE = 16 / (int)sizeof(T);     // elements per 16-byte load
   constexpr int NV = DP / VE;                 // loads per row
   constexpr int LD = DP + 4;                  // row stride of the tiles (floats)
   constexpr int kVecs = kRows * NV / kThreads;  // loads per thread and tile
   constexpr int KN = kKeys / 16;
+  typedef Walk<kKeys, kFixed, kDirect> CoreWalk;
   const AttnParams& p = kp.a;
   extern __shared__ float4 smem4[];
   float* sq = reinterpret_cast<float*>(smem4);
   float* sk = sq + kRows * LD;
-  __shared__ CoreWalk::Scratch scratch;
+  __shared__ typename CoreWalk::Scratch scratch;
   __shared__ const unsigned char* k_row[kKeys];
   __shared__ float neg[kRows];          // -lse log2(e) of the rows
   __shared__ float sums[kThreads / 32][kKeys];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const int cta = blockIdx.x;
+  const int cta = blockIdx.x;  // (of a grid of items not used)
   const int nvec = p.D / VE;
 
   griddep_launch_dependents();
   if (tid == 0 && kp.cuts != nullptr) kp.cuts[cta].nparts = 0;
   CoreWalk walk(p);
-  if (!walk.init<kThreads>(&scratch, cta, kMinPer)) return;
+  if (!walk.template init<kThreads>(&scratch, cta, kMinPer)) return;
 
   auto put = [&](float* dst, int x, const uint4& v) {
     float f[VE];
@@ -58,7 +58,7 @@ __global__ void __launch_bounds__(kThreads, ctas_of(DP)) fd_keyw_kernel(const __
     for (int e = 0; e < VE; e += 4)
       *reinterpret_cast<float4*>(dst + x / NV * LD + x % NV * VE + e) = make_float4(f[e], f[e + 1], f[e + 2], f[e + 3]);
   };
-  CoreWalk::Seg g;
+  typename CoreWalk::Seg g;
   while (walk.next(g)) {
     const Req rq = walk.rq;
     const int key0 = g.kt * kKeys, base = rq.klen - rq.qlen;
@@ -209,23 +209,24 @@ namespace {
 
 size_t base_workspace(const Plan& plan) { return plan.whole ? 0 : (workspace_bytes() + 255) / 256 * 256; }
 
-template <typename T, int DP>
-int core_launch_dp(KwParams& p, bool whole, cudaStream_t s) {
-  const void* kern = reinterpret_cast<const void*>(fd_keyw_kernel<T, DP>);
+template <typename T, int DP, bool kDirect>
+int core_launch_dp(KwParams& p, const Plan& plan, cudaStream_t s) {
+  const void* kern = reinterpret_cast<const void*>(fd_keyw_kernel<T, DP, kDirect>);
   static unsigned long long done = 0;
   int st = fdh::ensure_smem(kern, smem_bytes(DP), &done);
   if (st != FD_OK) return st;
-  st = fdh::launch_maybe_pdl(kern, dim3((unsigned)p.a.ctas), dim3(kThreads), smem_bytes(DP), s, false, p,
-                             "fd_keyw_kernel launch");
-  if (st != FD_OK || whole) return st;
+  const dim3 grid = kDirect ? dim3((unsigned)plan.tiles, (unsigned)p.a.KVH, (unsigned)p.a.n) : dim3((unsigned)p.a.ctas);
+  st = fdh::launch_maybe_pdl(kern, grid, dim3(kThreads), smem_bytes(DP), s, false, p, "fd_keyw_kernel launch");
+  if (st != FD_OK || plan.whole) return st;
   return combine_launch(p, kKeys, s);
 }
 
 template <typename T>
-int core_launch(KwParams& p, bool whole, cudaStream_t s) {
-  if (p.a.D <= 64) return core_launch_dp<T, 64>(p, whole, s);
-  if (p.a.D <= 128) return core_launch_dp<T, 128>(p, whole, s);
-  return core_launch_dp<T, 256>(p, whole, s);
+int core_launch(KwParams& p, const Plan& plan, cudaStream_t s) {
+  const bool direct = plan.tiles > 0;
+  if (p.a.D <= 64) return direct ? core_launch_dp<T, 64, true>(p, plan, s) : core_launch_dp<T, 64, false>(p, plan, s);
+  if (p.a.D <= 128) return direct ? core_launch_dp<T, 128, true>(p, plan, s) : core_launch_dp<T, 128, false>(p, plan, s);
+  return direct ? core_launch_dp<T, 256, true>(p, plan, s) : core_launch_dp<T, 256, false>(p, plan, s);
 }
 
 }  // namespace
@@ -251,6 +252,12 @@ Plan plan_of(const fd_attn_args* a) {
   if (!p.whole && a->max_k_len > 0) {
     const int64_t items = ((int64_t)a->max_k_len + keys - 1) / keys * a->n * a->num_kv_heads;
     p.whole = items <= p.ctas && chunks * (p.ctas - items) < kCutFrom * (int64_t)p.ctas;
+  }
+  // a grid of items: whole ones, at most two for each CTA that runs at once (where lengths differ most are not there)
+  p.tiles = 0;
+  if (!mma && p.whole && a->max_k_len > 0 && a->n <= 65535 && a->num_kv_heads <= 65535) {
+    const int64_t tiles = ((int64_t)a->max_k_len + keys - 1) / keys;
+    if (tiles * a->n * a->num_kv_heads <= 2 * p.ctas) p.tiles = (int)tiles;
   }
   return p;
 }
@@ -300,11 +307,11 @@ extern "C" int fd_key_weights(const fd_key_weights_args* args, void* stream) {
   p.a.tq = kw::kRows / p.a.G;
   switch (a->dtype) {
     case FD_DTYPE_F16:
-      return kw::core_launch<__half>(p, plan.whole, s);
+      return kw::core_launch<__half>(p, plan, s);
     case FD_DTYPE_BF16:
-      return kw::core_launch<__nv_bfloat16>(p, plan.whole, s);
+      return kw::core_launch<__nv_bfloat16>(p, plan, s);
     default:
-      return kw::core_launch<float>(p, plan.whole, s);
+      return kw::core_launch<float>(p, plan, s);
   }
 }
 

@@ -15,7 +15,9 @@
 // takes kW positions (K's load, the epilogue) and one per chunk.  The line is
 // cut into equal ranges, one per CTA; an item that a range's end cuts leaves
 // its keys' sums as partials, which the combine adds up in ascending order, or,
-// with `snap`, belongs whole to the CTA in whose range it starts.
+// with `snap`, belongs whole to the CTA in whose range it starts.  A call of few
+// items on the CUDA cores has a grid of them instead (kDirect: key tile, kv
+// head, request), whose CTAs need not look for their work.
 #pragma once
 
 #include "fd_attn.cuh"
@@ -67,7 +69,7 @@ __device__ __forceinline__ void give(const KwParams& p, const Req& rq, int r, in
   }
 }
 
-template <int kKT, int kW>
+template <int kKT, int kW, bool kDirect>
 struct Walk {
   struct Seg {
     int r, kh, kt;
@@ -110,17 +112,81 @@ struct Walk {
 
   struct Scratch {
     long long warp_sum[32];
-    long long start, per_head, item_start;
-    int found, item;
+    long long start, per_head;
+    int found;
     Req rq;
   };
+
+  // The range of CTA `c`, given the cost of all requests.  False: no work.
+  __device__ __forceinline__ bool range(long long total, int c, int min_per, long long& p0) {
+    if (total > (long long)at::kMaxLen * p.ctas) {  // positions of a range are 32 bits
+      set_error(p.err, FD_DEVERR_LEN);
+      return false;
+    }
+    per = (int)quot(total + p.ctas - 1, p.ctas);
+    if (per < min_per) per = min_per;
+    p0 = (long long)c * per;
+    if (p0 >= total) return false;
+    len = (int)min((long long)per, total - p0);
+    return true;
+  }
+
+  // A warp together: the item of request r (cost per_head for each kv head) at
+  // position off of the request's.
+  __device__ __forceinline__ void find(long long off, long long per_head) {
+    const int lane = threadIdx.x & 31;
+    kh = (int)quot(off, per_head);
+    const long long x = off - (long long)kh * per_head;
+    int lo = 0, hi = tiles(rq);
+    long long at_lo = 0;
+    while (hi - lo > 1) {  // the last item that starts at or before x, 32 candidates at a time
+      const int gap = (hi - lo + 31) / 32;
+      const int i = lo + lane * gap;
+      const long long v = i < hi ? before(p, rq, i) : 0;
+      const unsigned in = __ballot_sync(0xffffffffu, i < hi && v <= x);
+      const int last = 31 - __clz(in);  // lane 0 always: before(lo) <= x
+      at_lo = __shfl_sync(0xffffffffu, v, last);
+      lo += last * gap;
+      hi = min(hi, lo + gap);
+    }
+    item = lo;
+    s = (int)(at_lo - x);
+  }
 
   // All NT threads of the block together: the range of CTA `c` and the item
   // it starts in.  False: no work.
   template <int NT>
   __device__ bool init(Scratch* sc, int c, int min_per) {
+    if constexpr (kDirect) {
+      r = blockIdx.z;
+      kh = blockIdx.y;
+      rq = at::load_req(p, r);
+      item = blockIdx.x;
+      behind = false;
+      return item < tiles(rq);
+    }
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     constexpr int kWarps = NT / 32;
+    behind = false;
+    if (p.n <= 32) {  // every warp by itself, a lane per request: no barriers (32 requests: 2 us of a call less)
+      Req mine = {0, 0, 0, 0};
+      if (lane < p.n) mine = at::load_req(p, lane);
+      long long per_head = cost(p, mine), at = per_head * p.KVH, p0;
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) {
+        const long long y = __shfl_up_sync(0xffffffffu, at, off);
+        if (lane >= off) at += y;
+      }
+      if (!range(__shfl_sync(0xffffffffu, at, 31), c, min_per, p0)) return false;
+      at -= per_head * p.KVH;
+      r = __ffs(__ballot_sync(0xffffffffu, at <= p0 && p0 < at + per_head * p.KVH)) - 1;
+      rq.qlen = __shfl_sync(0xffffffffu, mine.qlen, r);
+      rq.klen = __shfl_sync(0xffffffffu, mine.klen, r);
+      rq.qst = __shfl_sync(0xffffffffu, mine.qst, r);
+      rq.kbase = __shfl_sync(0xffffffffu, mine.kbase, r);
+      find(p0 - __shfl_sync(0xffffffffu, at, r), __shfl_sync(0xffffffffu, per_head, r));
+      return true;
+    }
     long long total = 0, mine = 0, mine_at = 0, per_head = 0, p0 = 0;
     Req mine_rq = {0, 0, 0, 0};
     const bool one = p.n <= NT;
@@ -160,51 +226,31 @@ struct Walk {
       }
       if (pass == 0) {
         total = carry;
-        if (total > (long long)at::kMaxLen * p.ctas) {  // positions of a range are 32 bits
-          set_error(p.err, FD_DEVERR_LEN);
-          return false;
-        }
-        per = (int)quot(total + p.ctas - 1, p.ctas);
-        if (per < min_per) per = min_per;
-        p0 = (long long)c * per;
-        if (p0 >= total) return false;
-        len = (int)min((long long)per, total - p0);
+        if (!range(total, c, min_per, p0)) return false;
       }
     }
     __syncthreads();
     r = sc->found;
     rq = sc->rq;
-    per_head = sc->per_head;
-    const long long off = p0 - sc->start;
-    kh = (int)quot(off, per_head);
-    const long long x = off - (long long)kh * per_head;
-    if (warp == 0) {  // the last item that starts at or before x, 32 candidates at a time
-      int lo = 0, hi = tiles(rq);
-      long long at_lo = 0;
-      while (hi - lo > 1) {
-        const int gap = (hi - lo + 31) / 32;
-        const int i = lo + lane * gap;
-        const long long v = i < hi ? before(p, rq, i) : 0;
-        const unsigned in = __ballot_sync(0xffffffffu, i < hi && v <= x);
-        const int last = 31 - __clz(in);  // lane 0 always: before(lo) <= x
-        at_lo = __shfl_sync(0xffffffffu, v, last);
-        lo += last * gap;
-        hi = min(hi, lo + gap);
-      }
-      if (lane == 0) {
-        sc->item = lo;
-        sc->item_start = at_lo - x;
-      }
-    }
-    __syncthreads();
-    item = sc->item;
-    s = (int)sc->item_start;
-    behind = false;
+    find(p0 - sc->start, sc->per_head);  // (every warp by itself)
     return true;
   }
 
   // The next segment of this CTA's range.
   __device__ __forceinline__ bool next(Seg& g) {
+    if constexpr (kDirect) {  // (more than one item only where the keys are more than the caller's bound)
+      if (behind) item += gridDim.x;
+      behind = true;
+      if (item >= tiles(rq)) return false;
+      g.r = r;
+      g.kh = kh;
+      g.kt = item;
+      g.c0 = first_chunk(p, rq, item);
+      g.n = last_chunk(p, rq) - g.c0;
+      g.whole = g.head = true;
+      g.nparts = 0;
+      return true;
+    }
     while (true) {
       if (behind) {
         s += kW + last_chunk(p, rq) - first_chunk(p, rq, item);
@@ -244,6 +290,7 @@ struct Plan {
   int cols;   // query rows per chunk of the tensor-core kernel (its N), 0: the CUDA-core kernel
   int ctas;
   bool whole; // no item is cut
+  int tiles;  // > 0: a grid of items, this many key tiles wide (CUDA cores)
 };
 Plan plan_of(const fd_attn_args* a);
 // The tensor-core kernel: fp16 and bf16 heads of 64 to 128 dims.

@@ -15,8 +15,8 @@
 // Warps: the epilogue's first, four per key tile, and with N = 128 another four
 // per tile, the two groups taking turns at the steps (two warps per scheduler
 // leave the SFU idle while both wait; their sums are joined at the item's end);
-// then one for the schedule, the query chunks and their lse (a step ahead, so
-// that those loads cost no step its time), one per key tile that loads K, and
+// then one for the schedule, the query chunks and their lse (as many steps ahead
+// as there are slots), one per key tile that loads K, and
 // one whose first thread issues the MMAs.  A STEP is one chunk against one item;
 // its record goes through a ring to all roles.  Every wait is bounded, and a role
 // that gives up raises the CTA's abort flag for the others.
@@ -41,7 +41,7 @@ static_assert(kKeys == kMaxKeys, "partials per item");
 constexpr int kFixed = 2;             // an item's fixed cost in chunks
 constexpr int kMinPer = 3;            // least positions of a CTA
 
-typedef Walk<kKeys, kFixed> MmaWalk;
+typedef Walk<kKeys, kFixed, false> MmaWalk;
 
 struct KwMmaParams {
   at::mm::MmaParams m;  // m.a is k.a
@@ -79,9 +79,10 @@ struct Geo {
   static_assert(sizeof(MmaWalk::Scratch) <= kRingQ * (N < 32 ? 32 : N) * 4, "scratch of the schedule");
 };
 
-// What a step is the first or last of: its segment (K), its chunk's stay in a
-// slot (Q).  Flags 0: no more steps.
-enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8, kLastQ = 16 };
+// Whether a step is the first or last of its segment (K), and the first with a
+// chunk of queries (Q: the slot of the chunk before is done with the steps
+// before).  Flags 0: no more steps.
+enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8 };
 struct Step {
   int flags;
   int r, kh, kt, kbase;
@@ -150,7 +151,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);  // [kRingK][kTiles]
   uint64_t* k_empty = k_full + kRingK * kTiles;  // [kRingK] MMA commit after the item's last step
   uint64_t* q_full = k_empty + kRingK;           // [kRingQ]
-  uint64_t* q_empty = q_full + kRingQ;           // [kRingQ] MMA commit after the chunk's last step, and the epilogue warps
+  uint64_t* q_empty = q_full + kRingQ;           // [kRingQ] MMA commit when the next chunk begins, and the epilogue warps
   uint64_t* s_full = q_empty + kRingQ;           // [kBufs][kTiles] MMA commit
   uint64_t* s_empty = s_full + kBufs * kTiles;   // [kBufs][kTiles] four epilogue warps have the scores
   uint64_t* step_full = s_empty + kBufs * kTiles;
@@ -236,15 +237,14 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
       last_kh = g.kh;
       last_chunk = chunk++;
     };
-    Step cur, nxt;
-    Req rq = {0, 0, 0, 0}, rq_next = rq;
-    float ls[kPer], ls_next[kPer];
-    gen(cur, rq, ls);
+    Step cur;
+    Req rq = {0, 0, 0, 0};
+    float ls[kPer];
     int qs = -1;
     uint32_t nq = 0;
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
-      if (cur.flags != 0) gen(nxt, rq_next, ls_next);
+      gen(cur, rq, ls);
       const int ss = i % kSteps;
       if (i >= kSteps)
         ok = __all_sync(0xffffffffu, wait_or_abort(&step_empty[ss], (i / kSteps - 1) & 1u, misc, p.err));
@@ -273,15 +273,10 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           if (lane == 0) mbar_arrive(&q_full[qs]);
         }
       }
-      if (cur.flags != 0 && (nxt.flags == 0 || (nxt.flags & kNewQ) != 0)) cur.flags |= kLastQ;
       if (lane == 0) steps[ss] = cur;
       __syncwarp();
       if (lane == 0) mbar_arrive(&step_full[ss]);
       if (cur.flags == 0) break;
-      cur = nxt;
-      rq = rq_next;
-#pragma unroll
-      for (int x = 0; x < kPer; ++x) ls[x] = ls_next[x];
     }
     if (!ok) misc[0] = 1;
     // no copy of this warp is in flight when the CTA ends: the last chunk of each slot
@@ -341,6 +336,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         mbar_arrive(&step_empty[ss]);
         if (flags == 0) break;
         const bool new_k = (flags & kNewK) != 0, new_q = (flags & kNewQ) != 0;
+        if (new_q && nq > 0) umma_commit(&q_empty[(nq - 1) % kRingQ]);
         items += new_k;
         nq += new_q;
         const int ks = (int)((items - 1) % kRingK), qs = (int)((nq - 1) % kRingQ), b = (int)(i % kBufs);
@@ -360,7 +356,6 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           umma_commit(&s_full[b * kTiles + t]);
         }
         if (ok && (flags & kLastK) != 0) umma_commit(&k_empty[ks]);
-        if (ok && (flags & kLastQ) != 0) umma_commit(&q_empty[qs]);
       }
       if (!ok) misc[0] = 1;
       umma_commit(drain);  // all MMAs complete before TMEM is released
@@ -386,7 +381,10 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
       __syncwarp();
       if (lane == 0) mbar_arrive(&step_empty[ss]);
       if (s.flags == 0) break;
-      if ((s.flags & kNewQ) != 0) ++nq;
+      if ((s.flags & kNewQ) != 0) {
+        if (nq > 0 && lane == 0) mbar_arrive(&q_empty[(nq - 1) % kRingQ]);
+        ++nq;
+      }
       const int qs = (int)((nq - 1) % kRingQ);
       const int key0 = s.kt * kKeys + t * kKT + row, key = key0 + lane;
       if ((s.flags & kNewK) != 0) {
@@ -449,10 +447,6 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
         }
       }
-      if ((s.flags & kLastQ) != 0) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_empty[qs]);
-      }
       if ((s.flags & kLastK) != 0) {
         float a0, a1, a2, a3;
         f2_unpack(acc[0], a0, a1);
@@ -514,13 +508,12 @@ int launch_for(const KwMmaParams& kp, int n, cudaStream_t s) {
 }  // namespace mm
 
 int mma_launch(KwParams& p, const fd_attn_args* a, const Plan& plan, cudaStream_t s) {
-  const int n = plan.cols;
-  p.a.tq = n / p.a.G;
+  p.a.tq = plan.cols / p.a.G;
   mm::KwMmaParams kp{};
   kp.k = p;
   kp.m.a = p.a;
   at::mm::encode_maps(kp.m, a, true);
-  const int st = a->dtype == FD_DTYPE_BF16 ? mm::launch_for<__nv_bfloat16>(kp, n, s) : mm::launch_for<__half>(kp, n, s);
+  const int st = a->dtype == FD_DTYPE_BF16 ? mm::launch_for<__nv_bfloat16>(kp, plan.cols, s) : mm::launch_for<__half>(kp, plan.cols, s);
   if (st != FD_OK || plan.whole) return st;
   return combine_launch(p, mm::kKeys, s);
 }
