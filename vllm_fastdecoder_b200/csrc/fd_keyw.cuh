@@ -250,8 +250,7 @@ struct Walk {
       g.whole = g.head = true;
       g.nparts = 0;
       return true;
-    }
-    while (true) {
+    } else while (true) {
       if (behind) {
         s += kW + last_chunk(p, rq) - first_chunk(p, rq, item);
         if (++item == tiles(rq)) {

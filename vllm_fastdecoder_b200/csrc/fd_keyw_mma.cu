@@ -86,10 +86,11 @@ enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8 };
 struct Step {
   int flags;
   int r, kh, kt, kbase;
-  int tok0, rows;    // of the chunk: its first token, its rows
+  int first, last;   // the last key that the chunk's first, and its last token sees
+  int rows;          // of the chunk
   int qlen, klen;
   int slot;          // -1: whole, else its slot of the partials
-  int pad[2];
+  int pad;
 };
 static_assert(sizeof(Step) == 48, "step record");
 
@@ -114,13 +115,13 @@ __device__ __forceinline__ void wait_loaded(uint32_t (&r)[16]) {
                : "memory");
 }
 
-// 32 scores of a key (columns n0 ..): what they add.
-template <bool kMasked>
-__device__ __forceinline__ void add_up(const uint32_t (&s)[32], const float* neg, f2_t sl2, int n0, int from, int rows,
-                                       f2_t (&acc)[2]) {
+// What 32 scores of a key add up to; the e-th counts if see(e).  skip(c): none
+// of scores c .. c + 3 counts for any key of the warp.
+template <typename See, typename Skip>
+__device__ __forceinline__ void add_up(const uint32_t (&s)[32], const float* neg, f2_t sl2, f2_t (&acc)[2], See see, Skip skip) {
 #pragma unroll
   for (int c = 0; c < 32; c += 4) {
-    if (kMasked && n0 + c >= rows) break;  // the warp alike
+    if (skip(c)) break;
     const ulonglong2 ng = *reinterpret_cast<const ulonglong2*>(neg + c);
     const f2_t x0 = f2_fma(f2_pack(__uint_as_float(s[c]), __uint_as_float(s[c + 1])), sl2, ng.x);
     const f2_t x1 = f2_fma(f2_pack(__uint_as_float(s[c + 2]), __uint_as_float(s[c + 3])), sl2, ng.y);
@@ -130,11 +131,18 @@ __device__ __forceinline__ void add_up(const uint32_t (&s)[32], const float* neg
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       e[i] = at::ex2_approx(e[i]);
-      if (kMasked && (n0 + c + i < from || n0 + c + i >= rows)) e[i] = 0.f;
+      if (!see(c + i)) e[i] = 0.f;
     }
     acc[0] = f2_add(acc[0], f2_pack(e[0], e[1]));
     acc[1] = f2_add(acc[1], f2_pack(e[2], e[3]));
   }
+}
+
+// Bits from .. to - 1 of a word.
+__device__ __forceinline__ uint32_t bits_of(int from, int to) {
+  const uint32_t below_to = to >= 32 ? ~0u : to > 0 ? (1u << to) - 1u : 0u;
+  const uint32_t below_from = from >= 32 ? ~0u : from > 0 ? (1u << from) - 1u : 0u;
+  return below_to & ~below_from;
 }
 
 template <typename T, int KD, int N>
@@ -222,14 +230,17 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
       s.kh = g.kh;
       s.kt = g.kt;
       s.kbase = rq.kbase;
-      s.tok0 = chunk * p.tq;
-      s.rows = min(p.tq, rq.qlen - s.tok0) * p.G;
+      const int tok0 = chunk * p.tq, ntok = min(p.tq, rq.qlen - tok0);
+      rq.qst += tok0;  // the chunk's first row
+      s.rows = ntok * p.G;
+      s.first = rq.klen - rq.qlen + tok0;
+      s.last = s.first + ntok - 1;
       s.qlen = rq.qlen;
       s.klen = rq.klen;
       s.slot = g.whole ? -1 : 2 * cta + (g.head ? 1 : 0);
       if (g.r != last_r || g.kh != last_kh || chunk != last_chunk) {
         s.flags |= kNewQ;
-        const float* at = p.lse + (int64_t)(s.kh * p.G) * p.lse_sh + (int64_t)(rq.qst + s.tok0) * p.lse_st;
+        const float* at = p.lse + (int64_t)(s.kh * p.G) * p.lse_sh + (int64_t)rq.qst * p.lse_st;
 #pragma unroll
         for (int i = 0; i < kPer; ++i) ls[i] = 32 * i + lane < s.rows ? at[col_h[i] * p.lse_sh + col_t[i] * p.lse_st] : 0.f;
       }
@@ -263,12 +274,12 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           if (lane == 0) {
             mbar_expect_tx(&q_full[qs], (uint32_t)(Ge::kPanels * p.tq * p.G * 128));
             for (int x = 0; x < Ge::kPanels; ++x)
-              tma_load_4d(sq + x * N * 128, &mp.tmap_q, 64 * x, cur.kh * p.G, rq.qst + cur.tok0, 0, &q_full[qs],
+              tma_load_4d(sq + x * N * 128, &mp.tmap_q, 64 * x, cur.kh * p.G, rq.qst, 0, &q_full[qs],
                           l2_evict_normal_policy());
             mbar_arrive(&q_full[qs]);
           }
         } else {
-          at::mm::load_q<KD>(p, sq, N * 128, cur.kh, rq.qst + cur.tok0, cur.rows / p.G, lane);
+          at::mm::load_q<KD>(p, sq, N * 128, cur.kh, rq.qst, cur.rows / p.G, lane);
           __syncwarp();
           if (lane == 0) mbar_arrive(&q_full[qs]);
         }
@@ -289,19 +300,22 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
     const int t = warp - kWarpK;
     const uint64_t pol = l2_evict_first_policy();
     uint32_t i = 0, items = 0;
-    Step item;           // the item to load next, its block ids on the way
-    int id = -1;
-    auto take = [&]() {  // the next step that begins an item; false: given up
-      for (;; ++i) {
-        const int ss = i % kSteps;
-        if (!__all_sync(0xffffffffu, wait_or_abort(&step_full[ss], (i / kSteps) & 1u, misc, p.err))) return false;
-        item = steps[ss];
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&step_empty[ss]);
-        if (item.flags == 0 || (item.flags & kNewK) != 0) break;
-      }
+    Step item, ahead;    // the item to load, and the one after it where it is known already:
+    int id = -1, id_ahead = -1;  // their block ids are on the way
+    auto read = [&](Step& to, int& ids) {  // step i, which has been published; whether an item begins or all end with it
+      const int ss = i % kSteps;
+      to = steps[ss];
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&step_empty[ss]);
       ++i;
-      if (item.flags != 0) id = box_block(mp, false, item.kbase, item.klen, item.kt * kTiles + t, lane);
+      if (to.flags != 0 && (to.flags & kNewK) == 0) return false;
+      if (to.flags != 0) ids = box_block(mp, false, to.kbase, to.klen, to.kt * kTiles + t, lane);
+      return true;
+    };
+    auto take = [&]() {  // the next item; false: given up
+      do {
+        if (!__all_sync(0xffffffffu, wait_or_abort(&step_full[i % kSteps], (i / kSteps) & 1u, misc, p.err))) return false;
+      } while (!read(item, id));
       return true;
     };
     bool ok = take();
@@ -311,9 +325,16 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         ok = __all_sync(0xffffffffu, wait_or_abort(&k_empty[ks], (items / kRingK - 1) & 1u, misc, p.err));
       if (!ok) break;
       ++items;
+      // (not awaited: the step may wait for this item's products)
+      const bool known = __all_sync(0xffffffffu, mbar_test_wait(&step_full[i % kSteps], (i / kSteps) & 1u)) && read(ahead, id_ahead);
       load_tile<KD>(mp, false, smem + ks * Ge::kItem + t * kTile, &k_full[ks * kTiles + t], item.kt * kTiles + t, item.r,
                     item.kbase, item.klen, item.kh, id, lane, pol);
-      ok = take();
+      if (known) {
+        item = ahead;
+        id = id_ahead;
+      } else {
+        ok = take();
+      }
     }
     if (!ok) misc[0] = 1;
     for (uint32_t s = 0; s < (uint32_t)kRingK && s < items; ++s) {
@@ -396,16 +417,14 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         ok = __all_sync(0xffffffffu, wait_or_abort(&s_full[b * kTiles + t], (i / kBufs) & 1u, misc, p.err));
         if (!ok) break;
         tc_fence_after();
-        // column n (token tok0 + n / G) sees keys up to klen - qlen + its token
-        const int first = s.klen - s.qlen + s.tok0;
-        const int last_tok = s.rows / p.G - 1;
-        const bool any = key0 < s.klen && key0 <= first + last_tok;  // the warp alike
+        // column n sees keys up to first + n / G
+        const bool any = key0 < s.klen && key0 <= s.last;  // the warp alike
         const uint32_t ts = tmem + lanes + (uint32_t)((t * kBufs + b) * Ge::kCols);
         const float* neg = lse_sh + qs * kLseRow;
         if (any) {
-          const int over = key - first;
+          const int over = key - s.first;
           const int from = over > 0 ? over * p.G : 0;
-          const bool masked = key0 + 31 > first || s.rows < N;
+          const bool masked = key0 + 31 > s.first || s.rows < N;
           if constexpr (N <= 32) {
             uint32_t v[32];
             if constexpr (N == 16) {
@@ -421,7 +440,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
-            add_up<true>(v, neg, sl2, 0, from, s.rows, acc);
+            add_up(v, neg, sl2, acc, [&](int e) { return e >= from && e < s.rows; }, [&](int c) { return c >= s.rows; });
           } else {
             uint32_t v[2][32];
             tmem_ld32_nowait(ts, v[0]);
@@ -435,10 +454,13 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
               }
-              if (masked)
-                add_up<true>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
-              else
-                add_up<false>(v[c & 1], neg + 32 * c, sl2, 32 * c, from, s.rows, acc);
+              const auto no_skip = [](int) { return false; };
+              if (masked) {
+                const uint32_t seen = bits_of(from - 32 * c, s.rows - 32 * c);
+                add_up(v[c & 1], neg + 32 * c, sl2, acc, [&](int e) { return (seen >> e & 1u) != 0u; }, no_skip);
+              } else {
+                add_up(v[c & 1], neg + 32 * c, sl2, acc, [](int) { return true; }, no_skip);
+              }
             }
           }
         } else {
