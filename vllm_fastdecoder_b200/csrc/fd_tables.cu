@@ -418,28 +418,37 @@ __global__ void __launch_bounds__(kThreads, 1) fd_tables_kernel(const __grid_con
 // order, form a line of F entries; its place on the stacks is the running
 // count of HBM (or host) ids ahead of it.  The line is cut into equal spans,
 // one per CTA of a cluster, those into runs of one warp, so one request that
-// loses a thousand blocks and a thousand that lose one are dealt out alike.
-// Ids are read once and stay in registers from the count to the push where a
-// CTA's span is one pass of kTrimIds ids per thread.  Bound by latency: the
-// lengths, the ids, two cluster barriers.
-// Measured: 256 requests that lose up to 7 tokens in 10.2 us, 100 that lose 2000
-// to 14000 (50,000 blocks) in 16.4.
+// loses a thousand blocks and a thousand that lose one are dealt out alike.  A
+// lane looks its first entry's request up, and another's where that one's blocks
+// end.  Ids are read once and stay in registers from the count to the push where a CTA's span
+// is one pass of kTrimIds ids per thread.  Bound by latency: the lengths, the
+// ids, the barriers; a small CTA where the caller's bound says that few blocks
+// can go.
+// (figures)
 constexpr int kTrimIds = 8;
-constexpr int kTrimPass = kThreads * kTrimIds;
-// Freed blocks, as far as the caller's bounds tell, that one CTA takes: a
-// second pass costs it what the cluster's barriers do.
-constexpr int kTrimOneCta = 2 * kTrimPass;
+constexpr int kTrimSmall = 256;   // threads of the small CTA
+// Blocks that one CTA takes, as far as the caller's bounds tell.
+constexpr int kTrimOneCta = 2 * kThreads * kTrimIds;
 
-template <bool kPow2>
-__global__ void __launch_bounds__(kThreads, 1) fd_trim_kernel(const __grid_constant__ fd_trim_args a) {
+// Sum over the CTA's warps of v (one value per warp, in shared memory), and of
+// those before this one.
+template <int kNw>
+__device__ __forceinline__ void over_warps(const int* v, int warp, int lane, int& ahead, int& all) {
+  const int x = lane < kNw ? v[lane] : 0;
+  ahead = __reduce_add_sync(0xffffffffu, lane < warp ? x : 0);
+  all = __reduce_add_sync(0xffffffffu, x);
+}
+
+template <bool kPow2, int kNt>
+__global__ void __launch_bounds__(kNt, 1) fd_trim_kernel(const __grid_constant__ fd_trim_args a) {
+  constexpr int kNw = kNt / 32, kPass = kNt * kTrimIds;
   extern __shared__ int sm[];  // [R + 1] running sum of freed blocks, [R] first freed column, [R] lengths, [R] kept lengths
-  __shared__ long long warp_sum[kWarps];
-  __shared__ int warp_n[2][kWarps];
-  __shared__ int cta_n[kCluster][2];
-  __shared__ int cta_flags[kCluster];
-  __shared__ int shared_flags, shared_max;
+  __shared__ int warp_n[2][kNw];
+  __shared__ int cta_n[kCluster][3];  // HBM and host blocks, flags
+  __shared__ int shared_flags, shared_max, shared_high;
   cg::cluster_group cluster = cg::this_cluster();
   const int nct = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
+  if (nct > 1) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
   const int R = a.num_reqs, BS = a.block_size, W = a.bt_width;
   const Blocks<kPow2> blocks(BS);
   int* s_sum = sm;
@@ -447,19 +456,18 @@ __global__ void __launch_bounds__(kThreads, 1) fd_trim_kernel(const __grid_const
   int* s_len = s_col + R;
   int* s_left = s_len + R;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if (tid == 0) shared_flags = shared_max = 0;
-  for (int r = tid; r < R; r += kThreads) {
+  if (tid == 0) shared_flags = shared_max = shared_high = 0;
+  const int c0_in = a.counts_in[0], c1_in = a.counts_in[1];
+  for (int r = tid; r < R; r += kNt) {
     const int len = a.lens_in[r], keep = a.keep_lens[r];
     s_len[r] = len;
     s_left[r] = keep >= 0 && keep < len ? keep : len;
   }
-  const int c0_in = a.counts_in[0], c1_in = a.counts_in[1];
   __syncthreads();
 
   // running sum of the freed blocks: thread t takes requests [t per, (t + 1) per)
-  const int per = (R + kThreads - 1) / kThreads;
-  int flags = 0, longest = 0;
-  long long mine = 0;
+  const int per = (R + kNt - 1) / kNt;
+  int flags = 0, longest = 0, mine = 0, high = 0;
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r >= R) break;
@@ -469,38 +477,40 @@ __global__ void __launch_bounds__(kThreads, 1) fd_trim_kernel(const __grid_const
       s_col[r] = s_sum[r] = 0;
       continue;
     }
-    const int col = blocks.hold(s_left[r]);
+    const int col = blocks.hold(s_left[r]), n = blocks.hold(len) - col;
     s_col[r] = col;
-    s_sum[r] = blocks.hold(len) - col;
-    mine += s_sum[r];
+    s_sum[r] = n;
+    mine += n;       // (may wrap, with the sums below: then `high` tells)
+    high += n >> 12;
     longest = max(longest, s_left[r]);
   }
-  long long v = mine;
+  int v = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const long long u = __shfl_up_sync(0xffffffffu, v, off);
+    const int u = __shfl_up_sync(0xffffffffu, v, off);
     if (lane >= off) v += u;
   }
-  if (lane == 31) warp_sum[warp] = v;
+  if (lane == 31) warp_n[0][warp] = v;
   flags = __reduce_or_sync(0xffffffffu, flags);
   longest = __reduce_max_sync(0xffffffffu, longest);
+  high = __reduce_add_sync(0xffffffffu, min(high, 1 << 20));
   if (lane == 0) {
     if (flags != 0) atomicOr(&shared_flags, flags);
     atomicMax(&shared_max, longest);
+    if (high != 0) atomicAdd(&shared_high, high);
   }
   __syncthreads();
-  long long run = v - mine, total = 0;
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) run += warp_sum[w];
-    total += warp_sum[w];
-  }
-  if (total > kMaxCount && tid == 0) shared_flags |= FD_TABLES_BAD_POOL;
-  const int F = total > kMaxCount ? 0 : (int)total;
+  int run, F;
+  over_warps<kNw>(warp_n[0], warp, lane, run, F);
+  run += v - mine;
+  // more than 2^30 blocks: no stack holds them
+  const bool fits = shared_high <= kMaxCount >> 12;
+  if (!fits) F = 0;
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r >= R) break;
     const int n = s_sum[r];
-    s_sum[r] = F > 0 ? (int)run : 0;
+    s_sum[r] = fits ? run : 0;
     run += n;
   }
   if (tid == 0) s_sum[R] = F;
@@ -508,34 +518,41 @@ __global__ void __launch_bounds__(kThreads, 1) fd_trim_kernel(const __grid_const
 
   // this CTA's span of the line; warp w takes kTrimIds * 32 neighbours per pass
   const int lo = (int)((long long)F * rank / nct), hi = (int)((long long)F * (rank + 1) / nct);
-  const bool one = hi - lo <= kTrimPass;
+  const bool one = hi - lo <= kPass;
+  const int ids = (int)(a.num_gpu_blocks + a.num_cpu_blocks), hbm_ids = (int)a.num_gpu_blocks;
   int id[kTrimIds];
+  flags = fits ? 0 : FD_TABLES_BAD_POOL;
   auto load = [&](int base) {  // ids of the warp's run from `base` on, -1 behind the span
+    int r = 0;
 #pragma unroll
     for (int u = 0; u < kTrimIds; ++u) {
-      const int f = base + 32 * u + lane;
       id[u] = -1;
+      const int f = base + 32 * u + lane;
+      if (base + 32 * u >= hi) continue;  // the warp alike
       if (f >= hi) continue;
-      const int r = owner(s_sum, 0, R, f);
+      if (u == 0 || s_sum[r + 1] <= f) r = owner(s_sum, r, R, f);
       id[u] = a.block_table[(int64_t)r * a.bt_stride + s_col[r] + (f - s_sum[r])];
-      if (id[u] < 0 || id[u] >= a.num_gpu_blocks + a.num_cpu_blocks) {
+    }
+#pragma unroll
+    for (int u = 0; u < kTrimIds; ++u) {
+      if (base + 32 * u + lane < hi && (id[u] < 0 || id[u] >= ids)) {
         flags |= FD_TABLES_BAD_BLOCK;
         id[u] = 0;
       }
     }
   };
-  auto count = [&](bool hbm) {
-    int n = 0;
+  auto count = [&](int base, int& n0, int& n1) {
 #pragma unroll
-    for (int u = 0; u < kTrimIds; ++u) n += __popc(__ballot_sync(0xffffffffu, id[u] >= 0 && (id[u] < a.num_gpu_blocks) == hbm));
-    return n;
+    for (int u = 0; u < kTrimIds; ++u) {
+      if (base + 32 * u >= hi) break;  // the warp alike
+      n0 += __popc(__ballot_sync(0xffffffffu, id[u] >= 0 && id[u] < hbm_ids));
+      n1 += __popc(__ballot_sync(0xffffffffu, id[u] >= hbm_ids));
+    }
   };
-  flags = 0;
   int n0 = 0, n1 = 0;  // of this warp, over all passes
-  for (int base = lo; base < hi; base += kTrimPass) {
-    load(base + warp * kTrimIds * 32);
-    n0 += count(true);
-    n1 += count(false);
+  for (int base = lo + warp * kTrimIds * 32; base < hi; base += kPass) {
+    load(base);
+    count(base, n0, n1);
   }
   flags = __reduce_or_sync(0xffffffffu, flags);
   if (lane == 0) {
@@ -544,81 +561,83 @@ __global__ void __launch_bounds__(kThreads, 1) fd_trim_kernel(const __grid_const
     if (flags != 0) atomicOr(&shared_flags, flags);
   }
   __syncthreads();
-  if (nct > 1) cluster.sync();  // every CTA of the cluster has started
-  if (warp == 0) {
-    const int s0 = __reduce_add_sync(0xffffffffu, warp_n[0][lane]), s1 = __reduce_add_sync(0xffffffffu, warp_n[1][lane]);
-    if (lane < nct) {
-      int* to = cluster.map_shared_rank(&cta_n[rank][0], lane);
-      to[0] = s0;
-      to[1] = s1;
-      *cluster.map_shared_rank(&cta_flags[rank], lane) = shared_flags;
+  int ahead0, ahead1, all0, all1;
+  over_warps<kNw>(warp_n[0], warp, lane, ahead0, all0);
+  over_warps<kNw>(warp_n[1], warp, lane, ahead1, all1);
+  flags = shared_flags;
+  int at0 = c0_in, at1 = c1_in;
+  long long end0 = (long long)c0_in + all0, end1 = (long long)c1_in + all1;
+  if (nct > 1) {
+    cluster.barrier_wait();
+    if (tid < nct) {
+      int* to = cluster.map_shared_rank(&cta_n[rank][0], tid);
+      to[0] = all0;
+      to[1] = all1;
+      to[2] = flags;
     }
-  }
-  if (nct > 1)
     cluster.sync();  // also: every CTA has read the lengths and counts before any writes them
-  else
-    __syncthreads();
-  long long at0 = c0_in, at1 = c1_in, end0 = c0_in, end1 = c1_in;
-  flags = 0;
-  for (int c = 0; c < nct; ++c) {
-    if (c < rank) {
-      at0 += cta_n[c][0];
-      at1 += cta_n[c][1];
+    end0 = c0_in;
+    end1 = c1_in;
+#pragma unroll
+    for (int c = 0; c < kCluster; ++c) {
+      if (c >= nct) break;
+      const int x0 = cta_n[c][0], x1 = cta_n[c][1];
+      at0 += c < rank ? x0 : 0;
+      at1 += c < rank ? x1 : 0;
+      end0 += x0;
+      end1 += x1;
+      flags |= cta_n[c][2];
     }
-    end0 += cta_n[c][0];
-    end1 += cta_n[c][1];
-    flags |= cta_flags[c];
   }
   if (c0_in < 0 || c1_in < 0 || end0 > a.free_cap[0] || end1 > a.free_cap[1]) flags |= FD_TABLES_BAD_POOL;
-  for (int r = rank * kThreads + tid; r < R; r += nct * kThreads) {
+  if (flags == 0) {
+    const unsigned below = (1u << lane) - 1u;
+    for (int base = lo; base < hi; base += kPass) {
+      const int from = base + warp * kTrimIds * 32;
+      if (!one) {  // the pass's ids again, and its counts
+        n0 = n1 = 0;
+        if (from < hi) {
+          load(from);
+          count(from, n0, n1);
+        }
+        __syncthreads();  // the last pass's counts have been read
+        if (lane == 0) {
+          warp_n[0][warp] = n0;
+          warp_n[1][warp] = n1;
+        }
+        __syncthreads();
+        over_warps<kNw>(warp_n[0], warp, lane, ahead0, all0);
+        over_warps<kNw>(warp_n[1], warp, lane, ahead1, all1);
+      }
+      int to0 = at0 + ahead0, to1 = at1 + ahead1;
+#pragma unroll
+      for (int u = 0; u < kTrimIds; ++u) {
+        if (from + 32 * u >= hi) break;  // the warp alike
+        const bool in = id[u] >= 0, hbm = id[u] < hbm_ids;
+        const unsigned in0 = __ballot_sync(0xffffffffu, in && hbm), in1 = __ballot_sync(0xffffffffu, in && !hbm);
+        if (in && hbm) a.free_ids[0][to0 + __popc(in0 & below)] = id[u];
+        if (in && !hbm) a.free_ids[1][to1 + __popc(in1 & below)] = id[u];
+        to0 += __popc(in0);
+        to1 += __popc(in1);
+      }
+      at0 += all0;
+      at1 += all1;
+    }
+  }
+  for (int r = rank * kNt + tid; r < R; r += nct * kNt) {
     const int len = s_len[r], left = s_left[r];
     a.lens_out[r] = flags != 0 ? len : left;
     if (flags == 0 && a.evicted != nullptr && left < len) a.evicted[r] += len - left;
   }
   if (rank == 0 && tid < FD_TABLES_HEADER_LEN) {
-    const int freed0 = (int)(end0 - c0_in), freed1 = (int)(end1 - c1_in);
-    a.header[tid] = tid == FD_TABLES_FLAGS         ? flags
-                    : flags != 0                   ? 0
-                    : tid == FD_TABLES_FREED_HBM   ? freed0
-                    : tid == FD_TABLES_FREED_HOST  ? freed1
-                    : tid == FD_TABLES_MAX_SEQ     ? shared_max
-                                                   : 0;
+    a.header[tid] = tid == FD_TABLES_FLAGS        ? flags
+                    : flags != 0                  ? 0
+                    : tid == FD_TABLES_FREED_HBM  ? (int)(end0 - c0_in)
+                    : tid == FD_TABLES_FREED_HOST ? (int)(end1 - c1_in)
+                    : tid == FD_TABLES_MAX_SEQ    ? shared_max
+                                                  : 0;
     if (tid < 2) a.counts_out[tid] = flags != 0 ? (tid == 0 ? c0_in : c1_in) : (int)(tid == 0 ? end0 : end1);
     if (tid == 0 && flags != 0) set_error(a.error, FD_DEVERR_TABLES);
-  }
-  if (flags != 0) return;
-  const unsigned below = (1u << lane) - 1u;
-  for (int base = lo; base < hi; base += kTrimPass) {
-    if (!one) {
-      load(base + warp * kTrimIds * 32);
-      const int m0 = count(true), m1 = count(false);
-      __syncthreads();  // the last pass's counts have been read
-      if (lane == 0) {
-        warp_n[0][warp] = m0;
-        warp_n[1][warp] = m1;
-      }
-      __syncthreads();
-    }
-    int p0 = 0, p1 = 0;  // of the warps ahead, then of the whole pass
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) {
-        n0 = p0;
-        n1 = p1;
-      }
-      p0 += warp_n[0][w];
-      p1 += warp_n[1][w];
-    }
-#pragma unroll
-    for (int u = 0; u < kTrimIds; ++u) {
-      const bool in = id[u] >= 0, hbm = id[u] < a.num_gpu_blocks;
-      const unsigned in0 = __ballot_sync(0xffffffffu, in && hbm), in1 = __ballot_sync(0xffffffffu, in && !hbm);
-      if (in && hbm) a.free_ids[0][at0 + n0 + __popc(in0 & below)] = id[u];
-      if (in && !hbm) a.free_ids[1][at1 + n1 + __popc(in1 & below)] = id[u];
-      n0 += __popc(in0);
-      n1 += __popc(in1);
-    }
-    at0 += p0;
-    at1 += p1;
   }
 }
 
@@ -694,17 +713,23 @@ extern "C" int fd_trim_tables(const fd_trim_args* a, void* stream) {
     if (a->free_cap[t] < 0 || (a->free_cap[t] > 0 && a->free_ids[t] == nullptr))
       return fdh::fail(FD_ERR_INVALID, "fd_trim_tables: free stack %d has a capacity but no memory", t);
   const bool pow2 = (a->block_size & (a->block_size - 1)) == 0;
-  static unsigned long long done[2] = {0, 0};
-  const void* kern = pow2 ? reinterpret_cast<const void*>(fd_trim_kernel<true>)
-                          : reinterpret_cast<const void*>(fd_trim_kernel<false>);
-  const int st = fdh::ensure_smem(kern, (4 * FD_TABLES_MAX_REQS + 1) * 4, &done[pow2 ? 1 : 0]);
-  if (st != FD_OK) return st;
   int64_t most = a->bt_width;  // blocks that a request can lose
   if (a->max_cut > 0 && a->max_cut / a->block_size + 1 < most) most = a->max_cut / a->block_size + 1;
-  const int ctas = most * a->num_reqs <= kTrimOneCta ? 1 : kCluster;
+  most *= a->num_reqs;
+  const int ctas = most <= kTrimOneCta ? 1 : kCluster;
+  const bool small = ctas == 1 && most <= kTrimSmall * kTrimIds && a->num_reqs <= 4 * kTrimSmall;
+  static unsigned long long done[4] = {0, 0, 0, 0};
+  const void* const kerns[4] = {reinterpret_cast<const void*>(fd_trim_kernel<false, kThreads>),
+                                reinterpret_cast<const void*>(fd_trim_kernel<true, kThreads>),
+                                reinterpret_cast<const void*>(fd_trim_kernel<false, kTrimSmall>),
+                                reinterpret_cast<const void*>(fd_trim_kernel<true, kTrimSmall>)};
+  const int which = (small ? 2 : 0) + (pow2 ? 1 : 0);
+  const void* kern = kerns[which];
+  const int st = fdh::ensure_smem(kern, (4 * FD_TABLES_MAX_REQS + 1) * 4, &done[which]);
+  if (st != FD_OK) return st;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)ctas);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(small ? kTrimSmall : kThreads);
   cfg.dynamicSmemBytes = (size_t)(4 * a->num_reqs + 1) * 4;
   cfg.stream = static_cast<cudaStream_t>(stream);
   cudaLaunchAttribute attr[1];
