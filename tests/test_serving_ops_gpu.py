@@ -731,3 +731,406 @@ def test_verify_draws_by_the_probabilities():
     ok()
     got = torch.bincount(v.tokens[:, 0].cpu(), minlength=V).double()
     assert bool(((got - R * p.double()).abs() <= 5 * (R * p * (1 - p)).double().sqrt()).all())
+
+
+# ------------------------------------------------------------------ refusals that need a device's tensors
+
+
+def test_calls_refuse_mismatched_tensors():
+    pg = Paged([40, 50], 2, 16, 64, torch.float16, seed=1)
+    stats, q = pg.stats(), torch.randn(2, 4, 64).half().cuda()
+    lse, one = torch.zeros(4, 2, device="cuda"), i32([1, 1])
+
+    def weights(**k):
+        a = dict(q=q, tiers=pg.tiers, tier_split=pg.G, block_table=pg.table, q_start=i32([0, 1]), q_len=one, k_len=i32([40, 50]),
+                 scale=0.125, lse=lse, stats=stats)
+        a.update(k)
+        gpu_ops.key_weights(**a)
+
+    weights()
+    ok()
+    with pytest.raises(RuntimeError, match="lse"):
+        weights(lse=lse.T)
+    with pytest.raises(RuntimeError, match="lse"):
+        weights(lse=lse.double())
+    with pytest.raises(RuntimeError, match="q_len"):
+        weights(q_len=one.long())
+    with pytest.raises(RuntimeError, match="evicted"):
+        weights(evicted=one[:1])
+    with pytest.raises(RuntimeError, match="stats"):
+        weights(stats=KeyStats.zeros(pg.G, 2, 8, dev()))
+    with pytest.raises(RuntimeError, match="head size"):
+        weights(q=q[..., :32])
+    with pytest.raises(RuntimeError, match="workspace_buf"):
+        weights(q=q.expand(2, 4, 64).repeat(1000, 1, 1), lse=torch.zeros(4, 2000, device="cuda"), max_q_len=0,
+                workspace_buf=torch.zeros(16, dtype=torch.uint8, device="cuda"))
+    m = KeyMoves(2, 2, 30, dev())
+    with pytest.raises(RuntimeError, match="keep_lens"):
+        gpu_ops.select_keys(stats, pg.table, i32([40, 50]), i32([20]), m)
+    with pytest.raises(RuntimeError, match="moves"):
+        gpu_ops.select_keys(stats, pg.table, i32([40, 50]), i32([20, 20]), KeyMoves(1, 2, 30, dev()))
+    with pytest.raises(RuntimeError, match="moves"):
+        gpu_ops.move_keys(KeyMoves(2, 3, 30, dev()), pg.tiers, pg.G, pg.table)
+    with pytest.raises(RuntimeError, match="at least one KV tier"):
+        gpu_ops.move_keys(m, (None, None), pg.G, pg.table)
+    with pytest.raises(RuntimeError, match="too small"):
+        gpu_ops.trim_tables(i32([1, 1]), i32([40, 50]), pg.table, FreeBlocks(i32([0] * 9), None, i32([0, 0])), pg.G, 0, 16,
+                            TrimTables(1, dev()))
+    p, e = torch.rand(4, 10, device="cuda"), torch.zeros(2, 1, device="cuda")
+    t, u = torch.zeros(2, 1, dtype=torch.int64, device="cuda"), torch.zeros(2, device="cuda")
+    for bad, match in (((p, t.int(), None, one, one, e, u), "draft_tokens"), ((p, t, torch.rand(2, 1, 11, device="cuda"), one, one, e, u), "draft_probs"),
+                       ((p, t, torch.rand(2, 1, 10, device="cuda").half(), one, one, e, u), "draft_probs"),
+                       ((p, t, None, one, one, e[:1], u), "accept_u"), ((p, t, None, one, one, e, u[:1]), "sample_u"),
+                       ((p.T, t, None, one, one, e, u), "target_probs"), ((p, t, None, one[:1], one, e, u), "q_start")):
+        with pytest.raises(RuntimeError, match=match):
+            gpu_ops.verify_drafts(*bad)
+    with pytest.raises(RuntimeError, match="DraftVerdict"):
+        gpu_ops.verify_drafts(p, t, None, one, one, e, u, out=DraftVerdict(2, 2, dev()))
+
+
+def test_default_buffers():
+    """Calls without buffers of the caller's make their own."""
+    lens, keep = [100, 90], [30, 90]
+    _, stats, m, w, p, gone = _select(lens, keep)
+    pg = Paged(lens, 2, 16, 8, torch.float32, seed=0)
+    m2 = gpu_ops.select_keys(stats, pg.table, i32(lens), i32(keep), evicted=i32(gone), max_k_len=100)
+    assert m2.room == 50 and torch.equal(m2.counts, m.counts)
+    c = int(m.counts[0, 0])
+    assert torch.equal(m2.src[0, 0, :c], m.src[0, 0, :c]) and torch.equal(m2.dst[0, 0, :c], m.dst[0, 0, :c])
+    t = gpu_ops.trim_tables(i32(keep), i32(lens), pg.table, FreeBlocks(i32([0] * 20), None, i32([0, 0])), pg.G, 0, 16)
+    assert t.seq_lens.tolist() == [30, 90] and t.counts.tolist() == [5, 0]
+    ok()
+
+
+# ------------------------------------------------------------------ places past 32 bits
+
+
+def test_places_past_32_bits():
+    """Block ids whose cache and stats offsets (in elements) pass 2^31."""
+    KVH, BS, D = 8, 64, 128
+    blocks = (1 << 31) // (KVH * BS * 2) + 7              # stats: [2^31 / 1024, 8, 64], cache: a view that strides far apart
+    stats = KeyStats(torch.empty(2 * blocks, KVH, BS, device="cuda"), torch.empty(2 * blocks, KVH, BS, dtype=torch.int32, device="cuda"))
+    few = 40
+    far = (1 << 32) // (few - 1) // 8 * 8
+    store = torch.empty(far * (few - 1) + KVH * BS * D, dtype=torch.bfloat16, device="cuda")
+    k = store.as_strided((few, KVH, BS, D), (far, BS * D, D, 1))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    k.copy_(torch.randn(few, KVH, BS, D, generator=g, device="cuda"))
+    before = k.clone()
+    top = 2 * blocks - few
+    ids = [top + 37, top + 2, top + 39, top + 20]          # HBM ids: all below the split; the tier begins at id 0, so shift it
+    base = KVTier(k, k)
+    n, keep, H = 250, 100, 16
+    q = torch.randn(3, H, D, generator=g, device="cuda").bfloat16()
+    table = i32([[37, 2, 39, 20, 5]])
+    keys = torch.cat([before[b].transpose(0, 1) for b in (37, 2, 39, 20)])[:n]
+    lse = _lse(q, [keys], [3], D ** -0.5)
+    stats.weights[:few].zero_()
+    gpu_ops.key_weights(q, (base, None), few, table, i32([0]), i32([3]), i32([n]), D ** -0.5, lse, stats, max_q_len=3, max_k_len=n)
+    ok()
+    w, e = ref.key_weights(q, keys, lse, torch.zeros(KVH, n, device="cuda"), D ** -0.5)
+    got = torch.stack([stats.weights[b] for b in (37, 2, 39, 20)], 1).flatten(1, 2)[:, :n].double()
+    assert bool(((got - w).abs() <= e).all())
+    # the same weights at the far end of the stats decide there
+    for b, i in zip((37, 2, 39, 20), ids):
+        stats.weights[i], stats.positions[i] = stats.weights[b], 5
+    m = gpu_ops.select_keys(stats, i32([ids]), i32([n]), i32([keep]), KeyMoves(1, KVH, keep, dev()))
+    ok()
+    for h in range(KVH):
+        a, b = ref.select(got[h].tolist(), [5] * n, n, keep, 0, 0, 0)
+        c = int(m.counts[0, h])
+        assert m.src[0, h, :c].tolist() == a and m.dst[0, h, :c].tolist() == b
+    gpu_ops.move_keys(m, (base, None), few, table)
+    ok()
+    flat = lambda x, h: torch.cat([x[b, h] for b in (37, 2, 39, 20)])  # noqa: E731
+    for h in range(KVH):
+        c = int(m.counts[0, h])
+        at = torch.arange(4 * BS, device="cuda")
+        at[m.dst[0, h, :c].long()] = m.src[0, h, :c].long()
+        assert torch.equal(flat(k, h), flat(before, h)[at])
+
+
+# ------------------------------------------------------------------ streams and graphs
+
+
+def _far_apart():
+    """One call of each operator on buffers of its own; returns (call, results)."""
+    pg = Paged([3000, 700], 4, 16, 128, torch.bfloat16, seed=21)
+    g = torch.Generator().manual_seed(5)
+    q = torch.randn(800, 16, 128, generator=g).bfloat16().cuda()
+    lse = _lse(q, pg.keys, [500, 300], 128 ** -0.5)
+    stats = pg.stats(4)
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    start, ql, kl, keep = i32([0, 500]), i32([500, 300]), i32([3000, 700]), i32([900, 100])
+    m = KeyMoves(2, 4, 900, dev())
+    st, ct = i32([[-1] * 300] * 2), i32([0, 0])
+    tt = TrimTables(2, dev())
+    tp, dp = _probs(g, 6, 5000).cuda(), _probs(g, 2, 2, 5000).cuda()
+    toks, au, su = torch.randint(0, 5000, (2, 2), generator=g).cuda(), torch.rand(2, 2, generator=g).cuda(), torch.rand(2, generator=g).cuda()
+    v = DraftVerdict(2, 2, dev())
+    k0, v0 = pg.tiers[0].k.clone(), pg.tiers[0].v.clone()
+    vs, vl = i32([0, 3]), i32([3, 3])
+
+    def call():
+        stats.weights.copy_(w0)
+        stats.positions.copy_(p0)
+        pg.tiers[0].k.copy_(k0)
+        pg.tiers[0].v.copy_(v0)
+        gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, start, ql, kl, 128 ** -0.5, lse, stats)
+        gpu_ops.select_keys(stats, pg.table, kl, keep, m, recent=50)
+        gpu_ops.move_keys(m, pg.tiers, pg.G, pg.table, stats)
+        gpu_ops.trim_tables(keep, kl, pg.table, FreeBlocks(st[0], st[1], ct), pg.G, pg.C, 16, tt)
+        gpu_ops.verify_drafts(tp, toks, dp, vs, vl, au, su, seq_lens=kl, out=v)
+
+    return call, [stats.weights, stats.positions, pg.tiers[0].k, pg.tiers[0].v, m.src, m.dst, m.counts, st, tt.seq_lens, tt.counts, v.tokens,
+                  v.accepted, v.keep_lens]
+
+
+def _same(a, b):
+    return all(torch.equal(x.view(torch.int16) if x.dtype == torch.bfloat16 else x, y.view(torch.int16) if y.dtype == torch.bfloat16 else y)
+               for x, y in zip(a, b))
+
+
+def test_two_graphs_and_streams_do_not_share_anything():
+    """Two captured graphs replayed on two streams at once, and eager calls on a third: all as the first eager call."""
+    call, res = _far_apart()
+    call()
+    torch.cuda.synchronize()
+    ok()
+    want = [x.clone() for x in res]
+    sides = []
+    for _ in range(2):
+        c, r = _far_apart()
+        c()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            c()
+        sides.append((graph, r, torch.cuda.Stream()))
+    third = torch.cuda.Stream()
+    for _ in range(20):
+        for graph, _, s in sides:
+            with torch.cuda.stream(s):
+                graph.replay()
+        with torch.cuda.stream(third):
+            call()
+    torch.cuda.synchronize()
+    ok()
+    assert _same(res, want) and all(_same(r, want) for _, r, _ in sides)
+
+
+# ------------------------------------------------------------------ a run of them together
+
+
+class Serving:
+    """Requests whose drafted tokens are verified and whose caches are kept within a budget, one layer."""
+
+    def __init__(self, seed, budget=48, over=8):
+        self.R, self.K, self.KVH, self.H, self.D, self.BS, self.V = 4, 3, 2, 8, 64, 16, 50
+        self.budget, self.over, self.sinks, self.recent = budget, over, 2, budget // 3
+        self.G, self.C = 20, 24
+        g = torch.Generator().manual_seed(seed)
+        shape = (self.KVH, self.BS, self.D)
+        cache = torch.zeros(self.G, *shape, dtype=torch.float16, device="cuda")
+        host = [torch.zeros(self.C, *shape, dtype=torch.float16).pin_memory() for _ in range(2)]
+        self.tiers = (KVTier(cache, cache.clone()), KVTier(*host))
+        self.table = torch.zeros(self.R, 12, dtype=torch.int32, device="cuda")
+        self.stack = torch.zeros(2, self.G + self.C, dtype=torch.int32, device="cuda")
+        self.stack[0, :self.G] = torch.randperm(self.G, generator=g).int().cuda()
+        self.stack[1, :self.C] = (torch.randperm(self.C, generator=g) + self.G).int().cuda()
+        self.counts = i32([self.G, self.C])
+        self.free = FreeBlocks(self.stack[0], self.stack[1], self.counts)
+        self.lens, self.gone = i32([0] * self.R), i32([0] * self.R)
+        self.T = self.R * 40
+        self.t = StepTables(self.R, self.T, "cuda", seq_lens=self.lens, counts=self.counts)
+        self.trim = TrimTables(self.R, "cuda", seq_lens=self.lens, counts=self.counts)
+        self.stats = KeyStats.zeros(self.G + self.C, self.KVH, self.BS, "cuda")
+        self.moves = KeyMoves(self.R, self.KVH, self.budget, "cuda")
+        self.verdict = DraftVerdict(self.R, self.K, "cuda")
+        ang = torch.outer(torch.arange(4096, dtype=torch.float64), 100.0 ** (-torch.arange(0, self.D, 2).double() / self.D))
+        self.cos_sin = torch.cat([ang.cos(), ang.sin()], 1).float().cuda()
+        z = lambda *n: torch.zeros(n, dtype=torch.float16, device="cuda")  # noqa: E731
+        self.q, self.k, self.v = z(self.T, self.H, self.D), z(self.T, self.KVH, self.D), z(self.T, self.KVH, self.D)
+        self.out, self.lse = z(self.T, self.H, self.D), torch.zeros(self.H, self.T, device="cuda")
+        self.new, self.drafts = i32([0] * self.R), torch.zeros(self.R, self.K, dtype=torch.int64, device="cuda")
+        self.target, self.probs = torch.zeros(self.T, self.V, device="cuda"), torch.zeros(self.R, self.K, self.V, device="cuda")
+        self.au, self.su = torch.zeros(self.R, self.K, device="cuda"), torch.zeros(self.R, device="cuda")
+        self.used, self.kept = i32([0] * self.R), i32([0] * self.R)
+
+    def fill(self, step):
+        g = torch.Generator().manual_seed(1000 + step)
+        new = [30, 25, 0, 40] if step == 0 else [4, 0, 30, 4] if step == 1 else [4, -1, 2, 4] if step == 9 else [4, 3, 4, 1]
+        if step == 10:
+            new[1] = 35
+        self.new.copy_(i32(new))
+        for x in (self.q, self.k, self.v):
+            x.copy_(torch.randn(x.shape, generator=g))
+        p = _probs(g, self.T, self.V, spread=1.0)
+        self.target.copy_(p)
+        at = 0
+        for r, n in enumerate(new):
+            if 1 <= n <= self.K + 1:
+                for d in range(n - 1):
+                    self.probs[r, d] = (0.6 * p[at + d] + 0.4 * _probs(g, self.V, spread=1.0)).cuda()
+            at += max(0, n)
+        self.drafts.copy_(torch.randint(0, self.V, self.drafts.shape, generator=g))
+        self.au.copy_(torch.rand(self.au.shape, generator=g) * 0.5)
+        self.su.copy_(torch.rand(self.su.shape, generator=g))
+        return new
+
+    def attend(self):
+        t = self.t
+        gpu_ops.extend_tables(self.new, self.lens, self.table, self.free, self.G, self.C, self.BS, t, evicted=self.gone)
+        gpu_ops.rope_store_kv(self.q, self.k, self.v, t.positions, self.cos_sin, t.slot_mapping, self.tiers, self.G)
+        gpu_ops.chunk_attn(self.q, self.tiers, self.G, self.table, t.query_start_loc[:-1], t.query_lens, self.lens, self.D ** -0.5,
+                           self.out, self.lse, max_q_len=40, max_k_len=180)
+
+    def verify(self):
+        # a prompt's step has no drafts: it samples from its last row
+        ql, start = self.t.query_lens, self.t.query_start_loc[:-1]
+        prompt = ql > self.K + 1
+        first = torch.where(prompt, start + ql - 1, start)
+        rows = torch.where(prompt, 1, ql)
+        v = gpu_ops.verify_drafts(self.target, self.drafts, self.probs, first, rows, self.au, self.su, seq_lens=self.lens,
+                                  out=self.verdict)
+        self.used.copy_(torch.where(prompt | (ql == 0), ql, v.accepted + 1))
+        gpu_ops.trim_tables(v.keep_lens, self.lens, self.table, self.free, self.G, self.C, self.BS, self.trim, max_cut=self.K)
+        gpu_ops.key_weights(self.q, self.tiers, self.G, self.table, start, self.used, self.lens, self.D ** -0.5, self.lse, self.stats,
+                            evicted=self.gone, max_q_len=40, max_k_len=180)
+
+    def cut(self):
+        self.kept.copy_(torch.where(self.lens > self.budget + self.over, self.budget, self.lens))
+        gpu_ops.select_keys(self.stats, self.table, self.lens, self.kept, self.moves, sinks=self.sinks, recent=self.recent,
+                            evicted=self.gone, max_k_len=180)
+        gpu_ops.move_keys(self.moves, self.tiers, self.G, self.table, self.stats)
+        gpu_ops.trim_tables(self.kept, self.lens, self.table, self.free, self.G, self.C, self.BS, self.trim, evicted=self.gone)
+
+    def step(self):
+        self.attend()
+        self.verify()
+        self.cut()
+
+    def state(self):
+        return [self.tiers[0].k, self.tiers[0].v, self.tiers[1].k, self.tiers[1].v, self.table, self.stack, self.counts, self.lens, self.gone,
+                self.stats.weights, self.stats.positions, self.verdict.tokens, self.verdict.accepted, self.out, self.lse]
+
+    def cached(self, r, n):
+        """K, V [KVH, n, D], weights and positions [KVH, n] of request r."""
+        torch.cuda.synchronize()
+        ids = self.table[r].tolist()[:-(-n // self.BS)]
+        blk = lambda t, u, b: t[b] if b < self.G else u[b - self.G].cuda()  # noqa: E731
+        k, v = (torch.cat([blk(a, b, i) for i in ids], 1)[:, :n] if n else a[0][:, :0]
+                for a, b in ((self.tiers[0].k, self.tiers[1].k), (self.tiers[0].v, self.tiers[1].v)))
+        w, p = (torch.cat([x[i] for i in ids], 1)[:, :n] if n else x[0][:, :0] for x in (self.stats.weights, self.stats.positions))
+        return k, v, w, p
+
+
+@pytest.mark.parametrize("budget,over,least", [(48, 8, 2), (24, 0, 12)])
+def test_serving_steps_against_lists(budget, over, least):
+    """Twelve steps: attention over what stayed, accepted drafts, budgets, blocks; each against a plain account of every key."""
+    s = Serving(3, budget, over)
+    held = [[{} for _ in range(s.KVH)] for _ in range(s.R)]  # per head: position -> (k, v, weight)
+    total = [0] * s.R                                        # tokens that a request has had
+    cuts = 0
+    for step in range(12):
+        new = s.fill(step)
+        s.attend()
+        ok()
+        s.t.read_header()
+        for r in range(s.R):
+            if new[r] < 0:
+                held[r], total[r], new[r] = [{} for _ in range(s.KVH)], 0, 0
+        start = [sum(new[:r]) for r in range(s.R)]
+        assert s.t.positions.tolist()[:sum(new)] == [total[r] + i for r in range(s.R) for i in range(new[r])]
+        n_before = s.lens.tolist()
+        for r in range(s.R):
+            n = n_before[r]
+            assert n == len(held[r][0]) + new[r]
+            if new[r] == 0:
+                continue
+            k, v, _, _ = s.cached(r, n)
+            q = s.q[start[r]:start[r] + new[r]].double()
+            for h in range(s.H):
+                g = h // (s.H // s.KVH)
+                old = [held[r][g][p] for p in sorted(held[r][g])]
+                kk = torch.cat([torch.stack([x[0] for x in old]), k[g, n - new[r]:]]) if old else k[g]
+                vv = torch.cat([torch.stack([x[1] for x in old]), v[g, n - new[r]:]]) if old else v[g]
+                sc = q[:, h] @ kk.double().T * s.D ** -0.5
+                sc = sc.masked_fill(torch.arange(n, device="cuda") > (n - new[r] + torch.arange(new[r], device="cuda"))[:, None], -math.inf)
+                o = sc.softmax(-1) @ vv.double()
+                # P and the result are rounded to fp16, half a step of 2^-11 each, of |v| below 5; scores in fp32
+                assert float((s.out[start[r]:start[r] + new[r], h].double() - o).abs().max()) <= 2 * 2.0 ** -11 * 5 + 1e-4
+                assert float((s.lse[h, start[r]:start[r] + new[r]].double() - sc.logsumexp(-1)).abs().max()) <= 1e-4
+        fresh = [s.cached(r, n_before[r])[:2] for r in range(s.R)]
+        s.verify()
+        ok()
+        t64, used = s.target.double().tolist(), s.used.tolist()
+        for r in range(s.R):
+            if new[r] == 0:
+                assert s.verdict.tokens[r].tolist() == [-1] * (s.K + 1) and used[r] == 0
+                continue
+            prompt = new[r] > s.K + 1
+            got, a = ref.verify(t64, s.drafts[r].tolist(), s.probs[r].double().tolist(), start[r] + new[r] - 1 if prompt else start[r],
+                                1 if prompt else new[r], s.au[r].double().tolist(), float(s.su[r]))
+            assert s.verdict.tokens[r].tolist() == got + [-1] * (s.K + 1 - len(got))
+            assert used[r] == (new[r] if prompt else a + 1)
+        lens = s.lens.tolist()
+        for r in range(s.R):
+            assert lens[r] == n_before[r] - new[r] + used[r]
+            if used[r] == 0:
+                continue
+            k, v, w, p = s.cached(r, lens[r])
+            for g in range(s.KVH):
+                old = {x: held[r][g][x][2] for x in held[r][g]}
+                pos = p[g].tolist()
+                assert sorted(pos) == sorted(old) + [total[r] + i for i in range(used[r])]
+                before = torch.tensor([old.get(x, 0.0) for x in pos], device="cuda")
+                qh = s.q[start[r]:start[r] + used[r], g * 4:(g + 1) * 4]
+                want, tol = ref.key_weights(qh, k[g][:, None], s.lse[g * 4:(g + 1) * 4, start[r]:start[r] + used[r]], before[None], s.D ** -0.5)
+                assert bool(((w[g].double() - want[0]).abs() <= tol[0]).all())
+                assert torch.equal(k[g, lens[r] - used[r]:], fresh[r][0][g, n_before[r] - new[r]:n_before[r] - new[r] + used[r]])
+                held[r][g] = {x: (k[g, j].clone(), v[g, j].clone(), float(w[g, j])) for j, x in enumerate(pos)}
+            total[r] += used[r]
+        gone = s.gone.tolist()
+        s.cut()
+        ok()
+        for r in range(s.R):
+            n, keep = lens[r], s.budget if lens[r] > s.budget + s.over else lens[r]
+            assert s.lens.tolist()[r] == keep and s.gone.tolist()[r] == gone[r] + n - keep == total[r] - keep
+            cuts += keep < n
+            k, v, w, p = s.cached(r, keep)
+            for g in range(s.KVH):
+                if keep < n:
+                    guard = {x for x in held[r][g] if x < s.sinks or x >= total[r] - s.recent}
+                    rest = sorted((x for x in held[r][g] if x not in guard), key=lambda x: -held[r][g][x][2])
+                    ws = [held[r][g][x][2] for x in rest]
+                    assert len(set(ws)) == len(ws)  # (no ties: which of two stays depends on their places)
+                    held[r][g] = {x: held[r][g][x] for x in guard | set(rest[:keep - len(guard)])}
+                pos = p[g].tolist()
+                assert sorted(pos) == sorted(held[r][g])
+                for j, x in enumerate(pos):
+                    assert torch.equal(k[g, j], held[r][g][x][0]) and torch.equal(v[g, j], held[r][g][x][1])
+                    assert float(w[g, j]) == held[r][g][x][2]
+        # every block is on a stack or in a table once
+        c = s.counts.tolist()
+        used_ids = [b for r in range(s.R) for b in s.table[r].tolist()[:-(-s.lens.tolist()[r] // s.BS)]]
+        assert sorted(used_ids + s.stack[0, :c[0]].tolist() + s.stack[1, :c[1]].tolist()) == list(range(s.G + s.C))
+    assert cuts >= least
+
+
+def test_serving_steps_in_one_graph():
+    """The whole step captured once and replayed gives what eager steps give, bit for bit."""
+    a, b = Serving(3), Serving(3)
+    a.fill(0), b.fill(0)
+    a.step(), b.step()  # (warm: lazy loading does not fall into the capture)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        b.step()
+    for step in range(1, 12):
+        a.fill(step), b.fill(step)
+        a.step()
+        graph.replay()
+        ok()
+        for x, y in zip(a.state(), b.state()):
+            assert torch.equal(x, y), step

@@ -870,17 +870,33 @@ def extend_tables(new_lens: torch.Tensor, prior_lens: torch.Tensor, block_table:
     return out
 
 
-class TrimTables:
+class _Buffers:
+    """int32 buffers of one device, checked when they are made (a call then only
+    takes their addresses), so their names are not to be bound again."""
+
+    def __init__(self, device, **buffers):
+        made = {k: v if isinstance(v, torch.Tensor) else torch.zeros(v, dtype=torch.int32, device=device)
+                for k, (v, _) in buffers.items()}
+        idx = next(iter(made.values())).get_device()
+        for name, t in made.items():
+            need = buffers[name][1]
+            if t.dtype is not torch.int32 or t.get_device() != idx or t.numel() < need or not t.is_contiguous():
+                raise RuntimeError(f"{name} must be a contiguous int32 tensor of at least {need} entries on one device with the others")
+        self.__dict__.update(made, idx=idx)
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{type(self).__name__}.{name} is not to be bound again: make a new {type(self).__name__}")
+
+
+class TrimTables(_Buffers):
     """Device buffers that trim_tables fills for up to R requests: the lengths
     after it, the free stacks' counts and the header.  seq_lens and counts may
     be the caller's own tensors, to step them in place."""
 
     def __init__(self, R: int, device, seq_lens: torch.Tensor | None = None, counts: torch.Tensor | None = None):
-        z = lambda n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
-        self.R = int(R)
-        self.seq_lens = z(R) if seq_lens is None else seq_lens
-        self.counts = z(2) if counts is None else counts
-        self.header = z(nat.TABLES_HEADER_LEN)
+        super().__init__(device, seq_lens=(R if seq_lens is None else seq_lens, R), counts=(2 if counts is None else counts, 2),
+                         header=(nat.TABLES_HEADER_LEN, nat.TABLES_HEADER_LEN))
+        self.__dict__["R"] = int(R)
 
     def read_header(self) -> dict[str, int]:
         """The header by name (synchronises); raises if the call was refused."""
@@ -907,15 +923,15 @@ def trim_tables(keep_lens: torch.Tensor, seq_lens: torch.Tensor, block_table: to
     idx, R, W = _block_table(block_table)
     if out is None:
         out = TrimTables(R, block_table.device)
-    if out.R < R or out.header.get_device() != idx:
+    if out.R < R or out.idx != idx:
         raise RuntimeError("out is too small, or on another device")
     hbm, host, counts = free.hbm, free.host, free.counts
     packed = _TRIM_STRUCT.pack(
-        _i32(keep_lens, idx, R, "keep_lens"), _i32(seq_lens, idx, R, "seq_lens"), _i32(out.seq_lens, idx, R, "out.seq_lens"),
+        _i32(keep_lens, idx, R, "keep_lens"), _i32(seq_lens, idx, R, "seq_lens"), out.seq_lens.data_ptr(),
         0 if evicted is None else _i32(evicted, idx, R, "evicted"), block_table.data_ptr(), block_table.stride(0), W, R,
         0 if hbm is None else _i32(hbm, idx, 0, "free.hbm"), 0 if host is None else _i32(host, idx, 0, "free.host"),
         0 if hbm is None else hbm.numel(), 0 if host is None else host.numel(), _i32(counts, idx, 2, "free.counts"),
-        _i32(out.counts, idx, 2, "out.counts"), num_gpu_blocks, num_cpu_blocks, block_size, max_cut, out.header.data_ptr(),
+        out.counts.data_ptr(), num_gpu_blocks, num_cpu_blocks, block_size, max_cut, out.header.data_ptr(),
         _error_ptr(idx))
     _launch(nat.load().fd_trim_tables, packed, idx, "fd_trim_tables")
     return out
@@ -1147,7 +1163,7 @@ class KeyStats:
         return w.data_ptr(), self.positions.data_ptr(), B
 
 
-class KeyMoves:
+class KeyMoves(_Buffers):
     """Device buffers that select_keys fills and move_keys reads, for R requests
     of KVH kv heads and up to `room` moves each: src and dst int32 [R, KVH,
     room], counts int32 [R, KVH].  A request cut from n keys to b needs room for
@@ -1155,18 +1171,16 @@ class KeyMoves:
 
     def __init__(self, R: int, KVH: int, room: int, device, src: torch.Tensor | None = None,
                  dst: torch.Tensor | None = None, counts: torch.Tensor | None = None):
-        z = lambda *n: torch.zeros(n, dtype=torch.int32, device=device)  # noqa: E731
-        self.R, self.KVH, self.room = int(R), int(KVH), int(room)
-        self.src = z(R, KVH, room) if src is None else src
-        self.dst = z(R, KVH, room) if dst is None else dst
-        self.counts = z(R, KVH) if counts is None else counts
+        lists = (R, KVH, room)
+        super().__init__(device, src=(lists if src is None else src, R * KVH * room),
+                         dst=(lists if dst is None else dst, R * KVH * room),
+                         counts=((R, KVH) if counts is None else counts, R * KVH))
+        self.__dict__.update(R=int(R), KVH=int(KVH), room=int(room))
 
     def _fields(self, idx: int, R: int, KVH: int) -> tuple:
-        if self.KVH != KVH or self.R < R:
-            raise RuntimeError("moves must be of at least R requests and of KVH kv heads")
-        n = R * KVH * self.room
-        return (_i32(self.src, idx, n, "moves.src"), _i32(self.dst, idx, n, "moves.dst"),
-                _i32(self.counts, idx, R * KVH, "moves.counts"))
+        if self.KVH != KVH or self.R < R or self.idx != idx:
+            raise RuntimeError("moves must be of at least R requests and of KVH kv heads, on the call's device")
+        return self.src.data_ptr(), self.dst.data_ptr(), self.counts.data_ptr()
 
 
 def key_weights(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tier_split: int, block_table: torch.Tensor,
@@ -1247,16 +1261,14 @@ def move_keys(moves: KeyMoves, tiers: tuple[KVTier | None, KVTier | None], tier_
     _launch(nat.load().fd_move_keys, packed, idx, "fd_move_keys")
 
 
-class DraftVerdict:
+class DraftVerdict(_Buffers):
     """Device buffers that verify_drafts fills for R requests of up to K drafted
     tokens: tokens int64 [R, K + 1] (the accepted drafts, the token that
     follows, then -1), accepted int32 [R], keep_lens int32 [R]."""
 
     def __init__(self, R: int, K: int, device):
-        self.R, self.K = int(R), int(K)
-        self.tokens = torch.full((R, K + 1), -1, dtype=torch.int64, device=device)
-        self.accepted = torch.zeros(R, dtype=torch.int32, device=device)
-        self.keep_lens = torch.zeros(R, dtype=torch.int32, device=device)
+        super().__init__(device, accepted=(R, R), keep_lens=(R, R))
+        self.__dict__.update(R=int(R), K=int(K), tokens=torch.full((R, K + 1), -1, dtype=torch.int64, device=device))
 
 
 def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_probs: torch.Tensor | None,
@@ -1299,15 +1311,13 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_
         probs = (draft_probs.data_ptr(), draft_probs.stride(0), draft_probs.stride(1))
     if out is None:
         out = DraftVerdict(R, K, target_probs.device)
-    if (out.R < R or out.K != K or out.tokens.dtype is not torch.int64 or out.tokens.get_device() != idx
-            or not out.tokens.is_contiguous()):
+    if out.R < R or out.K != K or out.idx != idx:
         raise RuntimeError("out must be a DraftVerdict of at least R requests and of K drafts on target_probs' device")
     packed = _VERIFY_STRUCT.pack(
         target_probs.data_ptr(), target_probs.stride(0), *probs, draft_tokens.data_ptr(), draft_tokens.stride(0),
         _i32(q_start, idx, R, "q_start"), _i32(q_len, idx, R, "q_len"), accept_u.data_ptr(), accept_u.stride(0),
         sample_u.data_ptr(), 0 if seq_lens is None else _i32(seq_lens, idx, R, "seq_lens"), out.tokens.data_ptr(),
-        _i32(out.accepted, idx, R, "out.accepted"), _i32(out.keep_lens, idx, R, "out.keep_lens"), R, K, V, T, dtype_code(dt),
-        0, _error_ptr(idx))
+        out.accepted.data_ptr(), out.keep_lens.data_ptr(), R, K, V, T, dtype_code(dt), 0, _error_ptr(idx))
     _launch(nat.load().fd_verify_drafts, packed, idx, "fd_verify_drafts")
     return out
 
