@@ -351,8 +351,10 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
   int32_t* const src = a.src + (int64_t)unit * a.room;
   const unsigned below = (1u << lane) - 1u;
   for (int t0 = lo; t0 < hi; t0 += kTile) {
-    fetch(t0);
-    look(t0);
+    if (!(kMany && one)) {  // (else they are there from the count)
+      fetch(t0);
+      look(t0);
+    }
     // a running sum over the tile's groups of 32: group 16 u + warp is this warp's u-th
     int mine = 0;
 #pragma unroll

@@ -247,23 +247,26 @@ __global__ void __launch_bounds__(kThreads, 2) fd_verify_kernel(const __grid_con
   int owner = 0;
   while (owner < nct - 1 && !(target < before + part[attempt][owner])) before += part[attempt][owner++];
   if (owner != rank) return;
-  // the warp's span: where rounding leaves none past the target, the last one
-  // with any weight
-  int ws = 0;
-  double run = before, at_ws = before;
-  for (int w = 0; w < kWarps; ++w) {
-    const double s = warps[w];
-    if (!(s > 0.0)) continue;
-    ws = w;
-    at_ws = run;
-    run += s;
-    if (target < run) break;
+  // the warp's span: the first that passes the target, or, where rounding leaves
+  // none, the last one with any weight (every warp by itself)
+  const double own = lane < kWarps ? warps[lane] : 0.0;
+  double upto = before;
+  {
+    double incl = own;
+#pragma unroll
+    for (int off = 1; off < kWarps; off <<= 1) {
+      const double o = __shfl_up_sync(0xffffffffu, incl, off);
+      if (lane >= off) incl += o;
+    }
+    upto += incl;
   }
+  const unsigned some = __ballot_sync(0xffffffffu, own > 0.0), beyond = __ballot_sync(0xffffffffu, own > 0.0 && target < upto);
+  const int ws = beyond != 0u ? __ffs(beyond) - 1 : 31 - __clz(some);  // (some: the CTA's part is positive)
+  const double at_ws = __shfl_sync(0xffffffffu, upto - own, ws);
   // that span again, a vector per thread
   const long long from = cta_lo + cta_n * ws / kWarps;
   const long long to = cta_lo + cta_n * (ws + 1) / kWarps + (ws == kWarps - 1 && ntail > 0 ? 1 : 0);  // (the tail as a vector)
-  long long last = -1;  // the last element with weight so far
-  run = at_ws;
+  double run = at_ws;
   for (long long base = from; base < to; base += kThreads) {
     const long long i = base + tid;
     double w[kV], s = 0.0;
@@ -289,35 +292,38 @@ __global__ void __launch_bounds__(kThreads, 2) fd_verify_kernel(const __grid_con
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    double ahead = run;
-    for (int x = 0; x < kWarps; ++x) {
-      if (x < warp) ahead += scan[x];
-      run += scan[x];
+    double sums = lane < kWarps ? scan[lane] : 0.0;
+#pragma unroll
+    for (int off = 1; off < kWarps; off <<= 1) {
+      const double o = __shfl_up_sync(0xffffffffu, sums, off);
+      if (lane >= off) sums += o;
     }
+    const double to_here = __shfl_sync(0xffffffffu, sums, max(warp - 1, 0));
+    const double ahead = warp > 0 ? run + to_here : run;
+    run += __shfl_sync(0xffffffffu, sums, kWarps - 1);
     // threads with weight, of those the ones that pass the target
     const unsigned any = __ballot_sync(0xffffffffu, s > 0.0);
     const unsigned past = __ballot_sync(0xffffffffu, s > 0.0 && target < ahead + incl);
     if (lane == 0) s_found[warp] = past != 0u ? 64u + (unsigned)(__ffs(past) - 1) : any != 0u ? 32u + (31 - __clz(any)) : 0u;
     __syncthreads();
-    int pick = -1;
-    bool done = false;
-    for (int x = 0; x < kWarps && !done; ++x) {
-      const unsigned f = s_found[x];
-      if (f != 0u) pick = 32 * x + (int)(f & 31u);
-      done = f >= 64u;
-    }
+    const unsigned f = lane < kWarps ? s_found[lane] : 0u;
+    const unsigned hits = __ballot_sync(0xffffffffu, f >= 64u), full = __ballot_sync(0xffffffffu, f != 0u);
+    const bool done = hits != 0u;
+    const int w_at = done ? __ffs(hits) - 1 : 31 - __clz(full);  // -1: no weight in this pass
+    const int pick = w_at < 0 ? -1 : 32 * w_at + (int)(__shfl_sync(0xffffffffu, f, max(w_at, 0)) & 31u);
     if (pick == tid) {  // the vector's first element past the target, or its last one with weight
       double b = ahead + (incl - s);
       bool hit = false;
+      long long at = -1;
 #pragma unroll
       for (int e = 0; e < kV; ++e) {
         b += w[e];
         if (!hit && w[e] > 0.0) {
-          last = i * kV + e;
+          at = i * kV + e;
           hit = target < b;
         }
       }
-      a.tokens[(int64_t)r * (K + 1) + acc] = last;  // (a later pass with weight writes over it)
+      a.tokens[(int64_t)r * (K + 1) + acc] = at;  // (a later pass with weight writes over it)
     }
     if (done) return;
     __syncthreads();  // scan and s_found have been read; the write above is ordered before the next one
