@@ -9,23 +9,24 @@
 // bins, and the bin that holds T becomes the window, until few enough candidates
 // are left to rank each against all.  The first round tells exponents apart, the
 // second nine more bits; a third is seldom needed.  Then one running count in
-// index order, of the places that become
-// free and of the keys that move, gives each pair its place, so src and dst
-// ascend and no result depends on timing.  The keys are read once and stay in
+// index order, of the places that become free and of the keys that move, gives
+// each pair its place, so src and dst ascend and no result depends on timing.  The keys are read once and stay in
 // registers (in shared memory where a CTA has more than 4096), in one CTA, or
 // in a cluster that adds its counters up through distributed shared memory.
 // Bound by the latency of that chain (lengths, table, weights, then the
 // exchanges), not by its 8 bytes per key.
-// Measured: 32 requests x 8 heads of 2050 keys in 16.4 us, 4 x 8 of 11,000 to
-// 32,000 in 24.6.
+// Measured: 32 requests x 8 heads of 2050 keys, of which some hundred tie, in
+// 8.7 us; 4 x 8 of 11,000 to 32,000 in 16.0 on clusters of 8, of which a round
+// with its exchange takes 1.6 to 2.4.
 //
 // Move.  Only what lies behind the budget moves, into what goes before it, so
 // no pair reads what another writes, and the pairs are dealt out over the GPU
 // in any order.  A CTA takes kPairs pairs of one request and head at a time:
 // their rows' places first, then all 16-byte pieces of K and V, several per
 // thread in flight.  Bound by the bytes of the rows, read and written once.
-// Measured: 32 requests x 8 heads of up to 32 pairs of 512 bytes in 9.4 us, 4 x
-// 8 of 1500 in 16.4.
+// Measured: 32 requests x 8 heads of up to 32 pairs of 512 bytes in 3.9 us, 4 x
+// 8 of 1400 in 14.1 (48.8 MB, read and written in pieces of 512 bytes, at 3.5
+// TB/s).  A warp by itself with eight pairs at a time: 15.0.
 
 #include <cooperative_groups.h>
 

@@ -10,7 +10,8 @@
 // item's end.  The next rows are fetched into registers during the products.
 // Bound by the fp32 pipe, or, with few rows, by the loads of K.
 // Measured: 8 requests of up to 77 tokens over up to 512 keys, 8 heads x 64 of
-// fp32, in 17.1 us.
+// fp32, in 9.8 us (13.8 where each CTA looks for its work, 14.8 with the combine
+// as well).
 
 #include "fd_keyw.cuh"
 

@@ -22,7 +22,13 @@
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 32 single tokens of 32 heads over 512 to 8192 keys of 8 heads x 128
-// in 100 us; 2 x 2048 tokens over up to 12288 in 591 us (566 TFLOP/s).
+// in 58 us (342 MB, 5.9 TB/s; one warp loading both key tiles: 100).  2 x 2048
+// tokens over up to 12288 in 415 us (806 TFLOP/s): 1.3 G powers of two, of which
+// the SFUs take 16 per SM and clock, 290 us at 1.9 GHz; they are busy for three
+// quarters of the time.  Tried and slower: an eighth to a half of the powers by
+// a polynomial on the FMA pipe (510 to 630 us: the warps wait for their own
+// chains, not for the SFU), one group of warps with all 128 scores in registers
+// (512), TMEM loads of 16 columns (556).
 
 #include <type_traits>
 

@@ -34,6 +34,15 @@ serves (and larger than the 126 MB L2 where the kernel streams data):
                     decode step of the config-4 trace
   exchange1         fd_exchange_merge_kernel with one rank (push, flags, merge
                     of config 3's partial)
+  weights_few       fd_keyw_mma_kernel: weights that 32 requests of 4 new tokens
+                    give to 4096 keys each, 32/8 heads, D128, bf16
+  weights_many      the same kernel: 2 requests of 2048 tokens over 8192 keys
+  select_keys       fd_select_kernel: 32 requests x 8 heads, 2048 of 2080 keys
+  move_keys         fd_move_kernel: 4 requests x 8 heads cut from 16384 to 2048
+                    keys of D128 bf16
+  trim_tables       fd_trim_kernel: 100 requests from 8192 to 2048 tokens
+  verify_drafts     fd_verify_kernel: 64 requests of 4 drafts over 131072 fp32
+                    probabilities
   extend_tables     fd_tables_kernel: block tables, slots and positions of 601
                     requests with 0 to 400 new tokens over up to 1000 cached
   rope_store_kv     fd_rope_kernel: 16384 tokens x 32/8 heads x D128 bf16, three
@@ -358,6 +367,83 @@ def case_cross_fp32(dev):
     return _cross(dev, torch.float32, 4, 8, 64, 64, 1500), 4 * 4 * 8 * 64 * 64 * 1500, "fd_attn_kernel"
 
 
+def _stats(blocks, KVH, bs, dev):
+    g = torch.Generator(device=dev).manual_seed(3)
+    return gpu_ops.KeyStats(torch.rand(blocks, KVH, bs, generator=g, device=dev),
+                            torch.randint(0, 1000, (blocks, KVH, bs), generator=g, device=dev, dtype=torch.int32))
+
+
+def _weights(dev, R, ql, kl, flops: bool):
+    H, KVH, D, bs = 32, 8, 128, 16
+    W = kl // bs
+    kc = torch.randn(R * W, KVH, bs, D, device=dev, dtype=torch.bfloat16)
+    table = torch.randperm(R * W, device=dev).to(torch.int32).view(R, W)
+    q = torch.randn(R * ql, H, D, device=dev, dtype=torch.bfloat16)
+    lse = torch.full((H, R * ql), math.log(kl) + 0.5, device=dev)
+    start = torch.arange(R, device=dev, dtype=torch.int32) * ql
+    qlen, klen = (torch.full((R,), n, device=dev, dtype=torch.int32) for n in (ql, kl))
+    stats = _stats(R * W, KVH, bs, dev)
+    pairs = R * (ql * kl - ql * (ql - 1) // 2)
+    work = 2 * pairs * H * D if flops else R * kl * KVH * (2 * D + 8) + 2 * R * ql * H * D
+    return (lambda: gpu_ops.key_weights(q, (KVTier(kc, kc), None), R * W, table, start, qlen, klen, D ** -0.5, lse, stats,
+                                        max_q_len=ql, max_k_len=kl), work, "fd_keyw_mma_kernel")
+
+
+def case_weights_few(dev):
+    return _weights(dev, 32, 4, 4096, False)
+
+
+def case_weights_many(dev):
+    return _weights(dev, 2, 2048, 8192, True)
+
+
+def _cut(dev, R, n, keep):
+    KVH, bs = 8, 16
+    W = -(-n // bs)
+    stats = _stats(R * W, KVH, bs, dev)
+    table = torch.randperm(R * W, device=dev).to(torch.int32).view(R, W)
+    lens, kept = (torch.full((R,), x, device=dev, dtype=torch.int32) for x in (n, keep))
+    moves = gpu_ops.KeyMoves(R, KVH, min(keep, n - keep), dev)
+    return stats, table, lens, kept, moves, lambda: gpu_ops.select_keys(stats, table, lens, kept, moves, max_k_len=n)
+
+
+def case_select_keys(dev):
+    R, n = 32, 2080
+    *_, run = _cut(dev, R, n, 2048)
+    return run, R * 8 * n * 8, "fd_select_kernel"
+
+
+def case_move_keys(dev):
+    R, n, keep, KVH, bs, D = 4, 16384, 2048, 8, 16, 128
+    stats, table, lens, kept, moves, select = _cut(dev, R, n, keep)
+    select()
+    k, v = (torch.randn(table.numel(), KVH, bs, D, device=dev, dtype=torch.bfloat16) for _ in range(2))
+    nbytes = int(moves.counts.sum()) * (2 * (4 * D + 8) + 8)
+    return lambda: gpu_ops.move_keys(moves, (KVTier(k, v), None), table.numel(), table, stats), nbytes, "fd_move_kernel"
+
+
+def case_trim_tables(dev):
+    R, n, bs = 100, 8192, 16
+    W = n // bs
+    table = torch.randperm(R * W, device=dev).to(torch.int32).view(R, W)
+    lens, kept = (torch.full((R,), x, device=dev, dtype=torch.int32) for x in (n, 2048))
+    free = gpu_ops.FreeBlocks(torch.empty(R * W, dtype=torch.int32, device=dev), None, torch.zeros(2, dtype=torch.int32, device=dev))
+    out = gpu_ops.TrimTables(R, dev)
+    return (lambda: gpu_ops.trim_tables(kept, lens, table, free, R * W, 0, bs, out), 12 * R + 8 * R * (n - 2048) // bs,
+            "fd_trim_kernel")
+
+
+def case_verify_drafts(dev):
+    R, K, V = 64, 4, 131072
+    target, draft = (torch.rand(*n, V, device=dev) for n in ((R * (K + 1),), (R, K)))
+    tokens = torch.randint(0, V, (R, K), device=dev)
+    start = torch.arange(R, device=dev, dtype=torch.int32) * (K + 1)
+    qlen = torch.full((R,), K + 1, device=dev, dtype=torch.int32)
+    au, su = torch.full((R, K), 0.999, device=dev), torch.rand(R, device=dev)
+    out = gpu_ops.DraftVerdict(R, K, dev)
+    return lambda: gpu_ops.verify_drafts(target, tokens, draft, start, qlen, au, su, out=out), R * 2 * V * 4, "fd_verify_kernel"
+
+
 CASES = {
     "store_kv_prefill": lambda dev: case_store_kv(dev, False),
     "store_kv_decode": lambda dev: case_store_kv(dev, True),
@@ -372,6 +458,8 @@ CASES = {
     "exchange1": case_exchange1,
     "extend_tables": case_extend_tables, "rope_store_kv": case_rope_store_kv, "chunk_few": case_chunk_few,
     "chunk_many": case_chunk_many, "cross_few": case_cross_few, "cross_fp32": case_cross_fp32,
+    "weights_few": case_weights_few, "weights_many": case_weights_many, "select_keys": case_select_keys,
+    "move_keys": case_move_keys, "trim_tables": case_trim_tables, "verify_drafts": case_verify_drafts,
 }
 
 
@@ -395,7 +483,7 @@ def main() -> None:
                     "achieved_tflops": round(nbytes / t / 1e12, 1), "launches": args.launches}
             print(json.dumps(line), flush=True)
             continue
-        if name in ("prefill", "prefill_fa", "chunk_many"):  # flops, not bytes
+        if name in ("prefill", "prefill_fa", "chunk_many", "weights_many"):  # flops, not bytes
             tf = nbytes / t / 1e12
             peak_tf = _bf16_peak()
             line = {"case": name, "kernel": kernel, "us_per_launch": round(t * 1e6, 2), "flops": int(nbytes),
