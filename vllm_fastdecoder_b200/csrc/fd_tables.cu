@@ -469,7 +469,8 @@ __global__ void __launch_bounds__(kNt, 1) fd_trim_kernel(const __grid_constant__
 
   // running sum of the freed blocks: thread t takes requests [t per, (t + 1) per)
   const int per = (R + kNt - 1) / kNt;
-  int flags = 0, longest = 0, mine = 0, high = 0;
+  int flags = 0, longest = 0, high = 0;
+  unsigned sum = 0u;
   for (int i = 0; i < per; ++i) {
     const int r = tid * per + i;
     if (r >= R) break;
@@ -482,15 +483,16 @@ __global__ void __launch_bounds__(kNt, 1) fd_trim_kernel(const __grid_constant__
     const int col = blocks.hold(s_left[r]), n = blocks.hold(len) - col;
     s_col[r] = col;
     s_sum[r] = n;
-    mine += n;       // (may wrap, with the sums below: then `high` tells)
+    sum += (unsigned)n;  // (may wrap, as the sums below: then `high` tells)
     high += n >> 12;
     longest = max(longest, s_left[r]);
   }
+  const int mine = (int)sum;
   int v = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
     const int u = __shfl_up_sync(0xffffffffu, v, off);
-    if (lane >= off) v += u;
+    if (lane >= off) v = (int)((unsigned)v + (unsigned)u);
   }
   if (lane == 31) warp_n[0][warp] = v;
   flags = __reduce_or_sync(0xffffffffu, flags);
@@ -504,7 +506,7 @@ __global__ void __launch_bounds__(kNt, 1) fd_trim_kernel(const __grid_constant__
   __syncthreads();
   int run, F;
   over_warps<kNw>(warp_n[0], warp, lane, run, F);
-  run += v - mine;
+  run = (int)((unsigned)run + (unsigned)v - sum);
   // more than 2^30 blocks: no stack holds them
   const bool fits = shared_high <= kMaxCount >> 12;
   if (!fits) F = 0;
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(kNt, 1) fd_trim_kernel(const __grid_constant__
     if (r >= R) break;
     const int n = s_sum[r];
     s_sum[r] = fits ? run : 0;
-    run += n;
+    run = (int)((unsigned)run + (unsigned)n);
   }
   if (tid == 0) s_sum[R] = F;
   __syncthreads();
