@@ -507,6 +507,8 @@ extern "C" int fd_select_keys(const fd_select_args* a, void* stream) {
     return fdh::fail(FD_ERR_INVALID, "fd_select_keys: null buffer");
   const int64_t len = a->max_len > 0 && a->max_len < most ? a->max_len : most;
   const int64_t units = (int64_t)a->num_reqs * a->num_kv_heads;
+  // CTAs per request and head: enough that each has one tile, as long as they run at once (32 of 8000 keys: 12.0 us
+  // on clusters of 2, one CTA with two tiles 24; of 32,000: 12.8 on 8, 34, 60 and 84 on 4, 2 and 1)
   int ctas = 1;
   while (ctas < kMaxCluster && units * ctas < 296 && len > (int64_t)ctas * kTile) ctas *= 2;
   SelectParams sp;

@@ -234,8 +234,12 @@ int core_launch(KwParams& p, const Plan& plan, cudaStream_t s) {
 
 // Chunks of an item from which on cutting pays: what it evens out is at most
 // one item's time per CTA (or, with fewer items than CTAs, the idle ones'
-// share of it), what it costs the partials and the combine's launch.
-constexpr int kCutFrom = 3;
+// share of it), what it costs the partials and the combine's launch.  Tensor
+// cores (a chunk 1.2 us): 48 items of 10 chunks 18.8 us, whole 23.3; 96 of 10
+// 27.3 and 24.5; 512 of 4 51.2 and 45.7; 64 of 32 31.9 and 55.4.  CUDA cores:
+// 40 of 5 15.3 and 23.0; 256 of 5 40.8 and 32.0; 80 of 3 18.3 and 14.1; 1024 of 3
+// 88.8 and 94.1.
+constexpr int cut_from(bool mma) { return mma ? 5 : 3; }
 
 Plan plan_of(const fd_attn_args* a) {
   Plan p;
@@ -244,17 +248,21 @@ Plan plan_of(const fd_attn_args* a) {
   const int G = a->num_heads / a->num_kv_heads;
   const int64_t q = a->max_q_len > 0 && a->max_q_len < a->num_tokens ? a->max_q_len : a->num_tokens;
   const bool mma = at::mma_covers(a);
+  // as many columns as there are rows, if the caller is right: 32 requests of 1, 4
+  // and 8 tokens x 4 heads over 4096 keys 48, 51 and 55 us, with 128 columns 80 to
+  // 81; of 16 tokens 46, with 32 columns 78
   p.cols = !mma ? 0 : q * G <= 16 ? 16 : q * G <= 32 ? 32 : 128;
   p.ctas = mma ? sms : sms * ctas_of(a->head_size <= 64 ? 64 : a->head_size <= 128 ? 128 : 256);
   if (p.ctas > kMaxCtas) p.ctas = kMaxCtas;
   const int tq = (mma ? p.cols : kRows) / G, keys = mma ? kMaxKeys : kKeys;
   const int64_t chunks = (q + tq - 1) / tq;
-  p.whole = p.cols == 16 || p.cols == 32 || chunks < kCutFrom;
+  p.whole = p.cols == 16 || p.cols == 32 || chunks < cut_from(mma);
   if (!p.whole && a->max_k_len > 0) {
     const int64_t items = ((int64_t)a->max_k_len + keys - 1) / keys * a->n * a->num_kv_heads;
-    p.whole = items <= p.ctas && chunks * (p.ctas - items) < kCutFrom * (int64_t)p.ctas;
+    p.whole = items <= p.ctas && chunks * (p.ctas - items) < cut_from(mma) * (int64_t)p.ctas;
   }
-  // a grid of items: whole ones, at most two for each CTA that runs at once (where lengths differ most are not there)
+  // a grid of items: whole ones, at most two for each CTA that runs at once (where lengths differ most are not there).
+  // 320 items of one chunk 12.1 us, looked for 16.1; 80 6.3 and 10.1
   p.tiles = 0;
   if (!mma && p.whole && a->max_k_len > 0 && a->n <= 65535 && a->num_kv_heads <= 65535) {
     const int64_t tiles = ((int64_t)a->max_k_len + keys - 1) / keys;
