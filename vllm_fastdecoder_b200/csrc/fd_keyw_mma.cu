@@ -16,16 +16,16 @@
 // per tile, the two groups taking turns at the steps (two warps per scheduler
 // leave the SFU idle while both wait; their sums are joined at the item's end);
 // then one for the schedule, the query chunks and their lse (as many steps ahead
-// as there are slots), one per key tile that loads K, and
-// one whose first thread issues the MMAs.  A STEP is one chunk against one item;
-// its record goes through a ring to all roles.  Every wait is bounded, and a role
+// as there are slots), one per key tile that loads K, and one whose first thread
+// issues the MMAs.  A STEP is one chunk against one item; its record goes
+// through a ring to all roles.  Every wait is bounded, and a role
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 32 single tokens of 32 heads over 512 to 8192 keys of 8 heads x 128
 // in 58 us (342 MB, 5.9 TB/s; one warp loading both key tiles: 100).  2 x 2048
 // tokens over up to 12288 in 415 us (806 TFLOP/s): 1.3 G powers of two, of which
 // the SFUs take 16 per SM and clock, 290 us at 1.9 GHz; they are busy for three
-// quarters of the time.  Tried and slower: an eighth to a half of the powers by
+// quarters of the time.  Tried and slower: an eighth to three eighths of the powers by
 // a polynomial on the FMA pipe (510 to 630 us: the warps wait for their own
 // chains, not for the SFU), one group of warps with all 128 scores in registers
 // (512), TMEM loads of 16 columns (556).
