@@ -408,6 +408,28 @@ def test_select_refuses_a_bad_block_in_a_cluster():
     assert m.counts.tolist() == [[0]] and bool((m.src == -5).all())
 
 
+def test_select_in_clusters_again_and_again():
+    """Many calls on two streams, each request on a cluster of CTAs that write to one another's counters: the same lists every time."""
+    lens, keep = [33000, 20000, 30000], [500, 19000, 3000]
+    sides = []
+    for _ in range(2):
+        pg, stats, m, _, _, gone = _select(lens, keep, KVH=4, seed=9, recent=100)
+        ok()
+        sides.append((torch.cuda.Stream(), stats, pg.table, i32(lens), i32(keep), m, i32(gone)))
+    torch.cuda.synchronize()
+    want = [sides[0][5].src.clone(), sides[0][5].dst.clone(), sides[0][5].counts.clone()]
+    wrong = torch.zeros(2, dtype=torch.int64, device="cuda")
+    for _ in range(300):
+        for i, (stream, stats, table, ln, kp, m, gone) in enumerate(sides):
+            with torch.cuda.stream(stream):
+                gpu_ops.select_keys(stats, table, ln, kp, m, recent=100, evicted=gone, max_k_len=33000)
+                for x, y in zip((m.src, m.dst, m.counts), want):
+                    wrong[i] += (x != y).any()
+    torch.cuda.synchronize()
+    ok()
+    assert wrong.tolist() == [0, 0]
+
+
 # ------------------------------------------------------------------ move
 
 

@@ -84,7 +84,6 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
   const int nct = kMany ? (int)cluster.num_blocks() : 1, rank = kMany ? (int)cluster.block_rank() : 0;
   const int unit = blockIdx.x / nct, KVH = a.num_kv_heads, r = unit / KVH, h = unit - r * KVH;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  if constexpr (kMany) cluster.barrier_arrive();  // this CTA has started; awaited before the first write to another's memory
   const int n = a.lens[r], keep = a.keep_lens[r], BS = a.block_size;
   auto sync = [&]() {
     if constexpr (kMany)
@@ -112,7 +111,6 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
   }
   if (!ok || !cut || keep == 0) {
     if (rank == 0 && tid == 0) a.counts[unit] = 0;
-    if constexpr (kMany) cluster.barrier_wait();
     return;
   }
   const int span = ((n + nct - 1) / nct + 31) / 32 * 32;  // keys of a CTA
@@ -173,7 +171,10 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
   };
   if (tid == 0) taken = any_bad = 0;
   hist[tid] = 0;
-  if constexpr (kMany) whole[0][tid] = whole[1][tid] = whole[2][tid] = 0;
+  if constexpr (kMany) {
+    whole[0][tid] = whole[1][tid] = whole[2][tid] = 0;
+    cluster.barrier_arrive();  // awaited before the first write to another CTA's counters: they are clean by then
+  }
   __syncthreads();
   for (int t0 = lo; t0 < hi; t0 += kTile) {
     load(t0);
