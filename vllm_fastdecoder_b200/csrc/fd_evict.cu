@@ -25,8 +25,9 @@
 // their rows' places first, then all 16-byte pieces of K and V, several per
 // thread in flight.  Bound by the bytes of the rows, read and written once.
 // Measured: 32 requests x 8 heads of up to 32 pairs of 512 bytes in 3.9 us, 4 x
-// 8 of 1400 in 14.1 (48.8 MB, read and written in pieces of 512 bytes, at 3.5
-// TB/s).  A warp by itself with eight pairs at a time: 15.0.
+// 8 of 1400 in 12.7 (48.8 MB, read and written in pieces of 512 bytes, at 3.8
+// TB/s).  With 16, 32 and 128 pairs per CTA: 18.4, 14.2 and 13.7; with 2 and 8
+// pieces per thread 13.2 and 15.0; a warp by itself with eight pairs 15.0.
 
 #include <cooperative_groups.h>
 
@@ -395,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) fd_select_kernel(const __grid_con
 // ------------------------------------------------------------------ move
 
 constexpr int kMoveThreads = 256;
-constexpr int kPairs = 32;   // pairs of a CTA at a time
+constexpr int kPairs = 64;   // pairs of a CTA at a time
 constexpr int kInFlight = 4; // 16-byte pieces per thread
 
 struct MoveParams {
@@ -410,6 +411,7 @@ struct MoveParams {
   int64_t bt_stride;
   fd_key_stats stats;
   int W, KVH, BS, room, vec;  // vec: 16-byte pieces of a row of K
+  int vec_sh;                 // its log2, or -1
   int32_t* err;
 };
 
@@ -472,7 +474,7 @@ __global__ void __launch_bounds__(kMoveThreads) fd_move_kernel(const __grid_cons
         const int x = x0 + u * kMoveThreads;
         out[u] = nullptr;
         if (x >= total) continue;
-        const int row = x / p.vec, c = (x - row * p.vec) * 16, i = row >> 1;
+        const int row = p.vec_sh >= 0 ? x >> p.vec_sh : x / p.vec, c = (x - row * p.vec) * 16, i = row >> 1;
         if (from[i].k == nullptr || to[i].k == nullptr) continue;
         v[u] = *reinterpret_cast<const uint4*>(((row & 1) ? from[i].v : from[i].k) + c);
         out[u] = ((row & 1) ? to[i].v : to[i].k) + c;
@@ -588,6 +590,9 @@ extern "C" int fd_move_keys(const fd_move_args* a, void* stream) {
   p.BS = a->block_size;
   p.room = a->room;
   p.vec = a->head_size * es / 16;
+  p.vec_sh = -1;
+  for (int sh = 0; sh < 20; ++sh)
+    if (p.vec == 1 << sh) p.vec_sh = sh;
   p.err = a->error;
   // CTAs per request and head: as many as its pairs could fill, but no more
   // than fill the GPU eight times over (most of a large room stays unused)
