@@ -18,10 +18,12 @@
 // Bound by the bytes of one target row and one draft row per request, and for
 // a few requests by the chain of loads that leads to them (lengths, tokens,
 // two probabilities, the rows).
-// Measured: 1 request of 4 drafts over 32,000 fp32 values in 6.6 us; 64 of 5 over
-// 131,072 in 22.5, of which 13 are the stream of 67 MB (2 CTAs per SM, 87 % of
-// an SM's share of HBM), the rest the chain of loads before it, the exchange and
-// the search.  With 8 CTAs per request, in several waves, 55.
+// Measured: 1 request of 4 drafts over 32,000 fp32 values in 6.3 us; 64 of 5 over
+// 131,072 of 16 bits in 21.2, most of it the stream of 67 MB, the rest the chain
+// of loads before it, the exchange and the search.  With one vector of each row
+// in flight per thread 23.4, with 3, 6 and 8 22.3, 26.2 and 29.8 (a warp's span
+// ends inside its last round, whose loads are then few).  With 8 CTAs per
+// request, in several waves, 55.
 
 #include <cooperative_groups.h>
 
@@ -104,7 +106,7 @@ struct Rows {
 
 template <typename T, int kV>
 __global__ void __launch_bounds__(kThreads, 2) fd_verify_kernel(const __grid_constant__ VerifyParams vp) {
-  constexpr int kUnroll = kV == 8 ? 3 : 4;  // vectors of each row that a thread has in flight
+  constexpr int kUnroll = kV > 1 ? 2 : 4;  // pieces of each row that a thread has in flight
   const fd_verify_args& a = vp.a;
   __shared__ int s_accepted;  // -1: no tokens
   __shared__ double part[2][kMaxCluster];  // the CTAs' sums, of either attempt
