@@ -16,19 +16,21 @@
 // per tile, the two groups taking turns at the steps (two warps per scheduler
 // leave the SFU idle while both wait; their sums are joined at the item's end);
 // then one for the schedule, the query chunks and their lse (as many steps ahead
-// as there are slots), one per key tile that loads K, and one whose first thread
-// issues the MMAs.  A STEP is one chunk against one item; its record goes
+// as there are slots), one per key tile that loads K, and one per key tile (with
+// N = 128 one for both) whose first thread issues the MMAs.  A STEP is one chunk against one item; its record goes
 // through a ring to all roles.  Every wait is bounded, and a role
 // that gives up raises the CTA's abort flag for the others.
 //
 // Measured: 32 single tokens of 32 heads over 512 to 8192 keys of 8 heads x 128
-// in 58 us (342 MB, 5.9 TB/s; one warp loading both key tiles: 100).  2 x 2048
+// in 56 us (342 MB, 6.1 TB/s; one warp that issues for both key tiles: 58, one
+// that loads both: 100).  2 x 2048
 // tokens over up to 12288 in 415 us (806 TFLOP/s): 1.3 G powers of two, of which
 // the SFUs take 16 per SM and clock, 290 us at 1.9 GHz; they are busy for three
 // quarters of the time.  Tried and slower: an eighth to three eighths of the powers by
 // a polynomial on the FMA pipe (510 to 630 us: the warps wait for their own
 // chains, not for the SFU), one group of warps with all 128 scores in registers
-// (512), TMEM loads of 16 columns (556).
+// (512), TMEM loads of 16 columns (556), both groups' step records read at once
+// (503).
 
 #include <type_traits>
 
@@ -59,9 +61,12 @@ struct Geo {
   static constexpr int kGroups = N <= 32 ? 1 : 2;        // epilogue warpgroups of a key tile
   static constexpr int kSumWarps = 4 * kTiles * kGroups;
   static constexpr int kWarpSched = kSumWarps, kWarpK = kSumWarps + 1, kWarpMma = kWarpK + kTiles;
-  static constexpr int kThreads = (kWarpMma + 1) * 32;
+  // one issuer of MMAs per key tile; with N = 128 one for both (21 warps leave a thread 80 registers: 607 us instead of
+  // 415; one warp less for K instead: 412, but short calls take 16.7 instead of 13.6)
+  static constexpr int kMmaWarps = N <= 32 ? kTiles : 1;
+  static constexpr int kThreads = (kWarpMma + kMmaWarps) * 32;
   static constexpr int kSteps = N <= 32 ? 8 : 4;         // steps in flight between the roles
-  static constexpr int kStepReaders = kSumWarps + kTiles + 1;
+  static constexpr int kStepReaders = kSumWarps + kTiles + kMmaWarps;
   static constexpr int kPanels = KD / 64;
   static constexpr int kTile = kPanels * kPanel;
   static constexpr int kItem = kTiles * kTile;
@@ -77,8 +82,8 @@ struct Geo {
   static constexpr int kOffJoin = kOffStep + kSteps * 48;  // [kTiles][kKT] the second groups' sums
   static constexpr int kOffBar = kOffJoin + (kGroups - 1) * kKeys * 4;
   // k full [ring][tiles], k empty, q full, q empty, s full [bufs][tiles], s empty [bufs][tiles], step full, step empty,
-  // join full, empty [tiles], drain
-  static constexpr int kNumBars = kRingK * (kTiles + 1) + 2 * kRingQ + 2 * kBufs * kTiles + 2 * kSteps + 2 * kTiles + 1;
+  // join full, empty [tiles], drain [MMA warps]
+  static constexpr int kNumBars = kRingK * (kTiles + 1) + 2 * kRingQ + 2 * kBufs * kTiles + 2 * kSteps + 2 * kTiles + kMmaWarps;
   static constexpr int kOffMisc = kOffBar + kNumBars * 8;  // abort flag, TMEM address
   static constexpr int kSmem = kOffMisc + 16;
   static_assert(kSmem <= 227 * 1024, "smem budget");
@@ -163,16 +168,16 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
   const AttnParams& p = mp.a;
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Ge::kOffBar);  // [kRingK][kTiles]
-  uint64_t* k_empty = k_full + kRingK * kTiles;  // [kRingK] MMA commit after the item's last step
+  uint64_t* k_empty = k_full + kRingK * kTiles;  // [kRingK] MMA commits after the item's last step
   uint64_t* q_full = k_empty + kRingK;           // [kRingQ]
-  uint64_t* q_empty = q_full + kRingQ;           // [kRingQ] MMA commit when the next chunk begins, and the epilogue warps
+  uint64_t* q_empty = q_full + kRingQ;           // [kRingQ] MMA commits when the next chunk begins, and the epilogue warps
   uint64_t* s_full = q_empty + kRingQ;           // [kBufs][kTiles] MMA commit
   uint64_t* s_empty = s_full + kBufs * kTiles;   // [kBufs][kTiles] four epilogue warps have the scores
   uint64_t* step_full = s_empty + kBufs * kTiles;
   uint64_t* step_empty = step_full + kSteps;
   uint64_t* join_full = step_empty + kSteps;     // [kTiles] four warps of the second group wrote their sums
   uint64_t* join_empty = join_full + kTiles;     // [kTiles] four warps of the first have read them
-  uint64_t* drain = join_empty + kTiles;
+  uint64_t* drain = join_empty + kTiles;         // [kMmaWarps]
   Step* steps = reinterpret_cast<Step*>(smem + Ge::kOffStep);
   float* lse_sh = reinterpret_cast<float*>(smem + Ge::kOffLse);
   volatile int* misc = reinterpret_cast<volatile int*>(smem + Ge::kOffMisc);
@@ -183,7 +188,8 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
   prefetch_maps(mp, (int)threadIdx.x - 64);
   init_barriers(k_full, Ge::kNumBars, [&](int i) -> uint32_t {
     uint64_t* b = k_full + i;
-    if (b >= q_empty && b < s_full) return 1 + kSumWarps;
+    if (b >= k_empty && b < q_full) return Ge::kMmaWarps;
+    if (b >= q_empty && b < s_full) return Ge::kMmaWarps + kSumWarps;
     if (b >= s_empty && b < step_full) return 4;
     if (b >= join_full && b < drain) return 4;
     return b >= step_empty && b < join_full ? Ge::kStepReaders : 1;
@@ -347,8 +353,10 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
       const uint32_t last = s + kRingK * ((items - 1 - s) / kRingK);
       mbar_wait(&k_full[s * kTiles + t], (last / kRingK) & 1u, p.err);
     }
-  } else if (warp == Ge::kWarpMma) {
-    // ------------------------------------------------ MMA issuer
+  } else if (warp >= Ge::kWarpMma) {
+    // ------------------------------------------------ MMA issuer of key tiles t0 .. t0 + kMine - 1
+    constexpr int kMine = kTiles / Ge::kMmaWarps;
+    const int t0 = (warp - Ge::kWarpMma) * kMine;
     if (lane == 0) {
       const uint32_t base = smem_u32(smem) >> 4;
       const uint32_t panel = (uint32_t)mp.panel >> 4;
@@ -370,7 +378,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         if (new_q) ok = poll_or_abort(&q_full[qs], ((nq - 1) / kRingQ) & 1u, misc, p.err);
         const uint32_t q_lo = base + (uint32_t)((Ge::kOffQ + qs * Ge::kQ) >> 4) + (1u << 16);
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t) {
+        for (int t = t0; t < t0 + kMine; ++t) {
           if (ok && new_k) ok = poll_or_abort(&k_full[ks * kTiles + t], ((items - 1) / kRingK) & 1u, misc, p.err);
           if (ok && i >= kBufs) ok = poll_or_abort(&s_empty[b * kTiles + t], (i / kBufs - 1) & 1u, misc, p.err);
           if (!ok) break;
@@ -385,8 +393,8 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         if (ok && (flags & kLastK) != 0) umma_commit(&k_empty[ks]);
       }
       if (!ok) misc[0] = 1;
-      umma_commit(drain);  // all MMAs complete before TMEM is released
-      mbar_wait(drain, 0u, p.err);
+      umma_commit(drain + t0 / kMine);  // all MMAs complete before TMEM is released
+      mbar_wait(drain + t0 / kMine, 0u, p.err);
     }
     __syncwarp();
   } else {
