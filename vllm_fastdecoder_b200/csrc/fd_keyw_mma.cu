@@ -24,7 +24,7 @@
 // Measured: 32 single tokens of 32 heads over 512 to 8192 keys of 8 heads x 128
 // in 56 us (342 MB, 6.1 TB/s; one warp that issues for both key tiles: 58, one
 // that loads both: 100).  2 x 2048
-// tokens over up to 12288 in 415 us (806 TFLOP/s): 1.3 G powers of two, of which
+// tokens over up to 12288 in 420 us (797 TFLOP/s): 1.3 G powers of two, of which
 // the SFUs take 16 per SM and clock, 290 us at 1.9 GHz; they are busy for three
 // quarters of the time.  Tried and slower: an eighth to three eighths of the powers by
 // a polynomial on the FMA pipe (510 to 630 us: the warps wait for their own
@@ -62,7 +62,7 @@ struct Geo {
   static constexpr int kSumWarps = 4 * kTiles * kGroups;
   static constexpr int kWarpSched = kSumWarps, kWarpK = kSumWarps + 1, kWarpMma = kWarpK + kTiles;
   // one issuer of MMAs per key tile; with N = 128 one for both (21 warps leave a thread 80 registers: 607 us instead of
-  // 415; one warp less for K instead: 412, but short calls take 16.7 instead of 13.6)
+  // 420; one warp less for K instead: 412, but short calls take 16.7 instead of 13.6)
   static constexpr int kMmaWarps = N <= 32 ? kTiles : 1;
   static constexpr int kThreads = (kWarpMma + kMmaWarps) * 32;
   static constexpr int kSteps = N <= 32 ? 8 : 4;         // steps in flight between the roles
