@@ -216,6 +216,54 @@ def test_weights_of_rows_without_keys_and_nan(dtype, ql):
     assert int(stats.weights.isnan().sum()) == 300 - ql + 1
 
 
+@pytest.mark.parametrize("dtype,H,ql", [(torch.bfloat16, 8, 3), (torch.float16, 8, 7), (torch.bfloat16, 8, 90), (torch.float16, 20, 200),
+                                        (torch.float32, 8, 70)])
+def test_weights_of_infinite_rows_whatever_their_queries_hold(dtype, H, ql):
+    """A row with lse = -inf or +inf gives nothing where its scores are NaN, infinite or overflow, too."""
+    k_lens, KVH, D, scale = [700, 300, 513], 2, 64, 0.125
+    pg = Paged(k_lens, KVH, 16, D, dtype, seed=13)
+    T = 3 * ql
+    q = torch.randn(T, H, D, generator=torch.Generator().manual_seed(12)).to(dtype).cuda()
+    lse = _lse(q, pg.keys, [ql] * 3, scale)
+    big = torch.finfo(dtype).max
+    at = 0
+    for out in (-math.inf, math.inf):
+        for fill in (NAN, math.inf, -math.inf, big, -big):  # one row of some token and head each, and two whole tokens
+            t, h = (7 * at + 1) % T, (3 * at) % H
+            lse[h, t], q[t, h] = out, fill
+            at += 1
+        t = 0 if out < 0 else T - 1
+        lse[:, t], q[t] = out, NAN
+    stats = pg.stats()
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([0, ql, 2 * ql]), i32([ql] * 3), i32(k_lens), scale, lse, stats,
+                        max_q_len=ql, max_k_len=700)
+    ok()
+    assert not bool(torch.cat([stats.weights[pg.places(r)[0].cuda(), :, pg.places(r)[1].cuda()] for r in range(3)]).isnan().any())
+    _check_weights(pg, q, lse, [ql] * 3, k_lens, [0, ql, 2 * ql], scale, stats, w0, p0, [0, 0, 0])
+
+
+@pytest.mark.parametrize("dtype,ql", [(torch.bfloat16, 3), (torch.float16, 7), (torch.bfloat16, 90), (torch.float32, 70)])
+def test_weights_of_keys_with_an_infinite_value(dtype, ql):
+    """A key whose scores are +inf makes its rows' lse +inf: they give nothing; to those that it scores -inf it is nothing."""
+    k_lens, KVH, H, D, scale = [700, 300], 2, 8, 64, 0.125
+    pg = Paged(k_lens, KVH, 16, D, dtype, seed=14)
+    for r, j in ((0, 5), (0, 300), (1, 299)):
+        blk, off = pg.rows[r][j // 16], j % 16
+        pg.tiers[0].k[blk, 1, off, 3] = pg.keys[r][j, 1, 3] = math.inf
+    q = torch.randn(2 * ql, H, D, generator=torch.Generator().manual_seed(15)).to(dtype)
+    q[..., 3] = torch.where(q[..., 3] == 0, 1.0, q[..., 3])
+    q = q.cuda()
+    lse = _lse(q, pg.keys, [ql] * 2, scale)
+    assert 0 < int(lse.isinf().sum()) < lse.numel() and not bool(lse.isnan().any())
+    stats = pg.stats()
+    w0, p0 = stats.weights.clone(), stats.positions.clone()
+    gpu_ops.key_weights(q, pg.tiers, pg.G, pg.table, i32([0, ql]), i32([ql] * 2), i32(k_lens), scale, lse, stats, max_q_len=ql, max_k_len=700)
+    ok()
+    _check_weights(pg, q, lse, [ql] * 2, k_lens, [0, ql], scale, stats, w0, p0, [0, 0])
+    assert not bool(torch.cat([stats.weights[pg.places(r)[0].cuda(), :, pg.places(r)[1].cuda()] for r in range(2)]).isnan().any())
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_weights_strides_and_table_rows(dtype):
     """q out of a wider projection, lse [T, H] transposed, requests on other table rows."""

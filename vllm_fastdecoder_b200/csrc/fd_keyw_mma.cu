@@ -92,8 +92,9 @@ struct Geo {
 
 // Whether a step is the first or last of its segment (K), and the first with a
 // chunk of queries (Q: the slot of the chunk before is done with the steps
-// before).  Flags 0: no more steps.
-enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8 };
+// before).  kMute: not every column of the chunk gives something (no row, or
+// one whose lse is infinite).  Flags 0: no more steps.
+enum StepFlag { kLive = 1, kNewK = 2, kLastK = 4, kNewQ = 8, kMute = 16 };
 struct Step {
   int flags;
   int r, kh, kt, kbase;
@@ -263,7 +264,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
     Step cur;
     Req rq = {0, 0, 0, 0};
     float ls[kPer];
-    int qs = -1;
+    int qs = -1, mute = 0;
     uint32_t nq = 0;
     bool ok = true;
     for (uint32_t i = 0; ok; ++i) {
@@ -278,9 +279,13 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           ok = __all_sync(0xffffffffu, wait_or_abort(&q_empty[qs], (nq / kRingQ - 1) & 1u, misc, p.err));
         if (!ok) break;
         ++nq;
+        mute = 0;
 #pragma unroll
-        for (int x = 0; x < kPer; ++x)  // a row that saw nothing gives nothing
-          lse_sh[qs * kLseRow + 32 * x + lane] = isinf(ls[x]) ? -INFINITY : -ls[x] * kLog2e;
+        for (int x = 0; x < kPer; ++x) {  // a row that saw nothing gives nothing
+          const bool none = isinf(ls[x]);
+          lse_sh[qs * kLseRow + 32 * x + lane] = none ? -INFINITY : -ls[x] * kLog2e;
+          if (__any_sync(0xffffffffu, none)) mute = kMute;
+        }
         unsigned char* sq = smem + Ge::kOffQ + qs * Ge::kQ;
         if (mp.q_tma) {
           if (lane == 0) {
@@ -296,6 +301,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
           if (lane == 0) mbar_arrive(&q_full[qs]);
         }
       }
+      if (cur.flags != 0) cur.flags |= cur.rows < N ? kMute : mute;
       if (lane == 0) steps[ss] = cur;
       __syncwarp();
       if (lane == 0) mbar_arrive(&step_full[ss]);
@@ -438,7 +444,9 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
         if (any) {
           const int over = key - s.first;
           const int from = over > 0 ? over * p.G : 0;
-          const bool masked = key0 + 31 > s.first || s.rows < N;
+          const bool masked = key0 + 31 > s.first || (s.flags & kMute) != 0;
+          // rows with an infinite lse, as bits (that 2^-inf is 0 would not do: an infinite or NaN score makes it a NaN)
+          auto muted = [&](int c) { return (s.flags & kMute) != 0 ? __ballot_sync(0xffffffffu, neg[32 * c + lane] == -INFINITY) : 0u; };
           if constexpr (N <= 32) {
             uint32_t v[32];
             if constexpr (N == 16) {
@@ -454,7 +462,8 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&s_empty[b * kTiles + t]);
-            add_up(v, neg, sl2, acc, [&](int e) { return e >= from && e < s.rows; }, [&](int c) { return c >= s.rows; });
+            const uint32_t seen = bits_of(from, s.rows) & ~muted(0);
+            add_up(v, neg, sl2, acc, [&](int e) { return (seen >> e & 1u) != 0u; }, [&](int c) { return c >= s.rows; });
           } else {
             uint32_t v[2][32];
             tmem_ld32_nowait(ts, v[0]);
@@ -470,7 +479,7 @@ __global__ void __launch_bounds__(Geo<KD, N>::kThreads, 1) fd_keyw_mma_kernel(co
               }
               const auto no_skip = [](int) { return false; };
               if (masked) {
-                const uint32_t seen = bits_of(from - 32 * c, s.rows - 32 * c);
+                const uint32_t seen = bits_of(from - 32 * c, s.rows - 32 * c) & ~muted(c);
                 add_up(v[c & 1], neg + 32 * c, sl2, acc, [&](int e) { return (seen >> e & 1u) != 0u; }, no_skip);
               } else {
                 add_up(v[c & 1], neg + 32 * c, sl2, acc, [](int) { return true; }, no_skip);
