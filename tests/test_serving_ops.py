@@ -169,6 +169,21 @@ def test_key_weights_workspace_is_for_cut_items_and_host_copies():
     assert lib.fd_key_weights_workspace_size(ctypes.byref(a)) == 0
 
 
+@pytest.mark.parametrize("heads,kv_heads", [(4, 2), (32, 1), (64, 1)])
+@pytest.mark.parametrize("tokens,n", [(0, 2), (2, 0), (0, 0), (-1, 2), (2, -1)])
+@pytest.mark.parametrize("dtype,D", [(1, 64), (0, 128), (2, 64)])
+def test_key_weights_of_an_empty_step_needs_nothing(dtype, D, tokens, n, heads, kv_heads):
+    """No scratch memory, and no arithmetic on chunks of no rows (more heads per kv head than the fewest columns)."""
+    lib = nat.load()
+    a = _weights()
+    t = a.attn
+    t.num_tokens, t.n, t.num_heads, t.num_kv_heads, t.head_size, t.dtype = tokens, n, heads, kv_heads, D, dtype
+    t.q_stride_h, t.q_stride_t = D, heads * D
+    t.tier[1].host_mapped, t.tier[1].num_blocks = 1, 4
+    assert lib.fd_key_weights_workspace_size(ctypes.byref(a)) == 0
+    assert lib.fd_key_weights(ctypes.byref(a), None) == (0 if tokens >= 0 and n >= 0 else 1)
+
+
 def _select():
     a = nat.FdSelectArgs()
     a.stats.weights = a.stats.positions = 4096

@@ -276,6 +276,7 @@ Plan plan_of(const fd_attn_args* a) {
 
 extern "C" size_t fd_key_weights_workspace_size(const fd_key_weights_args* a) {
   if (a == nullptr || a->attn.head_size <= 0 || a->attn.head_size > 256) return 0;
+  if (a->attn.n <= 0 || a->attn.num_tokens <= 0) return 0;  // nothing to do
   if (a->attn.num_kv_heads <= 0 || a->attn.num_heads < a->attn.num_kv_heads ||
       a->attn.num_heads / a->attn.num_kv_heads > fdk::kw::kRows)
     return 0;
