@@ -6,6 +6,7 @@ from __future__ import annotations
 
 import math
 import random
+from pathlib import Path
 
 import pytest
 import serving_ref as ref
@@ -1204,3 +1205,80 @@ def test_serving_steps_in_one_graph():
         ok()
         for x, y in zip(a.state(), b.state()):
             assert torch.equal(x, y), step
+
+
+# ------------------------------------------------------------------ the documented step
+
+
+def _documented():
+    """The documents' python blocks that verify drafts, by their file's name."""
+    found = {}
+    for path in sorted(Path(__file__).resolve().parents[1].glob("*.md")):
+        for block in path.read_text().split("```python\n")[1:]:
+            code = block.split("```")[0]
+            if "verify_drafts(" in code:
+                found[path.stem] = code
+    return found
+
+
+@pytest.mark.parametrize("where", sorted(_documented()) or ["none"])
+def test_the_documented_step_of_prompts_and_drafts(where):
+    """What the documents tell a user to run after the attention, on a step that mixes a long prompt, a prompt shorter
+    than the drafts, drafts and a request without part."""
+    code = _documented()[where]
+    for new, prompt in (([4, 2, 30, 3], [False, True, True, False]), ([1, 0, 25, 4], [False, False, True, False])):
+        s = Serving(3)
+        s.fill(0)
+        s.attend()
+        s.verify()
+        ok()
+        s.fill(20)
+        s.new.copy_(i32(new))
+        total = s.lens.tolist()
+        s.attend()
+        ok()
+        start = [sum(new[:r]) for r in range(s.R)]
+        # one draft of each request that the target is sure of, so that some are accepted
+        for r in range(s.R):
+            if not prompt[r] and new[r] > 1:
+                s.target[start[r]] = 0.0
+                s.target[start[r], int(s.drafts[r, 0])] = 1.0
+        w0, p0 = s.stats.weights.clone(), s.stats.positions.clone()
+        ns = dict(torch=torch, gpu_ops=gpu_ops, R=s.R, K=s.K, KVH=s.KVH, G=s.G, C=s.C, BS=s.BS, device="cuda", counts=s.counts, free=s.free,
+                  t=s.t, block_table=s.table, tiers=s.tiers, scale=s.D ** -0.5, q=s.q, lse=s.lse, target_probs=s.target, drafts=s.drafts,
+                  draft_probs=s.probs, accept_u=s.au, sample_u=s.su, prompt=torch.tensor(prompt, device="cuda"), trim=s.trim, stats=s.stats,
+                  moves=s.moves, room=s.budget, evicted=s.gone, layers=1, l=0, max_q=40, max_k=180, keep_lens=i32([-1] * s.R))
+        exec(code, ns)
+        ok()
+        stats = ns["stats"]
+        if isinstance(stats, list):  # made by the block itself
+            stats, w0, p0 = stats[0], torch.zeros_like(w0), torch.zeros_like(p0)
+        t64 = s.target.double().tolist()
+        want_w, tol, want_p = w0.double(), torch.zeros_like(w0, dtype=torch.float64), p0.clone()
+        accepted = 0
+        for r in range(s.R):
+            if new[r] == 0:
+                used, got = 0, []
+            else:
+                first, rows = (start[r] + new[r] - 1, 1) if prompt[r] else (start[r], new[r])
+                got, a = ref.verify(t64, s.drafts[r].tolist(), s.probs[r].double().tolist(), first, rows, s.au[r].double().tolist(),
+                                    float(s.su[r]))
+                used = new[r] if prompt[r] else a + 1
+                accepted += 0 if prompt[r] else a
+            assert ns["v"].tokens[r].tolist() == got + [-1] * (s.K + 1 - len(got))
+            n = total[r] + used
+            assert s.lens.tolist()[r] == n
+            if used == 0:
+                continue
+            k = s.cached(r, n)[0]
+            ids = torch.tensor(s.table[r].tolist(), device="cuda")
+            j = torch.arange(n, device="cuda")
+            blk, off = ids[j // s.BS], j % s.BS
+            for g in range(s.KVH):
+                qh = s.q[start[r]:start[r] + used, g * 4:(g + 1) * 4]
+                w, e = ref.key_weights(qh, k[g][:, None], s.lse[g * 4:(g + 1) * 4, start[r]:start[r] + used], w0[blk, g, off][None], s.D ** -0.5)
+                want_w[blk, g, off], tol[blk, g, off] = w[0], e[0]
+                want_p[blk[total[r]:], g, off[total[r]:]] = j[total[r]:].int()
+        assert accepted > 0
+        assert bool(((stats.weights.double() - want_w).abs() <= tol).all())
+        assert torch.equal(stats.positions, want_p)

@@ -1197,7 +1197,9 @@ def key_weights(q: torch.Tensor, tiers: tuple[KVTier | None, KVTier | None], tie
     (int32 [n], see trim_tables).  Older keys' weights are added to.  So a key
     needs no reset when its block is handed to another request, and a step whose
     drafts were rejected can count the accepted ones alone (q_len and k_len
-    without the others)."""
+    without the others).  A key that no call had among the newest keeps the weight
+    and the position that its place held before, so a prompt's tokens count
+    whole."""
     KVH, BS, f0, f1, W = _paged(q, tiers, block_table, bt_row, q_len.numel())
     idx = q.get_device()
     lib = nat.load()
@@ -1279,7 +1281,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_
     ordinary sampling.
 
     target_probs [T, V]: a row per query of the step; q_start, q_len int32 [R]
-    as extend_tables gives them (q_len = 1 + drafts; 0: no part in the step);
+    as extend_tables gives them (q_len = 1 + drafts; 0: no part in the step), or,
+    where a request's new tokens are a prompt's, its last row and 1;
     draft_tokens int64 [R, K]; draft_probs [R, K, V] of target_probs' dtype
     (fp32, fp16 or bf16), or None where the draft is no distribution;
     accept_u fp32 [R, K] and sample_u fp32 [R]: uniform numbers in [0, 1).
