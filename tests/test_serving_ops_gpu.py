@@ -990,6 +990,32 @@ def test_two_graphs_and_streams_do_not_share_anything():
     assert _same(res, want) and all(_same(r, want) for _, r, _ in sides)
 
 
+@pytest.mark.parametrize("keep", [1, 150, 299])
+def test_select_s_bound_sizes_only_the_moves_that_it_makes(keep):
+    """A bound that is too small: nothing, with moves given; a refusal where the call makes them itself."""
+    lens = [300, 40]
+    kept = [keep, 20]
+    pg, stats, m, w, p, gone = _select(lens, kept, room=150, hint=10)
+    ok()
+    _check_select(m, lens, kept, w, p, gone, 0, 0)
+    for bound in (0, 300):
+        made = gpu_ops.select_keys(stats, pg.table, i32(lens), i32(kept), evicted=i32(gone), max_k_len=bound)
+        ok()
+        assert made.room >= 150 and made.counts.tolist() == m.counts.tolist()
+        for r in range(2):
+            for h in range(2):
+                c = int(m.counts[r, h])
+                assert torch.equal(made.src[r, h, :c], m.src[r, h, :c]) and torch.equal(made.dst[r, h, :c], m.dst[r, h, :c])
+    small = gpu_ops.select_keys(stats, pg.table, i32(lens), i32(kept), evicted=i32(gone), max_k_len=40)
+    if min(keep, 300 - keep) > 20:
+        fails("sequence length")
+        assert small.counts[0].tolist() == [0, 0]
+    else:
+        ok()
+        assert small.counts[0].tolist() == m.counts[0].tolist()
+    assert small.counts[1].tolist() == m.counts[1].tolist()
+
+
 # ------------------------------------------------------------------ a run of them together
 
 

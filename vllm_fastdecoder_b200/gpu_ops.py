@@ -1228,7 +1228,11 @@ def select_keys(stats: KeyStats, block_table: torch.Tensor, seq_lens: torch.Tens
     evicted int32 [R]: tokens cut earlier.  Writes to `moves` (default: a new
     one, with room for max_k_len / 2 moves) which keys move where, all from
     behind the budget to before it; nothing else changes.  A request that could
-    need more moves than there is room for has none, and sets the error word."""
+    need more moves than there is room for has none, and sets the error word.
+    max_k_len: the host's bound on seq_lens, if it knows one (0: what the table's
+    rows hold).  With `moves` given it only chooses the launch, and a wrong one
+    costs time, not the result; without, it also sizes the new one, and has to
+    hold."""
     idx, R, W = _block_table(block_table)
     _, KVH, BS = stats.weights.shape
     if moves is None:
