@@ -7,26 +7,33 @@
 // keep-th greatest, T, splits the keys without a rule for ties.  It is found by
 // narrowing: a window, at first of all 64-bit numbers, is cut into 512 equal
 // bins, and the bin that holds T becomes the window, until few enough candidates
-// are left to rank each against all.  The first round tells exponents apart, the
-// second nine more bits; a third is seldom needed.  Then one running count in
-// index order, of the places that become free and of the keys that move, gives
-// each pair its place, so src and dst ascend and no result depends on timing.  The keys are read once and stay in
-// registers (in shared memory where a CTA has more than 4096), in one CTA, or
-// in a cluster that adds its counters up through distributed shared memory.
+// are left to rank each against all.  The first round tells exponents apart, each
+// other one nine more bits.  A CTA by itself ranks after the first as a rule; a
+// cluster, where ranking costs two rounds, goes on until the window holds no more
+// keys than are wanted of it (two or three rounds), and ranks only among equal
+// weights.  Then one running count in index order, of the places that become free
+// and of the keys that move, gives each pair its place, so src and dst ascend and
+// no result depends on timing.  The keys are read once and stay in registers (in
+// shared memory where a CTA has more than 4096), in one CTA, or in a cluster that
+// adds its counters up through distributed shared memory.
 // Bound by the latency of that chain (lengths, table, weights, then the
 // exchanges), not by its 8 bytes per key.
-// Measured: 32 requests x 8 heads of 2050 keys, of which some hundred tie, in
-// 8.7 us; 4 x 8 of 11,000 to 32,000 in 16.0 on clusters of 8, of which a round
-// with its exchange takes 1.6 to 2.4.
+// Measured: 32 requests x 8 heads of up to 2080 keys in 8.9 us, 13.3 where the
+// border falls among a hundred keys that tie; 4 x 8 of 11,000 to 32,000 in 16.2 on
+// clusters of 8 (four or five cluster barriers: the start, two or three rounds, the
+// counts), of which a round with its exchange takes 1.6 to 2.4.
 //
 // Move.  Only what lies behind the budget moves, into what goes before it, so
 // no pair reads what another writes, and the pairs are dealt out over the GPU
 // in any order.  A CTA takes kPairs pairs of one request and head at a time:
 // their rows' places first, then all 16-byte pieces of K and V, several per
-// thread in flight.  Bound by the bytes of the rows, read and written once.
+// thread in flight.  The rows' bytes are its floor; what bounds it is latency, of
+// one wave of CTAs that go through count, pair and table before any row moves
+// (a warp's cycles are half waits for loads, DRAM is busy a quarter of the time).
 // Measured: 32 requests x 8 heads of up to 32 pairs of 512 bytes in 3.9 us, 4 x
-// 8 of 1400 in 12.7 (48.8 MB, read and written in pieces of 512 bytes, at 3.8
-// TB/s).  With 16, 32 and 128 pairs per CTA: 18.4, 14.2 and 13.7; with 2 and 8
+// 8 of 1400 in 13.2 (48.8 MB, read and written in pieces of 512 bytes, at 3.7
+// TB/s); with half of their blocks in the host tier 25 and 366, the link's time.
+// With 16, 32 and 128 pairs per CTA: 18.4, 14.2 and 13.7; with 2 and 8
 // pieces per thread 13.2 and 15.0; a warp by itself with eight pairs 15.0.
 
 #include <cooperative_groups.h>
@@ -510,8 +517,9 @@ extern "C" int fd_select_keys(const fd_select_args* a, void* stream) {
     return fdh::fail(FD_ERR_INVALID, "fd_select_keys: null buffer");
   const int64_t len = a->max_len > 0 && a->max_len < most ? a->max_len : most;
   const int64_t units = (int64_t)a->num_reqs * a->num_kv_heads;
-  // CTAs per request and head: enough that each has one tile, as long as they run at once (32 of 8000 keys: 12.0 us
-  // on clusters of 2, one CTA with two tiles 24; of 32,000: 12.8 on 8, 34, 60 and 84 on 4, 2 and 1)
+  // CTAs per request and head: enough that each has one tile, as long as they run at once (32 of 8000 keys: 12.1 us
+  // on clusters of 2, one CTA with two tiles 23.9; of 32,000: 17.1 on 8, 34, 60 and 84 on 4, 2 and 1; 8 of 32,000, a
+  // CTA per SM: 12.9 on 8)
   int ctas = 1;
   while (ctas < kMaxCluster && units * ctas < 296 && len > (int64_t)ctas * kTile) ctas *= 2;
   SelectParams sp;

@@ -18,12 +18,13 @@
 // Bound by the bytes of one target row and one draft row per request, and for
 // a few requests by the chain of loads that leads to them (lengths, tokens,
 // two probabilities, the rows).
-// Measured: 1 request of 4 drafts over 32,000 fp32 values in 6.3 us; 64 of 5 over
-// 131,072 of 16 bits in 21.2, most of it the stream of 67 MB, the rest the chain
-// of loads before it, the exchange and the search.  With one vector of each row
-// in flight per thread 23.4, with 3, 6 and 8 22.3, 26.2 and 29.8 (a warp's span
-// ends inside its last round, whose loads are then few).  With 8 CTAs per
-// request, in several waves, 55.
+// Measured: 1 request of 4 drafts over 32,000 fp32 values in 6.4 us; 64 of 5 over
+// 131,072 fp32 values in 21.4, most of it the stream of 67 MB (256 CTAs, of which
+// 108 SMs have two and the others one), the rest the chain of loads before it, the
+// exchange and the search; 19.2 without draft probabilities; of 16 bits 18.8 and
+// 16.8.  With one vector of each row in flight per thread 23.4, with 3, 6 and 8
+// 22.3, 26.2 and 29.8 (a warp's span ends inside its last round, whose loads are
+// then few).  With 8 CTAs per request, in several waves, 55.
 
 #include <cooperative_groups.h>
 
