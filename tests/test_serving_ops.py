@@ -261,6 +261,14 @@ def test_buffers_are_checked_when_made_and_stay():
         gpu_ops.KeyStats(torch.zeros(2, 3, 4), i32(2, 3, 4))
 
 
+def test_a_verdict_s_lengths_leave_requests_alone_until_they_are_filled():
+    """verify_drafts writes keep_lens where it is given the lengths; trim_tables leaves a request below 0 as it is."""
+    v = gpu_ops.DraftVerdict(3, 2, "cpu")
+    assert v.keep_lens.tolist() == [-1] * 3 and v.keep_lens.dtype is torch.int32
+    assert v.accepted.tolist() == [0] * 3 and v.tokens.tolist() == [[-1] * 3] * 3
+    assert gpu_ops.DraftVerdict(0, 2, "cpu").keep_lens.numel() == 0
+
+
 def test_calls_refuse_host_tensors():
     i32 = lambda *n: torch.zeros(n, dtype=torch.int32)  # noqa: E731
     free = gpu_ops.FreeBlocks(i32(4), None, i32(2))

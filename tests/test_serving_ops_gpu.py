@@ -1016,6 +1016,17 @@ def test_select_s_bound_sizes_only_the_moves_that_it_makes(keep):
     assert small.counts[1].tolist() == m.counts[1].tolist()
 
 
+def test_a_trim_by_a_verdict_without_lengths_cuts_nothing():
+    lens, block = [40, 33], 16
+    table, stacks, counts, hbm, host = _trim(lens, lens, block, 0.5)
+    g = torch.Generator().manual_seed(6)
+    v = _verify(_probs(g, 6, 20), torch.zeros(2, 2, dtype=torch.int64), None, [0, 3], [3, 3], torch.ones(2, 2), torch.rand(2, generator=g))
+    st, ct, ln = i32(stacks), i32(counts), i32(lens)
+    out = gpu_ops.trim_tables(v.keep_lens, ln, i32(table), FreeBlocks(st[0], st[1], ct), hbm, host, block)
+    ok()
+    assert out.seq_lens.tolist() == lens and out.counts.tolist() == counts and st.tolist() == stacks
+
+
 # ------------------------------------------------------------------ a run of them together
 
 

@@ -1270,10 +1270,11 @@ def move_keys(moves: KeyMoves, tiers: tuple[KVTier | None, KVTier | None], tier_
 class DraftVerdict(_Buffers):
     """Device buffers that verify_drafts fills for R requests of up to K drafted
     tokens: tokens int64 [R, K + 1] (the accepted drafts, the token that
-    follows, then -1), accepted int32 [R], keep_lens int32 [R]."""
+    follows, then -1), accepted int32 [R], keep_lens int32 [R] (-1, which
+    trim_tables leaves alone, until a call that is given seq_lens)."""
 
     def __init__(self, R: int, K: int, device):
-        super().__init__(device, accepted=(R, R), keep_lens=(R, R))
+        super().__init__(device, accepted=(R, R), keep_lens=(torch.full((R,), -1, dtype=torch.int32, device=device), R))
         self.__dict__.update(R=int(R), K=int(K), tokens=torch.full((R, K + 1), -1, dtype=torch.int64, device=device))
 
 
@@ -1294,7 +1295,8 @@ def verify_drafts(target_probs: torch.Tensor, draft_tokens: torch.Tensor, draft_
     comes from max(p - q, 0) of the rejected draft, or from the last row, by
     sample_u's place in the running sum.  A one-hot row is greedy decoding.
     Fills and returns `out`; keep_lens, with seq_lens int32 [R] (the drafts
-    included), is the cache that stays: trim_tables' keep_lens."""
+    included), is the cache that stays: trim_tables' keep_lens.  Without
+    seq_lens, keep_lens is left as it was."""
     idx, dt = target_probs.get_device(), target_probs.dtype
     if idx < 0:
         raise RuntimeError("target_probs must be a CUDA tensor")
